@@ -272,6 +272,50 @@ int ssdk_prompt_attn(const void* q, const void* k_cache, const void* v_cache,
                      int block_size, int max_blocks_per_seq, int64_t num_blocks, float scale,
                      uint32_t* gave_up, void* stream);
 
+/* Pages, positions and slots of a step's tokens from the lengths of its requests, on the device (what prepare_decode, prepare_prefill and
+ * BlockManager do on the host: engine/helpers/runner_helpers.py:50-121, engine/block_manager.py).  Sequence b has context_lens[b] tokens in
+ * the pages block_tables[b, 0 .. ceil(context / block_size)) and gets new_lens[b] more.  Pages that it lacks are taken from free_blocks
+ * [n_free], of which the first free_used[0] are gone (a negative count reads as 0), in the order of the sequences, and written into its
+ * table; other entries stay.  A sequence is placed as a whole or not at all: not with a negative length, nor past its table's end, nor when
+ * it or one in front of it lacks free pages (sequences that need no page are not held up), nor when it or one in front of it finds no more
+ * room in `rows`.
+ *   positions int64 [rows], slot_mapping int32 [rows] (-1: its page is none of the cache's num_blocks), row_seqs int32 [rows]: the new tokens
+ *   of the placed sequences one behind the other; rows behind the last: 0, -1, -1.  cu_rows [batch + 1]: first row of a sequence.
+ *   lens [batch]: context_lens + new_lens, of sequences that are not placed context_lens.  used [1]: free_used and the pages handed out. */
+int ssdk_place_tokens(const int32_t* context_lens, const int32_t* new_lens, int32_t* block_tables, const int32_t* free_blocks,
+                      const int32_t* free_used, int64_t* positions, int32_t* slot_mapping, int32_t* row_seqs, int32_t* cu_rows,
+                      int32_t* lens, int32_t* used, int batch, int max_blocks_per_seq, int n_free, int rows, int block_size,
+                      int64_t num_blocks, void* stream);
+
+/* ssdk_rope_store_kv with positions on several axes (1 to 4: time, height, width, ...): positions int64 [axes, M]; frequency i turns by
+ * positions[axis_of[i], m] (axis_of: host bytes [rot_dim / 2]).  rope_table fp32 [max_pos, rot_dim] cos | sin; the first rot_dim channels of
+ * a head turn (i with i + rot_dim / 2), the others pass.  Norm and rotation in fp32, one rounding.  A row with a position outside
+ * the table has NaN queries and stores nothing; slots below 0 or from num_slots on store nothing; slots of a call are distinct. */
+int ssdk_rope_axes_store_kv(const void* qkv, const int64_t* positions, int axes, const uint8_t* axis_of, const int32_t* slot_mapping,
+                            const float* rope_table, int64_t max_pos, int rot_dim, const void* q_norm_w, const void* k_norm_w,
+                            float norm_eps, void* q_out, void* k_cache, void* v_cache, int64_t num_slots, int M, int heads,
+                            int kv_heads, int head_dim, void* stream);
+
+/* Attention over a part of a long cache.  A span is `span` consecutive tokens of a page (a multiple of 16 that divides block_size).
+ * ssdk_span_bounds: bounds [num_blocks, block_size / span, KV, 2, hd]: per span, key head and channel the smallest and the largest value of
+ * the keys in the context, for the spans that hold one of the last new_tokens tokens of a sequence (more of them than are new costs time only).
+ * Spans on pages outside the cache are passed over. */
+int ssdk_span_bounds(const void* k_cache, const int32_t* block_tables, const int32_t* context_lens, void* bounds, int batch,
+                     int new_tokens, int kv_heads, int head_dim, int block_size, int max_blocks_per_seq, int64_t num_blocks,
+                     int span, void* stream);
+/* ssdk_select_spans: per sequence and key head the `count` spans to read, int32 [batch, KV, count], ascending, -1 behind the last: the first
+ * `first` and the last `last` spans of the context, then those with the largest score = max over the query rows of (sequence, key head) of
+ * sum_d max(q_d lo_d, q_d hi_d), which no key of the span exceeds; scores in 64 bits, the lowest index among equal ones, NaN above all.
+ * Spans on pages outside the cache are never listed.  Tables hold at most 24576 spans. */
+int ssdk_select_spans(const void* q, const void* bounds, const int32_t* block_tables, const int32_t* context_lens, int32_t* selected,
+                      int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size,
+                      int max_blocks_per_seq, int64_t num_blocks, int span, int count, int first, int last, void* stream);
+/* ssdk_span_attn: ssdk_paged_attn over the keys of the listed spans only.  Entries outside the context, or on pages outside the cache, are
+ * passed over; a span that is listed twice counts twice; a row that sees no key is zero.  At most 32 query heads to a key head, 4096 spans. */
+int ssdk_span_attn(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables, const int32_t* context_lens,
+                   const int32_t* selected, void* out, int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size,
+                   int max_blocks_per_seq, int64_t num_blocks, int span, int count, float scale, void* stream);
+
 /* Sampler.forward (layers/sampler.py:14-36): greedy where temp==0, else
  * argmax(softmax(l/T) / Exp(1)) with Philox(seed, step_id) exponentials.
  * logits bf16 [B, V] with row stride ld (elements); out int64 [B]. */

@@ -20,6 +20,7 @@
 //   and the default carve-out one CTA of eight warps was resident and the SMs issued 43 % of the time.
 // The grid is static (CUDA-graph friendly): each CTA derives its chunk range from context_lens[] at run time.
 #pragma once
+#include "async_copy.cuh"
 #include "common.cuh"
 
 namespace ssdk {
@@ -49,26 +50,6 @@ struct AttnParams {
   int pages;                     // of the caches, if they are known (0: nothing is asked for ahead)
 };
 
-SSDK_DEVINL void cp_async16(void* smem_dst, const void* gsrc, bool valid) {
-  const int sz = valid ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem_dst)), "l"(gsrc), "r"(sz)
-               : "memory");
-}
-SSDK_DEVINL void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-SSDK_DEVINL void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-SSDK_DEVINL void ldmatrix_x4(uint32_t* r, const void* smem_row) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(smem_u32(smem_row)));
-}
-SSDK_DEVINL void ldmatrix_x4_trans(uint32_t* r, const void* smem_row) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(smem_u32(smem_row)));
-}
 // OCC: CTAs that are to fit an SM
 template <int HD, int MT, int OCC>
 __global__ void __launch_bounds__(attn_warps(MT) * 32, OCC) paged_attn_kernel(AttnParams p) {

@@ -1,0 +1,180 @@
+// cache_ops.cu — entry points (include/ssdk.h) of the operators of cache_ops.cuh and span_ops.cuh.
+#include <atomic>
+#include <algorithm>
+#include <cstring>
+
+#include "../../include/ssdk.h"
+#include "cache_ops.cuh"
+#include "host.cuh"
+#include "span_ops.cuh"
+
+using namespace ssdk;
+typedef __nv_bfloat16 bf16;
+
+static bool off16(const void* a, const void* b = nullptr, const void* c = nullptr, const void* d = nullptr) {
+  return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) & 15) != 0;
+}
+// a cache whose slots are numbered in 32 bits, and tables over it
+static int check_pages(const char* who, int batch, int block_size, int max_blocks, int64_t num_blocks) {
+  if (batch < 1 || batch > 65535 || block_size < 1 || max_blocks < 1 || num_blocks < 1)
+    return fail("%s: batch=%d, pages of %d, %d to a sequence, %lld in all", who, batch, block_size, max_blocks, (long long)num_blocks);
+  if ((int64_t)max_blocks * block_size >= (1ll << 31) - 65536 || num_blocks * block_size >= (1ll << 31))
+    return fail("%s: tables of %d pages or a cache of %lld of %d tokens pass 32 bits", who, max_blocks, (long long)num_blocks, block_size);
+  return 0;
+}
+static int check_spans(const char* who, int heads, int kv_heads, int head_dim, int block_size, int span) {
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads || kv_heads > 65535 || (head_dim != 64 && head_dim != 128))
+    return fail("%s: %d heads over %d of %d (64 or 128)", who, heads, kv_heads, head_dim);
+  if (span < 16 || span % 16 || block_size % span) return fail("%s: spans of %d tokens (multiples of 16 that divide pages of %d)", who, span, block_size);
+  return 0;
+}
+// the attributes that a kernel needs, once per device
+template <typename Kernel>
+static int with_smem(Kernel* kernel, int bytes, std::atomic<bool>* done) {
+  int dev = 0;
+  CK(cudaGetDevice(&dev));
+  if (dev < 64 && done[dev].load(std::memory_order_acquire)) return 0;
+  CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  CK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  if (dev < 64) done[dev].store(true, std::memory_order_release);
+  return 0;
+}
+
+template <int HD>
+static int launch_rope_axes(Launcher& L, const RopeAxesParams& p) {
+  constexpr int GROUPS = kRopeAxesThreads / (HD / 16);
+  const int n = p.heads + 2 * p.kv_heads, groups = (n + GROUPS - 1) / GROUPS;
+  const int nh = (int64_t)p.M * groups <= 1024 ? 1 : (groups >= 4 ? 4 : groups >= 2 ? 2 : 1);
+  const dim3 grid(p.M, (groups + nh - 1) / nh);
+  if (nh == 1) return L.go(rope_axes_kernel<HD, 1>, grid, dim3(kRopeAxesThreads), 0, p);
+  if (nh == 2) return L.go(rope_axes_kernel<HD, 2>, grid, dim3(kRopeAxesThreads), 0, p);
+  return L.go(rope_axes_kernel<HD, 4>, grid, dim3(kRopeAxesThreads), 0, p);
+}
+
+constexpr int kMaxListed = 4096;   // spans of a list
+template <int HD, int MT>
+static int launch_span_attn(Launcher& L, const SpanAttnParams& p, int tiles) {
+  static std::atomic<bool> done[64];
+  CKI(with_smem(span_attn_kernel<HD, MT>, span_attn_smem(HD, kMaxListed), done));
+  return L.go(span_attn_kernel<HD, MT>, dim3(p.kv_heads, p.B, tiles), dim3(kSpanWarps * 32), span_attn_smem(HD, p.count), p);
+}
+
+template <int HD>
+static int launch_select(Launcher& L, const SelectParams& p, int64_t max_spans) {
+  static std::atomic<bool> done[64];
+  CKI(with_smem(span_select_kernel<HD>, kMaxSpans * 8, done));
+  return L.go(span_select_kernel<HD>, dim3(p.kv_heads, p.B), dim3(kPickThreads), (size_t)max_spans * 8, p);
+}
+
+extern "C" {
+
+int ssdk_place_tokens(const int32_t* context_lens, const int32_t* new_lens, int32_t* block_tables, const int32_t* free_blocks,
+                      const int32_t* free_used, int64_t* positions, int32_t* slot_mapping, int32_t* row_seqs, int32_t* cu_rows,
+                      int32_t* lens, int32_t* used, int batch, int max_blocks_per_seq, int n_free, int rows, int block_size,
+                      int64_t num_blocks, void* stream) {
+  CKI(check_pages("place_tokens", batch, block_size, max_blocks_per_seq, num_blocks));
+  if (batch > kPlaceMaxSeqs || rows < 1 || n_free < 0) return fail("place_tokens: %d sequences (at most %d), %d rows, %d free pages", batch, kPlaceMaxSeqs, rows, n_free);
+  if (!context_lens || !new_lens || !block_tables || !free_used || (n_free && !free_blocks) || !positions || !slot_mapping || !row_seqs || !cu_rows || !lens || !used)
+    return fail("place_tokens: null argument");
+  PlaceParams p;
+  p.ctx = context_lens; p.fresh = new_lens; p.tables = block_tables; p.free_blocks = free_blocks; p.free_used = free_used;
+  p.positions = positions; p.slots = slot_mapping; p.seqs = row_seqs; p.cu = cu_rows; p.lens = lens; p.used = used;
+  p.B = batch; p.max_blocks = max_blocks_per_seq; p.n_free = n_free; p.rows = rows; p.block_size = block_size; p.num_blocks = (int)num_blocks;
+  Launcher L;
+  L.st = (cudaStream_t)stream;
+  static std::atomic<bool> done[64];
+  if (place_smem(batch) > 48000) CKI(with_smem(place_tokens_kernel, place_smem(kPlaceMaxSeqs), done));
+  return L.go(place_tokens_kernel, dim3(std::min((rows + kPlaceThreads - 1) / kPlaceThreads, 148)), dim3(kPlaceThreads), place_smem(batch), p);
+}
+
+int ssdk_rope_axes_store_kv(const void* qkv, const int64_t* positions, int axes, const uint8_t* axis_of, const int32_t* slot_mapping,
+                            const float* rope_table, int64_t max_pos, int rot_dim, const void* q_norm_w, const void* k_norm_w,
+                            float norm_eps, void* q_out, void* k_cache, void* v_cache, int64_t num_slots, int M, int heads,
+                            int kv_heads, int head_dim, void* stream) {
+  if (M < 1 || heads < 1 || kv_heads < 1 || (head_dim != 64 && head_dim != 128 && head_dim != 256))
+    return fail("rope_axes: %d rows of %d heads over %d of %d (64, 128 or 256)", M, heads, kv_heads, head_dim);
+  if (rot_dim < 16 || rot_dim % 16 || rot_dim > head_dim) return fail("rope_axes: %d rotated channels of %d (a multiple of 16)", rot_dim, head_dim);
+  if (axes < 1 || axes > 4 || max_pos < 1 || num_slots < 1) return fail("rope_axes: %d axes (1 to 4), %lld positions, %lld slots", axes, (long long)max_pos, (long long)num_slots);
+  if (heads + 2 * (int64_t)kv_heads > 65535) return fail("rope_axes: too many heads");
+  if (!qkv || !positions || !axis_of || !slot_mapping || !rope_table || !q_out || !k_cache || !v_cache) return fail("rope_axes: null argument");
+  if (off16(qkv, q_out, k_cache, v_cache) || off16(q_norm_w, k_norm_w)) return fail("rope_axes: arrays must start at multiples of 16 bytes");
+  RopeAxesParams p;
+  memset(&p, 0, sizeof(p));
+  for (int i = 0; i < rot_dim / 2; ++i) {
+    if (axis_of[i] >= axes) return fail("rope_axes: frequency %d on axis %d of %d", i, axis_of[i], axes);
+    p.axis_of[i >> 4] |= (uint32_t)axis_of[i] << (2 * (i & 15));
+  }
+  p.qkv = (const bf16*)qkv; p.positions = positions; p.slots = slot_mapping; p.table = rope_table;
+  p.q_norm_w = (const bf16*)q_norm_w; p.k_norm_w = (const bf16*)k_norm_w; p.eps = norm_eps;
+  p.q = (bf16*)q_out; p.k_cache = (bf16*)k_cache; p.v_cache = (bf16*)v_cache;
+  p.top = max_pos; p.num_slots = num_slots; p.M = M; p.heads = heads; p.kv_heads = kv_heads; p.rot = rot_dim; p.axes = axes;
+  Launcher L;
+  L.st = (cudaStream_t)stream;
+  if (head_dim == 64) return launch_rope_axes<64>(L, p);
+  if (head_dim == 128) return launch_rope_axes<128>(L, p);
+  return launch_rope_axes<256>(L, p);
+}
+
+int ssdk_span_bounds(const void* k_cache, const int32_t* block_tables, const int32_t* context_lens, void* bounds, int batch,
+                     int new_tokens, int kv_heads, int head_dim, int block_size, int max_blocks_per_seq, int64_t num_blocks,
+                     int span, void* stream) {
+  CKI(check_pages("span_bounds", batch, block_size, max_blocks_per_seq, num_blocks));
+  CKI(check_spans("span_bounds", kv_heads, kv_heads, head_dim, block_size, span));
+  if (new_tokens < 1) return fail("span_bounds: %d new tokens", new_tokens);
+  if (!k_cache || !block_tables || !context_lens || !bounds) return fail("span_bounds: null argument");
+  if (off16(k_cache, bounds)) return fail("span_bounds: arrays must start at multiples of 16 bytes");
+  SpanBoundsParams p;
+  p.k_cache = (const bf16*)k_cache; p.tables = block_tables; p.lens = context_lens; p.bounds = (bf16*)bounds; p.num_blocks = num_blocks;
+  p.B = batch; p.max_blocks = max_blocks_per_seq; p.block_size = block_size; p.span = span; p.kv_heads = kv_heads; p.head_dim = head_dim;
+  p.fresh = (int)std::min<int64_t>(new_tokens, (int64_t)max_blocks_per_seq * block_size);
+  Launcher L;
+  L.st = (cudaStream_t)stream;
+  return L.go(span_bounds_kernel, dim3((p.fresh + span - 2) / span + 1, batch), dim3(kBoundsThreads), 0, p);
+}
+
+int ssdk_select_spans(const void* q, const void* bounds, const int32_t* block_tables, const int32_t* context_lens, int32_t* selected,
+                      int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size,
+                      int max_blocks_per_seq, int64_t num_blocks, int span, int count, int first, int last, void* stream) {
+  CKI(check_pages("select_spans", batch, block_size, max_blocks_per_seq, num_blocks));
+  CKI(check_spans("select_spans", heads, kv_heads, head_dim, block_size, span));
+  if (q_len < 1 || count < 1 || count > kMaxListed || first < 0 || last < 0 || (int64_t)first + last > count)
+    return fail("select_spans: q_len=%d, %d spans (at most %d), of them the first %d and the last %d", q_len, count, kMaxListed, first, last);
+  if (!q || !bounds || !block_tables || !context_lens || !selected) return fail("select_spans: null argument");
+  if (off16(q, bounds)) return fail("select_spans: arrays must start at multiples of 16 bytes");
+  const int64_t max_spans = (int64_t)max_blocks_per_seq * (block_size / span);
+  if (max_spans > kMaxSpans) return fail("select_spans: tables of %lld spans (at most %d)", (long long)max_spans, kMaxSpans);
+  SelectParams p;
+  p.q = (const bf16*)q; p.bounds = (const bf16*)bounds; p.tables = block_tables; p.lens = context_lens; p.out = selected;
+  p.num_blocks = num_blocks; p.B = batch; p.Q = q_len; p.heads = heads; p.kv_heads = kv_heads;
+  p.block_size = block_size; p.span = span; p.max_blocks = max_blocks_per_seq;
+  p.count = count; p.first = first; p.last = last;
+  Launcher L;
+  L.st = (cudaStream_t)stream;
+  return head_dim == 64 ? launch_select<64>(L, p, max_spans) : launch_select<128>(L, p, max_spans);
+}
+
+int ssdk_span_attn(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables, const int32_t* context_lens,
+                   const int32_t* selected, void* out, int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size,
+                   int max_blocks_per_seq, int64_t num_blocks, int span, int count, float scale, void* stream) {
+  CKI(check_pages("span_attn", batch, block_size, max_blocks_per_seq, num_blocks));
+  CKI(check_spans("span_attn", heads, kv_heads, head_dim, block_size, span));
+  const int G = heads / kv_heads;
+  if (q_len < 1 || count < 1 || count > kMaxListed || G > 32 || !(scale == scale))
+    return fail("span_attn: q_len=%d, %d spans (at most %d), %d query heads to a key head (at most 32)", q_len, count, kMaxListed, G);
+  if (!q || !k_cache || !v_cache || !block_tables || !context_lens || !selected || !out) return fail("span_attn: null argument");
+  if (off16(q, k_cache, v_cache, out)) return fail("span_attn: arrays must start at multiples of 16 bytes");
+  SpanAttnParams p;
+  p.q = (const bf16*)q; p.k_cache = (const bf16*)k_cache; p.v_cache = (const bf16*)v_cache; p.tables = block_tables; p.lens = context_lens;
+  p.spans = selected; p.out = (bf16*)out; p.num_blocks = num_blocks; p.B = batch; p.Q = q_len; p.heads = heads; p.kv_heads = kv_heads;
+  p.block_size = block_size; p.span = span; p.max_blocks = max_blocks_per_seq; p.count = count; p.scale_log2 = scale * 1.4426950408889634f;
+  const bool one = G * q_len <= 16;
+  const int most = (one ? 16 : 32) / G, tiles = (q_len + most - 1) / most;
+  if (tiles > 65535) return fail("span_attn: q_len=%d", q_len);
+  p.tokens = (q_len + tiles - 1) / tiles;
+  Launcher L;
+  L.st = (cudaStream_t)stream;
+  if (head_dim == 64) return one ? launch_span_attn<64, 1>(L, p, tiles) : launch_span_attn<64, 2>(L, p, tiles);
+  return one ? launch_span_attn<128, 1>(L, p, tiles) : launch_span_attn<128, 2>(L, p, tiles);
+}
+
+}  // extern "C"

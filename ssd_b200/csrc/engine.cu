@@ -23,6 +23,7 @@
 #include "gemm.cuh"
 #include "gemm_few.cuh"
 #include "gemm_pair.cuh"
+#include "host.cuh"
 #include "prompt_attention.cuh"
 #include "gemm_split.cuh"
 #include "sampling.cuh"
@@ -30,71 +31,6 @@
 
 using namespace ssdk;
 typedef __nv_bfloat16 bf16;
-
-// ------------------------------------------------------------------------------------------
-// errors
-// ------------------------------------------------------------------------------------------
-static thread_local std::string g_err;
-static int fail(const char* fmt, ...) {
-  char buf[1024];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  g_err = buf;
-  return -1;
-}
-#define CK(expr)                                                                              \
-  do {                                                                                        \
-    cudaError_t _e = (expr);                                                                  \
-    if (_e != cudaSuccess) return fail("%s:%d %s -> %s", __FILE__, __LINE__, #expr, cudaGetErrorString(_e)); \
-  } while (0)
-#define CKN(expr)                                                                             \
-  do {                                                                                        \
-    ncclResult_t _e = (expr);                                                                 \
-    if (_e != ncclSuccess) return fail("%s:%d %s -> nccl error %d", __FILE__, __LINE__, #expr, (int)_e); \
-  } while (0)
-#define CKI(expr)                 \
-  do {                            \
-    int _r = (expr);              \
-    if (_r != 0) return _r;       \
-  } while (0)
-
-static int env_int(const char* name, int dflt) {
-  const char* s = getenv(name);
-  return (s && *s) ? atoi(s) : dflt;
-}
-
-// ------------------------------------------------------------------------------------------
-// launch helper (optional programmatic dependent launch)
-// ------------------------------------------------------------------------------------------
-struct Launcher {
-  cudaStream_t st = nullptr;
-  unsigned* gave_up = nullptr;   // the engine's word for waits that run out (WaitWord)
-  bool pdl = false;       // PDL enabled at all
-  bool prev_kernel = false;  // the previous op on the stream was one of our kernels
-  int64_t count = 0;
-
-  template <typename... KArgs, typename... Args>
-  int go(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = (pdl && prev_kernel) ? 1 : 0;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
-    if (e != cudaSuccess) return fail("kernel launch failed: %s", cudaGetErrorString(e));
-    prev_kernel = true;
-    ++count;
-    return 0;
-  }
-  void barrier_op() { prev_kernel = false; }  // memcpy / NCCL / anything that is not our kernel
-};
 
 // ------------------------------------------------------------------------------------------
 // TMA descriptors

@@ -173,3 +173,143 @@ def verify(logits_p: torch.Tensor, logits_q: torch.Tensor, speculations: torch.T
                              _ptr(temperatures_draft), _ptr(hits), int(jit_speculate), B, K, V, seed, step_id, _ptr(n_acc),
                              _ptr(rec), _ptr(scratch), _stream()), "ssdk_verify")
     return n_acc, rec
+
+
+# ---- around a long paged cache: places of a step's tokens, positions with several axes, attention over selected spans ----
+_BF, _I32, _I64, _F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
+
+
+def _check(name: str, *args):
+    """(tensor, its name, dtype, shape with -1 for any size) of every argument; returns their device."""
+    dev = args[0][0].device
+    for t, what, dtype, shape in args:
+        if t.dtype is not dtype:
+            raise TypeError(f"{name}: {what}: expected {dtype}, got {t.dtype}")
+        if t.dim() != len(shape) or any(n not in (-1, have) for n, have in zip(shape, t.shape)):
+            raise ValueError(f"{name}: {what}: expected shape {shape}, got {tuple(t.shape)}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name}: {what}: must be contiguous")
+        if t.device != dev:
+            raise ValueError(f"{name}: {what}: on {t.device}, {args[0][1]} on {dev}")
+    if dev.type != "cuda":
+        raise RuntimeError(f"{name}: CUDA tensors required (libssdk has no CPU path)")
+    return dev
+
+
+def _launch(name: str, dev: torch.device, *args):
+    """One entry point of libssdk on the current stream of the tensors' device."""
+    fn = getattr(_L.load(), name)
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc:
+        _L.check(rc, name)
+
+
+def place_tokens(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor, free_blocks: torch.Tensor,
+                 free_used: torch.Tensor, rows: int, block_size: int, num_blocks: int):
+    """Pages, positions and slots of a step's tokens from the lengths of its requests, without the host (BlockManager and
+    prepare_decode / prepare_prefill: engine/block_manager.py, engine/helpers/runner_helpers.py:50-121).
+
+    context_lens, new_lens int32 [B]: tokens in the cache, and tokens to come; block_tables int32 [B, max_blocks], completed in
+    place; free_blocks int32 [F]: pages to hand out, the first free_used (int32 [1]) of which are gone; rows: room for new tokens.
+    Returns positions int64 [rows], slot_mapping int32 [rows], row_seqs int32 [rows] (rows behind the last token: 0, -1, -1),
+    cu_rows int32 [B + 1], lens int32 [B] (context_lens + new_lens; sequences that found no pages or rows: context_lens) and the
+    new free_used.  Sequences are served in order, each as a whole: see ssdk_place_tokens (include/ssdk.h)."""
+    B = context_lens.shape[0]
+    dev = _check("place_tokens", (context_lens, "context_lens", _I32, (B,)), (new_lens, "new_lens", _I32, (B,)),
+                 (block_tables, "block_tables", _I32, (B, -1)), (free_blocks, "free_blocks", _I32, (-1,)), (free_used, "free_used", _I32, (1,)))
+    positions = torch.empty(max(rows, 0), dtype=_I64, device=dev)
+    words = torch.empty(2 * positions.shape[0] + 2 * B + 2, dtype=_I32, device=dev)
+    slots, seqs, cu, lens, used = words.split((positions.shape[0], positions.shape[0], B + 1, B, 1))
+    _launch("ssdk_place_tokens", dev, context_lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(), free_blocks.data_ptr(), free_used.data_ptr(),
+            positions.data_ptr(), slots.data_ptr(), seqs.data_ptr(), cu.data_ptr(), lens.data_ptr(), used.data_ptr(), B, block_tables.shape[1],
+            free_blocks.shape[0], rows, block_size, num_blocks)
+    return positions, slots, seqs, cu, lens, used
+
+
+def rope_axes_store_kv(qkv: torch.Tensor, positions: torch.Tensor, axis_of, slot_mapping: torch.Tensor, rope_table: torch.Tensor,
+                       k_cache: torch.Tensor, v_cache: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
+                       q_norm_w: torch.Tensor | None = None, k_norm_w: torch.Tensor | None = None, norm_eps: float = 1e-6) -> torch.Tensor:
+    """rope_store_kv with positions on several axes (time, height and width of images and video).
+
+    positions int64 [axes, M], 1 to 4 axes; axis_of: the axis that each frequency turns by (rot_dim / 2 whole numbers, e.g.
+    [0] * 16 + [1] * 24 + [2] * 24); rope_table fp32 [max_pos, rot_dim] cos | sin: the first rot_dim channels of a head turn.
+    Norms and rotation in fp32 with one rounding.  Returns q [M, heads * head_dim]; keys and values are in their slots.  A row with a position
+    outside the table has NaN queries and stores nothing; slots are distinct, those outside the cache store nothing."""
+    M, rot = qkv.shape[0], rope_table.shape[-1]
+    cache = (k_cache.shape[0], k_cache.shape[1], kv_heads, head_dim) if k_cache.dim() == 4 else (-1, -1, kv_heads, head_dim)
+    args = [(qkv, "qkv", _BF, (M, (heads + 2 * kv_heads) * head_dim)), (positions, "positions", _I64, (-1, M)), (slot_mapping, "slot_mapping", _I32, (M,)),
+            (rope_table, "rope_table", _F32, (-1, rot)), (k_cache, "k_cache", _BF, cache), (v_cache, "v_cache", _BF, cache)]
+    for w, what in ((q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w")):
+        if w is not None:
+            args.append((w, what, _BF, (head_dim,)))
+    axis_of = bytes(axis_of)
+    if len(axis_of) * 2 != rot:
+        raise ValueError(f"rope_axes_store_kv: axis_of has {len(axis_of)} frequencies, rope_table {rot / 2}")
+    dev = _check("rope_axes_store_kv", *args)
+    q = torch.empty(M, heads * head_dim, dtype=_BF, device=dev)
+    _launch("ssdk_rope_axes_store_kv", dev, qkv.data_ptr(), positions.data_ptr(), positions.shape[0], axis_of, slot_mapping.data_ptr(), rope_table.data_ptr(),
+            rope_table.shape[0], rot, _ptr(q_norm_w), _ptr(k_norm_w), norm_eps, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            k_cache.shape[0] * k_cache.shape[1], M, heads, kv_heads, head_dim)
+    return q
+
+
+def span_bounds(bounds: torch.Tensor, k_cache: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor, new_tokens: int) -> torch.Tensor:
+    """Smallest and largest value of every channel over the keys of a span, for the spans that hold one of the last new_tokens
+    tokens of each sequence (at least the tokens stored since the last call; more costs time only).
+
+    bounds [num_blocks, block_size / span, KV, 2, hd] bf16, in place: its second size says how many spans a page has; k_cache
+    [num_blocks, block_size, KV, hd]; context_lens int32 [B] with the new tokens.  Returns bounds."""
+    n, block_size, KV, hd = k_cache.shape if k_cache.dim() == 4 else (-1,) * 4
+    subs = bounds.shape[1] if bounds.dim() == 5 else -1
+    B = context_lens.shape[0]
+    if subs == 0 or block_size % subs:
+        raise ValueError(f"span_bounds: pages of {block_size} tokens in {subs} spans")
+    dev = _check("span_bounds", (bounds, "bounds", _BF, (n, subs, KV, 2, hd)), (k_cache, "k_cache", _BF, (n, block_size, KV, hd)),
+                 (block_tables, "block_tables", _I32, (B, -1)), (context_lens, "context_lens", _I32, (B,)))
+    _launch("ssdk_span_bounds", dev, k_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), bounds.data_ptr(), B, new_tokens, KV, hd,
+            block_size, block_tables.shape[1], n, block_size // subs)
+    return bounds
+
+
+def select_spans(q: torch.Tensor, bounds: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor, q_len: int, block_size: int,
+                 count: int, first: int = 1, last: int | None = None) -> torch.Tensor:
+    """The `count` spans of each sequence's cache that its queries are to read, per key head: the first `first` and the last
+    `last` ones (None: as many as q_len tokens can lie in, if count has room), then those that a query of the group can score highest with,
+    max over its rows of sum_d max(q_d lo_d, q_d hi_d).
+
+    q [B * q_len, H, hd] bf16 (rotated); bounds as span_bounds keeps them.  Returns int32 [B, KV, count], ascending, -1 behind the
+    last: what span_attention takes.  The rows of a sequence share their spans."""
+    n, subs, KV, two, hd = bounds.shape if bounds.dim() == 5 else (-1,) * 5
+    B = context_lens.shape[0]
+    if subs == 0 or block_size % subs:
+        raise ValueError(f"select_spans: pages of {block_size} tokens in {subs} spans")
+    dev = _check("select_spans", (q, "q", _BF, (B * q_len, -1, hd)), (bounds, "bounds", _BF, (n, subs, KV, 2, hd)),
+                 (block_tables, "block_tables", _I32, (B, -1)), (context_lens, "context_lens", _I32, (B,)))
+    span = block_size // subs
+    if last is None:
+        last = min((q_len + span - 2) // span + 1, count - first)
+    out = torch.empty(B, KV, max(count, 0), dtype=_I32, device=dev)
+    _launch("ssdk_select_spans", dev, q.data_ptr(), bounds.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(),
+            B, q_len, q.shape[1], KV, hd, block_size, block_tables.shape[1], n, span, count, first, last)
+    return out
+
+
+def span_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
+                   spans: torch.Tensor, span: int, q_len: int, scale: float) -> torch.Tensor:
+    """paged_attention over the keys of the listed spans only: spans int32 [B, KV, count] (select_spans), `span` tokens each.
+
+    q [B * q_len, H, hd]; returns [B * q_len, H * hd].  Entries outside the context are passed over, a span listed twice counts twice, a row
+    that sees no key is zero."""
+    n, block_size, KV, hd = k_cache.shape if k_cache.dim() == 4 else (-1,) * 4
+    B = context_lens.shape[0]
+    dev = _check("span_attention", (q, "q", _BF, (B * q_len, -1, hd)), (k_cache, "k_cache", _BF, (n, block_size, KV, hd)),
+                 (v_cache, "v_cache", _BF, (n, block_size, KV, hd)), (block_tables, "block_tables", _I32, (B, -1)),
+                 (context_lens, "context_lens", _I32, (B,)), (spans, "spans", _I32, (B, KV, -1)))
+    out = torch.empty(q.shape[0], q.shape[1] * hd, dtype=_BF, device=dev)
+    _launch("ssdk_span_attn", dev, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), spans.data_ptr(),
+            out.data_ptr(), B, q_len, q.shape[1], KV, hd, block_size, block_tables.shape[1], n, span, spans.shape[2], scale)
+    return out
