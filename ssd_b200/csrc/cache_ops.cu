@@ -51,6 +51,7 @@ static int launch_rope_axes(Launcher& L, const RopeAxesParams& p) {
   return L.go(rope_axes_kernel<HD, 4>, grid, dim3(kRopeAxesThreads), 0, p);
 }
 
+constexpr int kSms = 148;
 constexpr int kMaxListed = 4096;   // spans of a list
 template <int HD, int MT>
 static int launch_span_attn(Launcher& L, const SpanAttnParams& p, int tiles) {
@@ -59,11 +60,13 @@ static int launch_span_attn(Launcher& L, const SpanAttnParams& p, int tiles) {
   return L.go(span_attn_kernel<HD, MT>, dim3(p.kv_heads, p.B, tiles), dim3(kSpanWarps * 32), span_attn_smem(HD, p.count), p);
 }
 
+// blocks of a cluster: two per SM, as long as each of their warps has spans to score
 template <int HD>
-static int launch_select(Launcher& L, const SelectParams& p, int64_t max_spans) {
+static int launch_select(Launcher& L, const SelectParams& p) {
   static std::atomic<bool> done[64];
-  CKI(with_smem(span_select_kernel<HD>, kMaxSpans * 8, done));
-  return L.go(span_select_kernel<HD>, dim3(p.kv_heads, p.B), dim3(kPickThreads), (size_t)max_spans * 8, p);
+  CKI(with_smem(span_select_kernel<HD>, select_smem(kMaxSpans), done));
+  while (L.cluster < 8 && (int64_t)p.B * p.kv_heads * L.cluster < 2 * kSms && L.cluster * kPickWarps * 8 < p.max_spans) L.cluster *= 2;
+  return L.go(span_select_kernel<HD>, dim3(p.kv_heads * L.cluster, p.B), dim3(kPickThreads), select_smem(p.max_spans), p);
 }
 
 extern "C" {
@@ -146,11 +149,11 @@ int ssdk_select_spans(const void* q, const void* bounds, const int32_t* block_ta
   SelectParams p;
   p.q = (const bf16*)q; p.bounds = (const bf16*)bounds; p.tables = block_tables; p.lens = context_lens; p.out = selected;
   p.num_blocks = num_blocks; p.B = batch; p.Q = q_len; p.heads = heads; p.kv_heads = kv_heads;
-  p.block_size = block_size; p.span = span; p.max_blocks = max_blocks_per_seq;
+  p.block_size = block_size; p.span = span; p.max_blocks = max_blocks_per_seq; p.max_spans = (int)max_spans;
   p.count = count; p.first = first; p.last = last;
   Launcher L;
   L.st = (cudaStream_t)stream;
-  return head_dim == 64 ? launch_select<64>(L, p, max_spans) : launch_select<128>(L, p, max_spans);
+  return head_dim == 64 ? launch_select<64>(L, p) : launch_select<128>(L, p);
 }
 
 int ssdk_span_attn(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables, const int32_t* context_lens,

@@ -1,5 +1,7 @@
 // span_ops.cuh — attention over a part of a long paged cache: spans of keys are chosen by a bound on their scores, and attention reads the chosen ones only.
 #pragma once
+#include <cooperative_groups.h>
+
 #include "async_copy.cuh"
 #include "cache_ops.cuh"
 #include "common.cuh"
@@ -7,9 +9,16 @@
 namespace ssdk {
 
 // ----------------------------------------------------------------------------------
-// select_spans: the score of span s for key head g is the largest over the query rows r of (sequence, g) of
-//   sum_d max(q[r, d] lo[s, d], q[r, d] hi[s, d])  >=  max over the span's keys of q[r] . k,
-// in 64 bits: products of bf16 values are exact, and sums of a head's size are off by less than two scores of different spans are apart.
+// span_select_kernel: the score of span s for key head g is the largest over the query rows r of (sequence, g) of
+//   sum_d max(q[r, d] lo[s, d], q[r, d] hi[s, d])  >=  max over the span's keys of q[r] . k.
+// Listed are the first and the last spans, then the best by score, the lowest index first among equal ones.  Scores count in 64 bits: 32 would let spans
+// change places whose scores differ in the last bits.
+// Bound by the bytes of the bounds.  The sum is a product, [min(q, 0) | max(q, 0)] . [lo | hi], so the tensor cores make an estimate of every score: a warp
+// takes eight spans, whose 16-byte loads are the fragments of mma.m16n8k16 (channels permuted alike on both sides), rows as its m.  The estimate is off by at
+// most eps = 2^-14 max_r sum_d |q[r, d]| max |lo, hi|: 2 hd / 16 steps, each adding 17 numbers with 2^-22 of the terms' size lost.  With t the want-th largest
+// estimate, a span above t + 2 eps is taken, one under t - 2 eps is not, and only the few in between are scored in 64 bits (products of bf16 values
+// are exact, sums of 128 of them off by 2^-46).  Where values are not finite, or so large that 32 bits overflow, all spans are.
+// A cluster of blocks shares a key head of a sequence: estimates go to the first block's shared memory, which picks.
 // ----------------------------------------------------------------------------------
 struct SelectParams {
   const __nv_bfloat16* q;        // [B * Q, H, hd]
@@ -18,10 +27,15 @@ struct SelectParams {
   const int32_t* lens;           // [B]
   int32_t* out;                  // [B, KV, count]
   int64_t num_blocks;
-  int B, Q, heads, kv_heads, block_size, span, max_blocks, count, first, last;
+  int B, Q, heads, kv_heads, block_size, span, max_blocks, max_spans, count, first, last;
 };
-constexpr int kPickThreads = 1024;
+constexpr int kPickThreads = 256, kPickWarps = kPickThreads / 32;
 constexpr int kMaxSpans = 24576;   // of a sequence
+constexpr int kPickBins = 2048;
+constexpr int kPickRanked = 256;   // spans between, up to which each is compared with each
+// scores (64 bits; before them the estimates) | taken | between (a bit per span) | bins, then the spans between
+constexpr int select_smem(int spans) { return spans * 8 + 2 * ((spans + 31) / 32) * 4 + kPickBins * 4; }
+constexpr uint32_t kNoSpan = 0xffffffffu;   // estimate of a span that has no page
 
 // 64-bit values in their order as unsigned words; zeros of both signs are one value, NaN is above all.  0 is no value
 SSDK_DEVINL unsigned long long score_key(double s) {
@@ -30,95 +44,368 @@ SSDK_DEVINL unsigned long long score_key(double s) {
   return b < 0 ? ~(unsigned long long)b : (unsigned long long)b | (1ull << 63);
 }
 
-// A block per key head of a sequence: its warps score the spans into shared memory, then the smallest key that is taken is found bit by bit: the
-// first and last spans, then by key, the lowest index first among equal ones.
-template <int HD>
-__global__ void __launch_bounds__(kPickThreads) span_select_kernel(SelectParams p) {
-  constexpr int E = HD / 32;   // channels of a lane
-  SSDK_DYN_SMEM(unsigned long long, keys);   // [n]
-  SSDK_STATIC_SMEM(int, sums, 64);
-  const int g = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, subs = p.block_size / p.span;
-  const int G = p.heads / p.kv_heads, rows = G * p.Q;
-  const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size), n = (len + p.span - 1) / p.span;
-  for (int s = warp; s < n; s += kPickThreads / 32) {
-    unsigned long long key = 0;
-    const int page = page_at(p.tables + (size_t)b * p.max_blocks + s / subs, p.num_blocks);
-    if (page >= 0) {
-      const __nv_bfloat16* both = p.bounds + (((size_t)page * subs + s % subs) * p.kv_heads + g) * 2 * HD;
-      float lo[E], hi[E];
+// the sum of v over the block's threads up to this one, and over all
+SSDK_DEVINL int pick_running_sum(int v, int* words, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        lo[e] = bf2f(both[lane * E + e]);
-        hi[e] = bf2f(both[HD + lane * E + e]);
-      }
-      for (int r = 0; r < rows; ++r) {
-        const __nv_bfloat16* q = p.q + ((size_t)(b * p.Q + r / G) * p.heads + g * G + r % G) * HD + lane * E;
-        double sum = 0.0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const double x = bf2f(q[e]), u = x * lo[e], v = x * hi[e];
-          sum += u != u || v != v ? __longlong_as_double(0x7ff8000000000000ll) : (u > v ? u : v);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        key = max(key, score_key(sum));
-      }
-    }
-    if (lane == 0) keys[s] = key;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
   }
   __syncthreads();
-  auto kept = [&](int s) { return s < p.first || s >= n - p.last; };
-  auto total = [&](int v) {   // over the block
-    v = __reduce_add_sync(0xffffffffu, v);
+  if (lane == 31) words[warp] = v;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kPickWarps; ++w) {
+    const int x = words[w];
+    before += w < warp ? x : 0;
+    all += x;
+  }
+  *total = all;
+  return before + v;
+}
+SSDK_DEVINL int pick_total(int v, int* words) {
+  v = __reduce_add_sync(0xffffffffu, v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int all = 0;
+#pragma unroll
+  for (int w = 0; w < kPickWarps; ++w) all += words[w];
+  return all;
+}
+
+// the spans of a bit map, ascending, then -1
+SSDK_DEVINL void pick_write(const uint32_t* bits, int words, int32_t* out, int count, int* sums) {
+  int done = 0;
+  for (int base = 0; base < words; base += kPickThreads) {
+    const int w = base + threadIdx.x;
+    uint32_t m = w < words ? bits[w] : 0;
+    int all, at = pick_running_sum(__popc(m), sums, &all);
+    at += done - __popc(m);
+    for (; m; m &= m - 1) out[at++] = w * 32 + __ffs(m) - 1;
+    done += all;
+  }
+  for (int i = done + threadIdx.x; i < count; i += kPickThreads) out[i] = -1;
+}
+
+// a warp: the score of one span in 64 bits
+template <int HD>
+SSDK_DEVINL unsigned long long exact_score(const SelectParams& p, int b, int g, int page, int sub) {
+  constexpr int E = HD / 32;   // channels of a lane
+  const int lane = threadIdx.x & 31, G = p.heads / p.kv_heads, rows = G * p.Q, subs = p.block_size / p.span;
+  const __nv_bfloat16* both = p.bounds + (((size_t)page * subs + sub) * p.kv_heads + g) * 2 * HD + lane * E;
+  float lo[E], hi[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    lo[e] = bf2f(both[e]);
+    hi[e] = bf2f(both[HD + e]);
+  }
+  unsigned long long key = 0;
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r) {
+    const __nv_bfloat16* q = p.q + ((size_t)(b * p.Q + r / G) * p.heads + g * G + r % G) * HD + lane * E;
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const double x = bf2f(q[e]), u = x * lo[e], v = x * hi[e];
+      sum += u != u || v != v ? __longlong_as_double(0x7ff8000000000000ll) : (u > v ? u : v);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    key = max(key, score_key(sum));
+  }
+  return key;
+}
+
+SSDK_DEVINL uint4 and4(uint4 v, uint32_t m) { return make_uint4(v.x & m, v.y & m, v.z & m, v.w & m); }
+
+template <int HD>
+__global__ void __launch_bounds__(kPickThreads, 2) span_select_kernel(SelectParams p) {
+  namespace cg = cooperative_groups;
+  constexpr int CH = HD / 32;   // 16-byte pieces of a lane per bound
+  extern __shared__ __align__(16) uint8_t select_smem_bytes[];
+  __shared__ int sums[kPickWarps], pick_bin;
+  __shared__ uint32_t widest;              // bits of the largest |lo|, |hi| (NaN above infinity above all)
+  __shared__ float low[kPickWarps], high[kPickWarps];
+  __shared__ uint32_t q_size[kPickWarps];
+  const int words = (p.max_spans + 31) / 32;
+  unsigned long long* keys = reinterpret_cast<unsigned long long*>(select_smem_bytes);
+  uint32_t* estimate = reinterpret_cast<uint32_t*>(select_smem_bytes);
+  uint32_t* taken = reinterpret_cast<uint32_t*>(keys + p.max_spans);
+  uint32_t* between = taken + words;
+  int* bins = reinterpret_cast<int*>(between + words);
+
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = cluster.num_blocks(), rank = cluster.block_rank();
+  const int head = blockIdx.x / C, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int G = p.heads / p.kv_heads, rows = G * p.Q, subs = p.block_size / p.span;
+  const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size), n = (len + p.span - 1) / p.span;
+  const int32_t* table = p.tables + (size_t)b * p.max_blocks;
+  int32_t* out = p.out + ((size_t)b * p.kv_heads + head) * p.count;
+
+  if (n <= p.count) {   // all of them (the same for every block of the cluster)
+    if (rank) return;
+    for (int base = warp * 32; base < n; base += kPickThreads) {
+      const int s = base + lane;
+      const uint32_t m = __ballot_sync(0xffffffffu, s < n && page_at(table + s / subs, p.num_blocks) >= 0);
+      if (lane == 0) taken[base / 32] = m;
+    }
     __syncthreads();
-    if (lane == 0) sums[warp] = v;
-    __syncthreads();
-    return __reduce_add_sync(0xffffffffu, sums[lane]);
+    pick_write(taken, (n + 31) / 32, out, p.count, sums);
+    return;
+  }
+
+  if (rank == 0) {
+    for (int i = threadIdx.x; i < kPickBins; i += kPickThreads) bins[i] = 0;
+    if (threadIdx.x == 0) widest = 0;
+  }
+  cluster.barrier_arrive();   // every block has started, and the first one's words are set
+  uint32_t* estimate0 = cluster.map_shared_rank(estimate, 0);
+  uint32_t* widest0 = cluster.map_shared_rank(&widest, 0);
+
+  // ---- estimates ----
+  auto load_q = [&](int mt, uint4* q0, uint4* q1) {
+    const int r0 = mt * 16 + g, r1 = r0 + 8;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int c = 8 * (t + 4 * i);
+      q0[i] = r0 < rows ? ld_nc_v4(p.q + ((size_t)(b * p.Q + r0 / G) * p.heads + head * G + r0 % G) * HD + c) : make_uint4(0, 0, 0, 0);
+      q1[i] = r1 < rows ? ld_nc_v4(p.q + ((size_t)(b * p.Q + r1 / G) * p.heads + head * G + r1 % G) * HD + c) : make_uint4(0, 0, 0, 0);
+    }
   };
-  int always = 0, others = 0;
-  for (int s = threadIdx.x; s < n; s += kPickThreads)
-    if (keys[s]) (kept(s) ? always : others) += 1;
-  always = total(always);
-  others = total(others);
-  const int want = min(p.count - always, others);
-  unsigned long long line = 0;   // the want-th largest key
-  int above = 0;
-  if (want > 0) {
-    for (int bit = 63; bit >= 0; --bit) {
-      const unsigned long long tried = line | (1ull << bit);
-      int c = 0;
-      for (int s = threadIdx.x; s < n; s += kPickThreads) c += !kept(s) && keys[s] >= tried;
-      if (total(c) >= want) line = tried;
+  auto load_group = [&](int group, uint4* v) {
+    const int s = group * 8 + g;
+    const int page = s < n ? page_at(table + s / subs, p.num_blocks) : -1;
+    const __nv_bfloat16* both = p.bounds + (((size_t)max(page, 0) * subs + s % subs) * p.kv_heads + head) * 2 * HD + 8 * t;
+#pragma unroll
+    for (int i = 0; i < 2 * CH; ++i) v[i] = page >= 0 ? ld_nc_v4(both + 32 * i) : make_uint4(0, 0, 0, 0);
+    return page >= 0;
+  };
+  const int tiles = (rows + 15) / 16, groups = (n + 7) / 8, step = C * kPickWarps;
+  uint4 q0[CH], q1[CH];
+  load_q(0, q0, q1);
+  uint32_t wide = 0;   // two channels
+  uint4 next[2 * CH];
+  int group = rank * kPickWarps + warp;
+  bool next_there = group < groups ? load_group(group, next) : false;
+  bool waited = false;
+  for (; group < groups; group += step) {
+    uint4 v[2 * CH];
+#pragma unroll
+    for (int i = 0; i < 2 * CH; ++i) v[i] = next[i];
+    const uint32_t there = __ballot_sync(0xffffffffu, next_there);
+    if (group + step < groups) next_there = load_group(group + step, next);
+#pragma unroll
+    for (int i = 0; i < 2 * CH; ++i) {
+      const uint4 a = and4(v[i], 0x7fff7fffu);
+      wide = max_bf16x2(wide, max_bf16x2(max_bf16x2(a.x, a.y), max_bf16x2(a.z, a.w)));
     }
-    for (int s = threadIdx.x; s < n; s += kPickThreads) above += !kept(s) && keys[s] > line;
-    above = total(above);
-  }
-  const int equal = want - above;   // so many of the keys on the line, the first ones
-  int32_t* out = p.out + ((size_t)b * p.kv_heads + g) * p.count;
-  int taken = 0, ties = 0;
-  for (int base = 0; base < n; base += kPickThreads) {
-    const int s = base + threadIdx.x;
-    const unsigned long long key = s < n ? keys[s] : 0;
-    const bool sure = key && (kept(s) || (want > 0 && key > line)), tie = key && !kept(s) && want > 0 && key == line;
-    const unsigned m_sure = __ballot_sync(0xffffffffu, sure), m_tie = __ballot_sync(0xffffffffu, tie), under = (1u << lane) - 1;
-    __syncthreads();
-    if (lane == 0) {
-      sums[warp] = __popc(m_sure);
-      sums[32 + warp] = __popc(m_tie);
-    }
-    __syncthreads();
-    int sure_before = taken + __popc(m_sure & under), tie_before = ties + __popc(m_tie & under);
-    for (int w = 0; w < 32; ++w) {
-      if (w < warp) {
-        sure_before += sums[w];
-        tie_before += sums[32 + w];
+    float best[2] = {-INFINITY, -INFINITY};   // spans 2 t, 2 t + 1
+    for (int mt = 0; mt < tiles; ++mt) {
+      if (tiles > 1) load_q(mt, q0, q1);
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 2 * CH; ++i) {
+        const uint4 u = q0[i % CH], w = q1[i % CH];
+        uint32_t a[4];
+        // lower bounds meet the negative parts of the query, upper bounds the positive ones
+        a[0] = i < CH ? min_bf16x2(u.x, 0u) : max_bf16x2(u.x, 0u);
+        a[1] = i < CH ? min_bf16x2(w.x, 0u) : max_bf16x2(w.x, 0u);
+        a[2] = i < CH ? min_bf16x2(u.y, 0u) : max_bf16x2(u.y, 0u);
+        a[3] = i < CH ? min_bf16x2(w.y, 0u) : max_bf16x2(w.y, 0u);
+        mma_bf16_16816(c, a, v[i].x, v[i].y);
+        a[0] = i < CH ? min_bf16x2(u.z, 0u) : max_bf16x2(u.z, 0u);
+        a[1] = i < CH ? min_bf16x2(w.z, 0u) : max_bf16x2(w.z, 0u);
+        a[2] = i < CH ? min_bf16x2(u.w, 0u) : max_bf16x2(u.w, 0u);
+        a[3] = i < CH ? min_bf16x2(w.w, 0u) : max_bf16x2(w.w, 0u);
+        mma_bf16_16816(c, a, v[i].z, v[i].w);
       }
-      taken += sums[w];
-      ties += sums[32 + w];
+      const int r0 = mt * 16 + g;
+      if (r0 < rows) {
+        best[0] = fmaxf(best[0], c[0]);
+        best[1] = fmaxf(best[1], c[1]);
+      }
+      if (r0 + 8 < rows) {
+        best[0] = fmaxf(best[0], c[2]);
+        best[1] = fmaxf(best[1], c[3]);
+      }
     }
-    if (sure || (tie && tie_before < equal)) out[sure_before + min(tie_before, equal)] = s;
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      best[0] = fmaxf(best[0], __shfl_xor_sync(0xffffffffu, best[0], o));
+      best[1] = fmaxf(best[1], __shfl_xor_sync(0xffffffffu, best[1], o));
+    }
+    if (!waited) cluster.barrier_wait();   // (once, by every thread)
+    waited = true;
+    if (lane < 8) {   // span `lane` of the group: column lane % 2 of the quad's thread lane / 2
+      const float e = __shfl_sync(0x000000ffu, best[0], lane >> 1), f = __shfl_sync(0x000000ffu, best[1], lane >> 1);
+      const int s = group * 8 + lane;
+      if (s < n) estimate0[s] = (there >> (4 * lane)) & 1 ? __float_as_uint(lane & 1 ? f : e) & 0xffffffffu : kNoSpan;
+    }
   }
-  for (int i = taken + min(ties, equal) + threadIdx.x; i < p.count; i += kPickThreads) out[i] = -1;
+  if (!waited) cluster.barrier_wait();
+  {
+    uint32_t w = max(wide & 0xffffu, wide >> 16);
+    w = __reduce_max_sync(0xffffffffu, w);
+    if (lane == 0) atomicMax(widest0, w << 16);
+  }
+  cluster.sync();
+  if (rank) return;
+
+  // ---- the first block: what is taken for sure, what is between ----
+  auto kept = [&](int s) { return s < p.first || s >= n - p.last; };
+  {
+    uint32_t size = 0;   // largest sum of |q| over a row, as its bits (NaN above infinity above all)
+    for (int r = warp; r < rows; r += kPickWarps) {
+      const __nv_bfloat16* q = p.q + ((size_t)(b * p.Q + r / G) * p.heads + head * G + r % G) * HD;
+      float x = 0.f;
+      for (int d = lane; d < HD; d += 32) x += fabsf(bf2f(q[d]));
+      x = warp_sum(x);
+      size = max(size, __float_as_uint(x));
+    }
+    if (lane == 0) q_size[warp] = size;
+  }
+  int always = 0, others = 0;
+  float lo = INFINITY, hi = -INFINITY;
+  for (int s = threadIdx.x; s < n; s += kPickThreads) {
+    const uint32_t e = estimate[s];
+    if (e == kNoSpan) continue;
+    if (kept(s)) {
+      ++always;
+    } else {
+      ++others;
+      lo = fminf(lo, __uint_as_float(e));
+      hi = fmaxf(hi, __uint_as_float(e));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  if (lane == 0) {
+    low[warp] = lo;
+    high[warp] = hi;
+  }
+  always = pick_total(always, sums);
+  others = pick_total(others, sums);
+  uint32_t q_most = 0;
+#pragma unroll
+  for (int w = 0; w < kPickWarps; ++w) {
+    lo = fminf(lo, low[w]);
+    hi = fmaxf(hi, high[w]);
+    q_most = max(q_most, q_size[w]);
+  }
+  const float size = __uint_as_float(q_most) * __uint_as_float(widest);
+  const int want = min(p.count - always, others);   // beside those that are kept
+  const bool all = want == others, none = want == 0;
+  const bool finite = size < 1e38f;
+  const float eps2 = size * 0x1p-13f + 0x1p-100f, scale = hi - lo > 1e-30f ? (float)(kPickBins - 1) / (hi - lo) : 0.f;
+  auto bin_of = [&](float x) { return (int)fminf(fmaxf((x - lo) * scale, -1.f), (float)(kPickBins - 1)); };   // (rises with x)
+  if (!all && !none && finite) {
+    for (int s = threadIdx.x; s < n; s += kPickThreads) {
+      const uint32_t e = estimate[s];
+      if (e != kNoSpan && !kept(s)) atomicAdd(&bins[bin_of(__uint_as_float(e))], 1);
+    }
+    __syncthreads();
+    // the bin of the want-th largest: from the top, each thread some bins
+    constexpr int PER = kPickBins / kPickThreads;
+    int mine = 0, total;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mine += bins[kPickBins - 1 - (int)threadIdx.x * PER - i];
+    int upto = pick_running_sum(mine, sums, &total) - mine;
+    if (upto < want && upto + mine >= want) {
+      int i = kPickBins - 1 - (int)threadIdx.x * PER;
+      for (;; --i) {
+        upto += bins[i];
+        if (upto >= want) break;
+      }
+      pick_bin = i;
+    }
+    __syncthreads();
+  }
+  const int line = pick_bin;
+  int sure = 0, open = 0;
+  for (int base = warp * 32; base < n; base += kPickThreads) {
+    const int s = base + lane;
+    const uint32_t e = s < n ? estimate[s] : kNoSpan;
+    const bool there = e != kNoSpan, keep = kept(s);
+    bool in = there && (keep || all), maybe = there && !keep && !all && !none;
+    if (maybe && finite) {
+      const float x = __uint_as_float(e);
+      in = bin_of(x - eps2) > line;
+      maybe = !in && bin_of(x + eps2) >= line;
+    }
+    const uint32_t m_in = __ballot_sync(0xffffffffu, in), m_open = __ballot_sync(0xffffffffu, maybe);
+    if (lane == 0) {
+      taken[base / 32] = m_in;
+      between[base / 32] = m_open;
+    }
+    sure += in && !keep;
+    open += maybe;
+  }
+  sure = pick_total(sure, sums);
+  open = pick_total(open, sums);
+  const int left = want - sure, n_words = (n + 31) / 32;   // so many of the `open` ones (0 where all or none are taken)
+
+  if (!all && left > 0 && left == open) {
+    for (int w = threadIdx.x; w < n_words; w += kPickThreads) taken[w] |= between[w];
+  } else if (!all && left > 0) {
+    // ---- scores in 64 bits ----
+    const bool listed = open <= kPickBins;
+    if (listed) {   // the spans between, ascending
+      int done = 0;
+      for (int base = 0; base < n_words; base += kPickThreads) {
+        const int w = base + threadIdx.x;
+        uint32_t m = w < n_words ? between[w] : 0;
+        int count, at = pick_running_sum(__popc(m), sums, &count);
+        at += done - __popc(m);
+        for (; m; m &= m - 1) bins[at++] = w * 32 + __ffs(m) - 1;
+        done += count;
+      }
+      __syncthreads();
+    }
+    const int m = listed ? open : n;
+    auto span_of = [&](int i) { return listed ? bins[i] : ((between[i >> 5] >> (i & 31)) & 1 ? i : -1); };
+    for (int i = warp; i < m; i += kPickWarps) {
+      const int s = span_of(i);
+      if (s < 0) continue;
+      const unsigned long long key = exact_score<HD>(p, b, head, page_at(table + s / subs, p.num_blocks), s % subs);
+      if (lane == 0) keys[i] = key;
+    }
+    __syncthreads();
+    if (open <= kPickRanked) {
+      for (int i = threadIdx.x; i < m; i += kPickThreads) {
+        const unsigned long long key = keys[i];
+        int before = 0;
+        for (int j = 0; j < m; ++j) before += keys[j] > key || (keys[j] == key && j < i);
+        if (before < left) atomicOr(&taken[bins[i] >> 5], 1u << (bins[i] & 31));
+      }
+    } else {   // the left-th largest score bit by bit, then as many of those on it as there is room for, in their order
+      unsigned long long score = 0;
+      for (int bit = 63; bit >= 0; --bit) {
+        const unsigned long long tried = score | (1ull << bit);
+        int c = 0;
+        for (int i = threadIdx.x; i < m; i += kPickThreads) c += span_of(i) >= 0 && keys[i] >= tried;
+        if (pick_total(c, sums) >= left) score = tried;
+      }
+      int above = 0;
+      for (int i = threadIdx.x; i < m; i += kPickThreads) above += span_of(i) >= 0 && keys[i] > score;
+      int room = left - pick_total(above, sums);
+      for (int base = 0; base < m; base += kPickThreads) {
+        const int i = base + threadIdx.x, s = i < m ? span_of(i) : -1;
+        const bool over = s >= 0 && keys[i] > score, on = s >= 0 && keys[i] == score;
+        int total;
+        const int at = pick_running_sum(on, sums, &total) - on;
+        if (over || (on && at < room)) atomicOr(&taken[s >> 5], 1u << (s & 31));
+        room -= total;
+      }
+    }
+  }
+  __syncthreads();
+  pick_write(taken, n_words, out, p.count, sums);
 }
 
 // ----------------------------------------------------------------------------------
