@@ -306,9 +306,11 @@ int ssdk_span_bounds(const void* k_cache, const int32_t* block_tables, const int
 /* ssdk_select_spans: per sequence and key head the `count` spans to read, int32 [batch, KV, count], ascending, -1 behind the last: the first
  * `first` and the last `last` spans of the context, then those with the largest score = max over the query rows of (sequence, key head) of
  * sum_d max(q_d lo_d, q_d hi_d), which no key of the span exceeds; scores in 64 bits, the lowest index among equal ones, NaN above all.
- * Spans on pages outside the cache are never listed.  Tables hold at most 24576 spans. */
+ * Spans on pages outside the cache are never listed.  Tables hold at most 24576 spans;
+ * bounds are ssdk_span_bounds's (lo <= hi).  `scratch`: ssdk_select_spans_scratch_bytes(...) bytes of the call's own. */
+int64_t ssdk_select_spans_scratch_bytes(int batch, int kv_heads, int block_size, int max_blocks_per_seq, int span);
 int ssdk_select_spans(const void* q, const void* bounds, const int32_t* block_tables, const int32_t* context_lens, int32_t* selected,
-                      int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size,
+                      void* scratch, int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size,
                       int max_blocks_per_seq, int64_t num_blocks, int span, int count, int first, int last, void* stream);
 /* ssdk_span_attn: ssdk_paged_attn over the keys of the listed spans only.  Entries outside the context, or on pages outside the cache, are
  * passed over; a span that is listed twice counts twice; a row that sees no key is zero.  At most 32 query heads to a key head, 4096 spans. */

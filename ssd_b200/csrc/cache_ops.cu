@@ -51,7 +51,7 @@ static int launch_rope_axes(Launcher& L, const RopeAxesParams& p) {
   return L.go(rope_axes_kernel<HD, 4>, grid, dim3(kRopeAxesThreads), 0, p);
 }
 
-constexpr int kSms = 148;
+constexpr int kSms = 148, kMaxSmem = 227 * 1024 - 1024;   // (statics beside it)
 constexpr int kMaxListed = 4096;   // spans of a list
 template <int HD, int MT>
 static int launch_span_attn(Launcher& L, const SpanAttnParams& p, int tiles) {
@@ -60,14 +60,21 @@ static int launch_span_attn(Launcher& L, const SpanAttnParams& p, int tiles) {
   return L.go(span_attn_kernel<HD, MT>, dim3(p.kv_heads, p.B, tiles), dim3(kSpanWarps * 32), span_attn_smem(HD, p.count), p);
 }
 
-// blocks of a cluster: two per SM, as long as each of their warps has spans to score
 template <int HD>
 static int launch_select(Launcher& L, const SelectParams& p) {
   static std::atomic<bool> done[64];
-  CKI(with_smem(span_select_kernel<HD>, select_smem(kMaxSpans), done));
-  while (L.cluster < 8 && (int64_t)p.B * p.kv_heads * L.cluster < 2 * kSms && L.cluster * kPickWarps * 8 < p.max_spans) L.cluster *= 2;
-  return L.go(span_select_kernel<HD>, dim3(p.kv_heads * L.cluster, p.B), dim3(kPickThreads), select_smem(p.max_spans), p);
+  CKI(with_smem(span_pick_kernel<HD>, kMaxSmem, done));
+  L.pdl = true;
+  constexpr int W = kEstimateThreads / 32;
+  CKI(L.go(span_estimate_kernel<HD>, dim3(p.warps / W, p.kv_heads, p.B), dim3(kEstimateThreads), 0, p));
+  return L.go(span_pick_kernel<HD>, dim3(p.kv_heads, p.B), dim3(kPickThreads), pick_smem(p.max_spans, p.Q * (p.heads / p.kv_heads), HD), p);
 }
+// groups of sixteen spans of a warp: one while the blocks are fewer than two per SM, four at most (they share the query's fragments)
+static int select_run(int batch, int kv_heads, int64_t max_spans) {
+  const int64_t blocks = (max_spans + 127) / 128 * batch * kv_heads;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(4, blocks / (2 * kSms)));
+}
+static int select_warps(int64_t max_spans, int run) { return (int)((max_spans + 128 * run - 1) / (128 * run)) * (kEstimateThreads / 32); }
 
 extern "C" {
 
@@ -135,22 +142,34 @@ int ssdk_span_bounds(const void* k_cache, const int32_t* block_tables, const int
   return L.go(span_bounds_kernel, dim3((p.fresh + span - 2) / span + 1, batch), dim3(kBoundsThreads), 0, p);
 }
 
+int64_t ssdk_select_spans_scratch_bytes(int batch, int kv_heads, int block_size, int max_blocks_per_seq, int span) {
+  if (batch < 1 || kv_heads < 1 || block_size < 1 || max_blocks_per_seq < 1 || span < 1) return 0;
+  const int64_t spans = (int64_t)max_blocks_per_seq * (block_size / span);
+  return (spans + (spans + 127) / 128 * (kEstimateThreads / 32)) * 4 * batch * kv_heads;
+}
+
 int ssdk_select_spans(const void* q, const void* bounds, const int32_t* block_tables, const int32_t* context_lens, int32_t* selected,
-                      int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size,
+                      void* scratch, int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size,
                       int max_blocks_per_seq, int64_t num_blocks, int span, int count, int first, int last, void* stream) {
   CKI(check_pages("select_spans", batch, block_size, max_blocks_per_seq, num_blocks));
   CKI(check_spans("select_spans", heads, kv_heads, head_dim, block_size, span));
   if (q_len < 1 || count < 1 || count > kMaxListed || first < 0 || last < 0 || (int64_t)first + last > count)
     return fail("select_spans: q_len=%d, %d spans (at most %d), of them the first %d and the last %d", q_len, count, kMaxListed, first, last);
-  if (!q || !bounds || !block_tables || !context_lens || !selected) return fail("select_spans: null argument");
-  if (off16(q, bounds)) return fail("select_spans: arrays must start at multiples of 16 bytes");
+  if (!q || !bounds || !block_tables || !context_lens || !selected || !scratch) return fail("select_spans: null argument");
+  if (off16(q, bounds, scratch)) return fail("select_spans: arrays must start at multiples of 16 bytes");
   const int64_t max_spans = (int64_t)max_blocks_per_seq * (block_size / span);
   if (max_spans > kMaxSpans) return fail("select_spans: tables of %lld spans (at most %d)", (long long)max_spans, kMaxSpans);
+  const int64_t rows = (int64_t)q_len * (heads / kv_heads);
+  if (rows > 4096 || pick_smem((int)max_spans, rows, head_dim) > kMaxSmem)
+    return fail("select_spans: %lld query rows to a key head beside tables of %lld spans pass the shared memory", (long long)rows, (long long)max_spans);
   SelectParams p;
+  p.sub_magic = ((1ull << 32) + block_size / span - 1) / (block_size / span);
   p.q = (const bf16*)q; p.bounds = (const bf16*)bounds; p.tables = block_tables; p.lens = context_lens; p.out = selected;
   p.num_blocks = num_blocks; p.B = batch; p.Q = q_len; p.heads = heads; p.kv_heads = kv_heads;
   p.block_size = block_size; p.span = span; p.max_blocks = max_blocks_per_seq; p.max_spans = (int)max_spans;
   p.count = count; p.first = first; p.last = last;
+  p.run = select_run(batch, kv_heads, max_spans); p.warps = select_warps(max_spans, p.run);
+  p.estimates = (uint32_t*)scratch; p.wide = p.estimates + (size_t)batch * kv_heads * max_spans;
   Launcher L;
   L.st = (cudaStream_t)stream;
   return head_dim == 64 ? launch_select<64>(L, p) : launch_select<128>(L, p);

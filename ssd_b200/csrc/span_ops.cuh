@@ -1,7 +1,5 @@
 // span_ops.cuh — attention over a part of a long paged cache: spans of keys are chosen by a bound on their scores, and attention reads the chosen ones only.
 #pragma once
-#include <cooperative_groups.h>
-
 #include "async_copy.cuh"
 #include "cache_ops.cuh"
 #include "common.cuh"
@@ -9,16 +7,18 @@
 namespace ssdk {
 
 // ----------------------------------------------------------------------------------
-// span_select_kernel: the score of span s for key head g is the largest over the query rows r of (sequence, g) of
+// select_spans: the score of span s for key head g is the largest over the query rows r of (sequence, g) of
 //   sum_d max(q[r, d] lo[s, d], q[r, d] hi[s, d])  >=  max over the span's keys of q[r] . k.
 // Listed are the first and the last spans, then the best by score, the lowest index first among equal ones.  Scores count in 64 bits: 32 would let spans
 // change places whose scores differ in the last bits.
-// Bound by the bytes of the bounds.  The sum is a product, [min(q, 0) | max(q, 0)] . [lo | hi], so the tensor cores make an estimate of every score: a warp
-// takes eight spans, whose 16-byte loads are the fragments of mma.m16n8k16 (channels permuted alike on both sides), rows as its m.  The estimate is off by at
-// most eps = 2^-14 max_r sum_d |q[r, d]| max |lo, hi|: 2 hd / 16 steps, each adding 17 numbers with 2^-22 of the terms' size lost.  With t the want-th largest
-// estimate, a span above t + 2 eps is taken, one under t - 2 eps is not, and only the few in between are scored in 64 bits (products of bf16 values
-// are exact, sums of 128 of them off by 2^-46).  Where values are not finite, or so large that 32 bits overflow, all spans are.
-// A cluster of blocks shares a key head of a sequence: estimates go to the first block's shared memory, which picks.
+// Bound by the bytes of the bounds.  The sum is a product, [lo | hi] . [min(q, 0) | max(q, 0)], so span_estimate_kernel makes an estimate of every score on the
+// tensor cores: a warp takes sixteen spans, whose 16-byte loads are the m16 fragments of mma.m16n8k16 (channels permuted alike on both sides), eight rows
+// are its n.  The estimate is off by at most eps = 2^-14 max_r sum_d |q[r, d]| max |lo, hi|: 2 hd / 16 steps, each adding 17 numbers with 2^-22 of the terms'
+// size lost.  With t the want-th largest estimate, a span above t + 2 eps is taken, one under t - 2 eps is not, and span_pick_kernel scores only the few
+// in between in 64 bits (products of bf16 values are exact, sums of 128 of them off by 2^-46).  Where values are not finite, or so large that 32 bits
+// overflow, it scores all.
+// Two kernels, the second's start under the first's end: with one, whose first block of a cluster picks, what was left of the blocks in a second wave
+// and the picking blocks held the SMs while the memory idled (24 contexts of 64000: 82 us, 47.7 with two).
 // ----------------------------------------------------------------------------------
 struct SelectParams {
   const __nv_bfloat16* q;        // [B * Q, H, hd]
@@ -26,15 +26,20 @@ struct SelectParams {
   const int32_t* tables;         // [B, max_blocks]
   const int32_t* lens;           // [B]
   int32_t* out;                  // [B, KV, count]
+  uint32_t* estimates;           // [B, KV, max_spans] bits of fp32, kNoSpan where there is no page
+  uint32_t* wide;                // [B, KV, warps] bits of the largest |lo|, |hi| that a warp saw
   int64_t num_blocks;
+  unsigned long long sub_magic;  // ceil(2^32 / spans of a page)
   int B, Q, heads, kv_heads, block_size, span, max_blocks, max_spans, count, first, last;
+  int run, warps;                // groups of sixteen spans of a warp; warps to a key head of a sequence
 };
-constexpr int kPickThreads = 256, kPickWarps = kPickThreads / 32;
+constexpr int kEstimateThreads = 256;
+constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 32;
 constexpr int kMaxSpans = 24576;   // of a sequence
 constexpr int kPickBins = 2048;
 constexpr int kPickRanked = 256;   // spans between, up to which each is compared with each
-// scores (64 bits; before them the estimates) | taken | between (a bit per span) | bins, then the spans between
-constexpr int select_smem(int spans) { return spans * 8 + 2 * ((spans + 31) / 32) * 4 + kPickBins * 4; }
+// rows of the query | scores (64 bits; before them the estimates) | taken | between (a bit per span) | bins, then the spans between
+constexpr int64_t pick_smem(int spans, int64_t rows, int HD) { return (rows + 7) / 8 * 8 * HD * 2 + spans * 8 + 2 * ((spans + 31) / 32) * 4 + kPickBins * 4; }
 constexpr uint32_t kNoSpan = 0xffffffffu;   // estimate of a span that has no page
 
 // 64-bit values in their order as unsigned words; zeros of both signs are one value, NaN is above all.  0 is no value
@@ -90,187 +95,202 @@ SSDK_DEVINL void pick_write(const uint32_t* bits, int words, int32_t* out, int c
   for (int i = done + threadIdx.x; i < count; i += kPickThreads) out[i] = -1;
 }
 
-// a warp: the score of one span in 64 bits
-template <int HD>
-SSDK_DEVINL unsigned long long exact_score(const SelectParams& p, int b, int g, int page, int sub) {
-  constexpr int E = HD / 32;   // channels of a lane
-  const int lane = threadIdx.x & 31, G = p.heads / p.kv_heads, rows = G * p.Q, subs = p.block_size / p.span;
-  const __nv_bfloat16* both = p.bounds + (((size_t)page * subs + sub) * p.kv_heads + g) * 2 * HD + lane * E;
-  float lo[E], hi[E];
+// a warp: the score of one span in 64 bits.  q: the rows [tiles * 8][HD], those behind the last one zero.  A lane has HD / 32 channels of eight rows at a time;
+// their sums halve their number with every exchange.  FINITE: lo <= hi and no product is NaN, so that the sign of q says which bound counts.
+template <int HD, bool FINITE>
+SSDK_DEVINL unsigned long long exact_score(const __nv_bfloat16* both, const __nv_bfloat16* q, int rows) {
+  constexpr int E = HD / 32;
+  const int lane = threadIdx.x & 31;
+  double lo[E], hi[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    lo[e] = bf2f(both[e]);
-    hi[e] = bf2f(both[HD + e]);
+    lo[e] = bf2f(both[lane * E + e]);
+    hi[e] = bf2f(both[HD + lane * E + e]);
   }
   unsigned long long key = 0;
-#pragma unroll 4
-  for (int r = 0; r < rows; ++r) {
-    const __nv_bfloat16* q = p.q + ((size_t)(b * p.Q + r / G) * p.heads + g * G + r % G) * HD + lane * E;
-    double sum = 0.0;
+  for (int r0 = 0; r0 < rows; r0 += 8) {
+    double sum[8];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const double x = bf2f(q[e]), u = x * lo[e], v = x * hi[e];
-      sum += u != u || v != v ? __longlong_as_double(0x7ff8000000000000ll) : (u > v ? u : v);
+    for (int r = 0; r < 8; ++r) {
+      sum[r] = 0.0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float f = bf2f(q[(r0 + r) * HD + lane * E + e]);
+        const double x = f;
+        if (FINITE) {
+          sum[r] += x * (f >= 0.f ? hi[e] : lo[e]);
+        } else {
+          const double u = x * lo[e], v = x * hi[e];
+          sum[r] += u != u || v != v ? __longlong_as_double(0x7ff8000000000000ll) : (u > v ? u : v);
+        }
+      }
     }
+    int row = 0;   // of the eight, the one that this lane ends with
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    key = max(key, score_key(sum));
+    for (int o = 16, m = 4; o >= 4; o >>= 1, m >>= 1) {
+      const bool up = (lane & o) != 0;
+      row += up ? m : 0;
+#pragma unroll
+      for (int r = 0; r < m; ++r) {
+        const double give = up ? sum[r] : sum[r + m], keep = up ? sum[r + m] : sum[r];
+        sum[r] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+      }
+    }
+    sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 2);
+    sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 1);
+    if (r0 + row < rows) key = max(key, score_key(sum[0]));
   }
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
   return key;
 }
 
-SSDK_DEVINL uint4 and4(uint4 v, uint32_t m) { return make_uint4(v.x & m, v.y & m, v.z & m, v.w & m); }
+SSDK_DEVINL int sub_page(const SelectParams& p, int s) { return (int)((unsigned)s * p.sub_magic >> 32); }   // s / spans of a page: below 2^15 and 2^16
+SSDK_DEVINL const __nv_bfloat16* bounds_at(const SelectParams& p, int page, int s, int head, int HD) {
+  const int subs = p.block_size / p.span;
+  return p.bounds + (((size_t)page * subs + (s - sub_page(p, s) * subs)) * p.kv_heads + head) * 2 * HD;
+}
 
 template <int HD>
-__global__ void __launch_bounds__(kPickThreads, 2) span_select_kernel(SelectParams p) {
-  namespace cg = cooperative_groups;
+__global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(SelectParams p) {
   constexpr int CH = HD / 32;   // 16-byte pieces of a lane per bound
-  extern __shared__ __align__(16) uint8_t select_smem_bytes[];
+  constexpr int W = kEstimateThreads / 32;
+  pdl_launch_dependents();
+  const int head = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int n = (tokens_of(p.lens, b, p.max_blocks, p.block_size) + p.span - 1) / p.span, groups = (n + 15) / 16;
+  if (n <= p.count) return;   // all are listed
+  const int G = p.heads / p.kv_heads, rows = G * p.Q, tiles = (rows + 7) / 8;
+  const int32_t* table = p.tables + (size_t)b * p.max_blocks;
+  uint32_t* estimates = p.estimates + ((size_t)b * p.kv_heads + head) * p.max_spans;
+  auto page_of = [&](int s) { return s < n ? page_at(table + sub_page(p, s), p.num_blocks) : -1; };
+  // the query's side: row g of a tile, step k of 16 channels: the lane's channels 8 (t + 4 (k / 2)) + 4 (k % 2) .. + 3; lower bounds (k < 2 CH) meet
+  // the negative parts, upper bounds the positive ones
+  uint2 qf[4 * CH];
+  auto load_q = [&](int tile) {
+    const int r = tile * 8 + g;
+    const __nv_bfloat16* q = p.q + ((size_t)(b * p.Q + r / G) * p.heads + head * G + r % G) * HD + 8 * t;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const uint4 x = r < rows ? *reinterpret_cast<const uint4*>(q + 32 * i) : make_uint4(0, 0, 0, 0);
+      qf[2 * i] = make_uint2(min_bf16x2(x.x, 0u), min_bf16x2(x.y, 0u));
+      qf[2 * i + 1] = make_uint2(min_bf16x2(x.z, 0u), min_bf16x2(x.w, 0u));
+      qf[2 * CH + 2 * i] = make_uint2(max_bf16x2(x.x, 0u), max_bf16x2(x.y, 0u));
+      qf[2 * CH + 2 * i + 1] = make_uint2(max_bf16x2(x.z, 0u), max_bf16x2(x.w, 0u));
+    }
+  };
+  int group = blockIdx.x * W * p.run + warp;
+  const int end = min(groups, (int)(blockIdx.x + 1) * W * p.run);
+  int page0 = page_of(group * 16 + g), page1 = page_of(group * 16 + 8 + g);
+  if (group < end) load_q(0);
+  uint32_t bottom = 0, top = 0;   // two channels: smallest lower, largest upper bound
+  for (; group < end; group += W) {
+    const int s0 = group * 16 + g, s1 = s0 + 8;
+    const __nv_bfloat16 *both0 = bounds_at(p, max(page0, 0), s0, head, HD) + 8 * t, *both1 = bounds_at(p, max(page1, 0), s1, head, HD) + 8 * t;
+    uint4 u[2 * CH], v[2 * CH];
+#pragma unroll
+    for (int i = 0; i < 2 * CH; ++i) {
+      u[i] = page0 >= 0 ? ld_nc_v4(both0 + 32 * i) : make_uint4(0, 0, 0, 0);
+      v[i] = page1 >= 0 ? ld_nc_v4(both1 + 32 * i) : make_uint4(0, 0, 0, 0);
+    }
+    const bool there0 = page0 >= 0, there1 = page1 >= 0;
+    page0 = page_of(s0 + 16 * W);
+    page1 = page_of(s1 + 16 * W);
+    float best[2] = {-INFINITY, -INFINITY};   // spans g, g + 8
+    for (int tile = 0; tile < tiles; ++tile) {
+      if (tiles > 1) load_q(tile);
+      float c[2][4] = {};
+#pragma unroll
+      for (int i = 0; i < 2 * CH; ++i) {
+        const uint32_t a0[4] = {u[i].x, v[i].x, u[i].y, v[i].y}, a1[4] = {u[i].z, v[i].z, u[i].w, v[i].w};
+        mma_bf16_16816(c[0], a0, qf[2 * i].x, qf[2 * i].y);
+        mma_bf16_16816(c[1], a1, qf[2 * i + 1].x, qf[2 * i + 1].y);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (tile * 8 + 2 * t + e < rows) {
+          best[0] = fmaxf(best[0], c[0][e] + c[1][e]);
+          best[1] = fmaxf(best[1], c[0][2 + e] + c[1][2 + e]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      bottom = min_bf16x2(bottom, min_bf16x2(min_bf16x2(u[i].x, u[i].y), min_bf16x2(u[i].z, u[i].w)));
+      bottom = min_bf16x2(bottom, min_bf16x2(min_bf16x2(v[i].x, v[i].y), min_bf16x2(v[i].z, v[i].w)));
+      top = max_bf16x2(top, max_bf16x2(max_bf16x2(u[i + CH].x, u[i + CH].y), max_bf16x2(u[i + CH].z, u[i + CH].w)));
+      top = max_bf16x2(top, max_bf16x2(max_bf16x2(v[i + CH].x, v[i + CH].y), max_bf16x2(v[i + CH].z, v[i + CH].w)));
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      best[0] = fmaxf(best[0], __shfl_xor_sync(0xffffffffu, best[0], o));
+      best[1] = fmaxf(best[1], __shfl_xor_sync(0xffffffffu, best[1], o));
+    }
+    if (t < 2) {
+      const int s = t ? s1 : s0;
+      if (s < n) estimates[s] = (t ? there1 : there0) ? __float_as_uint(t ? best[1] : best[0]) : kNoSpan;
+    }
+  }
+  const uint32_t both = max_bf16x2(bottom & 0x7fff7fffu, top);   // (top is not negative; NaN is above infinity above all)
+  const uint32_t most = __reduce_max_sync(0xffffffffu, max(both & 0xffffu, both >> 16));
+  if (lane == 0) p.wide[((size_t)b * p.kv_heads + head) * p.warps + blockIdx.x * W + warp] = most << 16;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kPickThreads) span_pick_kernel(SelectParams p) {
+  extern __shared__ __align__(16) uint8_t pick_smem_bytes[];
   __shared__ int sums[kPickWarps], pick_bin;
-  __shared__ uint32_t widest;              // bits of the largest |lo|, |hi| (NaN above infinity above all)
+  __shared__ uint32_t widest, q_most;      // bits of the largest |lo|, |hi|, and of the largest sum of |q| over a row
   __shared__ float low[kPickWarps], high[kPickWarps];
-  __shared__ uint32_t q_size[kPickWarps];
+  const int G = p.heads / p.kv_heads, rows = G * p.Q, padded = (rows + 7) / 8 * 8;
   const int words = (p.max_spans + 31) / 32;
-  unsigned long long* keys = reinterpret_cast<unsigned long long*>(select_smem_bytes);
-  uint32_t* estimate = reinterpret_cast<uint32_t*>(select_smem_bytes);
+  __nv_bfloat16* q_rows = reinterpret_cast<__nv_bfloat16*>(pick_smem_bytes);   // [padded][HD]
+  unsigned long long* keys = reinterpret_cast<unsigned long long*>(q_rows + padded * HD);
+  uint32_t* estimate = reinterpret_cast<uint32_t*>(keys);
   uint32_t* taken = reinterpret_cast<uint32_t*>(keys + p.max_spans);
   uint32_t* between = taken + words;
   int* bins = reinterpret_cast<int*>(between + words);
-
-  cg::cluster_group cluster = cg::this_cluster();
-  const int C = cluster.num_blocks(), rank = cluster.block_rank();
-  const int head = blockIdx.x / C, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int G = p.heads / p.kv_heads, rows = G * p.Q, subs = p.block_size / p.span;
-  const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size), n = (len + p.span - 1) / p.span;
+  const int head = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = (tokens_of(p.lens, b, p.max_blocks, p.block_size) + p.span - 1) / p.span;
   const int32_t* table = p.tables + (size_t)b * p.max_blocks;
   int32_t* out = p.out + ((size_t)b * p.kv_heads + head) * p.count;
 
-  if (n <= p.count) {   // all of them (the same for every block of the cluster)
-    if (rank) return;
+  if (n <= p.count) {   // all of them
     for (int base = warp * 32; base < n; base += kPickThreads) {
       const int s = base + lane;
-      const uint32_t m = __ballot_sync(0xffffffffu, s < n && page_at(table + s / subs, p.num_blocks) >= 0);
+      const uint32_t m = __ballot_sync(0xffffffffu, s < n && page_at(table + sub_page(p, s), p.num_blocks) >= 0);
       if (lane == 0) taken[base / 32] = m;
     }
     __syncthreads();
     pick_write(taken, (n + 31) / 32, out, p.count, sums);
     return;
   }
-
-  if (rank == 0) {
-    for (int i = threadIdx.x; i < kPickBins; i += kPickThreads) bins[i] = 0;
-    if (threadIdx.x == 0) widest = 0;
+  if (threadIdx.x == 0) widest = q_most = 0;
+  for (int i = threadIdx.x; i < kPickBins; i += kPickThreads) bins[i] = 0;
+  __syncthreads();
+  for (int base = warp * 32; base < padded * (HD / 8); base += kPickThreads) {   // (whole warps) the query's rows: 8 channels a thread
+    const int r = (base + lane) / (HD / 8), c = (base + lane) % (HD / 8) * 8;
+    const uint4 v = r < rows ? ld_nc_v4(p.q + ((size_t)(b * p.Q + r / G) * p.heads + head * G + r % G) * HD + c) : make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(q_rows + r * HD + c) = v;
+    float x[8], size = 0.f;
+    unpack_bf16x8(v, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) size += fabsf(x[j]);
+#pragma unroll
+    for (int o = HD / 16; o > 0; o >>= 1) size += __shfl_xor_sync(0xffffffffu, size, o);
+    const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(size));   // (NaN above infinity above all)
+    if (lane == 0) atomicMax(&q_most, most);
   }
-  cluster.barrier_arrive();   // every block has started, and the first one's words are set
-  uint32_t* estimate0 = cluster.map_shared_rank(estimate, 0);
-  uint32_t* widest0 = cluster.map_shared_rank(&widest, 0);
+  pdl_wait();   // the estimates are there
 
-  // ---- estimates ----
-  auto load_q = [&](int mt, uint4* q0, uint4* q1) {
-    const int r0 = mt * 16 + g, r1 = r0 + 8;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int c = 8 * (t + 4 * i);
-      q0[i] = r0 < rows ? ld_nc_v4(p.q + ((size_t)(b * p.Q + r0 / G) * p.heads + head * G + r0 % G) * HD + c) : make_uint4(0, 0, 0, 0);
-      q1[i] = r1 < rows ? ld_nc_v4(p.q + ((size_t)(b * p.Q + r1 / G) * p.heads + head * G + r1 % G) * HD + c) : make_uint4(0, 0, 0, 0);
-    }
-  };
-  auto load_group = [&](int group, uint4* v) {
-    const int s = group * 8 + g;
-    const int page = s < n ? page_at(table + s / subs, p.num_blocks) : -1;
-    const __nv_bfloat16* both = p.bounds + (((size_t)max(page, 0) * subs + s % subs) * p.kv_heads + head) * 2 * HD + 8 * t;
-#pragma unroll
-    for (int i = 0; i < 2 * CH; ++i) v[i] = page >= 0 ? ld_nc_v4(both + 32 * i) : make_uint4(0, 0, 0, 0);
-    return page >= 0;
-  };
-  const int tiles = (rows + 15) / 16, groups = (n + 7) / 8, step = C * kPickWarps;
-  uint4 q0[CH], q1[CH];
-  load_q(0, q0, q1);
-  uint32_t wide = 0;   // two channels
-  uint4 next[2 * CH];
-  int group = rank * kPickWarps + warp;
-  bool next_there = group < groups ? load_group(group, next) : false;
-  bool waited = false;
-  for (; group < groups; group += step) {
-    uint4 v[2 * CH];
-#pragma unroll
-    for (int i = 0; i < 2 * CH; ++i) v[i] = next[i];
-    const uint32_t there = __ballot_sync(0xffffffffu, next_there);
-    if (group + step < groups) next_there = load_group(group + step, next);
-#pragma unroll
-    for (int i = 0; i < 2 * CH; ++i) {
-      const uint4 a = and4(v[i], 0x7fff7fffu);
-      wide = max_bf16x2(wide, max_bf16x2(max_bf16x2(a.x, a.y), max_bf16x2(a.z, a.w)));
-    }
-    float best[2] = {-INFINITY, -INFINITY};   // spans 2 t, 2 t + 1
-    for (int mt = 0; mt < tiles; ++mt) {
-      if (tiles > 1) load_q(mt, q0, q1);
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 2 * CH; ++i) {
-        const uint4 u = q0[i % CH], w = q1[i % CH];
-        uint32_t a[4];
-        // lower bounds meet the negative parts of the query, upper bounds the positive ones
-        a[0] = i < CH ? min_bf16x2(u.x, 0u) : max_bf16x2(u.x, 0u);
-        a[1] = i < CH ? min_bf16x2(w.x, 0u) : max_bf16x2(w.x, 0u);
-        a[2] = i < CH ? min_bf16x2(u.y, 0u) : max_bf16x2(u.y, 0u);
-        a[3] = i < CH ? min_bf16x2(w.y, 0u) : max_bf16x2(w.y, 0u);
-        mma_bf16_16816(c, a, v[i].x, v[i].y);
-        a[0] = i < CH ? min_bf16x2(u.z, 0u) : max_bf16x2(u.z, 0u);
-        a[1] = i < CH ? min_bf16x2(w.z, 0u) : max_bf16x2(w.z, 0u);
-        a[2] = i < CH ? min_bf16x2(u.w, 0u) : max_bf16x2(u.w, 0u);
-        a[3] = i < CH ? min_bf16x2(w.w, 0u) : max_bf16x2(w.w, 0u);
-        mma_bf16_16816(c, a, v[i].z, v[i].w);
-      }
-      const int r0 = mt * 16 + g;
-      if (r0 < rows) {
-        best[0] = fmaxf(best[0], c[0]);
-        best[1] = fmaxf(best[1], c[1]);
-      }
-      if (r0 + 8 < rows) {
-        best[0] = fmaxf(best[0], c[2]);
-        best[1] = fmaxf(best[1], c[3]);
-      }
-    }
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) {
-      best[0] = fmaxf(best[0], __shfl_xor_sync(0xffffffffu, best[0], o));
-      best[1] = fmaxf(best[1], __shfl_xor_sync(0xffffffffu, best[1], o));
-    }
-    if (!waited) cluster.barrier_wait();   // (once, by every thread)
-    waited = true;
-    if (lane < 8) {   // span `lane` of the group: column lane % 2 of the quad's thread lane / 2
-      const float e = __shfl_sync(0x000000ffu, best[0], lane >> 1), f = __shfl_sync(0x000000ffu, best[1], lane >> 1);
-      const int s = group * 8 + lane;
-      if (s < n) estimate0[s] = (there >> (4 * lane)) & 1 ? __float_as_uint(lane & 1 ? f : e) & 0xffffffffu : kNoSpan;
-    }
-  }
-  if (!waited) cluster.barrier_wait();
-  {
-    uint32_t w = max(wide & 0xffffu, wide >> 16);
-    w = __reduce_max_sync(0xffffffffu, w);
-    if (lane == 0) atomicMax(widest0, w << 16);
-  }
-  cluster.sync();
-  if (rank) return;
-
-  // ---- the first block: what is taken for sure, what is between ----
   auto kept = [&](int s) { return s < p.first || s >= n - p.last; };
-  {
-    uint32_t size = 0;   // largest sum of |q| over a row, as its bits (NaN above infinity above all)
-    for (int r = warp; r < rows; r += kPickWarps) {
-      const __nv_bfloat16* q = p.q + ((size_t)(b * p.Q + r / G) * p.heads + head * G + r % G) * HD;
-      float x = 0.f;
-      for (int d = lane; d < HD; d += 32) x += fabsf(bf2f(q[d]));
-      x = warp_sum(x);
-      size = max(size, __float_as_uint(x));
-    }
-    if (lane == 0) q_size[warp] = size;
+  for (int i = threadIdx.x; i < p.warps; i += kPickThreads) {
+    const uint32_t w = __ldcg(p.wide + ((size_t)b * p.kv_heads + head) * p.warps + i);
+    if (w) atomicMax(&widest, w);
   }
   int always = 0, others = 0;
   float lo = INFINITY, hi = -INFINITY;
   for (int s = threadIdx.x; s < n; s += kPickThreads) {
-    const uint32_t e = estimate[s];
+    const uint32_t e = __ldcg(p.estimates + ((size_t)b * p.kv_heads + head) * p.max_spans + s);
+    estimate[s] = e;
     if (e == kNoSpan) continue;
     if (kept(s)) {
       ++always;
@@ -291,12 +311,10 @@ __global__ void __launch_bounds__(kPickThreads, 2) span_select_kernel(SelectPara
   }
   always = pick_total(always, sums);
   others = pick_total(others, sums);
-  uint32_t q_most = 0;
 #pragma unroll
   for (int w = 0; w < kPickWarps; ++w) {
     lo = fminf(lo, low[w]);
     hi = fmaxf(hi, high[w]);
-    q_most = max(q_most, q_size[w]);
   }
   const float size = __uint_as_float(q_most) * __uint_as_float(widest);
   const int want = min(p.count - always, others);   // beside those that are kept
@@ -372,7 +390,8 @@ __global__ void __launch_bounds__(kPickThreads, 2) span_select_kernel(SelectPara
     for (int i = warp; i < m; i += kPickWarps) {
       const int s = span_of(i);
       if (s < 0) continue;
-      const unsigned long long key = exact_score<HD>(p, b, head, page_at(table + s / subs, p.num_blocks), s % subs);
+      const __nv_bfloat16* both = bounds_at(p, page_at(table + sub_page(p, s), p.num_blocks), s, head, HD);
+      const unsigned long long key = finite ? exact_score<HD, true>(both, q_rows, rows) : exact_score<HD, false>(both, q_rows, rows);
       if (lane == 0) keys[i] = key;
     }
     __syncthreads();

@@ -148,7 +148,8 @@ SIGNATURES: dict[str, tuple] = {
     "ssdk_rope_axes_store_kv": (C.c_int, [VP, VP, C.c_int, C.c_char_p, VP, VP, C.c_int64, C.c_int, VP, VP, C.c_float, VP, VP, VP, C.c_int64,
                                           C.c_int, C.c_int, C.c_int, C.c_int, VP]),
     "ssdk_span_bounds": (C.c_int, [VP, VP, VP, VP] + [C.c_int] * 6 + [C.c_int64, C.c_int, VP]),
-    "ssdk_select_spans": (C.c_int, [VP] * 5 + [C.c_int] * 7 + [C.c_int64] + [C.c_int] * 4 + [VP]),
+    "ssdk_select_spans_scratch_bytes": (C.c_int64, [C.c_int] * 5),
+    "ssdk_select_spans": (C.c_int, [VP] * 6 + [C.c_int] * 7 + [C.c_int64] + [C.c_int] * 4 + [VP]),
     "ssdk_span_attn": (C.c_int, [VP] * 7 + [C.c_int] * 7 + [C.c_int64, C.c_int, C.c_int, C.c_float, VP]),
     "ssdk_sample": (C.c_int, [VP, C.c_int64, VP, C.c_int, C.c_int, C.c_uint64, C.c_uint64, VP, VP]),
     "ssdk_verify_scratch_bytes": (C.c_int64, [C.c_int, C.c_int]),

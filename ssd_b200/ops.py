@@ -293,8 +293,9 @@ def select_spans(q: torch.Tensor, bounds: torch.Tensor, block_tables: torch.Tens
     if last is None:
         last = min((q_len + span - 2) // span + 1, count - first)
     out = torch.empty(B, KV, max(count, 0), dtype=_I32, device=dev)
+    scratch = torch.empty(_L.load().ssdk_select_spans_scratch_bytes(B, KV, block_size, block_tables.shape[1], span), dtype=torch.uint8, device=dev)
     _launch("ssdk_select_spans", dev, q.data_ptr(), bounds.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(),
-            B, q_len, q.shape[1], KV, hd, block_size, block_tables.shape[1], n, span, count, first, last)
+            scratch.data_ptr(), B, q_len, q.shape[1], KV, hd, block_size, block_tables.shape[1], n, span, count, first, last)
     return out
 
 

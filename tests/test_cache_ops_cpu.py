@@ -195,8 +195,8 @@ P = 4096   # an address that no call below gets to use
      [(0, None), (3, None), (4, 0), (4, 70000), (5, 0), (6, 0), (7, 80), (8, 0), (9, 0), (10, 0), (11, 8), (11, 24), (11, 64), (0, P + 8)]),
     ("ssdk_span_attn", [P] * 7 + [2, 1, 4, 2, 64, 32, 2, 4, 16, 3, 0.1, None],
      [(0, None), (5, None), (7, 0), (8, 0), (9, 3), (9, 66), (10, 0), (11, 96), (12, 0), (13, 0), (14, 0), (15, 12), (16, 0), (16, 4097), (17, float("nan")), (6, P + 2), (13, 1 << 27)]),
-    ("ssdk_select_spans", [P] * 5 + [2, 1, 4, 2, 64, 32, 2, 4, 16, 3, 1, 1, None],
-     [(0, None), (4, None), (5, 0), (6, 0), (7, 3), (8, 0), (9, 96), (10, 0), (11, 0), (12, 0), (13, 20), (14, 0), (14, 4097), (15, -1), (16, -1), (16, 3), (1, P + 4)]),
+    ("ssdk_select_spans", [P] * 6 + [2, 1, 4, 2, 64, 32, 2, 4, 16, 3, 1, 1, None],
+     [(0, None), (4, None), (5, None), (6, 0), (7, 0), (8, 3), (9, 0), (10, 96), (11, 0), (12, 0), (13, 0), (14, 20), (15, 0), (15, 4097), (16, -1), (17, -1), (17, 3), (1, P + 4), (12, 20000), (7, 3000)]),
 ])
 def test_refusals_of_the_entry_points(name, good, bad):
     from ssd_b200 import lib
