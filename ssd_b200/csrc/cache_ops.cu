@@ -57,7 +57,11 @@ template <int HD, int MT>
 static int launch_span_attn(Launcher& L, const SpanAttnParams& p, int tiles) {
   static std::atomic<bool> done[64];
   CKI(with_smem(span_attn_kernel<HD, MT>, span_attn_smem(HD, kMaxListed), done));
-  return L.go(span_attn_kernel<HD, MT>, dim3(p.kv_heads, p.B, tiles), dim3(kSpanWarps * 32), span_attn_smem(HD, p.count), p);
+  CK(cudaFuncSetAttribute(span_attn_kernel<HD, MT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  const int forced = env_int("DEV_C", 0);
+  if (forced) L.cluster = forced; else
+  while (L.cluster < 16 && (int64_t)p.B * p.kv_heads * tiles * L.cluster < 2 * kSms && L.cluster * kSpanWarps < p.count * (p.span / kSpanKeys)) L.cluster *= 2;
+  return L.go(span_attn_kernel<HD, MT>, dim3(p.kv_heads * L.cluster, p.B, tiles), dim3(kSpanWarps * 32), span_attn_smem(HD, p.count), p);
 }
 
 template <int HD>

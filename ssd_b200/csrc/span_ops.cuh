@@ -1,5 +1,7 @@
 // span_ops.cuh — attention over a part of a long paged cache: spans of keys are chosen by a bound on their scores, and attention reads the chosen ones only.
 #pragma once
+#include <cooperative_groups.h>
+
 #include "async_copy.cuh"
 #include "cache_ops.cuh"
 #include "common.cuh"
@@ -448,6 +450,7 @@ struct SpanAttnParams {
   float scale_log2;              // scale * log2(e)
 };
 constexpr int kSpanWarps = 4, kSpanStages = 3, kSpanKeys = 16;
+constexpr int kSpanMost = 16;   // blocks of a cluster
 constexpr int span_stage_bytes(int HD) { return 2 * kSpanKeys * (HD + 8) * 2; }
 constexpr int span_attn_smem(int HD, int count) { return kSpanWarps * kSpanStages * span_stage_bytes(HD) + count * 8; }
 
@@ -455,7 +458,10 @@ template <int HD, int MT>
 __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnParams p) {
   constexpr int LDS = HD + 8, KS = HD / 16, ND = HD / 8, SEG = HD / 8;
   extern __shared__ __align__(16) uint8_t span_smem[];
-  const int kvh = blockIdx.x, b = blockIdx.y, tile = gridDim.z - 1 - blockIdx.z;
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = cluster.num_blocks(), rank = cluster.block_rank();
+  const int kvh = blockIdx.x / C, b = blockIdx.y, tile = gridDim.z - 1 - blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int G = p.heads / p.kv_heads, tq = min(p.tokens, p.Q - tile * p.tokens), R = G * tq;
   const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size);
@@ -530,14 +536,14 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
       cp_async16(dv + tok * LDS + seg * 8, p.v_cache + from, valid);
     }
   };
-  const int step = kSpanWarps;
+  const int step = kSpanWarps * C, own = rank * kSpanWarps + warp;
 #pragma unroll
   for (int s = 0; s < kSpanStages - 1; ++s) {
-    if (warp + s * step < pieces) load(warp + s * step, s);
+    if (own + s * step < pieces) load(own + s * step, s);
     cp_async_commit();
   }
   int stage = 0;
-  for (int piece = warp; piece < pieces; piece += step, stage = stage + 1 == kSpanStages ? 0 : stage + 1) {
+  for (int piece = own; piece < pieces; piece += step, stage = stage + 1 == kSpanStages ? 0 : stage + 1) {
     __syncwarp();   // every lane is done with the stage that is filled now
     if (piece + (kSpanStages - 1) * step < pieces) load(piece + (kSpanStages - 1) * step, stage == 0 ? kSpanStages - 1 : stage - 1);
     cp_async_commit();
@@ -628,9 +634,10 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
   cp_async_wait<0>();
   __syncthreads();
 
-  // the warps' parts meet: [warp][row][HD + 8] O | maximum, sum (row stride of 8 banks: fragment stores and row reads are free of conflicts)
+  // The warps' parts meet: [warp][row][HD + 8] O | maximum, sum (row stride of 8 banks: fragment stores and row reads are free of conflicts).
   constexpr int LDO = HD + 8;
   float* parts = reinterpret_cast<float*>(span_smem);
+  float* joined = parts + kSpanWarps * 16 * MT * LDO;   // [row][HD + 8]
   {
     float* w = parts + warp * (16 * MT) * LDO;
 #pragma unroll
@@ -647,6 +654,12 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
     }
   }
   __syncthreads();
+  // four columns of a row from n parts `stride` (or a block) apart
+  auto store = [&](int r, int d, float4 acc, float l) {
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    __nv_bfloat16* dst = p.out + ((size_t)(b * p.Q + tile * p.tokens + r / G) * p.heads + kvh * G + r % G) * HD + d;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  };
   for (int idx = threadIdx.x; idx < R * (HD / 4); idx += kSpanWarps * 32) {
     const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
     float top = -INFINITY;
@@ -665,10 +678,45 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
         l += ml.y * f;
       }
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    __nv_bfloat16* dst = p.out + ((size_t)(b * p.Q + tile * p.tokens + r / G) * p.heads + kvh * G + r % G) * HD + d;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    if (C == 1) {
+      store(r, d, acc, l);
+    } else {
+      *reinterpret_cast<float4*>(joined + r * LDO + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(joined + r * LDO + HD) = make_float2(top, l);
+    }
   }
+  if (C == 1) return;
+  // The blocks' parts meet over the cluster's shared memory, each block joins a share of the columns.
+  cluster.sync();
+  for (int idx = rank * kSpanWarps * 32 + threadIdx.x; idx < R * (HD / 4); idx += C * kSpanWarps * 32) {
+    const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
+    float2 ml[kSpanMost];
+    float4 v[kSpanMost];
+    float top = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kSpanMost; ++c) {
+      if (c < C) {
+        const float* row = cluster.map_shared_rank(joined, c) + r * LDO;
+        ml[c] = *reinterpret_cast<const float2*>(row + HD);
+        v[c] = *reinterpret_cast<const float4*>(row + d);
+        top = fmaxf(top, ml[c].x);
+      }
+    }
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+    if (top != -INFINITY) {
+#pragma unroll
+      for (int c = 0; c < kSpanMost; ++c) {
+        if (c < C) {
+          const float f = exp2f(ml[c].x - top);
+          acc.x += v[c].x * f; acc.y += v[c].y * f; acc.z += v[c].z * f; acc.w += v[c].w * f;
+          l += ml[c].y * f;
+        }
+      }
+    }
+    store(r, d, acc, l);
+  }
+  cluster.sync();   // no block leaves while its part is read
 }
 
 }  // namespace ssdk
