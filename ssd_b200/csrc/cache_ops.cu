@@ -192,7 +192,8 @@ int ssdk_span_attn(const void* q, const void* k_cache, const void* v_cache, cons
   SpanAttnParams p;
   p.q = (const bf16*)q; p.k_cache = (const bf16*)k_cache; p.v_cache = (const bf16*)v_cache; p.tables = block_tables; p.lens = context_lens;
   p.spans = selected; p.out = (bf16*)out; p.num_blocks = num_blocks; p.B = batch; p.Q = q_len; p.heads = heads; p.kv_heads = kv_heads;
-  p.block_size = block_size; p.span = span; p.max_blocks = max_blocks_per_seq; p.count = count; p.scale_log2 = scale * 1.4426950408889634f;
+  p.block_size = block_size; p.span = span; p.max_blocks = max_blocks_per_seq; p.count = count; p.scale_log2 = scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f;
+  p.q_sign = scale < 0.f ? 0x80008000u : 0u; p.q_keep = scale == 0.f ? 0u : ~0u;
   const bool one = G * q_len <= 16;
   const int most = (one ? 16 : 32) / G, tiles = (q_len + most - 1) / most;
   if (tiles > 65535) return fail("span_attn: q_len=%d", q_len);

@@ -447,8 +447,10 @@ struct SpanAttnParams {
   int64_t num_blocks;
   int B, Q, heads, kv_heads, block_size, span, max_blocks, count;
   int tokens;                    // query tokens of a block
-  float scale_log2;              // scale * log2(e)
+  uint32_t q_sign, q_keep;       // the sign of the scale, for two bf16 values; 0 where the scale is 0
+  float scale_log2;              // |scale| * log2(e), or 1
 };
+constexpr float kSpanSlack = 8.f;
 constexpr int kSpanWarps = 4, kSpanStages = 3, kSpanKeys = 16;
 constexpr int kSpanMost = 16;   // blocks of a cluster
 constexpr int span_stage_bytes(int HD) { return 2 * kSpanKeys * (HD + 8) * 2; }
@@ -496,20 +498,19 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
   int lim[MT][2];   // first position that a row does not see
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    const int r0 = mt * 16 + g, r1 = r0 + 8;
-    const __nv_bfloat16* q0 = p.q + ((size_t)(b * p.Q + tile * p.tokens + r0 / G) * p.heads + kvh * G + r0 % G) * HD;
-    const __nv_bfloat16* q1 = p.q + ((size_t)(b * p.Q + tile * p.tokens + r1 / G) * p.heads + kvh * G + r1 % G) * HD;
 #pragma unroll
-    for (int kk = 0; kk < KS; ++kk) {
-      const int c = kk * 16 + 2 * t;
-      qa[mt][kk][0] = r0 < R ? *reinterpret_cast<const uint32_t*>(q0 + c) : 0u;
-      qa[mt][kk][1] = r1 < R ? *reinterpret_cast<const uint32_t*>(q1 + c) : 0u;
-      qa[mt][kk][2] = r0 < R ? *reinterpret_cast<const uint32_t*>(q0 + c + 8) : 0u;
-      qa[mt][kk][3] = r1 < R ? *reinterpret_cast<const uint32_t*>(q1 + c + 8) : 0u;
+    for (int h = 0; h < 2; ++h) {
+      const int r = mt * 16 + g + 8 * h;
+      const __nv_bfloat16* q = p.q + ((size_t)(b * p.Q + tile * p.tokens + r / G) * p.heads + kvh * G + r % G) * HD + 2 * t;
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) {
+        qa[mt][kk][h] = r < R ? (*reinterpret_cast<const uint32_t*>(q + kk * 16) & p.q_keep) ^ p.q_sign : 0u;
+        qa[mt][kk][2 + h] = r < R ? (*reinterpret_cast<const uint32_t*>(q + kk * 16 + 8) & p.q_keep) ^ p.q_sign : 0u;
+      }
+      lim[mt][h] = r < R ? len - p.Q + tile * p.tokens + r / G + 1 : 0;
     }
-    lim[mt][0] = r0 < R ? len - p.Q + tile * p.tokens + r0 / G + 1 : 0;
-    lim[mt][1] = r1 < R ? len - p.Q + tile * p.tokens + r1 / G + 1 : 0;
   }
+  const int seen_by_all = len - p.Q + tile * p.tokens;   // positions below it are seen by every row of the tile
 
   float o[MT][ND][4], mrow[MT][2], lrow[MT][2];
 #pragma unroll
@@ -521,19 +522,29 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
   }
 
   const int per = p.span / kSpanKeys, pieces = n_list * per;
+  constexpr int TOK = 32 / SEG;   // keys that a warp copies at a time
+  const int tok0 = lane / SEG, seg = lane % SEG;
+  const size_t row_step = (size_t)TOK * p.kv_heads * HD;
   auto load = [&](int piece, int stage) {
     const int i = piece / per, off = (piece - i * per) * kSpanKeys;
     const int2 at = where[i];
-    __nv_bfloat16* dk = reinterpret_cast<__nv_bfloat16*>(ring + stage * span_stage_bytes(HD));
+    const bool there = at.x >= 0;
+    __nv_bfloat16* dk = reinterpret_cast<__nv_bfloat16*>(ring + stage * span_stage_bytes(HD)) + tok0 * LDS + seg * 8;
     __nv_bfloat16* dv = dk + kSpanKeys * LDS;
-    const size_t base = ((size_t)max(at.x, 0) + off) * p.kv_heads + kvh;
+    size_t from = there ? (((size_t)at.x + off + tok0) * p.kv_heads + kvh) * HD + seg * 8 : 0;
+    if (there && at.y + off + kSpanKeys <= len) {
 #pragma unroll
-    for (int u = 0; u < kSpanKeys * SEG / 32; ++u) {
-      const int idx = u * 32 + lane, tok = idx / SEG, seg = idx % SEG;
-      const bool valid = at.x >= 0 && at.y + off + tok < len;   // what is not in the context is zero: a stale NaN would pass a weight of 0
-      const size_t from = valid ? (base + (size_t)tok * p.kv_heads) * HD + seg * 8 : 0;
-      cp_async16(dk + tok * LDS + seg * 8, p.k_cache + from, valid);
-      cp_async16(dv + tok * LDS + seg * 8, p.v_cache + from, valid);
+      for (int u = 0; u < kSpanKeys / TOK; ++u, from += row_step) {
+        cp_async16(dk + u * TOK * LDS, p.k_cache + from, true);
+        cp_async16(dv + u * TOK * LDS, p.v_cache + from, true);
+      }
+    } else {
+#pragma unroll 1
+      for (int u = 0; u < kSpanKeys / TOK; ++u, from += row_step) {   // what is not in the context is zero: a stale NaN would pass a weight of 0
+        const bool valid = there && at.y + off + u * TOK + tok0 < len;
+        cp_async16(dk + u * TOK * LDS, p.k_cache + (valid ? from : 0), valid);
+        cp_async16(dv + u * TOK * LDS, p.v_cache + (valid ? from : 0), valid);
+      }
     }
   };
   const int step = kSpanWarps * C, own = rank * kSpanWarps + warp;
@@ -571,51 +582,55 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
         mma_bf16_16816(s[mt][1], qa[mt][kk], kb[2], kb[3]);
       }
     }
+    if (pos0 + kSpanKeys > seen_by_all) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (pos0 + nt * 8 + 2 * t + (e & 1) >= lim[mt][e >> 1]) s[mt][nt][e] = -INFINITY;
+    }
+    // A row's reference is raised, and its sums rescaled, only when a score passes it by kSpanSlack (base 2): weights stay below 2^kSpanSlack, where fp32
+    // and the two bf16 pieces are as fine relative to a value as below 1.
+    float most[MT][2];
+    bool grows = false;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        most[mt][h] = fmaxf(max3(s[mt][0][2 * h], s[mt][0][2 * h + 1], s[mt][1][2 * h]), s[mt][1][2 * h + 1]) * p.scale_log2;
+        grows = grows || most[mt][h] > mrow[mt][h] + kSpanSlack;
+      }
+    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float top = fmaxf(most[mt][h], __shfl_xor_sync(0xffffffffu, most[mt][h], 1));
+          top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)), mrow[mt][h]);
+          const float f = top == mrow[mt][h] ? 1.f : ex2_ftz(mrow[mt][h] - top);   // (from -inf: 0)
+          mrow[mt][h] = top;
+          lrow[mt][h] *= f;
+#pragma unroll
+          for (int i = 0; i < ND; ++i) {
+            o[mt][i][2 * h] *= f;
+            o[mt][i][2 * h + 1] *= f;
+          }
+        }
+    }
     uint32_t ph[MT][4], pl[MT][4];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      float top[2] = {mrow[mt][0], mrow[mt][1]};
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int h = e >> 1, pos = pos0 + nt * 8 + 2 * t + (e & 1);
-          s[mt][nt][e] = pos < lim[mt][h] ? s[mt][nt][e] * p.scale_log2 : -INFINITY;
-          top[h] = fmaxf(top[h], s[mt][nt][e]);
-        }
-      float corr[2], ref[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-        ref[h] = top[h] == -INFINITY ? 0.f : top[h];
-        corr[h] = exp2f(mrow[mt][h] - ref[h]);
-        mrow[mt][h] = top[h];
-      }
-      float sum[2] = {0.f, 0.f};
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[mt][nt][e] = exp2f(s[mt][nt][e] - ref[e >> 1]);
-          sum[e >> 1] += s[mt][nt][e];
-        }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) lrow[mt][h] = lrow[mt][h] * corr[h] + sum[h];
-      if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
-#pragma unroll
-        for (int i = 0; i < ND; ++i) {
-          o[mt][i][0] *= corr[0];
-          o[mt][i][1] *= corr[0];
-          o[mt][i][2] *= corr[1];
-          o[mt][i][3] *= corr[1];
-        }
-      }
+      const float ref[2] = {mrow[mt][0] == -INFINITY ? 0.f : mrow[mt][0], mrow[mt][1] == -INFINITY ? 0.f : mrow[mt][1]};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {   // rows g, g + 8 of keys 0 .. 7, then of keys 8 .. 15
-        const float x = s[mt][i >> 1][2 * (i & 1)], y = s[mt][i >> 1][2 * (i & 1) + 1];
-        ph[mt][i] = pack_bf16x2(x, y);
-        pl[mt][i] = pack_bf16x2(x - bf16_round(x), y - bf16_round(y));
+        const int h = i & 1;
+        const float x = ex2_ftz(fmaf(s[mt][i >> 1][2 * h], p.scale_log2, -ref[h])), y = ex2_ftz(fmaf(s[mt][i >> 1][2 * h + 1], p.scale_log2, -ref[h]));
+        lrow[mt][h] += x + y;
+        const uint32_t high = pack_bf16x2(x, y);
+        ph[mt][i] = high;
+        pl[mt][i] = pack_bf16x2(x - __uint_as_float(high << 16), y - __uint_as_float(high & 0xffff0000u));   // (exact differences)
       }
     }
 #pragma unroll
