@@ -2,11 +2,13 @@
 #include <atomic>
 #include <algorithm>
 #include <cstring>
+#include <numeric>
 
 #include "../../include/ssdk.h"
 #include "cache_ops.cuh"
 #include "host.cuh"
 #include "span_ops.cuh"
+#include "span_tiles.cuh"
 
 using namespace ssdk;
 typedef __nv_bfloat16 bf16;
@@ -53,15 +55,46 @@ static int launch_rope_axes(Launcher& L, const RopeAxesParams& p) {
 
 constexpr int kSms = 148, kMaxSmem = 227 * 1024 - 1024;   // (statics beside it)
 constexpr int kMaxListed = 4096;   // spans of a list
-template <int HD, int MT>
-static int launch_span_attn(Launcher& L, const SpanAttnParams& p, int tiles) {
+// Blocks that share the listed keys of a key head (a cluster).  Two blocks are resident on an SM, so that units x blocks take waves; a block's start and end
+// cost as much as some 512 keys, and the join grows with the blocks.  us for one, two, four, eight blocks: 48 sequences of 8 key heads and 4096 keys 159, 136,
+// 148, 184; one sequence of 8 key heads and 2048 keys 28.7, 17.6, 11.4, 8.6 (sixteen: 9.0); 8 x 7 rows over 8 key heads and 4096 keys (tiles) 96, 54, 36.
+static int span_cluster(int64_t units, int64_t keys, int most) {
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int c = 1; c <= most; c *= 2) {
+    const int64_t cost = (units * c + 2 * kSms - 1) / (2 * kSms) * (512 + 16 * c + keys / c);
+    if (cost < least) {
+      least = cost;
+      best = c;
+    }
+  }
+  return best;
+}
+template <int HD>
+static int launch_span_attn(Launcher& L, const SpanAttnParams& p) {
   static std::atomic<bool> done[64];
-  CKI(with_smem(span_attn_kernel<HD, MT>, span_attn_smem(HD, kMaxListed), done));
-  CK(cudaFuncSetAttribute(span_attn_kernel<HD, MT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  const int forced = env_int("DEV_C", 0);
-  if (forced) L.cluster = forced; else
-  while (L.cluster < 16 && (int64_t)p.B * p.kv_heads * tiles * L.cluster < 2 * kSms && L.cluster * kSpanWarps < p.count * (p.span / kSpanKeys)) L.cluster *= 2;
-  return L.go(span_attn_kernel<HD, MT>, dim3(p.kv_heads * L.cluster, p.B, tiles), dim3(kSpanWarps * 32), span_attn_smem(HD, p.count), p);
+  CKI(with_smem(span_attn_kernel<HD>, span_attn_smem(HD, kMaxListed), done));
+  CK(cudaFuncSetAttribute(span_attn_kernel<HD>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  L.cluster = span_cluster((int64_t)p.B * p.kv_heads, (int64_t)p.count * p.span, kSpanMost);
+  return L.go(span_attn_kernel<HD>, dim3(p.kv_heads * L.cluster, p.B), dim3(kSpanWarps * 32), span_attn_smem(HD, p.count), p);
+}
+template <int HD>
+static int launch_span_tiles(Launcher& L, SpanAttnParams p) {
+  static std::atomic<bool> done[64];
+  CKI(with_smem(span_tile_kernel<HD>, span_tile_smem(HD, kMaxListed), done));
+  WaitWord* waits = op_waits();
+  if (!waits) return fail("span_attn: pinned word for bounded waits not allocated");
+  CKI(waits->check("an earlier call of attention without an engine left is not complete (NaN rows)"));
+  const int G = p.heads / p.kv_heads, most = kTileRows64 / G, tiles = (p.Q + most - 1) / most, box = std::gcd(p.span, kTileKeys);
+  if (tiles > 65535) return fail("span_attn: q_len=%d", p.Q);
+  p.tokens = (p.Q + tiles - 1) / tiles;
+  const int64_t slots = p.num_blocks * p.block_size;
+  CUtensorMap tmQ, tmK, tmV;
+  CKI(make_tmap_heads(&tmQ, p.q, (int64_t)p.B * p.Q, p.heads, HD, G, most));
+  CKI(make_tmap_heads(&tmK, p.k_cache, slots, p.kv_heads, HD, 1, box));
+  CKI(make_tmap_heads(&tmV, p.v_cache, slots, p.kv_heads, HD, 1, box));
+  L.cluster = span_cluster((int64_t)p.B * p.kv_heads * tiles, (int64_t)p.count * p.span, kTileMost);
+  return L.go(span_tile_kernel<HD>, dim3(p.kv_heads * L.cluster, p.B, tiles), dim3(kTileThreads), span_tile_smem(HD, p.count), tmQ, tmK, tmV, p, box, most, waits->word);
 }
 
 template <int HD>
@@ -194,14 +227,10 @@ int ssdk_span_attn(const void* q, const void* k_cache, const void* v_cache, cons
   p.spans = selected; p.out = (bf16*)out; p.num_blocks = num_blocks; p.B = batch; p.Q = q_len; p.heads = heads; p.kv_heads = kv_heads;
   p.block_size = block_size; p.span = span; p.max_blocks = max_blocks_per_seq; p.count = count; p.scale_log2 = scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f;
   p.q_sign = scale < 0.f ? 0x80008000u : 0u; p.q_keep = scale == 0.f ? 0u : ~0u;
-  const bool one = G * q_len <= 16;
-  const int most = (one ? 16 : 32) / G, tiles = (q_len + most - 1) / most;
-  if (tiles > 65535) return fail("span_attn: q_len=%d", q_len);
-  p.tokens = (q_len + tiles - 1) / tiles;
   Launcher L;
   L.st = (cudaStream_t)stream;
-  if (head_dim == 64) return one ? launch_span_attn<64, 1>(L, p, tiles) : launch_span_attn<64, 2>(L, p, tiles);
-  return one ? launch_span_attn<128, 1>(L, p, tiles) : launch_span_attn<128, 2>(L, p, tiles);
+  if (G * (int64_t)q_len <= 16) return head_dim == 64 ? launch_span_attn<64>(L, p) : launch_span_attn<128>(L, p);
+  return head_dim == 64 ? launch_span_tiles<64>(L, p) : launch_span_tiles<128>(L, p);
 }
 
 }  // extern "C"

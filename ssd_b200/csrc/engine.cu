@@ -35,17 +35,6 @@ typedef __nv_bfloat16 bf16;
 // ------------------------------------------------------------------------------------------
 // TMA descriptors
 // ------------------------------------------------------------------------------------------
-static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
-static int get_encode() {
-  if (g_encode) return 0;
-  void* fn = nullptr;
-  cudaDriverEntryPointQueryResult qres;
-  cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres);
-  if (e != cudaSuccess || qres != cudaDriverEntryPointSuccess || !fn)
-    return fail("cuTensorMapEncodeTiled unavailable (%s)", cudaGetErrorString(e));
-  g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-  return 0;
-}
 // bf16 row-major [rows, cols] matrix with `ld` elements between rows (0: dense), box = [box_rows, 64 cols], 128B swizzle
 static int make_tmap(CUtensorMap* tm, const void* ptr, int64_t rows, int64_t cols, int box_rows, int64_t ld = 0) {
   CKI(get_encode());
@@ -77,18 +66,6 @@ static int make_tmap_glu(CUtensorMap* tm, const void* ptr, int64_t ff, int64_t K
   return 0;
 }
 
-// rows [rows][heads][hd] as {column, head, row}; box: 64 columns x box_heads x box_rows
-static int make_tmap_heads(CUtensorMap* tm, const void* ptr, int64_t rows, int64_t heads, int hd, int box_heads, int box_rows) {
-  CKI(get_encode());
-  if (hd % 64 != 0 || ((uintptr_t)ptr & 15) != 0) return fail("TMA: heads of %d", hd);
-  cuuint64_t gdim[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows};
-  cuuint64_t gstride[2] = {(cuuint64_t)hd * 2, (cuuint64_t)heads * hd * 2};
-  cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows}, estr[3] = {1, 1, 1};
-  CUresult r = g_encode(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), gdim, gstride, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled failed (%d) rows of %lld heads of %d x %lld", (int)r, (long long)heads, hd, (long long)rows);
-  return 0;
-}
 
 // ------------------------------------------------------------------------------------------
 // GEMM planning + launch
@@ -173,38 +150,6 @@ static int launch_gemm(Launcher& L, int umma_n, int epi, const CUtensorMap& tmW,
   return fail("no GEMM instance for umma_n=%d epi=%d", umma_n, epi);
 }
 
-// Word in host memory that the kernels of one engine set when a bounded wait of theirs runs out.  Read wherever a call has waited for the
-// stream: a call that does not wait (prompt passes without a token) leaves its report to the next one that does.
-struct WaitWord {
-  unsigned* word = nullptr;   // (unified addressing: the host pointer is the device's too)
-  WaitWord() = default;
-  WaitWord(const WaitWord&) = delete;
-  ~WaitWord() { if (word) cudaFreeHost(word); }
-  bool make() {
-    if (cudaHostAlloc(&word, sizeof(unsigned), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) { word = nullptr; return false; }
-    *word = 0;
-    return true;
-  }
-  int check(const char* whose = "this engine's calls left since the last check is not complete") {
-    volatile unsigned* w = word;
-    if (!*w) return 0;
-    *w = 0;
-    return fail("a bounded wait in a tile-pair product, the prompt attention or the streaming kernel ran out: what %s", whose);
-  }
-};
-// The same for calls without an engine, which do not wait for the stream: rows whose waits ran out are NaN, and the next such call reports it.  One word for the
-// process that is never freed (a kernel in flight may still write to it); made under relaxed capture rules, since the first such call may be a captured one.
-static WaitWord* op_waits() {
-  static WaitWord* const w = [] {
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    (void)cudaThreadExchangeStreamCaptureMode(&mode);
-    WaitWord* made = new WaitWord;
-    if (!made->make()) { delete made; made = nullptr; }
-    (void)cudaThreadExchangeStreamCaptureMode(&mode);
-    return made;
-  }();
-  return w;
-}
 
 // tile pairs of gemm_pair_kernel; p.timeout is filled in here
 static int launch_gemm_pair(Launcher& L, int epi, const CUtensorMap& tmW, const CUtensorMap& tmX, const CUtensorMap& tmXs, GemmPairParams p, int max_tiles) {

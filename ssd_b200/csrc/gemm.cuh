@@ -361,7 +361,7 @@ epilogue_done:
 
 // y[m, n] = bf16( sum_s P[s, m, n] )  — fixed-order split-K reduction (stand-alone op only;
 // inside the engine the consumer kernels fold this in).
-__global__ void splitk_reduce_kernel(const float* __restrict__ P, __nv_bfloat16* __restrict__ y, int S, int M, int N,
+static __global__ void splitk_reduce_kernel(const float* __restrict__ P, __nv_bfloat16* __restrict__ y, int S, int M, int N,
                                      int ldy) {
   pdl_launch_dependents();
   pdl_wait();

@@ -433,9 +433,9 @@ __global__ void __launch_bounds__(kPickThreads) span_pick_kernel(SelectParams p)
 // span_attn_kernel: softmax(scale q k^T) v over the keys of the listed spans, causal to the end of the context as in paged attention (query j of a sequence
 // sees positions <= len - Q + j); grouped heads.  A list may name spans in any order; what lies outside the context or on a page outside the cache
 // is passed over, a row that sees no key is zero.
-// Bound by the bytes of the listed keys and values.  A block owns one key head of one sequence and up to 16 MT of its query rows; its warps take pieces of 16
-// keys in turn, each with a ring of its own (cp.async, no barrier between warps) and a softmax of its own, and meet at the end.
-// Weights go into the second product as two bf16 pieces, sums are fp32.
+// Bound by the bytes of the listed keys and values.  A cluster of blocks owns one key head of one sequence and up to sixteen of its query rows (more:
+// span_tiles.cuh).  Pieces of 16 keys go round the blocks' warps, each with a ring of its own (cp.async, no barrier between warps) and a softmax of its own;
+// at the end warps meet, then blocks.  Weights go into the second product as two bf16 pieces, sums are fp32.
 // ----------------------------------------------------------------------------------
 struct SpanAttnParams {
   const __nv_bfloat16* q;        // [B * Q, H, hd]
@@ -446,7 +446,7 @@ struct SpanAttnParams {
   __nv_bfloat16* out;            // [B * Q, H, hd]
   int64_t num_blocks;
   int B, Q, heads, kv_heads, block_size, span, max_blocks, count;
-  int tokens;                    // query tokens of a block
+  int tokens;                    // query tokens of a tile
   uint32_t q_sign, q_keep;       // the sign of the scale, for two bf16 values; 0 where the scale is 0
   float scale_log2;              // |scale| * log2(e), or 1
 };
@@ -456,16 +456,16 @@ constexpr int kSpanMost = 16;   // blocks of a cluster
 constexpr int span_stage_bytes(int HD) { return 2 * kSpanKeys * (HD + 8) * 2; }
 constexpr int span_attn_smem(int HD, int count) { return kSpanWarps * kSpanStages * span_stage_bytes(HD) + count * 8; }
 
-template <int HD, int MT>
+template <int HD>
 __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnParams p) {
   constexpr int LDS = HD + 8, KS = HD / 16, ND = HD / 8, SEG = HD / 8;
   extern __shared__ __align__(16) uint8_t span_smem[];
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank();
-  const int kvh = blockIdx.x / C, b = blockIdx.y, tile = gridDim.z - 1 - blockIdx.z;
+  const int kvh = blockIdx.x / C, b = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int G = p.heads / p.kv_heads, tq = min(p.tokens, p.Q - tile * p.tokens), R = G * tq;
+  const int G = p.heads / p.kv_heads, R = G * p.Q;
   const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size);
   int2* where = reinterpret_cast<int2*>(span_smem + kSpanWarps * kSpanStages * span_stage_bytes(HD));   // [count] slot (-1: none) and position of a span's first key
   uint8_t* ring = span_smem + warp * kSpanStages * span_stage_bytes(HD);
@@ -494,32 +494,24 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
     for (int w = 0; w < kSpanWarps; ++w) n_list = max(n_list, last[w]);
   }
 
-  uint32_t qa[MT][KS][4];
-  int lim[MT][2];   // first position that a row does not see
+  uint32_t qa[KS][4];
+  int lim[2];   // first position that a row does not see
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
+  for (int h = 0; h < 2; ++h) {
+    const int r = g + 8 * h;
+    const __nv_bfloat16* q = p.q + ((size_t)(b * p.Q + r / G) * p.heads + kvh * G + r % G) * HD + 2 * t;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = mt * 16 + g + 8 * h;
-      const __nv_bfloat16* q = p.q + ((size_t)(b * p.Q + tile * p.tokens + r / G) * p.heads + kvh * G + r % G) * HD + 2 * t;
-#pragma unroll
-      for (int kk = 0; kk < KS; ++kk) {
-        qa[mt][kk][h] = r < R ? (*reinterpret_cast<const uint32_t*>(q + kk * 16) & p.q_keep) ^ p.q_sign : 0u;
-        qa[mt][kk][2 + h] = r < R ? (*reinterpret_cast<const uint32_t*>(q + kk * 16 + 8) & p.q_keep) ^ p.q_sign : 0u;
-      }
-      lim[mt][h] = r < R ? len - p.Q + tile * p.tokens + r / G + 1 : 0;
+    for (int kk = 0; kk < KS; ++kk) {
+      qa[kk][h] = r < R ? (*reinterpret_cast<const uint32_t*>(q + kk * 16) & p.q_keep) ^ p.q_sign : 0u;
+      qa[kk][2 + h] = r < R ? (*reinterpret_cast<const uint32_t*>(q + kk * 16 + 8) & p.q_keep) ^ p.q_sign : 0u;
     }
+    lim[h] = r < R ? len - p.Q + r / G + 1 : 0;
   }
-  const int seen_by_all = len - p.Q + tile * p.tokens;   // positions below it are seen by every row of the tile
+  const int seen_by_all = len - p.Q + 1;   // positions below it are seen by every row
 
-  float o[MT][ND][4], mrow[MT][2], lrow[MT][2];
+  float o[ND][4], mrow[2] = {-INFINITY, -INFINITY}, lrow[2] = {0.f, 0.f};
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-    for (int i = 0; i < ND; ++i) o[mt][i][0] = o[mt][i][1] = o[mt][i][2] = o[mt][i][3] = 0.f;
-    mrow[mt][0] = mrow[mt][1] = -INFINITY;
-    lrow[mt][0] = lrow[mt][1] = 0.f;
-  }
+  for (int i = 0; i < ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
   const int per = p.span / kSpanKeys, pieces = n_list * per;
   constexpr int TOK = 32 / SEG;   // keys that a warp copies at a time
@@ -567,125 +559,95 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
     const __nv_bfloat16* cV = cK + kSpanKeys * LDS;
     const int mi = lane >> 3, rr = lane & 7;
 
-    float s[MT][2][4];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
+    float s[2][4] = {};
 #pragma unroll
     for (int kk = 0; kk < KS; ++kk) {   // a 16 x 16 piece of the keys: tokens 0 .. 7 and 8 .. 15, channels 0 .. 7 and 8 .. 15
       uint32_t kb[4];
       ldmatrix_x4(kb, cK + ((mi >> 1) * 8 + rr) * LDS + kk * 16 + (mi & 1) * 8);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        mma_bf16_16816(s[mt][0], qa[mt][kk], kb[0], kb[1]);
-        mma_bf16_16816(s[mt][1], qa[mt][kk], kb[2], kb[3]);
-      }
+      mma_bf16_16816(s[0], qa[kk], kb[0], kb[1]);
+      mma_bf16_16816(s[1], qa[kk], kb[2], kb[3]);
     }
     if (pos0 + kSpanKeys > seen_by_all) {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (pos0 + nt * 8 + 2 * t + (e & 1) >= lim[mt][e >> 1]) s[mt][nt][e] = -INFINITY;
+        for (int e = 0; e < 4; ++e)
+          if (pos0 + nt * 8 + 2 * t + (e & 1) >= lim[e >> 1]) s[nt][e] = -INFINITY;
     }
     // A row's reference is raised, and its sums rescaled, only when a score passes it by kSpanSlack (base 2): weights stay below 2^kSpanSlack, where fp32
     // and the two bf16 pieces are as fine relative to a value as below 1.
-    float most[MT][2];
-    bool grows = false;
+    float most[2];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int h = 0; h < 2; ++h) most[h] = fmaxf(max3(s[0][2 * h], s[0][2 * h + 1], s[1][2 * h]), s[1][2 * h + 1]) * p.scale_log2;
+    if (__any_sync(0xffffffffu, most[0] > mrow[0] + kSpanSlack || most[1] > mrow[1] + kSpanSlack)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        most[mt][h] = fmaxf(max3(s[mt][0][2 * h], s[mt][0][2 * h + 1], s[mt][1][2 * h]), s[mt][1][2 * h + 1]) * p.scale_log2;
-        grows = grows || most[mt][h] > mrow[mt][h] + kSpanSlack;
-      }
-    if (__any_sync(0xffffffffu, grows)) {
+        float top = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
+        top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)), mrow[h]);
+        const float f = top == mrow[h] ? 1.f : ex2_ftz(mrow[h] - top);   // (from -inf: 0)
+        mrow[h] = top;
+        lrow[h] *= f;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float top = fmaxf(most[mt][h], __shfl_xor_sync(0xffffffffu, most[mt][h], 1));
-          top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)), mrow[mt][h]);
-          const float f = top == mrow[mt][h] ? 1.f : ex2_ftz(mrow[mt][h] - top);   // (from -inf: 0)
-          mrow[mt][h] = top;
-          lrow[mt][h] *= f;
-#pragma unroll
-          for (int i = 0; i < ND; ++i) {
-            o[mt][i][2 * h] *= f;
-            o[mt][i][2 * h + 1] *= f;
-          }
+        for (int i = 0; i < ND; ++i) {
+          o[i][2 * h] *= f;
+          o[i][2 * h + 1] *= f;
         }
-    }
-    uint32_t ph[MT][4], pl[MT][4];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const float ref[2] = {mrow[mt][0] == -INFINITY ? 0.f : mrow[mt][0], mrow[mt][1] == -INFINITY ? 0.f : mrow[mt][1]};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {   // rows g, g + 8 of keys 0 .. 7, then of keys 8 .. 15
-        const int h = i & 1;
-        const float x = ex2_ftz(fmaf(s[mt][i >> 1][2 * h], p.scale_log2, -ref[h])), y = ex2_ftz(fmaf(s[mt][i >> 1][2 * h + 1], p.scale_log2, -ref[h]));
-        lrow[mt][h] += x + y;
-        const uint32_t high = pack_bf16x2(x, y);
-        ph[mt][i] = high;
-        pl[mt][i] = pack_bf16x2(x - __uint_as_float(high << 16), y - __uint_as_float(high & 0xffff0000u));   // (exact differences)
       }
+    }
+    uint32_t ph[4], pl[4];
+    const float ref[2] = {mrow[0] == -INFINITY ? 0.f : mrow[0], mrow[1] == -INFINITY ? 0.f : mrow[1]};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {   // rows g, g + 8 of keys 0 .. 7, then of keys 8 .. 15
+      const int h = i & 1;
+      const float x = ex2_ftz(fmaf(s[i >> 1][2 * h], p.scale_log2, -ref[h])), y = ex2_ftz(fmaf(s[i >> 1][2 * h + 1], p.scale_log2, -ref[h]));
+      lrow[h] += x + y;
+      ph[i] = pack_bf16x2(x, y);
+      pl[i] = pack_bf16x2(x - __uint_as_float(ph[i] << 16), y - __uint_as_float(ph[i] & 0xffff0000u));   // (exact differences)
     }
 #pragma unroll
     for (int nd = 0; nd < ND; nd += 2) {
       uint32_t vb[4];
       ldmatrix_x4_trans(vb, cV + ((mi & 1) * 8 + rr) * LDS + nd * 8 + (mi >> 1) * 8);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        mma_bf16_16816(o[mt][nd], ph[mt], vb[0], vb[1]);
-        mma_bf16_16816(o[mt][nd + 1], ph[mt], vb[2], vb[3]);
-        mma_bf16_16816(o[mt][nd], pl[mt], vb[0], vb[1]);
-        mma_bf16_16816(o[mt][nd + 1], pl[mt], vb[2], vb[3]);
-      }
+      mma_bf16_16816(o[nd], ph, vb[0], vb[1]);
+      mma_bf16_16816(o[nd + 1], ph, vb[2], vb[3]);
+      mma_bf16_16816(o[nd], pl, vb[0], vb[1]);
+      mma_bf16_16816(o[nd + 1], pl, vb[2], vb[3]);
     }
   }
   cp_async_wait<0>();
   __syncthreads();
 
-  // The warps' parts meet: [warp][row][HD + 8] O | maximum, sum (row stride of 8 banks: fragment stores and row reads are free of conflicts).
+  // The warps' parts meet: [warp][row][HD + 8] O | reference, sum (row stride of 8 banks: fragment stores and row reads are free of conflicts).
   constexpr int LDO = HD + 8;
   float* parts = reinterpret_cast<float*>(span_smem);
-  float* joined = parts + kSpanWarps * 16 * MT * LDO;   // [row][HD + 8]
-  {
-    float* w = parts + warp * (16 * MT) * LDO;
+  float* joined = parts + kSpanWarps * 16 * LDO;   // [row][HD + 8]
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+  for (int h = 0; h < 2; ++h) {
+    lrow[h] += __shfl_xor_sync(0xffffffffu, lrow[h], 1);
+    lrow[h] += __shfl_xor_sync(0xffffffffu, lrow[h], 2);
+    float* row = parts + (warp * 16 + g + 8 * h) * LDO;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        lrow[mt][h] += __shfl_xor_sync(0xffffffffu, lrow[mt][h], 1);
-        lrow[mt][h] += __shfl_xor_sync(0xffffffffu, lrow[mt][h], 2);
-        float* row = w + (mt * 16 + g + 8 * h) * LDO;
-#pragma unroll
-        for (int i = 0; i < ND; ++i) *reinterpret_cast<float2*>(row + i * 8 + 2 * t) = make_float2(o[mt][i][2 * h], o[mt][i][2 * h + 1]);
-        if (t == 0) *reinterpret_cast<float2*>(row + HD) = make_float2(mrow[mt][h], lrow[mt][h]);
-      }
-    }
+    for (int i = 0; i < ND; ++i) *reinterpret_cast<float2*>(row + i * 8 + 2 * t) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+    if (t == 0) *reinterpret_cast<float2*>(row + HD) = make_float2(mrow[h], lrow[h]);
   }
   __syncthreads();
-  // four columns of a row from n parts `stride` (or a block) apart
+  // four columns of a row
   auto store = [&](int r, int d, float4 acc, float l) {
     const float inv = l > 0.f ? 1.f / l : 0.f;
-    __nv_bfloat16* dst = p.out + ((size_t)(b * p.Q + tile * p.tokens + r / G) * p.heads + kvh * G + r % G) * HD + d;
+    __nv_bfloat16* dst = p.out + ((size_t)(b * p.Q + r / G) * p.heads + kvh * G + r % G) * HD + d;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
   };
   for (int idx = threadIdx.x; idx < R * (HD / 4); idx += kSpanWarps * 32) {
     const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kSpanWarps; ++w) top = fmaxf(top, parts[(w * 16 * MT + r) * LDO + HD]);
+    for (int w = 0; w < kSpanWarps; ++w) top = fmaxf(top, parts[(w * 16 + r) * LDO + HD]);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
     if (top != -INFINITY) {
 #pragma unroll
       for (int w = 0; w < kSpanWarps; ++w) {
-        const float* row = parts + (w * 16 * MT + r) * LDO;
+        const float* row = parts + (w * 16 + r) * LDO;
         const float2 ml = *reinterpret_cast<const float2*>(row + HD);
         const float4 v = *reinterpret_cast<const float4*>(row + d);
         const float f = exp2f(ml.x - top);

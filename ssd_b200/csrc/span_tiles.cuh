@@ -1,0 +1,322 @@
+// span_tiles.cuh — span_attention of more than sixteen query rows to a key head, on tcgen05.
+//
+// The pipeline of prompt_attn_kernel's twin form: S = Q K^T of up to 64 rows and 64 keys into TMEM, P = exp2(S - m) one row per thread, O += P V with P out of
+// TMEM.  The queries lie in rows 0 .. 63 and again in 64 .. 127: these make the low bf16 pieces of the weights, add up in lanes of their own and are added
+// at the end.  A chunk of 64 keys is gathered from the listed spans by TMA boxes of gcd(span, 64) keys, in list order; what is missing from the last
+// chunk is loaded from behind the cache (zeros) and masked.  A cluster of blocks shares the chunks of a key head; their sums meet in shared memory.
+// Up to sixteen rows span_attn_kernel is as fast as the memory; with more its mma.sync products bound it: 8 sequences of 7 rows, 64 heads over 8 of 128,
+// 4096 listed keys each: 63 us on two m16 tiles a warp, 36 here.
+#pragma once
+#include <cooperative_groups.h>
+
+#include "prompt_attention.cuh"
+#include "span_ops.cuh"
+
+namespace ssdk {
+
+constexpr int kTileRows64 = 64, kTileKeys = 64, kTileStages = 2, kTileThreads = 192;
+constexpr int kTileMost = 8;   // blocks of a cluster
+// query twice | keys and values; behind them the places of the listed spans
+constexpr int span_tile_body(int HD) { return 2 * kTileRows64 * HD * 2 + kTileStages * 2 * kTileKeys * HD * 2; }
+constexpr int span_tile_smem(int HD, int count) { return span_tile_body(HD) + 1024 + count * 8; }
+
+template <int HD>
+__global__ void __launch_bounds__(kTileThreads, 2)
+span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const SpanAttnParams p,
+                 const int box, const int q_tokens, unsigned* timeout) {
+  namespace cg = cooperative_groups;
+  constexpr int HALVES = HD / 64;                    // 64-column boxes of a row
+  constexpr int kQHalf = 2 * kTileRows64 * 128, kKHalf = kTileKeys * 128, kTile = HALVES * kKHalf;
+  extern __shared__ uint8_t span_tile_raw[];
+  __shared__ __align__(8) uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int s_failed, found[kTileThreads / 32];
+  uint8_t* smem = span_tile_raw + ((1024u - (smem_u32(span_tile_raw) & 1023u)) & 1023u);
+  uint8_t* sQ = smem;
+  uint8_t* sK = sQ + HALVES * kQHalf;
+  uint8_t* sV = sK + kTileStages * kTile;
+  int2* where = reinterpret_cast<int2*>(smem + span_tile_body(HD));   // [count] slot and position of the first key of a span that is there
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = cluster.num_blocks(), rank = cluster.block_rank();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = blockIdx.x / C, b = blockIdx.y, tile = (int)gridDim.z - 1 - (int)blockIdx.z;
+  const int G = p.heads / p.kv_heads, tok0 = tile * p.tokens, tq = min(p.tokens, p.Q - tok0), rows = tq * G;
+  const int half = (rows + 31) & ~31;                // rows of the warps that have some
+  const int live = 2 * half;                         // threads that hand P over
+
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    mbar_init(&q_full, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1);
+      mbar_init(&s_full[s], 1); mbar_init(&p_full[s], live); mbar_init(&pv_done[s], 1);
+    }
+    fence_mbar_init();
+    s_failed = 0;
+  }
+  if (warp == 1) { tmem_alloc(&tmem_slot, 256); tmem_relinquish(); }
+  // the spans that are there, in the list's order
+  const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size);
+  int spans = 0;
+  for (int base = 0; base < p.count; base += kTileThreads) {
+    const int i = base + (int)threadIdx.x, s = i < p.count ? p.spans[((size_t)b * p.kv_heads + kvh) * p.count + i] : -1;
+    int2 at = make_int2(-1, 0);
+    if (s >= 0 && (long long)s * p.span < len) {
+      at.y = s * p.span;
+      const int page = page_at(p.tables + (size_t)b * p.max_blocks + at.y / p.block_size, p.num_blocks);
+      if (page >= 0) at.x = page * p.block_size + at.y % p.block_size;
+    }
+    const uint32_t there = __ballot_sync(0xffffffffu, at.x >= 0);
+    if (lane == 0) found[warp] = __popc(there);
+    __syncthreads();
+    int before = spans + __popc(there & ((1u << lane) - 1));
+#pragma unroll
+    for (int w = 0; w < kTileThreads / 32; ++w) {
+      before += w < warp ? found[w] : 0;
+      spans += found[w];
+    }
+    if (at.x >= 0) where[before] = at;
+    __syncthreads();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot, tmem_o = tmem + 128;   // S / P buffers at columns 0 and 64, O behind them
+
+  const int per = p.span / box, boxes = kTileKeys / box, pieces = spans * per;   // boxes of a span, of a chunk, in all
+  const int chunks = (pieces + boxes - 1) / boxes, share = (chunks + C - 1) / C;
+  const int first = rank * share, n = max(0, min(share, chunks - first));
+  // slot and position of a box: behind the last one no keys
+  auto box_at = [&](int piece) {
+    if (piece >= pieces) return make_int2((int)(p.num_blocks * p.block_size), 1 << 30);
+    const int i = piece / per, off = (piece - i * per) * box;
+    const int2 at = where[i];
+    return make_int2(at.x + off, at.y + off);
+  };
+  // chunk i on barrier i & 1; parity(i) is that use's.  A wait by parity is only right while the barrier is in that use or the one behind it: as in
+  // prompt_attn_kernel, whose order of products and waits this is.
+  auto parity = [](int i) { return (uint32_t)(i >> 1) & 1u; };
+  float l = 0.f, m = -INFINITY;
+  bool ok = true;
+  const int q4 = warp & 3, r = (q4 & 1) * 32 + lane;
+  const bool softmax = warp >= 2, low = q4 >= 2, in = softmax && (r & ~31) < half;   // (whole warps) low: the same row as two warps before, its low pieces
+  const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      mbar_arrive_expect_tx(&q_full, HALVES * 2 * 128 * G * q_tokens);
+      for (int h = 0; h < HALVES; ++h)
+        for (int x = 0; x < 2 * kTileRows64; x += kTileRows64) tma_load_3d(sQ + h * kQHalf + x * 128, &tmQ, &q_full, h * 64, kvh * G, b * p.Q + tok0);
+      int i = 0;
+      for (; i < n; ++i) {
+        const int s = i & 1;
+        int slots[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) slots[j] = j < boxes ? box_at((first + i) * boxes + j).x : 0;
+        if (!mbar_wait_cluster(&k_empty[s], parity(i) ^ 1u, timeout)) break;
+        mbar_arrive_expect_tx(&k_full[s], kTile);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j < boxes)
+            for (int h = 0; h < HALVES; ++h) tma_load_3d(sK + s * kTile + h * kKHalf + j * box * 128, &tmK, &k_full[s], h * 64, kvh, slots[j]);
+        if (!mbar_wait_cluster(&v_empty[s], parity(i) ^ 1u, timeout)) { mbar_wait_cluster(&k_full[s], parity(i), timeout); break; }
+        mbar_arrive_expect_tx(&v_full[s], kTile);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j < boxes)
+            for (int h = 0; h < HALVES; ++h) tma_load_3d(sV + s * kTile + h * kKHalf + j * box * 128, &tmV, &v_full[s], h * 64, kvh, slots[j]);
+      }
+      // nothing is in flight into this block's memory when it leaves, also after a wait ran out
+      mbar_wait_cluster(&q_full, 0, timeout);
+      for (int j = max(0, i - 2); j < i; ++j) {
+        mbar_wait_cluster(&k_full[j & 1], parity(j), timeout);
+        mbar_wait_cluster(&v_full[j & 1], parity(j), timeout);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = make_umma_idesc_bf16(2 * kTileRows64, kTileKeys);
+      constexpr uint32_t idesc_o = make_umma_idesc_bf16(2 * kTileRows64, HD) | (1u << 16);   // V: b_major = MN
+      auto scores = [&](int i) {
+        if (!mbar_wait_cluster(&k_full[i & 1], parity(i), timeout)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          const uint64_t qd = make_umma_desc_k128(sQ + h * kQHalf), kd = make_umma_desc_k128(sK + (i & 1) * kTile + h * kKHalf);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_bf16_ss(tmem + (i & 1) * 64, qd + 2 * k, kd + 2 * k, idesc_s, (uint32_t)((h | k) != 0));
+        }
+        umma_commit(&k_empty[i & 1]);
+        umma_commit(&s_full[i & 1]);
+        return true;
+      };
+      bool go = n > 0 && mbar_wait_cluster(&q_full, 0, timeout) && scores(0);
+      for (int i = 0; i < n && go; ++i) {
+        // the scores of chunk i + 1 go over the P that the product of chunk i - 1 reads: products of different shapes and accumulators
+        // have no order of their own
+        if (i > 0 && !(go = mbar_wait_cluster(&pv_done[(i - 1) & 1], parity(i - 1), timeout))) break;
+        if (i + 1 < n && !(go = scores(i + 1))) break;
+        if (!(go = mbar_wait_cluster(&p_full[i & 1], parity(i), timeout) && mbar_wait_cluster(&v_full[i & 1], parity(i), timeout))) break;
+        tc_fence_after();
+        const uint64_t vd = make_umma_desc_mn128(sV + (i & 1) * kTile, kKHalf);
+#pragma unroll
+        for (int k = 0; k < kTileKeys / 16; ++k)   // 16 keys: 2048 B of V, 8 columns of P
+          umma_bf16_ts(tmem_o, tmem + (i & 1) * 64 + 8 * k, vd + 128 * k, idesc_o, (uint32_t)((i | k) != 0));
+        umma_commit(&v_empty[i & 1]);
+        umma_commit(&pv_done[i & 1]);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int lim = len - p.Q + tok0 + r / G + 1;        // first position this row does not see (rows behind the tile's: some, dropped)
+    const int seen_by_all = len - p.Q + tok0 + 1;        // positions below it are seen by every row
+    ok = in;
+    for (int i = 0; i < n && in; ++i) {
+      const uint32_t sp = tmem + lanes + (uint32_t)(i & 1) * 64u;
+      // positions of the chunk's keys, sixteen at a time
+      const int piece = (first + i) * boxes;
+      const int mine = lane < boxes ? box_at(piece + lane).y : 0;
+      const bool whole = __all_sync(0xffffffffu, lane >= boxes || mine + box <= seen_by_all);
+      int pos[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = 16 * j / box;
+        pos[j] = __shfl_sync(0xffffffffu, mine, at) + (16 * j - at * box);
+      }
+      if (!(ok = warp_wait(&s_full[i & 1], parity(i), timeout))) break;
+      tc_fence_after();
+      uint32_t u[64];
+#pragma unroll
+      for (int c = 0; c < 64; c += 16) tmem_ld_32x32b_x16(sp + c, u + c);
+      tmem_ld_wait();
+      if (p.q_sign || !p.q_keep) {   // a scale that is not positive
+#pragma unroll
+        for (int c = 0; c < 64; ++c) u[c] = (u[c] & p.q_keep) ^ (p.q_sign & 0x80000000u);
+      }
+      if (!whole) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (pos[c / 16] + c % 16 >= lim) u[c] = 0xff800000u;   // -inf
+      }
+      const float mx = row_max(u) * p.scale_log2;
+      const bool grow = mx > m + kPromptSlack;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float f = grow ? exp2f(m - mx) : 1.f;   // (m = -inf: 0)
+        if (grow) m = mx;
+        l *= f;
+        if (i > 0) {
+          if (!(ok = warp_wait(&pv_done[(i - 1) & 1], parity(i - 1), timeout))) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 16) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(tmem_o + lanes + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+            tmem_st_32x32b_x16(tmem_o + lanes + c, o);
+          }
+        }
+      }
+      const float ms = m == -INFINITY ? 0.f : m;
+      l += low ? row_exp<false, true>(u, p.scale_log2, ms) : row_exp<true, false>(u, p.scale_log2, ms);
+#pragma unroll
+      for (int c = 0; c < 32; c += 16) tmem_st_32x32b_x16(sp + c, u + c);
+      tmem_st_wait();
+      if (!whole) {   // slots behind the context hold anything, and 0 x NaN is NaN
+        bool stale = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) stale = stale || (pos[j] < (1 << 29) && pos[j] + 16 > len);
+        if (stale) {   // (the same for all warps)
+          if (!(ok = warp_wait(&v_full[i & 1], parity(i), timeout))) break;
+          for (int j = low ? half + r : r; j < kTileKeys * 8; j += live) {
+            const int key = j >> 3, x = key >> 4;
+            if ((x == 0 ? pos[0] : x == 1 ? pos[1] : x == 2 ? pos[2] : pos[3]) + (key & 15) >= len)
+#pragma unroll
+              for (int h = 0; h < HALVES; ++h) *reinterpret_cast<uint4*>(sV + (i & 1) * kTile + h * kKHalf + j * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(&p_full[i & 1]);
+    }
+    if (ok && n > 0) ok = warp_wait(&pv_done[(n - 1) & 1], parity(n - 1), timeout);
+    tc_fence_after();
+  }
+
+  // ---- the sums of a row: low pieces to the row's warp, then [row][HD + 4] O | reference, sum in the stages (every product has read them) ----
+  constexpr int LDO = HD + 4;
+  float* joined = reinterpret_cast<float*>(sK);
+  if (softmax && in && low) {
+    if (!ok) s_failed = 1;
+    if (ok && n > 0)
+      for (int c = 0; c < HD; c += 16) {
+        uint32_t o[16];
+        tmem_ld_32x32b_x16(tmem_o + lanes + c, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) *reinterpret_cast<uint4*>(joined + r * LDO + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+      }
+  }
+  __syncthreads();
+  if (softmax && in && !low) {
+    const bool good = ok && !s_failed;
+    if (n > 0 && good)
+      for (int c = 0; c < HD; c += 16) {
+        uint32_t o[16];
+        tmem_ld_32x32b_x16(tmem_o + lanes + c, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          float4* at = reinterpret_cast<float4*>(joined + r * LDO + c + j);
+          const float4 x = *at;
+          *at = make_float4(x.x + __uint_as_float(o[j]), x.y + __uint_as_float(o[j + 1]), x.z + __uint_as_float(o[j + 2]), x.w + __uint_as_float(o[j + 3]));
+        }
+      }
+    // a wait ran out: the row is NaN.  Without chunks (or keys) the row has no part in the sum.
+    const float2 ml = !good ? make_float2(0.f, __int_as_float(0x7fffffff)) : n > 0 ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+    *reinterpret_cast<float2*>(joined + r * LDO + HD) = ml;
+    if (!good || n == 0)
+      for (int c = 0; c < HD; c += 4) *reinterpret_cast<float4*>(joined + r * LDO + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, 256);   // (before the other blocks are waited for: they may wait for tensor memory)
+  cluster.sync();
+  for (int idx = rank * kTileThreads + threadIdx.x; idx < rows * (HD / 4); idx += C * kTileThreads) {
+    const int row = idx / (HD / 4), d = idx % (HD / 4) * 4;
+    float2 ml[kTileMost];
+    float4 v[kTileMost];
+    float top = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kTileMost; ++c)
+      if (c < C) {
+        const float* part = cluster.map_shared_rank(joined, c) + row * LDO;
+        ml[c] = *reinterpret_cast<const float2*>(part + HD);
+        v[c] = *reinterpret_cast<const float4*>(part + d);
+        top = fmaxf(top, ml[c].x);
+      }
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+    if (top != -INFINITY) {
+#pragma unroll
+      for (int c = 0; c < kTileMost; ++c)
+        if (c < C) {
+          const float f = exp2f(ml[c].x - top);
+          acc.x += v[c].x * f; acc.y += v[c].y * f; acc.z += v[c].z * f; acc.w += v[c].w * f;
+          sum += ml[c].y * f;
+        }
+    }
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;   // (NaN stays)
+    __nv_bfloat16* dst = p.out + ((size_t)(b * p.Q + tok0 + row / G) * p.heads + kvh * G + row % G) * HD + d;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  }
+  cluster.sync();   // no block leaves while its part is read
+}
+
+}  // namespace ssdk
