@@ -46,11 +46,16 @@ template <int HD>
 static int launch_rope_axes(Launcher& L, const RopeAxesParams& p) {
   constexpr int GROUPS = kRopeAxesThreads / (HD / 16);
   const int n = p.heads + 2 * p.kv_heads, groups = (n + GROUPS - 1) / GROUPS;
-  const int nh = (int64_t)p.M * groups <= 1024 ? 1 : (groups >= 4 ? 4 : groups >= 2 ? 2 : 1);
-  const dim3 grid(p.M, (groups + nh - 1) / nh);
-  if (nh == 1) return L.go(rope_axes_kernel<HD, 1>, grid, dim3(kRopeAxesThreads), 0, p);
-  if (nh == 2) return L.go(rope_axes_kernel<HD, 2>, grid, dim3(kRopeAxesThreads), 0, p);
-  return L.go(rope_axes_kernel<HD, 4>, grid, dim3(kRopeAxesThreads), 0, p);
+  // heads of a thread: one while the blocks are few, else all of a row's in equal shares of up to five
+  const int shares = (int64_t)p.M * groups <= 1024 ? groups : (groups + 4) / 5, nh = (groups + shares - 1) / shares;
+  const dim3 grid(p.M, (groups + nh - 1) / nh), block(kRopeAxesThreads);
+  switch (nh) {
+    case 1: return L.go(rope_axes_kernel<HD, 1>, grid, block, 0, p);
+    case 2: return L.go(rope_axes_kernel<HD, 2>, grid, block, 0, p);
+    case 3: return L.go(rope_axes_kernel<HD, 3>, grid, block, 0, p);
+    case 4: return L.go(rope_axes_kernel<HD, 4>, grid, block, 0, p);
+    default: return L.go(rope_axes_kernel<HD, 5>, grid, block, 0, p);
+  }
 }
 
 constexpr int kSms = 148, kMaxSmem = 227 * 1024 - 1024;   // (statics beside it)
@@ -174,9 +179,13 @@ int ssdk_span_bounds(const void* k_cache, const int32_t* block_tables, const int
   p.k_cache = (const bf16*)k_cache; p.tables = block_tables; p.lens = context_lens; p.bounds = (bf16*)bounds; p.num_blocks = num_blocks;
   p.B = batch; p.max_blocks = max_blocks_per_seq; p.block_size = block_size; p.span = span; p.kv_heads = kv_heads; p.head_dim = head_dim;
   p.fresh = (int)std::min<int64_t>(new_tokens, (int64_t)max_blocks_per_seq * block_size);
+  const int cols = kv_heads * head_dim / 8;
+  p.width = cols >= 32 ? 32 : cols >= 16 ? 16 : 8;
+  const int64_t blocks = (((int64_t)p.fresh + span - 2) / span + 1) * ((cols + p.width - 1) / p.width);
+  if (blocks >= (1ll << 31)) return fail("span_bounds: %d new tokens of %d heads", new_tokens, kv_heads);
   Launcher L;
   L.st = (cudaStream_t)stream;
-  return L.go(span_bounds_kernel, dim3((p.fresh + span - 2) / span + 1, batch), dim3(kBoundsThreads), 0, p);
+  return L.go(span_bounds_kernel, dim3((unsigned)blocks, batch), dim3(kBoundsThreads), 0, p);
 }
 
 int64_t ssdk_select_spans_scratch_bytes(int batch, int kv_heads, int block_size, int max_blocks_per_seq, int span) {

@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(Sele
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kPickThreads) span_pick_kernel(SelectParams p) {
+__global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams p) {
   extern __shared__ __align__(16) uint8_t pick_smem_bytes[];
   __shared__ int sums[kPickWarps], pick_bin;
   __shared__ uint32_t widest, q_most;      // bits of the largest |lo|, |hi|, and of the largest sum of |q| over a row

@@ -100,7 +100,9 @@ int main(int argc, char** argv) {
     auto bounds = rd<bf16>(f, (size_t)p.num_blocks * (p.block_size / p.span) * p.kv_heads * 2 * p.head_dim);
     p.k_cache = keys.p; p.tables = tables.p; p.lens = lens.p; p.bounds = bounds.p;
     dim3 grid;
-    grid.x = (unsigned)((p.fresh + p.span - 2) / p.span + 1);
+    const int cols = p.kv_heads * p.head_dim / 8;
+    p.width = cols >= 32 ? 32 : cols >= 16 ? 16 : 8;
+    grid.x = (unsigned)(((p.fresh + p.span - 2) / p.span + 1) * ((cols + p.width - 1) / p.width));
     grid.y = (unsigned)p.B;
     emu::launch(+[](ssdk::SpanBoundsParams q) { ssdk::span_bounds_kernel(q); }, p, grid, ssdk::kBoundsThreads, 0, 4);
     wr(o, bounds);
