@@ -42,22 +42,6 @@ static int with_smem(Kernel* kernel, int bytes, std::atomic<bool>* done) {
   return 0;
 }
 
-template <int HD>
-static int launch_rope_axes(Launcher& L, const RopeAxesParams& p) {
-  constexpr int GROUPS = kRopeAxesThreads / (HD / 16);
-  const int n = p.heads + 2 * p.kv_heads, groups = (n + GROUPS - 1) / GROUPS;
-  // heads of a thread: one while the blocks are few, else all of a row's in equal shares of up to five
-  const int shares = (int64_t)p.M * groups <= 1024 ? groups : (groups + 4) / 5, nh = (groups + shares - 1) / shares;
-  const dim3 grid(p.M, (groups + nh - 1) / nh), block(kRopeAxesThreads);
-  switch (nh) {
-    case 1: return L.go(rope_axes_kernel<HD, 1>, grid, block, 0, p);
-    case 2: return L.go(rope_axes_kernel<HD, 2>, grid, block, 0, p);
-    case 3: return L.go(rope_axes_kernel<HD, 3>, grid, block, 0, p);
-    case 4: return L.go(rope_axes_kernel<HD, 4>, grid, block, 0, p);
-    default: return L.go(rope_axes_kernel<HD, 5>, grid, block, 0, p);
-  }
-}
-
 constexpr int kSms = 148, kMaxSmem = 227 * 1024 - 1024;   // (statics beside it)
 constexpr int kMaxListed = 4096;   // spans of a list
 // Blocks that share the listed keys of a key head (a cluster).  Two blocks are resident on an SM, so that units x blocks take waves; a block's start and end
@@ -102,6 +86,19 @@ static int launch_span_tiles(Launcher& L, SpanAttnParams p) {
   return L.go(span_tile_kernel<HD>, dim3(p.kv_heads * L.cluster, p.B, tiles), dim3(kTileThreads), span_tile_smem(HD, p.count), tmQ, tmK, tmV, p, box, most, waits->word);
 }
 
+template <int HD>
+static int launch_rope_axes(Launcher& L, RopeAxesParams p) {
+  // a row's heads to one warp when the rows fill the SMs (20 warps each), else as many warps as ask for all of them at once
+  const int n = p.heads + 2 * p.kv_heads, at_once = rope_axes_heads(HD), batches = (n + at_once - 1) / at_once;
+  const int most = (int)std::min<int64_t>(batches, std::max<int64_t>(1, (int64_t)kSms * 20 / p.M));
+  p.per = (batches + most - 1) / most * at_once;
+  p.shares = (n + p.per - 1) / p.per;
+  constexpr int W = kRopeAxesThreads / 32;
+  const int64_t units = (int64_t)p.M * p.shares;
+  if (units >= (1ll << 31) - W) return fail("rope_axes: %d rows of %d heads", p.M, n);
+  const dim3 grid((unsigned)((units + W - 1) / W)), block(kRopeAxesThreads);
+  return p.q_norm_w || p.k_norm_w ? L.go(rope_axes_kernel<HD, true>, grid, block, 0, p) : L.go(rope_axes_kernel<HD, false>, grid, block, 0, p);
+}
 template <int HD>
 static int launch_select(Launcher& L, const SelectParams& p) {
   static std::atomic<bool> done[64];
@@ -149,7 +146,7 @@ int ssdk_rope_axes_store_kv(const void* qkv, const int64_t* positions, int axes,
   if (axes < 1 || axes > 4 || max_pos < 1 || num_slots < 1) return fail("rope_axes: %d axes (1 to 4), %lld positions, %lld slots", axes, (long long)max_pos, (long long)num_slots);
   if (heads + 2 * (int64_t)kv_heads > 65535) return fail("rope_axes: too many heads");
   if (!qkv || !positions || !axis_of || !slot_mapping || !rope_table || !q_out || !k_cache || !v_cache) return fail("rope_axes: null argument");
-  if (off16(qkv, q_out, k_cache, v_cache) || off16(q_norm_w, k_norm_w)) return fail("rope_axes: arrays must start at multiples of 16 bytes");
+  if (off16(qkv, q_out, k_cache, v_cache) || off16(q_norm_w, k_norm_w, rope_table)) return fail("rope_axes: arrays must start at multiples of 16 bytes");
   RopeAxesParams p;
   memset(&p, 0, sizeof(p));
   for (int i = 0; i < rot_dim / 2; ++i) {

@@ -139,8 +139,9 @@ __global__ void __launch_bounds__(kPlaceThreads) place_tokens_kernel(PlaceParams
 // rope_axes_kernel: frequency i turns the channels (i, i + rot/2) of every query and key head by the angle of the row's position on axis
 // axis_of[i] (time, height, width, ...); channels from rot on pass.  Optional RMS norm per head in front.  Norm, rotation and the table's cosines and
 // sines are fp32, and a value is rounded once, where it is stored.  Queries go to q, keys and values to their slot of the cache.
-// Bound by memory: 2 bytes read and 2 written per channel.  HD / 16 lanes own a head, 16 channels each in two 16-byte pieces; a thread keeps its
-// frequencies over NH heads of its row, all asked for before the angles, which the block gathers from the rows of the axes into shared memory.
+// Bound by memory: 2 bytes read and 2 written per channel.  HD / 16 lanes own a head, 16 channels each in two 16-byte pieces.  A warp takes a row (or, when
+// rows are few, a share of its heads) and keeps the angles, four times 32 / (HD / 16) heads asked for at once, products and sums two at a time: with a row's heads
+// over four warps that gathered the angles through shared memory the instructions bound it (16000 rows of 32 heads of 128 with norms: 58 us, issue slots 70 % busy).
 // A row with a position outside the table has NaN queries and stores nothing.
 // ----------------------------------------------------------------------------------
 struct RopeAxesParams {
@@ -153,94 +154,154 @@ struct RopeAxesParams {
   int64_t top, num_slots;
   float eps;
   int M, heads, kv_heads, rot, axes;
+  int shares, per;               // warps of a row, heads of a warp (a multiple of the heads that it asks for at once)
   uint32_t axis_of[8];           // two bits per frequency
 };
-constexpr int kRopeAxesThreads = 128;
+constexpr int kRopeAxesThreads = 128, kRopeAxesAhead = 2;
+constexpr int rope_axes_heads(int HD) { return 32 / (HD / 16) * kRopeAxesAhead; }   // that a warp asks for at once
 
-SSDK_DEVINL void turn(float& x, float& y, float c, float s) {
-  const float u = x * c - y * s;
-  y = y * c + x * s;
-  x = u;
+#ifndef SSDK_HOST_EMU
+SSDK_DEVINL uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+#endif
+// eight bf16 values as four pairs of fp32, and back
+SSDK_DEVINL void pairs_of(const uint4& v, uint64_t* f) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = (uint64_t)(w[i] & 0xffff0000u) << 32 | w[i] << 16;
+}
+SSDK_DEVINL uint4 bf16_of(const uint64_t* f) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float x, y;
+    unpack2(f[i], &x, &y);
+    w[i] = pack_bf16x2(x, y);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <int HD, int NH>
-__global__ void __launch_bounds__(kRopeAxesThreads, NH <= 3 ? 8 : 6) rope_axes_kernel(RopeAxesParams p) {
-  constexpr int LPH = HD / 16, GROUPS = kRopeAxesThreads / LPH;
-  SSDK_STATIC_SMEM(float4, cs4, 64);
-  float* cs = reinterpret_cast<float*>(cs4);
-  const int m = blockIdx.x, lane = threadIdx.x % LPH, half = p.rot / 2;
-  const int head0 = blockIdx.y * (NH * GROUPS) + threadIdx.x / LPH, n_heads = p.heads + 2 * p.kv_heads;
-  const bool turns = lane < p.rot / 16;
-  const int c0 = turns ? lane * 8 : p.rot + (lane - p.rot / 16) * 16, c1 = turns ? half + lane * 8 : c0 + 8;
-
+template <int HD, bool NORM>
+__global__ void __launch_bounds__(kRopeAxesThreads, 4) rope_axes_kernel(RopeAxesParams p) {
+  constexpr int LPH = HD / 16, SIDE = 32 / LPH;   // lanes of a head, heads side by side
+  const int unit = (int)blockIdx.x * (kRopeAxesThreads / 32) + (int)(threadIdx.x >> 5);   // (below 2^31: the host sees to it)
+  const int m = unit / p.shares, share = unit - m * p.shares;
+  if (m >= p.M) return;
+  const int piece = threadIdx.x % LPH, side = threadIdx.x % 32 / LPH, half = p.rot / 2;
+  const int n_heads = p.heads + 2 * p.kv_heads, first = share * p.per, end = min(first + p.per, n_heads);
+  const bool turns = piece < p.rot / 16;
+  const int c0 = turns ? piece * 8 : p.rot + (piece - p.rot / 16) * 16, c1 = turns ? half + piece * 8 : c0 + 8;
   const __nv_bfloat16* src = p.qkv + (size_t)m * n_heads * HD;
-  const int slot = p.slots[m];
-  uint4 a[NH], b[NH];
+
+  uint4 a[kRopeAxesAhead], b[kRopeAxesAhead];
+  auto load = [&](int head0) {
 #pragma unroll
-  for (int i = 0; i < NH; ++i) {
-    const int head = head0 + i * GROUPS;
-    a[i] = b[i] = make_uint4(0, 0, 0, 0);
-    if (head < n_heads) {
-      a[i] = ld_nc_v4(src + (size_t)head * HD + c0);
-      b[i] = ld_nc_v4(src + (size_t)head * HD + c1);
+    for (int i = 0; i < kRopeAxesAhead; ++i) {
+      const int head = head0 + i * SIDE + side;
+      a[i] = b[i] = make_uint4(0, 0, 0, 0);
+      if (head < end) {
+        a[i] = ld_nc_v4(src + head * HD + c0);
+        b[i] = ld_nc_v4(src + head * HD + c1);
+      }
     }
-  }
+  };
+  load(first);
+  const int slot = p.slots[m];
   bool known = true;
   for (int x = 0; x < p.axes; ++x) {
     const int64_t at = p.positions[(size_t)x * p.M + m];
     known = known && at >= 0 && at < p.top;
   }
-  if (known)
-    for (int i = threadIdx.x; i < p.rot; i += kRopeAxesThreads) {
-      const int f = i < half ? i : i - half, axis = (p.axis_of[f >> 4] >> (2 * (f & 15))) & 3;
-      cs[i] = p.table[(size_t)p.positions[(size_t)axis * p.M + m] * p.rot + i];
-    }
-  __syncthreads();
-  const bool stores = known && slot >= 0 && slot < p.num_slots;
+  uint64_t co[4] = {}, si[4] = {}, minus[4] = {};   // cos, sin, -sin of this lane's eight frequencies
+  if (turns && known) {
+    const uint32_t axes = (p.axis_of[piece >> 1] >> (16 * (piece & 1))) & 0xffffu;
+    if (axes == (axes & 3) * 0x5555u) {
+      const float* row = p.table + (size_t)p.positions[(size_t)(axes & 3) * p.M + m] * p.rot + piece * 8;
 #pragma unroll
-  for (int i = 0; i < NH; ++i) {
-    const int head = head0 + i * GROUPS, kind = head < p.heads ? 0 : (head < p.heads + p.kv_heads ? 1 : 2);   // q, k, v
-    float x[8], y[8];
-    unpack_bf16x8(a[i], x);
-    unpack_bf16x8(b[i], y);
-    const __nv_bfloat16* w = kind == 0 ? p.q_norm_w : p.k_norm_w;
-    if (w) {   // (the same for all lanes of a head; every lane of a warp takes part in the sums)
-      float ss = 0.f;
+      for (int i = 0; i < 4; i += 2) {
+        const float4 c = *reinterpret_cast<const float4*>(row + 2 * i), s = *reinterpret_cast<const float4*>(row + half + 2 * i);
+        co[i] = pack2(c.x, c.y); co[i + 1] = pack2(c.z, c.w);
+        si[i] = pack2(s.x, s.y); si[i + 1] = pack2(s.z, s.w);
+      }
+    } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss += x[j] * x[j] + y[j] * y[j];
-#pragma unroll
-      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float r = rsqrtf(ss / (float)HD + p.eps);
-      float wx[8], wy[8];
-      unpack_bf16x8(ld_nc_v4(w + c0), wx);
-      unpack_bf16x8(ld_nc_v4(w + c1), wy);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] *= r * wx[j];
-        y[j] *= r * wy[j];
+      for (int i = 0; i < 4; ++i) {
+        const float* r0 = p.table + (size_t)p.positions[(size_t)(axes >> (4 * i) & 3) * p.M + m] * p.rot + piece * 8 + 2 * i;
+        const float* r1 = p.table + (size_t)p.positions[(size_t)(axes >> (4 * i + 2) & 3) * p.M + m] * p.rot + piece * 8 + 2 * i + 1;
+        co[i] = pack2(r0[0], r1[0]);
+        si[i] = pack2(r0[half], r1[half]);
       }
     }
-    if (head >= n_heads || (kind != 0 && !stores)) continue;
-    __nv_bfloat16* dst = kind == 0 ? p.q + ((size_t)m * p.heads + head) * HD
-                                   : (kind == 1 ? p.k_cache + ((size_t)slot * p.kv_heads + (head - p.heads)) * HD
-                                                : p.v_cache + ((size_t)slot * p.kv_heads + (head - p.heads - p.kv_heads)) * HD);
-    if (kind != 2) {
-      if (turns && known) {
 #pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-          const float4 co = *reinterpret_cast<const float4*>(cs + c0 + j), si = *reinterpret_cast<const float4*>(cs + c1 + j);
-          turn(x[j], y[j], co.x, si.x);
-          turn(x[j + 1], y[j + 1], co.y, si.y);
-          turn(x[j + 2], y[j + 2], co.z, si.z);
-          turn(x[j + 3], y[j + 3], co.w, si.w);
+    for (int i = 0; i < 4; ++i) minus[i] = si[i] ^ 0x8000000080000000ull;
+  }
+  const bool stores = known && slot >= 0 && slot < p.num_slots;
+  __nv_bfloat16* q_row = p.q + (size_t)m * p.heads * HD;
+  const size_t in_cache = (size_t)max(slot, 0) * p.kv_heads * HD;
+
+  for (int head0 = first; head0 < end; head0 += kRopeAxesAhead * SIDE) {
+    uint4 now_a[kRopeAxesAhead], now_b[kRopeAxesAhead];
+#pragma unroll
+    for (int i = 0; i < kRopeAxesAhead; ++i) {
+      now_a[i] = a[i];
+      now_b[i] = b[i];
+    }
+    load(head0 + kRopeAxesAhead * SIDE);   // (behind the last head nothing)
+#pragma unroll
+    for (int i = 0; i < kRopeAxesAhead; ++i) {
+      const int head = head0 + i * SIDE + side, kind = head < p.heads ? 0 : (head < p.heads + p.kv_heads ? 1 : 2);   // q, k, v
+      uint4 x = now_a[i], y = now_b[i];
+      if (head0 + i * SIDE < p.heads + p.kv_heads) {   // (the whole warp: some of its heads are no values)
+        uint64_t u[4], v[4];
+        pairs_of(x, u);
+        pairs_of(y, v);
+        if (NORM) {
+          uint64_t ss2 = mul2(u[0], u[0]);
+#pragma unroll
+          for (int j = 1; j < 4; ++j) ss2 = fma2(u[j], u[j], ss2);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) ss2 = fma2(v[j], v[j], ss2);
+          float s0, s1;
+          unpack2(ss2, &s0, &s1);
+          s0 += s1;
+#pragma unroll
+          for (int o = LPH / 2; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+          const __nv_bfloat16* weight = kind == 0 ? p.q_norm_w : p.k_norm_w;
+          if (weight) {
+            const float r = rsqrtf(s0 / (float)HD + p.eps);
+            const uint64_t rr = pack2(r, r);
+            uint64_t w[4];
+            pairs_of(*reinterpret_cast<const uint4*>(weight + c0), w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j] = mul2(mul2(u[j], rr), w[j]);
+            pairs_of(*reinterpret_cast<const uint4*>(weight + c1), w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = mul2(mul2(v[j], rr), w[j]);
+          }
+        }
+        if (turns) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint64_t t = fma2(u[j], co[j], mul2(v[j], minus[j]));
+            v[j] = fma2(v[j], co[j], mul2(u[j], si[j]));
+            u[j] = t;
+          }
+        }
+        if (kind != 2) {
+          x = bf16_of(u);
+          y = bf16_of(v);
+          if (!known) x = y = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
         }
       }
-      a[i] = pack_bf16x8(x);
-      b[i] = pack_bf16x8(y);
-      if (!known) a[i] = b[i] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+      if (head < end && (kind == 0 || stores)) {
+        __nv_bfloat16* dst = kind == 0 ? q_row + head * HD : (kind == 1 ? p.k_cache + in_cache + (head - p.heads) * HD : p.v_cache + in_cache + (head - p.heads - p.kv_heads) * HD);
+        *reinterpret_cast<uint4*>(dst + c0) = x;
+        *reinterpret_cast<uint4*>(dst + c1) = y;
+      }
     }
-    *reinterpret_cast<uint4*>(dst + c0) = a[i];
-    *reinterpret_cast<uint4*>(dst + c1) = b[i];
   }
 }
 

@@ -19,6 +19,30 @@ uint32_t pick_bf16x2(uint32_t a, uint32_t b) {
   }
   return out;
 }
+inline void unpack2(uint64_t v, float* x, float* y) {
+  const uint32_t a = (uint32_t)v, b = (uint32_t)(v >> 32);
+  std::memcpy(x, &a, 4);
+  std::memcpy(y, &b, 4);
+}
+inline uint64_t pack2(float x, float y) {
+  uint32_t a, b;
+  std::memcpy(&a, &x, 4);
+  std::memcpy(&b, &y, 4);
+  return (uint64_t)b << 32 | a;
+}
+inline uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  float x[2], y[2], z[2];
+  unpack2(a, x, x + 1);
+  unpack2(b, y, y + 1);
+  unpack2(c, z, z + 1);
+  return pack2(std::fma(x[0], y[0], z[0]), std::fma(x[1], y[1], z[1]));
+}
+inline uint64_t mul2(uint64_t a, uint64_t b) {
+  float x[2], y[2];
+  unpack2(a, x, x + 1);
+  unpack2(b, y, y + 1);
+  return pack2(x[0] * y[0], x[1] * y[1]);
+}
 inline uint32_t min_bf16x2(uint32_t a, uint32_t b) { return pick_bf16x2<false>(a, b); }
 inline uint32_t max_bf16x2(uint32_t a, uint32_t b) { return pick_bf16x2<true>(a, b); }
 }  // namespace ssdk
@@ -65,7 +89,7 @@ int main(int argc, char** argv) {
     return 0;
   }
   if (mode == "rope") {
-    auto h = rd<int32_t>(f, 10);   // M H KV hd rot axes top num_slots norm heads-per-thread
+    auto h = rd<int32_t>(f, 10);   // M H KV hd rot axes top num_slots norm most-shares
     auto eps = rd<float>(f, 1);
     const int hd = h.p[3], rot = h.p[4];
     ssdk::RopeAxesParams p;
@@ -80,14 +104,15 @@ int main(int argc, char** argv) {
     Exact<bf16> q((size_t)p.M * p.heads * hd), kc((size_t)p.num_slots * p.kv_heads * hd), vc((size_t)p.num_slots * p.kv_heads * hd);
     p.qkv = qkv.p; p.positions = positions.p; p.slots = slots.p; p.table = table.p; p.q = q.p; p.k_cache = kc.p; p.v_cache = vc.p;
     p.q_norm_w = h.p[8] ? qn.p : nullptr; p.k_norm_w = h.p[8] ? kn.p : nullptr;
-    const int nh = h.p[9], groups = ssdk::kRopeAxesThreads / (hd / 16);
+    // shares of a row, as the host cuts it
+    const int n = p.heads + 2 * p.kv_heads, at_once = ssdk::rope_axes_heads(hd), batches = (n + at_once - 1) / at_once, most = std::min(batches, h.p[9]);
+    p.per = (batches + most - 1) / most * at_once;
+    p.shares = (n + p.per - 1) / p.per;
     dim3 grid;
-    grid.x = (unsigned)p.M;
-    grid.y = (unsigned)((p.heads + 2 * p.kv_heads + groups * nh - 1) / (groups * nh));
-    if (hd == 64 && nh == 1) emu::launch(ssdk::rope_axes_kernel<64, 1>, p, grid, ssdk::kRopeAxesThreads, 0, 8);
-    else if (hd == 64) emu::launch(ssdk::rope_axes_kernel<64, 4>, p, grid, ssdk::kRopeAxesThreads, 0, 8);
-    else if (nh == 1) emu::launch(ssdk::rope_axes_kernel<128, 1>, p, grid, ssdk::kRopeAxesThreads, 0, 8);
-    else emu::launch(ssdk::rope_axes_kernel<128, 4>, p, grid, ssdk::kRopeAxesThreads, 0, 8);
+    grid.x = (unsigned)((p.M * p.shares + 3) / 4);
+    const auto kernel = hd == 64 ? (h.p[8] ? ssdk::rope_axes_kernel<64, true> : ssdk::rope_axes_kernel<64, false>)
+                                 : (h.p[8] ? ssdk::rope_axes_kernel<128, true> : ssdk::rope_axes_kernel<128, false>);
+    emu::launch(kernel, p, grid, ssdk::kRopeAxesThreads, 0, 8);
     wr(o, q); wr(o, kc); wr(o, vc);
     return 0;
   }

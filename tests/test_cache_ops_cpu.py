@@ -74,8 +74,8 @@ def test_place_source_bad_pages(tmp_path):
 
 
 @needs_gxx
-@pytest.mark.parametrize("H,KV,hd,rot,axes,norm,nh", [(2, 1, 64, 64, 3, 0, 1), (6, 2, 128, 128, 3, 1, 4), (5, 1, 128, 64, 2, 1, 1), (4, 2, 64, 32, 4, 0, 4), (1, 1, 128, 16, 1, 1, 1)])
-def test_rope_axes_source(tmp_path, H, KV, hd, rot, axes, norm, nh):
+@pytest.mark.parametrize("H,KV,hd,rot,axes,norm,shares", [(2, 1, 64, 64, 3, 0, 1), (6, 2, 128, 128, 3, 1, 4), (5, 1, 128, 64, 2, 1, 1), (4, 2, 64, 32, 4, 0, 4), (1, 1, 128, 16, 1, 1, 1), (20, 7, 128, 128, 3, 0, 2), (30, 5, 64, 64, 2, 1, 1)])
+def test_rope_axes_source(tmp_path, H, KV, hd, rot, axes, norm, shares):
     g = gen(H, hd, rot, axes)
     M, top, pages, S, eps = 7, 40, 2, 16, 1e-6
     qkv = torch.randn(M, (H + 2 * KV) * hd, generator=g).to(BF)
@@ -88,7 +88,7 @@ def test_rope_axes_source(tmp_path, H, KV, hd, rot, axes, norm, nh):
     axis_of = [i % axes for i in range(rot // 2)]
     qn, kn = (1 + 0.2 * torch.randn(2, hd, generator=g)).to(BF)
     table = angles(top, rot)
-    data = _run("rope", [i32([M, H, KV, hd, rot, axes, top, pages * S, norm, nh]), np.float32([eps]), i32(axis_of), positions.numpy(), slots, table, qn, kn, qkv], tmp_path)
+    data = _run("rope", [i32([M, H, KV, hd, rot, axes, top, pages * S, norm, shares]), np.float32([eps]), i32(axis_of), positions.numpy(), slots, table, qn, kn, qkv], tmp_path)
     q, kc, vc = _take(data, (BF, (M, H * hd)), (BF, (pages, S, KV, hd)), (BF, (pages, S, KV, hd)))
     zeros = torch.zeros(pages, S, KV, hd, dtype=BF)
     wq, wk, wv, slack_q, slack_k = plain.rope(qkv, positions, axis_of, slots, table, zeros, zeros, H, KV, hd, qn if norm else None, kn if norm else None, eps)
