@@ -32,12 +32,13 @@ static int check_spans(const char* who, int heads, int kv_heads, int head_dim, i
 }
 // the attributes that a kernel needs, once per device
 template <typename Kernel>
-static int with_smem(Kernel* kernel, int bytes, std::atomic<bool>* done) {
+static int with_smem(Kernel* kernel, int bytes, std::atomic<bool>* done, bool wide_clusters = false) {
   int dev = 0;
   CK(cudaGetDevice(&dev));
   if (dev < 64 && done[dev].load(std::memory_order_acquire)) return 0;
   CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   CK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  if (wide_clusters) CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   if (dev < 64) done[dev].store(true, std::memory_order_release);
   return 0;
 }
@@ -62,8 +63,7 @@ static int span_cluster(int64_t units, int64_t keys, int most) {
 template <int HD>
 static int launch_span_attn(Launcher& L, const SpanAttnParams& p) {
   static std::atomic<bool> done[64];
-  CKI(with_smem(span_attn_kernel<HD>, span_attn_smem(HD, kMaxListed), done));
-  CK(cudaFuncSetAttribute(span_attn_kernel<HD>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  CKI(with_smem(span_attn_kernel<HD>, span_attn_smem(HD, kMaxListed), done, true));
   L.cluster = span_cluster((int64_t)p.B * p.kv_heads, (int64_t)p.count * p.span, kSpanMost);
   return L.go(span_attn_kernel<HD>, dim3(p.kv_heads * L.cluster, p.B), dim3(kSpanWarps * 32), span_attn_smem(HD, p.count), p);
 }

@@ -179,31 +179,38 @@ def verify(logits_p: torch.Tensor, logits_q: torch.Tensor, speculations: torch.T
 _BF, _I32, _I64, _F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
 
 
-def _check(name: str, *args):
-    """(tensor, its name, dtype, shape with -1 for any size) of every argument; returns their device."""
-    dev = args[0][0].device
+def _check(name: str, *args) -> int:
+    """(tensor, its name, dtype, shape) of every argument; returns the index of their GPU.  (Small calls are bound by the host: one test
+    per argument, and the reason only where it fails.)"""
+    gpu = args[0][0].get_device()
     for t, what, dtype, shape in args:
+        if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == gpu:
+            continue
         if t.dtype is not dtype:
             raise TypeError(f"{name}: {what}: expected {dtype}, got {t.dtype}")
-        if t.dim() != len(shape) or any(n not in (-1, have) for n, have in zip(shape, t.shape)):
-            raise ValueError(f"{name}: {what}: expected shape {shape}, got {tuple(t.shape)}")
+        if t.shape != shape:
+            raise ValueError(f"{name}: {what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
         if not t.is_contiguous():
             raise ValueError(f"{name}: {what}: must be contiguous")
-        if t.device != dev:
-            raise ValueError(f"{name}: {what}: on {t.device}, {args[0][1]} on {dev}")
-    if dev.type != "cuda":
+        raise ValueError(f"{name}: {what}: on {t.device}, {args[0][1]} on {args[0][0].device}")
+    if gpu < 0:
         raise RuntimeError(f"{name}: CUDA tensors required (libssdk has no CPU path)")
-    return dev
+    return gpu
 
 
-def _launch(name: str, dev: torch.device, *args):
-    """One entry point of libssdk on the current stream of the tensors' device."""
-    fn = getattr(_L.load(), name)
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+def _last(t: torch.Tensor, dims: int) -> int:
+    """The last size of a tensor that is to have `dims` of them, else one that fits no tensor."""
+    return t.shape[-1] if t.dim() == dims else -1
+
+
+def _launch(name: str, gpu: int, *args):
+    """One entry point of libssdk on the tensors' GPU and its current stream."""
+    fn = getattr(_L._lib or _L.load(), name)
+    if gpu == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(gpu))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+        with torch.cuda.device(gpu):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(gpu))
     if rc:
         _L.check(rc, name)
 
@@ -218,15 +225,15 @@ def place_tokens(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table
     Returns positions int64 [rows], slot_mapping int32 [rows], row_seqs int32 [rows] (rows behind the last token: 0, -1, -1),
     cu_rows int32 [B + 1], lens int32 [B] (context_lens + new_lens; sequences that found no pages or rows: context_lens) and the
     new free_used.  Sequences are served in order, each as a whole: see ssdk_place_tokens (include/ssdk.h)."""
-    B = context_lens.shape[0]
-    dev = _check("place_tokens", (context_lens, "context_lens", _I32, (B,)), (new_lens, "new_lens", _I32, (B,)),
-                 (block_tables, "block_tables", _I32, (B, -1)), (free_blocks, "free_blocks", _I32, (-1,)), (free_used, "free_used", _I32, (1,)))
-    positions = torch.empty(max(rows, 0), dtype=_I64, device=dev)
-    words = torch.empty(2 * positions.shape[0] + 2 * B + 2, dtype=_I32, device=dev)
-    slots, seqs, cu, lens, used = words.split((positions.shape[0], positions.shape[0], B + 1, B, 1))
-    _launch("ssdk_place_tokens", dev, context_lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(), free_blocks.data_ptr(), free_used.data_ptr(),
-            positions.data_ptr(), slots.data_ptr(), seqs.data_ptr(), cu.data_ptr(), lens.data_ptr(), used.data_ptr(), B, block_tables.shape[1],
-            free_blocks.shape[0], rows, block_size, num_blocks)
+    B, width, F = _last(context_lens, 1), _last(block_tables, 2), _last(free_blocks, 1)
+    gpu = _check("place_tokens", (context_lens, "context_lens", _I32, (B,)), (new_lens, "new_lens", _I32, (B,)),
+                 (block_tables, "block_tables", _I32, (B, width)), (free_blocks, "free_blocks", _I32, (F,)), (free_used, "free_used", _I32, (1,)))
+    if rows < 1:
+        raise ValueError(f"place_tokens: {rows} rows")
+    positions = torch.empty(rows, dtype=_I64, device=context_lens.device)
+    slots, seqs, cu, lens, used = context_lens.new_empty(2 * rows + 2 * B + 2).split_with_sizes((rows, rows, B + 1, B, 1))
+    _launch("ssdk_place_tokens", gpu, context_lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(), free_blocks.data_ptr(), free_used.data_ptr(),
+            positions.data_ptr(), slots.data_ptr(), seqs.data_ptr(), cu.data_ptr(), lens.data_ptr(), used.data_ptr(), B, width, F, rows, block_size, num_blocks)
     return positions, slots, seqs, cu, lens, used
 
 
@@ -239,21 +246,21 @@ def rope_axes_store_kv(qkv: torch.Tensor, positions: torch.Tensor, axis_of, slot
     [0] * 16 + [1] * 24 + [2] * 24); rope_table fp32 [max_pos, rot_dim] cos | sin: the first rot_dim channels of a head turn.
     Norms and rotation in fp32 with one rounding.  Returns q [M, heads * head_dim]; keys and values are in their slots.  A row with a position
     outside the table has NaN queries and stores nothing; slots are distinct, those outside the cache store nothing."""
-    M, rot = qkv.shape[0], rope_table.shape[-1]
-    cache = (k_cache.shape[0], k_cache.shape[1], kv_heads, head_dim) if k_cache.dim() == 4 else (-1, -1, kv_heads, head_dim)
-    args = [(qkv, "qkv", _BF, (M, (heads + 2 * kv_heads) * head_dim)), (positions, "positions", _I64, (-1, M)), (slot_mapping, "slot_mapping", _I32, (M,)),
-            (rope_table, "rope_table", _F32, (-1, rot)), (k_cache, "k_cache", _BF, cache), (v_cache, "v_cache", _BF, cache)]
-    for w, what in ((q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w")):
-        if w is not None:
-            args.append((w, what, _BF, (head_dim,)))
+    M, rot, axes = qkv.shape[0], rope_table.shape[-1], positions.shape[0]
+    cache = torch.Size((*k_cache.shape[:2], kv_heads, head_dim))
     axis_of = bytes(axis_of)
     if len(axis_of) * 2 != rot:
         raise ValueError(f"rope_axes_store_kv: axis_of has {len(axis_of)} frequencies, rope_table {rot / 2}")
-    dev = _check("rope_axes_store_kv", *args)
-    q = torch.empty(M, heads * head_dim, dtype=_BF, device=dev)
-    _launch("ssdk_rope_axes_store_kv", dev, qkv.data_ptr(), positions.data_ptr(), positions.shape[0], axis_of, slot_mapping.data_ptr(), rope_table.data_ptr(),
+    args = [(qkv, "qkv", _BF, (M, (heads + 2 * kv_heads) * head_dim)), (positions, "positions", _I64, (axes, M)), (slot_mapping, "slot_mapping", _I32, (M,)),
+            (rope_table, "rope_table", _F32, (rope_table.shape[0], rot)), (k_cache, "k_cache", _BF, cache), (v_cache, "v_cache", _BF, cache)]
+    for w, what in ((q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w")):
+        if w is not None:
+            args.append((w, what, _BF, (head_dim,)))
+    gpu = _check("rope_axes_store_kv", *args)
+    q = qkv.new_empty(M, heads * head_dim)
+    _launch("ssdk_rope_axes_store_kv", gpu, qkv.data_ptr(), positions.data_ptr(), axes, axis_of, slot_mapping.data_ptr(), rope_table.data_ptr(),
             rope_table.shape[0], rot, _ptr(q_norm_w), _ptr(k_norm_w), norm_eps, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            k_cache.shape[0] * k_cache.shape[1], M, heads, kv_heads, head_dim)
+            cache[0] * cache[1], M, heads, kv_heads, head_dim)
     return q
 
 
@@ -265,13 +272,13 @@ def span_bounds(bounds: torch.Tensor, k_cache: torch.Tensor, block_tables: torch
     [num_blocks, block_size, KV, hd]; context_lens int32 [B] with the new tokens.  Returns bounds."""
     n, block_size, KV, hd = k_cache.shape if k_cache.dim() == 4 else (-1,) * 4
     subs = bounds.shape[1] if bounds.dim() == 5 else -1
-    B = context_lens.shape[0]
+    B, width = _last(context_lens, 1), _last(block_tables, 2)
     if subs == 0 or block_size % subs:
         raise ValueError(f"span_bounds: pages of {block_size} tokens in {subs} spans")
-    dev = _check("span_bounds", (bounds, "bounds", _BF, (n, subs, KV, 2, hd)), (k_cache, "k_cache", _BF, (n, block_size, KV, hd)),
-                 (block_tables, "block_tables", _I32, (B, -1)), (context_lens, "context_lens", _I32, (B,)))
-    _launch("ssdk_span_bounds", dev, k_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), bounds.data_ptr(), B, new_tokens, KV, hd,
-            block_size, block_tables.shape[1], n, block_size // subs)
+    gpu = _check("span_bounds", (bounds, "bounds", _BF, (n, subs, KV, 2, hd)), (k_cache, "k_cache", _BF, (n, block_size, KV, hd)),
+                 (block_tables, "block_tables", _I32, (B, width)), (context_lens, "context_lens", _I32, (B,)))
+    _launch("ssdk_span_bounds", gpu, k_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), bounds.data_ptr(), B, new_tokens, KV, hd,
+            block_size, width, n, block_size // subs)
     return bounds
 
 
@@ -283,19 +290,19 @@ def select_spans(q: torch.Tensor, bounds: torch.Tensor, block_tables: torch.Tens
 
     q [B * q_len, H, hd] bf16 (rotated); bounds as span_bounds keeps them.  Returns int32 [B, KV, count], ascending, -1 behind the
     last: what span_attention takes.  The rows of a sequence share their spans."""
-    n, subs, KV, two, hd = bounds.shape if bounds.dim() == 5 else (-1,) * 5
-    B = context_lens.shape[0]
+    n, subs, KV, _, hd = bounds.shape if bounds.dim() == 5 else (-1,) * 5
+    B, width, H = _last(context_lens, 1), _last(block_tables, 2), q.shape[1]
     if subs == 0 or block_size % subs:
         raise ValueError(f"select_spans: pages of {block_size} tokens in {subs} spans")
-    dev = _check("select_spans", (q, "q", _BF, (B * q_len, -1, hd)), (bounds, "bounds", _BF, (n, subs, KV, 2, hd)),
-                 (block_tables, "block_tables", _I32, (B, -1)), (context_lens, "context_lens", _I32, (B,)))
+    gpu = _check("select_spans", (q, "q", _BF, (B * q_len, H, hd)), (bounds, "bounds", _BF, (n, subs, KV, 2, hd)),
+                 (block_tables, "block_tables", _I32, (B, width)), (context_lens, "context_lens", _I32, (B,)))
     span = block_size // subs
     if last is None:
         last = min((q_len + span - 2) // span + 1, count - first)
-    out = torch.empty(B, KV, max(count, 0), dtype=_I32, device=dev)
-    scratch = torch.empty(_L.load().ssdk_select_spans_scratch_bytes(B, KV, block_size, block_tables.shape[1], span), dtype=torch.uint8, device=dev)
-    _launch("ssdk_select_spans", dev, q.data_ptr(), bounds.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(),
-            scratch.data_ptr(), B, q_len, q.shape[1], KV, hd, block_size, block_tables.shape[1], n, span, count, first, last)
+    out = context_lens.new_empty(B, KV, max(count, 0))
+    scratch = q.new_empty(_L.load().ssdk_select_spans_scratch_bytes(B, KV, block_size, width, span) // 2)
+    _launch("ssdk_select_spans", gpu, q.data_ptr(), bounds.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(),
+            scratch.data_ptr(), B, q_len, H, KV, hd, block_size, width, n, span, count, first, last)
     return out
 
 
@@ -305,12 +312,11 @@ def span_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 
     q [B * q_len, H, hd]; returns [B * q_len, H * hd].  Entries outside the context are passed over, a span listed twice counts twice, a row
     that sees no key is zero."""
-    n, block_size, KV, hd = k_cache.shape if k_cache.dim() == 4 else (-1,) * 4
-    B = context_lens.shape[0]
-    dev = _check("span_attention", (q, "q", _BF, (B * q_len, -1, hd)), (k_cache, "k_cache", _BF, (n, block_size, KV, hd)),
-                 (v_cache, "v_cache", _BF, (n, block_size, KV, hd)), (block_tables, "block_tables", _I32, (B, -1)),
-                 (context_lens, "context_lens", _I32, (B,)), (spans, "spans", _I32, (B, KV, -1)))
-    out = torch.empty(q.shape[0], q.shape[1] * hd, dtype=_BF, device=dev)
-    _launch("ssdk_span_attn", dev, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), spans.data_ptr(),
-            out.data_ptr(), B, q_len, q.shape[1], KV, hd, block_size, block_tables.shape[1], n, span, spans.shape[2], scale)
+    n, block_size, KV, hd = cache = k_cache.shape if k_cache.dim() == 4 else (-1,) * 4
+    B, width, H, count = _last(context_lens, 1), _last(block_tables, 2), q.shape[1], _last(spans, 3)
+    gpu = _check("span_attention", (q, "q", _BF, (B * q_len, H, hd)), (k_cache, "k_cache", _BF, cache), (v_cache, "v_cache", _BF, cache),
+                 (block_tables, "block_tables", _I32, (B, width)), (context_lens, "context_lens", _I32, (B,)), (spans, "spans", _I32, (B, KV, count)))
+    out = q.new_empty(B * q_len, H * hd)
+    _launch("ssdk_span_attn", gpu, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), spans.data_ptr(),
+            out.data_ptr(), B, q_len, H, KV, hd, block_size, width, n, span, count, scale)
     return out
