@@ -38,7 +38,7 @@ struct SelectParams {
 constexpr int kEstimateThreads = 256;
 constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 32;
 constexpr int kMaxSpans = 24576;   // of a sequence
-constexpr int kPickBins = 2048;
+constexpr int kPickBins = 1024;    // a multiple of kPickThreads
 constexpr int kPickRanked = 256;   // spans between, up to which each is compared with each
 // rows of the query | scores (64 bits; before them the estimates) | taken | between (a bit per span) | bins, then the spans between
 constexpr int64_t pick_smem(int spans, int64_t rows, int HD) { return (rows + 7) / 8 * 8 * HD * 2 + spans * 8 + 2 * ((spans + 31) / 32) * 4 + kPickBins * 4; }
@@ -51,7 +51,7 @@ SSDK_DEVINL unsigned long long score_key(double s) {
   return b < 0 ? ~(unsigned long long)b : (unsigned long long)b | (1ull << 63);
 }
 
-// the sum of v over the block's threads up to this one, and over all
+// the sum of v over the block's threads up to this one, and over all.  words: not those of the call before
 SSDK_DEVINL int pick_running_sum(int v, int* words, int* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -59,43 +59,29 @@ SSDK_DEVINL int pick_running_sum(int v, int* words, int* total) {
     const int u = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += u;
   }
-  __syncthreads();
   if (lane == 31) words[warp] = v;
   __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kPickWarps; ++w) {
-    const int x = words[w];
-    before += w < warp ? x : 0;
-    all += x;
-  }
-  *total = all;
-  return before + v;
-}
-SSDK_DEVINL int pick_total(int v, int* words) {
-  v = __reduce_add_sync(0xffffffffu, v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = v;
-  __syncthreads();
-  int all = 0;
-#pragma unroll
-  for (int w = 0; w < kPickWarps; ++w) all += words[w];
-  return all;
+  const int x = lane < kPickWarps ? words[lane] : 0;
+  *total = __reduce_add_sync(0xffffffffu, x);
+  return v + __reduce_add_sync(0xffffffffu, lane < warp ? x : 0);
 }
 
 // the spans of a bit map, ascending, then -1
 SSDK_DEVINL void pick_write(const uint32_t* bits, int words, int32_t* out, int count, int* sums) {
-  int done = 0;
-  for (int base = 0; base < words; base += kPickThreads) {
+  int done = 0, turn = 0;
+  for (int base = 0; base < words; base += kPickThreads, turn ^= 1) {
     const int w = base + threadIdx.x;
     uint32_t m = w < words ? bits[w] : 0;
-    int all, at = pick_running_sum(__popc(m), sums, &all);
+    int all, at = pick_running_sum(__popc(m), sums + turn * kPickWarps, &all);
     at += done - __popc(m);
     for (; m; m &= m - 1) out[at++] = w * 32 + __ffs(m) - 1;
     done += all;
   }
   for (int i = done + threadIdx.x; i < count; i += kPickThreads) out[i] = -1;
 }
+// floats in their order as unsigned words, and back
+SSDK_DEVINL uint32_t order_of(uint32_t f) { return f >> 31 ? ~f : f | 0x80000000u; }
+SSDK_DEVINL float of_order(uint32_t o) { return __uint_as_float(o >> 31 ? o & 0x7fffffffu : ~o); }
 
 // a warp: the score of one span in 64 bits.  q: the rows [tiles * 8][HD], those behind the last one zero.  A lane has HD / 32 channels of eight rows at a time;
 // their sums halve their number with every exchange.  FINITE: lo <= hi and no product is NaN, so that the sign of q says which bound counts.
@@ -239,9 +225,9 @@ __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(Sele
 template <int HD>
 __global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams p) {
   extern __shared__ __align__(16) uint8_t pick_smem_bytes[];
-  __shared__ int sums[kPickWarps], pick_bin;
-  __shared__ uint32_t widest, q_most;      // bits of the largest |lo|, |hi|, and of the largest sum of |q| over a row
-  __shared__ float low[kPickWarps], high[kPickWarps];
+  __shared__ int sums[4 * kPickWarps], pick_bin, n_sure, n_open;
+  __shared__ int4 stats[kPickWarps];
+  __shared__ uint32_t wides[kPickWarps], q_most;   // bits of the largest |lo|, |hi| of a warp's share, and of the largest sum of |q| over a row
   const int G = p.heads / p.kv_heads, rows = G * p.Q, padded = (rows + 7) / 8 * 8;
   const int words = (p.max_spans + 31) / 32;
   __nv_bfloat16* q_rows = reinterpret_cast<__nv_bfloat16*>(pick_smem_bytes);   // [padded][HD]
@@ -265,7 +251,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams
     pick_write(taken, (n + 31) / 32, out, p.count, sums);
     return;
   }
-  if (threadIdx.x == 0) widest = q_most = 0;
+  if (threadIdx.x == 0) q_most = n_sure = n_open = 0;
   for (int i = threadIdx.x; i < kPickBins; i += kPickThreads) bins[i] = 0;
   __syncthreads();
   for (int base = warp * 32; base < padded * (HD / 8); base += kPickThreads) {   // (whole warps) the query's rows: 8 channels a thread
@@ -284,12 +270,9 @@ __global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams
   pdl_wait();   // the estimates are there
 
   auto kept = [&](int s) { return s < p.first || s >= n - p.last; };
-  for (int i = threadIdx.x; i < p.warps; i += kPickThreads) {
-    const uint32_t w = __ldcg(p.wide + ((size_t)b * p.kv_heads + head) * p.warps + i);
-    if (w) atomicMax(&widest, w);
-  }
   int always = 0, others = 0;
-  float lo = INFINITY, hi = -INFINITY;
+  uint32_t lowest = ~0u, highest = 0, wide = 0;
+  for (int i = threadIdx.x; i < p.warps; i += kPickThreads) wide = max(wide, __ldcg(p.wide + ((size_t)b * p.kv_heads + head) * p.warps + i));
   for (int s = threadIdx.x; s < n; s += kPickThreads) {
     const uint32_t e = __ldcg(p.estimates + ((size_t)b * p.kv_heads + head) * p.max_spans + s);
     estimate[s] = e;
@@ -298,40 +281,42 @@ __global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams
       ++always;
     } else {
       ++others;
-      lo = fminf(lo, __uint_as_float(e));
-      hi = fmaxf(hi, __uint_as_float(e));
+      lowest = min(lowest, order_of(e));
+      highest = max(highest, order_of(e));
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
+  always = __reduce_add_sync(0xffffffffu, always);
+  others = __reduce_add_sync(0xffffffffu, others);
+  lowest = __reduce_min_sync(0xffffffffu, lowest);
+  highest = __reduce_max_sync(0xffffffffu, highest);
+  wide = __reduce_max_sync(0xffffffffu, wide);
   if (lane == 0) {
-    low[warp] = lo;
-    high[warp] = hi;
+    stats[warp] = make_int4(always, others, (int)lowest, (int)highest);
+    wides[warp] = wide;
   }
-  always = pick_total(always, sums);
-  others = pick_total(others, sums);
-#pragma unroll
-  for (int w = 0; w < kPickWarps; ++w) {
-    lo = fminf(lo, low[w]);
-    hi = fmaxf(hi, high[w]);
+  __syncthreads();
+  {
+    const int4 x = stats[lane % kPickWarps];
+    always = __reduce_add_sync(0xffffffffu, lane < kPickWarps ? x.x : 0);
+    others = __reduce_add_sync(0xffffffffu, lane < kPickWarps ? x.y : 0);
+    lowest = __reduce_min_sync(0xffffffffu, (uint32_t)x.z);
+    highest = __reduce_max_sync(0xffffffffu, (uint32_t)x.w);
+    wide = __reduce_max_sync(0xffffffffu, wides[lane % kPickWarps]);
   }
-  const float size = __uint_as_float(q_most) * __uint_as_float(widest);
+  const float lo = of_order(lowest), hi = of_order(highest), size = __uint_as_float(q_most) * __uint_as_float(wide);
   const int want = min(p.count - always, others);   // beside those that are kept
   const bool all = want == others, none = want == 0;
   const bool finite = size < 1e38f;
   const float eps2 = size * 0x1p-13f + 0x1p-100f, scale = hi - lo > 1e-30f ? (float)(kPickBins - 1) / (hi - lo) : 0.f;
   auto bin_of = [&](float x) { return (int)fminf(fmaxf((x - lo) * scale, -1.f), (float)(kPickBins - 1)); };   // (rises with x)
+  int line = 0;   // the bin of the want-th largest
   if (!all && !none && finite) {
     for (int s = threadIdx.x; s < n; s += kPickThreads) {
       const uint32_t e = estimate[s];
       if (e != kNoSpan && !kept(s)) atomicAdd(&bins[bin_of(__uint_as_float(e))], 1);
     }
     __syncthreads();
-    // the bin of the want-th largest: from the top, each thread some bins
-    constexpr int PER = kPickBins / kPickThreads;
+    constexpr int PER = kPickBins / kPickThreads;   // from the top, each thread some bins
     int mine = 0, total;
 #pragma unroll
     for (int i = 0; i < PER; ++i) mine += bins[kPickBins - 1 - (int)threadIdx.x * PER - i];
@@ -345,9 +330,9 @@ __global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams
       pick_bin = i;
     }
     __syncthreads();
+    line = pick_bin;
   }
-  const int line = pick_bin;
-  int sure = 0, open = 0;
+  int* list = bins;   // (the bins have been read) the spans between, in any order, as far as they are compared with one another
   for (int base = warp * 32; base < n; base += kPickThreads) {
     const int s = base + lane;
     const uint32_t e = s < n ? estimate[s] : kNoSpan;
@@ -358,37 +343,27 @@ __global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams
       in = bin_of(x - eps2) > line;
       maybe = !in && bin_of(x + eps2) >= line;
     }
-    const uint32_t m_in = __ballot_sync(0xffffffffu, in), m_open = __ballot_sync(0xffffffffu, maybe);
+    const uint32_t m_in = __ballot_sync(0xffffffffu, in), m_open = __ballot_sync(0xffffffffu, maybe), m_sure = __ballot_sync(0xffffffffu, in && !keep);
+    int at = 0;
     if (lane == 0) {
       taken[base / 32] = m_in;
       between[base / 32] = m_open;
+      if (m_sure) atomicAdd(&n_sure, __popc(m_sure));
+      if (m_open) at = atomicAdd(&n_open, __popc(m_open));
     }
-    sure += in && !keep;
-    open += maybe;
+    at = __shfl_sync(0xffffffffu, at, 0) + __popc(m_open & ((1u << lane) - 1));
+    if (maybe && at < kPickRanked) list[at] = s;
   }
-  sure = pick_total(sure, sums);
-  open = pick_total(open, sums);
-  const int left = want - sure, n_words = (n + 31) / 32;   // so many of the `open` ones (0 where all or none are taken)
+  __syncthreads();
+  const int open = n_open, left = want - n_sure, n_words = (n + 31) / 32;   // so many of the `open` ones are wanted (0 where all or none are)
 
-  if (!all && left > 0 && left == open) {
+  if (left > 0 && left == open) {
     for (int w = threadIdx.x; w < n_words; w += kPickThreads) taken[w] |= between[w];
-  } else if (!all && left > 0) {
-    // ---- scores in 64 bits ----
-    const bool listed = open <= kPickBins;
-    if (listed) {   // the spans between, ascending
-      int done = 0;
-      for (int base = 0; base < n_words; base += kPickThreads) {
-        const int w = base + threadIdx.x;
-        uint32_t m = w < n_words ? between[w] : 0;
-        int count, at = pick_running_sum(__popc(m), sums, &count);
-        at += done - __popc(m);
-        for (; m; m &= m - 1) bins[at++] = w * 32 + __ffs(m) - 1;
-        done += count;
-      }
-      __syncthreads();
-    }
+  } else if (left > 0) {
+    // ---- scores in 64 bits, over the estimates ----
+    const bool listed = open <= kPickRanked;
     const int m = listed ? open : n;
-    auto span_of = [&](int i) { return listed ? bins[i] : ((between[i >> 5] >> (i & 31)) & 1 ? i : -1); };
+    auto span_of = [&](int i) { return listed ? list[i] : ((between[i >> 5] >> (i & 31)) & 1 ? i : -1); };
     for (int i = warp; i < m; i += kPickWarps) {
       const int s = span_of(i);
       if (s < 0) continue;
@@ -397,36 +372,44 @@ __global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams
       if (lane == 0) keys[i] = key;
     }
     __syncthreads();
-    if (open <= kPickRanked) {
+    if (listed) {
       for (int i = threadIdx.x; i < m; i += kPickThreads) {
         const unsigned long long key = keys[i];
+        const int s = list[i];
         int before = 0;
-        for (int j = 0; j < m; ++j) before += keys[j] > key || (keys[j] == key && j < i);
-        if (before < left) atomicOr(&taken[bins[i] >> 5], 1u << (bins[i] & 31));
+        for (int j = 0; j < m; ++j) before += keys[j] > key || (keys[j] == key && list[j] < s);
+        if (before < left) atomicOr(&taken[s >> 5], 1u << (s & 31));
       }
     } else {   // the left-th largest score bit by bit, then as many of those on it as there is room for, in their order
+      auto total = [&](int v) {
+        v = __reduce_add_sync(0xffffffffu, v);
+        __syncthreads();
+        if (lane == 0) sums[warp] = v;
+        __syncthreads();
+        return __reduce_add_sync(0xffffffffu, lane < kPickWarps ? sums[lane] : 0);
+      };
       unsigned long long score = 0;
       for (int bit = 63; bit >= 0; --bit) {
         const unsigned long long tried = score | (1ull << bit);
         int c = 0;
         for (int i = threadIdx.x; i < m; i += kPickThreads) c += span_of(i) >= 0 && keys[i] >= tried;
-        if (pick_total(c, sums) >= left) score = tried;
+        if (total(c) >= left) score = tried;
       }
       int above = 0;
       for (int i = threadIdx.x; i < m; i += kPickThreads) above += span_of(i) >= 0 && keys[i] > score;
-      int room = left - pick_total(above, sums);
-      for (int base = 0; base < m; base += kPickThreads) {
+      int room = left - total(above);
+      for (int base = 0, turn = 1; base < m; base += kPickThreads, turn ^= 1) {
         const int i = base + threadIdx.x, s = i < m ? span_of(i) : -1;
         const bool over = s >= 0 && keys[i] > score, on = s >= 0 && keys[i] == score;
-        int total;
-        const int at = pick_running_sum(on, sums, &total) - on;
+        int equal;
+        const int at = pick_running_sum(on, sums + turn * kPickWarps, &equal) - on;
         if (over || (on && at < room)) atomicOr(&taken[s >> 5], 1u << (s & 31));
-        room -= total;
+        room -= equal;
       }
     }
   }
   __syncthreads();
-  pick_write(taken, n_words, out, p.count, sums);
+  pick_write(taken, n_words, out, p.count, sums + 2 * kPickWarps);
 }
 
 // ----------------------------------------------------------------------------------
