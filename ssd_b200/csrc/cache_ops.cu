@@ -178,11 +178,13 @@ int ssdk_span_bounds(const void* k_cache, const int32_t* block_tables, const int
   p.fresh = (int)std::min<int64_t>(new_tokens, (int64_t)max_blocks_per_seq * block_size);
   const int cols = kv_heads * head_dim / 8;
   p.width = cols >= 32 ? 32 : cols >= 16 ? 16 : 8;
-  const int64_t blocks = (((int64_t)p.fresh + span - 2) / span + 1) * ((cols + p.width - 1) / p.width);
-  if (blocks >= (1ll << 31)) return fail("span_bounds: %d new tokens of %d heads", new_tokens, kv_heads);
+  const int64_t units = (((int64_t)p.fresh + span - 2) / span + 1) * ((cols + p.width - 1) / p.width);
+  if (units >= (1ll << 31) - 8) return fail("span_bounds: %d new tokens of %d heads", new_tokens, kv_heads);
   Launcher L;
   L.st = (cudaStream_t)stream;
-  return L.go(span_bounds_kernel, dim3((unsigned)blocks, batch), dim3(kBoundsThreads), 0, p);
+  // a block to a span's columns while the blocks fit the SMs at once, else a warp
+  if (units * batch <= 8 * kSms) return L.go(span_bounds_kernel<true>, dim3((unsigned)units, batch), dim3(kBoundsThreads), 0, p);
+  return L.go(span_bounds_kernel<false>, dim3((unsigned)((units + kBoundsThreads / 32 - 1) / (kBoundsThreads / 32)), batch), dim3(kBoundsThreads), 0, p);
 }
 
 int64_t ssdk_select_spans_scratch_bytes(int batch, int kv_heads, int block_size, int max_blocks_per_seq, int span) {

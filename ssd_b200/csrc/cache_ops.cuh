@@ -309,9 +309,9 @@ __global__ void __launch_bounds__(kRopeAxesThreads, 4) rope_axes_kernel(RopeAxes
 // span_bounds_kernel: lo[d] = min, hi[d] = max of channel d over the keys of a span that are in the context, for every span that holds one of the last
 // `fresh` tokens of its sequence.  Read anew from the cache rather than kept up: a rejected draft token leaves no trace, a page that changes hands needs no
 // reset, and a span named by two tables gets the same values twice.  min and max are exact in any order; a NaN key makes its channel NaN.
-// Bound by memory: a span's keys once.  A block takes 32 columns of 8 channels (16 bytes) of a span, a warp beside another token after token, and the warps'
-// parts meet in shared memory: all loads of a short span are in flight together.  (With all columns in one block a thread walked half of the span's tokens:
-// 64 spans of 32 tokens 8.3 us, 64000 tokens 37.)
+// Bound by memory: a span's keys once.  A thread owns a column of 8 channels (16 bytes).  Few spans: a block takes 32 columns of one, its warps beside one
+// another token after token, and they meet in shared memory, so that all loads are in flight together (64 x 7 new rows 5.3 us; 8.2 with a span's tokens in
+// two lanes).  Many: a warp takes 32 columns of a span alone, eight tokens at a time (four prompts of 16001 XX us; 35 the other way, bound by its instructions).
 // ----------------------------------------------------------------------------------
 struct SpanBoundsParams {
   const __nv_bfloat16* k_cache;  // [num_blocks, block_size, KV, hd]
@@ -340,43 +340,62 @@ SSDK_DEVINL uint32_t max_bf16x2(uint32_t a, uint32_t b) {
 SSDK_DEVINL uint4 min_bf16x8(const uint4& a, const uint4& b) { return make_uint4(min_bf16x2(a.x, b.x), min_bf16x2(a.y, b.y), min_bf16x2(a.z, b.z), min_bf16x2(a.w, b.w)); }
 SSDK_DEVINL uint4 max_bf16x8(const uint4& a, const uint4& b) { return make_uint4(max_bf16x2(a.x, b.x), max_bf16x2(a.y, b.y), max_bf16x2(a.z, b.z), max_bf16x2(a.w, b.w)); }
 
-__global__ void __launch_bounds__(kBoundsThreads) span_bounds_kernel(SpanBoundsParams p) {
-  SSDK_STATIC_SMEM(uint4, meet, 2 * kBoundsThreads);
+SSDK_DEVINL uint4 shfl_xor_16(const uint4& v, int o) {
+  return make_uint4(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o), __shfl_xor_sync(0xffffffffu, v.z, o), __shfl_xor_sync(0xffffffffu, v.w, o));
+}
+
+template <bool SPLIT>
+__global__ void __launch_bounds__(kBoundsThreads, 4) span_bounds_kernel(SpanBoundsParams p) {
+  constexpr int WARPS = kBoundsThreads / 32;
   const int b = blockIdx.y;
   const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size);
-  const int slices = (p.kv_heads * p.head_dim / 8 + p.width - 1) / p.width, nth = (int)blockIdx.x / slices;
-  const int pos0 = (max(len - p.fresh, 0) / p.span + nth) * p.span;   // (below len + span, which the host holds under 2^31)
+  const int row = p.kv_heads * p.head_dim, slices = (row / 8 + p.width - 1) / p.width;   // columns of a warp: p.width
+  const int nth = SPLIT ? (int)blockIdx.x : (int)blockIdx.x * WARPS + (int)(threadIdx.x >> 5), span = nth / slices;
+  const int pos0 = (max(len - p.fresh, 0) / p.span + span) * p.span;   // (below len + span, which the host holds under 2^31)
   if (pos0 >= len) return;
   const int page = page_at(p.tables + (size_t)b * p.max_blocks + pos0 / p.block_size, p.num_blocks);
   if (page < 0) return;
   const int off = pos0 % p.block_size, tokens = min(p.span, len - pos0);
-  const int row = p.kv_heads * p.head_dim;
-  const int col = ((int)blockIdx.x - nth * slices) * p.width + (int)threadIdx.x % p.width;   // of 8 channels
-  const int lane = threadIdx.x / p.width, lanes = kBoundsThreads / p.width;                  // tokens beside one another
-  const bool works = col * 8 < row && lane < tokens;
-  uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-  if (works) {
-    const __nv_bfloat16* keys = p.k_cache + ((size_t)page * p.block_size + off) * row + col * 8;
-    lo = hi = ld_nc_v4(keys + (size_t)lane * row);
-#pragma unroll 7
-    for (int t = lane + lanes; t < tokens; t += lanes) {
-      const uint4 v = ld_nc_v4(keys + (size_t)t * row);
-      lo = min_bf16x8(lo, v);
-      hi = max_bf16x8(hi, v);
+  const int who = SPLIT ? (int)threadIdx.x : (int)threadIdx.x % 32;
+  const int col = (nth - span * slices) * p.width + who % p.width;                       // of 8 channels
+  const int lane = who / p.width, lanes = (SPLIT ? kBoundsThreads : 32) / p.width;       // tokens beside one another
+  const bool there = col * 8 < row;
+  uint4 lo = make_uint4(0x7f807f80u, 0x7f807f80u, 0x7f807f80u, 0x7f807f80u), hi = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);   // +- infinity
+  const __nv_bfloat16* keys = p.k_cache + ((size_t)page * p.block_size + off) * row + col * 8;
+  constexpr int AHEAD = SPLIT ? 4 : 8;
+  for (int t = lane; t < tokens; t += AHEAD * lanes) {
+    uint4 v[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (there && t + j * lanes < tokens) v[j] = ld_nc_v4(keys + (size_t)(t + j * lanes) * row);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (there && t + j * lanes < tokens) {
+        lo = min_bf16x8(lo, v[j]);
+        hi = max_bf16x8(hi, v[j]);
+      }
+  }
+  const int head = col * 8 / p.head_dim;
+  __nv_bfloat16* out = p.bounds + ((size_t)page * (p.block_size / p.span) + off / p.span) * 2 * row + (size_t)head * 2 * p.head_dim + (col * 8 - head * p.head_dim);
+  if (SPLIT) {
+    SSDK_STATIC_SMEM(uint4, meet, 2 * kBoundsThreads);
+    meet[threadIdx.x] = lo;
+    meet[kBoundsThreads + threadIdx.x] = hi;
+    __syncthreads();
+    if (lane > 1 || !there) return;   // the first lane joins the smallest values, the second the largest
+    const uint4* part = meet + lane * kBoundsThreads + threadIdx.x % p.width;
+    uint4 v = part[0];
+    for (int l = 1; l < lanes; ++l) v = lane ? max_bf16x8(v, part[l * p.width]) : min_bf16x8(v, part[l * p.width]);
+    *reinterpret_cast<uint4*>(out + lane * p.head_dim) = v;
+  } else {
+    for (int o = p.width; o < 32; o <<= 1) {
+      lo = min_bf16x8(lo, shfl_xor_16(lo, o));
+      hi = max_bf16x8(hi, shfl_xor_16(hi, o));
     }
+    if (lane > 0 || !there) return;
+    *reinterpret_cast<uint4*>(out) = lo;
+    *reinterpret_cast<uint4*>(out + p.head_dim) = hi;
   }
-  meet[threadIdx.x] = lo;
-  meet[kBoundsThreads + threadIdx.x] = hi;
-  __syncthreads();
-  if (lane > 1 || col * 8 >= row) return;   // the first lane joins the smallest values, the second the largest
-  const uint4* part = meet + lane * kBoundsThreads + threadIdx.x % p.width;
-  uint4 v = part[0];
-  for (int l = 1; l < min(lanes, tokens); ++l) {
-    const uint4 w = part[l * p.width];
-    v = lane ? max_bf16x8(v, w) : min_bf16x8(v, w);
-  }
-  __nv_bfloat16* out = p.bounds + ((size_t)page * (p.block_size / p.span) + off / p.span) * 2 * row + (size_t)(col * 8 / p.head_dim) * 2 * p.head_dim;
-  *reinterpret_cast<uint4*>(out + lane * p.head_dim + col * 8 % p.head_dim) = v;
 }
 
 }  // namespace ssdk

@@ -117,7 +117,7 @@ int main(int argc, char** argv) {
     return 0;
   }
   if (mode == "bounds") {
-    auto h = rd<int32_t>(f, 8);   // B max_blocks num_blocks block_size span KV hd fresh
+    auto h = rd<int32_t>(f, 9);   // B max_blocks num_blocks block_size span KV hd fresh split
     ssdk::SpanBoundsParams p;
     p.B = h.p[0]; p.max_blocks = h.p[1]; p.num_blocks = h.p[2]; p.block_size = h.p[3]; p.span = h.p[4]; p.kv_heads = h.p[5]; p.head_dim = h.p[6]; p.fresh = h.p[7];
     auto tables = rd<int32_t>(f, (size_t)p.B * p.max_blocks), lens = rd<int32_t>(f, p.B);
@@ -127,9 +127,11 @@ int main(int argc, char** argv) {
     dim3 grid;
     const int cols = p.kv_heads * p.head_dim / 8;
     p.width = cols >= 32 ? 32 : cols >= 16 ? 16 : 8;
-    grid.x = (unsigned)(((p.fresh + p.span - 2) / p.span + 1) * ((cols + p.width - 1) / p.width));
+    const int units = ((p.fresh + p.span - 2) / p.span + 1) * ((cols + p.width - 1) / p.width);
+    grid.x = (unsigned)(h.p[8] ? units : (units + 7) / 8);
     grid.y = (unsigned)p.B;
-    emu::launch(+[](ssdk::SpanBoundsParams q) { ssdk::span_bounds_kernel(q); }, p, grid, ssdk::kBoundsThreads, 0, 4);
+    if (h.p[8]) emu::launch(+[](ssdk::SpanBoundsParams q) { ssdk::span_bounds_kernel<true>(q); }, p, grid, ssdk::kBoundsThreads, 0, 4);
+    else emu::launch(+[](ssdk::SpanBoundsParams q) { ssdk::span_bounds_kernel<false>(q); }, p, grid, ssdk::kBoundsThreads, 0, 4);
     wr(o, bounds);
     return 0;
   }

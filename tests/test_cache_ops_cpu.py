@@ -99,14 +99,15 @@ def test_rope_axes_source(tmp_path, H, KV, hd, rot, axes, norm, shares):
 
 @needs_gxx
 @pytest.mark.parametrize("KV,hd,S,span,new,lens", [(1, 64, 32, 16, 3, [1, 0, 40, 64]), (5, 128, 16, 16, 40, [33, 16]), (2, 64, 64, 32, 1, [64, 65, -3, 1000]), (20, 128, 16, 16, 1, [16])])
-def test_span_bounds_source(tmp_path, KV, hd, S, span, new, lens):
+@pytest.mark.parametrize("split", [0, 1])
+def test_span_bounds_source(tmp_path, KV, hd, S, span, new, lens, split):
     g = gen(KV, S, span, new)
     table, total = tables(g, [min(max(n, 0), 3 * S) for n in lens], S, width=3)
     table[0, 0] = total if len(lens) > 2 else table[0, 0]   # outside the cache
     keys = torch.randn(total, S, KV, hd, generator=g).to(BF)
     keys[:, 1::7] = float("nan")
     old = torch.full((total, S // span, KV, 2, hd), 5.0, dtype=BF)
-    data = _run("bounds", [i32([len(lens), 3, total, S, span, KV, hd, new]), table, i32(lens), keys, old], tmp_path)
+    data = _run("bounds", [i32([len(lens), 3, total, S, span, KV, hd, new, split]), table, i32(lens), keys, old], tmp_path)
     got, = _take(data, (BF, tuple(old.shape)))
     want = plain.bounds(old, keys, table, lens, new)
     assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.nan_to_num(got.float()), torch.nan_to_num(want.float()))
