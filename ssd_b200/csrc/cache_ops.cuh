@@ -310,8 +310,8 @@ __global__ void __launch_bounds__(kRopeAxesThreads, 4) rope_axes_kernel(RopeAxes
 // `fresh` tokens of its sequence.  Read anew from the cache rather than kept up: a rejected draft token leaves no trace, a page that changes hands needs no
 // reset, and a span named by two tables gets the same values twice.  min and max are exact in any order; a NaN key makes its channel NaN.
 // Bound by memory: a span's keys once.  A thread owns a column of 8 channels (16 bytes).  Few spans: a block takes 32 columns of one, its warps beside one
-// another token after token, and they meet in shared memory, so that all loads are in flight together (64 x 7 new rows 5.3 us; 8.2 with a span's tokens in
-// two lanes).  Many: a warp takes 32 columns of a span alone, eight tokens at a time (four prompts of 16001 XX us; 35 the other way, bound by its instructions).
+// another token after token, and they meet in shared memory, so that all loads are in flight together (64 x 7 new rows 4.5 us; 8.2 with a span's tokens in
+// two lanes).  Many: a warp takes 32 columns of a span alone, eight tokens at a time (four prompts of 16001 24 us; 35 the other way, bound by its instructions).
 // ----------------------------------------------------------------------------------
 struct SpanBoundsParams {
   const __nv_bfloat16* k_cache;  // [num_blocks, block_size, KV, hd]
