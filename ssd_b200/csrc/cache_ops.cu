@@ -70,7 +70,7 @@ static int launch_span_attn(Launcher& L, const SpanAttnParams& p) {
 template <int HD>
 static int launch_span_tiles(Launcher& L, SpanAttnParams p) {
   static std::atomic<bool> done[64];
-  CKI(with_smem(span_tile_kernel<HD>, span_tile_smem(HD, kMaxListed), done));
+  CKI(with_smem(span_tile_kernel<HD>, span_tile_smem(HD, kMaxListed), done, true));
   WaitWord* waits = op_waits();
   if (!waits) return fail("span_attn: pinned word for bounded waits not allocated");
   CKI(waits->check("an earlier call of attention without an engine left is not complete (NaN rows)"));

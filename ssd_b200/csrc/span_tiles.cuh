@@ -1,11 +1,13 @@
 // span_tiles.cuh — span_attention of more than sixteen query rows to a key head, on tcgen05.
 //
-// The pipeline of prompt_attn_kernel's twin form: S = Q K^T of up to 64 rows and 64 keys into TMEM, P = exp2(S - m) one row per thread, O += P V with P out of
-// TMEM.  The queries lie in rows 0 .. 63 and again in 64 .. 127: these make the low bf16 pieces of the weights, add up in lanes of their own and are added
-// at the end.  A chunk of 64 keys is gathered from the listed spans by TMA boxes of gcd(span, 64) keys, in list order; what is missing from the last
+// The order of loads, products and waits of prompt_attn_kernel: S = Q K^T of up to 64 rows and 64 keys into TMEM, P = exp2(S - m) per thread, O += P V with P
+// out of TMEM.  The queries lie in rows 0 .. 63 and again in 64 .. 127: a row's first lane takes the first 32 keys of a chunk and its second the others, each with
+// a reference, a sum and an accumulator of its own (its P is zero at the other's keys), so that four warps share the exponentials of 64 rows.  Weights are two
+// bf16 pieces side by side, with a product each.  (With the low pieces in the second lanes, as prompt_attn_kernel has them, both lanes made all exponentials: 2500
+// clocks a chunk, XX so.)  A chunk of 64 keys is gathered from the listed spans by TMA boxes of gcd(span, 64) keys, in list order; what is missing from the last
 // chunk is loaded from behind the cache (zeros) and masked.  A cluster of blocks shares the chunks of a key head; their sums meet in shared memory.
 // Up to sixteen rows span_attn_kernel is as fast as the memory; with more its mma.sync products bound it: 8 sequences of 7 rows, 64 heads over 8 of 128,
-// 4096 listed keys each: 63 us on two m16 tiles a warp, 36 here.
+// 4096 listed keys each: 63 us on two m16 tiles a warp, YY here.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -14,11 +16,59 @@
 
 namespace ssdk {
 
-constexpr int kTileRows64 = 64, kTileKeys = 64, kTileStages = 2, kTileThreads = 192;
-constexpr int kTileMost = 8;   // blocks of a cluster
+constexpr int kTileRows64 = 64, kTileKeys = 64, kTileStages = 2, kTileThreads = 224;   // warps: loads, scores, 4 of softmax, products with V
+constexpr int kTileMost = 16;   // blocks of a cluster
 // query twice | keys and values; behind them the places of the listed spans
 constexpr int span_tile_body(int HD) { return 2 * kTileRows64 * HD * 2 + kTileStages * 2 * kTileKeys * HD * 2; }
 constexpr int span_tile_smem(int HD, int count) { return span_tile_body(HD) + 1024 + count * 8; }
+
+// A bounded wait (about two seconds; then the word is set and false comes back): the clock is read only where the first look fails.
+SSDK_DEVINL bool tile_wait(uint64_t* bar, uint32_t parity, unsigned* timeout) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity))
+    if (clock64() - t0 > 4000000000LL) {
+      if (timeout) *(volatile unsigned*)timeout = 1u;
+      return false;
+    }
+  return true;
+}
+SSDK_DEVINL bool tile_wait_warp(uint64_t* bar, uint32_t parity, unsigned* timeout) { return __all_sync(0xffffffffu, tile_wait(bar, parity, timeout)); }
+
+SSDK_DEVINL float half_row_max(const uint32_t (&u)[32]) {
+  float m[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) m[e] = max3(__uint_as_float(u[e]), __uint_as_float(u[e + 4]), __uint_as_float(u[e + 8]));
+#pragma unroll
+  for (int c = 12; c < 28; c += 8)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[e] = max3(m[e], __uint_as_float(u[c + e]), __uint_as_float(u[c + 4 + e]));
+  return fmaxf(max3(m[0], m[1], __uint_as_float(u[28])), max3(m[2], m[3], max3(__uint_as_float(u[29]), __uint_as_float(u[30]), __uint_as_float(u[31]))));
+}
+// 2^(score * scale - ms) of 32 keys as two bf16 pieces: the first in the first 16 words, what it leaves in the others; their sum (unrounded) back
+SSDK_DEVINL float half_row_exp(uint32_t (&u)[32], float scale, float ms) {
+  const uint64_t sc = pack2(scale, scale), off = pack2(-ms, -ms), minus = pack2(-1.f, -1.f);
+  uint64_t sum[2] = {0, 0};
+  uint32_t low[16];
+#pragma unroll
+  for (int c = 0; c < 32; c += 2) {
+    float a, e, x, y;
+    unpack2(fma2(pack2(__uint_as_float(u[c]), __uint_as_float(u[c + 1])), sc, off), &a, &e);
+    a = ex2_ftz(a); e = ex2_ftz(e);
+    const uint64_t ae = pack2(a, e);
+    sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], ae);
+    const uint32_t h = pack_bf16x2(a, e);
+    unpack2(fma2(pack2(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u)), minus, ae), &x, &y);   // (exact differences)
+    u[c >> 1] = h;
+    low[c >> 1] = pack_bf16x2(x, y);
+  }
+#pragma unroll
+  for (int c = 0; c < 16; ++c) u[16 + c] = low[c];
+  float s0, s1, s2, s3;
+  unpack2(sum[0], &s0, &s1);
+  unpack2(sum[1], &s2, &s3);
+  return (s0 + s1) + (s2 + s3);
+}
 
 template <int HD>
 __global__ void __launch_bounds__(kTileThreads, 2)
@@ -28,7 +78,7 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   constexpr int HALVES = HD / 64;                    // 64-column boxes of a row
   constexpr int kQHalf = 2 * kTileRows64 * 128, kKHalf = kTileKeys * 128, kTile = HALVES * kKHalf;
   extern __shared__ uint8_t span_tile_raw[];
-  __shared__ __align__(8) uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2];
+  __shared__ __align__(8) uint64_t q_full, k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int s_failed, found[kTileThreads / 32];
   uint8_t* smem = span_tile_raw + ((1024u - (smem_u32(span_tile_raw) & 1023u)) & 1023u);
@@ -50,8 +100,7 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     tma_prefetch_desc(&tmV);
     mbar_init(&q_full, 1);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1);
-      mbar_init(&s_full[s], 1); mbar_init(&p_full[s], live); mbar_init(&pv_done[s], 1);
+      mbar_init(&k_full[s], 1); mbar_init(&v_full[s], 1); mbar_init(&s_full[s], 1); mbar_init(&p_full[s], live); mbar_init(&pv_done[s], 1);
     }
     fence_mbar_init();
     s_failed = 0;
@@ -71,6 +120,11 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const uint32_t there = __ballot_sync(0xffffffffu, at.x >= 0);
     if (lane == 0) found[warp] = __popc(there);
     __syncthreads();
+    if (base == 0 && threadIdx.x == 0) {   // the queries need no list
+      mbar_arrive_expect_tx(&q_full, HALVES * 2 * 128 * G * q_tokens);
+      for (int h = 0; h < HALVES; ++h)
+        for (int x = 0; x < 2 * kTileRows64; x += kTileRows64) tma_load_3d(sQ + h * kQHalf + x * 128, &tmQ, &q_full, h * 64, kvh * G, b * p.Q + tok0);
+    }
     int before = spans + __popc(there & ((1u << lane) - 1));
 #pragma unroll
     for (int w = 0; w < kTileThreads / 32; ++w) {
@@ -95,33 +149,35 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const int2 at = where[i];
     return make_int2(at.x + off, at.y + off);
   };
-  // chunk i on barrier i & 1; parity(i) is that use's.  A wait by parity is only right while the barrier is in that use or the one behind it: as in
-  // prompt_attn_kernel, whose order of products and waits this is.
+  // Chunk i on barrier i & 1; parity(i) is that use's.  A wait by parity is only right while the barrier is in that use or the one behind it:
+  //   k_full, v_full, p_full: whoever waits for chunk i has to be through with it before the stage, or P, is made anew for chunk i + 2.
+  //   s_full: the softmax asks for chunk i, and scores of chunk i + 2 need its P (through pv_done of chunk i); the loads ask for chunk i - 2 before they bring
+  //     the keys that scores of chunk i need.
+  //   pv_done: the scores of chunk i + 1 ask for chunk i - 1, the softmax of chunk i for chunk i - 1 or nothing, the loads of chunk i for chunk i - 2, the end for
+  //     chunk n - 1.  Chunk i + 1's product, the next on that barrier, needs the P of chunk i + 1, so its scores, so the first of them; the P of a warp that
+  //     has not gone on, so the second; and the values of chunk i + 1, so the third.
   auto parity = [](int i) { return (uint32_t)(i >> 1) & 1u; };
   float l = 0.f, m = -INFINITY;
   bool ok = true;
   const int q4 = warp & 3, r = (q4 & 1) * 32 + lane;
-  const bool softmax = warp >= 2, low = q4 >= 2, in = softmax && (r & ~31) < half;   // (whole warps) low: the same row as two warps before, its low pieces
+  const bool softmax = warp >= 2 && warp < 6, second = q4 >= 2, in = softmax && (r & ~31) < half;   // (whole warps) second: the same row as two warps before, the other keys
   const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
 
   if (warp == 0) {
-    if (lane == 0 && n > 0) {
-      mbar_arrive_expect_tx(&q_full, HALVES * 2 * 128 * G * q_tokens);
-      for (int h = 0; h < HALVES; ++h)
-        for (int x = 0; x < 2 * kTileRows64; x += kTileRows64) tma_load_3d(sQ + h * kQHalf + x * 128, &tmQ, &q_full, h * 64, kvh * G, b * p.Q + tok0);
+    if (lane == 0) {
       int i = 0;
       for (; i < n; ++i) {
         const int s = i & 1;
         int slots[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) slots[j] = j < boxes ? box_at((first + i) * boxes + j).x : 0;
-        if (!mbar_wait_cluster(&k_empty[s], parity(i) ^ 1u, timeout)) break;
+        if (i > 1 && !tile_wait(&s_full[s], parity(i - 2), timeout)) break;   // the keys of chunk i - 2 have been read
         mbar_arrive_expect_tx(&k_full[s], kTile);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (j < boxes)
             for (int h = 0; h < HALVES; ++h) tma_load_3d(sK + s * kTile + h * kKHalf + j * box * 128, &tmK, &k_full[s], h * 64, kvh, slots[j]);
-        if (!mbar_wait_cluster(&v_empty[s], parity(i) ^ 1u, timeout)) { mbar_wait_cluster(&k_full[s], parity(i), timeout); break; }
+        if (i > 1 && !tile_wait(&pv_done[s], parity(i - 2), timeout)) { tile_wait(&k_full[s], parity(i), timeout); break; }
         mbar_arrive_expect_tx(&v_full[s], kTile);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -129,19 +185,21 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             for (int h = 0; h < HALVES; ++h) tma_load_3d(sV + s * kTile + h * kKHalf + j * box * 128, &tmV, &v_full[s], h * 64, kvh, slots[j]);
       }
       // nothing is in flight into this block's memory when it leaves, also after a wait ran out
-      mbar_wait_cluster(&q_full, 0, timeout);
+      tile_wait(&q_full, 0, timeout);
       for (int j = max(0, i - 2); j < i; ++j) {
-        mbar_wait_cluster(&k_full[j & 1], parity(j), timeout);
-        mbar_wait_cluster(&v_full[j & 1], parity(j), timeout);
+        tile_wait(&k_full[j & 1], parity(j), timeout);
+        tile_wait(&v_full[j & 1], parity(j), timeout);
       }
     }
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t idesc_s = make_umma_idesc_bf16(2 * kTileRows64, kTileKeys);
-      constexpr uint32_t idesc_o = make_umma_idesc_bf16(2 * kTileRows64, HD) | (1u << 16);   // V: b_major = MN
-      auto scores = [&](int i) {
-        if (!mbar_wait_cluster(&k_full[i & 1], parity(i), timeout)) return false;
+      bool go = n > 0 && tile_wait(&q_full, 0, timeout);
+      for (int i = 0; i < n && go; ++i) {
+        // the scores of chunk i go over the P that the product of chunk i - 2 reads
+        if (i > 1 && !(go = tile_wait(&pv_done[i & 1], parity(i - 2), timeout))) break;
+        if (!(go = tile_wait(&k_full[i & 1], parity(i), timeout))) break;
         tc_fence_after();
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
@@ -149,23 +207,23 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
           for (int k = 0; k < 4; ++k) umma_bf16_ss(tmem + (i & 1) * 64, qd + 2 * k, kd + 2 * k, idesc_s, (uint32_t)((h | k) != 0));
         }
-        umma_commit(&k_empty[i & 1]);
         umma_commit(&s_full[i & 1]);
-        return true;
-      };
-      bool go = n > 0 && mbar_wait_cluster(&q_full, 0, timeout) && scores(0);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 6) {
+    if (lane == 0) {
+      constexpr uint32_t idesc_o = make_umma_idesc_bf16(2 * kTileRows64, HD) | (1u << 16);   // V: b_major = MN
+      bool go = true;
       for (int i = 0; i < n && go; ++i) {
-        // the scores of chunk i + 1 go over the P that the product of chunk i - 1 reads: products of different shapes and accumulators
-        // have no order of their own
-        if (i > 0 && !(go = mbar_wait_cluster(&pv_done[(i - 1) & 1], parity(i - 1), timeout))) break;
-        if (i + 1 < n && !(go = scores(i + 1))) break;
-        if (!(go = mbar_wait_cluster(&p_full[i & 1], parity(i), timeout) && mbar_wait_cluster(&v_full[i & 1], parity(i), timeout))) break;
+        if (!(go = tile_wait(&v_full[i & 1], parity(i), timeout) && tile_wait(&p_full[i & 1], parity(i), timeout))) break;
         tc_fence_after();
         const uint64_t vd = make_umma_desc_mn128(sV + (i & 1) * kTile, kKHalf);
 #pragma unroll
         for (int k = 0; k < kTileKeys / 16; ++k)   // 16 keys: 2048 B of V, 8 columns of P
           umma_bf16_ts(tmem_o, tmem + (i & 1) * 64 + 8 * k, vd + 128 * k, idesc_o, (uint32_t)((i | k) != 0));
-        umma_commit(&v_empty[i & 1]);
+#pragma unroll
+        for (int k = 0; k < kTileKeys / 16; ++k) umma_bf16_ts(tmem_o, tmem + (i & 1) * 64 + 32 + 8 * k, vd + 128 * k, idesc_o, 1u);
         umma_commit(&pv_done[i & 1]);
       }
     }
@@ -186,29 +244,29 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const int at = 16 * j / box;
         pos[j] = __shfl_sync(0xffffffffu, mine, at) + (16 * j - at * box);
       }
-      if (!(ok = warp_wait(&s_full[i & 1], parity(i), timeout))) break;
+      if (!(ok = tile_wait_warp(&s_full[i & 1], parity(i), timeout))) break;
       tc_fence_after();
-      uint32_t u[64];
-#pragma unroll
-      for (int c = 0; c < 64; c += 16) tmem_ld_32x32b_x16(sp + c, u + c);
+      uint32_t u[32];
+      tmem_ld_32x32b_x16(sp + (second ? 32 : 0), u);
+      tmem_ld_32x32b_x16(sp + (second ? 48 : 16), u + 16);
       tmem_ld_wait();
       if (p.q_sign || !p.q_keep) {   // a scale that is not positive
 #pragma unroll
-        for (int c = 0; c < 64; ++c) u[c] = (u[c] & p.q_keep) ^ (p.q_sign & 0x80000000u);
+        for (int c = 0; c < 32; ++c) u[c] = (u[c] & p.q_keep) ^ (p.q_sign & 0x80000000u);
       }
       if (!whole) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (pos[c / 16] + c % 16 >= lim) u[c] = 0xff800000u;   // -inf
+        for (int c = 0; c < 32; ++c)
+          if ((second ? pos[2 + c / 16] : pos[c / 16]) + c % 16 >= lim) u[c] = 0xff800000u;   // -inf
       }
-      const float mx = row_max(u) * p.scale_log2;
+      const float mx = half_row_max(u) * p.scale_log2;
       const bool grow = mx > m + kPromptSlack;
       if (__any_sync(0xffffffffu, grow)) {
         const float f = grow ? exp2f(m - mx) : 1.f;   // (m = -inf: 0)
         if (grow) m = mx;
         l *= f;
         if (i > 0) {
-          if (!(ok = warp_wait(&pv_done[(i - 1) & 1], parity(i - 1), timeout))) break;
+          if (!(ok = tile_wait_warp(&pv_done[(i - 1) & 1], parity(i - 1), timeout))) break;
           tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < HD; c += 16) {
@@ -222,17 +280,20 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         }
       }
       const float ms = m == -INFINITY ? 0.f : m;
-      l += low ? row_exp<false, true>(u, p.scale_log2, ms) : row_exp<true, false>(u, p.scale_log2, ms);
-#pragma unroll
-      for (int c = 0; c < 32; c += 16) tmem_st_32x32b_x16(sp + c, u + c);
+      l += half_row_exp(u, p.scale_log2, ms);
+      const uint32_t zero[16] = {};
+      tmem_st_32x32b_x16(sp + (second ? 16 : 0), u);
+      tmem_st_32x32b_x16(sp + (second ? 0 : 16), zero);
+      tmem_st_32x32b_x16(sp + (second ? 48 : 32), u + 16);
+      tmem_st_32x32b_x16(sp + (second ? 32 : 48), zero);
       tmem_st_wait();
       if (!whole) {   // slots behind the context hold anything, and 0 x NaN is NaN
         bool stale = false;
 #pragma unroll
         for (int j = 0; j < 4; ++j) stale = stale || (pos[j] < (1 << 29) && pos[j] + 16 > len);
         if (stale) {   // (the same for all warps)
-          if (!(ok = warp_wait(&v_full[i & 1], parity(i), timeout))) break;
-          for (int j = low ? half + r : r; j < kTileKeys * 8; j += live) {
+          if (!(ok = tile_wait_warp(&v_full[i & 1], parity(i), timeout))) break;
+          for (int j = second ? half + r : r; j < kTileKeys * 8; j += live) {
             const int key = j >> 3, x = key >> 4;
             if ((x == 0 ? pos[0] : x == 1 ? pos[1] : x == 2 ? pos[2] : pos[3]) + (key & 15) >= len)
 #pragma unroll
@@ -244,44 +305,49 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       tc_fence_before();
       mbar_arrive(&p_full[i & 1]);
     }
-    if (ok && n > 0) ok = warp_wait(&pv_done[(n - 1) & 1], parity(n - 1), timeout);
+    if (ok && n > 0) ok = tile_wait_warp(&pv_done[(n - 1) & 1], parity(n - 1), timeout);
     tc_fence_after();
   }
 
-  // ---- the sums of a row: low pieces to the row's warp, then [row][HD + 4] O | reference, sum in the stages (every product has read them) ----
+  // ---- a row's two parts, then the blocks': [row][HD + 4] O | reference, sum over queries, keys and values (every product has read them) ----
   constexpr int LDO = HD + 4;
-  float* joined = reinterpret_cast<float*>(sK);
-  if (softmax && in && low) {
+  float* joined = reinterpret_cast<float*>(smem);
+  auto sums = [&](int c, float* f) {   // 16 columns
+    uint32_t o[16];
+    tmem_ld_32x32b_x16(tmem_o + lanes + c, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(o[j]);
+  };
+  __syncthreads();   // nothing is on its way into them
+  if (softmax && in && second) {
     if (!ok) s_failed = 1;
+    *reinterpret_cast<float2*>(joined + r * LDO + HD) = make_float2(m, l);
     if (ok && n > 0)
       for (int c = 0; c < HD; c += 16) {
-        uint32_t o[16];
-        tmem_ld_32x32b_x16(tmem_o + lanes + c, o);
-        tmem_ld_wait();
+        float f[16];
+        sums(c, f);
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) *reinterpret_cast<uint4*>(joined + r * LDO + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+        for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(joined + r * LDO + c + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
       }
   }
   __syncthreads();
-  if (softmax && in && !low) {
+  if (softmax && in && !second) {
     const bool good = ok && !s_failed;
-    if (n > 0 && good)
-      for (int c = 0; c < HD; c += 16) {
-        uint32_t o[16];
-        tmem_ld_32x32b_x16(tmem_o + lanes + c, o);
-        tmem_ld_wait();
+    const float2 other = *reinterpret_cast<const float2*>(joined + r * LDO + HD);
+    const float top = fmaxf(m, other.x), f0 = m == -INFINITY ? 0.f : exp2f(m - top), f1 = other.x == -INFINITY ? 0.f : exp2f(other.x - top);
+    for (int c = 0; c < HD; c += 16) {
+      float f[16];
+      if (good && n > 0) sums(c, f);
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          float4* at = reinterpret_cast<float4*>(joined + r * LDO + c + j);
-          const float4 x = *at;
-          *at = make_float4(x.x + __uint_as_float(o[j]), x.y + __uint_as_float(o[j + 1]), x.z + __uint_as_float(o[j + 2]), x.w + __uint_as_float(o[j + 3]));
-        }
+      for (int j = 0; j < 16; j += 4) {
+        float4* at = reinterpret_cast<float4*>(joined + r * LDO + c + j);
+        const float4 x = *at;
+        *at = good && n > 0 ? make_float4(f[j] * f0 + x.x * f1, f[j + 1] * f0 + x.y * f1, f[j + 2] * f0 + x.z * f1, f[j + 3] * f0 + x.w * f1) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
+    }
     // a wait ran out: the row is NaN.  Without chunks (or keys) the row has no part in the sum.
-    const float2 ml = !good ? make_float2(0.f, __int_as_float(0x7fffffff)) : n > 0 ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
-    *reinterpret_cast<float2*>(joined + r * LDO + HD) = ml;
-    if (!good || n == 0)
-      for (int c = 0; c < HD; c += 4) *reinterpret_cast<float4*>(joined + r * LDO + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+    *reinterpret_cast<float2*>(joined + r * LDO + HD) = good ? make_float2(top, l * f0 + other.y * f1) : make_float2(0.f, __int_as_float(0x7fffffff));
   }
   tc_fence_before();
   __syncthreads();
@@ -290,27 +356,21 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   cluster.sync();
   for (int idx = rank * kTileThreads + threadIdx.x; idx < rows * (HD / 4); idx += C * kTileThreads) {
     const int row = idx / (HD / 4), d = idx % (HD / 4) * 4;
-    float2 ml[kTileMost];
-    float4 v[kTileMost];
     float top = -INFINITY;
-#pragma unroll
-    for (int c = 0; c < kTileMost; ++c)
-      if (c < C) {
-        const float* part = cluster.map_shared_rank(joined, c) + row * LDO;
-        ml[c] = *reinterpret_cast<const float2*>(part + HD);
-        v[c] = *reinterpret_cast<const float4*>(part + d);
-        top = fmaxf(top, ml[c].x);
-      }
+#pragma unroll 4
+    for (int c = 0; c < C; ++c) top = fmaxf(top, cluster.map_shared_rank(joined, c)[row * LDO + HD]);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
     if (top != -INFINITY) {
-#pragma unroll
-      for (int c = 0; c < kTileMost; ++c)
-        if (c < C) {
-          const float f = exp2f(ml[c].x - top);
-          acc.x += v[c].x * f; acc.y += v[c].y * f; acc.z += v[c].z * f; acc.w += v[c].w * f;
-          sum += ml[c].y * f;
-        }
+#pragma unroll 4
+      for (int c = 0; c < C; ++c) {
+        const float* part = cluster.map_shared_rank(joined, c) + row * LDO;
+        const float2 ml = *reinterpret_cast<const float2*>(part + HD);
+        const float4 v = *reinterpret_cast<const float4*>(part + d);
+        const float f = exp2f(ml.x - top);
+        acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+        sum += ml.y * f;
+      }
     }
     const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;   // (NaN stays)
     __nv_bfloat16* dst = p.out + ((size_t)(b * p.Q + tok0 + row / G) * p.heads + kvh * G + row % G) * HD + d;
