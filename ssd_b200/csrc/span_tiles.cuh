@@ -1,13 +1,14 @@
 // span_tiles.cuh — span_attention of more than sixteen query rows to a key head, on tcgen05.
 //
-// The order of loads, products and waits of prompt_attn_kernel: S = Q K^T of up to 64 rows and 64 keys into TMEM, P = exp2(S - m) per thread, O += P V with P
-// out of TMEM.  The queries lie in rows 0 .. 63 and again in 64 .. 127: a row's first lane takes the first 32 keys of a chunk and its second the others, each with
-// a reference, a sum and an accumulator of its own (its P is zero at the other's keys), so that four warps share the exponentials of 64 rows.  Weights are two
-// bf16 pieces side by side, with a product each.  (With the low pieces in the second lanes, as prompt_attn_kernel has them, both lanes made all exponentials: 2500
-// clocks a chunk, XX so.)  A chunk of 64 keys is gathered from the listed spans by TMA boxes of gcd(span, 64) keys, in list order; what is missing from the last
+// As in prompt_attn_kernel's twin form: S = Q K^T of up to 64 rows and 64 keys into TMEM, P = exp2(S - m) one row per thread, O += P V with P out of TMEM.  The
+// queries lie in rows 0 .. 63 and again in 64 .. 127: these make the low bf16 pieces of the weights, add up in lanes of their own and are added at the
+// end.  (With a row's keys shared by its two lanes, zeros in P at the other's keys and the two pieces in a product each, the exponentials halve and the
+// products double: 37.0 us against 36.5 where this is 36.5, one warp issuing; tensor and shared memory are what two blocks share.)  Scores and products with V are issued
+// by a warp each, with one commit a product: one thread that issued both and looked at five barriers a chunk held it at 2500 clocks a chunk (36.5 -> 33.4 us).
+// A chunk of 64 keys is gathered from the listed spans by TMA boxes of gcd(span, 64) keys, in list order; what is missing from the last
 // chunk is loaded from behind the cache (zeros) and masked.  A cluster of blocks shares the chunks of a key head; their sums meet in shared memory.
 // Up to sixteen rows span_attn_kernel is as fast as the memory; with more its mma.sync products bound it: 8 sequences of 7 rows, 64 heads over 8 of 128,
-// 4096 listed keys each: 63 us on two m16 tiles a warp, YY here.
+// 4096 listed keys each: 63 us on two m16 tiles a warp, 33.4 here (32 sequences: 105 us, 79 % of the copy rate).
 #pragma once
 #include <cooperative_groups.h>
 
@@ -34,41 +35,6 @@ SSDK_DEVINL bool tile_wait(uint64_t* bar, uint32_t parity, unsigned* timeout) {
   return true;
 }
 SSDK_DEVINL bool tile_wait_warp(uint64_t* bar, uint32_t parity, unsigned* timeout) { return __all_sync(0xffffffffu, tile_wait(bar, parity, timeout)); }
-
-SSDK_DEVINL float half_row_max(const uint32_t (&u)[32]) {
-  float m[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) m[e] = max3(__uint_as_float(u[e]), __uint_as_float(u[e + 4]), __uint_as_float(u[e + 8]));
-#pragma unroll
-  for (int c = 12; c < 28; c += 8)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) m[e] = max3(m[e], __uint_as_float(u[c + e]), __uint_as_float(u[c + 4 + e]));
-  return fmaxf(max3(m[0], m[1], __uint_as_float(u[28])), max3(m[2], m[3], max3(__uint_as_float(u[29]), __uint_as_float(u[30]), __uint_as_float(u[31]))));
-}
-// 2^(score * scale - ms) of 32 keys as two bf16 pieces: the first in the first 16 words, what it leaves in the others; their sum (unrounded) back
-SSDK_DEVINL float half_row_exp(uint32_t (&u)[32], float scale, float ms) {
-  const uint64_t sc = pack2(scale, scale), off = pack2(-ms, -ms), minus = pack2(-1.f, -1.f);
-  uint64_t sum[2] = {0, 0};
-  uint32_t low[16];
-#pragma unroll
-  for (int c = 0; c < 32; c += 2) {
-    float a, e, x, y;
-    unpack2(fma2(pack2(__uint_as_float(u[c]), __uint_as_float(u[c + 1])), sc, off), &a, &e);
-    a = ex2_ftz(a); e = ex2_ftz(e);
-    const uint64_t ae = pack2(a, e);
-    sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], ae);
-    const uint32_t h = pack_bf16x2(a, e);
-    unpack2(fma2(pack2(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u)), minus, ae), &x, &y);   // (exact differences)
-    u[c >> 1] = h;
-    low[c >> 1] = pack_bf16x2(x, y);
-  }
-#pragma unroll
-  for (int c = 0; c < 16; ++c) u[16 + c] = low[c];
-  float s0, s1, s2, s3;
-  unpack2(sum[0], &s0, &s1);
-  unpack2(sum[1], &s2, &s3);
-  return (s0 + s1) + (s2 + s3);
-}
 
 template <int HD>
 __global__ void __launch_bounds__(kTileThreads, 2)
@@ -160,7 +126,7 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   float l = 0.f, m = -INFINITY;
   bool ok = true;
   const int q4 = warp & 3, r = (q4 & 1) * 32 + lane;
-  const bool softmax = warp >= 2 && warp < 6, second = q4 >= 2, in = softmax && (r & ~31) < half;   // (whole warps) second: the same row as two warps before, the other keys
+  const bool softmax = warp >= 2 && warp < 6, second = q4 >= 2, in = softmax && (r & ~31) < half;   // (whole warps) second: the same row as two warps before, its low pieces
   const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
 
   if (warp == 0) {
@@ -222,8 +188,6 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
         for (int k = 0; k < kTileKeys / 16; ++k)   // 16 keys: 2048 B of V, 8 columns of P
           umma_bf16_ts(tmem_o, tmem + (i & 1) * 64 + 8 * k, vd + 128 * k, idesc_o, (uint32_t)((i | k) != 0));
-#pragma unroll
-        for (int k = 0; k < kTileKeys / 16; ++k) umma_bf16_ts(tmem_o, tmem + (i & 1) * 64 + 32 + 8 * k, vd + 128 * k, idesc_o, 1u);
         umma_commit(&pv_done[i & 1]);
       }
     }
@@ -246,20 +210,20 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       if (!(ok = tile_wait_warp(&s_full[i & 1], parity(i), timeout))) break;
       tc_fence_after();
-      uint32_t u[32];
-      tmem_ld_32x32b_x16(sp + (second ? 32 : 0), u);
-      tmem_ld_32x32b_x16(sp + (second ? 48 : 16), u + 16);
+      uint32_t u[64];
+#pragma unroll
+      for (int c = 0; c < 64; c += 16) tmem_ld_32x32b_x16(sp + c, u + c);
       tmem_ld_wait();
       if (p.q_sign || !p.q_keep) {   // a scale that is not positive
 #pragma unroll
-        for (int c = 0; c < 32; ++c) u[c] = (u[c] & p.q_keep) ^ (p.q_sign & 0x80000000u);
+        for (int c = 0; c < 64; ++c) u[c] = (u[c] & p.q_keep) ^ (p.q_sign & 0x80000000u);
       }
       if (!whole) {
 #pragma unroll
-        for (int c = 0; c < 32; ++c)
-          if ((second ? pos[2 + c / 16] : pos[c / 16]) + c % 16 >= lim) u[c] = 0xff800000u;   // -inf
+        for (int c = 0; c < 64; ++c)
+          if (pos[c / 16] + c % 16 >= lim) u[c] = 0xff800000u;   // -inf
       }
-      const float mx = half_row_max(u) * p.scale_log2;
+      const float mx = row_max(u) * p.scale_log2;
       const bool grow = mx > m + kPromptSlack;
       if (__any_sync(0xffffffffu, grow)) {
         const float f = grow ? exp2f(m - mx) : 1.f;   // (m = -inf: 0)
@@ -280,12 +244,9 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         }
       }
       const float ms = m == -INFINITY ? 0.f : m;
-      l += half_row_exp(u, p.scale_log2, ms);
-      const uint32_t zero[16] = {};
-      tmem_st_32x32b_x16(sp + (second ? 16 : 0), u);
-      tmem_st_32x32b_x16(sp + (second ? 0 : 16), zero);
-      tmem_st_32x32b_x16(sp + (second ? 48 : 32), u + 16);
-      tmem_st_32x32b_x16(sp + (second ? 32 : 48), zero);
+      l += second ? row_exp<false, true>(u, p.scale_log2, ms) : row_exp<true, false>(u, p.scale_log2, ms);
+      tmem_st_32x32b_x16(sp, u);
+      tmem_st_32x32b_x16(sp + 16, u + 16);
       tmem_st_wait();
       if (!whole) {   // slots behind the context hold anything, and 0 x NaN is NaN
         bool stale = false;
@@ -309,7 +270,7 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     tc_fence_after();
   }
 
-  // ---- a row's two parts, then the blocks': [row][HD + 4] O | reference, sum over queries, keys and values (every product has read them) ----
+  // ---- the sums of a row: low pieces to the row's warp, then [row][HD + 4] O | reference, sum over queries, keys and values (every product has read them) ----
   constexpr int LDO = HD + 4;
   float* joined = reinterpret_cast<float*>(smem);
   auto sums = [&](int c, float* f) {   // 16 columns
@@ -322,7 +283,6 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   __syncthreads();   // nothing is on its way into them
   if (softmax && in && second) {
     if (!ok) s_failed = 1;
-    *reinterpret_cast<float2*>(joined + r * LDO + HD) = make_float2(m, l);
     if (ok && n > 0)
       for (int c = 0; c < HD; c += 16) {
         float f[16];
@@ -334,8 +294,6 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   __syncthreads();
   if (softmax && in && !second) {
     const bool good = ok && !s_failed;
-    const float2 other = *reinterpret_cast<const float2*>(joined + r * LDO + HD);
-    const float top = fmaxf(m, other.x), f0 = m == -INFINITY ? 0.f : exp2f(m - top), f1 = other.x == -INFINITY ? 0.f : exp2f(other.x - top);
     for (int c = 0; c < HD; c += 16) {
       float f[16];
       if (good && n > 0) sums(c, f);
@@ -343,11 +301,11 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       for (int j = 0; j < 16; j += 4) {
         float4* at = reinterpret_cast<float4*>(joined + r * LDO + c + j);
         const float4 x = *at;
-        *at = good && n > 0 ? make_float4(f[j] * f0 + x.x * f1, f[j + 1] * f0 + x.y * f1, f[j + 2] * f0 + x.z * f1, f[j + 3] * f0 + x.w * f1) : make_float4(0.f, 0.f, 0.f, 0.f);
+        *at = good && n > 0 ? make_float4(f[j] + x.x, f[j + 1] + x.y, f[j + 2] + x.z, f[j + 3] + x.w) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
     }
     // a wait ran out: the row is NaN.  Without chunks (or keys) the row has no part in the sum.
-    *reinterpret_cast<float2*>(joined + r * LDO + HD) = good ? make_float2(top, l * f0 + other.y * f1) : make_float2(0.f, __int_as_float(0x7fffffff));
+    *reinterpret_cast<float2*>(joined + r * LDO + HD) = good ? make_float2(m, l) : make_float2(0.f, __int_as_float(0x7fffffff));
   }
   tc_fence_before();
   __syncthreads();
