@@ -496,13 +496,27 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
 #pragma unroll
   for (int i = 0; i < ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
-  const int per = p.span / kSpanKeys, pieces = n_list * per;
+  const int per = p.span / kSpanKeys;   // pieces of a span
   constexpr int TOK = 32 / SEG;   // keys that a warp copies at a time
   const int tok0 = lane / SEG, seg = lane % SEG;
   const size_t row_step = (size_t)TOK * p.kv_heads * HD;
-  auto load = [&](int piece, int stage) {
-    const int i = piece / per, off = (piece - i * per) * kSpanKeys;
-    const int2 at = where[i];
+  // places in the list advance by a warp's stride without a division
+  const int step = kSpanWarps * C, step_i = step / per, step_r = step - step_i * per;
+  struct Place { int i, r; };   // span of the list, piece of the span
+  auto advance = [&](Place& at) {
+    at.i += step_i;
+    at.r += step_r;
+    if (at.r >= per) {
+      at.r -= per;
+      ++at.i;
+    }
+  };
+  const int own = rank * kSpanWarps + warp;
+  Place ahead = {own / per, own % per}, now = ahead;
+  auto load = [&](int stage) {   // the piece that is next to be asked for
+    if (ahead.i >= n_list) return;
+    const int off = ahead.r * kSpanKeys;
+    const int2 at = where[ahead.i];
     const bool there = at.x >= 0;
     __nv_bfloat16* dk = reinterpret_cast<__nv_bfloat16*>(ring + stage * span_stage_bytes(HD)) + tok0 * LDS + seg * 8;
     __nv_bfloat16* dv = dk + kSpanKeys * LDS;
@@ -522,22 +536,23 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
       }
     }
   };
-  const int step = kSpanWarps * C, own = rank * kSpanWarps + warp;
 #pragma unroll
   for (int s = 0; s < kSpanStages - 1; ++s) {
-    if (own + s * step < pieces) load(own + s * step, s);
+    load(s);
+    advance(ahead);
     cp_async_commit();
   }
-  int stage = 0;
-  for (int piece = own; piece < pieces; piece += step, stage = stage + 1 == kSpanStages ? 0 : stage + 1) {
+  for (int stage = 0; now.i < n_list; stage = stage + 1 == kSpanStages ? 0 : stage + 1) {
     __syncwarp();   // every lane is done with the stage that is filled now
-    if (piece + (kSpanStages - 1) * step < pieces) load(piece + (kSpanStages - 1) * step, stage == 0 ? kSpanStages - 1 : stage - 1);
+    load(stage == 0 ? kSpanStages - 1 : stage - 1);
+    advance(ahead);
     cp_async_commit();
     cp_async_wait<kSpanStages - 1>();
     __syncwarp();   // every lane's copies of this stage have landed
-    const int2 at = where[piece / per];
+    const int2 at = where[now.i];
+    const int pos0 = at.y + now.r * kSpanKeys;
+    advance(now);
     if (at.x < 0) continue;
-    const int pos0 = at.y + (piece % per) * kSpanKeys;
     const __nv_bfloat16* cK = reinterpret_cast<const __nv_bfloat16*>(ring + stage * span_stage_bytes(HD));
     const __nv_bfloat16* cV = cK + kSpanKeys * LDS;
     const int mi = lane >> 3, rr = lane & 7;
