@@ -105,8 +105,16 @@ static int launch_select(Launcher& L, const SelectParams& p) {
   CKI(with_smem(span_pick_kernel<HD>, kMaxSmem, done));
   L.pdl = true;
   constexpr int W = kEstimateThreads / 32;
-  CKI(L.go(span_estimate_kernel<HD>, dim3(p.warps / W, p.kv_heads, p.B), dim3(kEstimateThreads), 0, p));
-  return L.go(span_pick_kernel<HD>, dim3(p.kv_heads, p.B), dim3(kPickThreads), pick_smem(p.max_spans, p.Q * (p.heads / p.kv_heads), HD), p);
+  const int64_t rows = (int64_t)p.Q * (p.heads / p.kv_heads);
+  const dim3 grid(p.warps / W, p.kv_heads, p.B), block(kEstimateThreads);
+  if (rows > 8) {
+    static std::atomic<bool> many_done[64];
+    CKI(with_smem(span_estimate_kernel<HD, true>, kMaxSmem, many_done));
+    CKI(L.go(span_estimate_kernel<HD, true>, grid, block, estimate_smem(rows, HD), p));
+  } else {
+    CKI(L.go(span_estimate_kernel<HD, false>, grid, block, 0, p));
+  }
+  return L.go(span_pick_kernel<HD>, dim3(p.kv_heads, p.B), dim3(kPickThreads), pick_smem(p.max_spans, rows, HD), p);
 }
 // groups of sixteen spans of a warp: one while the blocks are fewer than two per SM, four at most (they share the query's fragments)
 static int select_run(int batch, int kv_heads, int64_t max_spans) {
@@ -205,7 +213,7 @@ int ssdk_select_spans(const void* q, const void* bounds, const int32_t* block_ta
   const int64_t max_spans = (int64_t)max_blocks_per_seq * (block_size / span);
   if (max_spans > kMaxSpans) return fail("select_spans: tables of %lld spans (at most %d)", (long long)max_spans, kMaxSpans);
   const int64_t rows = (int64_t)q_len * (heads / kv_heads);
-  if (rows > 4096 || pick_smem((int)max_spans, rows, head_dim) > kMaxSmem)
+  if (rows > 4096 || pick_smem((int)max_spans, rows, head_dim) > kMaxSmem || estimate_smem(rows, head_dim) > kMaxSmem)
     return fail("select_spans: %lld query rows to a key head beside tables of %lld spans pass the shared memory", (long long)rows, (long long)max_spans);
   SelectParams p;
   p.sub_magic = ((1ull << 32) + block_size / span - 1) / (block_size / span);

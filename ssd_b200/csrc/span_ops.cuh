@@ -42,6 +42,7 @@ constexpr int kPickBins = 1024;    // a multiple of kPickThreads
 constexpr int kPickRanked = 256;   // spans between, up to which each is compared with each
 // rows of the query | scores (64 bits; before them the estimates) | taken | between (a bit per span) | bins, then the spans between
 constexpr int64_t pick_smem(int spans, int64_t rows, int HD) { return (rows + 7) / 8 * 8 * HD * 2 + spans * 8 + 2 * ((spans + 31) / 32) * 4 + kPickBins * 4; }
+constexpr int64_t estimate_smem(int64_t rows, int HD) { return rows > 8 ? (rows + 7) / 8 * 32 * HD : 0; }
 constexpr uint32_t kNoSpan = 0xffffffffu;   // estimate of a span that has no page
 
 // 64-bit values in their order as unsigned words; zeros of both signs are one value, NaN is above all.  0 is no value
@@ -74,7 +75,7 @@ SSDK_DEVINL void pick_write(const uint32_t* bits, int words, int32_t* out, int c
     uint32_t m = w < words ? bits[w] : 0;
     int all, at = pick_running_sum(__popc(m), sums + turn * kPickWarps, &all);
     at += done - __popc(m);
-    for (; m; m &= m - 1) out[at++] = w * 32 + __ffs(m) - 1;
+    for (; m && at < count; m &= m - 1) out[at++] = w * 32 + __ffs(m) - 1;
     done += all;
   }
   for (int i = done + threadIdx.x; i < count; i += kPickThreads) out[i] = -1;
@@ -139,59 +140,74 @@ SSDK_DEVINL const __nv_bfloat16* bounds_at(const SelectParams& p, int page, int 
   return p.bounds + (((size_t)page * subs + (s - sub_page(p, s) * subs)) * p.kv_heads + head) * 2 * HD;
 }
 
-template <int HD>
+// MANY: more than eight rows, whose fragments lie in shared memory
+template <int HD, bool MANY>
 __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(SelectParams p) {
+  extern __shared__ __align__(16) uint2 frags[];   // [tiles][4 CH][32]
   constexpr int CH = HD / 32;   // 16-byte pieces of a lane per bound
   constexpr int W = kEstimateThreads / 32;
   pdl_launch_dependents();
   const int head = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int n = (tokens_of(p.lens, b, p.max_blocks, p.block_size) + p.span - 1) / p.span, groups = (n + 15) / 16;
   if (n <= p.count) return;   // all are listed
-  const int G = p.heads / p.kv_heads, rows = G * p.Q, tiles = (rows + 7) / 8;
+  const int G = p.heads / p.kv_heads, rows = G * p.Q, tiles = (rows + 7) / 8, subs = p.block_size / p.span;
   const int32_t* table = p.tables + (size_t)b * p.max_blocks;
   uint32_t* estimates = p.estimates + ((size_t)b * p.kv_heads + head) * p.max_spans;
-  auto page_of = [&](int s) { return s < n ? page_at(table + sub_page(p, s), p.num_blocks) : -1; };
+  // where the bounds of span s start (in channels; negative: no such span, or on no page)
+  auto place_of = [&](int s) {
+    const int entry = sub_page(p, s), page = s < n ? page_at(table + entry, p.num_blocks) : -1;
+    return page < 0 ? -1ll : (((long long)page * subs + (s - entry * subs)) * p.kv_heads + head) * (2 * HD);
+  };
   // the query's side: row g of a tile, step k of 16 channels: the lane's channels 8 (t + 4 (k / 2)) + 4 (k % 2) .. + 3; lower bounds (k < 2 CH) meet
   // the negative parts, upper bounds the positive ones
-  uint2 qf[4 * CH];
-  auto load_q = [&](int tile) {
+  auto load_q = [&](int tile, uint2* f) {
     const int r = tile * 8 + g;
     const __nv_bfloat16* q = p.q + ((size_t)(b * p.Q + r / G) * p.heads + head * G + r % G) * HD + 8 * t;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const uint4 x = r < rows ? *reinterpret_cast<const uint4*>(q + 32 * i) : make_uint4(0, 0, 0, 0);
-      qf[2 * i] = make_uint2(min_bf16x2(x.x, 0u), min_bf16x2(x.y, 0u));
-      qf[2 * i + 1] = make_uint2(min_bf16x2(x.z, 0u), min_bf16x2(x.w, 0u));
-      qf[2 * CH + 2 * i] = make_uint2(max_bf16x2(x.x, 0u), max_bf16x2(x.y, 0u));
-      qf[2 * CH + 2 * i + 1] = make_uint2(max_bf16x2(x.z, 0u), max_bf16x2(x.w, 0u));
+      f[2 * i] = make_uint2(min_bf16x2(x.x, 0u), min_bf16x2(x.y, 0u));
+      f[2 * i + 1] = make_uint2(min_bf16x2(x.z, 0u), min_bf16x2(x.w, 0u));
+      f[2 * CH + 2 * i] = make_uint2(max_bf16x2(x.x, 0u), max_bf16x2(x.y, 0u));
+      f[2 * CH + 2 * i + 1] = make_uint2(max_bf16x2(x.z, 0u), max_bf16x2(x.w, 0u));
     }
   };
   int group = blockIdx.x * W * p.run + warp;
   const int end = min(groups, (int)(blockIdx.x + 1) * W * p.run);
-  int page0 = page_of(group * 16 + g), page1 = page_of(group * 16 + 8 + g);
-  if (group < end) load_q(0);
+  long long at0 = place_of(group * 16 + g), at1 = place_of(group * 16 + 8 + g);
+  uint2 qf[4 * CH];
+  if (MANY) {   // every tile's fragments into shared memory, a tile per warp
+    for (int tile = warp; tile < tiles; tile += W) {
+      load_q(tile, qf);
+#pragma unroll
+      for (int k = 0; k < 4 * CH; ++k) frags[(tile * 4 * CH + k) * 32 + lane] = qf[k];
+    }
+    __syncthreads();
+  } else if (group < end) {
+    load_q(0, qf);
+  }
   uint32_t bottom = 0, top = 0;   // two channels: smallest lower, largest upper bound
   for (; group < end; group += W) {
     const int s0 = group * 16 + g, s1 = s0 + 8;
-    const __nv_bfloat16 *both0 = bounds_at(p, max(page0, 0), s0, head, HD) + 8 * t, *both1 = bounds_at(p, max(page1, 0), s1, head, HD) + 8 * t;
+    const bool there0 = at0 >= 0, there1 = at1 >= 0;
+    const __nv_bfloat16 *both0 = p.bounds + at0 + 8 * t, *both1 = p.bounds + at1 + 8 * t;
     uint4 u[2 * CH], v[2 * CH];
 #pragma unroll
     for (int i = 0; i < 2 * CH; ++i) {
-      u[i] = page0 >= 0 ? ld_nc_v4(both0 + 32 * i) : make_uint4(0, 0, 0, 0);
-      v[i] = page1 >= 0 ? ld_nc_v4(both1 + 32 * i) : make_uint4(0, 0, 0, 0);
+      u[i] = there0 ? ld_nc_v4(both0 + 32 * i) : make_uint4(0, 0, 0, 0);
+      v[i] = there1 ? ld_nc_v4(both1 + 32 * i) : make_uint4(0, 0, 0, 0);
     }
-    const bool there0 = page0 >= 0, there1 = page1 >= 0;
-    page0 = page_of(s0 + 16 * W);
-    page1 = page_of(s1 + 16 * W);
+    at0 = place_of(s0 + 16 * W);
+    at1 = place_of(s1 + 16 * W);
     float best[2] = {-INFINITY, -INFINITY};   // spans g, g + 8
-    for (int tile = 0; tile < tiles; ++tile) {
-      if (tiles > 1) load_q(tile);
+    for (int tile = 0; tile < (MANY ? tiles : 1); ++tile) {
       float c[2][4] = {};
 #pragma unroll
       for (int i = 0; i < 2 * CH; ++i) {
         const uint32_t a0[4] = {u[i].x, v[i].x, u[i].y, v[i].y}, a1[4] = {u[i].z, v[i].z, u[i].w, v[i].w};
-        mma_bf16_16816(c[0], a0, qf[2 * i].x, qf[2 * i].y);
-        mma_bf16_16816(c[1], a1, qf[2 * i + 1].x, qf[2 * i + 1].y);
+        const uint2 f0 = MANY ? frags[(tile * 4 * CH + 2 * i) * 32 + lane] : qf[2 * i], f1 = MANY ? frags[(tile * 4 * CH + 2 * i + 1) * 32 + lane] : qf[2 * i + 1];
+        mma_bf16_16816(c[0], a0, f0.x, f0.y);
+        mma_bf16_16816(c[1], a1, f1.x, f1.y);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e)
@@ -251,7 +267,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams
     pick_write(taken, (n + 31) / 32, out, p.count, sums);
     return;
   }
-  if (threadIdx.x == 0) q_most = n_sure = n_open = 0;
+  if (threadIdx.x == 0) q_most = n_sure = n_open = pick_bin = 0;
   for (int i = threadIdx.x; i < kPickBins; i += kPickThreads) bins[i] = 0;
   __syncthreads();
   for (int base = warp * 32; base < padded * (HD / 8); base += kPickThreads) {   // (whole warps) the query's rows: 8 channels a thread
@@ -308,12 +324,12 @@ __global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams
   const bool all = want == others, none = want == 0;
   const bool finite = size < 1e38f;
   const float eps2 = size * 0x1p-13f + 0x1p-100f, scale = hi - lo > 1e-30f ? (float)(kPickBins - 1) / (hi - lo) : 0.f;
-  auto bin_of = [&](float x) { return (int)fminf(fmaxf((x - lo) * scale, -1.f), (float)(kPickBins - 1)); };   // (rises with x)
+  auto bin_of = [&](float x) { return (int)fminf(fmaxf((x - lo) * scale, -1.f), (float)(kPickBins - 1)); };   // (rises with x; NaN: -1)
   int line = 0;   // the bin of the want-th largest
   if (!all && !none && finite) {
     for (int s = threadIdx.x; s < n; s += kPickThreads) {
       const uint32_t e = estimate[s];
-      if (e != kNoSpan && !kept(s)) atomicAdd(&bins[bin_of(__uint_as_float(e))], 1);
+      if (e != kNoSpan && !kept(s)) atomicAdd(&bins[max(bin_of(__uint_as_float(e)), 0)], 1);
     }
     __syncthreads();
     constexpr int PER = kPickBins / kPickThreads;   // from the top, each thread some bins
