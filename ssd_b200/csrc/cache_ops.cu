@@ -30,15 +30,17 @@ static int check_spans(const char* who, int heads, int kv_heads, int head_dim, i
   if (span < 16 || span % 16 || block_size % span) return fail("%s: spans of %d tokens (multiples of 16 that divide pages of %d)", who, span, block_size);
   return 0;
 }
-// the attributes that a kernel needs, once per device
+// The attributes that a kernel needs, once per device.  The large carve-out is for kernels whose blocks are to share an SM: loads into registers wait in the cache
+// that it takes (span_estimate_kernel for sixteen rows, 24 contexts of 64000: 67 us with it, 37 without).
+enum { kSmemOnly = 0, kSmemCarveout = 1, kSmemClusters = 3 };
 template <typename Kernel>
-static int with_smem(Kernel* kernel, int bytes, std::atomic<bool>* done, bool wide_clusters = false) {
+static int with_smem(Kernel* kernel, int bytes, int what, std::atomic<bool>* done) {
   int dev = 0;
   CK(cudaGetDevice(&dev));
   if (dev < 64 && done[dev].load(std::memory_order_acquire)) return 0;
   CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  CK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-  if (wide_clusters) CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  if (what & 1) CK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  if (what & 2) CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   if (dev < 64) done[dev].store(true, std::memory_order_release);
   return 0;
 }
@@ -63,14 +65,14 @@ static int span_cluster(int64_t units, int64_t keys, int most) {
 template <int HD>
 static int launch_span_attn(Launcher& L, const SpanAttnParams& p) {
   static std::atomic<bool> done[64];
-  CKI(with_smem(span_attn_kernel<HD>, span_attn_smem(HD, kMaxListed), done, true));
+  CKI(with_smem(span_attn_kernel<HD>, span_attn_smem(HD, kMaxListed), kSmemClusters, done));
   L.cluster = span_cluster((int64_t)p.B * p.kv_heads, (int64_t)p.count * p.span, kSpanMost);
   return L.go(span_attn_kernel<HD>, dim3(p.kv_heads * L.cluster, p.B), dim3(kSpanWarps * 32), span_attn_smem(HD, p.count), p);
 }
 template <int HD>
 static int launch_span_tiles(Launcher& L, SpanAttnParams p) {
   static std::atomic<bool> done[64];
-  CKI(with_smem(span_tile_kernel<HD>, span_tile_smem(HD, kMaxListed), done, true));
+  CKI(with_smem(span_tile_kernel<HD>, span_tile_smem(HD, kMaxListed), kSmemClusters, done));
   WaitWord* waits = op_waits();
   if (!waits) return fail("span_attn: pinned word for bounded waits not allocated");
   CKI(waits->check("an earlier call of attention without an engine left is not complete (NaN rows)"));
@@ -102,14 +104,14 @@ static int launch_rope_axes(Launcher& L, RopeAxesParams p) {
 template <int HD>
 static int launch_select(Launcher& L, const SelectParams& p) {
   static std::atomic<bool> done[64];
-  CKI(with_smem(span_pick_kernel<HD>, kMaxSmem, done));
+  CKI(with_smem(span_pick_kernel<HD>, kMaxSmem, kSmemOnly, done));
   L.pdl = true;
   constexpr int W = kEstimateThreads / 32;
   const int64_t rows = (int64_t)p.Q * (p.heads / p.kv_heads);
   const dim3 grid(p.warps / W, p.kv_heads, p.B), block(kEstimateThreads);
   if (rows > 8) {
     static std::atomic<bool> many_done[64];
-    CKI(with_smem(span_estimate_kernel<HD, true>, kMaxSmem, many_done));
+    CKI(with_smem(span_estimate_kernel<HD, true>, kMaxSmem, kSmemOnly, many_done));
     CKI(L.go(span_estimate_kernel<HD, true>, grid, block, estimate_smem(rows, HD), p));
   } else {
     CKI(L.go(span_estimate_kernel<HD, false>, grid, block, 0, p));
@@ -140,7 +142,7 @@ int ssdk_place_tokens(const int32_t* context_lens, const int32_t* new_lens, int3
   Launcher L;
   L.st = (cudaStream_t)stream;
   static std::atomic<bool> done[64];
-  if (place_smem(batch) > 48000) CKI(with_smem(place_tokens_kernel, place_smem(kPlaceMaxSeqs), done));
+  if (place_smem(batch) > 48000) CKI(with_smem(place_tokens_kernel, place_smem(kPlaceMaxSeqs), kSmemOnly, done));
   return L.go(place_tokens_kernel, dim3(std::min((rows + kPlaceThreads - 1) / kPlaceThreads, 148)), dim3(kPlaceThreads), place_smem(batch), p);
 }
 

@@ -19,8 +19,8 @@ namespace ssdk {
 // size lost.  With t the want-th largest estimate, a span above t + 2 eps is taken, one under t - 2 eps is not, and span_pick_kernel scores only the few
 // in between in 64 bits (products of bf16 values are exact, sums of 128 of them off by 2^-46).  Where values are not finite, or so large that 32 bits
 // overflow, it scores all.
-// Two kernels, the second's start under the first's end: with one, whose first block of a cluster picks, what was left of the blocks in a second wave
-// and the picking blocks held the SMs while the memory idled (24 contexts of 64000: 82 us, 47.7 with two).
+// Two kernels, the second's start under the first's end: the estimates fill all SMs in even shares whatever the number of heads, and what picks is one block
+// of a head.  24 contexts of 64000 tokens (150 MB of bounds): 34 us and 8 us.
 // ----------------------------------------------------------------------------------
 struct SelectParams {
   const __nv_bfloat16* q;        // [B * Q, H, hd]
@@ -289,16 +289,22 @@ __global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams
   int always = 0, others = 0;
   uint32_t lowest = ~0u, highest = 0, wide = 0;
   for (int i = threadIdx.x; i < p.warps; i += kPickThreads) wide = max(wide, __ldcg(p.wide + ((size_t)b * p.kv_heads + head) * p.warps + i));
-  for (int s = threadIdx.x; s < n; s += kPickThreads) {
-    const uint32_t e = __ldcg(p.estimates + ((size_t)b * p.kv_heads + head) * p.max_spans + s);
-    estimate[s] = e;
-    if (e == kNoSpan) continue;
-    if (kept(s)) {
-      ++always;
-    } else {
-      ++others;
-      lowest = min(lowest, order_of(e));
-      highest = max(highest, order_of(e));
+  const uint32_t* estimates = p.estimates + ((size_t)b * p.kv_heads + head) * p.max_spans;
+  for (int base = threadIdx.x; base < n; base += 4 * kPickThreads) {   // four at a time
+    uint32_t e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = base + i * kPickThreads < n ? __ldcg(estimates + base + i * kPickThreads) : kNoSpan;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = base + i * kPickThreads;
+      if (s < n) estimate[s] = e[i];
+      const bool there = e[i] != kNoSpan, keep = kept(s);
+      always += there && keep;
+      others += there && !keep;
+      if (there && !keep) {
+        lowest = min(lowest, order_of(e[i]));
+        highest = max(highest, order_of(e[i]));
+      }
     }
   }
   always = __reduce_add_sync(0xffffffffu, always);
@@ -327,6 +333,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams
   auto bin_of = [&](float x) { return (int)fminf(fmaxf((x - lo) * scale, -1.f), (float)(kPickBins - 1)); };   // (rises with x; NaN: -1)
   int line = 0;   // the bin of the want-th largest
   if (!all && !none && finite) {
+#pragma unroll 4
     for (int s = threadIdx.x; s < n; s += kPickThreads) {
       const uint32_t e = estimate[s];
       if (e != kNoSpan && !kept(s)) atomicAdd(&bins[max(bin_of(__uint_as_float(e)), 0)], 1);
