@@ -45,6 +45,16 @@ static int with_smem(Kernel* kernel, int bytes, int what, std::atomic<bool>* don
   return 0;
 }
 
+// Every kernel here may be scheduled under the end of the one in front (whatever it is): it touches no global memory before griddepcontrol.wait, and lets its own
+// successor be scheduled only behind that wait.  (So span_pick_kernel may read before its wait what span_estimate_kernel, right in front of it, waited for.)  us a call, back to back
+// on one stream, without and with: 4003 rows rotated 22.5 -> 20.7, four prompts' bounds 25.6 -> 24.3, 24 selections 44.4 -> 40.0, 8 x 7 rows' attention 38.0 -> 36.8.
+static Launcher launcher(void* stream) {
+  Launcher L;
+  L.st = (cudaStream_t)stream;
+  L.pdl = L.prev_kernel = true;
+  return L;
+}
+
 constexpr int kSms = 148, kMaxSmem = 227 * 1024 - 1024;   // (statics beside it)
 constexpr int kMaxListed = 4096;   // spans of a list
 // Blocks that share the listed keys of a key head (a cluster).  Two blocks are resident on an SM, so that units x blocks take waves; a block's start and end
@@ -105,7 +115,6 @@ template <int HD>
 static int launch_select(Launcher& L, const SelectParams& p) {
   static std::atomic<bool> done[64];
   CKI(with_smem(span_pick_kernel<HD>, kMaxSmem, kSmemOnly, done));
-  L.pdl = true;
   constexpr int W = kEstimateThreads / 32;
   const int64_t rows = (int64_t)p.Q * (p.heads / p.kv_heads);
   const dim3 grid(p.warps / W, p.kv_heads, p.B), block(kEstimateThreads);
@@ -139,8 +148,7 @@ int ssdk_place_tokens(const int32_t* context_lens, const int32_t* new_lens, int3
   p.ctx = context_lens; p.fresh = new_lens; p.tables = block_tables; p.free_blocks = free_blocks; p.free_used = free_used;
   p.positions = positions; p.slots = slot_mapping; p.seqs = row_seqs; p.cu = cu_rows; p.lens = lens; p.used = used;
   p.B = batch; p.max_blocks = max_blocks_per_seq; p.n_free = n_free; p.rows = rows; p.block_size = block_size; p.num_blocks = (int)num_blocks;
-  Launcher L;
-  L.st = (cudaStream_t)stream;
+  Launcher L = launcher(stream);
   static std::atomic<bool> done[64];
   if (place_smem(batch) > 48000) CKI(with_smem(place_tokens_kernel, place_smem(kPlaceMaxSeqs), kSmemOnly, done));
   return L.go(place_tokens_kernel, dim3(std::min((rows + kPlaceThreads - 1) / kPlaceThreads, 148)), dim3(kPlaceThreads), place_smem(batch), p);
@@ -167,8 +175,7 @@ int ssdk_rope_axes_store_kv(const void* qkv, const int64_t* positions, int axes,
   p.q_norm_w = (const bf16*)q_norm_w; p.k_norm_w = (const bf16*)k_norm_w; p.eps = norm_eps;
   p.q = (bf16*)q_out; p.k_cache = (bf16*)k_cache; p.v_cache = (bf16*)v_cache;
   p.top = max_pos; p.num_slots = num_slots; p.M = M; p.heads = heads; p.kv_heads = kv_heads; p.rot = rot_dim; p.axes = axes;
-  Launcher L;
-  L.st = (cudaStream_t)stream;
+  Launcher L = launcher(stream);
   if (head_dim == 64) return launch_rope_axes<64>(L, p);
   if (head_dim == 128) return launch_rope_axes<128>(L, p);
   return launch_rope_axes<256>(L, p);
@@ -190,8 +197,7 @@ int ssdk_span_bounds(const void* k_cache, const int32_t* block_tables, const int
   p.width = cols >= 32 ? 32 : cols >= 16 ? 16 : 8;
   const int64_t units = (((int64_t)p.fresh + span - 2) / span + 1) * ((cols + p.width - 1) / p.width);
   if (units >= (1ll << 31) - 8) return fail("span_bounds: %d new tokens of %d heads", new_tokens, kv_heads);
-  Launcher L;
-  L.st = (cudaStream_t)stream;
+  Launcher L = launcher(stream);
   // a block to a span's columns while the blocks fit the SMs at once, else a warp
   if (units * batch <= 8 * kSms) return L.go(span_bounds_kernel<true>, dim3((unsigned)units, batch), dim3(kBoundsThreads), 0, p);
   return L.go(span_bounds_kernel<false>, dim3((unsigned)((units + kBoundsThreads / 32 - 1) / (kBoundsThreads / 32)), batch), dim3(kBoundsThreads), 0, p);
@@ -225,8 +231,7 @@ int ssdk_select_spans(const void* q, const void* bounds, const int32_t* block_ta
   p.count = count; p.first = first; p.last = last;
   p.run = select_run(batch, kv_heads, max_spans); p.warps = select_warps(max_spans, p.run);
   p.estimates = (uint32_t*)scratch; p.wide = p.estimates + (size_t)batch * kv_heads * max_spans;
-  Launcher L;
-  L.st = (cudaStream_t)stream;
+  Launcher L = launcher(stream);
   return head_dim == 64 ? launch_select<64>(L, p) : launch_select<128>(L, p);
 }
 
@@ -245,8 +250,7 @@ int ssdk_span_attn(const void* q, const void* k_cache, const void* v_cache, cons
   p.spans = selected; p.out = (bf16*)out; p.num_blocks = num_blocks; p.B = batch; p.Q = q_len; p.heads = heads; p.kv_heads = kv_heads;
   p.block_size = block_size; p.span = span; p.max_blocks = max_blocks_per_seq; p.count = count; p.scale_log2 = scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f;
   p.q_sign = scale < 0.f ? 0x80008000u : 0u; p.q_keep = scale == 0.f ? 0u : ~0u;
-  Launcher L;
-  L.st = (cudaStream_t)stream;
+  Launcher L = launcher(stream);
   if (G * (int64_t)q_len <= 16) return head_dim == 64 ? launch_span_attn<64>(L, p) : launch_span_attn<128>(L, p);
   return head_dim == 64 ? launch_span_tiles<64>(L, p) : launch_span_tiles<128>(L, p);
 }

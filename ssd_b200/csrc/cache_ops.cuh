@@ -64,6 +64,8 @@ SSDK_DEVINL long long block_running_sum(long long v, long long* part, long long*
 
 __global__ void __launch_bounds__(kPlaceThreads) place_tokens_kernel(PlaceParams p) {
   SSDK_DYN_SMEM(int32_t, place_words);
+  pdl_wait();
+  pdl_launch_dependents();
   SSDK_STATIC_SMEM(long long, part, kPlaceThreads / 32);
   SSDK_STATIC_SMEM(int, most, 2);   // pages and rows of all that is placed
   int32_t* cu = place_words;                // [B + 1] first row of a sequence
@@ -187,6 +189,8 @@ SSDK_DEVINL uint4 bf16_of(const uint64_t* f) {
 template <int HD, bool NORM>
 __global__ void __launch_bounds__(kRopeAxesThreads, 4) rope_axes_kernel(RopeAxesParams p) {
   constexpr int LPH = HD / 16, SIDE = 32 / LPH;   // lanes of a head, heads side by side
+  pdl_wait();
+  pdl_launch_dependents();
   const int unit = (int)blockIdx.x * (kRopeAxesThreads / 32) + (int)(threadIdx.x >> 5);   // (below 2^31: the host sees to it)
   const int m = unit / p.shares, share = unit - m * p.shares;
   if (m >= p.M) return;
@@ -347,6 +351,8 @@ SSDK_DEVINL uint4 shfl_xor_16(const uint4& v, int o) {
 template <bool SPLIT>
 __global__ void __launch_bounds__(kBoundsThreads, 4) span_bounds_kernel(SpanBoundsParams p) {
   constexpr int WARPS = kBoundsThreads / 32;
+  pdl_wait();
+  pdl_launch_dependents();
   const int b = blockIdx.y;
   const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size);
   const int row = p.kv_heads * p.head_dim, slices = (row / 8 + p.width - 1) / p.width;   // columns of a warp: p.width

@@ -146,6 +146,7 @@ __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(Sele
   extern __shared__ __align__(16) uint2 frags[];   // [tiles][4 CH][32]
   constexpr int CH = HD / 32;   // 16-byte pieces of a lane per bound
   constexpr int W = kEstimateThreads / 32;
+  pdl_wait();
   pdl_launch_dependents();
   const int head = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int n = (tokens_of(p.lens, b, p.max_blocks, p.block_size) + p.span - 1) / p.span, groups = (n + 15) / 16;
@@ -258,6 +259,8 @@ __global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams
   int32_t* out = p.out + ((size_t)b * p.kv_heads + head) * p.count;
 
   if (n <= p.count) {   // all of them
+    pdl_wait();
+    pdl_launch_dependents();
     for (int base = warp * 32; base < n; base += kPickThreads) {
       const int s = base + lane;
       const uint32_t m = __ballot_sync(0xffffffffu, s < n && page_at(table + sub_page(p, s), p.num_blocks) >= 0);
@@ -283,7 +286,8 @@ __global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams
     const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(size));   // (NaN above infinity above all)
     if (lane == 0) atomicMax(&q_most, most);
   }
-  pdl_wait();   // the estimates are there
+  pdl_wait();   // the estimates are there (what is read above was there before they began: see launcher())
+  pdl_launch_dependents();
 
   auto kept = [&](int s) { return s < p.first || s >= n - p.last; };
   int always = 0, others = 0;
@@ -466,6 +470,8 @@ template <int HD>
 __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnParams p) {
   constexpr int LDS = HD + 8, KS = HD / 16, ND = HD / 8, SEG = HD / 8;
   extern __shared__ __align__(16) uint8_t span_smem[];
+  pdl_wait();
+  pdl_launch_dependents();
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank();

@@ -72,6 +72,8 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     s_failed = 0;
   }
   if (warp == 1) { tmem_alloc(&tmem_slot, 256); tmem_relinquish(); }
+  pdl_wait();
+  pdl_launch_dependents();
   // the spans that are there, in the list's order
   const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size);
   int spans = 0;
