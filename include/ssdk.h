@@ -205,6 +205,8 @@ int ssdk_debug_trace(void* dev_buf, int cap);
 /* Host word that this engine's kernels set when one of their bounded waits runs out.  Every call that waits for the stream fails
  * once (and clears it) if it is set. */
 uint32_t* ssdk_debug_wait_word(ssdk_handle h);
+/* The same of the calls without an engine (paged attention and attention over spans, on tiles): the next such call fails once. */
+uint32_t* ssdk_debug_op_wait_word(void);
 /* number of kernels this library launched (or replayed inside graphs) so far */
 int64_t ssdk_launch_count(ssdk_handle h);
 
@@ -313,7 +315,9 @@ int ssdk_select_spans(const void* q, const void* bounds, const int32_t* block_ta
                       void* scratch, int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size,
                       int max_blocks_per_seq, int64_t num_blocks, int span, int count, int first, int last, void* stream);
 /* ssdk_span_attn: ssdk_paged_attn over the keys of the listed spans only.  Entries outside the context, or on pages outside the cache, are
- * passed over; a span that is listed twice counts twice; a row that sees no key is zero.  At most 32 query heads to a key head, 4096 spans. */
+ * passed over; a span that is listed twice counts twice; a row that sees no key is zero.  At most 32 query heads to a key head, 4096 spans.
+ * More than sixteen query rows to a key head take a kernel with bounded waits: as with ssdk_paged_attn_pages, a wait that runs out leaves NaN
+ * rows, and the next such call of the process returns an error. */
 int ssdk_span_attn(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables, const int32_t* context_lens,
                    const int32_t* selected, void* out, int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size,
                    int max_blocks_per_seq, int64_t num_blocks, int span, int count, float scale, void* stream);

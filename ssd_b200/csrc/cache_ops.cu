@@ -136,12 +136,17 @@ static int select_warps(int64_t max_spans, int run) { return (int)((max_spans + 
 
 extern "C" {
 
+uint32_t* ssdk_debug_op_wait_word(void) {
+  WaitWord* waits = op_waits();
+  return waits ? waits->word : nullptr;
+}
+
 int ssdk_place_tokens(const int32_t* context_lens, const int32_t* new_lens, int32_t* block_tables, const int32_t* free_blocks,
                       const int32_t* free_used, int64_t* positions, int32_t* slot_mapping, int32_t* row_seqs, int32_t* cu_rows,
                       int32_t* lens, int32_t* used, int batch, int max_blocks_per_seq, int n_free, int rows, int block_size,
                       int64_t num_blocks, void* stream) {
   CKI(check_pages("place_tokens", batch, block_size, max_blocks_per_seq, num_blocks));
-  if (batch > kPlaceMaxSeqs || rows < 1 || n_free < 0) return fail("place_tokens: %d sequences (at most %d), %d rows, %d free pages", batch, kPlaceMaxSeqs, rows, n_free);
+  if (batch > kPlaceMaxSeqs || rows < 1 || rows > (1 << 30) || n_free < 0) return fail("place_tokens: %d sequences (at most %d), %d rows, %d free pages", batch, kPlaceMaxSeqs, rows, n_free);
   if (!context_lens || !new_lens || !block_tables || !free_used || (n_free && !free_blocks) || !positions || !slot_mapping || !row_seqs || !cu_rows || !lens || !used)
     return fail("place_tokens: null argument");
   PlaceParams p;
@@ -216,6 +221,7 @@ int ssdk_select_spans(const void* q, const void* bounds, const int32_t* block_ta
   CKI(check_spans("select_spans", heads, kv_heads, head_dim, block_size, span));
   if (q_len < 1 || count < 1 || count > kMaxListed || first < 0 || last < 0 || (int64_t)first + last > count)
     return fail("select_spans: q_len=%d, %d spans (at most %d), of them the first %d and the last %d", q_len, count, kMaxListed, first, last);
+  if ((int64_t)batch * q_len >= (1ll << 31)) return fail("select_spans: %d rows of %d sequences", q_len, batch);
   if (!q || !bounds || !block_tables || !context_lens || !selected || !scratch) return fail("select_spans: null argument");
   if (off16(q, bounds, scratch)) return fail("select_spans: arrays must start at multiples of 16 bytes");
   const int64_t max_spans = (int64_t)max_blocks_per_seq * (block_size / span);
@@ -243,6 +249,7 @@ int ssdk_span_attn(const void* q, const void* k_cache, const void* v_cache, cons
   const int G = heads / kv_heads;
   if (q_len < 1 || count < 1 || count > kMaxListed || G > 32 || !(scale == scale))
     return fail("span_attn: q_len=%d, %d spans (at most %d), %d query heads to a key head (at most 32)", q_len, count, kMaxListed, G);
+  if ((int64_t)count * span >= (1ll << 31) || (int64_t)batch * q_len >= (1ll << 31)) return fail("span_attn: %d spans of %d tokens, %d rows of %d sequences", count, span, q_len, batch);
   if (!q || !k_cache || !v_cache || !block_tables || !context_lens || !selected || !out) return fail("span_attn: null argument");
   if (off16(q, k_cache, v_cache, out)) return fail("span_attn: arrays must start at multiples of 16 bytes");
   SpanAttnParams p;

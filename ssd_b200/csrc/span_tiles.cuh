@@ -18,6 +18,7 @@
 namespace ssdk {
 
 constexpr int kTileRows64 = 64, kTileKeys = 64, kTileStages = 2, kTileThreads = 224;   // warps: loads, scores, 4 of softmax, products with V
+constexpr int kNoPosition = 0x7fffff00;   // of a key that is not there: behind every context
 constexpr int kTileMost = 16;   // blocks of a cluster
 // query twice | keys and values; behind them the places of the listed spans
 constexpr int span_tile_body(int HD) { return 2 * kTileRows64 * HD * 2 + kTileStages * 2 * kTileKeys * HD * 2; }
@@ -112,7 +113,7 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   const int first = rank * share, n = max(0, min(share, chunks - first));
   // slot and position of a box: behind the last one no keys
   auto box_at = [&](int piece) {
-    if (piece >= pieces) return make_int2((int)(p.num_blocks * p.block_size), 1 << 30);
+    if (piece >= pieces) return make_int2((int)(p.num_blocks * p.block_size), kNoPosition);
     const int i = piece / per, off = (piece - i * per) * box;
     const int2 at = where[i];
     return make_int2(at.x + off, at.y + off);
@@ -253,7 +254,7 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (!whole) {   // slots behind the context hold anything, and 0 x NaN is NaN
         bool stale = false;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) stale = stale || (pos[j] < (1 << 29) && pos[j] + 16 > len);
+        for (int j = 0; j < 4; ++j) stale = stale || (pos[j] < kNoPosition && pos[j] + 16 > len);
         if (stale) {   // (the same for all warps)
           if (!(ok = tile_wait_warp(&v_full[i & 1], parity(i), timeout))) break;
           for (int j = second ? half + r : r; j < kTileKeys * 8; j += live) {

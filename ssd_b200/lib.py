@@ -130,6 +130,7 @@ SIGNATURES: dict[str, tuple] = {
     "ssdk_logits_last": (VP, [VP]),
     "ssdk_debug_trace": (C.c_int, [VP, C.c_int]),
     "ssdk_debug_wait_word": (C.POINTER(C.c_uint32), [VP]),
+    "ssdk_debug_op_wait_word": (C.POINTER(C.c_uint32), []),
     "ssdk_launch_count": (C.c_int64, [VP]),
     "ssdk_gemm_small_m": (C.c_int, [VP, VP, VP, VP, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, VP]),
     "ssdk_gemm_gate_up_silu": (C.c_int, [VP, VP, VP, C.c_int, C.c_int, C.c_int, VP]),

@@ -248,7 +248,8 @@ def rope_axes_store_kv(qkv: torch.Tensor, positions: torch.Tensor, axis_of, slot
     outside the table has NaN queries and stores nothing; slots are distinct, those outside the cache store nothing."""
     M, rot, axes = qkv.shape[0], rope_table.shape[-1], positions.shape[0]
     cache = torch.Size((*k_cache.shape[:2], kv_heads, head_dim))
-    axis_of = bytes(axis_of)
+    if type(axis_of) is not bytes:
+        axis_of = bytes(list(axis_of))
     if len(axis_of) * 2 != rot:
         raise ValueError(f"rope_axes_store_kv: axis_of has {len(axis_of)} frequencies, rope_table {rot / 2}")
     args = [(qkv, "qkv", _BF, (M, (heads + 2 * kv_heads) * head_dim)), (positions, "positions", _I64, (axes, M)), (slot_mapping, "slot_mapping", _I32, (M,)),
@@ -277,7 +278,7 @@ def span_bounds(bounds: torch.Tensor, k_cache: torch.Tensor, block_tables: torch
         raise ValueError(f"span_bounds: pages of {block_size} tokens in {subs} spans")
     gpu = _check("span_bounds", (bounds, "bounds", _BF, (n, subs, KV, 2, hd)), (k_cache, "k_cache", _BF, (n, block_size, KV, hd)),
                  (block_tables, "block_tables", _I32, (B, width)), (context_lens, "context_lens", _I32, (B,)))
-    _launch("ssdk_span_bounds", gpu, k_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), bounds.data_ptr(), B, new_tokens, KV, hd,
+    _launch("ssdk_span_bounds", gpu, k_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), bounds.data_ptr(), B, min(new_tokens, 2 ** 31 - 1), KV, hd,
             block_size, width, n, block_size // subs)
     return bounds
 
@@ -291,7 +292,7 @@ def select_spans(q: torch.Tensor, bounds: torch.Tensor, block_tables: torch.Tens
     q [B * q_len, H, hd] bf16 (rotated); bounds as span_bounds keeps them.  Returns int32 [B, KV, count], ascending, -1 behind the
     last: what span_attention takes.  The rows of a sequence share their spans."""
     n, subs, KV, _, hd = bounds.shape if bounds.dim() == 5 else (-1,) * 5
-    B, width, H = _last(context_lens, 1), _last(block_tables, 2), q.shape[1]
+    B, width, H = _last(context_lens, 1), _last(block_tables, 2), q.shape[1] if q.dim() == 3 else -1
     if subs == 0 or block_size % subs:
         raise ValueError(f"select_spans: pages of {block_size} tokens in {subs} spans")
     gpu = _check("select_spans", (q, "q", _BF, (B * q_len, H, hd)), (bounds, "bounds", _BF, (n, subs, KV, 2, hd)),
@@ -313,7 +314,7 @@ def span_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     q [B * q_len, H, hd]; returns [B * q_len, H * hd].  Entries outside the context are passed over, a span listed twice counts twice, a row
     that sees no key is zero."""
     n, block_size, KV, hd = cache = k_cache.shape if k_cache.dim() == 4 else (-1,) * 4
-    B, width, H, count = _last(context_lens, 1), _last(block_tables, 2), q.shape[1], _last(spans, 3)
+    B, width, H, count = _last(context_lens, 1), _last(block_tables, 2), q.shape[1] if q.dim() == 3 else -1, _last(spans, 3)
     gpu = _check("span_attention", (q, "q", _BF, (B * q_len, H, hd)), (k_cache, "k_cache", _BF, cache), (v_cache, "v_cache", _BF, cache),
                  (block_tables, "block_tables", _I32, (B, width)), (context_lens, "context_lens", _I32, (B,)), (spans, "spans", _I32, (B, KV, count)))
     out = q.new_empty(B * q_len, H * hd)

@@ -152,6 +152,10 @@ def test_refusals_of_types_and_shapes():
         ops.rope_axes_store_kv(**_rope_args(axis_of=[0] * 31))
     with pytest.raises(ValueError):
         ops.rope_axes_store_kv(**_rope_args(axis_of=[-1] * 32))
+    with pytest.raises(TypeError):
+        ops.rope_axes_store_kv(**_rope_args(axis_of=32))
+    with pytest.raises(ValueError, match="axis_of"):
+        ops.rope_axes_store_kv(**_rope_args(axis_of=np.zeros(4, dtype=np.int64)))   # (its bytes would be 32)
     with pytest.raises(ValueError, match="qkv"):
         ops.rope_axes_store_kv(**_rope_args(heads=3))
     with pytest.raises(ValueError, match="v_cache"):
@@ -164,6 +168,8 @@ def test_refusals_of_types_and_shapes():
         ops.span_bounds(**_of(a, *names[1:], bounds=torch.zeros(4, 2, 2, 64, dtype=BF), new_tokens=1))
     with pytest.raises(ValueError, match="spans"):
         ops.span_bounds(**_of(a, *names[1:], bounds=torch.zeros(4, 3, 2, 2, 64, dtype=BF), new_tokens=1))
+    with pytest.raises(ValueError, match="q"):
+        ops.select_spans(torch.zeros(8, dtype=BF), **_of(a, "bounds", "block_tables", "context_lens", q_len=1, block_size=32, count=3))
     with pytest.raises(ValueError, match="q"):
         ops.select_spans(**_of(a, "q", "bounds", "block_tables", "context_lens", q_len=2, block_size=32, count=3))
     with pytest.raises(ValueError, match="spans"):
@@ -189,7 +195,7 @@ P = 4096   # an address that no call below gets to use
 @pytest.mark.parametrize("name,good,bad", [
     # (index of an argument, value) that an entry point refuses before it touches the device
     ("ssdk_place_tokens", [P] * 11 + [2, 4, 8, 4, 16, 8, None],
-     [(0, None), (3, None), (10, None), (11, 0), (11, 20000), (12, 0), (13, -1), (14, 0), (15, 0), (16, 0), (12, 1 << 28), (16, 1 << 28)]),
+     [(0, None), (3, None), (10, None), (11, 0), (11, 20000), (12, 0), (13, -1), (14, 0), (15, 0), (16, 0), (12, 1 << 28), (16, 1 << 28), (14, (1 << 30) + 1)]),
     ("ssdk_rope_axes_store_kv", [P, P, 2, bytes(32), P, P, 10, 64, None, None, 1e-6, P, P, P, 32, 3, 2, 1, 64, None],
      [(0, None), (1, None), (2, 0), (2, 5), (3, None), (3, bytes([2] * 32)), (6, 0), (7, 8), (7, 24), (7, 80), (0, P + 2), (8, P + 8), (14, 0), (15, 0), (16, 0), (17, 0), (18, 96)]),
     ("ssdk_span_bounds", [P, P, P, P, 2, 1, 2, 64, 32, 2, 4, 16, None],

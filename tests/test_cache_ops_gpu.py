@@ -89,6 +89,25 @@ def test_rope_axes_store_kv(dev, M, H, KV, hd, rot, axes, norm, turns):
     assert torch.equal(vc.double().cpu(), wv)
 
 
+def test_rope_axes_many_rows(dev):
+    """More rows than warps: a warp has all heads of its row."""
+    from ssd_b200 import ops
+    g = gen(31)
+    M, H, KV, hd, rot, axes, S = 3001, 20, 5, 64, 64, 3, 64
+    qkv = torch.randn(M, (H + 2 * KV) * hd, generator=g).to(BF)
+    positions = torch.randint(0, 200, (axes, M), generator=g)
+    slots = torch.randperm(50 * S, generator=g)[:M].to(torch.int32)
+    w = (1 + 0.2 * torch.randn(2, hd, generator=g)).to(BF)
+    table, axis_of = angles(200, rot), [0] * 8 + [1] * 13 + [2] * 11
+    kc, vc = torch.zeros(2, 50, S, KV, hd, dtype=BF, device=dev)
+    q = ops.rope_axes_store_kv(qkv.to(dev), positions.to(dev), axis_of, slots.to(dev), table.to(dev), kc, vc, H, KV, hd, w[0].to(dev), w[1].to(dev))
+    zero = torch.zeros(50, S, KV, hd, dtype=BF)
+    wq, wk, wv, slack_q, slack_k = plain.rope(qkv, positions, axis_of, slots, table, zero, zero, H, KV, hd, w[0], w[1], 1e-6)
+    within(q, wq, slack_q)
+    within(kc, wk, slack_k)
+    assert torch.equal(vc.double().cpu(), wv)
+
+
 def test_rope_axes_passes_what_does_not_turn(dev):
     """Channels behind rot_dim keep their bits, infinities among them; a norm on one side only."""
     from ssd_b200 import ops
@@ -120,12 +139,14 @@ def _same(a, b):
 
 @pytest.mark.parametrize("KV,hd,S,span,new,lens", [
     (8, 128, 256, 32, 1, [1, 31, 32, 33, 255, 256, 257, 1000]), (8, 128, 256, 32, 1000, [1000, 5, 0]), (1, 64, 64, 16, 7, [64, 70, 3]), (5, 128, 16, 16, 40, [33, 16, 100]),
+    (8, 128, 256, 32, 16000, [16000, 9001, 77]), (1, 64, 64, 16, 64000, [64000]), (5, 128, 64, 16, 9000, [9000, 8100]), (5, 64, 128, 64, 20000, [20000, 19999]), (2, 64, 32, 32, 40000, [40000]),
     (2, 64, 128, 128, 1, [1, 128, 129, 384]), (20, 128, 32, 32, 9, [40, 41]), (8, 64, 256, 64, 300, [-5, 768, 100000]), (1, 128, 16, 16, 1 << 30, [48]),
 ])
 def test_span_bounds(dev, KV, hd, S, span, new, lens):
     from ssd_b200 import ops
     g = gen(KV, hd, S, span, new)
-    table, total = tables(g, [min(max(n, 0), 4 * S) for n in lens], S, width=4)
+    width = 4 if max(lens) < 5000 or max(lens) == 100000 else -(-max(lens) // S)
+    table, total = tables(g, [min(max(n, 0), width * S) for n in lens], S, width=width)
     if len(lens) > 2:
         table[0, 0] = total       # outside the cache
         table[1, 0] = -5
@@ -172,6 +193,17 @@ def test_select_spans_long(dev, n, count, first, last):
     table, total = tables(g, lens, S)
     q = torch.randn(2, 4, hd, generator=g).to(BF)
     _select(dev, q, _bounds(g, total, S // span, KV, hd), table, lens, 1, S, count, first, last)
+
+
+@pytest.mark.parametrize("q_len,count", [(1, 40), (3, 7)])
+def test_select_spans_batch(dev, q_len, count):
+    """Enough sequences that a warp has several groups of spans, of very uneven lengths."""
+    g = gen(17, q_len)
+    S, span, KV, hd, H = 64, 16, 8, 64, 32
+    lens = [max(q_len, (i * 2477) % 9600) for i in range(24)] + [9600, q_len]
+    table, total = tables(g, lens, S)
+    q = torch.randn(len(lens) * q_len, H, hd, generator=g).to(BF)
+    _select(dev, q, _bounds(g, total, S // span, KV, hd), table, lens, q_len, S, count)
 
 
 def test_select_spans_ties_and_odd_values(dev):
@@ -269,6 +301,40 @@ def test_span_attention_long(dev, count, q_len, H, KV, hd):
     kc, vc = torch.randn(2, total, S, KV, hd, generator=g).to(BF)
     q = (3 * torch.randn(2 * q_len, H, hd, generator=g)).to(BF)
     _attend(dev, q, kc, vc, table, lens, _lists(g, lens, KV, span, count), span, q_len, hd ** -0.5)
+
+
+@pytest.mark.parametrize("B,H,KV,hd,q_len", [(40, 16, 8, 64, 1), (70, 8, 8, 128, 2), (33, 32, 4, 64, 3)])
+def test_span_attention_batch(dev, B, H, KV, hd, q_len):
+    """Batches that fill the SMs with a block per key head."""
+    g = gen(B, H, q_len)
+    S, span, count = 32, 16, 3
+    lens = [q_len + (i * 37) % 90 for i in range(B)]
+    table, total = tables(g, lens, S)
+    kc, vc = torch.randn(2, total, S, KV, hd, generator=g).to(BF)
+    q = torch.randn(B * q_len, H, hd, generator=g).to(BF)
+    _attend(dev, q, kc, vc, table, lens, _lists(g, lens, KV, span, count), span, q_len, hd ** -0.5)
+
+
+def test_span_attention_many_rows_stale_and_odd(dev):
+    """The same for more than sixteen rows to a key head: stale values, odd lists, spans of 48 tokens, scales of both signs and zero."""
+    g = gen(24)
+    S, span, KV, hd, H, q_len = 96, 48, 2, 128, 16, 5
+    lens = [200, 131, 96, 5, 3, 0, 400]
+    table, total = tables(g, [min(n, 4 * S) for n in lens], S, spare=3, width=4)
+    kc, vc = torch.randn(2, total, S, KV, hd, generator=g).to(BF)
+    for c, v in ((kc, NAN), (vc, INF)):
+        c[[p for p in range(total) if p not in table.flatten().tolist()]] = v
+        for b, n in enumerate(lens[:5]):
+            page, off = divmod(n, S)
+            if off:
+                c[table[b, page], off:] = v
+    table[6, 1] = total
+    spans = torch.tensor([[4, 0, 2, -1, 1], [2, 2, 1, 0, 9], [1, -7, 0, 5, 1], [0, 1, 2, 3, 4], [0, -1, 0, 7, 7], [0, 1, 2, 3, 4], [2, 8, 0, 7, 3]], dtype=torch.int32)
+    spans = torch.stack([spans, spans.flip(1)], 1).contiguous()
+    q = torch.randn(len(lens) * q_len, H, hd, generator=g).to(BF)
+    for scale in (0.09, -0.09, 0.0):
+        got = _attend(dev, q, kc, vc, table, lens, spans, span, q_len, scale)
+        assert bool(torch.isfinite(got.float()).all()) and not bool(got.view(len(lens), -1)[5].any())
 
 
 def test_span_attention_stale_values(dev):
@@ -445,6 +511,43 @@ def test_step_captured(dev):
             s.table.copy_(s.host["table"])
             for x, y in zip(s.run(), o):
                 assert torch.equal(x, y)
+
+
+def test_a_call_behind_an_event(dev):
+    """Inputs that another stream makes: the call waits for them, also where a call of its own stream is right in front."""
+    s = Step(dev, 18, [900, 640, 77], 2)
+    want = s.run()[0].clone()
+    qkv, other = s.qkv.clone(), torch.cuda.Stream()
+    for _ in range(3):
+        s.qkv.zero_()
+        torch.cuda.synchronize()
+        s.run()
+        with torch.cuda.stream(other):
+            torch.cuda._sleep(20000000)
+            s.qkv.copy_(qkv)
+            ready = torch.cuda.Event()
+            ready.record()
+        torch.cuda.current_stream().wait_event(ready)
+        got = s.run()[0]
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+def test_a_wait_that_ran_out_is_reported_once(dev):
+    """The word that a bounded wait would set is set by the host here: calls on tiles look at it, the others leave it."""
+    from ssd_b200 import lib
+    word = lib.load().ssdk_debug_op_wait_word()
+    s = Step(dev, 19, [300, 64], 6, H=16)
+    s.run()
+    few = Step(dev, 20, [300, 64], 1)
+    torch.cuda.synchronize()
+    word[0] = 1
+    few.run()
+    assert word[0] == 1
+    with pytest.raises(RuntimeError, match="ran out"):
+        s.run()
+    assert word[0] == 0
+    s.run()
 
 
 def test_offsets_past_32_bits(dev):
