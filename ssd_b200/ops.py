@@ -177,6 +177,7 @@ def verify(logits_p: torch.Tensor, logits_q: torch.Tensor, speculations: torch.T
 
 # ---- around a long paged cache: places of a step's tokens, positions with several axes, attention over selected spans ----
 _BF, _I32, _I64, _F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
+_gpu_now, _stream_of = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def _check(name: str, *args) -> int:
@@ -184,7 +185,7 @@ def _check(name: str, *args) -> int:
     per argument, and the reason only where it fails.)"""
     gpu = args[0][0].get_device()
     for t, what, dtype, shape in args:
-        if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == gpu:
+        if t.dtype is dtype and t.shape == shape and t.get_device() == gpu and t.is_contiguous():
             continue
         if t.dtype is not dtype:
             raise TypeError(f"{name}: {what}: expected {dtype}, got {t.dtype}")
@@ -206,11 +207,11 @@ def _last(t: torch.Tensor, dims: int) -> int:
 def _launch(name: str, gpu: int, *args):
     """One entry point of libssdk on the tensors' GPU and its current stream."""
     fn = getattr(_L._lib or _L.load(), name)
-    if gpu == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(gpu))
+    if gpu == _gpu_now():
+        rc = fn(*args, _stream_of(gpu))
     else:
         with torch.cuda.device(gpu):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(gpu))
+            rc = fn(*args, _stream_of(gpu))
     if rc:
         _L.check(rc, name)
 
@@ -230,8 +231,8 @@ def place_tokens(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table
                  (block_tables, "block_tables", _I32, (B, width)), (free_blocks, "free_blocks", _I32, (F,)), (free_used, "free_used", _I32, (1,)))
     if rows < 1:
         raise ValueError(f"place_tokens: {rows} rows")
-    positions = torch.empty(rows, dtype=_I64, device=context_lens.device)
-    slots, seqs, cu, lens, used = context_lens.new_empty(2 * rows + 2 * B + 2).split_with_sizes((rows, rows, B + 1, B, 1))
+    positions = context_lens.new_empty(rows, dtype=_I64)
+    slots, seqs, cu, lens, used = torch.unsafe_split_with_sizes(context_lens.new_empty(2 * rows + 2 * B + 2), (rows, rows, B + 1, B, 1))
     _launch("ssdk_place_tokens", gpu, context_lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(), free_blocks.data_ptr(), free_used.data_ptr(),
             positions.data_ptr(), slots.data_ptr(), seqs.data_ptr(), cu.data_ptr(), lens.data_ptr(), used.data_ptr(), B, width, F, rows, block_size, num_blocks)
     return positions, slots, seqs, cu, lens, used
@@ -246,22 +247,23 @@ def rope_axes_store_kv(qkv: torch.Tensor, positions: torch.Tensor, axis_of, slot
     [0] * 16 + [1] * 24 + [2] * 24); rope_table fp32 [max_pos, rot_dim] cos | sin: the first rot_dim channels of a head turn.
     Norms and rotation in fp32 with one rounding.  Returns q [M, heads * head_dim]; keys and values are in their slots.  A row with a position
     outside the table has NaN queries and stores nothing; slots are distinct, those outside the cache store nothing."""
-    M, rot, axes = qkv.shape[0], rope_table.shape[-1], positions.shape[0]
-    cache = torch.Size((*k_cache.shape[:2], kv_heads, head_dim))
-    if type(axis_of) is not bytes:
-        axis_of = bytes(list(axis_of))
+    M, axes = qkv.shape[0], positions.shape[0]
+    top, rot = rope_table.shape if rope_table.dim() == 2 else (-1, -1)
+    num_blocks, block_size, _, _ = k_cache.shape if k_cache.dim() == 4 else (-1,) * 4
+    cache = (num_blocks, block_size, kv_heads, head_dim)
+    axis_of = bytes(axis_of if type(axis_of) in (list, tuple, bytes) else list(axis_of))
     if len(axis_of) * 2 != rot:
         raise ValueError(f"rope_axes_store_kv: axis_of has {len(axis_of)} frequencies, rope_table {rot / 2}")
     args = [(qkv, "qkv", _BF, (M, (heads + 2 * kv_heads) * head_dim)), (positions, "positions", _I64, (axes, M)), (slot_mapping, "slot_mapping", _I32, (M,)),
-            (rope_table, "rope_table", _F32, (rope_table.shape[0], rot)), (k_cache, "k_cache", _BF, cache), (v_cache, "v_cache", _BF, cache)]
+            (rope_table, "rope_table", _F32, (top, rot)), (k_cache, "k_cache", _BF, cache), (v_cache, "v_cache", _BF, cache)]
     for w, what in ((q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w")):
         if w is not None:
             args.append((w, what, _BF, (head_dim,)))
     gpu = _check("rope_axes_store_kv", *args)
     q = qkv.new_empty(M, heads * head_dim)
     _launch("ssdk_rope_axes_store_kv", gpu, qkv.data_ptr(), positions.data_ptr(), axes, axis_of, slot_mapping.data_ptr(), rope_table.data_ptr(),
-            rope_table.shape[0], rot, _ptr(q_norm_w), _ptr(k_norm_w), norm_eps, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            cache[0] * cache[1], M, heads, kv_heads, head_dim)
+            top, rot, _ptr(q_norm_w), _ptr(k_norm_w), norm_eps, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), num_blocks * block_size, M,
+            heads, kv_heads, head_dim)
     return q
 
 
