@@ -276,35 +276,36 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   // ---- the sums of a row: low pieces to the row's warp, then [row][HD + 4] O | reference, sum over queries, keys and values (every product has read them) ----
   constexpr int LDO = HD + 4;
   float* joined = reinterpret_cast<float*>(smem);
-  auto sums = [&](int c, float* f) {   // 16 columns
-    uint32_t o[16];
+  auto sums = [&](int c, uint32_t* o) {   // 32 columns
     tmem_ld_32x32b_x16(tmem_o + lanes + c, o);
+    tmem_ld_32x32b_x16(tmem_o + lanes + c + 16, o + 16);
     tmem_ld_wait();
-#pragma unroll
-    for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(o[j]);
   };
   __syncthreads();   // nothing is on its way into them
   if (softmax && in && second) {
     if (!ok) s_failed = 1;
     if (ok && n > 0)
-      for (int c = 0; c < HD; c += 16) {
-        float f[16];
-        sums(c, f);
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t o[32];
+        sums(c, o);
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(joined + r * LDO + c + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+        for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(joined + r * LDO + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
       }
   }
   __syncthreads();
   if (softmax && in && !second) {
-    const bool good = ok && !s_failed;
-    for (int c = 0; c < HD; c += 16) {
-      float f[16];
-      if (good && n > 0) sums(c, f);
+    const bool good = ok && !s_failed, some = good && n > 0;
+#pragma unroll 1
+    for (int c = 0; c < HD; c += 32) {
+      uint32_t o[32];
+      if (some) sums(c, o);
 #pragma unroll
-      for (int j = 0; j < 16; j += 4) {
+      for (int j = 0; j < 32; j += 4) {
         float4* at = reinterpret_cast<float4*>(joined + r * LDO + c + j);
         const float4 x = *at;
-        *at = good && n > 0 ? make_float4(f[j] + x.x, f[j + 1] + x.y, f[j + 2] + x.z, f[j + 3] + x.w) : make_float4(0.f, 0.f, 0.f, 0.f);
+        *at = some ? make_float4(__uint_as_float(o[j]) + x.x, __uint_as_float(o[j + 1]) + x.y, __uint_as_float(o[j + 2]) + x.z, __uint_as_float(o[j + 3]) + x.w)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
       }
     }
     // a wait ran out: the row is NaN.  Without chunks (or keys) the row has no part in the sum.
@@ -315,27 +316,30 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, 256);   // (before the other blocks are waited for: they may wait for tensor memory)
   cluster.sync();
-  for (int idx = rank * kTileThreads + threadIdx.x; idx < rows * (HD / 4); idx += C * kTileThreads) {
-    const int row = idx / (HD / 4), d = idx % (HD / 4) * 4;
-    float top = -INFINITY;
-#pragma unroll 4
-    for (int c = 0; c < C; ++c) top = fmaxf(top, cluster.map_shared_rank(joined, c)[row * LDO + HD]);
+  constexpr int PER = HD / 4, SIDE = 32 / PER;   // lanes of a row, rows side by side in a warp
+  const int part_lane = lane % PER;
+  for (int base = (rank * (kTileThreads / 32) + warp) * SIDE; base < rows; base += C * (kTileThreads / 32) * SIDE) {
+    const int row = min(base + lane / PER, rows - 1);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (part_lane < C) ml = *reinterpret_cast<const float2*>(cluster.map_shared_rank(joined, part_lane) + row * LDO + HD);
+    float top = ml.x;
+#pragma unroll
+    for (int w = PER / 2; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    float f = top == -INFINITY ? 0.f : exp2f(ml.x - top), sum = part_lane < C ? ml.y * f : 0.f;   // (of this lane's block)
+#pragma unroll
+    for (int w = PER / 2; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    f *= sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;   // (NaN stays)
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-    if (top != -INFINITY) {
 #pragma unroll 4
-      for (int c = 0; c < C; ++c) {
-        const float* part = cluster.map_shared_rank(joined, c) + row * LDO;
-        const float2 ml = *reinterpret_cast<const float2*>(part + HD);
-        const float4 v = *reinterpret_cast<const float4*>(part + d);
-        const float f = exp2f(ml.x - top);
-        acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
-        sum += ml.y * f;
-      }
+    for (int c = 0; c < C; ++c) {
+      const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(joined, c) + row * LDO + part_lane * 4);
+      const float g = __shfl_sync(0xffffffffu, f, (lane & ~(PER - 1)) + c);
+      acc.x += x.x * g; acc.y += x.y * g; acc.z += x.z * g; acc.w += x.w * g;
     }
-    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;   // (NaN stays)
-    __nv_bfloat16* dst = p.out + ((size_t)(b * p.Q + tok0 + row / G) * p.heads + kvh * G + row % G) * HD + d;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    if (base + lane / PER < rows) {
+      __nv_bfloat16* dst = p.out + ((size_t)(b * p.Q + tok0 + row / G) * p.heads + kvh * G + row % G) * HD + part_lane * 4;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+    }
   }
   cluster.sync();   // no block leaves while its part is read
 }
