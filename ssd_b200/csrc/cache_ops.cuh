@@ -357,8 +357,9 @@ __global__ void __launch_bounds__(kBoundsThreads, 4) span_bounds_kernel(SpanBoun
   const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size);
   const int row = p.kv_heads * p.head_dim, slices = (row / 8 + p.width - 1) / p.width;   // columns of a warp: p.width
   const int nth = SPLIT ? (int)blockIdx.x : (int)blockIdx.x * WARPS + (int)(threadIdx.x >> 5), span = nth / slices;
-  const int pos0 = (max(len - p.fresh, 0) / p.span + span) * p.span;   // (below len + span, which the host holds under 2^31)
-  if (pos0 >= len) return;
+  const long long from = (max(len - p.fresh, 0) / p.span + (long long)span) * p.span;   // (the grid's last warps may be some long spans behind the end)
+  if (from >= len) return;
+  const int pos0 = (int)from;
   const int page = page_at(p.tables + (size_t)b * p.max_blocks + pos0 / p.block_size, p.num_blocks);
   if (page < 0) return;
   const int off = pos0 % p.block_size, tokens = min(p.span, len - pos0);

@@ -113,6 +113,15 @@ def test_span_bounds_source(tmp_path, KV, hd, S, span, new, lens, split):
     assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.nan_to_num(got.float()), torch.nan_to_num(want.float()))
 
 
+@needs_gxx
+def test_span_bounds_source_long_spans(tmp_path):
+    """Spans so long that some of the grid's rounded-up warps are past 2^31 tokens: they are behind the end.  (No entry is a page: nothing is read.)"""
+    long, width = 1 << 28, 7
+    table, lens = torch.full((1, width), -1, dtype=torch.int32), [width * long]
+    data = _run("bounds", [i32([1, width, 0, long, long, 1, 64, 1, 0]), table, i32(lens), torch.zeros(0, dtype=BF), torch.zeros(0, dtype=BF)], tmp_path)
+    assert data == b""
+
+
 # ---------------------------------------------------------------------------------------------------- refusals
 def _place_args(**change):
     a = dict(context_lens=torch.zeros(2, dtype=torch.int32), new_lens=torch.ones(2, dtype=torch.int32), block_tables=torch.zeros(2, 4, dtype=torch.int32),
