@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
   __syncthreads();
   // four columns of a row
   auto store = [&](int r, int d, float4 acc, float l) {
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;   // (a row that sees no key is zero, NaN stays)
     __nv_bfloat16* dst = p.out + ((size_t)(b * p.Q + r / G) * p.heads + kvh * G + r % G) * HD + d;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
   };
@@ -671,16 +671,15 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
     for (int w = 0; w < kSpanWarps; ++w) top = fmaxf(top, parts[(w * 16 + r) * LDO + HD]);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
-    if (top != -INFINITY) {
+    const float ref = top == -INFINITY ? 0.f : top;   // (no score seen, or NaN only: sums of 0, or NaN)
 #pragma unroll
-      for (int w = 0; w < kSpanWarps; ++w) {
-        const float* row = parts + (w * 16 + r) * LDO;
-        const float2 ml = *reinterpret_cast<const float2*>(row + HD);
-        const float4 v = *reinterpret_cast<const float4*>(row + d);
-        const float f = exp2f(ml.x - top);
-        acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
-        l += ml.y * f;
-      }
+    for (int w = 0; w < kSpanWarps; ++w) {
+      const float* row = parts + (w * 16 + r) * LDO;
+      const float2 ml = *reinterpret_cast<const float2*>(row + HD);
+      const float4 v = *reinterpret_cast<const float4*>(row + d);
+      const float f = exp2f(ml.x - ref);
+      acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+      l += ml.y * f;
     }
     if (C == 1) {
       store(r, d, acc, l);
@@ -708,14 +707,13 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
     }
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
-    if (top != -INFINITY) {
+    const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-      for (int c = 0; c < kSpanMost; ++c) {
-        if (c < C) {
-          const float f = exp2f(ml[c].x - top);
-          acc.x += v[c].x * f; acc.y += v[c].y * f; acc.z += v[c].z * f; acc.w += v[c].w * f;
-          l += ml[c].y * f;
-        }
+    for (int c = 0; c < kSpanMost; ++c) {
+      if (c < C) {
+        const float f = exp2f(ml[c].x - ref);
+        acc.x += v[c].x * f; acc.y += v[c].y * f; acc.z += v[c].z * f; acc.w += v[c].w * f;
+        l += ml[c].y * f;
       }
     }
     store(r, d, acc, l);

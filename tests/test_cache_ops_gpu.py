@@ -359,6 +359,26 @@ def test_span_attention_stale_values(dev):
     assert bool(torch.isfinite(got.float()).all())
 
 
+@pytest.mark.parametrize("q_len,H", [(1, 4), (3, 8), (6, 16)])
+def test_span_attention_nan_rows(dev, q_len, H):
+    """A query of NaN (a position outside the angles' table makes one) has NaN in its row, and only there; a key of NaN in every row that sees it."""
+    g = gen(25, q_len)
+    S, span, KV, hd = 64, 16, 2, 128
+    lens = [200, 70, 3000]
+    table, total = tables(g, lens, S)
+    kc, vc = torch.randn(2, total, S, KV, hd, generator=g).to(BF)
+    q = torch.randn(len(lens) * q_len, H, hd, generator=g).to(BF)
+    q[0], q[q_len, 1] = NAN, NAN
+    q[2 * q_len, 0, 5] = NAN
+    spans = _lists(g, lens, KV, span, 9)
+    spans[0] = torch.tensor([0, 1, 2, 3, -1, -1, -1, -1, 12])
+    got = _attend(dev, q, kc, vc, table, lens, spans, span, q_len, 0.09).view(-1, H, hd)
+    assert bool(torch.isnan(got[0]).all()) and bool(torch.isnan(got[q_len, 1]).all()) and not bool(torch.isnan(got[q_len, 0]).any())
+    kc[table[0, 0], 3, 0, 7] = NAN
+    kc[table[0, 3], 6, 1] = NAN   # token 198: of three queries or more the last two see it
+    _attend(dev, q, kc, vc, table, lens, spans, span, q_len, 0.09)
+
+
 def test_span_attention_odd_lists(dev):
     """Any order, entries twice, outside the context, on bad pages; rows that see nothing."""
     g = gen(22)
