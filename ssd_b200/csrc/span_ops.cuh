@@ -460,6 +460,50 @@ struct SpanAttnParams {
   uint32_t q_sign, q_keep;       // the sign of the scale, for two bf16 values; 0 where the scale is 0
   float scale_log2;              // |scale| * log2(e), or 1
 };
+// Values that are not finite.  A product with the weight 0 of a query that does not see their token is NaN, so from the first token on that some query does not see
+// they go into the product as 0 (take_out), and a row adds those that it sees where it is stored (add_taken_out), read from the cache again.  Where every query sees them the
+// two pieces of a weight can make NaN of an infinity: columns that are NaN in a row whose weights are not are the sum of what is not finite in them.
+SSDK_DEVINL bool not_finite(uint32_t half) { return (half & 0x7f80u) == 0x7f80u; }
+SSDK_DEVINL bool take_out(uint4* at) {
+  uint32_t w[4] = {at->x, at->y, at->z, at->w};
+  bool some = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool lo = not_finite(w[i]), hi = not_finite(w[i] >> 16);
+    some = some || lo || hi;
+    w[i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+  }
+  if (some) *at = make_uint4(w[0], w[1], w[2], w[3]);
+  return some;
+}
+// four columns of a row that sees the tokens below lim; all queries see those below `from`.  odd: values were taken out; l: the row's sum
+__device__ __noinline__ float4 with_taken_out(const SpanAttnParams& p, int head_dim, int b, int kvh, int from, int lim, int d, float4 acc) {
+  float out[4] = {acc.x, acc.y, acc.z, acc.w}, sum[4] = {};
+  const bool nan = out[0] != out[0] || out[1] != out[1] || out[2] != out[2] || out[3] != out[3];
+#pragma unroll 1
+  for (int i = 0; i < p.count; ++i) {
+    const int s = p.spans[((size_t)b * p.kv_heads + kvh) * p.count + i];
+    if (s < 0 || (long long)s * p.span >= lim) continue;
+    const int first = s * p.span, page = page_at(p.tables + (size_t)b * p.max_blocks + first / p.block_size, p.num_blocks);
+    if (page < 0) continue;
+#pragma unroll 1
+    for (int pos = nan ? first : max(first, from); pos < lim && pos - first < p.span; ++pos) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p.v_cache + (((size_t)page * p.block_size + pos % p.block_size) * p.kv_heads + kvh) * head_dim + d);
+      const uint32_t x[4] = {v.x & 0xffffu, v.x >> 16, v.y & 0xffffu, v.y >> 16};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (not_finite(x[j])) sum[j] += __uint_as_float(x[j] << 16);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) out[j] = out[j] == out[j] ? out[j] + sum[j] : sum[j] != 0.f ? sum[j] : out[j];
+  return make_float4(out[0], out[1], out[2], out[3]);
+}
+SSDK_DEVINL void add_taken_out(const SpanAttnParams& p, int head_dim, int b, int kvh, int from, int lim, int d, bool odd, float l, float4* acc) {
+  const float any = (acc->x + acc->y) + (acc->z + acc->w);   // (NaN if one is, or of infinities of both signs, which come from values that are not finite too)
+  if ((odd || any != any) && l == l) *acc = with_taken_out(p, head_dim, b, kvh, from, lim, d, *acc);
+}
+
 constexpr float kSpanSlack = 8.f;
 constexpr int kSpanWarps = 4, kSpanStages = 3, kSpanKeys = 16;
 constexpr int kSpanMost = 16;   // blocks of a cluster
@@ -467,7 +511,7 @@ constexpr int span_stage_bytes(int HD) { return 2 * kSpanKeys * (HD + 8) * 2; }
 constexpr int span_attn_smem(int HD, int count) { return kSpanWarps * kSpanStages * span_stage_bytes(HD) + count * 8; }
 
 template <int HD>
-__global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnParams p) {
+__global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(const __grid_constant__ SpanAttnParams p) {
   constexpr int LDS = HD + 8, KS = HD / 16, ND = HD / 8, SEG = HD / 8;
   extern __shared__ __align__(16) uint8_t span_smem[];
   pdl_wait();
@@ -482,6 +526,7 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
   int2* where = reinterpret_cast<int2*>(span_smem + kSpanWarps * kSpanStages * span_stage_bytes(HD));   // [count] slot (-1: none) and position of a span's first key
   uint8_t* ring = span_smem + warp * kSpanStages * span_stage_bytes(HD);
 
+  __shared__ int s_odd;   // values were taken out
   int n_list = 0;
   {
     const int32_t* list = p.spans + ((size_t)b * p.kv_heads + kvh) * p.count;
@@ -499,6 +544,7 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
   }
   {
     __shared__ int last[kSpanWarps];
+    if (threadIdx.x == 0) s_odd = 0;
     n_list = __reduce_max_sync(0xffffffffu, n_list);   // behind the last entry of any use
     if (lane == 0) last[warp] = n_list;
     __syncthreads();
@@ -600,6 +646,13 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (pos0 + nt * 8 + 2 * t + (e & 1) >= lim[e >> 1]) s[nt][e] = -INFINITY;
+      if (seen_by_all < len) {   // the sequence's own new tokens
+        bool odd = false;
+        for (int i = lane; i < kSpanKeys * SEG; i += 32)
+          if (pos0 + i / SEG >= seen_by_all) odd |= take_out(const_cast<uint4*>(reinterpret_cast<const uint4*>(cV + i / SEG * LDS + i % SEG * 8)));
+        if (odd) s_odd = 1;
+        __syncwarp();
+      }
     }
     // A row's reference is raised, and its sums rescaled, only when a score passes it by kSpanSlack (base 2): weights stay below 2^kSpanSlack, where fp32
     // and the two bf16 pieces are as fine relative to a value as below 1.
@@ -659,10 +712,12 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
   }
   __syncthreads();
   // four columns of a row
-  auto store = [&](int r, int d, float4 acc, float l) {
+  auto store = [&](int r, int d, float4 acc, float l, bool odd) {
     const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;   // (a row that sees no key is zero, NaN stays)
+    acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
+    add_taken_out(p, HD, b, kvh, seen_by_all, len - p.Q + r / G + 1, d, odd, l, &acc);
     __nv_bfloat16* dst = p.out + ((size_t)(b * p.Q + r / G) * p.heads + kvh * G + r % G) * HD + d;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
   };
   for (int idx = threadIdx.x; idx < R * (HD / 4); idx += kSpanWarps * 32) {
     const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
@@ -671,21 +726,24 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
     for (int w = 0; w < kSpanWarps; ++w) top = fmaxf(top, parts[(w * 16 + r) * LDO + HD]);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
-    const float ref = top == -INFINITY ? 0.f : top;   // (no score seen, or NaN only: sums of 0, or NaN)
+    if (top != -INFINITY) {
 #pragma unroll
-    for (int w = 0; w < kSpanWarps; ++w) {
-      const float* row = parts + (w * 16 + r) * LDO;
-      const float2 ml = *reinterpret_cast<const float2*>(row + HD);
-      const float4 v = *reinterpret_cast<const float4*>(row + d);
-      const float f = exp2f(ml.x - ref);
-      acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
-      l += ml.y * f;
+      for (int w = 0; w < kSpanWarps; ++w) {
+        const float* row = parts + (w * 16 + r) * LDO;
+        const float2 ml = *reinterpret_cast<const float2*>(row + HD);
+        const float4 v = *reinterpret_cast<const float4*>(row + d);
+        const float f = exp2f(ml.x - top);
+        acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+        l += ml.y * f;
+      }
+    } else {   // no score, or NaN only
+      for (int w = 0; w < kSpanWarps; ++w) l += parts[(w * 16 + r) * LDO + HD + 1];
     }
     if (C == 1) {
-      store(r, d, acc, l);
+      store(r, d, acc, l, s_odd);
     } else {
       *reinterpret_cast<float4*>(joined + r * LDO + d) = acc;
-      if (d == 0) *reinterpret_cast<float2*>(joined + r * LDO + HD) = make_float2(top, l);
+      if (d == 0) *reinterpret_cast<float2*>(joined + r * LDO + HD) = make_float2(top, s_odd ? -l : l);   // (a sum's sign is that word)
     }
   }
   if (C == 1) return;
@@ -707,16 +765,23 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(SpanAttnP
     }
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
-    const float ref = top == -INFINITY ? 0.f : top;
+    bool odd = false;
+    if (top != -INFINITY) {
 #pragma unroll
-    for (int c = 0; c < kSpanMost; ++c) {
-      if (c < C) {
-        const float f = exp2f(ml[c].x - ref);
-        acc.x += v[c].x * f; acc.y += v[c].y * f; acc.z += v[c].z * f; acc.w += v[c].w * f;
-        l += ml[c].y * f;
+      for (int c = 0; c < kSpanMost; ++c) {
+        if (c < C) {
+          const float f = exp2f(ml[c].x - top);
+          acc.x += v[c].x * f; acc.y += v[c].y * f; acc.z += v[c].z * f; acc.w += v[c].w * f;
+          l += fabsf(ml[c].y) * f;
+          odd |= __float_as_int(ml[c].y) < 0;
+        }
       }
+    } else {
+#pragma unroll
+      for (int c = 0; c < kSpanMost; ++c)
+        if (c < C) l += ml[c].y;
     }
-    store(r, d, acc, l);
+    store(r, d, acc, l, odd);
   }
   cluster.sync();   // no block leaves while its part is read
 }

@@ -39,7 +39,7 @@ SSDK_DEVINL bool tile_wait_warp(uint64_t* bar, uint32_t parity, unsigned* timeou
 
 template <int HD>
 __global__ void __launch_bounds__(kTileThreads, 2)
-span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const SpanAttnParams p,
+span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ SpanAttnParams p,
                  const int box, const int q_tokens, unsigned* timeout) {
   namespace cg = cooperative_groups;
   constexpr int HALVES = HD / 64;                    // 64-column boxes of a row
@@ -47,7 +47,7 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   extern __shared__ uint8_t span_tile_raw[];
   __shared__ __align__(8) uint64_t q_full, k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ int s_failed, found[kTileThreads / 32];
+  __shared__ int s_failed, s_odd, found[kTileThreads / 32];   // s_odd: values were taken out
   uint8_t* smem = span_tile_raw + ((1024u - (smem_u32(span_tile_raw) & 1023u)) & 1023u);
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + HALVES * kQHalf;
@@ -70,7 +70,7 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       mbar_init(&k_full[s], 1); mbar_init(&v_full[s], 1); mbar_init(&s_full[s], 1); mbar_init(&p_full[s], live); mbar_init(&pv_done[s], 1);
     }
     fence_mbar_init();
-    s_failed = 0;
+    s_failed = s_odd = 0;
   }
   if (warp == 1) { tmem_alloc(&tmem_slot, 256); tmem_relinquish(); }
   pdl_wait();
@@ -251,18 +251,25 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       tmem_st_32x32b_x16(sp, u);
       tmem_st_32x32b_x16(sp + 16, u + 16);
       tmem_st_wait();
-      if (!whole) {   // slots behind the context hold anything, and 0 x NaN is NaN
+      if (!whole) {   // slots behind the context hold anything, new tokens values that are not finite: 0 x NaN is NaN
+        const int edge = min(seen_by_all, len);
         bool stale = false;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) stale = stale || (pos[j] < kNoPosition && pos[j] + 16 > len);
+        for (int j = 0; j < 4; ++j) stale = stale || (pos[j] < kNoPosition && pos[j] + 16 > edge);
         if (stale) {   // (the same for all warps)
           if (!(ok = tile_wait_warp(&v_full[i & 1], parity(i), timeout))) break;
+          bool odd = false;
           for (int j = second ? half + r : r; j < kTileKeys * 8; j += live) {
-            const int key = j >> 3, x = key >> 4;
-            if ((x == 0 ? pos[0] : x == 1 ? pos[1] : x == 2 ? pos[2] : pos[3]) + (key & 15) >= len)
+            const int key = j >> 3, x = key >> 4, at = (x == 0 ? pos[0] : x == 1 ? pos[1] : x == 2 ? pos[2] : pos[3]) + (key & 15);
+            if (at >= edge)
 #pragma unroll
-              for (int h = 0; h < HALVES; ++h) *reinterpret_cast<uint4*>(sV + (i & 1) * kTile + h * kKHalf + j * 16) = make_uint4(0u, 0u, 0u, 0u);
+              for (int h = 0; h < HALVES; ++h) {
+                uint4* v = reinterpret_cast<uint4*>(sV + (i & 1) * kTile + h * kKHalf + j * 16);
+                if (at >= len) *v = make_uint4(0u, 0u, 0u, 0u);
+                else odd |= take_out(v);
+              }
           }
+          if (odd) s_odd = 1;
           fence_proxy_async_smem();
         }
       }
@@ -308,8 +315,8 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                    : make_float4(0.f, 0.f, 0.f, 0.f);
       }
     }
-    // a wait ran out: the row is NaN.  Without chunks (or keys) the row has no part in the sum.
-    *reinterpret_cast<float2*>(joined + r * LDO + HD) = good ? make_float2(m, l) : make_float2(0.f, __int_as_float(0x7fffffff));
+    // a wait ran out: the row is NaN.  Without chunks (or keys) the row has no part in the sum.  The sum's sign: s_odd.
+    *reinterpret_cast<float2*>(joined + r * LDO + HD) = good ? make_float2(m, s_odd ? -l : l) : make_float2(0.f, __int_as_float(0x7fffffff));
   }
   tc_fence_before();
   __syncthreads();
@@ -322,6 +329,8 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const int row = min(base + lane / PER, rows - 1);
     float2 ml = make_float2(-INFINITY, 0.f);
     if (part_lane < C) ml = *reinterpret_cast<const float2*>(cluster.map_shared_rank(joined, part_lane) + row * LDO + HD);
+    const bool odd = __any_sync(0xffffffffu, __float_as_int(ml.y) < 0);
+    ml.y = fabsf(ml.y);
     float top = ml.x;
 #pragma unroll
     for (int w = PER / 2; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
@@ -337,6 +346,7 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       acc.x += x.x * g; acc.y += x.y * g; acc.z += x.z * g; acc.w += x.w * g;
     }
     if (base + lane / PER < rows) {
+      add_taken_out(p, HD, b, kvh, len - p.Q + tok0 + 1, len - p.Q + tok0 + row / G + 1, part_lane * 4, odd, sum, &acc);
       __nv_bfloat16* dst = p.out + ((size_t)(b * p.Q + tok0 + row / G) * p.heads + kvh * G + row % G) * HD + part_lane * 4;
       *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
     }

@@ -272,9 +272,13 @@ def _lists(g, lens, KV, span, count):
     return out
 
 
-def _attend(dev, q, kc, vc, table, lens, spans, span, q_len, scale):
+def ops_attention(dev, q, kc, vc, table, lens, spans, span, q_len, scale):
     from ssd_b200 import ops
-    got = ops.span_attention(q.to(dev), kc.to(dev), vc.to(dev), table.to(dev), i32(lens, dev), spans.to(dev), span, q_len, scale)
+    return ops.span_attention(q.to(dev), kc.to(dev), vc.to(dev), table.to(dev), i32(lens, dev), spans.to(dev), span, q_len, scale)
+
+
+def _attend(dev, q, kc, vc, table, lens, spans, span, q_len, scale):
+    got = ops_attention(dev, q, kc, vc, table, lens, spans, span, q_len, scale)
     want, slack = plain.attention(q, kc, vc, table, lens, spans, span, q_len, scale)
     within(got, want, slack)
     return got
@@ -292,7 +296,7 @@ def test_span_attention(dev, H, KV, hd, q_len, S, span, count, lens):
     _attend(dev, q, kc, vc, table, lens, _lists(g, lens, KV, span, count), span, q_len, hd ** -0.5)
 
 
-@pytest.mark.parametrize("count,q_len,H,KV,hd", [(256, 1, 8, 1, 128), (512, 3, 8, 2, 64), (4096, 1, 4, 1, 64), (300, 8, 8, 1, 128), (1000, 2, 16, 1, 128)])
+@pytest.mark.parametrize("count,q_len,H,KV,hd", [(256, 1, 8, 1, 128), (512, 3, 8, 2, 64), (4096, 1, 4, 1, 64), (300, 8, 8, 1, 128), (1000, 2, 16, 1, 128), (4096, 9, 4, 1, 128)])
 def test_span_attention_long(dev, count, q_len, H, KV, hd):
     g = gen(count, q_len, H)
     S, span = 64, 16
@@ -377,6 +381,30 @@ def test_span_attention_nan_rows(dev, q_len, H):
     kc[table[0, 0], 3, 0, 7] = NAN
     kc[table[0, 3], 6, 1] = NAN   # token 198: of three queries or more the last two see it
     _attend(dev, q, kc, vc, table, lens, spans, span, q_len, 0.09)
+
+
+@pytest.mark.parametrize("q_len,H,hd,span,count", [(2, 4, 128, 16, 9), (8, 4, 64, 32, 5), (3, 10, 64, 16, 200), (9, 8, 128, 16, 9), (40, 8, 64, 32, 40), (70, 16, 128, 16, 5), (4, 16, 128, 64, 64)])
+def test_span_attention_values_of_new_tokens(dev, q_len, H, hd, span, count):
+    """Infinite and NaN values of new tokens reach the queries that see them, as often as they are listed, and no others."""
+    g = gen(26, q_len, H)
+    S, KV = 64, 2
+    lens = [200, 70, 3000, 65, 4000]
+    table, total = tables(g, lens, S)
+    kc, vc = torch.randn(2, total, S, KV, hd, generator=g).to(BF)
+    spans = _lists(g, lens, KV, span, count)
+    for b, n in enumerate(lens):
+        ends = [(n - 1) // span, max(n - q_len, 0) // span]
+        spans[b, :, :2] = torch.tensor(ends if b % 2 else ends[:1] * 2, dtype=torch.int32)   # (one span twice)
+        for j, (d, v) in enumerate([(3, INF), (hd - 1, NAN), (5, -INF), (3, -INF), (20, INF)]):
+            pos = n - 1 - j * q_len // 8 - (b == 1)
+            vc[table[b, pos // S], pos % S, j % KV, d] = v
+            kc[table[b, pos // S], pos % S, 0, d] = NAN if b == 3 and j == 0 else 1.0
+    q = torch.randn(len(lens) * q_len, H, hd, generator=g).to(BF)
+    got = ops_attention(dev, q, kc, vc, table, lens, spans, span, q_len, 0.09).double().cpu()
+    want, slack = plain.attention(q, kc, vc, table, lens, spans, span, q_len, 0.09)
+    odd = ~torch.isfinite(want)
+    assert bool(odd.any()) and torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[odd].nan_to_num(7.0, INF, -INF), want[odd].nan_to_num(7.0, INF, -INF))
+    within(got.masked_fill(odd, 0), want.masked_fill(odd, 0), slack.masked_fill(odd, 0))
 
 
 def test_span_attention_odd_lists(dev):
