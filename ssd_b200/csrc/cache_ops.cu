@@ -1,6 +1,7 @@
 // cache_ops.cu — entry points (include/ssdk.h) of the operators of cache_ops.cuh and span_ops.cuh.
 #include <atomic>
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <numeric>
 
@@ -15,6 +16,10 @@ typedef __nv_bfloat16 bf16;
 
 static bool off16(const void* a, const void* b = nullptr, const void* c = nullptr, const void* d = nullptr) {
   return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) & 15) != 0;
+}
+// do n bytes at a and m bytes at b share some
+static bool overlap(const void* a, int64_t n, const void* b, int64_t m) {
+  return (uintptr_t)a < (uintptr_t)b + (uintptr_t)m && (uintptr_t)b < (uintptr_t)a + (uintptr_t)n;
 }
 // a cache whose slots are numbered in 32 bits, and tables over it
 static int check_pages(const char* who, int batch, int block_size, int max_blocks, int64_t num_blocks) {
@@ -149,6 +154,9 @@ int ssdk_place_tokens(const int32_t* context_lens, const int32_t* new_lens, int3
   if (batch > kPlaceMaxSeqs || rows < 1 || rows > (1 << 30) || n_free < 0) return fail("place_tokens: %d sequences (at most %d), %d rows, %d free pages", batch, kPlaceMaxSeqs, rows, n_free);
   if (!context_lens || !new_lens || !block_tables || !free_used || (n_free && !free_blocks) || !positions || !slot_mapping || !row_seqs || !cu_rows || !lens || !used)
     return fail("place_tokens: null argument");
+  // (every block reads the lengths and the pages handed out while the first one writes)
+  if (overlap(lens, 4ll * batch, context_lens, 4ll * batch) || overlap(lens, 4ll * batch, new_lens, 4ll * batch) || overlap(used, 4, free_used, 4))
+    return fail("place_tokens: lens and used need arrays of their own");
   PlaceParams p;
   p.ctx = context_lens; p.fresh = new_lens; p.tables = block_tables; p.free_blocks = free_blocks; p.free_used = free_used;
   p.positions = positions; p.slots = slot_mapping; p.seqs = row_seqs; p.cu = cu_rows; p.lens = lens; p.used = used;
@@ -170,6 +178,7 @@ int ssdk_rope_axes_store_kv(const void* qkv, const int64_t* positions, int axes,
   if (heads + 2 * (int64_t)kv_heads > 65535) return fail("rope_axes: too many heads");
   if (!qkv || !positions || !axis_of || !slot_mapping || !rope_table || !q_out || !k_cache || !v_cache) return fail("rope_axes: null argument");
   if (off16(qkv, q_out, k_cache, v_cache) || off16(q_norm_w, k_norm_w, rope_table)) return fail("rope_axes: arrays must start at multiples of 16 bytes");
+  if (overlap(q_out, 2ll * M * heads * head_dim, qkv, 2ll * M * (heads + 2 * (int64_t)kv_heads) * head_dim)) return fail("rope_axes: q_out needs an array of its own");
   RopeAxesParams p;
   memset(&p, 0, sizeof(p));
   for (int i = 0; i < rot_dim / 2; ++i) {
@@ -247,8 +256,8 @@ int ssdk_span_attn(const void* q, const void* k_cache, const void* v_cache, cons
   CKI(check_pages("span_attn", batch, block_size, max_blocks_per_seq, num_blocks));
   CKI(check_spans("span_attn", heads, kv_heads, head_dim, block_size, span));
   const int G = heads / kv_heads;
-  if (q_len < 1 || count < 1 || count > kMaxListed || G > 32 || !(scale == scale))
-    return fail("span_attn: q_len=%d, %d spans (at most %d), %d query heads to a key head (at most 32)", q_len, count, kMaxListed, G);
+  if (q_len < 1 || count < 1 || count > kMaxListed || G > 32 || !std::isfinite(scale))
+    return fail("span_attn: q_len=%d, %d spans (at most %d), %d query heads to a key head (at most 32), scale %g", q_len, count, kMaxListed, G, (double)scale);
   if ((int64_t)count * span >= (1ll << 31) || (int64_t)batch * q_len >= (1ll << 31)) return fail("span_attn: %d spans of %d tokens, %d rows of %d sequences", count, span, q_len, batch);
   if (!q || !k_cache || !v_cache || !block_tables || !context_lens || !selected || !out) return fail("span_attn: null argument");
   if (off16(q, k_cache, v_cache, out)) return fail("span_attn: arrays must start at multiples of 16 bytes");

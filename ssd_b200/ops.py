@@ -272,7 +272,8 @@ def span_bounds(bounds: torch.Tensor, k_cache: torch.Tensor, block_tables: torch
     tokens of each sequence (at least the tokens stored since the last call; more costs time only).
 
     bounds [num_blocks, block_size / span, KV, 2, hd] bf16, in place: its second size says how many spans a page has; k_cache
-    [num_blocks, block_size, KV, hd]; context_lens int32 [B] with the new tokens.  Returns bounds."""
+    [num_blocks, block_size, KV, hd]; context_lens int32 [B] with the new tokens.  Sequences that share a page have the same number of its tokens in the context (shared prefixes
+    of whole pages do).  Returns bounds."""
     n, block_size, KV, hd = k_cache.shape if k_cache.dim() == 4 else (-1,) * 4
     subs = bounds.shape[1] if bounds.dim() == 5 else -1
     B, width = _last(context_lens, 1), _last(block_tables, 2)

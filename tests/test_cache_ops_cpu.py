@@ -201,16 +201,31 @@ def test_no_cpu_path():
 P = 4096   # an address that no call below gets to use
 
 
+def test_refusals_of_shared_arrays():
+    """Outputs that lie over inputs which other blocks still read."""
+    from ssd_b200 import lib
+    so = lib.load()
+    place = [P * i for i in range(1, 12)] + [2, 4, 8, 4, 16, 8, None]
+    for at, over in ((9, 0), (9, 1), (10, 4)):
+        for off in (0, 4) if at == 9 else (0,):
+            args = list(place)
+            args[at] = args[over] + off
+            assert so.ssdk_place_tokens(*args) < 0 and "of their own" in so.ssdk_last_error().decode()
+    row = 4 * 64 * 2
+    rope = [16 * P, P, 2, bytes(32), P, P, 10, 64, None, None, 1e-6, 16 * P + 2 * row, 8 * P, 8 * P, 32, 3, 2, 1, 64, None]
+    assert so.ssdk_rope_axes_store_kv(*rope) < 0 and "of its own" in so.ssdk_last_error().decode()
+
+
 @pytest.mark.parametrize("name,good,bad", [
     # (index of an argument, value) that an entry point refuses before it touches the device
-    ("ssdk_place_tokens", [P] * 11 + [2, 4, 8, 4, 16, 8, None],
+    ("ssdk_place_tokens", [P * i for i in range(1, 12)] + [2, 4, 8, 4, 16, 8, None],
      [(0, None), (3, None), (10, None), (11, 0), (11, 20000), (12, 0), (13, -1), (14, 0), (15, 0), (16, 0), (12, 1 << 28), (16, 1 << 28), (14, (1 << 30) + 1)]),
-    ("ssdk_rope_axes_store_kv", [P, P, 2, bytes(32), P, P, 10, 64, None, None, 1e-6, P, P, P, 32, 3, 2, 1, 64, None],
+    ("ssdk_rope_axes_store_kv", [P, P, 2, bytes(32), P, P, 10, 64, None, None, 1e-6, 64 * P, P, P, 32, 3, 2, 1, 64, None],
      [(0, None), (1, None), (2, 0), (2, 5), (3, None), (3, bytes([2] * 32)), (6, 0), (7, 8), (7, 24), (7, 80), (0, P + 2), (8, P + 8), (14, 0), (15, 0), (16, 0), (17, 0), (18, 96)]),
     ("ssdk_span_bounds", [P, P, P, P, 2, 1, 2, 64, 32, 2, 4, 16, None],
      [(0, None), (3, None), (4, 0), (4, 70000), (5, 0), (6, 0), (7, 80), (8, 0), (9, 0), (10, 0), (11, 8), (11, 24), (11, 64), (0, P + 8)]),
     ("ssdk_span_attn", [P] * 7 + [2, 1, 4, 2, 64, 32, 2, 4, 16, 3, 0.1, None],
-     [(0, None), (5, None), (7, 0), (8, 0), (9, 3), (9, 66), (10, 0), (11, 96), (12, 0), (13, 0), (14, 0), (15, 12), (16, 0), (16, 4097), (17, float("nan")), (6, P + 2), (13, 1 << 27)]),
+     [(0, None), (5, None), (7, 0), (8, 0), (9, 3), (9, 66), (10, 0), (11, 96), (12, 0), (13, 0), (14, 0), (15, 12), (16, 0), (16, 4097), (17, float("nan")), (17, float("inf")), (6, P + 2), (13, 1 << 27)]),
     ("ssdk_select_spans", [P] * 6 + [2, 1, 4, 2, 64, 32, 2, 4, 16, 3, 1, 1, None],
      [(0, None), (4, None), (5, None), (6, 0), (7, 0), (8, 3), (9, 0), (10, 96), (11, 0), (12, 0), (13, 0), (14, 20), (15, 0), (15, 4097), (16, -1), (17, -1), (17, 3), (1, P + 4), (12, 20000), (7, 3000)]),
 ])
