@@ -122,7 +122,7 @@ static int launch_select(Launcher& L, const SelectParams& p) {
   CKI(with_smem(span_pick_kernel<HD>, kMaxSmem, kSmemOnly, done));
   constexpr int W = kEstimateThreads / 32;
   const int64_t rows = (int64_t)p.Q * (p.heads / p.kv_heads);
-  const dim3 grid(p.warps / W, p.kv_heads, p.B), block(kEstimateThreads);
+  const dim3 grid(rows > 8 ? p.warps / W : (p.warps * p.kv_heads + W - 1) / W, rows > 8 ? p.kv_heads : 1, p.B), block(kEstimateThreads);
   if (rows > 8) {
     static std::atomic<bool> many_done[64];
     CKI(with_smem(span_estimate_kernel<HD, true>, kMaxSmem, kSmemOnly, many_done));
@@ -132,12 +132,25 @@ static int launch_select(Launcher& L, const SelectParams& p) {
   }
   return L.go(span_pick_kernel<HD>, dim3(p.kv_heads, p.B), dim3(kPickThreads), pick_smem(p.max_spans, rows, HD), p);
 }
-// groups of sixteen spans of a warp: one while the blocks are fewer than two per SM, four at most (they share the query's fragments)
-static int select_run(int batch, int kv_heads, int64_t max_spans) {
-  const int64_t blocks = (max_spans + 127) / 128 * batch * kv_heads;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(4, blocks / (2 * kSms)));
+// Warps to a key head, which go over its groups of sixteen spans in turns: as many as make the fewest turns and waves (two blocks on an SM), a block's start and the
+// query's fragments as long as two turns.  us for 1, 2, 4, 6, 8, 11 turns of 24 contexts of 64000 (8 key heads): 49.3, 42.7, 40.4, 39.2, 41.4, 39.2; 8 of them 24.7, 22.9, 21.7,
+// 22.8, 25.1, 26.7; one of 32000 9.2, 10.3, 12.6, 14.9.
+static int select_warps(int batch, int kv_heads, int64_t max_spans, bool many) {
+  constexpr int W = kEstimateThreads / 32;
+  const int groups = (int)((max_spans + 15) / 16);
+  int best = groups;
+  int64_t least = INT64_MAX;
+  for (int turns = 1; turns <= std::min(groups, 32); ++turns) {
+    int warps = (groups + turns - 1) / turns;
+    if (many) warps = (warps + W - 1) / W * W;   // (a block's are of one head)
+    const int64_t blocks = ((int64_t)warps * kv_heads + W - 1) / W * batch, cost = (blocks + 2 * kSms - 1) / (2 * kSms) * (turns + 2);
+    if (cost < least) {
+      least = cost;
+      best = warps;
+    }
+  }
+  return best;
 }
-static int select_warps(int64_t max_spans, int run) { return (int)((max_spans + 128 * run - 1) / (128 * run)) * (kEstimateThreads / 32); }
 
 extern "C" {
 
@@ -244,7 +257,7 @@ int ssdk_select_spans(const void* q, const void* bounds, const int32_t* block_ta
   p.num_blocks = num_blocks; p.B = batch; p.Q = q_len; p.heads = heads; p.kv_heads = kv_heads;
   p.block_size = block_size; p.span = span; p.max_blocks = max_blocks_per_seq; p.max_spans = (int)max_spans;
   p.count = count; p.first = first; p.last = last;
-  p.run = select_run(batch, kv_heads, max_spans); p.warps = select_warps(max_spans, p.run);
+  p.warps = select_warps(batch, kv_heads, max_spans, rows > 8);
   p.estimates = (uint32_t*)scratch; p.wide = p.estimates + (size_t)batch * kv_heads * max_spans;
   Launcher L = launcher(stream);
   return head_dim == 64 ? launch_select<64>(L, p) : launch_select<128>(L, p);

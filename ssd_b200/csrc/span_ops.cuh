@@ -20,7 +20,8 @@ namespace ssdk {
 // in between in 64 bits (products of bf16 values are exact, sums of 128 of them off by 2^-46).  Where values are not finite, or so large that 32 bits
 // overflow, it scores all.
 // Two kernels, the second's start under the first's end: the estimates fill all SMs in even shares whatever the number of heads, and what picks is one block
-// of a head.  24 contexts of 64000 tokens (150 MB of bounds): 34 us and 8 us.
+// of a head.  24 contexts of 64000 tokens (150 MB of bounds): 39 us, of it 8 the second's.  The first has its loads in flight one turn at a time (registers hold one);
+// a ring of cp.async stages, each lane its own pieces or a span's bounds by whole lines, was slower: 49 and 41 us.
 // ----------------------------------------------------------------------------------
 struct SelectParams {
   const __nv_bfloat16* q;        // [B * Q, H, hd]
@@ -33,7 +34,7 @@ struct SelectParams {
   int64_t num_blocks;
   unsigned long long sub_magic;  // ceil(2^32 / spans of a page)
   int B, Q, heads, kv_heads, block_size, span, max_blocks, max_spans, count, first, last;
-  int run, warps;                // groups of sixteen spans of a warp; warps to a key head of a sequence
+  int warps;                     // to a key head of a sequence: warp w takes groups w, w + warps, ... of sixteen spans
 };
 constexpr int kEstimateThreads = 256;
 constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 32;
@@ -148,7 +149,10 @@ __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(Sele
   constexpr int W = kEstimateThreads / 32;
   pdl_wait();
   pdl_launch_dependents();
-  const int head = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  // neighbouring warps take neighbouring heads, whose bounds of a span lie together (MANY: a block's warps share the fragments of their head)
+  const int unit = blockIdx.x * W + warp, head = MANY ? (int)blockIdx.y : unit % p.kv_heads, slot = MANY ? unit : unit / p.kv_heads;
+  if (slot >= p.warps) return;   // (MANY: none)
   const int n = (tokens_of(p.lens, b, p.max_blocks, p.block_size) + p.span - 1) / p.span, groups = (n + 15) / 16;
   if (n <= p.count) return;   // all are listed
   const int G = p.heads / p.kv_heads, rows = G * p.Q, tiles = (rows + 7) / 8, subs = p.block_size / p.span;
@@ -173,8 +177,7 @@ __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(Sele
       f[2 * CH + 2 * i + 1] = make_uint2(max_bf16x2(x.z, 0u), max_bf16x2(x.w, 0u));
     }
   };
-  int group = blockIdx.x * W * p.run + warp;
-  const int end = min(groups, (int)(blockIdx.x + 1) * W * p.run);
+  int group = slot;
   long long at0 = place_of(group * 16 + g), at1 = place_of(group * 16 + 8 + g);
   uint2 qf[4 * CH];
   if (MANY) {   // every tile's fragments into shared memory, a tile per warp
@@ -184,11 +187,11 @@ __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(Sele
       for (int k = 0; k < 4 * CH; ++k) frags[(tile * 4 * CH + k) * 32 + lane] = qf[k];
     }
     __syncthreads();
-  } else if (group < end) {
+  } else if (group < groups) {
     load_q(0, qf);
   }
   uint32_t bottom = 0, top = 0;   // two channels: smallest lower, largest upper bound
-  for (; group < end; group += W) {
+  for (; group < groups; group += p.warps) {
     const int s0 = group * 16 + g, s1 = s0 + 8;
     const bool there0 = at0 >= 0, there1 = at1 >= 0;
     const __nv_bfloat16 *both0 = p.bounds + at0 + 8 * t, *both1 = p.bounds + at1 + 8 * t;
@@ -198,8 +201,8 @@ __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(Sele
       u[i] = there0 ? ld_nc_v4(both0 + 32 * i) : make_uint4(0, 0, 0, 0);
       v[i] = there1 ? ld_nc_v4(both1 + 32 * i) : make_uint4(0, 0, 0, 0);
     }
-    at0 = place_of(s0 + 16 * W);
-    at1 = place_of(s1 + 16 * W);
+    at0 = place_of(s0 + 16 * p.warps);
+    at1 = place_of(s1 + 16 * p.warps);
     float best[2] = {-INFINITY, -INFINITY};   // spans g, g + 8
     for (int tile = 0; tile < (MANY ? tiles : 1); ++tile) {
       float c[2][4] = {};
@@ -236,7 +239,7 @@ __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(Sele
   }
   const uint32_t both = max_bf16x2(bottom & 0x7fff7fffu, top);   // (top is not negative; NaN is above infinity above all)
   const uint32_t most = __reduce_max_sync(0xffffffffu, max(both & 0xffffu, both >> 16));
-  if (lane == 0) p.wide[((size_t)b * p.kv_heads + head) * p.warps + blockIdx.x * W + warp] = most << 16;
+  if (lane == 0) p.wide[((size_t)b * p.kv_heads + head) * p.warps + slot] = most << 16;
 }
 
 template <int HD>
