@@ -43,7 +43,7 @@ constexpr int kPickBins = 1024;    // a multiple of kPickThreads
 constexpr int kPickRanked = 256;   // spans between, up to which each is compared with each
 // rows of the query | scores (64 bits; before them the estimates) | taken | between (a bit per span) | bins, then the spans between
 constexpr int64_t pick_smem(int spans, int64_t rows, int HD) { return (rows + 7) / 8 * 8 * HD * 2 + spans * 8 + 2 * ((spans + 31) / 32) * 4 + kPickBins * 4; }
-constexpr int64_t estimate_smem(int64_t rows, int HD) { return rows > 8 ? (rows + 7) / 8 * 32 * HD : 0; }
+constexpr int64_t estimate_smem(int64_t rows, int HD) { return rows > 8 ? (rows + 7) / 8 * 16 * HD : 0; }
 constexpr uint32_t kNoSpan = 0xffffffffu;   // estimate of a span that has no page
 
 // 64-bit values in their order as unsigned words; zeros of both signs are one value, NaN is above all.  0 is no value
@@ -144,7 +144,7 @@ SSDK_DEVINL const __nv_bfloat16* bounds_at(const SelectParams& p, int page, int 
 // MANY: more than eight rows, whose fragments lie in shared memory
 template <int HD, bool MANY>
 __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(SelectParams p) {
-  extern __shared__ __align__(16) uint2 frags[];   // [tiles][4 CH][32]
+  extern __shared__ __align__(16) uint2 frags[];   // [tiles][2 CH][32]
   constexpr int CH = HD / 32;   // 16-byte pieces of a lane per bound
   constexpr int W = kEstimateThreads / 32;
   pdl_wait();
@@ -163,28 +163,28 @@ __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(Sele
     const int entry = sub_page(p, s), page = s < n ? page_at(table + entry, p.num_blocks) : -1;
     return page < 0 ? -1ll : (((long long)page * subs + (s - entry * subs)) * p.kv_heads + head) * (2 * HD);
   };
-  // the query's side: row g of a tile, step k of 16 channels: the lane's channels 8 (t + 4 (k / 2)) + 4 (k % 2) .. + 3; lower bounds (k < 2 CH) meet
-  // the negative parts, upper bounds the positive ones
+  // the query's side: row g of a tile, step k of 16 channels: the lane's channels 8 (t + 4 (k / 2)) + 4 (k % 2) .. + 3.  Lower bounds meet the negative parts,
+  // upper bounds the positive ones
   auto load_q = [&](int tile, uint2* f) {
     const int r = tile * 8 + g;
     const __nv_bfloat16* q = p.q + ((size_t)(b * p.Q + r / G) * p.heads + head * G + r % G) * HD + 8 * t;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const uint4 x = r < rows ? *reinterpret_cast<const uint4*>(q + 32 * i) : make_uint4(0, 0, 0, 0);
-      f[2 * i] = make_uint2(min_bf16x2(x.x, 0u), min_bf16x2(x.y, 0u));
-      f[2 * i + 1] = make_uint2(min_bf16x2(x.z, 0u), min_bf16x2(x.w, 0u));
-      f[2 * CH + 2 * i] = make_uint2(max_bf16x2(x.x, 0u), max_bf16x2(x.y, 0u));
-      f[2 * CH + 2 * i + 1] = make_uint2(max_bf16x2(x.z, 0u), max_bf16x2(x.w, 0u));
+      f[2 * i] = make_uint2(x.x, x.y);
+      f[2 * i + 1] = make_uint2(x.z, x.w);
     }
   };
+  auto negative = [](const uint2& f) { return make_uint2(min_bf16x2(f.x, 0u), min_bf16x2(f.y, 0u)); };
+  auto positive = [](const uint2& f) { return make_uint2(max_bf16x2(f.x, 0u), max_bf16x2(f.y, 0u)); };
   int group = slot;
   long long at0 = place_of(group * 16 + g), at1 = place_of(group * 16 + 8 + g);
-  uint2 qf[4 * CH];
+  uint2 qf[2 * CH];
   if (MANY) {   // every tile's fragments into shared memory, a tile per warp
     for (int tile = warp; tile < tiles; tile += W) {
       load_q(tile, qf);
 #pragma unroll
-      for (int k = 0; k < 4 * CH; ++k) frags[(tile * 4 * CH + k) * 32 + lane] = qf[k];
+      for (int k = 0; k < 2 * CH; ++k) frags[(tile * 2 * CH + k) * 32 + lane] = qf[k];
     }
     __syncthreads();
   } else if (group < groups) {
@@ -207,11 +207,13 @@ __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(Sele
     for (int tile = 0; tile < (MANY ? tiles : 1); ++tile) {
       float c[2][4] = {};
 #pragma unroll
-      for (int i = 0; i < 2 * CH; ++i) {
-        const uint32_t a0[4] = {u[i].x, v[i].x, u[i].y, v[i].y}, a1[4] = {u[i].z, v[i].z, u[i].w, v[i].w};
-        const uint2 f0 = MANY ? frags[(tile * 4 * CH + 2 * i) * 32 + lane] : qf[2 * i], f1 = MANY ? frags[(tile * 4 * CH + 2 * i + 1) * 32 + lane] : qf[2 * i + 1];
-        mma_bf16_16816(c[0], a0, f0.x, f0.y);
-        mma_bf16_16816(c[1], a1, f1.x, f1.y);
+      for (int k = 0; k < 2 * CH; ++k) {
+        const uint2 f = MANY ? frags[(tile * 2 * CH + k) * 32 + lane] : qf[k], lo = negative(f), hi = positive(f);
+        const uint4 &ul = u[k / 2], &vl = v[k / 2], &uh = u[CH + k / 2], &vh = v[CH + k / 2];
+        const uint32_t al[4] = {k & 1 ? ul.z : ul.x, k & 1 ? vl.z : vl.x, k & 1 ? ul.w : ul.y, k & 1 ? vl.w : vl.y};
+        const uint32_t ah[4] = {k & 1 ? uh.z : uh.x, k & 1 ? vh.z : vh.x, k & 1 ? uh.w : uh.y, k & 1 ? vh.w : vh.y};
+        mma_bf16_16816(c[0], al, lo.x, lo.y);
+        mma_bf16_16816(c[1], ah, hi.x, hi.y);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e)
