@@ -143,11 +143,12 @@ static int select_warps(int batch, int kv_heads, int64_t max_spans, bool many) {
   for (int turns = 1; turns <= std::min(groups, 32); ++turns) {
     int warps = (groups + turns - 1) / turns;
     if (many) warps = (warps + W - 1) / W * W;   // (a block's are of one head)
-    const int64_t blocks = ((int64_t)warps * kv_heads + W - 1) / W * batch, cost = (blocks + 2 * kSms - 1) / (2 * kSms) * (turns + 2);
+    const int64_t blocks = (int64_t)((warps * (unsigned)kv_heads + W - 1) / W) * batch, cost = (blocks + 2 * kSms - 1) / (2 * kSms) * (turns + 2);
     if (cost < least) {
       least = cost;
       best = warps;
     }
+    if (blocks <= 2 * kSms) break;   // (more turns of one wave only last longer)
   }
   return best;
 }

@@ -7,6 +7,8 @@ the extension is missing — there is no eager fallback.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import lib as _L
@@ -286,6 +288,11 @@ def span_bounds(bounds: torch.Tensor, k_cache: torch.Tensor, block_tables: torch
     return bounds
 
 
+@functools.lru_cache(maxsize=256)
+def _select_scratch(*sizes: int) -> int:
+    return _L.load().ssdk_select_spans_scratch_bytes(*sizes) // 2
+
+
 def select_spans(q: torch.Tensor, bounds: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor, q_len: int, block_size: int,
                  count: int, first: int = 1, last: int | None = None) -> torch.Tensor:
     """The `count` spans of each sequence's cache that its queries are to read, per key head: the first `first` and the last
@@ -304,7 +311,7 @@ def select_spans(q: torch.Tensor, bounds: torch.Tensor, block_tables: torch.Tens
     if last is None:
         last = min((q_len + span - 2) // span + 1, count - first)
     out = context_lens.new_empty(B, KV, max(count, 0))
-    scratch = q.new_empty(_L.load().ssdk_select_spans_scratch_bytes(B, KV, block_size, width, span) // 2)
+    scratch = q.new_empty(_select_scratch(B, KV, block_size, width, span))
     _launch("ssdk_select_spans", gpu, q.data_ptr(), bounds.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(),
             scratch.data_ptr(), B, q_len, H, KV, hd, block_size, width, n, span, count, first, last)
     return out
