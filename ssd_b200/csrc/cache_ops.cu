@@ -63,8 +63,8 @@ static Launcher launcher(void* stream) {
 constexpr int kSms = 148, kMaxSmem = 227 * 1024 - 1024;   // (statics beside it)
 constexpr int kMaxListed = 4096;   // spans of a list
 // Blocks that share the listed keys of a key head (a cluster).  Two blocks are resident on an SM, so that units x blocks take waves; a block's start and end
-// cost as much as some 512 keys, and the join grows with the blocks.  us for one, two, four, eight blocks: 48 sequences of 8 key heads and 4096 keys 159, 136,
-// 148, 184; one sequence of 8 key heads and 2048 keys 28.7, 17.6, 11.4, 8.6 (sixteen: 9.0); 8 x 7 rows over 8 key heads and 4096 keys (tiles) 96, 54, 36.
+// cost as much as some 512 keys, and the join grows with the blocks.  us for one, two, four, eight blocks: 48 sequences of 8 key heads and 4096 keys 143, 131,
+// 145, 178; one sequence of 8 key heads and 2048 keys 24.9, 15.9, 10.8, 8.1 (sixteen: 8.6); 8 x 7 rows over 8 key heads and 4096 keys (tiles) 77, 46, 34, 44.
 static int span_cluster(int64_t units, int64_t keys, int most) {
   int best = 1;
   int64_t least = INT64_MAX;
