@@ -8,7 +8,8 @@
 // A chunk of 64 keys is gathered from the listed spans by TMA boxes of gcd(span, 64) keys, in list order; what is missing from the last
 // chunk is loaded from behind the cache (zeros) and masked.  A cluster of blocks shares the chunks of a key head; their sums meet in shared memory.
 // Up to sixteen rows span_attn_kernel is as fast as the memory; with more its mma.sync products bound it: 8 sequences of 7 rows, 64 heads over 8 of 128,
-// 4096 listed keys each: 63 us on two m16 tiles a warp, 33.4 here (32 sequences: 105 us, 79 % of the copy rate).
+// 4096 listed keys each: 63 us on two m16 tiles a warp, 33.2 here (32 sequences: 98 us, 85 % of the copy rate).  Of these 33 a block takes 5 until its first scores are
+// weights, 24 for its 16 chunks and 6 to join; a chunk waits for its keys as long as two stages in flight make it (a third does not fit twice on an SM), its exponentials take 700 of 2700 clocks.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -199,18 +200,20 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const int lim = len - p.Q + tok0 + r / G + 1;        // first position this row does not see (rows behind the tile's: some, dropped)
     const int seen_by_all = len - p.Q + tok0 + 1;        // positions below it are seen by every row
     ok = in;
+    // the lane's box of a chunk, of the spans and of the boxes of a span (advancing by a chunk's boxes without a division)
+    const int step_i = boxes / per, step_r = boxes - step_i * per;
+    int at_i = (first * boxes + lane) / per, at_r = first * boxes + lane - at_i * per;
     for (int i = 0; i < n && in; ++i) {
       const uint32_t sp = tmem + lanes + (uint32_t)(i & 1) * 64u;
-      // positions of the chunk's keys, sixteen at a time
-      const int piece = (first + i) * boxes;
-      const int mine = lane < boxes ? box_at(piece + lane).y : 0;
-      const bool whole = __all_sync(0xffffffffu, lane >= boxes || mine + box <= seen_by_all);
-      int pos[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int at = 16 * j / box;
-        pos[j] = __shfl_sync(0xffffffffu, mine, at) + (16 * j - at * box);
+      // positions of the chunk's keys: a lane has a box's, sixteen keys' are taken from there where some row does not see all
+      const int mine = lane < boxes ? (at_i < spans ? where[at_i].y + at_r * box : kNoPosition) : 0;
+      at_i += step_i;
+      at_r += step_r;
+      if (at_r >= per) {
+        at_r -= per;
+        ++at_i;
       }
+      const bool whole = __all_sync(0xffffffffu, lane >= boxes || mine + box <= seen_by_all);
       if (!(ok = tile_wait_warp(&s_full[i & 1], parity(i), timeout))) break;
       tc_fence_after();
       uint32_t u[64];
@@ -221,7 +224,13 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
         for (int c = 0; c < 64; ++c) u[c] = (u[c] & p.q_keep) ^ (p.q_sign & 0x80000000u);
       }
+      int pos[4];   // of sixteen keys each
       if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int x = 16 * j / box;
+          pos[j] = __shfl_sync(0xffffffffu, mine, x) + (16 * j - x * box);
+        }
 #pragma unroll
         for (int c = 0; c < 64; ++c)
           if (pos[c / 16] + c % 16 >= lim) u[c] = 0xff800000u;   // -inf
