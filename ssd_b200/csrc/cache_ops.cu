@@ -105,15 +105,15 @@ static int launch_span_tiles(Launcher& L, SpanAttnParams p) {
 
 template <int HD>
 static int launch_rope_axes(Launcher& L, RopeAxesParams p) {
-  // a row's heads to one warp when the rows fill the SMs (20 warps each), else as many warps as ask for all of them at once
-  const int n = p.heads + 2 * p.kv_heads, at_once = rope_axes_heads(HD), batches = (n + at_once - 1) / at_once;
-  const int most = (int)std::min<int64_t>(batches, std::max<int64_t>(1, (int64_t)kSms * 20 / p.M));
-  p.per = (batches + most - 1) / most * at_once;
-  p.shares = (n + p.per - 1) / p.per;
+  const int n = p.heads + 2 * p.kv_heads;
+  p.batches = (n + rope_axes_heads(HD) - 1) / rope_axes_heads(HD);
   constexpr int W = kRopeAxesThreads / 32;
-  const int64_t units = (int64_t)p.M * p.shares;
-  if (units >= (1ll << 31) - W) return fail("rope_axes: %d rows of %d heads", p.M, n);
-  const dim3 grid((unsigned)((units + W - 1) / W)), block(kRopeAxesThreads);
+  const int64_t units = (int64_t)p.M * p.batches;
+  if (units >= (1ll << 31)) return fail("rope_axes: %d rows of %d heads", p.M, n);
+  p.warps = (int)std::min<int64_t>(units, kSms * 4 * W);   // four blocks on an SM
+  p.each = (int)(units / p.warps);
+  p.longer = (int)(units - (int64_t)p.each * p.warps);
+  const dim3 grid((unsigned)((p.warps + W - 1) / W)), block(kRopeAxesThreads);
   return p.q_norm_w || p.k_norm_w ? L.go(rope_axes_kernel<HD, true>, grid, block, 0, p) : L.go(rope_axes_kernel<HD, false>, grid, block, 0, p);
 }
 template <int HD>

@@ -141,9 +141,11 @@ __global__ void __launch_bounds__(kPlaceThreads) place_tokens_kernel(PlaceParams
 // rope_axes_kernel: frequency i turns the channels (i, i + rot/2) of every query and key head by the angle of the row's position on axis
 // axis_of[i] (time, height, width, ...); channels from rot on pass.  Optional RMS norm per head in front.  Norm, rotation and the table's cosines and
 // sines are fp32, and a value is rounded once, where it is stored.  Queries go to q, keys and values to their slot of the cache.
-// Bound by memory: 2 bytes read and 2 written per channel.  HD / 16 lanes own a head, 16 channels each in two 16-byte pieces.  A warp takes a row (or, when
-// rows are few, a share of its heads) and keeps the angles, four times 32 / (HD / 16) heads asked for at once, products and sums two at a time: with a row's heads
-// over four warps that gathered the angles through shared memory the instructions bound it (16000 rows of 32 heads of 128 with norms: 58 us, issue slots 70 % busy).
+// Bound by memory: 2 bytes read and 2 written per channel.  HD / 16 lanes own a head, 16 channels each in two 16-byte pieces, and a warp asks for a batch of
+// 2 * 32 / (HD / 16) heads at once, a batch ahead.  The rows' batches lie one behind the other and each warp has a stretch of them: the angles stay in registers for a row,
+// the next row's heads are on their way when it begins, and few rows still make as many warps as batches.  Products and sums two at a time.  16000 rows of 32 heads of 128
+// with norms 49.4 us (a warp per row 52; four warps a row that gathered the angles through shared memory 58, issue slots 70 % busy; norm weights of the queries kept in
+// registers 51), 4003 rows of 48 heads 20.9.
 // A row with a position outside the table has NaN queries and stores nothing.
 // ----------------------------------------------------------------------------------
 struct RopeAxesParams {
@@ -156,7 +158,8 @@ struct RopeAxesParams {
   int64_t top, num_slots;
   float eps;
   int M, heads, kv_heads, rot, axes;
-  int shares, per;               // warps of a row, heads of a warp (a multiple of the heads that it asks for at once)
+  int batches;                   // of heads that a warp asks for at once, in a row
+  int warps, each, longer;       // the rows' batches one behind the other: a warp has a stretch of `each`, the first `longer` one more
   uint32_t axis_of[8];           // two bits per frequency
 };
 constexpr int kRopeAxesThreads = 128, kRopeAxesAhead = 2;
@@ -191,69 +194,82 @@ __global__ void __launch_bounds__(kRopeAxesThreads, 4) rope_axes_kernel(RopeAxes
   constexpr int LPH = HD / 16, SIDE = 32 / LPH;   // lanes of a head, heads side by side
   pdl_wait();
   pdl_launch_dependents();
-  const int unit = (int)blockIdx.x * (kRopeAxesThreads / 32) + (int)(threadIdx.x >> 5);   // (below 2^31: the host sees to it)
-  const int m = unit / p.shares, share = unit - m * p.shares;
-  if (m >= p.M) return;
+  const int warp = (int)blockIdx.x * (kRopeAxesThreads / 32) + (int)(threadIdx.x >> 5);
+  if (warp >= p.warps) return;
+  int unit = warp * p.each + min(warp, p.longer);   // (below 2^31: the host sees to it)
+  const int last = unit + p.each + (warp < p.longer);
   const int piece = threadIdx.x % LPH, side = threadIdx.x % 32 / LPH, half = p.rot / 2;
-  const int n_heads = p.heads + 2 * p.kv_heads, first = share * p.per, end = min(first + p.per, n_heads);
+  const int n_heads = p.heads + 2 * p.kv_heads;
   const bool turns = piece < p.rot / 16;
   const int c0 = turns ? piece * 8 : p.rot + (piece - p.rot / 16) * 16, c1 = turns ? half + piece * 8 : c0 + 8;
-  const __nv_bfloat16* src = p.qkv + (size_t)m * n_heads * HD;
 
   uint4 a[kRopeAxesAhead], b[kRopeAxesAhead];
-  auto load = [&](int head0) {
+  auto load = [&](int m, int batch) {
+    const __nv_bfloat16* src = p.qkv + (size_t)m * n_heads * HD;
 #pragma unroll
     for (int i = 0; i < kRopeAxesAhead; ++i) {
-      const int head = head0 + i * SIDE + side;
+      const int head = (batch * kRopeAxesAhead + i) * SIDE + side;
       a[i] = b[i] = make_uint4(0, 0, 0, 0);
-      if (head < end) {
+      if (head < n_heads) {
         a[i] = ld_nc_v4(src + head * HD + c0);
         b[i] = ld_nc_v4(src + head * HD + c1);
       }
     }
   };
-  load(first);
-  const int slot = p.slots[m];
-  bool known = true;
-  for (int x = 0; x < p.axes; ++x) {
-    const int64_t at = p.positions[(size_t)x * p.M + m];
-    known = known && at >= 0 && at < p.top;
-  }
+  int m = unit / p.batches, batch = unit - m * p.batches, row = -1;
+  load(m, batch);
+  bool known = true, stores = false;
   uint64_t co[4] = {}, si[4] = {}, minus[4] = {};   // cos, sin, -sin of this lane's eight frequencies
-  if (turns && known) {
-    const uint32_t axes = (p.axis_of[piece >> 1] >> (16 * (piece & 1))) & 0xffffu;
-    if (axes == (axes & 3) * 0x5555u) {
-      const float* row = p.table + (size_t)p.positions[(size_t)(axes & 3) * p.M + m] * p.rot + piece * 8;
-#pragma unroll
-      for (int i = 0; i < 4; i += 2) {
-        const float4 c = *reinterpret_cast<const float4*>(row + 2 * i), s = *reinterpret_cast<const float4*>(row + half + 2 * i);
-        co[i] = pack2(c.x, c.y); co[i + 1] = pack2(c.z, c.w);
-        si[i] = pack2(s.x, s.y); si[i + 1] = pack2(s.z, s.w);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float* r0 = p.table + (size_t)p.positions[(size_t)(axes >> (4 * i) & 3) * p.M + m] * p.rot + piece * 8 + 2 * i;
-        const float* r1 = p.table + (size_t)p.positions[(size_t)(axes >> (4 * i + 2) & 3) * p.M + m] * p.rot + piece * 8 + 2 * i + 1;
-        co[i] = pack2(r0[0], r1[0]);
-        si[i] = pack2(r0[half], r1[half]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) minus[i] = si[i] ^ 0x8000000080000000ull;
-  }
-  const bool stores = known && slot >= 0 && slot < p.num_slots;
-  __nv_bfloat16* q_row = p.q + (size_t)m * p.heads * HD;
-  const size_t in_cache = (size_t)max(slot, 0) * p.kv_heads * HD;
+  __nv_bfloat16* q_row = p.q;
+  size_t in_cache = 0;
 
-  for (int head0 = first; head0 < end; head0 += kRopeAxesAhead * SIDE) {
+  for (; unit < last; ++unit) {
+    if (m != row) {
+      row = m;
+      const int slot = p.slots[m];
+      known = true;
+      for (int x = 0; x < p.axes; ++x) {
+        const int64_t at = p.positions[(size_t)x * p.M + m];
+        known = known && at >= 0 && at < p.top;
+      }
+      if (turns && known) {
+        const uint32_t axes = (p.axis_of[piece >> 1] >> (16 * (piece & 1))) & 0xffffu;
+        if (axes == (axes & 3) * 0x5555u) {
+          const float* angles = p.table + (size_t)p.positions[(size_t)(axes & 3) * p.M + m] * p.rot + piece * 8;
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const float4 c = *reinterpret_cast<const float4*>(angles + 2 * i), s = *reinterpret_cast<const float4*>(angles + half + 2 * i);
+            co[i] = pack2(c.x, c.y); co[i + 1] = pack2(c.z, c.w);
+            si[i] = pack2(s.x, s.y); si[i + 1] = pack2(s.z, s.w);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float* r0 = p.table + (size_t)p.positions[(size_t)(axes >> (4 * i) & 3) * p.M + m] * p.rot + piece * 8 + 2 * i;
+            const float* r1 = p.table + (size_t)p.positions[(size_t)(axes >> (4 * i + 2) & 3) * p.M + m] * p.rot + piece * 8 + 2 * i + 1;
+            co[i] = pack2(r0[0], r1[0]);
+            si[i] = pack2(r0[half], r1[half]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) minus[i] = si[i] ^ 0x8000000080000000ull;
+      }
+      stores = known && slot >= 0 && slot < p.num_slots;
+      q_row = p.q + (size_t)m * p.heads * HD;
+      in_cache = (size_t)max(slot, 0) * p.kv_heads * HD;
+    }
+    const int head0 = batch * kRopeAxesAhead * SIDE;
     uint4 now_a[kRopeAxesAhead], now_b[kRopeAxesAhead];
 #pragma unroll
     for (int i = 0; i < kRopeAxesAhead; ++i) {
       now_a[i] = a[i];
       now_b[i] = b[i];
     }
-    load(head0 + kRopeAxesAhead * SIDE);   // (behind the last head nothing)
+    if (++batch == p.batches) {
+      batch = 0;
+      ++m;
+    }
+    if (unit + 1 < last) load(m, batch);
 #pragma unroll
     for (int i = 0; i < kRopeAxesAhead; ++i) {
       const int head = head0 + i * SIDE + side, kind = head < p.heads ? 0 : (head < p.heads + p.kv_heads ? 1 : 2);   // q, k, v
@@ -300,7 +316,7 @@ __global__ void __launch_bounds__(kRopeAxesThreads, 4) rope_axes_kernel(RopeAxes
           if (!known) x = y = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
         }
       }
-      if (head < end && (kind == 0 || stores)) {
+      if (head < n_heads && (kind == 0 || stores)) {
         __nv_bfloat16* dst = kind == 0 ? q_row + head * HD : (kind == 1 ? p.k_cache + in_cache + (head - p.heads) * HD : p.v_cache + in_cache + (head - p.heads - p.kv_heads) * HD);
         *reinterpret_cast<uint4*>(dst + c0) = x;
         *reinterpret_cast<uint4*>(dst + c1) = y;

@@ -89,7 +89,7 @@ int main(int argc, char** argv) {
     return 0;
   }
   if (mode == "rope") {
-    auto h = rd<int32_t>(f, 10);   // M H KV hd rot axes top num_slots norm most-shares
+    auto h = rd<int32_t>(f, 10);   // M H KV hd rot axes top num_slots norm most-warps
     auto eps = rd<float>(f, 1);
     const int hd = h.p[3], rot = h.p[4];
     ssdk::RopeAxesParams p;
@@ -104,12 +104,13 @@ int main(int argc, char** argv) {
     Exact<bf16> q((size_t)p.M * p.heads * hd), kc((size_t)p.num_slots * p.kv_heads * hd), vc((size_t)p.num_slots * p.kv_heads * hd);
     p.qkv = qkv.p; p.positions = positions.p; p.slots = slots.p; p.table = table.p; p.q = q.p; p.k_cache = kc.p; p.v_cache = vc.p;
     p.q_norm_w = h.p[8] ? qn.p : nullptr; p.k_norm_w = h.p[8] ? kn.p : nullptr;
-    // shares of a row, as the host cuts it
-    const int n = p.heads + 2 * p.kv_heads, at_once = ssdk::rope_axes_heads(hd), batches = (n + at_once - 1) / at_once, most = std::min(batches, h.p[9]);
-    p.per = (batches + most - 1) / most * at_once;
-    p.shares = (n + p.per - 1) / p.per;
+    const int n = p.heads + 2 * p.kv_heads, at_once = ssdk::rope_axes_heads(hd);
+    p.batches = (n + at_once - 1) / at_once;
+    p.warps = std::min(p.M * p.batches, h.p[9]);
+    p.each = p.M * p.batches / p.warps;
+    p.longer = p.M * p.batches % p.warps;
     dim3 grid;
-    grid.x = (unsigned)((p.M * p.shares + 3) / 4);
+    grid.x = (unsigned)((p.warps + 3) / 4);
     const auto kernel = hd == 64 ? (h.p[8] ? ssdk::rope_axes_kernel<64, true> : ssdk::rope_axes_kernel<64, false>)
                                  : (h.p[8] ? ssdk::rope_axes_kernel<128, true> : ssdk::rope_axes_kernel<128, false>);
     emu::launch(kernel, p, grid, ssdk::kRopeAxesThreads, 0, 8);
