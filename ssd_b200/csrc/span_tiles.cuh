@@ -4,12 +4,14 @@
 // queries lie in rows 0 .. 63 and again in 64 .. 127: these make the low bf16 pieces of the weights, add up in lanes of their own and are added at the
 // end.  (With a row's keys shared by its two lanes, zeros in P at the other's keys and the two pieces in a product each, the exponentials halve and the
 // products double: 37.0 us against 36.5 where this is 36.5, one warp issuing; tensor and shared memory are what two blocks share.)  Scores and products with V are issued
-// by a warp each, with one commit a product: one thread that issued both and looked at five barriers a chunk held it at 2500 clocks a chunk (36.5 -> 33.4 us).
+// by a warp each, with one commit a product: one thread that issued both and looked at five barriers a chunk held it at 2500 clocks a chunk (36.5 -> 33.4 us at the time).
 // A chunk of 64 keys is gathered from the listed spans by TMA boxes of gcd(span, 64) keys, in list order; what is missing from the last
 // chunk is loaded from behind the cache (zeros) and masked.  A cluster of blocks shares the chunks of a key head; their sums meet in shared memory.
 // Up to sixteen rows span_attn_kernel is as fast as the memory; with more its mma.sync products bound it: 8 sequences of 7 rows, 64 heads over 8 of 128,
-// 4096 listed keys each: 63 us on two m16 tiles a warp, 33.2 here (32 sequences: 98 us, 85 % of the copy rate).  Of these 33 a block takes 5 until its first scores are
-// weights, 24 for its 16 chunks and 6 to join; a chunk waits for its keys as long as two stages in flight make it (a third does not fit twice on an SM), its exponentials take 700 of 2700 clocks.
+// 4096 listed keys each: 63 us on two m16 tiles a warp, 32.7 here (32 sequences: 99 us, 84 % of the copy rate).  Of these 33 a block takes 5 until its first scores are
+// weights, some 22 for its 16 chunks and 6 to join.  Keys and values are asked for by a warp each, the moment that their stage is read: one thread for both, with a division a box,
+// asked for a chunk's keys 1200 clocks late (33.5 us; 32 sequences 102; boxes of 16 keys, one sequence of 160 rows, 32 -> 27).  Two stages of both are what fits twice on an SM; heads of
+// 64 have four (32 sequences 84.5 -> 81).
 #pragma once
 #include <cooperative_groups.h>
 
@@ -18,11 +20,12 @@
 
 namespace ssdk {
 
-constexpr int kTileRows64 = 64, kTileKeys = 64, kTileStages = 2, kTileThreads = 224;   // warps: loads, scores, 4 of softmax, products with V
+constexpr int kTileRows64 = 64, kTileKeys = 64, kTileThreads = 256;   // warps: loads of keys, scores, 4 of softmax, products with V, loads of values
 constexpr int kNoPosition = 0x7fffff00;   // of a key that is not there: behind every context
 constexpr int kTileMost = 16;   // blocks of a cluster
+constexpr int tile_stages(int HD) { return HD == 64 ? 4 : 2; }   // of keys and of values: as many as fit when two blocks share an SM
 // query twice | keys and values; behind them the places of the listed spans
-constexpr int span_tile_body(int HD) { return 2 * kTileRows64 * HD * 2 + kTileStages * 2 * kTileKeys * HD * 2; }
+constexpr int span_tile_body(int HD) { return 2 * kTileRows64 * HD * 2 + tile_stages(HD) * 2 * kTileKeys * HD * 2; }
 constexpr int span_tile_smem(int HD, int count) { return span_tile_body(HD) + 1024 + count * 8; }
 
 // A bounded wait (about two seconds; then the word is set and false comes back): the clock is read only where the first look fails.
@@ -44,15 +47,16 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                  const int box, const int q_tokens, unsigned* timeout) {
   namespace cg = cooperative_groups;
   constexpr int HALVES = HD / 64;                    // 64-column boxes of a row
+  constexpr int STAGES = tile_stages(HD);
   constexpr int kQHalf = 2 * kTileRows64 * 128, kKHalf = kTileKeys * 128, kTile = HALVES * kKHalf;
   extern __shared__ uint8_t span_tile_raw[];
-  __shared__ __align__(8) uint64_t q_full, k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2];
+  __shared__ __align__(8) uint64_t q_full, k_full[STAGES], v_full[STAGES], k_free[STAGES], v_free[STAGES], s_full[2], p_full[2], pv_done[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int s_failed, s_odd, found[kTileThreads / 32];   // s_odd: values were taken out
   uint8_t* smem = span_tile_raw + ((1024u - (smem_u32(span_tile_raw) & 1023u)) & 1023u);
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + HALVES * kQHalf;
-  uint8_t* sV = sK + kTileStages * kTile;
+  uint8_t* sV = sK + STAGES * kTile;
   int2* where = reinterpret_cast<int2*>(smem + span_tile_body(HD));   // [count] slot and position of the first key of a span that is there
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank();
@@ -67,9 +71,8 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
     mbar_init(&q_full, 1);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&k_full[s], 1); mbar_init(&v_full[s], 1); mbar_init(&s_full[s], 1); mbar_init(&p_full[s], live); mbar_init(&pv_done[s], 1);
-    }
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&k_full[s], 1); mbar_init(&v_full[s], 1); mbar_init(&k_free[s], 1); mbar_init(&v_free[s], 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&p_full[s], live); mbar_init(&pv_done[s], 1); }
     fence_mbar_init();
     s_failed = s_odd = 0;
   }
@@ -112,54 +115,49 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   const int per = p.span / box, boxes = kTileKeys / box, pieces = spans * per;   // boxes of a span, of a chunk, in all
   const int chunks = (pieces + boxes - 1) / boxes, share = (chunks + C - 1) / C;
   const int first = rank * share, n = max(0, min(share, chunks - first));
-  // slot and position of a box: behind the last one no keys
-  auto box_at = [&](int piece) {
-    if (piece >= pieces) return make_int2((int)(p.num_blocks * p.block_size), kNoPosition);
-    const int i = piece / per, off = (piece - i * per) * box;
-    const int2 at = where[i];
-    return make_int2(at.x + off, at.y + off);
-  };
-  // Chunk i on barrier i & 1; parity(i) is that use's.  A wait by parity is only right while the barrier is in that use or the one behind it:
-  //   k_full, v_full, p_full: whoever waits for chunk i has to be through with it before the stage, or P, is made anew for chunk i + 2.
-  //   s_full: the softmax asks for chunk i, and scores of chunk i + 2 need its P (through pv_done of chunk i); the loads ask for chunk i - 2 before they bring
-  //     the keys that scores of chunk i need.
-  //   pv_done: the scores of chunk i + 1 ask for chunk i - 1, the softmax of chunk i for chunk i - 1 or nothing, the loads of chunk i for chunk i - 2, the end for
-  //     chunk n - 1.  Chunk i + 1's product, the next on that barrier, needs the P of chunk i + 1, so its scores, so the first of them; the P of a warp that
-  //     has not gone on, so the second; and the values of chunk i + 1, so the third.
+  // Chunk i's scores, weights and product on barrier i & 1, parity(i) is that use's; its keys and values in stage i % STAGES, turn(i).  A wait by parity is only right
+  // while the barrier is in that use or the one behind it:
+  //   k_full, v_full, p_full: whoever waits for chunk i has to be through with it before the stage, or P, is made anew.
+  //   k_free, v_free (with two stages s_full and pv_done): the loads ask for chunk i - STAGES before they bring what the next use of that barrier needs.
+  //   s_full: the softmax asks for chunk i, and scores of chunk i + 2 need its P (through pv_done of chunk i).
+  //   pv_done: the scores of chunk i + 1 ask for chunk i - 1, the softmax of chunk i for chunk i - 1 or nothing, the end for
+  //     chunk n - 1.  Chunk i + 1's product, the next on that barrier, needs the P of chunk i + 1, so its scores, so the first of them; and the P of a warp that
+  //     has not gone on, so the second.
   auto parity = [](int i) { return (uint32_t)(i >> 1) & 1u; };
+  auto turn = [](int i) { return (uint32_t)(i / STAGES) & 1u; };
   float l = 0.f, m = -INFINITY;
   bool ok = true;
   const int q4 = warp & 3, r = (q4 & 1) * 32 + lane;
   const bool softmax = warp >= 2 && warp < 6, second = q4 >= 2, in = softmax && (r & ~31) < half;   // (whole warps) second: the same row as two warps before, its low pieces
   const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
 
-  if (warp == 0) {
+  if (warp == 0 || warp == 7) {
     if (lane == 0) {
-      int i = 0;
+      const CUtensorMap* tm = warp ? &tmV : &tmK;
+      uint8_t* ring = warp ? sV : sK;
+      uint64_t *full = warp ? v_full : k_full, *free = STAGES == 2 ? (warp ? pv_done : s_full) : (warp ? v_free : k_free);
+      int i = 0, at_i = first * boxes / per, at_r = first * boxes - at_i * per;
       for (; i < n; ++i) {
-        const int s = i & 1;
-        int slots[4];
+        const int s = i % STAGES;
+        int slots[4];   // of the chunk's boxes, behind the last one no keys
 #pragma unroll
-        for (int j = 0; j < 4; ++j) slots[j] = j < boxes ? box_at((first + i) * boxes + j).x : 0;
-        if (i > 1 && !tile_wait(&s_full[s], parity(i - 2), timeout)) break;   // the keys of chunk i - 2 have been read
-        mbar_arrive_expect_tx(&k_full[s], kTile);
+        for (int j = 0; j < 4; ++j) {
+          slots[j] = at_i < spans ? where[at_i].x + at_r * box : (int)(p.num_blocks * p.block_size);
+          if (j < boxes && ++at_r == per) {
+            at_r = 0;
+            ++at_i;
+          }
+        }
+        if (i >= STAGES && !tile_wait(&free[s], turn(i - STAGES), timeout)) break;   // chunk i - STAGES has been read
+        mbar_arrive_expect_tx(&full[s], kTile);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (j < boxes)
-            for (int h = 0; h < HALVES; ++h) tma_load_3d(sK + s * kTile + h * kKHalf + j * box * 128, &tmK, &k_full[s], h * 64, kvh, slots[j]);
-        if (i > 1 && !tile_wait(&pv_done[s], parity(i - 2), timeout)) { tile_wait(&k_full[s], parity(i), timeout); break; }
-        mbar_arrive_expect_tx(&v_full[s], kTile);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j < boxes)
-            for (int h = 0; h < HALVES; ++h) tma_load_3d(sV + s * kTile + h * kKHalf + j * box * 128, &tmV, &v_full[s], h * 64, kvh, slots[j]);
+            for (int h = 0; h < HALVES; ++h) tma_load_3d(ring + s * kTile + h * kKHalf + j * box * 128, tm, &full[s], h * 64, kvh, slots[j]);
       }
       // nothing is in flight into this block's memory when it leaves, also after a wait ran out
-      tile_wait(&q_full, 0, timeout);
-      for (int j = max(0, i - 2); j < i; ++j) {
-        tile_wait(&k_full[j & 1], parity(j), timeout);
-        tile_wait(&v_full[j & 1], parity(j), timeout);
-      }
+      if (warp == 0) tile_wait(&q_full, 0, timeout);
+      for (int j = max(0, i - STAGES); j < i; ++j) tile_wait(&full[j % STAGES], turn(j), timeout);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -169,15 +167,16 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       for (int i = 0; i < n && go; ++i) {
         // the scores of chunk i go over the P that the product of chunk i - 2 reads
         if (i > 1 && !(go = tile_wait(&pv_done[i & 1], parity(i - 2), timeout))) break;
-        if (!(go = tile_wait(&k_full[i & 1], parity(i), timeout))) break;
+        if (!(go = tile_wait(&k_full[i % STAGES], turn(i), timeout))) break;
         tc_fence_after();
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
-          const uint64_t qd = make_umma_desc_k128(sQ + h * kQHalf), kd = make_umma_desc_k128(sK + (i & 1) * kTile + h * kKHalf);
+          const uint64_t qd = make_umma_desc_k128(sQ + h * kQHalf), kd = make_umma_desc_k128(sK + i % STAGES * kTile + h * kKHalf);
 #pragma unroll
           for (int k = 0; k < 4; ++k) umma_bf16_ss(tmem + (i & 1) * 64, qd + 2 * k, kd + 2 * k, idesc_s, (uint32_t)((h | k) != 0));
         }
         umma_commit(&s_full[i & 1]);
+        if (STAGES > 2) umma_commit(&k_free[i % STAGES]);
       }
     }
     __syncwarp();
@@ -186,13 +185,14 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       constexpr uint32_t idesc_o = make_umma_idesc_bf16(2 * kTileRows64, HD) | (1u << 16);   // V: b_major = MN
       bool go = true;
       for (int i = 0; i < n && go; ++i) {
-        if (!(go = tile_wait(&v_full[i & 1], parity(i), timeout) && tile_wait(&p_full[i & 1], parity(i), timeout))) break;
+        if (!(go = tile_wait(&v_full[i % STAGES], turn(i), timeout) && tile_wait(&p_full[i & 1], parity(i), timeout))) break;
         tc_fence_after();
-        const uint64_t vd = make_umma_desc_mn128(sV + (i & 1) * kTile, kKHalf);
+        const uint64_t vd = make_umma_desc_mn128(sV + i % STAGES * kTile, kKHalf);
 #pragma unroll
         for (int k = 0; k < kTileKeys / 16; ++k)   // 16 keys: 2048 B of V, 8 columns of P
           umma_bf16_ts(tmem_o, tmem + (i & 1) * 64 + 8 * k, vd + 128 * k, idesc_o, (uint32_t)((i | k) != 0));
         umma_commit(&pv_done[i & 1]);
+        if (STAGES > 2) umma_commit(&v_free[i % STAGES]);
       }
     }
     __syncwarp();
@@ -266,14 +266,14 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
         for (int j = 0; j < 4; ++j) stale = stale || (pos[j] < kNoPosition && pos[j] + 16 > edge);
         if (stale) {   // (the same for all warps)
-          if (!(ok = tile_wait_warp(&v_full[i & 1], parity(i), timeout))) break;
+          if (!(ok = tile_wait_warp(&v_full[i % STAGES], turn(i), timeout))) break;
           bool odd = false;
           for (int j = second ? half + r : r; j < kTileKeys * 8; j += live) {
             const int key = j >> 3, x = key >> 4, at = (x == 0 ? pos[0] : x == 1 ? pos[1] : x == 2 ? pos[2] : pos[3]) + (key & 15);
             if (at >= edge)
 #pragma unroll
               for (int h = 0; h < HALVES; ++h) {
-                uint4* v = reinterpret_cast<uint4*>(sV + (i & 1) * kTile + h * kKHalf + j * 16);
+                uint4* v = reinterpret_cast<uint4*>(sV + i % STAGES * kTile + h * kKHalf + j * 16);
                 if (at >= len) *v = make_uint4(0u, 0u, 0u, 0u);
                 else odd |= take_out(v);
               }
