@@ -116,12 +116,21 @@ static int launch_rope_axes(Launcher& L, RopeAxesParams p) {
   const dim3 grid((unsigned)((p.warps + W - 1) / W)), block(kRopeAxesThreads);
   return p.q_norm_w || p.k_norm_w ? L.go(rope_axes_kernel<HD, true>, grid, block, 0, p) : L.go(rope_axes_kernel<HD, false>, grid, block, 0, p);
 }
+// One launch while an SM brings in a head's bounds about as fast as a second launch begins.  us on the device, two kernels and one: contexts of 250 spans, 8 heads 8.4 and
+// 7.8, 64 heads 9.4 and 8.3; of 500, 144 heads 14.4 and 11.9; of 1000, 64 heads 14.5 and 14.0, but 8 heads 9.0 and 12.6 (2 us less of the host either way).
+constexpr int kOwnSpans = 512;
 template <int HD>
 static int launch_select(Launcher& L, const SelectParams& p) {
-  static std::atomic<bool> done[64];
-  CKI(with_smem(span_pick_kernel<HD>, kMaxSmem, kSmemOnly, done));
   constexpr int W = kEstimateThreads / 32;
   const int64_t rows = (int64_t)p.Q * (p.heads / p.kv_heads);
+  const dim3 heads(p.kv_heads, p.B);
+  if (rows <= 8 && p.max_spans <= kOwnSpans && (int64_t)p.kv_heads * p.B <= kSms) {
+    static std::atomic<bool> own_done[64];
+    CKI(with_smem(span_pick_kernel<HD, true>, kMaxSmem, kSmemOnly, own_done));
+    return L.go(span_pick_kernel<HD, true>, heads, dim3(kPickThreads), pick_smem(p.max_spans, rows, HD), p);
+  }
+  static std::atomic<bool> done[64];
+  CKI(with_smem(span_pick_kernel<HD, false>, kMaxSmem, kSmemOnly, done));
   const dim3 grid(rows > 8 ? p.warps / W : (p.warps * p.kv_heads + W - 1) / W, rows > 8 ? p.kv_heads : 1, p.B), block(kEstimateThreads);
   if (rows > 8) {
     static std::atomic<bool> many_done[64];
@@ -130,7 +139,7 @@ static int launch_select(Launcher& L, const SelectParams& p) {
   } else {
     CKI(L.go(span_estimate_kernel<HD, false>, grid, block, 0, p));
   }
-  return L.go(span_pick_kernel<HD>, dim3(p.kv_heads, p.B), dim3(kPickThreads), pick_smem(p.max_spans, rows, HD), p);
+  return L.go(span_pick_kernel<HD, false>, heads, dim3(kPickThreads), pick_smem(p.max_spans, rows, HD), p);
 }
 // Warps to a key head, which go over its groups of sixteen spans in turns: as many as make the fewest turns and waves (two blocks on an SM), a block's start and the
 // query's fragments as long as two turns.  us for 1, 2, 4, 6, 8, 11 turns of 24 contexts of 64000 (8 key heads): 49.3, 42.7, 40.4, 39.2, 41.4, 39.2; 8 of them 24.7, 22.9, 21.7,

@@ -20,7 +20,7 @@ namespace ssdk {
 // in between in 64 bits (products of bf16 values are exact, sums of 128 of them off by 2^-46).  Where values are not finite, or so large that 32 bits
 // overflow, it scores all.
 // Two kernels, the second's start under the first's end: the estimates fill all SMs in even shares whatever the number of heads, and what picks is one block
-// of a head.  24 contexts of 64000 tokens (150 MB of bounds): 39 us, of it 8 the second's.  The first has its loads in flight one turn at a time (registers hold one);
+// of a head (short tables: the block that picks makes its estimates itself).  24 contexts of 64000 tokens (150 MB of bounds): 39 us, of it 8 the second's.  The first has its loads in flight one turn at a time (registers hold one);
 // a ring of cp.async stages, each lane its own pieces or a span's bounds by whole lines, was slower: 49 and 41 us.
 // ----------------------------------------------------------------------------------
 struct SelectParams {
@@ -141,23 +141,14 @@ SSDK_DEVINL const __nv_bfloat16* bounds_at(const SelectParams& p, int page, int 
   return p.bounds + (((size_t)page * subs + (s - sub_page(p, s) * subs)) * p.kv_heads + head) * 2 * HD;
 }
 
-// MANY: more than eight rows, whose fragments lie in shared memory
-template <int HD, bool MANY>
-__global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(SelectParams p) {
-  extern __shared__ __align__(16) uint2 frags[];   // [tiles][2 CH][32]
+// A warp: the estimates of the groups `group`, `group` + step, ... of sixteen spans of a key head, put(s, bits) by one lane; returns the largest |lo|, |hi| seen (bits
+// of bf16).  MANY: more than eight rows, whose fragments the block's warps put into shared memory (all of them are here).
+template <int HD, bool MANY, typename Put>
+SSDK_DEVINL uint32_t estimate_groups(const SelectParams& p, int b, int head, int n, int group, int step, uint2* frags, Put put) {   // frags [tiles][2 CH][32]
   constexpr int CH = HD / 32;   // 16-byte pieces of a lane per bound
-  constexpr int W = kEstimateThreads / 32;
-  pdl_wait();
-  pdl_launch_dependents();
-  const int b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  // neighbouring warps take neighbouring heads, whose bounds of a span lie together (MANY: a block's warps share the fragments of their head)
-  const int unit = blockIdx.x * W + warp, head = MANY ? (int)blockIdx.y : unit % p.kv_heads, slot = MANY ? unit : unit / p.kv_heads;
-  if (slot >= p.warps) return;   // (MANY: none)
-  const int n = (tokens_of(p.lens, b, p.max_blocks, p.block_size) + p.span - 1) / p.span, groups = (n + 15) / 16;
-  if (n <= p.count) return;   // all are listed
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, groups = (n + 15) / 16;
   const int G = p.heads / p.kv_heads, rows = G * p.Q, tiles = (rows + 7) / 8, subs = p.block_size / p.span;
   const int32_t* table = p.tables + (size_t)b * p.max_blocks;
-  uint32_t* estimates = p.estimates + ((size_t)b * p.kv_heads + head) * p.max_spans;
   // where the bounds of span s start (in channels; negative: no such span, or on no page)
   auto place_of = [&](int s) {
     const int entry = sub_page(p, s), page = s < n ? page_at(table + entry, p.num_blocks) : -1;
@@ -177,11 +168,10 @@ __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(Sele
   };
   auto negative = [](const uint2& f) { return make_uint2(min_bf16x2(f.x, 0u), min_bf16x2(f.y, 0u)); };
   auto positive = [](const uint2& f) { return make_uint2(max_bf16x2(f.x, 0u), max_bf16x2(f.y, 0u)); };
-  int group = slot;
   long long at0 = place_of(group * 16 + g), at1 = place_of(group * 16 + 8 + g);
   uint2 qf[2 * CH];
   if (MANY) {   // every tile's fragments into shared memory, a tile per warp
-    for (int tile = warp; tile < tiles; tile += W) {
+    for (int tile = threadIdx.x >> 5; tile < tiles; tile += (int)(blockDim.x >> 5)) {
       load_q(tile, qf);
 #pragma unroll
       for (int k = 0; k < 2 * CH; ++k) frags[(tile * 2 * CH + k) * 32 + lane] = qf[k];
@@ -191,7 +181,7 @@ __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(Sele
     load_q(0, qf);
   }
   uint32_t bottom = 0, top = 0;   // two channels: smallest lower, largest upper bound
-  for (; group < groups; group += p.warps) {
+  for (; group < groups; group += step) {
     const int s0 = group * 16 + g, s1 = s0 + 8;
     const bool there0 = at0 >= 0, there1 = at1 >= 0;
     const __nv_bfloat16 *both0 = p.bounds + at0 + 8 * t, *both1 = p.bounds + at1 + 8 * t;
@@ -201,8 +191,8 @@ __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(Sele
       u[i] = there0 ? ld_nc_v4(both0 + 32 * i) : make_uint4(0, 0, 0, 0);
       v[i] = there1 ? ld_nc_v4(both1 + 32 * i) : make_uint4(0, 0, 0, 0);
     }
-    at0 = place_of(s0 + 16 * p.warps);
-    at1 = place_of(s1 + 16 * p.warps);
+    at0 = place_of(s0 + 16 * step);
+    at1 = place_of(s1 + 16 * step);
     float best[2] = {-INFINITY, -INFINITY};   // spans g, g + 8
     for (int tile = 0; tile < (MANY ? tiles : 1); ++tile) {
       float c[2][4] = {};
@@ -236,16 +226,33 @@ __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(Sele
     }
     if (t < 2) {
       const int s = t ? s1 : s0;
-      if (s < n) estimates[s] = (t ? there1 : there0) ? __float_as_uint(t ? best[1] : best[0]) : kNoSpan;
+      if (s < n) put(s, (t ? there1 : there0) ? __float_as_uint(t ? best[1] : best[0]) : kNoSpan);
     }
   }
   const uint32_t both = max_bf16x2(bottom & 0x7fff7fffu, top);   // (top is not negative; NaN is above infinity above all)
-  const uint32_t most = __reduce_max_sync(0xffffffffu, max(both & 0xffffu, both >> 16));
-  if (lane == 0) p.wide[((size_t)b * p.kv_heads + head) * p.warps + slot] = most << 16;
+  return __reduce_max_sync(0xffffffffu, max(both & 0xffffu, both >> 16));
 }
 
-template <int HD>
-__global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams p) {
+template <int HD, bool MANY>
+__global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(SelectParams p) {
+  extern __shared__ __align__(16) uint2 frags[];
+  constexpr int W = kEstimateThreads / 32;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int b = blockIdx.z;
+  // neighbouring warps take neighbouring heads, whose bounds of a span lie together (MANY: a block's warps share the fragments of their head)
+  const int unit = blockIdx.x * W + (int)(threadIdx.x >> 5), head = MANY ? (int)blockIdx.y : unit % p.kv_heads, slot = MANY ? unit : unit / p.kv_heads;
+  if (slot >= p.warps) return;   // (MANY: none)
+  const int n = (tokens_of(p.lens, b, p.max_blocks, p.block_size) + p.span - 1) / p.span;
+  if (n <= p.count) return;   // all are listed
+  uint32_t* estimates = p.estimates + ((size_t)b * p.kv_heads + head) * p.max_spans;
+  const uint32_t most = estimate_groups<HD, MANY>(p, b, head, n, slot, p.warps, frags, [&](int s, uint32_t e) { estimates[s] = e; });
+  if ((threadIdx.x & 31) == 0) p.wide[((size_t)b * p.kv_heads + head) * p.warps + slot] = most << 16;
+}
+
+// OWN: the block makes the estimates itself, where a head's are few and heads fewer than SMs: one launch
+template <int HD, bool OWN>
+__global__ void __launch_bounds__(kPickThreads, OWN ? 1 : 2) span_pick_kernel(SelectParams p) {
   extern __shared__ __align__(16) uint8_t pick_smem_bytes[];
   __shared__ int sums[4 * kPickWarps], pick_bin, n_sure, n_open;
   __shared__ int4 stats[kPickWarps];
@@ -259,13 +266,19 @@ __global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams
   uint32_t* between = taken + words;
   int* bins = reinterpret_cast<int*>(between + words);
   const int head = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (OWN) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
   const int n = (tokens_of(p.lens, b, p.max_blocks, p.block_size) + p.span - 1) / p.span;
   const int32_t* table = p.tables + (size_t)b * p.max_blocks;
   int32_t* out = p.out + ((size_t)b * p.kv_heads + head) * p.count;
 
   if (n <= p.count) {   // all of them
-    pdl_wait();
-    pdl_launch_dependents();
+    if (!OWN) {
+      pdl_wait();
+      pdl_launch_dependents();
+    }
     for (int base = warp * 32; base < n; base += kPickThreads) {
       const int s = base + lane;
       const uint32_t m = __ballot_sync(0xffffffffu, s < n && page_at(table + sub_page(p, s), p.num_blocks) >= 0);
@@ -291,22 +304,28 @@ __global__ void __launch_bounds__(kPickThreads, 2) span_pick_kernel(SelectParams
     const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(size));   // (NaN above infinity above all)
     if (lane == 0) atomicMax(&q_most, most);
   }
-  pdl_wait();   // the estimates are there (what is read above was there before they began: see launcher())
-  pdl_launch_dependents();
+  uint32_t wide = 0;
+  if (OWN) {
+    wide = estimate_groups<HD, false>(p, b, head, n, warp, kPickWarps, nullptr, [&](int s, uint32_t e) { estimate[s] = e; }) << 16;
+    __syncthreads();
+  } else {
+    pdl_wait();   // the estimates are there (what is read above was there before they began: see launcher())
+    pdl_launch_dependents();
+    for (int i = threadIdx.x; i < p.warps; i += kPickThreads) wide = max(wide, __ldcg(p.wide + ((size_t)b * p.kv_heads + head) * p.warps + i));
+  }
 
   auto kept = [&](int s) { return s < p.first || s >= n - p.last; };
   int always = 0, others = 0;
-  uint32_t lowest = ~0u, highest = 0, wide = 0;
-  for (int i = threadIdx.x; i < p.warps; i += kPickThreads) wide = max(wide, __ldcg(p.wide + ((size_t)b * p.kv_heads + head) * p.warps + i));
+  uint32_t lowest = ~0u, highest = 0;
   const uint32_t* estimates = p.estimates + ((size_t)b * p.kv_heads + head) * p.max_spans;
   for (int base = threadIdx.x; base < n; base += 4 * kPickThreads) {   // four at a time
     uint32_t e[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = base + i * kPickThreads < n ? __ldcg(estimates + base + i * kPickThreads) : kNoSpan;
+    for (int i = 0; i < 4; ++i) e[i] = base + i * kPickThreads >= n ? kNoSpan : OWN ? estimate[base + i * kPickThreads] : __ldcg(estimates + base + i * kPickThreads);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int s = base + i * kPickThreads;
-      if (s < n) estimate[s] = e[i];
+      if (!OWN && s < n) estimate[s] = e[i];
       const bool there = e[i] != kNoSpan, keep = kept(s);
       always += there && keep;
       others += there && !keep;

@@ -206,12 +206,14 @@ def test_select_spans_batch(dev, q_len, count):
     _select(dev, q, _bounds(g, total, S // span, KV, hd), table, lens, q_len, S, count)
 
 
-def test_select_spans_ties_and_odd_values(dev):
-    """Whole numbers make equal scores: the lowest index goes first.  Zeros of both signs are equal, NaN is above all, infinities are in order."""
+@pytest.mark.parametrize("width", [None, 200])
+def test_select_spans_ties_and_odd_values(dev, width):
+    """Whole numbers make equal scores: the lowest index goes first.  Zeros of both signs are equal, NaN is above all, infinities are in order.  Short tables take one
+    kernel, wide ones two."""
     g = gen(11)
     S, span, KV, hd, H = 64, 16, 2, 64, 8
     lens = [40 * span, 40 * span - 3, 17]
-    table, total = tables(g, lens, S)
+    table, total = tables(g, lens, S, width=width)
     for kind in range(6):
         q = torch.randint(-1, 2, (3, H, hd), generator=g).to(BF)
         both = torch.randint(-1, 2, (total, S // span, KV, 2, hd), generator=g).to(BF)
@@ -249,11 +251,12 @@ def test_select_spans_close_scores(dev):
         _select(dev, q, both, table, [n * span], 1, S, count)
 
 
-def test_select_spans_bad_pages(dev):
+@pytest.mark.parametrize("width", [10, 300])
+def test_select_spans_bad_pages(dev, width):
     g = gen(13)
     S, span, KV, hd = 32, 16, 2, 64
     lens = [300, 299, -4, 100000]
-    table, total = tables(g, [300, 299, 0, 320], S, width=10)
+    table, total = tables(g, [300, 299, 0, 320], S, width=width)
     table[0, 2], table[0, 5], table[1, 0], table[1, 9], table[3, 4] = total, -9, 2147483647, -2147483648, total + 1
     q = torch.randn(4, 4, hd, generator=g).to(BF)
     for count in (4, 30):
