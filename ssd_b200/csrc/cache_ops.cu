@@ -288,7 +288,7 @@ int ssdk_span_attn(const void* q, const void* k_cache, const void* v_cache, cons
   p.q = (const bf16*)q; p.k_cache = (const bf16*)k_cache; p.v_cache = (const bf16*)v_cache; p.tables = block_tables; p.lens = context_lens;
   p.spans = selected; p.out = (bf16*)out; p.num_blocks = num_blocks; p.B = batch; p.Q = q_len; p.heads = heads; p.kv_heads = kv_heads;
   p.block_size = block_size; p.span = span; p.max_blocks = max_blocks_per_seq; p.count = count; p.scale_log2 = scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f;
-  p.q_sign = scale < 0.f ? 0x80008000u : 0u; p.q_keep = scale == 0.f ? 0u : ~0u;
+  p.q_sign = scale < 0.f ? 0x80008000u : 0u; p.zero_scale = scale == 0.f;
   Launcher L = launcher(stream);
   if (G * (int64_t)q_len <= 16) return head_dim == 64 ? launch_span_attn<64>(L, p) : launch_span_attn<128>(L, p);
   return head_dim == 64 ? launch_span_tiles<64>(L, p) : launch_span_tiles<128>(L, p);

@@ -481,8 +481,9 @@ struct SpanAttnParams {
   int64_t num_blocks;
   int B, Q, heads, kv_heads, block_size, span, max_blocks, count;
   int tokens;                    // query tokens of a tile
-  uint32_t q_sign, q_keep;       // the sign of the scale, for two bf16 values; 0 where the scale is 0
-  float scale_log2;              // |scale| * log2(e), or 1
+  uint32_t q_sign;               // the sign of the scale, for two bf16 values
+  bool zero_scale;
+  float scale_log2;              // |scale| * log2(e), or 1 where the scale is 0
 };
 // Values that are not finite.  A product with the weight 0 of a query that does not see their token is NaN, so from the first token on that some query does not see
 // they go into the product as 0 (take_out), and a row adds those that it sees where it is stored (add_taken_out), read from the cache again.  Where every query sees them the
@@ -500,6 +501,8 @@ SSDK_DEVINL bool take_out(uint4* at) {
   if (some) *at = make_uint4(w[0], w[1], w[2], w[3]);
   return some;
 }
+// 0 times two bf16 values: NaN where one is not finite, so that its row's scores are
+SSDK_DEVINL uint32_t zero_times(uint32_t w) { return (not_finite(w) ? 0x7fffu : 0u) | (not_finite(w >> 16) ? 0x7fff0000u : 0u); }
 // four columns of a row that sees the tokens below lim; all queries see those below `from`.  odd: values were taken out; l: the row's sum
 __device__ __noinline__ float4 with_taken_out(const SpanAttnParams& p, int head_dim, int b, int kvh, int from, int lim, int d, float4 acc) {
   float out[4] = {acc.x, acc.y, acc.z, acc.w}, sum[4] = {};
@@ -584,8 +587,15 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(const __g
     const __nv_bfloat16* q = p.q + ((size_t)(b * p.Q + r / G) * p.heads + kvh * G + r % G) * HD + 2 * t;
 #pragma unroll
     for (int kk = 0; kk < KS; ++kk) {
-      qa[kk][h] = r < R ? (*reinterpret_cast<const uint32_t*>(q + kk * 16) & p.q_keep) ^ p.q_sign : 0u;
-      qa[kk][2 + h] = r < R ? (*reinterpret_cast<const uint32_t*>(q + kk * 16 + 8) & p.q_keep) ^ p.q_sign : 0u;
+      qa[kk][h] = r < R ? *reinterpret_cast<const uint32_t*>(q + kk * 16) ^ p.q_sign : 0u;
+      qa[kk][2 + h] = r < R ? *reinterpret_cast<const uint32_t*>(q + kk * 16 + 8) ^ p.q_sign : 0u;
+    }
+    if (p.zero_scale) {   // (scale_log2 is 1: 0 times the mask's minus infinity would be NaN)
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) {
+        qa[kk][h] = zero_times(qa[kk][h]);
+        qa[kk][2 + h] = zero_times(qa[kk][2 + h]);
+      }
     }
     lim[h] = r < R ? len - p.Q + r / G + 1 : 0;
   }

@@ -220,9 +220,12 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
       for (int c = 0; c < 64; c += 16) tmem_ld_32x32b_x16(sp + c, u + c);
       tmem_ld_wait();
-      if (p.q_sign || !p.q_keep) {   // a scale that is not positive
+      if (p.zero_scale) {   // (NaN where a score is not finite)
 #pragma unroll
-        for (int c = 0; c < 64; ++c) u[c] = (u[c] & p.q_keep) ^ (p.q_sign & 0x80000000u);
+        for (int c = 0; c < 64; ++c) u[c] = __float_as_uint(__uint_as_float(u[c]) * 0.f);
+      } else if (p.q_sign) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c) u[c] ^= 0x80000000u;
       }
       int pos[4];   // of sixteen keys each
       if (!whole) {
