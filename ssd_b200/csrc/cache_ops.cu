@@ -279,15 +279,16 @@ int ssdk_span_attn(const void* q, const void* k_cache, const void* v_cache, cons
   CKI(check_pages("span_attn", batch, block_size, max_blocks_per_seq, num_blocks));
   CKI(check_spans("span_attn", heads, kv_heads, head_dim, block_size, span));
   const int G = heads / kv_heads;
-  if (q_len < 1 || count < 1 || count > kMaxListed || G > 32 || !std::isfinite(scale))
-    return fail("span_attn: q_len=%d, %d spans (at most %d), %d query heads to a key head (at most 32), scale %g", q_len, count, kMaxListed, G, (double)scale);
+  const float scale_log2 = fabsf(scale) * 1.4426950408889634f;
+  if (q_len < 1 || count < 1 || count > kMaxListed || G > 32 || !std::isfinite(scale_log2))
+    return fail("span_attn: q_len=%d, %d spans (at most %d), %d query heads to a key head (at most 32), scale %g (finite, log2(e) times it too)", q_len, count, kMaxListed, G, (double)scale);
   if ((int64_t)count * span >= (1ll << 31) || (int64_t)batch * q_len >= (1ll << 31)) return fail("span_attn: %d spans of %d tokens, %d rows of %d sequences", count, span, q_len, batch);
   if (!q || !k_cache || !v_cache || !block_tables || !context_lens || !selected || !out) return fail("span_attn: null argument");
   if (off16(q, k_cache, v_cache, out)) return fail("span_attn: arrays must start at multiples of 16 bytes");
   SpanAttnParams p;
   p.q = (const bf16*)q; p.k_cache = (const bf16*)k_cache; p.v_cache = (const bf16*)v_cache; p.tables = block_tables; p.lens = context_lens;
   p.spans = selected; p.out = (bf16*)out; p.num_blocks = num_blocks; p.B = batch; p.Q = q_len; p.heads = heads; p.kv_heads = kv_heads;
-  p.block_size = block_size; p.span = span; p.max_blocks = max_blocks_per_seq; p.count = count; p.scale_log2 = scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f;
+  p.block_size = block_size; p.span = span; p.max_blocks = max_blocks_per_seq; p.count = count; p.scale_log2 = scale == 0.f ? 1.f : scale_log2;
   p.q_sign = scale < 0.f ? 0x80008000u : 0u; p.zero_scale = scale == 0.f;
   Launcher L = launcher(stream);
   if (G * (int64_t)q_len <= 16) return head_dim == 64 ? launch_span_attn<64>(L, p) : launch_span_attn<128>(L, p);
