@@ -1,8 +1,10 @@
 // span_ops.cuh — attention over a part of a long paged cache: spans of keys are chosen by a bound on their scores, and attention reads the chosen ones only.
 #pragma once
+#ifndef SSDK_HOST_EMU
 #include <cooperative_groups.h>
 
 #include "async_copy.cuh"
+#endif
 #include "cache_ops.cuh"
 #include "common.cuh"
 
@@ -235,7 +237,7 @@ SSDK_DEVINL uint32_t estimate_groups(const SelectParams& p, int b, int head, int
 
 template <int HD, bool MANY>
 __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(SelectParams p) {
-  extern __shared__ __align__(16) uint2 frags[];
+  SSDK_DYN_SMEM(uint2, frags);
   constexpr int W = kEstimateThreads / 32;
   pdl_wait();
   pdl_launch_dependents();
@@ -253,10 +255,14 @@ __global__ void __launch_bounds__(kEstimateThreads, 2) span_estimate_kernel(Sele
 // OWN: the block makes the estimates itself, where a head's are few and heads fewer than SMs: one launch
 template <int HD, bool OWN>
 __global__ void __launch_bounds__(kPickThreads, OWN ? 1 : 2) span_pick_kernel(SelectParams p) {
-  extern __shared__ __align__(16) uint8_t pick_smem_bytes[];
-  __shared__ int sums[4 * kPickWarps], pick_bin, n_sure, n_open;
-  __shared__ int4 stats[kPickWarps];
-  __shared__ uint32_t wides[kPickWarps], q_most;   // bits of the largest |lo|, |hi| of a warp's share, and of the largest sum of |q| over a row
+  SSDK_DYN_SMEM(uint8_t, pick_smem_bytes);
+  SSDK_STATIC_SMEM(int, sums, 4 * kPickWarps);
+  SSDK_SHARED_VAR(int, pick_bin);
+  SSDK_SHARED_VAR(int, n_sure);
+  SSDK_SHARED_VAR(int, n_open);
+  SSDK_STATIC_SMEM(int4, stats, kPickWarps);
+  SSDK_STATIC_SMEM(uint32_t, wides, kPickWarps);   // bits of the largest |lo|, |hi| of a warp's share
+  SSDK_SHARED_VAR(uint32_t, q_most);               // and of the largest sum of |q| over a row
   const int G = p.heads / p.kv_heads, rows = G * p.Q, padded = (rows + 7) / 8 * 8;
   const int words = (p.max_spans + 31) / 32;
   __nv_bfloat16* q_rows = reinterpret_cast<__nv_bfloat16*>(pick_smem_bytes);   // [padded][HD]
@@ -418,8 +424,12 @@ __global__ void __launch_bounds__(kPickThreads, OWN ? 1 : 2) span_pick_kernel(Se
     for (int i = warp; i < m; i += kPickWarps) {
       const int s = span_of(i);
       if (s < 0) continue;
-      const __nv_bfloat16* both = bounds_at(p, page_at(table + sub_page(p, s), p.num_blocks), s, head, HD);
-      const unsigned long long key = finite ? exact_score<HD, true>(both, q_rows, rows) : exact_score<HD, false>(both, q_rows, rows);
+      unsigned long long key = 0;
+      const int page = page_at(table + sub_page(p, s), p.num_blocks);
+      if (page >= 0) {   // (it was when the estimate was made, unless the table has changed since)
+        const __nv_bfloat16* both = bounds_at(p, page, s, head, HD);
+        key = finite ? exact_score<HD, true>(both, q_rows, rows) : exact_score<HD, false>(both, q_rows, rows);
+      }
       if (lane == 0) keys[i] = key;
     }
     __syncthreads();
@@ -463,6 +473,7 @@ __global__ void __launch_bounds__(kPickThreads, OWN ? 1 : 2) span_pick_kernel(Se
   pick_write(taken, n_words, out, p.count, sums + 2 * kPickWarps);
 }
 
+#ifndef SSDK_HOST_EMU
 // ----------------------------------------------------------------------------------
 // span_attn_kernel: softmax(scale q k^T) v over the keys of the listed spans, causal to the end of the context as in paged attention (query j of a sequence
 // sees positions <= len - Q + j); grouped heads.  A list may name spans in any order; what lies outside the context or on a page outside the cache
@@ -819,5 +830,6 @@ __global__ void __launch_bounds__(kSpanWarps * 32, 2) span_attn_kernel(const __g
   }
   cluster.sync();   // no block leaves while its part is read
 }
+#endif  // SSDK_HOST_EMU
 
 }  // namespace ssdk
