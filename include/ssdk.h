@@ -284,7 +284,7 @@ int ssdk_prompt_attn(const void* q, const void* k_cache, const void* v_cache,
  *   positions int64 [rows], slot_mapping int32 [rows] (-1: its page is none of the cache's num_blocks), row_seqs int32 [rows]: the new tokens
  *   of the placed sequences one behind the other; rows behind the last: 0, -1, -1.  cu_rows [batch + 1]: first row of a sequence.
  *   lens [batch]: context_lens + new_lens, of sequences that are not placed context_lens.  used [1]: free_used and the pages handed out.
- *   lens and used are arrays of their own. */
+ * Here and in the entry points below what is written shares no memory with anything else that the call is given. */
 int ssdk_place_tokens(const int32_t* context_lens, const int32_t* new_lens, int32_t* block_tables, const int32_t* free_blocks,
                       const int32_t* free_used, int64_t* positions, int32_t* slot_mapping, int32_t* row_seqs, int32_t* cu_rows,
                       int32_t* lens, int32_t* used, int batch, int max_blocks_per_seq, int n_free, int rows, int block_size,
@@ -293,8 +293,7 @@ int ssdk_place_tokens(const int32_t* context_lens, const int32_t* new_lens, int3
 /* ssdk_rope_store_kv with positions on several axes (1 to 4: time, height, width, ...): positions int64 [axes, M]; frequency i turns by
  * positions[axis_of[i], m] (axis_of: host bytes [rot_dim / 2]).  rope_table fp32 [max_pos, rot_dim] cos | sin; the first rot_dim channels of
  * a head turn (i with i + rot_dim / 2), the others pass.  Norm and rotation in fp32, one rounding.  A row with a position outside
- * the table has NaN queries and stores nothing; slots below 0 or from num_slots on store nothing; slots of a call are distinct, q_out is an
- * array of its own. */
+ * the table has NaN queries and stores nothing; slots below 0 or from num_slots on store nothing; slots of a call are distinct. */
 int ssdk_rope_axes_store_kv(const void* qkv, const int64_t* positions, int axes, const uint8_t* axis_of, const int32_t* slot_mapping,
                             const float* rope_table, int64_t max_pos, int rot_dim, const void* q_norm_w, const void* k_norm_w,
                             float norm_eps, void* q_out, void* k_cache, void* v_cache, int64_t num_slots, int M, int heads,
@@ -318,7 +317,7 @@ int ssdk_select_spans(const void* q, const void* bounds, const int32_t* block_ta
                       int max_blocks_per_seq, int64_t num_blocks, int span, int count, int first, int last, void* stream);
 /* ssdk_span_attn: ssdk_paged_attn over the keys of the listed spans only.  Entries outside the context, or on pages outside the cache, are
  * passed over; a span that is listed twice counts twice; a row that sees no key is zero.  Keys and values that a row does not see are of no account to it, whatever
- * they hold; NaN that it sees makes NaN, a value of infinity stays one (with a scale of 0 a key or query of infinity makes NaN too).  At most 32 query heads to a key head, 4096 spans.
+ * they hold; NaN that it sees makes NaN, a value of infinity stays one (with a scale of 0 a key or query of infinity makes NaN too).  At most 32 query heads to a key head, 4096 spans; out may be q itself.
  * More than sixteen query rows to a key head take a kernel with bounded waits: as with ssdk_paged_attn_pages, a wait that runs out leaves NaN
  * rows, and the next such call of the process returns an error. */
 int ssdk_span_attn(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables, const int32_t* context_lens,

@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <numeric>
 
 #include "../../include/ssdk.h"
@@ -17,9 +18,25 @@ typedef __nv_bfloat16 bf16;
 static bool off16(const void* a, const void* b = nullptr, const void* c = nullptr, const void* d = nullptr) {
   return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) & 15) != 0;
 }
-// do n bytes at a and m bytes at b share some
-static bool overlap(const void* a, int64_t n, const void* b, int64_t m) {
-  return (uintptr_t)a < (uintptr_t)b + (uintptr_t)m && (uintptr_t)b < (uintptr_t)a + (uintptr_t)n;
+// An array of a call.  What is written lies apart from everything else: other blocks still read the inputs, or write the other outputs, while one writes.
+struct Array {
+  const char* name;
+  const void* at;
+  int64_t bytes;
+};
+static bool overlap(const Array& a, const Array& b) {
+  return a.at && b.at && (uintptr_t)a.at < (uintptr_t)b.at + (uintptr_t)b.bytes && (uintptr_t)b.at < (uintptr_t)a.at + (uintptr_t)a.bytes;
+}
+static int check_apart(const char* who, std::initializer_list<Array> written, std::initializer_list<Array> read) {
+  for (const Array* w = written.begin(); w != written.end(); ++w) {
+    const Array* other = nullptr;
+    for (const Array* x = w + 1; x != written.end(); ++x)
+      if (overlap(*w, *x)) other = x;
+    for (const Array& x : read)
+      if (overlap(*w, x)) other = &x;
+    if (other) return fail("%s: %s lies over %s (an output needs memory of its own, inputs keep theirs: arrays of their own)", who, w->name, other->name);
+  }
+  return 0;
 }
 // a cache whose slots are numbered in 32 bits, and tables over it
 static int check_pages(const char* who, int batch, int block_size, int max_blocks, int64_t num_blocks) {
@@ -177,9 +194,11 @@ int ssdk_place_tokens(const int32_t* context_lens, const int32_t* new_lens, int3
   if (batch > kPlaceMaxSeqs || rows < 1 || rows > (1 << 30) || n_free < 0) return fail("place_tokens: %d sequences (at most %d), %d rows, %d free pages", batch, kPlaceMaxSeqs, rows, n_free);
   if (!context_lens || !new_lens || !block_tables || !free_used || (n_free && !free_blocks) || !positions || !slot_mapping || !row_seqs || !cu_rows || !lens || !used)
     return fail("place_tokens: null argument");
-  // (every block reads the lengths and the pages handed out while the first one writes)
-  if (overlap(lens, 4ll * batch, context_lens, 4ll * batch) || overlap(lens, 4ll * batch, new_lens, 4ll * batch) || overlap(used, 4, free_used, 4))
-    return fail("place_tokens: lens and used need arrays of their own");
+  const int64_t n_seq = batch, n_rows = rows;
+  CKI(check_apart("place_tokens",
+                  {{"block_tables", block_tables, n_seq * max_blocks_per_seq * 4}, {"positions", positions, n_rows * 8}, {"slot_mapping", slot_mapping, n_rows * 4},
+                   {"row_seqs", row_seqs, n_rows * 4}, {"cu_rows", cu_rows, (n_seq + 1) * 4}, {"lens", lens, n_seq * 4}, {"used", used, 4}},
+                  {{"context_lens", context_lens, n_seq * 4}, {"new_lens", new_lens, n_seq * 4}, {"free_blocks", free_blocks, 4ll * n_free}, {"free_used", free_used, 4}}));
   PlaceParams p;
   p.ctx = context_lens; p.fresh = new_lens; p.tables = block_tables; p.free_blocks = free_blocks; p.free_used = free_used;
   p.positions = positions; p.slots = slot_mapping; p.seqs = row_seqs; p.cu = cu_rows; p.lens = lens; p.used = used;
@@ -197,11 +216,14 @@ int ssdk_rope_axes_store_kv(const void* qkv, const int64_t* positions, int axes,
   if (M < 1 || heads < 1 || kv_heads < 1 || (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return fail("rope_axes: %d rows of %d heads over %d of %d (64, 128 or 256)", M, heads, kv_heads, head_dim);
   if (rot_dim < 16 || rot_dim % 16 || rot_dim > head_dim) return fail("rope_axes: %d rotated channels of %d (a multiple of 16)", rot_dim, head_dim);
-  if (axes < 1 || axes > 4 || max_pos < 1 || num_slots < 1) return fail("rope_axes: %d axes (1 to 4), %lld positions, %lld slots", axes, (long long)max_pos, (long long)num_slots);
+  if (axes < 1 || axes > 4 || max_pos < 1 || max_pos >= (1ll << 40) || num_slots < 1 || num_slots >= (1ll << 40)) return fail("rope_axes: %d axes (1 to 4), %lld positions, %lld slots", axes, (long long)max_pos, (long long)num_slots);
   if (heads + 2 * (int64_t)kv_heads > 65535) return fail("rope_axes: too many heads");
   if (!qkv || !positions || !axis_of || !slot_mapping || !rope_table || !q_out || !k_cache || !v_cache) return fail("rope_axes: null argument");
   if (off16(qkv, q_out, k_cache, v_cache) || off16(q_norm_w, k_norm_w, rope_table)) return fail("rope_axes: arrays must start at multiples of 16 bytes");
-  if (overlap(q_out, 2ll * M * heads * head_dim, qkv, 2ll * M * (heads + 2 * (int64_t)kv_heads) * head_dim)) return fail("rope_axes: q_out needs an array of its own");
+  const int64_t row = 2ll * M * head_dim, cache = 2 * num_slots * kv_heads * head_dim;
+  CKI(check_apart("rope_axes", {{"q_out", q_out, row * heads}, {"k_cache", k_cache, cache}, {"v_cache", v_cache, cache}},
+                  {{"qkv", qkv, row * (heads + 2 * (int64_t)kv_heads)}, {"positions", positions, 8ll * axes * M}, {"slot_mapping", slot_mapping, 4ll * M},
+                   {"rope_table", rope_table, 4 * max_pos * rot_dim}, {"q_norm_w", q_norm_w, 2ll * head_dim}, {"k_norm_w", k_norm_w, 2ll * head_dim}}));
   RopeAxesParams p;
   memset(&p, 0, sizeof(p));
   for (int i = 0; i < rot_dim / 2; ++i) {
@@ -226,6 +248,9 @@ int ssdk_span_bounds(const void* k_cache, const int32_t* block_tables, const int
   if (new_tokens < 1) return fail("span_bounds: %d new tokens", new_tokens);
   if (!k_cache || !block_tables || !context_lens || !bounds) return fail("span_bounds: null argument");
   if (off16(k_cache, bounds)) return fail("span_bounds: arrays must start at multiples of 16 bytes");
+  const int64_t token = 2ll * kv_heads * head_dim, n_spans = num_blocks * (block_size / span);
+  CKI(check_apart("span_bounds", {{"bounds", bounds, n_spans * 2 * token}},
+                  {{"k_cache", k_cache, num_blocks * block_size * token}, {"block_tables", block_tables, 4ll * batch * max_blocks_per_seq}, {"context_lens", context_lens, 4ll * batch}}));
   SpanBoundsParams p;
   p.k_cache = (const bf16*)k_cache; p.tables = block_tables; p.lens = context_lens; p.bounds = (bf16*)bounds; p.num_blocks = num_blocks;
   p.B = batch; p.max_blocks = max_blocks_per_seq; p.block_size = block_size; p.span = span; p.kv_heads = kv_heads; p.head_dim = head_dim;
@@ -261,6 +286,10 @@ int ssdk_select_spans(const void* q, const void* bounds, const int32_t* block_ta
   const int64_t rows = (int64_t)q_len * (heads / kv_heads);
   if (rows > 4096 || pick_smem((int)max_spans, rows, head_dim) > kMaxSmem || estimate_smem(rows, head_dim) > kMaxSmem)
     return fail("select_spans: %lld query rows to a key head beside tables of %lld spans pass the shared memory", (long long)rows, (long long)max_spans);
+  CKI(check_apart("select_spans", {{"selected", selected, 4ll * batch * kv_heads * count},
+                                   {"scratch", scratch, ssdk_select_spans_scratch_bytes(batch, kv_heads, block_size, max_blocks_per_seq, span)}},
+                  {{"q", q, 2ll * batch * q_len * heads * head_dim}, {"bounds", bounds, num_blocks * (block_size / span) * kv_heads * 4ll * head_dim},
+                   {"block_tables", block_tables, 4ll * batch * max_blocks_per_seq}, {"context_lens", context_lens, 4ll * batch}}));
   SelectParams p;
   p.sub_magic = ((1ull << 32) + block_size / span - 1) / (block_size / span);
   p.q = (const bf16*)q; p.bounds = (const bf16*)bounds; p.tables = block_tables; p.lens = context_lens; p.out = selected;
@@ -285,6 +314,11 @@ int ssdk_span_attn(const void* q, const void* k_cache, const void* v_cache, cons
   if ((int64_t)count * span >= (1ll << 31) || (int64_t)batch * q_len >= (1ll << 31)) return fail("span_attn: %d spans of %d tokens, %d rows of %d sequences", count, span, q_len, batch);
   if (!q || !k_cache || !v_cache || !block_tables || !context_lens || !selected || !out) return fail("span_attn: null argument");
   if (off16(q, k_cache, v_cache, out)) return fail("span_attn: arrays must start at multiples of 16 bytes");
+  // (a row's query is read before its output is written, by the blocks that write it: out may be q itself)
+  const int64_t rows = 2ll * batch * q_len * heads * head_dim, cache = num_blocks * block_size * kv_heads * 2ll * head_dim;
+  CKI(check_apart("span_attn", {{"out", out, rows}},
+                  {{"q", out == q ? nullptr : q, rows}, {"k_cache", k_cache, cache}, {"v_cache", v_cache, cache}, {"block_tables", block_tables, 4ll * batch * max_blocks_per_seq},
+                   {"context_lens", context_lens, 4ll * batch}, {"selected", selected, 4ll * batch * kv_heads * count}}));
   SpanAttnParams p;
   p.q = (const bf16*)q; p.k_cache = (const bf16*)k_cache; p.v_cache = (const bf16*)v_cache; p.tables = block_tables; p.lens = context_lens;
   p.spans = selected; p.out = (bf16*)out; p.num_blocks = num_blocks; p.B = batch; p.Q = q_len; p.heads = heads; p.kv_heads = kv_heads;

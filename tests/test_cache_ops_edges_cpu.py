@@ -18,3 +18,36 @@ def test_scales_past_32_bits_in_base_2(scale):
     """Scores are scaled by scale log2(e): where that is infinite a score of 0 would be NaN."""
     for q_len in (1, 40):
         _refused("ssdk_span_attn", [P * i for i in range(1, 8)] + [2, q_len, 4, 2, 64, 32, 2, 4, 16, 3, scale, None], "scale")
+
+
+# (arguments, {index: bytes} of the arrays that are written, of those that are read, pairs that may be one array)
+M = 1 << 20
+APART = {
+    "ssdk_place_tokens": ([M * i for i in range(1, 12)] + [2, 4, 8, 6, 16, 8, None], {2: 32, 5: 48, 6: 24, 7: 24, 8: 12, 9: 8, 10: 4}, {0: 8, 1: 8, 3: 32, 4: 4}, ()),
+    "ssdk_rope_axes_store_kv": ([M, 2 * M, 2, bytes(32), 3 * M, 4 * M, 10, 64, 5 * M, 6 * M, 1e-6, 7 * M, 8 * M, 9 * M, 32, 3, 2, 1, 64, None],
+                                {11: 768, 12: 4096, 13: 4096}, {0: 1536, 1: 48, 4: 12, 5: 2560, 8: 128, 9: 128}, ()),
+    "ssdk_span_bounds": ([M, 2 * M, 3 * M, 4 * M, 2, 1, 2, 64, 32, 2, 4, 16, None], {3: 4096}, {0: 32768, 1: 16, 2: 8}, ()),
+    "ssdk_select_spans": ([M, 2 * M, 3 * M, 4 * M, 5 * M, 6 * M, 2, 1, 4, 2, 64, 32, 2, 4, 16, 3, 1, 1, None], {4: 48, 5: 192}, {0: 1024, 1: 4096, 2: 16, 3: 8}, ()),
+    "ssdk_span_attn": ([M, 2 * M, 3 * M, 4 * M, 5 * M, 6 * M, 7 * M, 2, 1, 4, 2, 64, 32, 2, 4, 16, 3, 0.1, None], {6: 1024}, {0: 1024, 1: 32768, 2: 32768, 3: 16, 4: 8, 5: 48}, ((6, 0),)),
+}
+
+
+@pytest.mark.parametrize("name", sorted(APART))
+def test_outputs_over_other_arrays(name):
+    """Every output beside every other array of a call: sharing its first or its last sixteen bytes is refused."""
+    from ssd_b200 import lib
+    so = lib.load()
+    good, written, read, one = APART[name]
+    sizes = {**read, **written}
+    for w in written:
+        for other in sizes:
+            if other == w:
+                continue
+            for at in (good[other], good[other] + (sizes[other] - 1) // 16 * 16, good[other] - (written[w] - 1) // 16 * 16):
+                args = list(good)
+                args[w] = at
+                if (w, other) in one and at == good[other]:
+                    continue
+                _refused(name, args, "of its own")
+    if name == "ssdk_select_spans":
+        assert so.ssdk_select_spans_scratch_bytes(2, 2, 32, 2, 16) == written[5]
