@@ -179,7 +179,9 @@ def verify(logits_p: torch.Tensor, logits_q: torch.Tensor, speculations: torch.T
 
 # ---- around a long paged cache: places of a step's tokens, positions with several axes, attention over selected spans ----
 _BF, _I32, _I64, _F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
-_gpu_now, _stream_of = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# private functions, since small calls are bound by the host; a PyTorch that lacks them (one without CUDA does) takes the public ones
+_gpu_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", lambda gpu: torch.cuda.current_stream(gpu).cuda_stream)
 
 
 def _check(name: str, *args) -> int:

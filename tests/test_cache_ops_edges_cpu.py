@@ -1,6 +1,11 @@
 """Refusals of the operators around a long paged cache that need no GPU."""
+import os
+import subprocess
+import sys
+
 import pytest
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 P = 4096   # an address that no call below gets to use
 
 
@@ -51,3 +56,23 @@ def test_outputs_over_other_arrays(name):
                 _refused(name, args, "of its own")
     if name == "ssdk_select_spans":
         assert so.ssdk_select_spans_scratch_bytes(2, 2, 32, 2, 16) == written[5]
+
+
+def test_import_without_the_private_names():
+    """A PyTorch that lacks the two private functions of its CUDA build (one without CUDA does) imports the module, and a call says what it needs."""
+    code = """
+import torch
+for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+    if hasattr(torch._C, name):
+        delattr(torch._C, name)
+from ssd_b200 import ops
+one = torch.zeros(1, dtype=torch.int32)
+try:
+    ops.place_tokens(one, one, one[None], one, one, 1, 16, 1)
+except RuntimeError as e:
+    assert "CUDA" in str(e), e
+else:
+    raise SystemExit("no error")
+"""
+    res = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0, res.stderr[-2000:]
