@@ -179,6 +179,7 @@ def verify(logits_p: torch.Tensor, logits_q: torch.Tensor, speculations: torch.T
 
 # ---- around a long paged cache: places of a step's tokens, positions with several axes, attention over selected spans ----
 _BF, _I32, _I64, _F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
+_TOP = 1 << 31   # numbers from here on, and below -_TOP, would be cut to 32 bits without a word
 # private functions, since small calls are bound by the host; a PyTorch that lacks them (one without CUDA does) takes the public ones
 _gpu_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", lambda gpu: torch.cuda.current_stream(gpu).cuda_stream)
@@ -201,6 +202,10 @@ def _check(name: str, *args) -> int:
     if gpu < 0:
         raise RuntimeError(f"{name}: CUDA tensors required (libssdk has no CPU path)")
     return gpu
+
+
+def _past_32_bits(name: str, *values: int):
+    raise ValueError(f"{name}: {max(values, key=abs)} passes 32 bits")
 
 
 def _last(t: torch.Tensor, dims: int) -> int:
@@ -231,6 +236,8 @@ def place_tokens(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table
     cu_rows int32 [B + 1], lens int32 [B] (context_lens + new_lens; sequences that found no pages or rows: context_lens) and the
     new free_used.  Sequences are served in order, each as a whole: see ssdk_place_tokens (include/ssdk.h)."""
     B, width, F = _last(context_lens, 1), _last(block_tables, 2), _last(free_blocks, 1)
+    if not (-_TOP <= rows < _TOP and -_TOP <= block_size < _TOP):
+        _past_32_bits("place_tokens", rows, block_size)
     gpu = _check("place_tokens", (context_lens, "context_lens", _I32, (B,)), (new_lens, "new_lens", _I32, (B,)),
                  (block_tables, "block_tables", _I32, (B, width)), (free_blocks, "free_blocks", _I32, (F,)), (free_used, "free_used", _I32, (1,)))
     if rows < 1:
@@ -281,11 +288,15 @@ def span_bounds(bounds: torch.Tensor, k_cache: torch.Tensor, block_tables: torch
     n, block_size, KV, hd = k_cache.shape if k_cache.dim() == 4 else (-1,) * 4
     subs = bounds.shape[1] if bounds.dim() == 5 else -1
     B, width = _last(context_lens, 1), _last(block_tables, 2)
+    if not -_TOP <= new_tokens < _TOP:
+        if new_tokens < 0:
+            _past_32_bits("span_bounds", new_tokens)
+        new_tokens = _TOP - 1
     if subs == 0 or block_size % subs:
         raise ValueError(f"span_bounds: pages of {block_size} tokens in {subs} spans")
     gpu = _check("span_bounds", (bounds, "bounds", _BF, (n, subs, KV, 2, hd)), (k_cache, "k_cache", _BF, (n, block_size, KV, hd)),
                  (block_tables, "block_tables", _I32, (B, width)), (context_lens, "context_lens", _I32, (B,)))
-    _launch("ssdk_span_bounds", gpu, k_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), bounds.data_ptr(), B, min(new_tokens, 2 ** 31 - 1), KV, hd,
+    _launch("ssdk_span_bounds", gpu, k_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), bounds.data_ptr(), B, new_tokens, KV, hd,
             block_size, width, n, block_size // subs)
     return bounds
 
@@ -305,6 +316,8 @@ def select_spans(q: torch.Tensor, bounds: torch.Tensor, block_tables: torch.Tens
     last: what span_attention takes.  The rows of a sequence share their spans."""
     n, subs, KV, _, hd = bounds.shape if bounds.dim() == 5 else (-1,) * 5
     B, width, H = _last(context_lens, 1), _last(block_tables, 2), q.shape[1] if q.dim() == 3 else -1
+    if not (-_TOP <= block_size < _TOP and -_TOP <= count < _TOP and -_TOP <= first < _TOP and (last is None or -_TOP <= last < _TOP)):
+        _past_32_bits("select_spans", block_size, count, first, last or 0)
     if subs == 0 or block_size % subs:
         raise ValueError(f"select_spans: pages of {block_size} tokens in {subs} spans")
     gpu = _check("select_spans", (q, "q", _BF, (B * q_len, H, hd)), (bounds, "bounds", _BF, (n, subs, KV, 2, hd)),
@@ -327,6 +340,8 @@ def span_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     that sees no key is zero."""
     n, block_size, KV, hd = cache = k_cache.shape if k_cache.dim() == 4 else (-1,) * 4
     B, width, H, count = _last(context_lens, 1), _last(block_tables, 2), q.shape[1] if q.dim() == 3 else -1, _last(spans, 3)
+    if not -_TOP <= span < _TOP:
+        _past_32_bits("span_attention", span)
     gpu = _check("span_attention", (q, "q", _BF, (B * q_len, H, hd)), (k_cache, "k_cache", _BF, cache), (v_cache, "v_cache", _BF, cache),
                  (block_tables, "block_tables", _I32, (B, width)), (context_lens, "context_lens", _I32, (B,)), (spans, "spans", _I32, (B, KV, count)))
     out = q.new_empty(B * q_len, H * hd)

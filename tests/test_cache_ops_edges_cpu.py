@@ -4,6 +4,9 @@ import subprocess
 import sys
 
 import pytest
+import torch
+
+from tests.cache_ops_util import BF
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 P = 4096   # an address that no call below gets to use
@@ -76,3 +79,23 @@ else:
 """
     res = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert res.returncode == 0, res.stderr[-2000:]
+
+
+@pytest.mark.parametrize("far", [(1 << 32) + 16, -(1 << 32) + 16])
+def test_numbers_past_32_bits(far):
+    """Whole numbers that the library's 32 bits would hold as another one (16)."""
+    from ssd_b200 import ops
+    ints = lambda *shape: torch.ones(*shape, dtype=torch.int32)  # noqa: E731
+    place = dict(context_lens=ints(2), new_lens=ints(2), block_tables=ints(2, 4), free_blocks=ints(8), free_used=ints(1), rows=16, block_size=16, num_blocks=8)
+    cache, both = torch.zeros(4, 32, 2, 64, dtype=BF), torch.zeros(4, 1, 2, 2, 64, dtype=BF)
+    q, lens, table = torch.zeros(2, 4, 64, dtype=BF), ints(2), ints(2, 2)
+    select = dict(q=q, bounds=both, block_tables=table, context_lens=lens, q_len=1, block_size=16, count=16, first=0, last=0)
+    attend = dict(q=q, k_cache=cache, v_cache=cache.clone(), block_tables=table, context_lens=lens, spans=ints(2, 2, 16), span=16, q_len=1, scale=1.0)
+    bound = dict(bounds=both, k_cache=cache, block_tables=table, context_lens=lens, new_tokens=16)
+    for call, args, names in ((ops.place_tokens, place, ("rows", "block_size")), (ops.select_spans, select, ("block_size", "count", "first", "last")), (ops.span_attention, attend, ("span",)),
+                              (ops.span_bounds, bound, ("new_tokens",))):
+        for name in names:
+            if name == "new_tokens" and far > 0:   # more new tokens than there are cost time only
+                continue
+            with pytest.raises(ValueError, match="32 bits"):
+                call(**{**args, name: far})
