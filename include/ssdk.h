@@ -316,7 +316,7 @@ int ssdk_select_spans(const void* q, const void* bounds, const int32_t* block_ta
                       void* scratch, int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size,
                       int max_blocks_per_seq, int64_t num_blocks, int span, int count, int first, int last, void* stream);
 /* ssdk_span_attn: ssdk_paged_attn over the keys of the listed spans only.  Entries outside the context, or on pages outside the cache, are
- * passed over; a span that is listed twice counts twice; a row that sees no key is zero.  Keys and values that a row does not see are of no account to it, whatever
+ * passed over; a span that is listed twice counts twice; a row that sees no key, or whose scores are all minus infinity, is zero.  Keys and values that a row does not see are of no account to it, whatever
  * they hold; NaN that it sees makes NaN, a value of infinity stays one (with a scale of 0 a key or query of infinity makes NaN too).  At most 32 query heads to a key head, 4096 spans; out may be q itself.
  * More than sixteen query rows to a key head take a kernel with bounded waits: as with ssdk_paged_attn_pages, a wait that runs out leaves NaN
  * rows, and the next such call of the process returns an error. */

@@ -337,7 +337,7 @@ def span_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     """paged_attention over the keys of the listed spans only: spans int32 [B, KV, count] (select_spans), `span` tokens each.
 
     q [B * q_len, H, hd]; returns [B * q_len, H * hd].  Entries outside the context are passed over, a span listed twice counts twice, a row
-    that sees no key is zero."""
+    that sees no key, or whose scores are all minus infinity, is zero (as in paged_attention)."""
     n, block_size, KV, hd = cache = k_cache.shape if k_cache.dim() == 4 else (-1,) * 4
     B, width, H, count = _last(context_lens, 1), _last(block_tables, 2), q.shape[1] if q.dim() == 3 else -1, _last(spans, 3)
     if not -_TOP <= span < _TOP:

@@ -53,3 +53,49 @@ def test_pages_that_go_between_the_kernels(tmp_path, zero, q_len):
     later[0, 2], later[0, 4], later[0, 7] = -1, total, -2147483648
     got = _run(tmp_path, q, both, table, [300], q_len, S, 9, 1, 1, 0, later=later)
     assert bool(((got >= 0) & (got < 19)).all()) and bool((got[..., 1:] > got[..., :-1]).all())
+
+
+# one kernel, two, and two with more than eight rows to a key head
+FORMS = [(1, 4, 2, 1), (1, 4, 2, 0), (5, 4, 2, 0)]
+
+
+@pytest.mark.parametrize("q_len,H,KV,own", FORMS)
+@pytest.mark.parametrize("kind", ["whole", "zero", "infinite", "nan", "query", "random"])
+def test_select_source(tmp_path, q_len, H, KV, own, kind):
+    """Equal scores, zeros of both signs, what is not finite in bounds and queries, and pages outside the cache."""
+    g = gen(72, q_len, len(kind), own)
+    S, span, hd, width = 32, 16, 64, 11
+    lens = [310, 299, 20]
+    table, total = tables(g, lens, S, width=width)
+    table[0, 3], table[1, 0], table[1, 8] = total, -9, 2147483647
+    q = torch.randint(-1, 2, (3 * q_len, H, hd), generator=g).to(BF)
+    both = torch.randint(-1, 2, (total, S // span, KV, 2, hd), generator=g).to(BF).sort(3).values.contiguous()
+    if kind == "zero":
+        both = torch.where(both == 0, torch.tensor(-0.0, dtype=BF), both) * 0
+    if kind == "infinite":
+        both[::3, 1, 0, 1, 5] = float("inf")
+        both[1::3, 0, 0, :, 7] = -float("inf")
+    if kind == "nan":
+        both[::2, 1, KV - 1, 0, 9] = float("nan")
+    if kind == "query":
+        q[q_len - 1, H - 1, 2], q[q_len, 0, 0] = float("inf"), float("nan")
+        both = both * 3e38
+    if kind == "random":
+        q, both = torch.randn(q.shape, generator=g).to(BF), torch.randn(both.shape, generator=g).sort(3).values.to(BF).contiguous()
+    for count, first, last in ((5, 1, 1), (13, 0, 0)):
+        got = _run(tmp_path, q, both, table, lens, q_len, S, count, first, last, own)
+        assert torch.equal(got, plain.select(q, both, table, lens, q_len, S, count, first, last))
+
+
+@pytest.mark.parametrize("hd,q_len,H,KV,own,warps", [(128, 1, 3, 1, 1, 8), (128, 2, 3, 1, 0, 3), (128, 9, 2, 2, 0, 8), (64, 3, 8, 1, 0, 16)])
+def test_select_source_sizes(tmp_path, hd, q_len, H, KV, own, warps):
+    """Heads of 128, odd groups, warps that take several groups of spans and warps that find none; count, first and last at their ends."""
+    g = gen(73, hd, q_len, H)
+    S, span = 48, 16
+    lens = [900, 33, 5]
+    table, total = tables(g, lens, S)
+    q = torch.randn(3 * q_len, H, hd, generator=g).to(BF)
+    both = torch.randn(total, S // span, KV, 2, hd, generator=g).sort(3).values.to(BF).contiguous()
+    for count, first, last in ((1, 0, 0), (7, 3, 4), (56, 1, 2)):
+        got = _run(tmp_path, q, both, table, lens, q_len, S, count, first, last, own, warps)
+        assert torch.equal(got, plain.select(q, both, table, lens, q_len, S, count, first, last))
