@@ -78,7 +78,6 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   }
   if (warp == 1) { tmem_alloc(&tmem_slot, 256); tmem_relinquish(); }
   pdl_wait();
-  pdl_launch_dependents();
   // the spans that are there, in the list's order
   const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size);
   int spans = 0;
@@ -111,6 +110,7 @@ span_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot, tmem_o = tmem + 128;   // S / P buffers at columns 0 and 64, O behind them
+  pdl_launch_dependents();   // (this block has its tensor memory: what is scheduled now may take the rest of the SM's and wait for this grid)
 
   const int per = p.span / box, boxes = kTileKeys / box, pieces = spans * per;   // boxes of a span, of a chunk, in all
   const int chunks = (pieces + boxes - 1) / boxes, share = (chunks + C - 1) / C;
