@@ -17,12 +17,13 @@ namespace ssdk {
 // change places whose scores differ in the last bits.
 // Bound by the bytes of the bounds.  The sum is a product, [lo | hi] . [min(q, 0) | max(q, 0)], so span_estimate_kernel makes an estimate of every score on the
 // tensor cores: a warp takes sixteen spans, whose 16-byte loads are the m16 fragments of mma.m16n8k16 (channels permuted alike on both sides), eight rows
-// are its n.  The estimate is off by at most eps = 2^-14 max_r sum_d |q[r, d]| max |lo, hi|: 2 hd / 16 steps, each adding 17 numbers with 2^-22 of the terms'
-// size lost.  With t the want-th largest estimate, a span above t + 2 eps is taken, one under t - 2 eps is not, and span_pick_kernel scores only the few
+// are its n.  The estimate is off by at most eps = 2^-14 max_r sum_d |q[r, d]| max |lo, hi|: lower and upper bounds are a chain of hd / 16 steps each,
+// a step adds 17 numbers with 2^-22 of its chain's terms' size lost, and 17 hd / 16 2^-22 is below 2^-14.9 for hd = 128.  With t the want-th largest estimate, a span above t + 2 eps is taken, one under t - 2 eps is not, and span_pick_kernel scores only the few
 // in between in 64 bits (products of bf16 values are exact, sums of 128 of them off by 2^-46).  Where values are not finite, or so large that 32 bits
 // overflow, it scores all.
 // Two kernels, the second's start under the first's end: the estimates fill all SMs in even shares whatever the number of heads, and what picks is one block
-// of a head (short tables: the block that picks makes its estimates itself).  24 contexts of 64000 tokens (150 MB of bounds): 39 us, of it 8 the second's.  The first has its loads in flight one turn at a time (registers hold one);
+// of a head (short tables, few rows and few heads: the block that picks makes its estimates itself, kOwnSpans).  24 contexts of 64000 tokens (150 MB of bounds): 37 us, of it 8 the
+// second's.  The first has its loads in flight one turn at a time (registers hold one);
 // a ring of cp.async stages, each lane its own pieces or a span's bounds by whole lines, was slower: 49 and 41 us.
 // ----------------------------------------------------------------------------------
 struct SelectParams {
@@ -480,7 +481,9 @@ __global__ void __launch_bounds__(kPickThreads, OWN ? 1 : 2) span_pick_kernel(Se
 // is passed over, a row that sees no key is zero.
 // Bound by the bytes of the listed keys and values.  A cluster of blocks owns one key head of one sequence and up to sixteen of its query rows (more:
 // span_tiles.cuh).  Pieces of 16 keys go round the blocks' warps, each with a ring of its own (cp.async, no barrier between warps) and a softmax of its own;
-// at the end warps meet, then blocks.  Weights go into the second product as two bf16 pieces, sums are fp32.
+// at the end warps meet, then blocks.  Sums are fp32.  Weights go into the second product as two bf16 pieces, 16 bits of them: with 4096 keys an output is off by 2.4e-6 of
+// itself before its own rounding to 8 bits (1e-7 with fp32 weights), 0.24 % of the outputs round to the neighbouring value, and their error against 64 bits stays what their
+// rounding makes it, 0.00165 either way.  A third piece would be half as many products again for nothing that the output's type can hold.
 // ----------------------------------------------------------------------------------
 struct SpanAttnParams {
   const __nv_bfloat16* q;        // [B * Q, H, hd]

@@ -1,7 +1,7 @@
 // span_tiles.cuh — span_attention of more than sixteen query rows to a key head, on tcgen05.
 //
 // As in prompt_attn_kernel's twin form: S = Q K^T of up to 64 rows and 64 keys into TMEM, P = exp2(S - m) one row per thread, O += P V with P out of TMEM.  The
-// queries lie in rows 0 .. 63 and again in 64 .. 127: these make the low bf16 pieces of the weights, add up in lanes of their own and are added at the
+// queries lie in rows 0 .. 63 and again in 64 .. 127: these make the low bf16 pieces of the weights (two pieces: see span_attn_kernel), add up in lanes of their own and are added at the
 // end.  (With a row's keys shared by its two lanes, zeros in P at the other's keys and the two pieces in a product each, the exponentials halve and the
 // products double: 37.0 us against 36.5 where this is 36.5, one warp issuing; tensor and shared memory are what two blocks share.)  Scores and products with V are issued
 // by a warp each, with one commit a product: one thread that issued both and looked at five barriers a chunk held it at 2500 clocks a chunk (36.5 -> 33.4 us at the time).
@@ -11,7 +11,7 @@
 // 4096 listed keys each: 63 us on two m16 tiles a warp, 32.7 here (32 sequences: 99 us, 84 % of the copy rate).  Of these 33 a block takes 5 until its first scores are
 // weights, some 22 for its 16 chunks and 6 to join.  Keys and values are asked for by a warp each, the moment that their stage is read: one thread for both, with a division a box,
 // asked for a chunk's keys 1200 clocks late (33.5 us; 32 sequences 102; boxes of 16 keys, one sequence of 160 rows, 32 -> 27).  Two stages of both are what fits twice on an SM; heads of
-// 64 have four (32 sequences 84.5 -> 81).
+// 64 have four (32 sequences 84.5 -> 82).
 #pragma once
 #include <cooperative_groups.h>
 
