@@ -216,14 +216,15 @@ int ssdk_rope_axes_store_kv(const void* qkv, const int64_t* positions, int axes,
   if (M < 1 || heads < 1 || kv_heads < 1 || (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return fail("rope_axes: %d rows of %d heads over %d of %d (64, 128 or 256)", M, heads, kv_heads, head_dim);
   if (rot_dim < 16 || rot_dim % 16 || rot_dim > head_dim) return fail("rope_axes: %d rotated channels of %d (a multiple of 16)", rot_dim, head_dim);
-  if (axes < 1 || axes > 4 || max_pos < 1 || max_pos >= (1ll << 40) || num_slots < 1 || num_slots >= (1ll << 40)) return fail("rope_axes: %d axes (1 to 4), %lld positions, %lld slots", axes, (long long)max_pos, (long long)num_slots);
+  if (axes < 1 || axes > 4 || max_pos < 1 || num_slots < 1) return fail("rope_axes: %d axes (1 to 4), %lld positions, %lld slots", axes, (long long)max_pos, (long long)num_slots);
   if (heads + 2 * (int64_t)kv_heads > 65535) return fail("rope_axes: too many heads");
   if (!qkv || !positions || !axis_of || !slot_mapping || !rope_table || !q_out || !k_cache || !v_cache) return fail("rope_axes: null argument");
   if (off16(qkv, q_out, k_cache, v_cache) || off16(q_norm_w, k_norm_w, rope_table)) return fail("rope_axes: arrays must start at multiples of 16 bytes");
-  const int64_t row = 2ll * M * head_dim, cache = 2 * num_slots * kv_heads * head_dim;
+  // (a slot has 32 bits; of larger numbers only as much counts as keeps the bytes in 64)
+  const int64_t row = 2ll * M * head_dim, cache = 2 * std::min<int64_t>(num_slots, 1ll << 31) * kv_heads * head_dim, angles = 4 * std::min<int64_t>(max_pos, 1ll << 40) * rot_dim;
   CKI(check_apart("rope_axes", {{"q_out", q_out, row * heads}, {"k_cache", k_cache, cache}, {"v_cache", v_cache, cache}},
                   {{"qkv", qkv, row * (heads + 2 * (int64_t)kv_heads)}, {"positions", positions, 8ll * axes * M}, {"slot_mapping", slot_mapping, 4ll * M},
-                   {"rope_table", rope_table, 4 * max_pos * rot_dim}, {"q_norm_w", q_norm_w, 2ll * head_dim}, {"k_norm_w", k_norm_w, 2ll * head_dim}}));
+                   {"rope_table", rope_table, angles}, {"q_norm_w", q_norm_w, 2ll * head_dim}, {"k_norm_w", k_norm_w, 2ll * head_dim}}));
   RopeAxesParams p;
   memset(&p, 0, sizeof(p));
   for (int i = 0; i < rot_dim / 2; ++i) {

@@ -57,6 +57,8 @@ def test_outputs_over_other_arrays(name):
                 if (w, other) in one and at == good[other]:
                     continue
                 _refused(name, args, "of its own")
+    if name == "ssdk_rope_axes_store_kv":   # (more slots and positions than an address space holds: the bytes are counted without passing 64 bits)
+        _refused(name, [*good[:6], 1 << 61, *good[7:13], 8 * M + 16, 1 << 61, *good[15:]], "of its own")
     if name == "ssdk_select_spans":
         assert so.ssdk_select_spans_scratch_bytes(2, 2, 32, 2, 16) == written[5]
 
