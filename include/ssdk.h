@@ -324,6 +324,32 @@ int ssdk_span_attn(const void* q, const void* k_cache, const void* v_cache, cons
                    const int32_t* selected, void* out, int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size,
                    int max_blocks_per_seq, int64_t num_blocks, int span, int count, float scale, void* stream);
 
+/* ---- the paged cache held in 4 bits (beside store_kvcache and flash_attn_with_kvcache, layers/attention.py:35-41,107-111) ----
+ * k_cache, v_cache: uint8 [num_blocks, KV, block_size * (head_dim / 2 + 4)].  Of a page and key head first the codes of its tokens, head_dim / 2 bytes each (byte i:
+ * channel 2 i in the low half, 2 i + 1 in the high one), then their pairs (scale, minimum) in bf16.  Of a row x of one head in bf16: minimum = min x,
+ * scale = (max x - minimum) / 15 rounded to bf16 (0 where below 2^-126), code = floor((x - minimum) / scale + 1/2), 0 where the scale is 0; the value that stands there is
+ * scale * code + minimum, rounded once to bf16.  A row that holds something that is not finite, or whose spread passes fp32, is NaN as a whole.  head_dim 64 or 128, block_size a multiple of 16
+ * of at most 65536, fewer than 2^31 slots.  Written or read rows of one call have distinct slots where they are written; slots outside the cache store nothing. */
+/* ssdk_rope_store_kv4: ssdk_rope_store_kv into such a cache.  positions int64 [M]; rope_table fp32 [max_pos, rot_dim] cos | sin: the first rot_dim channels of a head turn (a
+ * multiple of 16).  Queries: fp32, one rounding, to q_out [M, heads * head_dim].  Keys: norm and rotation in 64 bits, rounded to bf16, then quantised.  k_values, v_values [M, KV, head_dim] (both or
+ * null): the values that then stand in the cache, of every row, also of those without a slot.  A row with a position outside the table has NaN queries and values and stores nothing. */
+int ssdk_rope_store_kv4(const void* qkv, const int64_t* positions, const int32_t* slot_mapping, const float* rope_table, int64_t max_pos,
+                        int rot_dim, const void* q_norm_w, const void* k_norm_w, float norm_eps, void* q_out, void* k_cache, void* v_cache,
+                        void* k_values, void* v_values, int64_t num_blocks, int block_size, int M, int heads, int kv_heads, int head_dim,
+                        void* stream);
+/* ssdk_store_kv4: rows of keys and values [M, KV, head_dim] as they are; k_row, v_row: elements from row to row (multiples of 8). */
+int ssdk_store_kv4(const void* k, const void* v, int64_t k_row, int64_t v_row, const int32_t* slot_mapping, void* k_cache, void* v_cache,
+                   void* k_values, void* v_values, int64_t num_blocks, int block_size, int M, int kv_heads, int head_dim, void* stream);
+/* ssdk_load_kv4: the values of the slots, k and v bf16 [M, KV, head_dim]; rows with a slot outside the cache are zero. */
+int ssdk_load_kv4(const void* k_cache, const void* v_cache, const int32_t* slot_mapping, void* k, void* v, int64_t num_blocks, int block_size,
+                  int M, int kv_heads, int head_dim, void* stream);
+/* ssdk_paged_attn_kv4: ssdk_paged_attn over the values scale * code + minimum (not rounded to bf16), causal to the end of the context.  At most 32 query heads to a key head.  Pages
+ * outside the cache are passed over, lengths are held to what a table has room for, a row that sees no key is zero.  A NaN row of the cache makes NaN of the rows that see it, a query that is
+ * not finite makes its row NaN. */
+int ssdk_paged_attn_kv4(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables, const int32_t* context_lens,
+                        void* out, int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size, int max_blocks_per_seq,
+                        int64_t num_blocks, float scale, void* stream);
+
 /* Sampler.forward (layers/sampler.py:14-36): greedy where temp==0, else
  * argmax(softmax(l/T) / Exp(1)) with Philox(seed, step_id) exponentials.
  * logits bf16 [B, V] with row stride ld (elements); out int64 [B]. */

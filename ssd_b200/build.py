@@ -50,7 +50,7 @@ def _nccl_paths() -> tuple[list[str], list[str]]:
 
 
 def sources() -> list[Path]:
-    return [CSRC / "engine.cu", CSRC / "cache_ops.cu"]
+    return [CSRC / "engine.cu", CSRC / "cache_ops.cu", CSRC / "kv4_ops.cu"]
 
 
 def headers() -> list[Path]:

@@ -1,20 +1,9 @@
 // cache_ops.cuh — what surrounds attention over a part of a long paged cache: pages, positions and slots of a step's tokens from the lengths of its
 // requests, rotary positions with several axes beside the cache write, and per span of keys the smallest and largest value of every channel.
 #pragma once
-#include "common.cuh"
+#include "paged.cuh"
 
 namespace ssdk {
-
-// the page that a table names, -1 where it is none of the cache's
-SSDK_DEVINL int page_at(const int32_t* entry, int64_t num_blocks) {
-  const int page = *entry;
-  return page >= 0 && page < num_blocks ? page : -1;
-}
-// tokens of a sequence, held to what its table has room for
-SSDK_DEVINL int tokens_of(const int32_t* lens, int b, int max_blocks, int block_size) {
-  const long long cap = (long long)max_blocks * block_size, len = lens[b];
-  return (int)(len < 0 ? 0 : len < cap ? len : cap);
-}
 
 // ----------------------------------------------------------------------------------
 // place_tokens_kernel.  Sequence b has ctx[b] tokens in ceil(ctx / S) pages of S tokens and gets new[b] more; need[b] = ceil((ctx + new) / S) - ceil(ctx / S)
@@ -344,19 +333,6 @@ struct SpanBoundsParams {
 };
 constexpr int kBoundsThreads = 256;
 
-// two channels at once, NaN if one is
-#ifndef SSDK_HOST_EMU
-SSDK_DEVINL uint32_t min_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-SSDK_DEVINL uint32_t max_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-#endif
 SSDK_DEVINL uint4 min_bf16x8(const uint4& a, const uint4& b) { return make_uint4(min_bf16x2(a.x, b.x), min_bf16x2(a.y, b.y), min_bf16x2(a.z, b.z), min_bf16x2(a.w, b.w)); }
 SSDK_DEVINL uint4 max_bf16x8(const uint4& a, const uint4& b) { return make_uint4(max_bf16x2(a.x, b.x), max_bf16x2(a.y, b.y), max_bf16x2(a.z, b.z), max_bf16x2(a.w, b.w)); }
 

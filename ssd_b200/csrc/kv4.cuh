@@ -1,0 +1,289 @@
+// kv4.cuh — a paged cache whose keys and values are held in 4 bits: rows quantised as they are written (behind a norm and a rotation, or as they are), and read back.
+//
+// A cache is uint8 [num_blocks, KV, block_size * (hd / 2 + 4)]: of a page and head first the codes of its tokens, hd / 2 bytes each (byte i: channel 2 i in its low half,
+// 2 i + 1 in its high one), then their pairs (scale, minimum) in bf16.  A page's keys of a head are one piece, 17408 bytes for 256 tokens of 128.
+// Of a row x of hd bf16 values: minimum m = min x, scale s = (max x - m) / 15 rounded to bf16 (0 where below 2^-126), code = floor((x - m) / s + 1/2), 0 where s = 0;
+// the value that stands there is s code + m, rounded once to bf16.  m is one of the values, so it is exact; s rounded down by at most 2^-8 leaves (x - m) / s below 15.06,
+// so no code passes 15.  A row that holds something that is not finite, or whose spread passes fp32, is NaN as a whole (both of its pair are).
+#pragma once
+#include "paged.cuh"
+
+namespace ssdk {
+
+constexpr int kv4_row_bytes(int HD) { return HD / 2 + 4; }   // of a token and head: codes and pair
+constexpr uint32_t kKv4Nan = 0x7fc07fc0u;
+
+// Codes of a row whose 16 x LPH values lie with LPH neighbouring lanes, 16 a lane in two pieces of eight.  code: a word of eight channels for each piece; pair: scale | minimum;
+// VALUES: the pieces become what the codes stand for.
+// A quotient is often a code and a half exactly (x - m has some sixteen bits, s has eight), where a product with 1 / s goes either way.  So the product is made with something below
+// 1 / s, which gives the code or the one in front of it, and what it leaves, x - m - code s, is exact in fp32 and decides.  The nearest whole number stands in the low bits of
+// (x - m) r + 1.5 2^23; these words are put together as they are, and their constant parts taken off at the end.
+template <int LPH, bool VALUES>
+SSDK_DEVINL void kv4_codes(uint4& x, uint4& y, uint32_t (&code)[2], uint32_t& pair) {
+  uint32_t w[2][4] = {{x.x, x.y, x.z, x.w}, {y.x, y.y, y.z, y.w}};
+  uint32_t lo = w[0][0], hi = w[0][0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    lo = min_bf16x2(lo, w[i >> 2][i & 3]);
+    hi = max_bf16x2(hi, w[i >> 2][i & 3]);
+  }
+#pragma unroll
+  for (int o = LPH / 2; o > 0; o >>= 1) {
+    lo = min_bf16x2(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max_bf16x2(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  lo = min_bf16x2(lo, __byte_perm(lo, lo, 0x1032));
+  hi = max_bf16x2(hi, __byte_perm(hi, hi, 0x1032));
+  float m = __uint_as_float(lo << 16) + 0.f;   // (a minimum of zero has no sign)
+  const float spread = __uint_as_float(hi << 16) - m;
+  const bool fine = spread < INFINITY;   // (no NaN, no infinity)
+  float s = bf16_round(spread / 15.f);
+  if (s < 1.17549435e-38f) s = 0.f;
+  pair = fine ? __float_as_uint(s) >> 16 | (__float_as_uint(m) & 0xffff0000u) : kKv4Nan;
+  if (!fine) s = m = __uint_as_float(kKv4Nan);
+  const float r = s > 0.f ? 1.f / s * (1.f - 0x1p-20f) : 0.f, half = s > 0.f ? 0.5f * s : INFINITY;
+  constexpr float kWhole = 12582912.f;   // 1.5 2^23, the word 0x4b400000
+  constexpr uint32_t kOff = 0x4b400000u * 0x11111111u;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t acc = 0;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {
+      float v[2];
+#pragma unroll
+      for (int e = 1; e >= 0; --e) {
+        const float d = __uint_as_float(e ? w[h][i] & 0xffff0000u : w[h][i] << 16) - m;
+        const float u = fmaf(d, r, kWhole), c = u - kWhole;
+        const bool up = fmaf(-c, s, d) >= half;
+        acc = acc * 16u + __float_as_uint(u) + (up ? 1u : 0u);
+        if (VALUES) v[e] = fmaf(s, up ? c + 1.f : c, m);
+      }
+      if (VALUES) w[h][i] = pack_bf16x2(v[0], v[1]);
+    }
+    code[h] = fine ? acc - kOff : 0u;
+  }
+  if (VALUES) {
+    x = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
+    y = make_uint4(w[1][0], w[1][1], w[1][2], w[1][3]);
+  }
+}
+
+// ----------------------------------------------------------------------------------
+// kv4_store_kernel.  ROPE: queries and keys turn (rope_axes_kernel with one axis), optional norms in front, queries go to q_out; without it rows of keys and values are quantised
+// as they are.  Queries are fp32 with one rounding.  A key is rounded to bf16 (what an unquantised cache would hold) and then quantised, and that rounding decides its code next to a
+// border: keys' norm and rotation are in 64 bits, so that codes are those of the definition whatever the order of sums.  (Keys are an eighth to a third of the heads.)
+// Bound by memory: 2 bytes read a channel, 2 written for queries and values that are asked for, 0.53 for codes.  HD / 16 lanes own a head, a warp takes groups of
+// 32 / (HD / 16) heads of one kind, the next group's loads in flight; the rows' groups lie one behind the other and each warp has a stretch of them.
+// A row with a position outside the table has NaN queries (and values) and stores nothing; slots outside the cache store nothing.
+// ----------------------------------------------------------------------------------
+struct Kv4StoreParams {
+  const __nv_bfloat16 *q, *k, *v;   // rows of heads
+  int64_t q_row, k_row, v_row;      // elements from row to row
+  const int64_t* positions;         // [M]
+  const int32_t* slots;             // [M]
+  const float* table;               // [top, rot] cos | sin
+  const __nv_bfloat16 *q_norm_w, *k_norm_w;   // [hd] or null
+  __nv_bfloat16 *q_out, *k_values, *v_values;   // [M, H, hd], [M, KV, hd] each or null
+  uint8_t *k_cache, *v_cache;
+  int64_t top, num_slots;
+  float eps;
+  int M, heads, kv_heads, rot, block_size;
+  int q_groups, kv_groups;          // of heads that a warp takes at once, in a row
+  int warps, each, longer;          // the rows' groups one behind the other: a warp has a stretch of `each`, the first `longer` one more
+};
+constexpr int kKv4StoreThreads = 128;
+
+SSDK_DEVINL double shfl_xor_f64(double v, int o) {
+  union { double d; uint32_t w[2]; } u;
+  u.d = v;
+  u.w[0] = __shfl_xor_sync(0xffffffffu, u.w[0], o);
+  u.w[1] = __shfl_xor_sync(0xffffffffu, u.w[1], o);
+  return u.d;
+}
+
+// norm (weights w0, w1 of the two pieces, or none) and rotation of a lane's two pieces in T, rounded to bf16 by way of fp32
+template <typename T, int LPH>
+SSDK_DEVINL void kv4_turn(uint4& x, uint4& y, const __nv_bfloat16* w0, const __nv_bfloat16* w1, float eps, bool turns, const float (&co)[8], const float (&si)[8]) {
+  float a[8], b[8];
+  unpack_bf16x8(x, a);
+  unpack_bf16x8(y, b);
+  T scale = 1;
+  float wa[8], wb[8];
+  if (w0) {   // (the whole warp)
+    T sum = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += (T)a[i] * (T)a[i] + (T)b[i] * (T)b[i];
+#pragma unroll
+    for (int o = LPH / 2; o > 0; o >>= 1) {
+      if constexpr (sizeof(T) == 8) sum += shfl_xor_f64(sum, o);
+      else sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    if constexpr (sizeof(T) == 8) scale = 1.0 / sqrt(sum / (16.0 * LPH) + (double)eps);
+    else scale = rsqrtf(sum / (16.f * LPH) + eps);
+    unpack_bf16x8(*reinterpret_cast<const uint4*>(w0), wa);
+    unpack_bf16x8(*reinterpret_cast<const uint4*>(w1), wb);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    T u = a[i], v = b[i];
+    if (w0) {
+      u = u * scale * (T)wa[i];
+      v = v * scale * (T)wb[i];
+    }
+    a[i] = (float)(turns ? u * (T)co[i] - v * (T)si[i] : u);
+    b[i] = (float)(turns ? v * (T)co[i] + u * (T)si[i] : v);
+  }
+  x = pack_bf16x8(a);
+  y = pack_bf16x8(b);
+}
+
+template <int HD, bool ROPE, bool VALUES>
+__global__ void __launch_bounds__(kKv4StoreThreads, 4) kv4_store_kernel(Kv4StoreParams p) {
+  constexpr int LPH = HD / 16, SIDE = 32 / LPH;   // lanes of a head, heads side by side
+  pdl_wait();
+  pdl_launch_dependents();
+  const int warp = (int)blockIdx.x * (kKv4StoreThreads / 32) + (int)(threadIdx.x >> 5);
+  if (warp >= p.warps) return;
+  int unit = warp * p.each + min(warp, p.longer);   // (below 2^31: the host sees to it)
+  const int last = unit + p.each + (warp < p.longer);
+  const int piece = threadIdx.x % LPH, side = threadIdx.x % 32 / LPH, half = p.rot / 2, groups = p.q_groups + 2 * p.kv_groups;
+  const bool turns = ROPE && piece < p.rot / 16;
+  // channels of a lane's pieces: of heads that turn, and of others
+  const int t0 = turns ? piece * 8 : p.rot + (piece - p.rot / 16) * 16, t1 = turns ? half + piece * 8 : t0 + 8;
+
+  uint4 a, b;
+  auto load = [&](int m, int group) {
+    const int kind = group < p.q_groups ? 0 : group < p.q_groups + p.kv_groups ? 1 : 2;
+    const int head = (group - (kind ? p.q_groups : 0) - (kind == 2 ? p.kv_groups : 0)) * SIDE + side;
+    const __nv_bfloat16* row = kind == 0 ? p.q + m * p.q_row : kind == 1 ? p.k + m * p.k_row : p.v + m * p.v_row;
+    const bool turned = ROPE && kind != 2;
+    a = b = make_uint4(0, 0, 0, 0);
+    if (head < (kind == 0 ? p.heads : p.kv_heads)) {
+      a = ld_nc_v4(row + head * HD + (turned ? t0 : piece * 16));
+      b = ld_nc_v4(row + head * HD + (turned ? t1 : piece * 16 + 8));
+    }
+  };
+  int m = unit / groups, group = unit - m * groups, row = -1;
+  if (unit < last) load(m, group);
+  bool known = true, stores = false;
+  float co[8] = {}, si[8] = {};
+  size_t page = 0;
+  int off = 0;
+  for (; unit < last; ++unit) {
+    if (m != row) {
+      row = m;
+      const int slot = p.slots[m];
+      known = true;
+      if (ROPE) {
+        const int64_t at = p.positions[m];
+        known = at >= 0 && at < p.top;
+        if (turns && known) {
+          const float* angles = p.table + (size_t)at * p.rot + piece * 8;
+#pragma unroll
+          for (int i = 0; i < 8; i += 4) {
+            const float4 c = *reinterpret_cast<const float4*>(angles + i), s = *reinterpret_cast<const float4*>(angles + half + i);
+            co[i] = c.x; co[i + 1] = c.y; co[i + 2] = c.z; co[i + 3] = c.w;
+            si[i] = s.x; si[i + 1] = s.y; si[i + 2] = s.z; si[i + 3] = s.w;
+          }
+        }
+      }
+      stores = known && slot >= 0 && slot < p.num_slots;
+      page = stores ? slot / p.block_size : 0;
+      off = stores ? slot - (int)page * p.block_size : 0;
+    }
+    uint4 x = a, y = b;
+    const int kind = group < p.q_groups ? 0 : group < p.q_groups + p.kv_groups ? 1 : 2;
+    const int head = (group - (kind ? p.q_groups : 0) - (kind == 2 ? p.kv_groups : 0)) * SIDE + side;
+    const bool there = head < (kind == 0 ? p.heads : p.kv_heads);
+    if (++group == groups) {
+      group = 0;
+      ++m;
+    }
+    if (unit + 1 < last) load(m, group);
+    const bool turned = ROPE && kind != 2;
+    const int c0 = turned ? t0 : piece * 16, c1 = turned ? t1 : piece * 16 + 8;
+    if (ROPE && kind == 0) kv4_turn<float, LPH>(x, y, p.q_norm_w ? p.q_norm_w + c0 : nullptr, p.q_norm_w ? p.q_norm_w + c1 : nullptr, p.eps, turns, co, si);
+    if (ROPE && kind == 1) kv4_turn<double, LPH>(x, y, p.k_norm_w ? p.k_norm_w + c0 : nullptr, p.k_norm_w ? p.k_norm_w + c1 : nullptr, p.eps, turns, co, si);
+    uint32_t code[2], pair;
+    if (kind) kv4_codes<LPH, VALUES>(x, y, code, pair);
+    if (ROPE && !known) x = y = make_uint4(kKv4Nan, kKv4Nan, kKv4Nan, kKv4Nan);
+    if (!there) continue;
+    if (kind == 0 || VALUES) {
+      __nv_bfloat16* dst = kind == 0 ? p.q_out + ((size_t)row * p.heads + head) * HD : (kind == 1 ? p.k_values : p.v_values) + ((size_t)row * p.kv_heads + head) * HD;
+      *reinterpret_cast<uint4*>(dst + c0) = x;
+      *reinterpret_cast<uint4*>(dst + c1) = y;
+    }
+    if (kind && stores) {
+      uint8_t* at = (kind == 1 ? p.k_cache : p.v_cache) + (page * p.kv_heads + head) * ((size_t)p.block_size * kv4_row_bytes(HD));
+      uint8_t* codes = at + (size_t)off * (HD / 2);
+      *reinterpret_cast<uint32_t*>(codes + c0 / 2) = code[0];
+      *reinterpret_cast<uint32_t*>(codes + c1 / 2) = code[1];
+      if (piece == 0) *reinterpret_cast<uint32_t*>(at + (size_t)p.block_size * (HD / 2) + off * 4) = pair;
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------
+// kv4_load_kernel: value = s code + m of the rows in `slots`, rounded once; rows with a slot outside the cache are zero.
+// Bound by memory, mostly by what is written: 2 bytes a channel of 2.53.  HD / 8 lanes own a row of a head, eight channels each; a warp takes kKv4LoadRows times as many rows
+// as it has room for, all loads in front of the first use.
+// ----------------------------------------------------------------------------------
+struct Kv4LoadParams {
+  const uint8_t *k_cache, *v_cache;
+  const int32_t* slots;             // [M]
+  __nv_bfloat16 *k, *v;             // [M, KV, hd]
+  int64_t num_slots;
+  int M, kv_heads, block_size;
+};
+constexpr int kKv4LoadThreads = 256, kKv4LoadRows = 4;
+constexpr int kv4_load_tile(int HD) { return 32 / (HD / 8) * kKv4LoadRows; }   // rows of a warp's tile, of one head
+
+SSDK_DEVINL uint4 kv4_values(uint32_t codes, uint32_t pair) {
+  const float s = __uint_as_float(pair << 16), m = __uint_as_float(pair & 0xffff0000u);
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = fmaf(s, (float)(codes >> (4 * i) & 15u), m);
+  return pack_bf16x8(f);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kKv4LoadThreads) kv4_load_kernel(Kv4LoadParams p) {
+  constexpr int LPR = HD / 8, SIDE = 32 / LPR, ROWS = kKv4LoadRows;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int piece = threadIdx.x % LPR, side = threadIdx.x % 32 / LPR;
+  const long long tiles = (long long)((p.M + SIDE * ROWS - 1) / (SIDE * ROWS)) * p.kv_heads, step = (long long)gridDim.x * (kKv4LoadThreads / 32);
+  const size_t record = (size_t)p.block_size * kv4_row_bytes(HD), pairs = (size_t)p.block_size * (HD / 2);
+  for (long long tile = (long long)blockIdx.x * (kKv4LoadThreads / 32) + (threadIdx.x >> 5); tile < tiles; tile += step) {
+    const int m0 = (int)(tile / p.kv_heads) * (SIDE * ROWS) + side, head = (int)(tile % p.kv_heads);
+    int slot[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int m = m0 + i * SIDE;
+      slot[i] = m < p.M ? p.slots[m] : -1;
+    }
+    uint32_t c[2][ROWS], w[2][ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      c[0][i] = c[1][i] = w[0][i] = w[1][i] = 0;
+      if (slot[i] >= 0 && slot[i] < p.num_slots) {
+        const int page = slot[i] / p.block_size, off = slot[i] - page * p.block_size;
+        const size_t at = ((size_t)page * p.kv_heads + head) * record, code = at + (size_t)off * (HD / 2) + piece * 4, pair = at + pairs + (size_t)off * 4;
+        c[0][i] = *reinterpret_cast<const uint32_t*>(p.k_cache + code);
+        c[1][i] = *reinterpret_cast<const uint32_t*>(p.v_cache + code);
+        w[0][i] = *reinterpret_cast<const uint32_t*>(p.k_cache + pair);
+        w[1][i] = *reinterpret_cast<const uint32_t*>(p.v_cache + pair);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int m = m0 + i * SIDE;
+      if (m >= p.M) continue;
+      const size_t to = ((size_t)m * p.kv_heads + head) * HD + piece * 8;
+      *reinterpret_cast<uint4*>(p.k + to) = kv4_values(c[0][i], w[0][i]);
+      *reinterpret_cast<uint4*>(p.v + to) = kv4_values(c[1][i], w[1][i]);
+    }
+  }
+}
+
+}  // namespace ssdk

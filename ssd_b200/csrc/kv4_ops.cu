@@ -1,0 +1,153 @@
+// kv4_ops.cu — entry points (include/ssdk.h) of the paged cache held in 4 bits: kv4.cuh, kv4_attention.cuh.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "../../include/ssdk.h"
+#include "kv4_attention.cuh"
+#include "op_host.cuh"
+
+using namespace ssdk;
+typedef __nv_bfloat16 bf16;
+
+constexpr int kSms = 148, kMaxSmem = 227 * 1024 - 1024;   // (statics beside it)
+
+// a cache of pages whose slots are numbered in 32 bits
+static int check_kv4(const char* who, int64_t num_blocks, int block_size, int kv_heads, int head_dim) {
+  if (head_dim != 64 && head_dim != 128) return fail("%s: heads of %d (64 or 128)", who, head_dim);
+  if (kv_heads < 1 || kv_heads > 65535 || num_blocks < 1 || block_size < 16 || block_size % 16 || block_size > 65536)
+    return fail("%s: %lld pages of %d tokens (a multiple of 16, at most 65536), %d key heads", who, (long long)num_blocks, block_size, kv_heads);
+  if (num_blocks >= (1ll << 31) / block_size) return fail("%s: a cache of %lld pages of %d tokens passes 32 bits", who, (long long)num_blocks, block_size);
+  return 0;
+}
+static int64_t kv4_bytes(int64_t num_blocks, int block_size, int kv_heads, int head_dim) { return num_blocks * block_size * kv_heads * kv4_row_bytes(head_dim); }
+
+template <int HD, bool ROPE, bool VALUES>
+static int launch_store(Launcher& L, Kv4StoreParams p) {
+  constexpr int SIDE = 32 / (HD / 16), W = kKv4StoreThreads / 32;
+  p.q_groups = ROPE ? (p.heads + SIDE - 1) / SIDE : 0;
+  p.kv_groups = (p.kv_heads + SIDE - 1) / SIDE;
+  const int64_t units = (int64_t)p.M * (p.q_groups + 2 * p.kv_groups);
+  if (units >= (1ll << 31)) return fail("store_kv4: %d rows of %d heads", p.M, p.heads + 2 * p.kv_heads);
+  p.warps = (int)std::min<int64_t>(units, kSms * 4 * W);   // four blocks on an SM
+  p.each = (int)(units / p.warps);
+  p.longer = (int)(units - (int64_t)p.each * p.warps);
+  return L.go(kv4_store_kernel<HD, ROPE, VALUES>, dim3((unsigned)((p.warps + W - 1) / W)), dim3(kKv4StoreThreads), 0, p);
+}
+template <bool ROPE>
+static int store(const Kv4StoreParams& p, int head_dim, void* stream) {
+  Launcher L = launcher(stream);
+  if (head_dim == 64) return p.k_values ? launch_store<64, ROPE, true>(L, p) : launch_store<64, ROPE, false>(L, p);
+  return p.k_values ? launch_store<128, ROPE, true>(L, p) : launch_store<128, ROPE, false>(L, p);
+}
+
+// Blocks that share the keys of a key head (a cluster): as many as make the fewest waves of the longest context's pieces, a block's start and end as long as some 512 keys.
+static int kv4_cluster(int64_t units, int64_t keys, int resident) {
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int c = 1; c <= kKv4Most; c *= 2) {
+    const int64_t cost = (units * c + resident * kSms - 1) / (resident * kSms) * (512 + 16 * c + keys / c);
+    if (cost < least) {
+      least = cost;
+      best = c;
+    }
+  }
+  return best;
+}
+template <int HD, int NT>
+static int launch_attn(Launcher& L, const Kv4AttnParams& p) {
+  static std::atomic<bool> done[64];
+  CKI(with_smem(kv4_attn_kernel<HD, NT>, kv4_attn_smem(HD, NT), kSmemOnly | 2, done));
+  const int64_t rows = (int64_t)(p.heads / p.kv_heads) * p.Q, tiles = (rows + 8 * NT - 1) / (8 * NT);
+  if (tiles > 65535) return fail("paged_attn_kv4: q_len=%d", p.Q);
+  L.cluster = kv4_cluster((int64_t)p.B * p.kv_heads * tiles, (int64_t)p.max_blocks * p.block_size, NT == 1 ? 2 : 1);
+  return L.go(kv4_attn_kernel<HD, NT>, dim3(p.kv_heads * L.cluster, p.B, (unsigned)tiles), dim3(kKv4Warps * 32), kv4_attn_smem(HD, NT), p);
+}
+
+extern "C" {
+
+int ssdk_rope_store_kv4(const void* qkv, const int64_t* positions, const int32_t* slot_mapping, const float* rope_table, int64_t max_pos,
+                        int rot_dim, const void* q_norm_w, const void* k_norm_w, float norm_eps, void* q_out, void* k_cache, void* v_cache,
+                        void* k_values, void* v_values, int64_t num_blocks, int block_size, int M, int heads, int kv_heads, int head_dim,
+                        void* stream) {
+  CKI(check_kv4("rope_store_kv4", num_blocks, block_size, kv_heads, head_dim));
+  if (M < 1 || heads < 1 || heads > 65535) return fail("rope_store_kv4: %d rows of %d heads", M, heads);
+  if (rot_dim < 16 || rot_dim % 16 || rot_dim > head_dim || max_pos < 1) return fail("rope_store_kv4: %d rotated channels of %d (a multiple of 16), %lld positions", rot_dim, head_dim, (long long)max_pos);
+  if (!qkv || !positions || !slot_mapping || !rope_table || !q_out || !k_cache || !v_cache || !k_values != !v_values) return fail("rope_store_kv4: null argument");
+  if (off16(qkv, q_out, k_cache, v_cache) || off16(q_norm_w, k_norm_w, rope_table) || off16(k_values, v_values)) return fail("rope_store_kv4: arrays must start at multiples of 16 bytes");
+  const int64_t row = 2ll * M * head_dim, all = heads + 2 * (int64_t)kv_heads, cache = kv4_bytes(num_blocks, block_size, kv_heads, head_dim);
+  // (of larger numbers of positions only as much counts as keeps the bytes in 64 bits)
+  CKI(check_apart("rope_store_kv4", {{"q_out", q_out, row * heads}, {"k_cache", k_cache, cache}, {"v_cache", v_cache, cache}, {"k_values", k_values, row * kv_heads}, {"v_values", v_values, row * kv_heads}},
+                  {{"qkv", qkv, row * all}, {"positions", positions, 8ll * M}, {"slot_mapping", slot_mapping, 4ll * M}, {"rope_table", rope_table, 4 * std::min<int64_t>(max_pos, 1ll << 40) * rot_dim},
+                   {"q_norm_w", q_norm_w, 2ll * head_dim}, {"k_norm_w", k_norm_w, 2ll * head_dim}}));
+  Kv4StoreParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = (const bf16*)qkv; p.k = p.q + (int64_t)heads * head_dim; p.v = p.k + (int64_t)kv_heads * head_dim;
+  p.q_row = p.k_row = p.v_row = all * head_dim;
+  p.positions = positions; p.slots = slot_mapping; p.table = rope_table; p.top = max_pos; p.rot = rot_dim;
+  p.q_norm_w = (const bf16*)q_norm_w; p.k_norm_w = (const bf16*)k_norm_w; p.eps = norm_eps;
+  p.q_out = (bf16*)q_out; p.k_cache = (uint8_t*)k_cache; p.v_cache = (uint8_t*)v_cache; p.k_values = (bf16*)k_values; p.v_values = (bf16*)v_values;
+  p.num_slots = num_blocks * block_size; p.block_size = block_size; p.M = M; p.heads = heads; p.kv_heads = kv_heads;
+  return store<true>(p, head_dim, stream);
+}
+
+int ssdk_store_kv4(const void* k, const void* v, int64_t k_row, int64_t v_row, const int32_t* slot_mapping, void* k_cache, void* v_cache,
+                   void* k_values, void* v_values, int64_t num_blocks, int block_size, int M, int kv_heads, int head_dim, void* stream) {
+  CKI(check_kv4("store_kv4", num_blocks, block_size, kv_heads, head_dim));
+  const int64_t n = (int64_t)kv_heads * head_dim, most = 1ll << 31;
+  if (M < 1 || k_row < 0 || v_row < 0 || k_row % 8 || v_row % 8 || k_row >= most || v_row >= most) return fail("store_kv4: %d rows, %lld and %lld elements apart (multiples of 8)", M, (long long)k_row, (long long)v_row);
+  if (!k || !v || !slot_mapping || !k_cache || !v_cache || !k_values != !v_values) return fail("store_kv4: null argument");
+  if (off16(k, v, k_cache, v_cache) || off16(k_values, v_values)) return fail("store_kv4: arrays must start at multiples of 16 bytes");
+  const int64_t values = 2ll * M * n, cache = kv4_bytes(num_blocks, block_size, kv_heads, head_dim);
+  CKI(check_apart("store_kv4", {{"k_cache", k_cache, cache}, {"v_cache", v_cache, cache}, {"k_values", k_values, values}, {"v_values", v_values, values}},
+                  {{"k", k, 2 * ((M - 1) * k_row + n)}, {"v", v, 2 * ((M - 1) * v_row + n)}, {"slot_mapping", slot_mapping, 4ll * M}}));
+  Kv4StoreParams p;
+  memset(&p, 0, sizeof(p));
+  p.k = (const bf16*)k; p.v = (const bf16*)v; p.k_row = k_row; p.v_row = v_row; p.slots = slot_mapping;
+  p.k_cache = (uint8_t*)k_cache; p.v_cache = (uint8_t*)v_cache; p.k_values = (bf16*)k_values; p.v_values = (bf16*)v_values;
+  p.num_slots = num_blocks * block_size; p.block_size = block_size; p.M = M; p.kv_heads = kv_heads;
+  return store<false>(p, head_dim, stream);
+}
+
+int ssdk_load_kv4(const void* k_cache, const void* v_cache, const int32_t* slot_mapping, void* k, void* v, int64_t num_blocks, int block_size,
+                  int M, int kv_heads, int head_dim, void* stream) {
+  CKI(check_kv4("load_kv4", num_blocks, block_size, kv_heads, head_dim));
+  if (M < 1 || M > (1 << 30)) return fail("load_kv4: %d rows", M);
+  if (!k_cache || !v_cache || !slot_mapping || !k || !v) return fail("load_kv4: null argument");
+  if (off16(k_cache, v_cache, k, v)) return fail("load_kv4: arrays must start at multiples of 16 bytes");
+  const int64_t rows = 2ll * M * kv_heads * head_dim, cache = kv4_bytes(num_blocks, block_size, kv_heads, head_dim);
+  CKI(check_apart("load_kv4", {{"k", k, rows}, {"v", v, rows}}, {{"k_cache", k_cache, cache}, {"v_cache", v_cache, cache}, {"slot_mapping", slot_mapping, 4ll * M}}));
+  Kv4LoadParams p;
+  p.k_cache = (const uint8_t*)k_cache; p.v_cache = (const uint8_t*)v_cache; p.slots = slot_mapping; p.k = (bf16*)k; p.v = (bf16*)v;
+  p.num_slots = num_blocks * block_size; p.M = M; p.kv_heads = kv_heads; p.block_size = block_size;
+  Launcher L = launcher(stream);
+  const int tile = kv4_load_tile(head_dim), W = kKv4LoadThreads / 32;
+  const int64_t tiles = (int64_t)((M + tile - 1) / tile) * kv_heads;
+  const dim3 grid((unsigned)std::min<int64_t>((tiles + W - 1) / W, kSms * 32)), block(kKv4LoadThreads);
+  return head_dim == 64 ? L.go(kv4_load_kernel<64>, grid, block, 0, p) : L.go(kv4_load_kernel<128>, grid, block, 0, p);
+}
+
+int ssdk_paged_attn_kv4(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables, const int32_t* context_lens,
+                        void* out, int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size, int max_blocks_per_seq,
+                        int64_t num_blocks, float scale, void* stream) {
+  CKI(check_kv4("paged_attn_kv4", num_blocks, block_size, kv_heads, head_dim));
+  CKI(check_pages("paged_attn_kv4", batch, block_size, max_blocks_per_seq, num_blocks));
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (q_len < 1 || heads < 1 || heads % kv_heads || heads / kv_heads > 32 || !std::isfinite(scale_log2))
+    return fail("paged_attn_kv4: q_len=%d, %d heads over %d (at most 32 to a key head), scale %g (finite, log2(e) times it too)", q_len, heads, kv_heads, (double)scale);
+  if ((int64_t)batch * q_len >= (1ll << 31) || (int64_t)q_len * (heads / kv_heads) >= (1ll << 31) - 65536) return fail("paged_attn_kv4: %d rows of %d sequences", q_len, batch);
+  if (!q || !k_cache || !v_cache || !block_tables || !context_lens || !out) return fail("paged_attn_kv4: null argument");
+  if (off16(q, k_cache, v_cache, out)) return fail("paged_attn_kv4: arrays must start at multiples of 16 bytes");
+  const int64_t rows = 2ll * batch * q_len * heads * head_dim, cache = kv4_bytes(num_blocks, block_size, kv_heads, head_dim);
+  CKI(check_apart("paged_attn_kv4", {{"out", out, rows}},
+                  {{"q", q, rows}, {"k_cache", k_cache, cache}, {"v_cache", v_cache, cache}, {"block_tables", block_tables, 4ll * batch * max_blocks_per_seq}, {"context_lens", context_lens, 4ll * batch}}));
+  Kv4AttnParams p;
+  p.q = (const bf16*)q; p.k_cache = (const uint8_t*)k_cache; p.v_cache = (const uint8_t*)v_cache; p.tables = block_tables; p.lens = context_lens; p.out = (bf16*)out;
+  p.num_blocks = num_blocks; p.B = batch; p.Q = q_len; p.heads = heads; p.kv_heads = kv_heads; p.block_size = block_size; p.max_blocks = max_blocks_per_seq;
+  p.scale_log2 = scale_log2;
+  Launcher L = launcher(stream);
+  if ((int64_t)(heads / kv_heads) * q_len <= 8) return head_dim == 64 ? launch_attn<64, 1>(L, p) : launch_attn<128, 1>(L, p);
+  return head_dim == 64 ? launch_attn<64, 2>(L, p) : launch_attn<128, 2>(L, p);
+}
+
+}  // extern "C"

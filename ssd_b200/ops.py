@@ -348,3 +348,101 @@ def span_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _launch("ssdk_span_attn", gpu, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), spans.data_ptr(),
             out.data_ptr(), B, q_len, H, KV, hd, block_size, width, n, span, count, scale)
     return out
+
+
+# ---- a paged cache whose keys and values are held in 4 bits ----
+_U8 = torch.uint8
+
+
+def kv4_caches(num_blocks: int, block_size: int, kv_heads: int, head_dim: int, device="cuda"):
+    """(k_cache, v_cache) of zeros: uint8 [num_blocks, kv_heads, block_size * (head_dim / 2 + 4)], the codes of a page's tokens and behind them their scales and
+    minima (include/ssdk.h has the format).  17 bytes where the bf16 cache has 64 (heads of 128); a page of one head is one piece, so pages are copied as they are."""
+    if head_dim not in (64, 128) or block_size < 16 or block_size % 16 or num_blocks < 1 or kv_heads < 1:
+        raise ValueError(f"kv4_caches: {num_blocks} pages of {block_size} tokens (a multiple of 16), {kv_heads} heads of {head_dim} (64 or 128)")
+    return tuple(torch.zeros(2, num_blocks, kv_heads, block_size * (head_dim // 2 + 4), dtype=_U8, device=device).unbind(0))
+
+
+def _kv4(name: str, k_cache: torch.Tensor, head_dim: int):
+    """Shape of the caches, and the tokens of a page."""
+    n, KV, size = k_cache.shape if k_cache.dim() == 3 else (-1,) * 3
+    if not (head_dim == 64 or head_dim == 128):
+        raise ValueError(f"{name}: heads of {head_dim} (64 or 128)")
+    row = head_dim // 2 + 4
+    if size < row or size % row or size // row >= _TOP:
+        raise ValueError(f"{name}: k_cache: {tuple(k_cache.shape)} is not [num_blocks, KV, block_size * {row}]")
+    return (n, KV, size), size // row
+
+
+def rope_store_kv4(qkv: torch.Tensor, positions: torch.Tensor, slot_mapping: torch.Tensor, rope_table: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   heads: int, kv_heads: int, head_dim: int, q_norm_w: torch.Tensor | None = None, k_norm_w: torch.Tensor | None = None, norm_eps: float = 1e-6,
+                   values: bool = False):
+    """rope_store_kv into a cache of 4 bits (kv4_caches).
+
+    qkv [M, (heads + 2 kv_heads) * head_dim] bf16; positions int64 [M]; slot_mapping int32 [M], distinct (outside the cache: stores nothing); rope_table fp32
+    [max_pos, rot_dim] cos | sin: the first rot_dim channels of a head turn.  Returns q [M, heads * head_dim], and with `values` (q, k, v): k, v [M, kv_heads, head_dim] are
+    what then stands in the cache, for attention among the new tokens.  A row with a position outside the table has NaN queries and stores nothing."""
+    M = qkv.shape[0]
+    top, rot = rope_table.shape if rope_table.dim() == 2 else (-1, -1)
+    cache, block_size = _kv4("rope_store_kv4", k_cache, head_dim)
+    cache = (cache[0], kv_heads, cache[2])
+    args = [(qkv, "qkv", _BF, (M, (heads + 2 * kv_heads) * head_dim)), (positions, "positions", _I64, (M,)), (slot_mapping, "slot_mapping", _I32, (M,)),
+            (rope_table, "rope_table", _F32, (top, rot)), (k_cache, "k_cache", _U8, cache), (v_cache, "v_cache", _U8, cache)]
+    for w, what in ((q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w")):
+        if w is not None:
+            args.append((w, what, _BF, (head_dim,)))
+    gpu = _check("rope_store_kv4", *args)
+    q = qkv.new_empty(M, heads * head_dim)
+    k, v = qkv.new_empty(2, M, kv_heads, head_dim).unbind(0) if values else (None, None)
+    _launch("ssdk_rope_store_kv4", gpu, qkv.data_ptr(), positions.data_ptr(), slot_mapping.data_ptr(), rope_table.data_ptr(), top, rot, _ptr(q_norm_w), _ptr(k_norm_w),
+            norm_eps, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k), _ptr(v), cache[0], block_size, M, heads, kv_heads, head_dim)
+    return (q, k, v) if values else q
+
+
+def store_kv4(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, values: bool = False):
+    """Rows of keys and values as they are, into a cache of 4 bits (kv4_caches): a model without rotation, pages of an unquantised cache that is taken over.
+
+    k, v [M, KV, head_dim] bf16; their rows may lie apart (views of a projection's output: heads and channels contiguous, rows at multiples of 8 elements); slot_mapping int32
+    [M], distinct (outside the cache: stores nothing).  With `values` returns (k, v) as they then stand in the cache."""
+    M, KV, hd = shape = k.shape if k.dim() == 3 else (-1,) * 3
+    cache, block_size = _kv4("store_kv4", k_cache, hd)
+    cache = (cache[0], KV, cache[2])
+    for t, what in ((k, "k"), (v, "v")):
+        if t.dtype is not _BF:
+            raise TypeError(f"store_kv4: {what}: expected {_BF}, got {t.dtype}")
+        if t.shape != shape:
+            raise ValueError(f"store_kv4: {what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+        if t.get_device() != slot_mapping.get_device():
+            raise ValueError(f"store_kv4: {what}: on {t.device}, slot_mapping on {slot_mapping.device}")
+        if t.stride(2) != 1 or (KV > 1 and t.stride(1) != hd):
+            raise ValueError(f"store_kv4: {what}: heads and channels of a row must be contiguous")
+    gpu = _check("store_kv4", (slot_mapping, "slot_mapping", _I32, (M,)), (k_cache, "k_cache", _U8, cache), (v_cache, "v_cache", _U8, cache))
+    a, b = both = k.new_empty(2, M, KV, hd).unbind(0) if values else (None, None)
+    _launch("ssdk_store_kv4", gpu, k.data_ptr(), v.data_ptr(), k.stride(0) if M > 1 else 0, v.stride(0) if M > 1 else 0, slot_mapping.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            _ptr(a), _ptr(b), cache[0], block_size, M, KV, hd)
+    return both if values else None
+
+
+def load_kv4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor, head_dim: int):
+    """Rows of a cache of 4 bits read back: (k, v) bf16 [M, KV, head_dim] of the slots (int32 [M], any order; outside the cache: zeros)."""
+    M = _last(slot_mapping, 1)
+    cache, block_size = _kv4("load_kv4", k_cache, head_dim)
+    gpu = _check("load_kv4", (k_cache, "k_cache", _U8, cache), (v_cache, "v_cache", _U8, cache), (slot_mapping, "slot_mapping", _I32, (M,)))
+    k, v = both = torch.empty(2, M, cache[1], head_dim, dtype=_BF, device=k_cache.device).unbind(0)
+    _launch("ssdk_load_kv4", gpu, k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr(), k.data_ptr(), v.data_ptr(), cache[0], block_size, M, cache[1], head_dim)
+    return both
+
+
+def paged_attention_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor, q_len: int,
+                        scale: float) -> torch.Tensor:
+    """paged_attention over a cache of 4 bits (kv4_caches): q [B * q_len, H, hd] bf16, block_tables int32 [B, max_blocks], context_lens int32 [B] with the new tokens.
+
+    Returns [B * q_len, H * hd].  Scale and minimum of a row act on scores and weights, so keys and values are not rounded.  Pages outside the cache are passed over, a row
+    that sees no key is zero, a NaN row of the cache makes NaN of the rows that see it."""
+    B, width, H, hd = _last(context_lens, 1), _last(block_tables, 2), *(q.shape[1:] if q.dim() == 3 else (-1, -1))
+    cache, block_size = _kv4("paged_attention_kv4", k_cache, hd)
+    gpu = _check("paged_attention_kv4", (q, "q", _BF, (B * q_len, H, hd)), (k_cache, "k_cache", _U8, cache), (v_cache, "v_cache", _U8, cache),
+                 (block_tables, "block_tables", _I32, (B, width)), (context_lens, "context_lens", _I32, (B,)))
+    out = q.new_empty(B * q_len, H * hd)
+    _launch("ssdk_paged_attn_kv4", gpu, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(), B, q_len, H, cache[1],
+            hd, block_size, width, cache[0], scale)
+    return out
