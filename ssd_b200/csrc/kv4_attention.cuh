@@ -2,6 +2,9 @@
 #pragma once
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
+#include "async_copy.cuh"
 #include "kv4.cuh"
 
 namespace ssdk {
@@ -10,14 +13,18 @@ namespace ssdk {
 // kv4_attn_kernel: softmax(scale q k^T) v, causal to the end of the context as in paged attention (query j of a sequence sees positions <= len - Q + j), grouped heads.
 // With k = s c + m and v = s' c' + m' of a token (c codes)
 //   q k = s (q c) + m sum(q)          O = sum_j (P_j s'_j) (c'_j - 8) + sum_j P_j (m'_j + 8 s'_j)
-// so that what meets in the products are codes, exact in bf16: keys and values are not rounded at all.  What is rounded is P s' (bf16, 2^-9 of a term at most, the codes
+// so that what meets in the products are codes, which are exact: keys and values are not rounded at all.  What is rounded is P s' (bf16, 2^-8 of a term at most, the codes
 // around their middle so that it is of the value's size); sums, references and the second term are fp32.
 // Bound by the bytes of the cache, then by the instructions that make codes into fragments.  The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that
-// keys (sixteen) and channels (sixteen) are the m of mma and the eight query rows of a usual group its n.  Nothing goes through shared memory: a quad's lanes read a key's row, 16
-// bytes each, as the A fragment of any eight products (which channels a product's k stands for is free, the query's fragments follow), eight lanes a value's row, and a
-// word of eight channels is four pairs of bf16 by a shift and a mask each: 16 + c has c in the top of its mantissa.  Of two values' words one byte_perm makes words whose halves
-// are the two keys of a fragment's register.
-// A cluster of blocks shares the keys of a key head of one sequence: pieces of 16 keys go round the blocks' warps, each with a softmax of its own; at the end warps meet, then blocks.
+// keys (sixteen) and channels (sixteen) are the m of mma and the eight query rows of a usual group its n.
+//   Scores are whole numbers: a mask (and a shift) makes four codes of a word bytes, and a query row, scaled by a power of two so that its largest lies in 2^14 .. 2^15 and rounded, is 256 h + l with a
+// byte each, so that its values are off by at most 2^-15 of its largest (those above 2^-7 of it by nothing).  The sums start at the word of 1.5 2^23, so that they are floats without a
+// conversion.  (bf16 codes take 64 instructions for sixteen keys where these take 24; mma on e4m3 is made of conversions and f16 here: four times as slow.)  Which channels a product's k stands for is
+// free: a quad's lanes read a key's row, 16 bytes each, and the query's fragments follow.
+//   Values: P has no such range, it is bf16 and so are the codes: 16 + c has c in the top of bf16's mantissa; of two values' words one byte_perm makes words whose halves are the
+// two keys of a fragment's register.
+// A cluster of blocks shares the keys of a key head of one sequence: chunks of 32 keys go round the blocks' warps, each with a ring of its own (cp.async, no barrier between
+// warps) and a softmax of its own; at the end warps meet, then blocks.
 // A page outside the cache is passed over, a row that sees no key is zero; a NaN row of keys or values makes NaN of the rows that see it and of no other.
 // ----------------------------------------------------------------------------------
 struct Kv4AttnParams {
@@ -31,28 +38,19 @@ struct Kv4AttnParams {
   float scale_log2;              // scale * log2(e)
 };
 constexpr float kKv4Slack = 8.f;
-constexpr int kKv4Warps = 8, kKv4Most = 16;   // warps of a block, blocks of a cluster
-constexpr int kv4_attn_smem(int HD, int NT) { return (kKv4Warps + 1) * 8 * NT * (HD + 8) * 4; }
+constexpr int kKv4Warps = 8, kKv4Most = 16, kKv4Stages = 3, kKv4Keys = 32;   // warps of a block, blocks of a cluster, a warp's ring, keys of a chunk
+constexpr int kv4_stage_bytes(int HD) { return 2 * kKv4Keys * (HD / 2 + 4); }   // keys' codes | values' codes | keys' pairs | values' pairs
+constexpr int kv4_attn_smem(int HD, int NT) {
+  const int ring = kKv4Warps * kKv4Stages * kv4_stage_bytes(HD), join = (kKv4Warps + 1) * 8 * NT * (HD + 8) * 4;
+  return ring > join ? ring : join;
+}
 
-SSDK_DEVINL uint32_t ld_nc_u32(const void* p) {
-  uint32_t r;
-  asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r) : "l"(p));
-  return r;
-}
-SSDK_DEVINL uint2 ld_nc_v2(const void* p) {
-  uint2 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
-}
-// nibbles P and P + 4 of a word as 16 + c in bf16
+// nibbles P and P + 4 of a word as c - 8 in bf16: 16 + c less 24
 template <int P>
 SSDK_DEVINL uint32_t kv4_pair(uint32_t w) {
-  const uint32_t x = P == 0 ? w << 3 : w >> (4 * P - 3);
-  return (x & 0x00780078u) | 0x41804180u;
-}
-SSDK_DEVINL uint32_t minus24(uint32_t x) {   // of both halves: codes around their middle (exact)
+  const uint32_t x = P == 0 ? w << 3 : w >> (4 * P - 3), y = (x & 0x00780078u) | 0x41804180u;
   uint32_t d;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(0x41c041c0u));
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(y), "r"(0x41c041c0u));
   return d;
 }
 SSDK_DEVINL uint32_t transpose_8x8(uint32_t x) {
@@ -60,17 +58,28 @@ SSDK_DEVINL uint32_t transpose_8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
   return d;
 }
-
-// what a lane holds of sixteen keys: words of the keys' rows g, g + 8 (of S^T) and of the values' rows, their pairs
+// 16 x 8 (+)= codes (bytes) x 32 bytes of a query, signed or not
+template <bool SIGNED>
+SSDK_DEVINL void mma_u8_16832(uint32_t* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if (SIGNED)
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+constexpr float kKv4Whole = 12582912.f;            // 1.5 2^23
+constexpr uint32_t kKv4WholeWord = 0x4b400000u;    // its word: a whole number below 2^22 added to it is added to the float
+// where the 16-byte piece c of the codes of value r lies in its stage: four lanes read the rows 2 t + const at a time, 8 (4) bytes a lane, from banks of their own
 template <int HD>
-struct Kv4Piece {
-  uint32_t k[2][HD / 32], v[4][HD / 64], pk[2], pv[2];
-  int pos;   // of the first key, -1: no page
-};
+SSDK_DEVINL int kv4_v_place(int r, int c) {
+  if (HD == 128) return (r >> 1) * 128 + (((r ^ (r >> 1)) & 1) << 6) + ((c ^ ((r >> 2 & 1) << 1)) << 4);
+  return (r >> 3) * 256 + ((r & 1) << 7) + ((r >> 1 & 3) << 5) + (c << 4);
+}
 
 template <int HD, int NT>
 __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 2 : 1) kv4_attn_kernel(const __grid_constant__ Kv4AttnParams p) {
-  constexpr int KS = HD / 16, KW = HD / 32, VW = HD / 64, CODES = HD / 2;
+  constexpr int KW = HD / 32, VW = HD / 64, CODES = HD / 2, K = kKv4Keys, STAGE = kv4_stage_bytes(HD);
   extern __shared__ __align__(16) uint8_t kv4_smem[];
   pdl_wait();
   pdl_launch_dependents();
@@ -83,224 +92,293 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 2 : 1) kv4_attn_kern
   const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size), ctx = len - p.Q;
   const int seen = min(len, ctx + (r0 + R - 1) / G + 1), seen_by_all = ctx + r0 / G + 1;   // positions that some row sees, that all do
 
-  // ---- queries: fragments in the order of the keys' words, sums ----
-  uint32_t qb[NT][KS][2];
-  float qs[NT][2];
-  int lim[NT][2];   // first position that rows 2 t, 2 t + 1 do not see
+  // ---- a warp's chunks of 32 keys: own, own + stride, ... ----
+  const int tiles = (max(seen, 0) + 15) >> 4, chunks = (tiles + 1) >> 1, stride = C * kKv4Warps, own = rank * kKv4Warps + warp;
+  const int n = own < chunks ? (chunks - own + stride - 1) / stride : 0;
+  const size_t record = (size_t)p.block_size * kv4_row_bytes(HD);
+  uint8_t* ring = kv4_smem + warp * kKv4Stages * STAGE;
+  // pages of the sixteen keys that lane & 1 says, of chunk first + lane / 2 of this warp's: sixteen chunks at a time, the next sixteen's on their way
+  struct Where { int page, off; };
+  auto look_up = [&](int first) {
+    Where w = {-1, 0};
+    const long long tile = 2 * (own + (long long)(first + (lane >> 1)) * stride) + (lane & 1);
+    if (tile < tiles) {
+      const int pos = (int)tile * 16, x = pos / p.block_size;
+      w.off = pos - x * p.block_size;
+      w.page = page_at(p.tables + (size_t)b * p.max_blocks + x, p.num_blocks);
+    }
+    return w;
+  };
+  Where here = {-1, 0}, next = look_up(0);
+  uint32_t missing = 0;   // two bits a stage: sixteen keys without a page
+  auto load = [&](int i, int stage) {
+    if (i >= n) return;
+    if ((i & 15) == 0) {
+      here = next;
+      next = look_up(i + 16);
+    }
+    uint8_t* to = ring + stage * STAGE;
+    missing &= ~(3u << (2 * stage));
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int r = r0 + n * 8 + g;
+    for (int h = 0; h < 2; ++h) {
+      const int page = __shfl_sync(0xffffffffu, here.page, (2 * i + h) & 31), off = __shfl_sync(0xffffffffu, here.off, (2 * i + h) & 31);
+      if (page < 0) {
+        missing |= 1u << (2 * stage + h);
+        continue;
+      }
+      const size_t base = ((size_t)page * p.kv_heads + kvh) * record;
+      const uint8_t *kc = p.k_cache + base + (size_t)off * CODES, *vc = p.v_cache + base + (size_t)off * CODES;
+      constexpr int PIECES = CODES;   // of 16 bytes, of sixteen keys' codes
+#pragma unroll
+      for (int u = 0; u < PIECES; u += 32) {
+        const int x = u + lane;
+        cp_async16(to + h * 16 * CODES + x * 16, kc + x * 16, true);
+        cp_async16(to + K * CODES + h * 16 * CODES + kv4_v_place<HD>(x / (CODES / 16), x % (CODES / 16)), vc + x * 16, true);
+      }
+      // pairs: four pieces of keys' and four of values'
+      if (lane < 8) {
+        const uint8_t* from = (lane < 4 ? p.k_cache : p.v_cache) + base + (size_t)p.block_size * CODES + (size_t)off * 4 + (lane & 3) * 16;
+        cp_async16(to + 2 * K * CODES + (lane >> 2) * K * 4 + h * 64 + (lane & 3) * 16, from, true);
+      }
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < kKv4Stages - 1; ++s) {
+    load(s, s);
+    cp_async_commit();
+  }
+
+  // ---- queries: fragments in the order of the keys' words (channels 0, 2, 4, 6 and 1, 3, 5, 7 of a word), sums ----
+  uint32_t qb[NT][KW][2][2];   // [.., byte, half of k]
+  float qs[NT][2], qf[NT][2];  // of rows 2 t, 2 t + 1: sum and unit, times scale * log2(e)
+  int lim[NT][2];              // first position that they do not see
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = r0 + nt * 8 + g;
     const __nv_bfloat16* q = p.q + ((size_t)(b * p.Q + r / G) * p.heads + kvh * G + r % G) * HD + t * (HD / 4);
-    float sum = 0.f;
+    float f[KW][8], sum = 0.f, top = 0.f;
 #pragma unroll
     for (int j = 0; j < KW; ++j) {
-      const uint4 x = n * 8 + g < R ? *reinterpret_cast<const uint4*>(q + j * 8) : make_uint4(0, 0, 0, 0);
-      qb[n][2 * j][0] = __byte_perm(x.x, x.z, 0x5410);   // channels 0 and 4 of the word, 1 and 5, 2 and 6, 3 and 7
-      qb[n][2 * j][1] = __byte_perm(x.x, x.z, 0x7632);
-      qb[n][2 * j + 1][0] = __byte_perm(x.y, x.w, 0x5410);
-      qb[n][2 * j + 1][1] = __byte_perm(x.y, x.w, 0x7632);
-      float f[8];
-      unpack_bf16x8(x, f);
-      sum += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
-    }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      unpack_bf16x8(nt * 8 + g < R ? *reinterpret_cast<const uint4*>(q + j * 8) : make_uint4(0, 0, 0, 0), f[j]);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      qs[n][e] = __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4) * p.scale_log2;
-      const int row = n * 8 + 2 * t + e;
-      lim[n][e] = row < R ? ctx + (r0 + row) / G + 1 : 0;
+      for (int c = 0; c < 8; ++c) {
+        sum += f[j][c];
+        top = fmaxf(top, fabsf(f[j][c]));
+      }
+    }
+#pragma unroll
+    for (int w = 1; w < 4; w *= 2) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, w);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    }
+    const int e = max((int)(__float_as_uint(top) >> 23), 14);   // (biased exponent)
+    const float up = __uint_as_float((uint32_t)(268 - e) << 23);   // 2^(14 - (e - 127))
+#pragma unroll
+    for (int j = 0; j < KW; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        qb[nt][j][0][h] = qb[nt][j][1][h] = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t w = (uint32_t)__float2int_rn(f[j][2 * c + h] * up);   // 256 h + l
+          qb[nt][j][0][h] |= (w >> 8 & 0xffu) << (8 * c);
+          qb[nt][j][1][h] |= (w & 0xffu) << (8 * c);
+        }
+      }
+    // a score is 1 / up = 2^(e - 127) 2^-14 times what the products give; a query that is not finite makes NaN (its sum alone might not)
+    float unit = __uint_as_float((uint32_t)min(e, 254) << 23) * p.scale_log2 * 0x1p-14f;
+    if (!(fabsf(sum) < INFINITY) || e == 255) unit = __uint_as_float(kKv4Nan);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = nt * 8 + 2 * t + i;
+      qs[nt][i] = __shfl_sync(0xffffffffu, sum, (2 * t + i) * 4) * p.scale_log2;
+      qf[nt][i] = __shfl_sync(0xffffffffu, unit, (2 * t + i) * 4);
+      lim[nt][i] = row < R ? ctx + (r0 + row) / G + 1 : 0;
     }
   }
 
   float o[NT][HD / 16][4], ref[NT][2], l[NT][2], low[NT][2];   // O^T, reference, sum, sum of P (m' + 8 s')
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+  for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-    for (int i = 0; i < HD / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+    for (int i = 0; i < HD / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      ref[n][e] = -INFINITY;
-      l[n][e] = low[n][e] = 0.f;
+      ref[nt][e] = -INFINITY;
+      l[nt][e] = low[nt][e] = 0.f;
     }
   }
 
-  // ---- pieces of 16 keys: own, own + stride, ...; pages of 32 of them at a time, one a lane ----
-  const int pieces = (max(seen, 0) + 15) >> 4, stride = C * kKv4Warps, own = rank * kKv4Warps + warp;
-  const size_t record = (size_t)p.block_size * kv4_row_bytes(HD);
-  // The keys of a piece as S^T's rows: row 2 t + (i & 1) + 8 (i >> 1) is key 4 i + t, so that a value's load i takes four neighbouring rows and a key's load eight.
-  const int key = 4 * (g & 1) + (g >> 1);
-  const int k_at = key * CODES + t * (CODES / 4), v_at = t * CODES + g * (CODES / 8), pair_at = p.block_size * CODES + key * 4;
-  int page = -1, off = 0;   // of piece own + (base + lane) * stride
-  auto look_up = [&](int first) {
-    const long long piece = own + (long long)(first + lane) * stride;
-    page = -1;
-    if (piece < pieces) {
-      const int pos = (int)piece * 16, x = pos / p.block_size;
-      off = pos - x * p.block_size;
-      page = page_at(p.tables + (size_t)b * p.max_blocks + x, p.num_blocks);
-    }
-  };
-  auto load = [&](Kv4Piece<HD>& x, int i) {   // this warp's piece i
-    if ((i & 31) == 0) look_up(i);
-    const int at_page = __shfl_sync(0xffffffffu, page, i & 31), at = __shfl_sync(0xffffffffu, off, i & 31);
-    x.pos = -1;
-    if (at_page < 0) return;
-    x.pos = (own + i * stride) * 16;
-    const size_t base = ((size_t)at_page * p.kv_heads + kvh) * record;
-    const uint8_t *kc = p.k_cache + base, *vc = p.v_cache + base;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint8_t* row = kc + at * CODES + k_at + h * 8 * CODES;
-      if constexpr (HD == 128) {
-        const uint4 w = ld_nc_v4(row);
-        x.k[h][0] = w.x; x.k[h][1] = w.y; x.k[h][2] = w.z; x.k[h][3] = w.w;
-      } else {
-        const uint2 w = ld_nc_v2(row);
-        x.k[h][0] = w.x; x.k[h][1] = w.y;
-      }
-      x.pk[h] = ld_nc_u32(kc + pair_at + at * 4 + h * 32);
-      x.pv[h] = ld_nc_u32(vc + pair_at + at * 4 + h * 32);
-    }
-#pragma unroll
-    for (int i4 = 0; i4 < 4; ++i4) {
-      const uint8_t* row = vc + at * CODES + v_at + i4 * 4 * CODES;
-      if constexpr (HD == 128) {
-        const uint2 w = ld_nc_v2(row);
-        x.v[i4][0] = w.x; x.v[i4][1] = w.y;
-      } else {
-        x.v[i4][0] = ld_nc_u32(row);
-      }
-    }
-  };
-
-  auto work = [&](const Kv4Piece<HD>& x) {
-    if (x.pos < 0) return;
-    float s[NT][4] = {};
-#pragma unroll
-    for (int j = 0; j < KW; ++j) {
-      const uint32_t a0[4] = {kv4_pair<0>(x.k[0][j]), kv4_pair<0>(x.k[1][j]), kv4_pair<1>(x.k[0][j]), kv4_pair<1>(x.k[1][j])};
-      const uint32_t a1[4] = {kv4_pair<2>(x.k[0][j]), kv4_pair<2>(x.k[1][j]), kv4_pair<3>(x.k[0][j]), kv4_pair<3>(x.k[1][j])};
-#pragma unroll
-      for (int n = 0; n < NT; ++n) mma_bf16_16816(s[n], a0, qb[n][2 * j][0], qb[n][2 * j][1]);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) mma_bf16_16816(s[n], a1, qb[n][2 * j + 1][0], qb[n][2 * j + 1][1]);
-    }
-    float sv[2], mv[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float sk = __uint_as_float(x.pk[h] << 16), mk = fmaf(-16.f, sk, __uint_as_float(x.pk[h] & 0xffff0000u)), f = sk * p.scale_log2;
-      sv[h] = __uint_as_float(x.pv[h] << 16);
-      mv[h] = fmaf(8.f, sv[h], __uint_as_float(x.pv[h] & 0xffff0000u));
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) s[n][2 * h + e] = fmaf(s[n][2 * h + e], f, mk * qs[n][e]);
-    }
-    const bool whole = x.pos + 16 <= seen_by_all;   // (the same for the warp)
-    uint32_t out_of_sight = 0;   // bits of the scores
-    if (!whole) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (x.pos + key + 8 * (e >> 1) >= lim[n][e & 1]) {
-            s[n][e] = -INFINITY;
-            out_of_sight |= 1u << (n * 4 + e);
-          }
-    }
-    // a row's reference is raised, and its sums rescaled, only when a score passes it by kKv4Slack (base 2)
-    bool grow = false;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) grow = grow || fmaxf(s[n][e], s[n][2 + e]) > ref[n][e] + kKv4Slack;
-    if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float top = fmaxf(s[n][e], s[n][2 + e]);
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)), ref[n][e]);
-          const float f = top == ref[n][e] ? 1.f : ex2_ftz(ref[n][e] - top);   // (from -inf: 0)
-          ref[n][e] = top;
-          l[n][e] *= f;
-          low[n][e] *= f;
-#pragma unroll
-          for (int i = 0; i < HD / 16; ++i) {
-            o[n][i][e] *= f;
-            o[n][i][2 + e] *= f;
-          }
-        }
-    }
-    uint32_t pb[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
+  // scores of a chunk's keys g, g + 8, .. and rows 2 t, 2 t + 1 to weights, and their product with the values.  MASK: some row does not see some key, or a page is missing
+  auto work = [&](const uint8_t* at, int x, int pos, uint32_t none, auto mask) {   // (x: which sixteen of the chunk)
+    constexpr bool MASK = decltype(mask)::value;
+    const uint32_t* pairs = reinterpret_cast<const uint32_t*>(at + 2 * K * CODES) + g;
+    float s[NT][4];
+    uint32_t hidden = 0;   // bits of the scores
+    {
+      uint32_t k[2][KW];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float w[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float y = ex2_ftz(s[n][2 * h + e] - (ref[n][e] == -INFINITY ? 0.f : ref[n][e]));
-          l[n][e] += y;
-          const bool none = out_of_sight >> (n * 4 + 2 * h + e) & 1u;   // (its pair may be anything: 0 x NaN is NaN)
-          low[n][e] = none ? low[n][e] : fmaf(y, mv[h], low[n][e]);
-          w[e] = none ? 0.f : y * sv[h];
+        const uint8_t* row = at + (x * 16 + h * 8 + g) * CODES + t * (CODES / 4);
+        if constexpr (HD == 128) {
+          const uint4 w = *reinterpret_cast<const uint4*>(row);
+          k[h][0] = w.x; k[h][1] = w.y; k[h][2] = w.z; k[h][3] = w.w;
+        } else {
+          const uint2 w = *reinterpret_cast<const uint2*>(row);
+          k[h][0] = w.x; k[h][1] = w.y;
         }
-        pb[n][h] = transpose_8x8(pack_bf16x2(w[0], w[1]));
+      }
+      uint32_t whole[NT][2][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) whole[nt][0][i] = whole[nt][1][i] = kKv4WholeWord;
+#pragma unroll
+      for (int j = 0; j < KW; ++j) {
+        const uint32_t a[4] = {k[0][j] & 0x0f0f0f0fu, k[1][j] & 0x0f0f0f0fu, k[0][j] >> 4 & 0x0f0f0f0fu, k[1][j] >> 4 & 0x0f0f0f0fu};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma_u8_16832<true>(whole[nt][0], a, qb[nt][j][0][0], qb[nt][j][0][1]);
+          mma_u8_16832<false>(whole[nt][1], a, qb[nt][j][1][0], qb[nt][j][1][1]);
+        }
       }
 #pragma unroll
-    for (int j = 0; j < VW; ++j) {
-      const uint32_t a01 = __byte_perm(x.v[0][j], x.v[1][j], 0x5410), b01 = __byte_perm(x.v[0][j], x.v[1][j], 0x7632);
-      const uint32_t a23 = __byte_perm(x.v[2][j], x.v[3][j], 0x5410), b23 = __byte_perm(x.v[2][j], x.v[3][j], 0x7632);
-      const uint32_t a[4][4] = {{minus24(kv4_pair<0>(a01)), minus24(kv4_pair<0>(b01)), minus24(kv4_pair<0>(a23)), minus24(kv4_pair<0>(b23))},
-                                {minus24(kv4_pair<1>(a01)), minus24(kv4_pair<1>(b01)), minus24(kv4_pair<1>(a23)), minus24(kv4_pair<1>(b23))},
-                                {minus24(kv4_pair<2>(a01)), minus24(kv4_pair<2>(b01)), minus24(kv4_pair<2>(a23)), minus24(kv4_pair<2>(b23))},
-                                {minus24(kv4_pair<3>(a01)), minus24(kv4_pair<3>(b01)), minus24(kv4_pair<3>(a23)), minus24(kv4_pair<3>(b23))}};
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t w = pairs[x * 16 + h * 8];
+        const float sk = __uint_as_float(w << 16), mk = __uint_as_float(w & 0xffff0000u);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_bf16_16816(o[n][4 * j + i], a[i], pb[n][0], pb[n][1]);
+          for (int e = 0; e < 2; ++e) {
+            float& v = s[nt][2 * h + e];
+            v = fmaf(__uint_as_float(whole[nt][0][2 * h + e]) - kKv4Whole, 256.f, __uint_as_float(whole[nt][1][2 * h + e]) - kKv4Whole);   // (exact to 2^-24)
+            v = fmaf(v, sk * qf[nt][e], mk * qs[nt][e]);
+            if (MASK && ((none >> x & 1u) || pos + x * 16 + h * 8 + g >= lim[nt][e])) {
+              v = -INFINITY;
+              hidden |= 1u << (nt * 4 + 2 * h + e);
+            }
+          }
+      }
+    }
+    // a row's reference is raised, and its sums rescaled, only when a score passes it by kKv4Slack (base 2)
+    float most[NT][2];
+    bool grow = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        most[nt][e] = fmaxf(s[nt][e], s[nt][2 + e]);
+        grow = grow || most[nt][e] > ref[nt][e] + kKv4Slack;
+      }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = most[nt][e];
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)), ref[nt][e]);
+          const float f = top == ref[nt][e] ? 1.f : ex2_ftz(ref[nt][e] - top);   // (from -inf: 0)
+          ref[nt][e] = top;
+          l[nt][e] *= f;
+          low[nt][e] *= f;
+#pragma unroll
+          for (int i = 0; i < HD / 16; ++i) {
+            o[nt][i][e] *= f;
+            o[nt][i][2 + e] *= f;
+          }
+        }
+    }
+    {
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t pair = pairs[K + x * 16 + h * 8];
+        const float sv = __uint_as_float(pair << 16), mv = fmaf(8.f, sv, __uint_as_float(pair & 0xffff0000u));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float w[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float y = ex2_ftz(s[nt][2 * h + e] - (MASK && ref[nt][e] == -INFINITY ? 0.f : ref[nt][e]));
+            l[nt][e] += y;
+            if (MASK && (hidden >> (nt * 4 + 2 * h + e) & 1u)) {   // (its pair may be anything: 0 x NaN is NaN)
+              w[e] = 0.f;
+            } else {
+              low[nt][e] = fmaf(y, mv, low[nt][e]);
+              w[e] = y * sv;
+            }
+          }
+          pb[nt][h] = transpose_8x8(pack_bf16x2(w[0], w[1]));
+        }
+      }
+      const uint8_t* values = at + K * CODES + x * 16 * CODES;
+      uint32_t v[4][VW];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {   // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+        const uint8_t* row = values + kv4_v_place<HD>(2 * t + (i & 1) + 8 * (i >> 1), g * (CODES / 8) / 16) + g * (CODES / 8) % 16;
+        if constexpr (HD == 128) {
+          const uint2 w = *reinterpret_cast<const uint2*>(row);
+          v[i][0] = w.x; v[i][1] = w.y;
+        } else {
+          v[i][0] = *reinterpret_cast<const uint32_t*>(row);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < VW; ++j) {
+        const uint32_t a01 = __byte_perm(v[0][j], v[1][j], 0x5410), b01 = __byte_perm(v[0][j], v[1][j], 0x7632);
+        const uint32_t a23 = __byte_perm(v[2][j], v[3][j], 0x5410), b23 = __byte_perm(v[2][j], v[3][j], 0x7632);
+        const uint32_t a[4][4] = {{kv4_pair<0>(a01), kv4_pair<0>(b01), kv4_pair<0>(a23), kv4_pair<0>(b23)}, {kv4_pair<1>(a01), kv4_pair<1>(b01), kv4_pair<1>(a23), kv4_pair<1>(b23)},
+                                  {kv4_pair<2>(a01), kv4_pair<2>(b01), kv4_pair<2>(a23), kv4_pair<2>(b23)}, {kv4_pair<3>(a01), kv4_pair<3>(b01), kv4_pair<3>(a23), kv4_pair<3>(b23)}};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(o[nt][4 * j + i], a[i], pb[nt][0], pb[nt][1]);
+      }
     }
   };
 
-  const int n_own = own < pieces ? (pieces - own + stride - 1) / stride : 0;
-  if (n_own > 0) {
-    Kv4Piece<HD> x, y;
-    load(x, 0);
-    for (int i = 0; i < n_own; i += 2) {
-      y.pos = -1;
-      if (i + 1 < n_own) load(y, i + 1);
-      work(x);
-      x.pos = -1;
-      if (i + 2 < n_own) load(x, i + 2);
-      work(y);
+  for (int i = 0, stage = 0; i < n; ++i, stage = stage + 1 == kKv4Stages ? 0 : stage + 1) {
+    __syncwarp();   // every lane is done with the stage that is filled now
+    load(i + kKv4Stages - 1, stage == 0 ? kKv4Stages - 1 : stage - 1);
+    cp_async_commit();
+    cp_async_wait<kKv4Stages - 1>();
+    __syncwarp();   // every lane's copies of this stage have landed
+    const int pos = (own + i * stride) * K;
+    const uint32_t none = missing >> (2 * stage) & 3u;
+    if (pos + K <= seen_by_all && !none) {
+#pragma unroll 1
+      for (int x = 0; x < 2; ++x) work(ring + stage * STAGE, x, pos, 0u, std::false_type());
+    } else {
+#pragma unroll 1
+      for (int x = 0; x < 2; ++x) work(ring + stage * STAGE, x, pos, none, std::true_type());
     }
   }
+  cp_async_wait<0>();
+  __syncthreads();   // the rings are read: their memory is the parts' now
 
   // ---- the warps' parts meet: [warp][row][HD + 8] O | reference, sum ----
   constexpr int LDO = HD + 8, ROWS = 8 * NT;
   float* parts = reinterpret_cast<float*>(kv4_smem);
   float* joined = parts + kKv4Warps * ROWS * LDO;   // [row][HD + 8]
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
 #pragma unroll
       for (int w = 4; w < 32; w *= 2) {
-        l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], w);
-        low[n][e] += __shfl_xor_sync(0xffffffffu, low[n][e], w);
+        l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], w);
+        low[nt][e] += __shfl_xor_sync(0xffffffffu, low[nt][e], w);
       }
-      float* row = parts + (warp * ROWS + n * 8 + 2 * t + e) * LDO;
+      float* row = parts + (warp * ROWS + nt * 8 + 2 * t + e) * LDO;
 #pragma unroll
       for (int j = 0; j < VW; ++j)   // channels g HD / 8 + 8 j ..
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           *reinterpret_cast<float4*>(row + g * (HD / 8) + 8 * j + 4 * h) =
-              make_float4(o[n][4 * j][2 * h + e] + low[n][e], o[n][4 * j + 1][2 * h + e] + low[n][e], o[n][4 * j + 2][2 * h + e] + low[n][e], o[n][4 * j + 3][2 * h + e] + low[n][e]);
-      if (g == 0) *reinterpret_cast<float2*>(row + HD) = make_float2(ref[n][e], l[n][e]);
+              make_float4(o[nt][4 * j][2 * h + e] + low[nt][e], o[nt][4 * j + 1][2 * h + e] + low[nt][e], o[nt][4 * j + 2][2 * h + e] + low[nt][e], o[nt][4 * j + 3][2 * h + e] + low[nt][e]);
+      if (g == 0) *reinterpret_cast<float2*>(row + HD) = make_float2(ref[nt][e], l[nt][e]);
     }
   __syncthreads();
   // four columns of a row
@@ -336,25 +414,19 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 2 : 1) kv4_attn_kern
   cluster.sync();
   for (int idx = rank * kKv4Warps * 32 + threadIdx.x; idx < R * (HD / 4); idx += C * kKv4Warps * 32) {
     const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
-    float2 ml[kKv4Most];
-    float4 v[kKv4Most];
     float top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int c = 0; c < kKv4Most; ++c)
-      if (c < C) {
-        const float* row = cluster.map_shared_rank(joined, c) + r * LDO;
-        ml[c] = *reinterpret_cast<const float2*>(row + HD);
-        v[c] = *reinterpret_cast<const float4*>(row + d);
-        top = fmaxf(top, ml[c].x);
-      }
+#pragma unroll 4
+    for (int c = 0; c < C; ++c) top = fmaxf(top, cluster.map_shared_rank(joined, c)[r * LDO + HD]);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int c = 0; c < kKv4Most; ++c)
-      if (c < C) {
-        const float f = top == -INFINITY ? 1.f : exp2f(ml[c].x - top);
-        acc.x += v[c].x * f; acc.y += v[c].y * f; acc.z += v[c].z * f; acc.w += v[c].w * f;
-        sum += ml[c].y * f;
-      }
+#pragma unroll 4
+    for (int c = 0; c < C; ++c) {
+      const float* row = cluster.map_shared_rank(joined, c) + r * LDO;
+      const float2 ml = *reinterpret_cast<const float2*>(row + HD);
+      const float4 v = *reinterpret_cast<const float4*>(row + d);
+      const float f = top == -INFINITY ? 1.f : exp2f(ml.x - top);
+      acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+      sum += ml.y * f;
+    }
     store(r, d, acc, sum);
   }
   cluster.sync();   // no block leaves while its part is read

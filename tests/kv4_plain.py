@@ -98,10 +98,12 @@ def attention(q, k_cache, v_cache, table, lens, q_len, scale):
                 # the two sums of an output: codes around their middle, and what is left
                 one = p @ (vpair[seen, :1] * (vcode[seen] - 8)).abs()
                 two = p @ (vpair[seen, 1:] + 8 * vpair[seen, :1]).abs().expand(-1, hd)
-                # scores: hd / 16 sums of 16 products with 16 + code in fp32, each off by 2^-22 of the terms' size, and the minimum's part; a weight moves by as much as its score
+                # scores: hd / 16 sums of 16 products with 16 + code in fp32 at most, each off by 2^-22 of the terms' size, and the minimum's part; a weight moves by as much as its score
                 size = rows.abs() @ (pair[seen, :1].abs() * (16 + c[seen])).t() + rows.abs().sum(1, keepdim=True) * (pair[seen, 1:] - 16 * pair[seen, :1]).abs().t()
-                spread = (size * abs(scale)).amax(1, keepdim=True)
+                spread = (size * abs(scale)).amax(1, keepdim=True) * 2 ** -19
+                # a query's values as whole numbers of sixteen bits: off by half a unit, 2^-15 of the row's largest, before they meet scale x code
+                spread = spread + abs(scale) * rows.abs().amax(1, keepdim=True) * 2 ** -15 * (pair[seen, :1].abs() * c[seen]).sum(1).amax()
                 # weights times scale are rounded to bf16 once (2^-8 at most), the output once more; sums over all keys in fp32
                 out[b * q_len + j, g * G:(g + 1) * G] = o
-                slack[b * q_len + j, g * G:(g + 1) * G] = (o.abs() + one) * 2 ** -8 + (one + two) * (2 ** -16 + 2 * spread * 2 ** -19 + 2 * int(seen.sum()) * 2 ** -23) + 1e-30
+                slack[b * q_len + j, g * G:(g + 1) * G] = (o.abs() + one) * 2 ** -8 + (one + two) * (2 ** -16 + 2 * spread + 2 * int(seen.sum()) * 2 ** -23) + 1e-30
     return out.view(M, H * hd), slack.view(M, H * hd)
