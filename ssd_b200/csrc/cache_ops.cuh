@@ -154,13 +154,6 @@ struct RopeAxesParams {
 constexpr int kRopeAxesThreads = 128, kRopeAxesAhead = 2;
 constexpr int rope_axes_heads(int HD) { return 32 / (HD / 16) * kRopeAxesAhead; }   // that a warp asks for at once
 
-#ifndef SSDK_HOST_EMU
-SSDK_DEVINL uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-#endif
 // eight bf16 values as four pairs of fp32, and back
 SSDK_DEVINL void pairs_of(const uint4& v, uint64_t* f) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};

@@ -1,10 +1,11 @@
-// kv4_ops.cu — entry points (include/ssdk.h) of the paged cache held in 4 bits: kv4.cuh, kv4_attention.cuh.
+// kv4_ops.cu — entry points (include/ssdk.h) of the paged cache held in 4 bits: kv4.cuh, kv4_attention.cuh, kv4_tiles.cuh.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
 
 #include "../../include/ssdk.h"
 #include "kv4_attention.cuh"
+#include "kv4_tiles.cuh"
 #include "op_host.cuh"
 
 using namespace ssdk;
@@ -42,10 +43,10 @@ static int store(const Kv4StoreParams& p, int head_dim, void* stream) {
 }
 
 // Blocks that share the keys of a key head (a cluster): as many as make the fewest waves of the longest context's pieces, a block's start and end as long as some 512 keys.
-static int kv4_cluster(int64_t units, int64_t keys, int resident) {
+static int kv4_cluster(int64_t units, int64_t keys, int resident, int most) {
   int best = 1;
   int64_t least = INT64_MAX;
-  for (int c = 1; c <= kKv4Most; c *= 2) {
+  for (int c = 1; c <= most; c *= 2) {
     const int64_t cost = (units * c + resident * kSms - 1) / (resident * kSms) * (512 + 16 * c + keys / c);
     if (cost < least) {
       least = cost;
@@ -60,8 +61,25 @@ static int launch_attn(Launcher& L, const Kv4AttnParams& p) {
   CKI(with_smem(kv4_attn_kernel<HD, NT>, kv4_attn_smem(HD, NT), kSmemOnly | 2, done));
   const int64_t rows = (int64_t)(p.heads / p.kv_heads) * p.Q, tiles = (rows + 8 * NT - 1) / (8 * NT);
   if (tiles > 65535) return fail("paged_attn_kv4: q_len=%d", p.Q);
-  L.cluster = kv4_cluster((int64_t)p.B * p.kv_heads * tiles, (int64_t)p.max_blocks * p.block_size, NT == 1 ? 2 : 1);
+  L.cluster = kv4_cluster((int64_t)p.B * p.kv_heads * tiles, (int64_t)p.max_blocks * p.block_size, NT == 1 ? 2 : 1, kKv4Most);
   return L.go(kv4_attn_kernel<HD, NT>, dim3(p.kv_heads * L.cluster, p.B, (unsigned)tiles), dim3(kKv4Warps * 32), kv4_attn_smem(HD, NT), p);
+}
+template <int HD, bool TWIN>
+static int launch_tiles(Launcher& L, const Kv4AttnParams& a) {
+  static std::atomic<bool> done[64];
+  CKI(with_smem(kv4_tile_kernel<HD, TWIN>, kv4_tile_smem(HD), kSmemClusters, done));
+  WaitWord* waits = op_waits();
+  if (!waits) return fail("paged_attn_kv4: pinned word for bounded waits not allocated");
+  CKI(waits->check("an earlier call of attention without an engine left is not complete (NaN rows)"));
+  Kv4TileParams p;
+  p.a = a;
+  const int most = kKv4TileRows / (TWIN ? 2 : 1) / (a.heads / a.kv_heads), tiles = (a.Q + most - 1) / most;
+  if (tiles > 65535) return fail("paged_attn_kv4: q_len=%d", a.Q);
+  p.tokens = (a.Q + tiles - 1) / tiles;
+  p.timeout = waits->word;
+  const int blocks = TWIN && HD == 64 ? 8 : kKv4Most;   // (their join has a lane of HD / 4 for each part)
+  L.cluster = kv4_cluster((int64_t)a.B * a.kv_heads * tiles, (int64_t)a.max_blocks * a.block_size, 2, blocks);
+  return L.go(kv4_tile_kernel<HD, TWIN>, dim3(a.kv_heads * L.cluster, a.B, tiles), dim3(kKv4TileThreads), kv4_tile_smem(HD), p);
 }
 
 extern "C" {
@@ -147,7 +165,9 @@ int ssdk_paged_attn_kv4(const void* q, const void* k_cache, const void* v_cache,
   p.scale_log2 = scale_log2;
   Launcher L = launcher(stream);
   if ((int64_t)(heads / kv_heads) * q_len <= 8) return head_dim == 64 ? launch_attn<64, 1>(L, p) : launch_attn<128, 1>(L, p);
-  return head_dim == 64 ? launch_attn<64, 2>(L, p) : launch_attn<128, 2>(L, p);
+  if ((int64_t)(heads / kv_heads) * q_len <= 16) return head_dim == 64 ? launch_attn<64, 2>(L, p) : launch_attn<128, 2>(L, p);
+  if ((int64_t)(heads / kv_heads) * q_len <= 64) return head_dim == 64 ? launch_tiles<64, true>(L, p) : launch_tiles<128, true>(L, p);
+  return head_dim == 64 ? launch_tiles<64, false>(L, p) : launch_tiles<128, false>(L, p);
 }
 
 }  // extern "C"

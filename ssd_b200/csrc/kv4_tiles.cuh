@@ -1,0 +1,423 @@
+// kv4_tiles.cuh — attention over a paged cache held in 4 bits (kv4.cuh) of more than sixteen query rows to a key head, on tcgen05.
+//
+// S = Q C^T of up to 128 rows (query tokens x the heads that share a key head) and 64 keys' codes into TMEM, P = exp2(S s + m sum(q) - reference) one row per thread, O += (P s') (C' - 8) with
+// P s' out of TMEM; what the minima give is a sum of its own (kv4_attn_kernel has the formulas).  Codes become bf16 on their way into shared memory: 16 + c for keys, c - 8 for values, both exact,
+// by a shift and a mask for two.  A word of eight channels gives them in the order 0, 4, 1, 5, 2, 6, 3, 7: the queries are stored in that order too, and the outputs put back.
+// Four warps bring codes in (registers, a chunk ahead of the one that they write, its pages two ahead), one issues the products, four have the rows.  Scales and minima of a chunk's keys lie beside its
+// values, as pairs of keys, so that a row takes two at a time.  A cluster of blocks shares the chunks of a key head; their sums meet in shared memory.
+// A row takes 32 keys at a time (64 scores and as many scales pass the registers of nine warps twice on an SM).  TWIN: up to 64 rows lie in the tile twice, rows 0 .. 63 take a chunk's first 32 keys and
+// 64 .. 127 the others, each with zeros for weights of the other half and a reference of its own: all four warps work on half of the scores where two would on all, and the products are no more.
+#pragma once
+#include "kv4_attention.cuh"
+#include "prompt_attention.cuh"
+
+namespace ssdk {
+
+constexpr int kKv4TileRows = 128, kKv4TileKeys = 64, kKv4TileThreads = 288, kKv4Producers = 128;   // warps: 4 of rows, 4 of codes, one of products
+constexpr int kv4_tile_body(int HD) { return kKv4TileRows * HD * 2 + 2 * 2 * kKv4TileKeys * HD * 2; }   // queries | two stages of keys | of values
+constexpr int kv4_tile_smem(int HD) {
+  const int join = kKv4TileRows * (HD + 4) * 4, body = kv4_tile_body(HD);
+  return (body > join ? body : join) + 1024;
+}
+
+// nibbles P and P + 4 of a word as 16 + c in bf16
+template <int P>
+SSDK_DEVINL uint32_t kv4_pair16(uint32_t w) {
+  const uint32_t x = P == 0 ? w << 3 : w >> (4 * P - 3);
+  return (x & 0x00780078u) | 0x41804180u;
+}
+SSDK_DEVINL uint4 kv4_words16(uint32_t w) { return make_uint4(kv4_pair16<0>(w), kv4_pair16<1>(w), kv4_pair16<2>(w), kv4_pair16<3>(w)); }
+SSDK_DEVINL uint4 kv4_words(uint32_t w) { return make_uint4(kv4_pair<0>(w), kv4_pair<1>(w), kv4_pair<2>(w), kv4_pair<3>(w)); }
+// 16-byte piece c of a row of 128 bytes under the 128-byte swizzle
+SSDK_DEVINL int swizzled(int row, int c) { return row * 128 + ((c ^ (row & 7)) << 4); }
+
+struct Kv4TileParams {
+  Kv4AttnParams a;
+  int tokens;                    // query tokens of a tile
+  unsigned* timeout;             // (rows whose waits ran out are NaN)
+};
+
+template <int HD, bool TWIN>
+__global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __grid_constant__ Kv4TileParams pp) {
+  namespace cg = cooperative_groups;
+  constexpr int HALVES = HD / 64, CODES = HD / 2, K = kKv4TileKeys;
+  constexpr int kQHalf = kKv4TileRows * 128, kKHalf = K * 128, kTile = HALVES * kKHalf;
+  const Kv4AttnParams& p = pp.a;
+  extern __shared__ uint8_t kv4_tile_raw[];
+  __shared__ __align__(8) uint64_t k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2];
+  __shared__ __align__(16) float key_pairs[2][K * 2], value_pairs[2][K * 2];   // of two keys: scale, scale, what goes with the sum, the same (times scale * log2(e) for keys)
+  __shared__ __align__(16) int at_pos[2][4];   // position of a chunk's sixteen keys, behind every context where they have no page
+  __shared__ uint32_t tmem_slot;
+  uint8_t* smem = kv4_tile_raw + ((1024u - (smem_u32(kv4_tile_raw) & 1023u)) & 1023u);
+  uint8_t* sQ = smem;
+  uint8_t* sK = sQ + HALVES * kQHalf;
+  uint8_t* sV = sK + 2 * kTile;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = cluster.num_blocks(), rank = cluster.block_rank();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = blockIdx.x / C, b = blockIdx.y, tile = (int)gridDim.z - 1 - (int)blockIdx.z;   // (the tiles that see most keys first)
+  const int G = p.heads / p.kv_heads, tok0 = tile * pp.tokens, tq = min(pp.tokens, p.Q - tok0), rows = tq * G;
+  const int half = (rows + 31) & ~31;                // rows of the warps that have some
+  const int live = TWIN ? 2 * half : half;           // threads that hand P over
+
+  if (warp == 8) {
+    if (lane == 0) {
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(&k_full[s], kKv4Producers);
+        mbar_init(&v_full[s], kKv4Producers);
+        mbar_init(&s_full[s], 1);
+        mbar_init(&p_full[s], live);
+        mbar_init(&pv_done[s], 1);
+      }
+      fence_mbar_init();
+    }
+    __syncwarp();
+    tmem_alloc(&tmem_slot, 256);
+    tmem_relinquish();
+  }
+  pdl_wait();
+  // queries, eight channels in the order of a word's pairs; rows behind the last one are zero
+  for (int i = threadIdx.x; i < kKv4TileRows * (HD / 8); i += kKv4TileThreads) {
+    const int at = i / (HD / 8), c = i % (HD / 8), r = TWIN ? at & 63 : at;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (r < rows) x = *reinterpret_cast<const uint4*>(p.q + ((size_t)(b * p.Q + tok0 + r / G) * p.heads + kvh * G + r % G) * HD + c * 8);
+    *reinterpret_cast<uint4*>(sQ + (c >> 3) * kQHalf + swizzled(at, c & 7)) =
+        make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+  }
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot, tmem_o = tmem + 128;   // S / P buffers at columns 0 and 64, O behind them
+  pdl_launch_dependents();   // (this block has its tensor memory: what is scheduled now may take the rest of the SM's and wait for this grid)
+
+  const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size), ctx = len - p.Q + tok0;
+  const int seen = max(0, min(len, ctx + tq)), seen_by_all = ctx + 1;   // positions that some row sees, that all do
+  const int chunks = (seen + K - 1) / K, n = rank < chunks ? (chunks - rank + C - 1) / C : 0;   // chunk i of this block is rank + i C
+  // Chunk i is in stage and on barriers i & 1, parity(i) is that use's.  A wait by parity is only right while the barrier is in that use or the one behind it:
+  //   k_full, v_full: whoever waits for chunk i has to be through with it before its stage is written anew (the keys' behind s_full, the values' behind pv_done, which needs every row's P).
+  //   s_full: the producers and the rows ask for chunk i, and chunk i + 2's needs keys of the former and, through p_full, P of the latter.
+  //   p_full: chunk i + 2's needs the rows to have seen its scores, which are issued behind the product of chunk i.
+  //   pv_done: the scores of chunk i + 1 ask for chunk i - 1; the producers ask for chunk i - 2 before they bring chunk i's values; the rows ask for chunk i - 1, and chunk i + 1's product needs their P.
+  auto parity = [](int i) { return (uint32_t)(i >> 1) & 1u; };
+  float l = 0.f, m = -INFINITY, low = 0.f;
+  bool ok = true;
+
+  if (warp >= 4 && warp < 8) {
+    // ---- codes: a thread has PER pieces of 32 channels (eight lanes are eight rows) of the keys and of the values, and the pair of one of either ----
+    constexpr int NP = HD / 32, PER = K * NP / kKv4Producers;
+    const int tid = threadIdx.x - 128, pw = tid >> 5, piece = (lane >> 3) % NP;
+    const size_t record = (size_t)p.block_size * kv4_row_bytes(HD);
+    const int step = C * K, step_x = step / p.block_size, step_off = step - step_x * p.block_size;
+    // where sixteen keys of this block's next chunk to be looked up are: entry of the table, offset in the page
+    struct Place { int x, off, page, at, pos; };
+    auto first = [&](int sixteen) {
+      Place w;
+      w.pos = rank * K + sixteen * 16;
+      w.x = w.pos / p.block_size;
+      w.off = w.pos - w.x * p.block_size;
+      w.page = -1;
+      w.at = 0;
+      return w;
+    };
+    auto look_up = [&](Place& w) {   // (positions stay below 2^31: the host sees to it; what a page is, is looked at where it is used, a chunk later)
+      w.page = -1;
+      if (w.pos < seen) w.page = p.tables[(size_t)b * p.max_blocks + w.x];
+      w.at = w.off;
+      w.pos += step;
+      w.x += step_x;
+      w.off += step_off;
+      if (w.off >= p.block_size) {
+        w.off -= p.block_size;
+        ++w.x;
+      }
+    };
+    int row[PER];
+    Place of[PER], mine = first((tid & 63) >> 4);
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      row[u] = (HD == 128 ? u * 4 + pw : 2 * pw + (lane >> 4)) * 8 + (lane & 7);
+      of[u] = first(row[u] >> 4);
+      look_up(of[u]);
+    }
+    look_up(mine);
+    uint4 kc[PER], vc[PER];
+    uint32_t pair = 0;
+    int pos = 0;
+    auto load = [&]() {   // of the chunk that was looked up; then the next one's pages
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        kc[u] = vc[u] = make_uint4(0, 0, 0, 0);
+        if (of[u].page >= 0 && of[u].page < p.num_blocks) {
+          const size_t at = ((size_t)of[u].page * p.kv_heads + kvh) * record + (size_t)(of[u].at + (row[u] & 15)) * CODES + piece * 16;
+          kc[u] = ld_nc_v4(p.k_cache + at);
+          vc[u] = ld_nc_v4(p.v_cache + at);
+        }
+        look_up(of[u]);
+      }
+      pair = 0;
+      const bool there = mine.page >= 0 && mine.page < p.num_blocks;
+      pos = there ? mine.pos - step : kNoPosition;
+      if (there && pos + (tid & 15) < len)   // (behind the context it may be anything)
+        pair = *reinterpret_cast<const uint32_t*>((tid < 64 ? p.k_cache : p.v_cache) + ((size_t)mine.page * p.kv_heads + kvh) * record + (size_t)p.block_size * CODES + (size_t)(mine.at + (tid & 15)) * 4);
+      look_up(mine);
+    };
+    if (n > 0) load();
+    for (int i = 0; i < n; ++i) {
+      uint4 k_now[PER], v_now[PER];
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        k_now[u] = kc[u];
+        v_now[u] = vc[u];
+      }
+      const uint32_t pair_now = pair;
+      const int pos_now = pos, s = i & 1;
+      if (i + 1 < n) load();
+      if (i >= 2 && !tile_wait_warp(&s_full[s], parity(i - 2), pp.timeout)) break;   // the scores of chunk i - 2 have read their keys
+      uint8_t* dst = sK + s * kTile;
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        const uint32_t w[4] = {k_now[u].x, k_now[u].y, k_now[u].z, k_now[u].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + (piece >> 1) * kKHalf + swizzled(row[u], (piece & 1) * 4 + j)) = kv4_words16(w[j]);
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&k_full[s]);
+      if (i >= 2 && !tile_wait_warp(&pv_done[s], parity(i - 2), pp.timeout)) break;   // its product has read its values, its rows their pairs
+      dst = sV + s * kTile;
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        const uint32_t w[4] = {v_now[u].x, v_now[u].y, v_now[u].z, v_now[u].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + (piece >> 1) * kKHalf + swizzled(row[u], (piece & 1) * 4 + j)) = kv4_words(w[j]);
+      }
+      {
+        const int key = tid & 63;
+        const float scale = __uint_as_float(pair_now << 16), minimum = __uint_as_float(pair_now & 0xffff0000u);
+        float* to = (tid < 64 ? key_pairs[s] : value_pairs[s]) + (key >> 1) * 4 + (key & 1);
+        to[0] = tid < 64 ? scale * p.scale_log2 : scale;
+        to[2] = tid < 64 ? fmaf(-16.f, scale, minimum) * p.scale_log2 : fmaf(8.f, scale, minimum);
+        if (tid < 64 && (key & 15) == 0) at_pos[s][key >> 4] = pos_now;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&v_full[s]);
+    }
+  } else if (warp == 8) {
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = make_umma_idesc_bf16(kKv4TileRows, K);
+      constexpr uint32_t idesc_o = make_umma_idesc_bf16(kKv4TileRows, HD) | (1u << 16);   // V: b_major = MN
+      auto scores = [&](int i) {
+        if (!tile_wait(&k_full[i & 1], parity(i), pp.timeout)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          const uint64_t qd = make_umma_desc_k128(sQ + h * kQHalf), kd = make_umma_desc_k128(sK + (i & 1) * kTile + h * kKHalf);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_bf16_ss(tmem + (i & 1) * 64, qd + 2 * k, kd + 2 * k, idesc_s, (uint32_t)((h | k) != 0));
+        }
+        umma_commit(&s_full[i & 1]);
+        return true;
+      };
+      bool go = n > 0 && scores(0);
+      for (int i = 0; i < n && go; ++i) {
+        // the scores of chunk i + 1 go over the P that the product of chunk i - 1 reads
+        if (i > 0 && !(go = tile_wait(&pv_done[(i - 1) & 1], parity(i - 1), pp.timeout))) break;
+        if (i + 1 < n && !(go = scores(i + 1))) break;
+        if (!(go = tile_wait(&v_full[i & 1], parity(i), pp.timeout) && tile_wait(&p_full[i & 1], parity(i), pp.timeout))) break;
+        tc_fence_after();
+        const uint64_t vd = make_umma_desc_mn128(sV + (i & 1) * kTile, kKHalf);
+#pragma unroll
+        for (int k = 0; k < K / 16; ++k)   // 16 keys: 2048 B of V, 8 columns of P
+          umma_bf16_ts(tmem_o, tmem + (i & 1) * 64 + 8 * k, vd + 128 * k, idesc_o, (uint32_t)((i | k) != 0));
+        umma_commit(&pv_done[i & 1]);
+      }
+    }
+    __syncwarp();
+  } else if (warp < 4 && (TWIN ? (warp & 1) * 32 : warp * 32) < half) {
+    const int at = warp * 32 + lane, r = TWIN ? at & 63 : at;
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const int lim = ctx + r / G + 1;   // first position this row does not see (rows behind the tile's: some, dropped)
+    float sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < HD / 8; ++c) {
+      float f[8];
+      unpack_bf16x8(*reinterpret_cast<const uint4*>(sQ + (c >> 3) * kQHalf + swizzled(at, c & 7)), f);
+      sum += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+    }
+    if (!(fabsf(sum) < INFINITY)) sum = __uint_as_float(kKv4Nan);   // (a query that is not finite makes NaN, not one infinity less another or more)
+    const uint64_t sum2 = pack2(sum, sum);
+    for (int i = 0; i < n && ok; ++i) {
+      const uint32_t sp = tmem + lanes + (uint32_t)(i & 1) * 64u;
+      if (!(ok = tile_wait_warp(&v_full[i & 1], parity(i), pp.timeout) && tile_wait_warp(&s_full[i & 1], parity(i), pp.timeout))) break;
+      tc_fence_after();
+#pragma unroll 1
+      for (int h = TWIN ? warp >> 1 : 0; h < (TWIN ? (warp >> 1) + 1 : 2); ++h) {   // 32 keys
+        const int2 pos2 = *reinterpret_cast<const int2*>(&at_pos[i & 1][2 * h]);
+        const int pos[2] = {pos2.x, pos2.y};
+        const bool whole = max(pos[0], pos[1]) + 16 <= seen_by_all;
+        const ulonglong2 *kp = reinterpret_cast<const ulonglong2*>(key_pairs[i & 1]) + 16 * h, *vp = reinterpret_cast<const ulonglong2*>(value_pairs[i & 1]) + 16 * h;
+        uint32_t u[32];
+        tmem_ld_32x32b_x16(sp + 32 * h, u);
+        tmem_ld_32x32b_x16(sp + 32 * h + 16, u + 16);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          const ulonglong2 w = kp[c >> 1];
+          float x, y;
+          unpack2(fma2(pack2(__uint_as_float(u[c]), __uint_as_float(u[c + 1])), w.x, mul2(sum2, w.y)), &x, &y);
+          u[c] = __float_as_uint(x);
+          u[c + 1] = __float_as_uint(y);
+        }
+        if (!whole) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (pos[c / 16] + c % 16 >= lim) u[c] = 0xff800000u;   // -inf
+        }
+        float top[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) top[c] = max3(__uint_as_float(u[c]), __uint_as_float(u[c + 4]), __uint_as_float(u[c + 8]));
+#pragma unroll
+        for (int c = 12; c < 28; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(u[c + e]), __uint_as_float(u[c + 4 + e]));
+        const float mx = fmaxf(max3(max3(top[0], top[1], __uint_as_float(u[28])), max3(top[2], top[3], __uint_as_float(u[29])), __uint_as_float(u[30])), __uint_as_float(u[31]));
+        const bool grow = mx > m + kPromptSlack;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float f = grow ? exp2f(m - mx) : 1.f;   // (m = -inf: 0)
+          if (grow) m = mx;
+          l *= f;
+          low *= f;
+          if (i > 0) {
+            if (!(ok = tile_wait_warp(&pv_done[(i - 1) & 1], parity(i - 1), pp.timeout))) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 16) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(tmem_o + lanes + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st_32x32b_x16(tmem_o + lanes + c, o);
+            }
+          }
+          if (!TWIN && h) {   // the weights of the 32 keys before (rounded twice then)
+            uint32_t o[16];
+            tmem_st_wait();
+            tmem_ld_32x32b_x16(sp, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j] = pack_bf16x2(__uint_as_float(o[j] << 16) * f, __uint_as_float(o[j] & 0xffff0000u) * f);
+            tmem_st_32x32b_x16(sp, o);
+          }
+        }
+        const float ms = m == -INFINITY ? 0.f : m;
+        if (whole) {
+          const uint64_t off = pack2(-ms, -ms);
+          uint64_t sums = 0, lows = 0;
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            const ulonglong2 w = vp[c >> 1];
+            float x, y;
+            unpack2(add2(pack2(__uint_as_float(u[c]), __uint_as_float(u[c + 1])), off), &x, &y);
+            const uint64_t e = pack2(ex2_ftz(x), ex2_ftz(y));
+            sums = add2(sums, e);
+            lows = fma2(e, w.y, lows);
+            unpack2(mul2(e, w.x), &x, &y);
+            u[c >> 1] = pack_bf16x2(x, y);
+          }
+          float x, y;
+          unpack2(sums, &x, &y);
+          l += x + y;
+          unpack2(lows, &x, &y);
+          low += x + y;
+        } else {   // (a pair that a row does not see may be NaN: 0 x NaN)
+          const float* w = value_pairs[i & 1] + 64 * h;
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            float z[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const bool there = pos[c / 16] + c % 16 + e < lim;
+              const float y = ex2_ftz(__uint_as_float(u[c + e]) - ms);
+              l += y;
+              if (there) low = fmaf(y, w[2 * c + 2 + e], low);
+              z[e] = there ? y * w[2 * c + e] : 0.f;
+            }
+            u[c >> 1] = pack_bf16x2(z[0], z[1]);
+          }
+        }
+        tmem_st_32x32b_x16(sp + 16 * h, u);
+        if (TWIN) {
+#pragma unroll
+          for (int c = 0; c < 16; ++c) u[c] = 0;
+          tmem_st_32x32b_x16(sp + 16 * (1 - h), u);
+        }
+      }
+      if (!ok) break;
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&p_full[i & 1]);
+    }
+    if (ok && n > 0) ok = tile_wait_warp(&pv_done[(n - 1) & 1], parity(n - 1), pp.timeout);
+    tc_fence_after();
+  }
+
+  // ---- the sums of a row: [row][HD + 4] O | reference, sum over queries, keys and values (every product has read them) ----
+  constexpr int LDO = HD + 4;
+  float* joined = reinterpret_cast<float*>(smem);
+  __syncthreads();
+  if (warp < 4 && (TWIN ? (warp & 1) * 32 : warp * 32) < half) {
+    const int r = warp * 32 + lane;
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const bool some = ok && n > 0;
+#pragma unroll 1
+    for (int c = 0; c < HD; c += 16) {
+      uint32_t o[16];
+      if (some) {
+        tmem_ld_32x32b_x16(tmem_o + lanes + c, o);
+        tmem_ld_wait();
+      }
+      float f[16];   // channels 0, 4, 1, 5, 2, 6, 3, 7 of eight
+#pragma unroll
+      for (int j = 0; j < 16; ++j) f[(j & 8) + ((j & 7) >> 1) + 4 * (j & 1)] = some ? __uint_as_float(o[j]) + low : 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(joined + r * LDO + c + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+    }
+    // a wait ran out: the row is NaN.  Without chunks (or keys) the row has no part in the sum.
+    *reinterpret_cast<float2*>(joined + r * LDO + HD) = ok ? make_float2(m, l) : make_float2(0.f, __uint_as_float(kKv4Nan));
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) tmem_dealloc(tmem, 256);   // (before the other blocks are waited for: they may wait for tensor memory)
+  cluster.sync();
+  constexpr int PER = HD / 4, SIDE = 32 / PER, W = kKv4TileThreads / 32;   // lanes of a row, rows side by side in a warp
+  const int part_lane = lane % PER, parts = TWIN ? 2 * C : C;
+  for (int base = (rank * W + warp) * SIDE; base < rows; base += C * W * SIDE) {
+    const int row = min(base + lane / PER, rows - 1);
+    // a part: a block's, or one of the two of a block
+    auto part = [&](int x) { return cluster.map_shared_rank(joined, TWIN ? x >> 1 : x) + (row + (TWIN ? (x & 1) * 64 : 0)) * LDO; };
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (part_lane < parts) ml = *reinterpret_cast<const float2*>(part(part_lane) + HD);
+    float top = ml.x;
+#pragma unroll
+    for (int w = PER / 2; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    float f = top == -INFINITY ? 1.f : exp2f(ml.x - top), total = part_lane < parts ? ml.y * f : 0.f;   // (of this lane's part; no score, or NaN only: zeros and NaN add up)
+#pragma unroll
+    for (int w = PER / 2; w > 0; w >>= 1) total += __shfl_xor_sync(0xffffffffu, total, w);
+    f *= total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;   // (a row that sees no key is zero, NaN stays)
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = 0; c < parts; ++c) {
+      const float4 x = *reinterpret_cast<const float4*>(part(c) + part_lane * 4);
+      const float w = __shfl_sync(0xffffffffu, f, (lane & ~(PER - 1)) + c);
+      acc.x += x.x * w; acc.y += x.y * w; acc.z += x.z * w; acc.w += x.w * w;
+    }
+    if (base + lane / PER < rows)
+      *reinterpret_cast<uint2*>(p.out + ((size_t)(b * p.Q + tok0 + row / G) * p.heads + kvh * G + row % G) * HD + part_lane * 4) =
+          make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+  }
+  cluster.sync();   // no block leaves while its part is read
+}
+
+}  // namespace ssdk

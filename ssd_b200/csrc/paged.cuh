@@ -1,4 +1,4 @@
-// paged.cuh — what kernels over a paged cache share: pages of a table, lengths, bf16 pairs.
+// paged.cuh — what kernels over a paged cache share: pages of a table, lengths, pairs of values, bounded waits.
 #pragma once
 #include "common.cuh"
 
@@ -27,6 +27,26 @@ SSDK_DEVINL uint32_t max_bf16x2(uint32_t a, uint32_t b) {
   asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
+SSDK_DEVINL uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// A bounded wait (about two seconds; then the word is set and false comes back): the clock is read only where the first look fails.
+SSDK_DEVINL bool tile_wait(uint64_t* bar, uint32_t parity, unsigned* timeout) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity))
+    if (clock64() - t0 > 4000000000LL) {
+      if (timeout) *(volatile unsigned*)timeout = 1u;
+      return false;
+    }
+  return true;
+}
+SSDK_DEVINL bool tile_wait_warp(uint64_t* bar, uint32_t parity, unsigned* timeout) { return __all_sync(0xffffffffu, tile_wait(bar, parity, timeout)); }
 #endif
+
+constexpr int kNoPosition = 0x7fffff00;   // of a key that is not there: behind every context
 
 }  // namespace ssdk

@@ -21,25 +21,11 @@
 namespace ssdk {
 
 constexpr int kTileRows64 = 64, kTileKeys = 64, kTileThreads = 256;   // warps: loads of keys, scores, 4 of softmax, products with V, loads of values
-constexpr int kNoPosition = 0x7fffff00;   // of a key that is not there: behind every context
 constexpr int kTileMost = 16;   // blocks of a cluster
 constexpr int tile_stages(int HD) { return HD == 64 ? 4 : 2; }   // of keys and of values: as many as fit when two blocks share an SM
 // query twice | keys and values; behind them the places of the listed spans
 constexpr int span_tile_body(int HD) { return 2 * kTileRows64 * HD * 2 + tile_stages(HD) * 2 * kTileKeys * HD * 2; }
 constexpr int span_tile_smem(int HD, int count) { return span_tile_body(HD) + 1024 + count * 8; }
-
-// A bounded wait (about two seconds; then the word is set and false comes back): the clock is read only where the first look fails.
-SSDK_DEVINL bool tile_wait(uint64_t* bar, uint32_t parity, unsigned* timeout) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!mbar_try_wait(bar, parity))
-    if (clock64() - t0 > 4000000000LL) {
-      if (timeout) *(volatile unsigned*)timeout = 1u;
-      return false;
-    }
-  return true;
-}
-SSDK_DEVINL bool tile_wait_warp(uint64_t* bar, uint32_t parity, unsigned* timeout) { return __all_sync(0xffffffffu, tile_wait(bar, parity, timeout)); }
 
 template <int HD>
 __global__ void __launch_bounds__(kTileThreads, 2)
