@@ -22,7 +22,8 @@ namespace ssdk {
 // conversion.  (bf16 codes take 64 instructions for sixteen keys where these take 24; mma on e4m3 is made of conversions and f16 here: four times as slow.)  Which channels a product's k stands for is
 // free: a quad's lanes read a key's row, 16 bytes each, and the query's fragments follow.
 //   Values: P has no such range, it is bf16 and so are the codes: 16 + c has c in the top of bf16's mantissa; of two values' words one byte_perm makes words whose halves are the
-// two keys of a fragment's register.
+// two keys of a fragment's register.  A product of P s' with ones beside them sums what the 16 + 8 too many amount to, of the rounded weights, and is taken off every 512 keys, while the sums
+// that cancel are small (32 subtractions a piece less).
 // A cluster of blocks shares the keys of a key head of one sequence: chunks of 32 keys go round the blocks' warps, each with a ring of its own (cp.async, no barrier between
 // warps) and a softmax of its own; at the end warps meet, then blocks.
 // A page outside the cache is passed over, a row that sees no key is zero; a NaN row of keys or values makes NaN of the rows that see it and of no other.
@@ -45,28 +46,26 @@ constexpr int kv4_attn_smem(int HD, int NT) {
   return ring > join ? ring : join;
 }
 
-// nibbles P and P + 4 of a word as c - 8 in bf16: 16 + c less 24
+// nibbles P and P + 4 of a word as 16 + c in bf16
 template <int P>
-SSDK_DEVINL uint32_t kv4_pair(uint32_t w) {
-  const uint32_t x = P == 0 ? w << 3 : w >> (4 * P - 3), y = (x & 0x00780078u) | 0x41804180u;
-  uint32_t d;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(y), "r"(0x41c041c0u));
-  return d;
+SSDK_DEVINL uint32_t kv4_pair16(uint32_t w) {
+  const uint32_t x = P == 0 ? w << 3 : w >> (4 * P - 3);
+  return (x & 0x00780078u) | 0x41804180u;
 }
 SSDK_DEVINL uint32_t transpose_8x8(uint32_t x) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
   return d;
 }
-// 16 x 8 (+)= codes (bytes) x 32 bytes of a query, signed or not
+// 16 x 8 = c + codes (bytes) x 32 bytes of a query, signed or not
 template <bool SIGNED>
-SSDK_DEVINL void mma_u8_16832(uint32_t* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+SSDK_DEVINL void mma_u8_16832(uint32_t* d, const uint32_t* a, uint32_t b0, uint32_t b1, const uint32_t* c) {
   if (SIGNED)
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
   else
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
 }
 constexpr float kKv4Whole = 12582912.f;            // 1.5 2^23
 constexpr uint32_t kKv4WholeWord = 0x4b400000u;    // its word: a whole number below 2^22 added to it is added to the float
@@ -95,51 +94,73 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 2 : 1) kv4_attn_kern
   // ---- a warp's chunks of 32 keys: own, own + stride, ... ----
   const int tiles = (max(seen, 0) + 15) >> 4, chunks = (tiles + 1) >> 1, stride = C * kKv4Warps, own = rank * kKv4Warps + warp;
   const int n = own < chunks ? (chunks - own + stride - 1) / stride : 0;
-  const size_t record = (size_t)p.block_size * kv4_row_bytes(HD);
+  const int record = p.block_size * kv4_row_bytes(HD);   // bytes of a page and head
   uint8_t* ring = kv4_smem + warp * kKv4Stages * STAGE;
-  // pages of the sixteen keys that lane & 1 says, of chunk first + lane / 2 of this warp's: sixteen chunks at a time, the next sixteen's on their way
-  struct Where { int page, off; };
+  // Where a chunk lies is looked up by a lane: pages of whole chunks 32 chunks at a time, others sixteen, two lanes (of sixteen keys each) a chunk; the next ones' on their way.
+  const bool one_page = p.block_size % K == 0;
+  const int per = one_page ? 1 : 2, ahead = 32 / per;
+  const int64_t page_step = (int64_t)p.kv_heads * record;
+  struct Where { int64_t codes; int pairs; };   // bytes from the head's first code of the cache (-1: no page), and from there to the pairs
   auto look_up = [&](int first) {
     Where w = {-1, 0};
-    const long long tile = 2 * (own + (long long)(first + (lane >> 1)) * stride) + (lane & 1);
+    const long long chunk = own + (long long)(first + lane / per) * stride, tile = one_page ? 2 * chunk : 2 * chunk + (lane & 1);
     if (tile < tiles) {
-      const int pos = (int)tile * 16, x = pos / p.block_size;
-      w.off = pos - x * p.block_size;
-      w.page = page_at(p.tables + (size_t)b * p.max_blocks + x, p.num_blocks);
+      const int pos = (int)tile * 16, x = pos / p.block_size, off = pos - x * p.block_size;
+      const int page = page_at(p.tables + (size_t)b * p.max_blocks + x, p.num_blocks);
+      if (page >= 0) w.codes = page * page_step + off * CODES;
+      w.pairs = (p.block_size - off) * CODES + off * 4;
     }
     return w;
   };
   Where here = {-1, 0}, next = look_up(0);
+  const uint8_t *k_from = p.k_cache + (int64_t)kvh * record + lane * 16, *v_from = p.v_cache + (int64_t)kvh * record + lane * 16;
+  const uint8_t* pair_from = ((one_page ? lane & 8 : lane & 4) ? p.v_cache : p.k_cache) + (int64_t)kvh * record + (one_page ? lane & 7 : lane & 3) * 16;
+  const int v_to = K * CODES + kv4_v_place<HD>(lane / (CODES / 16), lane % (CODES / 16));
+  const int pair_to = 2 * K * CODES + (one_page ? lane * 16 : (lane >> 2) * K * 4 + (lane & 3) * 16);
   uint32_t missing = 0;   // two bits a stage: sixteen keys without a page
   auto load = [&](int i, int stage) {
     if (i >= n) return;
-    if ((i & 15) == 0) {
+    if ((i & (ahead - 1)) == 0) {
       here = next;
-      next = look_up(i + 16);
+      next = look_up(i + ahead);
     }
     uint8_t* to = ring + stage * STAGE;
     missing &= ~(3u << (2 * stage));
+    auto from_lane = [&](int src) {
+      Where w;
+      w.codes = (int64_t)((uint64_t)(uint32_t)__shfl_sync(0xffffffffu, (int)(here.codes >> 32), src) << 32 | (uint32_t)__shfl_sync(0xffffffffu, (int)here.codes, src));
+      w.pairs = __shfl_sync(0xffffffffu, here.pairs, src);
+      return w;
+    };
+    if (one_page) {
+      const Where w = from_lane(i & 31);
+      if (w.codes < 0) {
+        missing |= 3u << (2 * stage);
+        return;
+      }
+      const uint8_t *kc = k_from + w.codes, *vc = v_from + w.codes;
+#pragma unroll
+      for (int u = 0; u < K * CODES; u += 512) {   // (32 rows of a values' place are 512 bytes on, too)
+        cp_async16(to + u + lane * 16, kc + u, true);
+        cp_async16(to + u + v_to, vc + u, true);
+      }
+      if (lane < 16) cp_async16(to + pair_to, pair_from + w.codes + w.pairs, true);
+      return;
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int page = __shfl_sync(0xffffffffu, here.page, (2 * i + h) & 31), off = __shfl_sync(0xffffffffu, here.off, (2 * i + h) & 31);
-      if (page < 0) {
+      const Where w = from_lane((2 * i + h) & 31);
+      if (w.codes < 0) {
         missing |= 1u << (2 * stage + h);
         continue;
       }
-      const size_t base = ((size_t)page * p.kv_heads + kvh) * record;
-      const uint8_t *kc = p.k_cache + base + (size_t)off * CODES, *vc = p.v_cache + base + (size_t)off * CODES;
-      constexpr int PIECES = CODES;   // of 16 bytes, of sixteen keys' codes
+      const uint8_t *kc = k_from + w.codes, *vc = v_from + w.codes;
 #pragma unroll
-      for (int u = 0; u < PIECES; u += 32) {
-        const int x = u + lane;
-        cp_async16(to + h * 16 * CODES + x * 16, kc + x * 16, true);
-        cp_async16(to + K * CODES + h * 16 * CODES + kv4_v_place<HD>(x / (CODES / 16), x % (CODES / 16)), vc + x * 16, true);
+      for (int u = 0; u < 16 * CODES; u += 512) {
+        cp_async16(to + h * 16 * CODES + u + lane * 16, kc + u, true);
+        cp_async16(to + h * 16 * CODES + u + v_to, vc + u, true);
       }
-      // pairs: four pieces of keys' and four of values'
-      if (lane < 8) {
-        const uint8_t* from = (lane < 4 ? p.k_cache : p.v_cache) + base + (size_t)p.block_size * CODES + (size_t)off * 4 + (lane & 3) * 16;
-        cp_async16(to + 2 * K * CODES + (lane >> 2) * K * 4 + h * 64 + (lane & 3) * 16, from, true);
-      }
+      if (lane < 8) cp_async16(to + h * 64 + pair_to, pair_from + w.codes + w.pairs, true);
     }
   };
 #pragma unroll
@@ -197,9 +218,10 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 2 : 1) kv4_attn_kern
     }
   }
 
-  float o[NT][HD / 16][4], ref[NT][2], l[NT][2], low[NT][2];   // O^T, reference, sum, sum of P (m' + 8 s')
+  float o[NT][HD / 16][4], one[NT][4], ref[NT][2], l[NT][2], low[NT][2];   // O^T, sum of P s', reference, sum, sum of P (m' + 8 s')
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
+    one[nt][0] = one[nt][1] = one[nt][2] = one[nt][3] = 0.f;
 #pragma unroll
     for (int i = 0; i < HD / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
 #pragma unroll
@@ -210,6 +232,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 2 : 1) kv4_attn_kern
   }
 
   // scores of a chunk's keys g, g + 8, .. and rows 2 t, 2 t + 1 to weights, and their product with the values.  MASK: some row does not see some key, or a page is missing
+  const uint32_t start[4] = {kKv4WholeWord, kKv4WholeWord, kKv4WholeWord, kKv4WholeWord}, ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
   auto work = [&](const uint8_t* at, int x, int pos, uint32_t none, auto mask) {   // (x: which sixteen of the chunk)
     constexpr bool MASK = decltype(mask)::value;
     const uint32_t* pairs = reinterpret_cast<const uint32_t*>(at + 2 * K * CODES) + g;
@@ -230,16 +253,12 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 2 : 1) kv4_attn_kern
       }
       uint32_t whole[NT][2][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) whole[nt][0][i] = whole[nt][1][i] = kKv4WholeWord;
-#pragma unroll
       for (int j = 0; j < KW; ++j) {
         const uint32_t a[4] = {k[0][j] & 0x0f0f0f0fu, k[1][j] & 0x0f0f0f0fu, k[0][j] >> 4 & 0x0f0f0f0fu, k[1][j] >> 4 & 0x0f0f0f0fu};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma_u8_16832<true>(whole[nt][0], a, qb[nt][j][0][0], qb[nt][j][0][1]);
-          mma_u8_16832<false>(whole[nt][1], a, qb[nt][j][1][0], qb[nt][j][1][1]);
+          mma_u8_16832<true>(whole[nt][0], a, qb[nt][j][0][0], qb[nt][j][0][1], j ? whole[nt][0] : start);
+          mma_u8_16832<false>(whole[nt][1], a, qb[nt][j][1][0], qb[nt][j][1][1], j ? whole[nt][1] : start);
         }
       }
 #pragma unroll
@@ -283,6 +302,8 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 2 : 1) kv4_attn_kern
           ref[nt][e] = top;
           l[nt][e] *= f;
           low[nt][e] *= f;
+          one[nt][e] *= f;
+          one[nt][2 + e] *= f;
 #pragma unroll
           for (int i = 0; i < HD / 16; ++i) {
             o[nt][i][e] *= f;
@@ -329,16 +350,28 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 2 : 1) kv4_attn_kern
       for (int j = 0; j < VW; ++j) {
         const uint32_t a01 = __byte_perm(v[0][j], v[1][j], 0x5410), b01 = __byte_perm(v[0][j], v[1][j], 0x7632);
         const uint32_t a23 = __byte_perm(v[2][j], v[3][j], 0x5410), b23 = __byte_perm(v[2][j], v[3][j], 0x7632);
-        const uint32_t a[4][4] = {{kv4_pair<0>(a01), kv4_pair<0>(b01), kv4_pair<0>(a23), kv4_pair<0>(b23)}, {kv4_pair<1>(a01), kv4_pair<1>(b01), kv4_pair<1>(a23), kv4_pair<1>(b23)},
-                                  {kv4_pair<2>(a01), kv4_pair<2>(b01), kv4_pair<2>(a23), kv4_pair<2>(b23)}, {kv4_pair<3>(a01), kv4_pair<3>(b01), kv4_pair<3>(a23), kv4_pair<3>(b23)}};
+        const uint32_t a[4][4] = {{kv4_pair16<0>(a01), kv4_pair16<0>(b01), kv4_pair16<0>(a23), kv4_pair16<0>(b23)}, {kv4_pair16<1>(a01), kv4_pair16<1>(b01), kv4_pair16<1>(a23), kv4_pair16<1>(b23)},
+                                  {kv4_pair16<2>(a01), kv4_pair16<2>(b01), kv4_pair16<2>(a23), kv4_pair16<2>(b23)}, {kv4_pair16<3>(a01), kv4_pair16<3>(b01), kv4_pair16<3>(a23), kv4_pair16<3>(b23)}};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(o[nt][4 * j + i], a[i], pb[nt][0], pb[nt][1]);
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(one[nt], ones, pb[nt][0], pb[nt][1]);
     }
   };
 
+  auto take_off = [&]() {   // (the rows of `one` are alike)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][i][e] = fmaf(-24.f, one[nt][e], o[nt][i][e]);
+      one[nt][0] = one[nt][1] = one[nt][2] = one[nt][3] = 0.f;
+    }
+  };
   for (int i = 0, stage = 0; i < n; ++i, stage = stage + 1 == kKv4Stages ? 0 : stage + 1) {
     __syncwarp();   // every lane is done with the stage that is filled now
     load(i + kKv4Stages - 1, stage == 0 ? kKv4Stages - 1 : stage - 1);
@@ -354,7 +387,9 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 2 : 1) kv4_attn_kern
 #pragma unroll 1
       for (int x = 0; x < 2; ++x) work(ring + stage * STAGE, x, pos, none, std::true_type());
     }
+    if ((i & 15) == 15) take_off();
   }
+  take_off();
   cp_async_wait<0>();
   __syncthreads();   // the rings are read: their memory is the parts' now
 

@@ -20,11 +20,12 @@ constexpr int kv4_tile_smem(int HD) {
   return (body > join ? body : join) + 1024;
 }
 
-// nibbles P and P + 4 of a word as 16 + c in bf16
+// nibbles P and P + 4 of a word as c - 8 in bf16
 template <int P>
-SSDK_DEVINL uint32_t kv4_pair16(uint32_t w) {
-  const uint32_t x = P == 0 ? w << 3 : w >> (4 * P - 3);
-  return (x & 0x00780078u) | 0x41804180u;
+SSDK_DEVINL uint32_t kv4_pair(uint32_t w) {
+  uint32_t d;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(kv4_pair16<P>(w)), "r"(0x41c041c0u));
+  return d;
 }
 SSDK_DEVINL uint4 kv4_words16(uint32_t w) { return make_uint4(kv4_pair16<0>(w), kv4_pair16<1>(w), kv4_pair16<2>(w), kv4_pair16<3>(w)); }
 SSDK_DEVINL uint4 kv4_words(uint32_t w) { return make_uint4(kv4_pair<0>(w), kv4_pair<1>(w), kv4_pair<2>(w), kv4_pair<3>(w)); }
@@ -105,12 +106,21 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
 
   if (warp >= 4 && warp < 8) {
     // ---- codes: a thread has PER pieces of 32 channels (eight lanes are eight rows) of the keys and of the values, and the pair of one of either ----
-    constexpr int NP = HD / 32, PER = K * NP / kKv4Producers;
-    const int tid = threadIdx.x - 128, pw = tid >> 5, piece = (lane >> 3) % NP;
-    const size_t record = (size_t)p.block_size * kv4_row_bytes(HD);
+    constexpr int NP = HD / 32, PER = K * NP / kKv4Producers;   // (PER = 2: the second piece is 32 rows on)
+    const int tid = threadIdx.x - 128, pw = tid >> 5, piece = (lane >> 3) % NP, key = tid & 63;
+    const int row = (HD == 128 ? pw : 2 * pw + (lane >> 4)) * 8 + (lane & 7);
+    const int record = p.block_size * kv4_row_bytes(HD), pairs = p.block_size * CODES;   // (bytes of a page and head, of its codes)
+    const int64_t page_step = (int64_t)p.kv_heads * record;
+    const uint8_t *k_from = p.k_cache + (int64_t)kvh * record + piece * 16, *v_from = p.v_cache + (int64_t)kvh * record + piece * 16;
+    const uint8_t* pair_from = (tid < 64 ? p.k_cache : p.v_cache) + (int64_t)kvh * record + pairs;
+    const int32_t* table = p.tables + (size_t)b * p.max_blocks;
     const int step = C * K, step_x = step / p.block_size, step_off = step - step_x * p.block_size;
-    // where sixteen keys of this block's next chunk to be looked up are: entry of the table, offset in the page
-    struct Place { int x, off, page, at, pos; };
+    uint4 kc[PER], vc[PER];
+    uint32_t pair = 0;
+    int pos = 0;
+    // A page of whole chunks is looked up once a chunk by each warp, others by sixteens of keys.  What a page is, is looked at where it is used, a chunk later.
+    const bool one_page = p.block_size % K == 0;
+    struct Place { int x, off, pos, page, at; };   // the next chunk's entry of the table, offset in its page and position, and the page and offset that were looked up
     auto first = [&](int sixteen) {
       Place w;
       w.pos = rank * K + sixteen * 16;
@@ -120,9 +130,8 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
       w.at = 0;
       return w;
     };
-    auto look_up = [&](Place& w) {   // (positions stay below 2^31: the host sees to it; what a page is, is looked at where it is used, a chunk later)
-      w.page = -1;
-      if (w.pos < seen) w.page = p.tables[(size_t)b * p.max_blocks + w.x];
+    auto look_up = [&](Place& w) {   // (positions stay below 2^31: the host sees to it)
+      w.page = w.pos < seen ? table[w.x] : -1;
       w.at = w.off;
       w.pos += step;
       w.x += step_x;
@@ -132,36 +141,52 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
         ++w.x;
       }
     };
-    int row[PER];
-    Place of[PER], mine = first((tid & 63) >> 4);
-#pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      row[u] = (HD == 128 ? u * 4 + pw : 2 * pw + (lane >> 4)) * 8 + (lane & 7);
-      of[u] = first(row[u] >> 4);
-      look_up(of[u]);
-    }
+    Place mine = first(one_page ? 0 : key >> 4), of[PER];
     look_up(mine);
-    uint4 kc[PER], vc[PER];
-    uint32_t pair = 0;
-    int pos = 0;
-    auto load = [&]() {   // of the chunk that was looked up; then the next one's pages
+    if (!one_page) {
 #pragma unroll
       for (int u = 0; u < PER; ++u) {
-        kc[u] = vc[u] = make_uint4(0, 0, 0, 0);
-        if (of[u].page >= 0 && of[u].page < p.num_blocks) {
-          const size_t at = ((size_t)of[u].page * p.kv_heads + kvh) * record + (size_t)(of[u].at + (row[u] & 15)) * CODES + piece * 16;
-          kc[u] = ld_nc_v4(p.k_cache + at);
-          vc[u] = ld_nc_v4(p.v_cache + at);
-        }
+        of[u] = first((row + 32 * u) >> 4);
         look_up(of[u]);
       }
+    }
+    auto there = [&](int page) { return page >= 0 && page < p.num_blocks; };
+    auto load = [&]() {   // of the chunk that was looked up; then the next one's pages
       pair = 0;
-      const bool there = mine.page >= 0 && mine.page < p.num_blocks;
-      pos = there ? mine.pos - step : kNoPosition;
-      if (there && pos + (tid & 15) < len)   // (behind the context it may be anything)
-        pair = *reinterpret_cast<const uint32_t*>((tid < 64 ? p.k_cache : p.v_cache) + ((size_t)mine.page * p.kv_heads + kvh) * record + (size_t)p.block_size * CODES + (size_t)(mine.at + (tid & 15)) * 4);
+      if (one_page) {
+        const bool is = there(mine.page);
+        const int64_t at = mine.page * page_step + (mine.at + row) * CODES;
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+          kc[u] = vc[u] = make_uint4(0, 0, 0, 0);
+          if (is) {
+            kc[u] = ld_nc_v4(k_from + at + u * 32 * CODES);
+            vc[u] = ld_nc_v4(v_from + at + u * 32 * CODES);
+          }
+        }
+        pos = is ? mine.pos - step + (key & 48) : kNoPosition;
+        if (is && pos + (key & 15) < len) pair = *reinterpret_cast<const uint32_t*>(pair_from + mine.page * page_step + (mine.at + key) * 4);   // (behind the context it may be anything)
+      } else {
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+          kc[u] = vc[u] = make_uint4(0, 0, 0, 0);
+          if (there(of[u].page)) {
+            const int64_t at = of[u].page * page_step + (of[u].at + (row & 15)) * CODES;
+            kc[u] = ld_nc_v4(k_from + at);
+            vc[u] = ld_nc_v4(v_from + at);
+          }
+          look_up(of[u]);
+        }
+        const bool is = there(mine.page);
+        pos = is ? mine.pos - step : kNoPosition;
+        if (is && pos + (key & 15) < len) pair = *reinterpret_cast<const uint32_t*>(pair_from + mine.page * page_step + (mine.at + (key & 15)) * 4);
+      }
       look_up(mine);
     };
+    // where a piece's four words (16 bytes of bf16 each) go in a stage
+    uint8_t* to[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) to[j] = sK + (piece >> 1) * kKHalf + swizzled(row, (piece & 1) * 4 + j);
     if (n > 0) load();
     for (int i = 0; i < n; ++i) {
       uint4 k_now[PER], v_now[PER];
@@ -174,29 +199,26 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
       const int pos_now = pos, s = i & 1;
       if (i + 1 < n) load();
       if (i >= 2 && !tile_wait_warp(&s_full[s], parity(i - 2), pp.timeout)) break;   // the scores of chunk i - 2 have read their keys
-      uint8_t* dst = sK + s * kTile;
 #pragma unroll
       for (int u = 0; u < PER; ++u) {
         const uint32_t w[4] = {k_now[u].x, k_now[u].y, k_now[u].z, k_now[u].w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + (piece >> 1) * kKHalf + swizzled(row[u], (piece & 1) * 4 + j)) = kv4_words16(w[j]);
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(to[j] + s * kTile + u * 32 * 128) = kv4_words16(w[j]);
       }
       fence_proxy_async_smem();
       mbar_arrive(&k_full[s]);
       if (i >= 2 && !tile_wait_warp(&pv_done[s], parity(i - 2), pp.timeout)) break;   // its product has read its values, its rows their pairs
-      dst = sV + s * kTile;
 #pragma unroll
       for (int u = 0; u < PER; ++u) {
         const uint32_t w[4] = {v_now[u].x, v_now[u].y, v_now[u].z, v_now[u].w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + (piece >> 1) * kKHalf + swizzled(row[u], (piece & 1) * 4 + j)) = kv4_words(w[j]);
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(to[j] + 2 * kTile + s * kTile + u * 32 * 128) = kv4_words(w[j]);
       }
       {
-        const int key = tid & 63;
         const float scale = __uint_as_float(pair_now << 16), minimum = __uint_as_float(pair_now & 0xffff0000u);
-        float* to = (tid < 64 ? key_pairs[s] : value_pairs[s]) + (key >> 1) * 4 + (key & 1);
-        to[0] = tid < 64 ? scale * p.scale_log2 : scale;
-        to[2] = tid < 64 ? fmaf(-16.f, scale, minimum) * p.scale_log2 : fmaf(8.f, scale, minimum);
+        float* dst = (tid < 64 ? key_pairs[s] : value_pairs[s]) + (key >> 1) * 4 + (key & 1);
+        dst[0] = tid < 64 ? scale * p.scale_log2 : scale;
+        dst[2] = tid < 64 ? fmaf(-16.f, scale, minimum) * p.scale_log2 : fmaf(8.f, scale, minimum);
         if (tid < 64 && (key & 15) == 0) at_pos[s][key >> 4] = pos_now;
       }
       fence_proxy_async_smem();
