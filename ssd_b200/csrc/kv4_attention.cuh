@@ -39,10 +39,10 @@ struct Kv4AttnParams {
   float scale_log2;              // scale * log2(e)
 };
 constexpr float kKv4Slack = 8.f;
-constexpr int kKv4Warps = 8, kKv4Most = 16, kKv4Stages = 3, kKv4Keys = 32;   // warps of a block, blocks of a cluster, a warp's ring, keys of a chunk
+constexpr int kKv4Most = 16, kKv4Stages = 3, kKv4Keys = 32;   // blocks of a cluster, a warp's ring, keys of a chunk
 constexpr int kv4_stage_bytes(int HD) { return 2 * kKv4Keys * (HD / 2 + 4); }   // keys' codes | values' codes | keys' pairs | values' pairs
-constexpr int kv4_attn_smem(int HD, int NT) {
-  const int ring = kKv4Warps * kKv4Stages * kv4_stage_bytes(HD), join = (kKv4Warps + 1) * 8 * NT * (HD + 8) * 4;
+constexpr int kv4_attn_smem(int HD, int NT, int W) {
+  const int ring = W * kKv4Stages * kv4_stage_bytes(HD), join = (W + 1) * 8 * NT * (HD + 8) * 4;
   return ring > join ? ring : join;
 }
 
@@ -76,8 +76,9 @@ SSDK_DEVINL int kv4_v_place(int r, int c) {
   return (r >> 3) * 256 + ((r & 1) << 7) + ((r >> 1 & 3) << 5) + (c << 4);
 }
 
-template <int HD, int NT>
-__global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 2 : 1) kv4_attn_kernel(const __grid_constant__ Kv4AttnParams p) {
+// NT tiles of eight rows, W warps; sixteen (eight with two tiles) warps are resident on an SM
+template <int HD, int NT, int W>
+__global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __grid_constant__ Kv4AttnParams p) {
   constexpr int KW = HD / 32, VW = HD / 64, CODES = HD / 2, K = kKv4Keys, STAGE = kv4_stage_bytes(HD);
   extern __shared__ __align__(16) uint8_t kv4_smem[];
   pdl_wait();
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 2 : 1) kv4_attn_kern
   const int seen = min(len, ctx + (r0 + R - 1) / G + 1), seen_by_all = ctx + r0 / G + 1;   // positions that some row sees, that all do
 
   // ---- a warp's chunks of 32 keys: own, own + stride, ... ----
-  const int tiles = (max(seen, 0) + 15) >> 4, chunks = (tiles + 1) >> 1, stride = C * kKv4Warps, own = rank * kKv4Warps + warp;
+  const int tiles = (max(seen, 0) + 15) >> 4, chunks = (tiles + 1) >> 1, stride = C * W, own = rank * W + warp;
   const int n = own < chunks ? (chunks - own + stride - 1) / stride : 0;
   const int record = p.block_size * kv4_row_bytes(HD);   // bytes of a page and head
   uint8_t* ring = kv4_smem + warp * kKv4Stages * STAGE;
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 2 : 1) kv4_attn_kern
     const int pos = (own + i * stride) * K;
     const uint32_t none = missing >> (2 * stage) & 3u;
     if (pos + K <= seen_by_all && !none) {
-#pragma unroll 1
+#pragma unroll
       for (int x = 0; x < 2; ++x) work(ring + stage * STAGE, x, pos, 0u, std::false_type());
     } else {
 #pragma unroll 1
@@ -396,7 +397,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 2 : 1) kv4_attn_kern
   // ---- the warps' parts meet: [warp][row][HD + 8] O | reference, sum ----
   constexpr int LDO = HD + 8, ROWS = 8 * NT;
   float* parts = reinterpret_cast<float*>(kv4_smem);
-  float* joined = parts + kKv4Warps * ROWS * LDO;   // [row][HD + 8]
+  float* joined = parts + W * ROWS * LDO;   // [row][HD + 8]
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -422,14 +423,14 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 2 : 1) kv4_attn_kern
     __nv_bfloat16* dst = p.out + ((size_t)(b * p.Q + (r0 + r) / G) * p.heads + kvh * G + (r0 + r) % G) * HD + d;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
   };
-  for (int idx = threadIdx.x; idx < R * (HD / 4); idx += kKv4Warps * 32) {
+  for (int idx = threadIdx.x; idx < R * (HD / 4); idx += W * 32) {
     const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
     float top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kKv4Warps; ++w) top = fmaxf(top, parts[(w * ROWS + r) * LDO + HD]);
+    for (int w = 0; w < W; ++w) top = fmaxf(top, parts[(w * ROWS + r) * LDO + HD]);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kKv4Warps; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float* row = parts + (w * ROWS + r) * LDO;
       const float2 ml = *reinterpret_cast<const float2*>(row + HD);
       const float4 v = *reinterpret_cast<const float4*>(row + d);
@@ -447,7 +448,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, NT == 1 ? 2 : 1) kv4_attn_kern
   if (C == 1) return;
   // the blocks' parts meet over the cluster's shared memory, each block joins a share of the columns
   cluster.sync();
-  for (int idx = rank * kKv4Warps * 32 + threadIdx.x; idx < R * (HD / 4); idx += C * kKv4Warps * 32) {
+  for (int idx = rank * W * 32 + threadIdx.x; idx < R * (HD / 4); idx += C * W * 32) {
     const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
     float top = -INFINITY, sum = 0.f;
 #pragma unroll 4

@@ -55,14 +55,20 @@ static int kv4_cluster(int64_t units, int64_t keys, int resident, int most) {
   }
   return best;
 }
+template <int HD, int NT, int W>
+static int launch_warps(Launcher& L, const Kv4AttnParams& p, int64_t units) {
+  static std::atomic<bool> done[64];
+  CKI(with_smem(kv4_attn_kernel<HD, NT, W>, kv4_attn_smem(HD, NT, W), kSmemClusters, done));
+  const int64_t tiles = units / ((int64_t)p.B * p.kv_heads);
+  if (tiles > 65535) return fail("paged_attn_kv4: q_len=%d", p.Q);
+  L.cluster = kv4_cluster(units, (int64_t)p.max_blocks * p.block_size, 16 / NT / W, kKv4Most);
+  return L.go(kv4_attn_kernel<HD, NT, W>, dim3(p.kv_heads * L.cluster, p.B, (unsigned)tiles), dim3(W * 32), kv4_attn_smem(HD, NT, W), p);
+}
 template <int HD, int NT>
 static int launch_attn(Launcher& L, const Kv4AttnParams& p) {
-  static std::atomic<bool> done[64];
-  CKI(with_smem(kv4_attn_kernel<HD, NT>, kv4_attn_smem(HD, NT), kSmemOnly | 2, done));
-  const int64_t rows = (int64_t)(p.heads / p.kv_heads) * p.Q, tiles = (rows + 8 * NT - 1) / (8 * NT);
-  if (tiles > 65535) return fail("paged_attn_kv4: q_len=%d", p.Q);
-  L.cluster = kv4_cluster((int64_t)p.B * p.kv_heads * tiles, (int64_t)p.max_blocks * p.block_size, NT == 1 ? 2 : 1, kKv4Most);
-  return L.go(kv4_attn_kernel<HD, NT>, dim3(p.kv_heads * L.cluster, p.B, (unsigned)tiles), dim3(kKv4Warps * 32), kv4_attn_smem(HD, NT), p);
+  const int64_t rows = (int64_t)(p.heads / p.kv_heads) * p.Q, units = (rows + 8 * NT - 1) / (8 * NT) * p.B * p.kv_heads;
+  if (units * kKv4Most <= kSms) return launch_warps<HD, NT, 16 / NT>(L, p, units);   // a block to an SM at most
+  return launch_warps<HD, NT, 4>(L, p, units);
 }
 template <int HD, bool TWIN>
 static int launch_tiles(Launcher& L, const Kv4AttnParams& a) {

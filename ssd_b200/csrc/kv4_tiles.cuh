@@ -225,36 +225,42 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
       mbar_arrive(&v_full[s]);
     }
   } else if (warp == 8) {
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = make_umma_idesc_bf16(kKv4TileRows, K);
-      constexpr uint32_t idesc_o = make_umma_idesc_bf16(kKv4TileRows, HD) | (1u << 16);   // V: b_major = MN
-      auto scores = [&](int i) {
-        if (!tile_wait(&k_full[i & 1], parity(i), pp.timeout)) return false;
-        tc_fence_after();
+    // (the whole warp goes through the waits, and one lane issues: what a product takes stays uniform)
+    constexpr uint32_t idesc_s = make_umma_idesc_bf16(kKv4TileRows, K);
+    constexpr uint32_t idesc_o = make_umma_idesc_bf16(kKv4TileRows, HD) | (1u << 16);   // V: b_major = MN
+    const uint64_t q_desc = make_umma_desc_k128(sQ), k_desc = make_umma_desc_k128(sK), v_desc = make_umma_desc_mn128(sV, kKHalf);
+    auto scores = [&](int i) {
+      if (!tile_wait_warp(&k_full[i & 1], parity(i), pp.timeout)) return false;
+      tc_fence_after();
+      const uint64_t kd = k_desc + (uint64_t)((i & 1) * (kTile >> 4));
+      const uint32_t to = tmem + (uint32_t)(i & 1) * 64u;
+      if (elect_one()) {
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) {
-          const uint64_t qd = make_umma_desc_k128(sQ + h * kQHalf), kd = make_umma_desc_k128(sK + (i & 1) * kTile + h * kKHalf);
+        for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16_ss(tmem + (i & 1) * 64, qd + 2 * k, kd + 2 * k, idesc_s, (uint32_t)((h | k) != 0));
-        }
+          for (int k = 0; k < 4; ++k) umma_bf16_ss(to, q_desc + (h * kQHalf >> 4) + 2 * k, kd + (h * kKHalf >> 4) + 2 * k, idesc_s, (uint32_t)((h | k) != 0));
         umma_commit(&s_full[i & 1]);
-        return true;
-      };
-      bool go = n > 0 && scores(0);
-      for (int i = 0; i < n && go; ++i) {
-        // the scores of chunk i + 1 go over the P that the product of chunk i - 1 reads
-        if (i > 0 && !(go = tile_wait(&pv_done[(i - 1) & 1], parity(i - 1), pp.timeout))) break;
-        if (i + 1 < n && !(go = scores(i + 1))) break;
-        if (!(go = tile_wait(&v_full[i & 1], parity(i), pp.timeout) && tile_wait(&p_full[i & 1], parity(i), pp.timeout))) break;
-        tc_fence_after();
-        const uint64_t vd = make_umma_desc_mn128(sV + (i & 1) * kTile, kKHalf);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool go = n > 0 && scores(0);
+    for (int i = 0; i < n && go; ++i) {
+      // the scores of chunk i + 1 go over the P that the product of chunk i - 1 reads
+      if (i > 0 && !(go = tile_wait_warp(&pv_done[(i - 1) & 1], parity(i - 1), pp.timeout))) break;
+      if (i + 1 < n && !(go = scores(i + 1))) break;
+      if (!(go = tile_wait_warp(&v_full[i & 1], parity(i), pp.timeout) && tile_wait_warp(&p_full[i & 1], parity(i), pp.timeout))) break;
+      tc_fence_after();
+      const uint64_t vd = v_desc + (uint64_t)((i & 1) * (kTile >> 4));
+      const uint32_t from = tmem + (uint32_t)(i & 1) * 64u;
+      if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < K / 16; ++k)   // 16 keys: 2048 B of V, 8 columns of P
-          umma_bf16_ts(tmem_o, tmem + (i & 1) * 64 + 8 * k, vd + 128 * k, idesc_o, (uint32_t)((i | k) != 0));
+          umma_bf16_ts(tmem_o, from + 8 * k, vd + 128 * k, idesc_o, (uint32_t)((i | k) != 0));
         umma_commit(&pv_done[i & 1]);
       }
+      __syncwarp();
     }
-    __syncwarp();
   } else if (warp < 4 && (TWIN ? (warp & 1) * 32 : warp * 32) < half) {
     const int at = warp * 32 + lane, r = TWIN ? at & 63 : at;
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
