@@ -1,20 +1,25 @@
 // kv4_tiles.cuh — attention over a paged cache held in 4 bits (kv4.cuh) of more than sixteen query rows to a key head, on tcgen05.
 //
 // S = Q C^T of up to 128 rows (query tokens x the heads that share a key head) and 64 keys' codes into TMEM, P = exp2(S s + m sum(q) - reference) one row per thread, O += (P s') (C' - 8) with
-// P s' out of TMEM; what the minima give is a sum of its own (kv4_attn_kernel has the formulas).  Codes become bf16 on their way into shared memory: 16 + c for keys, c - 8 for values, both exact,
-// by a shift and a mask for two.  A word of eight channels gives them in the order 0, 4, 1, 5, 2, 6, 3, 7: the queries are stored in that order too, and the outputs put back.
+// P s' out of TMEM; what the minima give is a sum of its own (kv4_attn_kernel has the formulas).
+// Scores are products in e4m3: a byte that holds a code c in 0 .. 15 is the number c 2^-9, so codes become bytes with a mask (and a shift) for four.  A query row, scaled by a power of two so that its largest
+// lies in 2^7 .. 2^8, is the sum of two e4m3 numbers, exactly where it is above 2^-10 of the largest, else off by at most 2^-17 of that; both meet the same codes.  The sums are fp32.
+// Values stay bf16, c - 8, as P has no such range.  A word of eight channels gives them in the order 0, 4, 1, 5, 2, 6, 3, 7 (outputs are put back), and keys' codes as 0, 2, 4, 6, 1, 3, 5, 7 (queries are
+// stored in that order).
 // Four warps bring codes in (registers, a chunk ahead of the one that they write, its pages two ahead), one issues the products, four have the rows.  Scales and minima of a chunk's keys lie beside its
 // values, as pairs of keys, so that a row takes two at a time.  A cluster of blocks shares the chunks of a key head; their sums meet in shared memory.
 // A row takes 32 keys at a time (64 scores and as many scales pass the registers of nine warps twice on an SM).  TWIN: up to 64 rows lie in the tile twice, rows 0 .. 63 take a chunk's first 32 keys and
 // 64 .. 127 the others, each with zeros for weights of the other half and a reference of its own: all four warps work on half of the scores where two would on all, and the products are no more.
 #pragma once
+#include <cuda_fp8.h>
+
 #include "kv4_attention.cuh"
 #include "prompt_attention.cuh"
 
 namespace ssdk {
 
 constexpr int kKv4TileRows = 128, kKv4TileKeys = 64, kKv4TileThreads = 288, kKv4Producers = 128;   // warps: 4 of rows, 4 of codes, one of products
-constexpr int kv4_tile_body(int HD) { return kKv4TileRows * HD * 2 + 2 * 2 * kKv4TileKeys * HD * 2; }   // queries | two stages of keys | of values
+constexpr int kv4_tile_body(int HD) { return kKv4TileRows * HD * 2 + 2 * kKv4TileKeys * 128 + 2 * kKv4TileKeys * HD * 2; }   // queries | two stages of keys | of values
 constexpr int kv4_tile_smem(int HD) {
   const int join = kKv4TileRows * (HD + 4) * 4, body = kv4_tile_body(HD);
   return (body > join ? body : join) + 1024;
@@ -27,7 +32,29 @@ SSDK_DEVINL uint32_t kv4_pair(uint32_t w) {
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(kv4_pair16<P>(w)), "r"(0x41c041c0u));
   return d;
 }
-SSDK_DEVINL uint4 kv4_words16(uint32_t w) { return make_uint4(kv4_pair16<0>(w), kv4_pair16<1>(w), kv4_pair16<2>(w), kv4_pair16<3>(w)); }
+// four values as e4m3, and what that leaves of them as e4m3
+SSDK_DEVINL void e4m3_twice(const float (&x)[4], uint32_t* high, uint32_t* low) {
+  *high = *low = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const __nv_fp8x2_storage_t h = __nv_cvt_float2_to_fp8x2(make_float2(x[i], x[i + 1]), __NV_SATFINITE, __NV_E4M3);
+    const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(h, __NV_E4M3)));
+    const __nv_fp8x2_storage_t l = __nv_cvt_float2_to_fp8x2(make_float2(x[i] - f.x, x[i + 1] - f.y), __NV_SATFINITE, __NV_E4M3);
+    *high |= (uint32_t)h << (8 * i);
+    *low |= (uint32_t)l << (8 * i);
+  }
+}
+// D[tmem] (+)= A[smem desc] * B[smem desc], e4m3 x e4m3 -> fp32, 32 bytes of k
+SSDK_DEVINL void umma_e4m3_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// its descriptor: A = B = e4m3 (K-major), D = fp32
+constexpr uint32_t make_umma_idesc_e4m3(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
 SSDK_DEVINL uint4 kv4_words(uint32_t w) { return make_uint4(kv4_pair<0>(w), kv4_pair<1>(w), kv4_pair<2>(w), kv4_pair<3>(w)); }
 // 16-byte piece c of a row of 128 bytes under the 128-byte swizzle
 SSDK_DEVINL int swizzled(int row, int c) { return row * 128 + ((c ^ (row & 7)) << 4); }
@@ -42,17 +69,18 @@ template <int HD, bool TWIN>
 __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __grid_constant__ Kv4TileParams pp) {
   namespace cg = cooperative_groups;
   constexpr int HALVES = HD / 64, CODES = HD / 2, K = kKv4TileKeys;
-  constexpr int kQHalf = kKv4TileRows * 128, kKHalf = K * 128, kTile = HALVES * kKHalf;
+  constexpr int kQHalf = kKv4TileRows * 128, kKTile = K * 128, kVHalf = K * 128, kVTile = HALVES * kVHalf;
   const Kv4AttnParams& p = pp.a;
   extern __shared__ uint8_t kv4_tile_raw[];
   __shared__ __align__(8) uint64_t k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2];
   __shared__ __align__(16) float key_pairs[2][K * 2], value_pairs[2][K * 2];   // of two keys: scale, scale, what goes with the sum, the same (times scale * log2(e) for keys)
   __shared__ __align__(16) int at_pos[2][4];   // position of a chunk's sixteen keys, behind every context where they have no page
+  __shared__ float2 row_units[kKv4TileRows];   // of a row of queries: what a unit of its products is (NaN: it is not finite), and its sum in them
   __shared__ uint32_t tmem_slot;
   uint8_t* smem = kv4_tile_raw + ((1024u - (smem_u32(kv4_tile_raw) & 1023u)) & 1023u);
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + HALVES * kQHalf;
-  uint8_t* sV = sK + 2 * kTile;
+  uint8_t* sV = sK + 2 * kKTile;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -77,13 +105,35 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     tmem_relinquish();
   }
   pdl_wait();
-  // queries, eight channels in the order of a word's pairs; rows behind the last one are zero
-  for (int i = threadIdx.x; i < kKv4TileRows * (HD / 8); i += kKv4TileThreads) {
-    const int at = i / (HD / 8), c = i % (HD / 8), r = TWIN ? at & 63 : at;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (r < rows) x = *reinterpret_cast<const uint4*>(p.q + ((size_t)(b * p.Q + tok0 + r / G) * p.heads + kvh * G + r % G) * HD + c * 8);
-    *reinterpret_cast<uint4*>(sQ + (c >> 3) * kQHalf + swizzled(at, c & 7)) =
-        make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+  // Queries: HD / 8 lanes a row, eight channels each.  Heads of 128: high and low parts in halves of their own, heads of 64: in a row's 128 bytes behind one another (the keys' codes stand there twice).
+  // Rows behind the last one are zero.
+  constexpr int LPR = HD / 8;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < kKv4TileRows * LPR; i += kKv4TileThreads) {   // (a warp's lanes stay together: both numbers are multiples of 32)
+    const int at = i / LPR, c = i % LPR, r = TWIN ? at & 63 : at;
+    float f[8], sum = 0.f, top = 0.f;
+    unpack_bf16x8(r < rows ? *reinterpret_cast<const uint4*>(p.q + ((size_t)(b * p.Q + tok0 + r / G) * p.heads + kvh * G + r % G) * HD + c * 8) : make_uint4(0, 0, 0, 0), f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      sum += f[j];
+      top = fmaxf(top, fabsf(f[j]));
+    }
+#pragma unroll
+    for (int w = 1; w < LPR; w *= 2) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, w);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    }
+    const int e = max((int)(__float_as_uint(top) >> 23), 9);   // (biased exponent; a unit is 2^9 2^(e - 134), of which the keys' scales have 2^2)
+    const float up = __uint_as_float((uint32_t)(261 - e) << 23), unit = __uint_as_float((uint32_t)min(e, 254) << 23);   // 2^(7 - (e - 127)), 2^(e - 127)
+    const float even[4] = {f[0] * up, f[2] * up, f[4] * up, f[6] * up}, odd[4] = {f[1] * up, f[3] * up, f[5] * up, f[7] * up};
+    uint2 high, low;
+    e4m3_twice(even, &high.x, &low.x);
+    e4m3_twice(odd, &high.y, &low.y);
+    uint8_t* to = sQ + swizzled(at, c >> 1) + (c & 1) * 8;
+    *reinterpret_cast<uint2*>(to) = high;
+    if (HD == 128) *reinterpret_cast<uint2*>(to + kQHalf) = low;
+    else *reinterpret_cast<uint2*>(sQ + swizzled(at, 4 + (c >> 1)) + (c & 1) * 8) = low;
+    if (c == 0) row_units[at] = fabsf(sum) < INFINITY && e < 255 ? make_float2(unit, sum / unit) : make_float2(__uint_as_float(kKv4Nan), 0.f);
   }
   fence_proxy_async_smem();
   tc_fence_before();
@@ -115,7 +165,9 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     const uint8_t* pair_from = (tid < 64 ? p.k_cache : p.v_cache) + (int64_t)kvh * record + pairs;
     const int32_t* table = p.tables + (size_t)b * p.max_blocks;
     const int step = C * K, step_x = step / p.block_size, step_off = step - step_x * p.block_size;
-    uint4 kc[PER], vc[PER];
+    uint4 kc[PER], vc[PER];   // (without a page they stay what they were: no row sees what comes of it)
+#pragma unroll
+    for (int u = 0; u < PER; ++u) kc[u] = vc[u] = make_uint4(0, 0, 0, 0);
     uint32_t pair = 0;
     int pos = 0;
     // A page of whole chunks is looked up once a chunk by each warp, others by sixteens of keys.  What a page is, is looked at where it is used, a chunk later.
@@ -158,7 +210,6 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
         const int64_t at = mine.page * page_step + (mine.at + row) * CODES;
 #pragma unroll
         for (int u = 0; u < PER; ++u) {
-          kc[u] = vc[u] = make_uint4(0, 0, 0, 0);
           if (is) {
             kc[u] = ld_nc_v4(k_from + at + u * 32 * CODES);
             vc[u] = ld_nc_v4(v_from + at + u * 32 * CODES);
@@ -169,7 +220,6 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
       } else {
 #pragma unroll
         for (int u = 0; u < PER; ++u) {
-          kc[u] = vc[u] = make_uint4(0, 0, 0, 0);
           if (there(of[u].page)) {
             const int64_t at = of[u].page * page_step + (of[u].at + (row & 15)) * CODES;
             kc[u] = ld_nc_v4(k_from + at);
@@ -183,10 +233,12 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
       }
       look_up(mine);
     };
-    // where a piece's four words (16 bytes of bf16 each) go in a stage
-    uint8_t* to[4];
+    // where a piece's 32 bytes of a key go in a stage, and its four words (16 bytes of bf16 each) of a value
+    uint8_t *k_to[2], *v_to[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) to[j] = sK + (piece >> 1) * kKHalf + swizzled(row, (piece & 1) * 4 + j);
+    for (int j = 0; j < 2; ++j) k_to[j] = sK + swizzled(row, piece * 2 + j);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v_to[j] = sV + (piece >> 1) * kVHalf + swizzled(row, (piece & 1) * 4 + j);
     if (n > 0) load();
     for (int i = 0; i < n; ++i) {
       uint4 k_now[PER], v_now[PER];
@@ -203,7 +255,11 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
       for (int u = 0; u < PER; ++u) {
         const uint32_t w[4] = {k_now[u].x, k_now[u].y, k_now[u].z, k_now[u].w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(to[j] + s * kTile + u * 32 * 128) = kv4_words16(w[j]);
+        for (int j = 0; j < 2; ++j) {
+          const uint4 x = make_uint4(w[2 * j] & 0x0f0f0f0fu, w[2 * j] >> 4 & 0x0f0f0f0fu, w[2 * j + 1] & 0x0f0f0f0fu, w[2 * j + 1] >> 4 & 0x0f0f0f0fu);
+          *reinterpret_cast<uint4*>(k_to[j] + s * kKTile + u * 32 * 128) = x;
+          if (HD == 64) *reinterpret_cast<uint4*>(sK + s * kKTile + swizzled(row, 4 + piece * 2 + j)) = x;
+        }
       }
       fence_proxy_async_smem();
       mbar_arrive(&k_full[s]);
@@ -212,13 +268,13 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
       for (int u = 0; u < PER; ++u) {
         const uint32_t w[4] = {v_now[u].x, v_now[u].y, v_now[u].z, v_now[u].w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(to[j] + 2 * kTile + s * kTile + u * 32 * 128) = kv4_words(w[j]);
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(v_to[j] + s * kVTile + u * 32 * 128) = kv4_words(w[j]);
       }
       {
         const float scale = __uint_as_float(pair_now << 16), minimum = __uint_as_float(pair_now & 0xffff0000u);
         float* dst = (tid < 64 ? key_pairs[s] : value_pairs[s]) + (key >> 1) * 4 + (key & 1);
-        dst[0] = tid < 64 ? scale * p.scale_log2 : scale;
-        dst[2] = tid < 64 ? fmaf(-16.f, scale, minimum) * p.scale_log2 : fmaf(8.f, scale, minimum);
+        dst[0] = tid < 64 ? scale * p.scale_log2 * 4.f : scale;   // (a row's unit has 2^2 less)
+        dst[2] = tid < 64 ? minimum * p.scale_log2 : fmaf(8.f, scale, minimum);
         if (tid < 64 && (key & 15) == 0) at_pos[s][key >> 4] = pos_now;
       }
       fence_proxy_async_smem();
@@ -226,19 +282,19 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     }
   } else if (warp == 8) {
     // (the whole warp goes through the waits, and one lane issues: what a product takes stays uniform)
-    constexpr uint32_t idesc_s = make_umma_idesc_bf16(kKv4TileRows, K);
+    constexpr uint32_t idesc_s = make_umma_idesc_e4m3(kKv4TileRows, K);
     constexpr uint32_t idesc_o = make_umma_idesc_bf16(kKv4TileRows, HD) | (1u << 16);   // V: b_major = MN
-    const uint64_t q_desc = make_umma_desc_k128(sQ), k_desc = make_umma_desc_k128(sK), v_desc = make_umma_desc_mn128(sV, kKHalf);
+    const uint64_t q_desc = make_umma_desc_k128(sQ), k_desc = make_umma_desc_k128(sK), v_desc = make_umma_desc_mn128(sV, kVHalf);
     auto scores = [&](int i) {
       if (!tile_wait_warp(&k_full[i & 1], parity(i), pp.timeout)) return false;
       tc_fence_after();
-      const uint64_t kd = k_desc + (uint64_t)((i & 1) * (kTile >> 4));
+      const uint64_t kd = k_desc + (uint64_t)((i & 1) * (kKTile >> 4));
       const uint32_t to = tmem + (uint32_t)(i & 1) * 64u;
       if (elect_one()) {
 #pragma unroll
         for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16_ss(to, q_desc + (h * kQHalf >> 4) + 2 * k, kd + (h * kKHalf >> 4) + 2 * k, idesc_s, (uint32_t)((h | k) != 0));
+          for (int k = 0; k < 4; ++k) umma_e4m3_ss(to, q_desc + (h * kQHalf >> 4) + 2 * k, kd + 2 * k, idesc_s, (uint32_t)((h | k) != 0));   // (heads of 128: high parts, then low)
         umma_commit(&s_full[i & 1]);
       }
       __syncwarp();
@@ -251,7 +307,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
       if (i + 1 < n && !(go = scores(i + 1))) break;
       if (!(go = tile_wait_warp(&v_full[i & 1], parity(i), pp.timeout) && tile_wait_warp(&p_full[i & 1], parity(i), pp.timeout))) break;
       tc_fence_after();
-      const uint64_t vd = v_desc + (uint64_t)((i & 1) * (kTile >> 4));
+      const uint64_t vd = v_desc + (uint64_t)((i & 1) * (kVTile >> 4));
       const uint32_t from = tmem + (uint32_t)(i & 1) * 64u;
       if (elect_one()) {
 #pragma unroll
@@ -265,15 +321,8 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     const int at = warp * 32 + lane, r = TWIN ? at & 63 : at;
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     const int lim = ctx + r / G + 1;   // first position this row does not see (rows behind the tile's: some, dropped)
-    float sum = 0.f;
-#pragma unroll
-    for (int c = 0; c < HD / 8; ++c) {
-      float f[8];
-      unpack_bf16x8(*reinterpret_cast<const uint4*>(sQ + (c >> 3) * kQHalf + swizzled(at, c & 7)), f);
-      sum += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
-    }
-    if (!(fabsf(sum) < INFINITY)) sum = __uint_as_float(kKv4Nan);   // (a query that is not finite makes NaN, not one infinity less another or more)
-    const uint64_t sum2 = pack2(sum, sum);
+    const float unit = row_units[at].x;
+    const uint64_t sum2 = pack2(row_units[at].y, row_units[at].y);
     for (int i = 0; i < n && ok; ++i) {
       const uint32_t sp = tmem + lanes + (uint32_t)(i & 1) * 64u;
       if (!(ok = tile_wait_warp(&v_full[i & 1], parity(i), pp.timeout) && tile_wait_warp(&s_full[i & 1], parity(i), pp.timeout))) break;
@@ -308,7 +357,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
         for (int c = 12; c < 28; c += 8)
 #pragma unroll
           for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(u[c + e]), __uint_as_float(u[c + 4 + e]));
-        const float mx = fmaxf(max3(max3(top[0], top[1], __uint_as_float(u[28])), max3(top[2], top[3], __uint_as_float(u[29])), __uint_as_float(u[30])), __uint_as_float(u[31]));
+        const float mx = fmaxf(max3(max3(top[0], top[1], __uint_as_float(u[28])), max3(top[2], top[3], __uint_as_float(u[29])), __uint_as_float(u[30])), __uint_as_float(u[31])) * unit;
         const bool grow = mx > m + kPromptSlack;
         if (__any_sync(0xffffffffu, grow)) {
           const float f = grow ? exp2f(m - mx) : 1.f;   // (m = -inf: 0)
@@ -340,13 +389,13 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
         }
         const float ms = m == -INFINITY ? 0.f : m;
         if (whole) {
-          const uint64_t off = pack2(-ms, -ms);
+          const uint64_t off = pack2(-ms, -ms), unit2 = pack2(unit, unit);
           uint64_t sums = 0, lows = 0;
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
             const ulonglong2 w = vp[c >> 1];
             float x, y;
-            unpack2(add2(pack2(__uint_as_float(u[c]), __uint_as_float(u[c + 1])), off), &x, &y);
+            unpack2(fma2(pack2(__uint_as_float(u[c]), __uint_as_float(u[c + 1])), unit2, off), &x, &y);
             const uint64_t e = pack2(ex2_ftz(x), ex2_ftz(y));
             sums = add2(sums, e);
             lows = fma2(e, w.y, lows);
@@ -366,7 +415,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const bool there = pos[c / 16] + c % 16 + e < lim;
-              const float y = ex2_ftz(__uint_as_float(u[c + e]) - ms);
+              const float y = ex2_ftz(fmaf(__uint_as_float(u[c + e]), unit, -ms));
               l += y;
               if (there) low = fmaf(y, w[2 * c + 2 + e], low);
               z[e] = there ? y * w[2 * c + e] : 0.f;
