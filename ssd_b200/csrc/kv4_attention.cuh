@@ -24,8 +24,10 @@ namespace ssdk {
 //   Values: P has no such range, it is bf16 and so are the codes: 16 + c has c in the top of bf16's mantissa; of two values' words one byte_perm makes words whose halves are the
 // two keys of a fragment's register.  A product of P s' with ones beside them sums what the 16 + 8 too many amount to, of the rounded weights, and is taken off every 512 keys, while the sums
 // that cancel are small (32 subtractions a piece less).
-// A cluster of blocks shares the keys of a key head of one sequence: chunks of 32 keys go round the blocks' warps, each with a ring of its own (cp.async, no barrier between
-// warps) and a softmax of its own; at the end warps meet, then blocks.
+// Chunks of 32 keys go round a block's warps, each with a ring of its own (cp.async, no barrier between warps) and a softmax of its own; at the end warps meet, then blocks.
+// Which blocks work on which keys: few keys are shared by the blocks of a cluster, one to a sequence and key head, whose parts meet in shared memory (one launch).  Many keys (SHARED) are one
+// long row of turns, W chunks each, of which every block has an equal stretch, whatever the lengths: where a stretch begins or ends inside a head's keys it leaves a part in global memory, and
+// kv4_join_kernel puts the parts together.
 // A page outside the cache is passed over, a row that sees no key is zero; a NaN row of keys or values makes NaN of the rows that see it and of no other.
 // ----------------------------------------------------------------------------------
 struct Kv4AttnParams {
@@ -37,6 +39,7 @@ struct Kv4AttnParams {
   int64_t num_blocks;
   int B, Q, heads, kv_heads, block_size, max_blocks;
   float scale_log2;              // scale * log2(e)
+  float* parts;                  // SHARED: [blocks][2][rows of a key head][HD + 4]: O, reference, sum of a block's first stretch where it began in front of it, and of its last
 };
 constexpr float kKv4Slack = 8.f;
 constexpr int kKv4Most = 16, kKv4Stages = 3, kKv4Keys = 32;   // blocks of a cluster, a warp's ring, keys of a chunk
@@ -76,8 +79,59 @@ SSDK_DEVINL int kv4_v_place(int r, int c) {
   return (r >> 3) * 256 + ((r & 1) << 7) + ((r >> 1 & 3) << 5) + (c << 4);
 }
 
+// ---- shares of all turns: turn x of the row of them is one of the key heads of sequence b, kv_heads * (turns of a head of those in front) + head * turns(b) + ..; fewer than 2^31 in all (the host sees
+// to it) ----
+// turns of a key head's keys, one at least (whose block writes the zeros of rows that see nothing)
+template <int KEYS>
+SSDK_DEVINL int kv4_turns(const Kv4AttnParams& p, int b) { return max(1, (tokens_of(p.lens, b, p.max_blocks, p.block_size) + KEYS - 1) / KEYS); }
+// turns of a head of all sequences, and of those in front of sequence b (every lane of a warp asks, and gets them)
+template <int KEYS>
+SSDK_DEVINL int2 kv4_turns_of_all(const Kv4AttnParams& p, int b) {
+  int all = 0, before = 0;
+  for (int x = threadIdx.x & 31; x < p.B; x += 32) {
+    const int turns = kv4_turns<KEYS>(p, x);
+    all += turns;
+    before += x < b ? turns : 0;
+  }
+  return make_int2((int)__reduce_add_sync(0xffffffffu, (unsigned)all), (int)__reduce_add_sync(0xffffffffu, (unsigned)before));
+}
+// the sequence that turn `at` of the whole row belongs to, and the turns of a head in front of it
+template <int KEYS>
+SSDK_DEVINL int kv4_sequence_of(const Kv4AttnParams& p, int at, int* before) {
+  const int lane = threadIdx.x & 31;
+  int run = 0;
+  for (int base = 0; base < p.B; base += 32) {
+    const int mine = base + lane < p.B ? kv4_turns<KEYS>(p, base + lane) : 0;
+    int sum = mine;
+#pragma unroll
+    for (int w = 1; w < 32; w *= 2) {
+      const int x = __shfl_up_sync(0xffffffffu, sum, w);
+      if (lane >= w) sum += x;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, base + lane < p.B && at < (run + sum) * p.kv_heads);
+    if (past) {
+      const int x = __ffs(past) - 1;
+      *before = run + __shfl_sync(0xffffffffu, sum - mine, x);
+      return base + x;
+    }
+    run += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  *before = run;
+  return p.B;   // (behind the end)
+}
+// stretches of `all` turns for so many blocks: the first ones have one more; where block x begins, and which block has turn t
+struct Kv4Stretch {
+  int each, longer;
+  SSDK_DEVINL Kv4Stretch(int all, int blocks) : each(all / blocks), longer(all - all / blocks * blocks) {}
+  SSDK_DEVINL int first(int x) const { return x * each + min(x, longer); }
+  SSDK_DEVINL int block(int t) const {
+    const int split = longer * (each + 1);
+    return t < split ? t / (each + 1) : longer + (t - split) / each;   // (each > 0 where t >= split)
+  }
+};
+
 // NT tiles of eight rows, W warps; sixteen (eight with two tiles) warps are resident on an SM
-template <int HD, int NT, int W>
+template <int HD, int NT, int W, bool SHARED>
 __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __grid_constant__ Kv4AttnParams p) {
   constexpr int KW = HD / 32, VW = HD / 64, CODES = HD / 2, K = kKv4Keys, STAGE = kv4_stage_bytes(HD);
   extern __shared__ __align__(16) uint8_t kv4_smem[];
@@ -85,15 +139,42 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
   pdl_launch_dependents();
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = cluster.num_blocks(), rank = cluster.block_rank();
-  const int kvh = blockIdx.x / C, b = blockIdx.y;
+  const int C = SHARED ? 1 : (int)cluster.num_blocks(), rank = SHARED ? 0 : (int)cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int G = p.heads / p.kv_heads, r0 = blockIdx.z * 8 * NT, R = min(G * p.Q - r0, 8 * NT);   // rows of this block: r0 ..
+  const int G = p.heads / p.kv_heads, R = G * p.Q;   // at most 8 NT rows
+  int kvh = blockIdx.x / C, b = blockIdx.y;
+  // SHARED: this block's turns at .. end, the first of them turn `turn` of its head
+  int at = 0, end = 1, turn = 0, turns = 0;
+  if constexpr (SHARED) {
+    const Kv4Stretch stretch(kv4_turns_of_all<W * K>(p, 0).x * p.kv_heads, gridDim.x);
+    at = stretch.first(blockIdx.x);
+    end = stretch.first(blockIdx.x + 1);
+    if (at >= end) return;
+    int before;
+    b = kv4_sequence_of<W * K>(p, at, &before);
+    turns = kv4_turns<W * K>(p, b);
+    const int from = at - before * p.kv_heads;
+    kvh = from / turns;
+    turn = from - kvh * turns;
+  }
+#pragma unroll 1
+  for (bool again = false;; again = true) {
+  if constexpr (SHARED) {
+    if (again) {
+      if (at >= end) break;
+      turn = 0;
+      if (++kvh == p.kv_heads) {
+        kvh = 0;
+        turns = kv4_turns<W * K>(p, ++b);
+      }
+    }
+  }
   const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size), ctx = len - p.Q;
-  const int seen = min(len, ctx + (r0 + R - 1) / G + 1), seen_by_all = ctx + r0 / G + 1;   // positions that some row sees, that all do
+  const int seen_by_all = ctx + 1;   // positions that all rows see
 
   // ---- a warp's chunks of 32 keys: own, own + stride, ... ----
-  const int tiles = (max(seen, 0) + 15) >> 4, chunks = (tiles + 1) >> 1, stride = C * W, own = rank * W + warp;
+  const int tiles = (len + 15) >> 4, last_turn = SHARED ? min(turns, turn + (end - at)) : 0;
+  const int chunks = SHARED ? min((tiles + 1) >> 1, last_turn * W) : (tiles + 1) >> 1, stride = C * W, own = (SHARED ? turn * W : rank * W) + warp;
   const int n = own < chunks ? (chunks - own + stride - 1) / stride : 0;
   const int record = p.block_size * kv4_row_bytes(HD);   // bytes of a page and head
   uint8_t* ring = kv4_smem + warp * kKv4Stages * STAGE;
@@ -176,7 +257,7 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
   int lim[NT][2];              // first position that they do not see
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int r = r0 + nt * 8 + g;
+    const int r = nt * 8 + g;
     const __nv_bfloat16* q = p.q + ((size_t)(b * p.Q + r / G) * p.heads + kvh * G + r % G) * HD + t * (HD / 4);
     float f[KW][8], sum = 0.f, top = 0.f;
 #pragma unroll
@@ -215,7 +296,7 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
       const int row = nt * 8 + 2 * t + i;
       qs[nt][i] = __shfl_sync(0xffffffffu, sum, (2 * t + i) * 4) * p.scale_log2;
       qf[nt][i] = __shfl_sync(0xffffffffu, unit, (2 * t + i) * 4);
-      lim[nt][i] = row < R ? ctx + (r0 + row) / G + 1 : 0;
+      lim[nt][i] = row < R ? ctx + row / G + 1 : 0;
     }
   }
 
@@ -234,16 +315,16 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
 
   // scores of a chunk's keys g, g + 8, .. and rows 2 t, 2 t + 1 to weights, and their product with the values.  MASK: some row does not see some key, or a page is missing
   const uint32_t start[4] = {kKv4WholeWord, kKv4WholeWord, kKv4WholeWord, kKv4WholeWord}, ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-  auto work = [&](const uint8_t* at, int x, int pos, uint32_t none, auto mask) {   // (x: which sixteen of the chunk)
+  auto work = [&](const uint8_t* in, int x, int pos, uint32_t none, auto mask) {   // (x: which sixteen of the chunk)
     constexpr bool MASK = decltype(mask)::value;
-    const uint32_t* pairs = reinterpret_cast<const uint32_t*>(at + 2 * K * CODES) + g;
+    const uint32_t* pairs = reinterpret_cast<const uint32_t*>(in + 2 * K * CODES) + g;
     float s[NT][4];
     uint32_t hidden = 0;   // bits of the scores
     {
       uint32_t k[2][KW];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint8_t* row = at + (x * 16 + h * 8 + g) * CODES + t * (CODES / 4);
+        const uint8_t* row = in + (x * 16 + h * 8 + g) * CODES + t * (CODES / 4);
         if constexpr (HD == 128) {
           const uint4 w = *reinterpret_cast<const uint4*>(row);
           k[h][0] = w.x; k[h][1] = w.y; k[h][2] = w.z; k[h][3] = w.w;
@@ -335,7 +416,7 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
           pb[nt][h] = transpose_8x8(pack_bf16x2(w[0], w[1]));
         }
       }
-      const uint8_t* values = at + K * CODES + x * 16 * CODES;
+      const uint8_t* values = in + K * CODES + x * 16 * CODES;
       uint32_t v[4][VW];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {   // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
@@ -417,10 +498,17 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
       if (g == 0) *reinterpret_cast<float2*>(row + HD) = make_float2(ref[nt][e], l[nt][e]);
     }
   __syncthreads();
-  // four columns of a row
-  auto store = [&](int r, int d, float4 acc, float sum) {
+  // four columns of a row; SHARED: of a head's part, unless the whole of it is here
+  const bool whole_head = !SHARED || (turn == 0 && last_turn == turns);
+  auto store = [&](int r, int d, float4 acc, float top, float sum) {
+    if (!whole_head) {
+      float* part = p.parts + ((size_t)(2 * blockIdx.x + (turn == 0)) * R + r) * (HD + 4);
+      *reinterpret_cast<float4*>(part + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(part + HD) = make_float2(top, sum);
+      return;
+    }
     const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;   // (a row that sees no key is zero, NaN stays)
-    __nv_bfloat16* dst = p.out + ((size_t)(b * p.Q + (r0 + r) / G) * p.heads + kvh * G + (r0 + r) % G) * HD + d;
+    __nv_bfloat16* dst = p.out + ((size_t)(b * p.Q + r / G) * p.heads + kvh * G + r % G) * HD + d;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
   };
   for (int idx = threadIdx.x; idx < R * (HD / 4); idx += W * 32) {
@@ -439,12 +527,17 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
       sum += ml.y * f;
     }
     if (C == 1) {
-      store(r, d, acc, sum);
+      store(r, d, acc, top, sum);
     } else {
       *reinterpret_cast<float4*>(joined + r * LDO + d) = acc;
       if (d == 0) *reinterpret_cast<float2*>(joined + r * LDO + HD) = make_float2(top, sum);
     }
   }
+  if constexpr (SHARED) {
+    at += last_turn - turn;
+    __syncthreads();   // (the parts are read: their memory is the rings' again)
+    continue;
+  } else {
   if (C == 1) return;
   // the blocks' parts meet over the cluster's shared memory, each block joins a share of the columns
   cluster.sync();
@@ -463,9 +556,63 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
       acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
       sum += ml.y * f;
     }
-    store(r, d, acc, sum);
+    store(r, d, acc, top, sum);
   }
   cluster.sync();   // no block leaves while its part is read
+  return;
+  }
+  }
+}
+
+// ----------------------------------------------------------------------------------
+// kv4_join_kernel: the parts that the blocks of a shared launch left of a head's keys, put together; heads that one block had whole are in their place already.  A block a row, its warps take the
+// parts in turns.  KEYS: of a turn; blocks: of the launch in front.
+// ----------------------------------------------------------------------------------
+constexpr int kKv4JoinThreads = 128;
+template <int HD, int KEYS>
+__global__ void __launch_bounds__(kKv4JoinThreads) kv4_join_kernel(const __grid_constant__ Kv4AttnParams p, const int blocks) {
+  constexpr int W = kKv4JoinThreads / 32, V = HD / 32;   // channels of a lane
+  __shared__ float sums[W][HD], tops[W], totals[W];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int G = p.heads / p.kv_heads, R = G * p.Q, r = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int2 heads = kv4_turns_of_all<KEYS>(p, b);
+  const Kv4Stretch stretch(heads.x * p.kv_heads, blocks);
+  const int turns = kv4_turns<KEYS>(p, b), first = heads.y * p.kv_heads + kvh * turns, from = stretch.block(first), to = stretch.block(first + turns - 1);
+  if (from == to) return;   // (the whole block)
+  float top = -INFINITY, sum = 0.f, acc[V] = {};
+#pragma unroll 4
+  for (int x = from + warp; x <= to; x += W) {
+    const float* part = p.parts + ((size_t)(2 * x + (x == from)) * R + r) * (HD + 4);
+    const float2 ml = *reinterpret_cast<const float2*>(part + HD);
+    float v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = part[lane + 32 * i];
+    const float now = fmaxf(top, ml.x), f = now == -INFINITY ? 1.f : exp2f(top - now), w = now == -INFINITY ? 1.f : exp2f(ml.x - now);   // (no score, or NaN only: zeros and NaN add up)
+    top = now;
+    sum = sum * f + ml.y * w;
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = acc[i] * f + v[i] * w;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) sums[warp][lane + 32 * i] = acc[i];
+  if (lane == 0) {
+    tops[warp] = top;
+    totals[warp] = sum;
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < HD; d += kKv4JoinThreads) {
+    float most = -INFINITY, out = 0.f, total = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) most = fmaxf(most, tops[w]);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float f = most == -INFINITY ? 1.f : exp2f(tops[w] - most);
+      out += sums[w][d] * f;
+      total += totals[w] * f;
+    }
+    p.out[((size_t)(b * p.Q + r / G) * p.heads + kvh * G + r % G) * HD + d] = f2bf(out * (total > 0.f ? 1.f / total : total == 0.f ? 0.f : total));
+  }
 }
 
 }  // namespace ssdk

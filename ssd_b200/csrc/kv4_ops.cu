@@ -42,33 +42,44 @@ static int store(const Kv4StoreParams& p, int head_dim, void* stream) {
   return p.k_values ? launch_store<128, ROPE, true>(L, p) : launch_store<128, ROPE, false>(L, p);
 }
 
-// Blocks that share the keys of a key head (a cluster): as many as make the fewest waves of the longest context's pieces, a block's start and end as long as some 512 keys.
-static int kv4_cluster(int64_t units, int64_t keys, int resident, int most) {
-  int best = 1;
+// How a call's keys are shared.  Costs are in keys of a block: a block's start and end as long as some 512, the join of a cluster grows with its blocks; the longest context that the tables have room for.
+struct Kv4Plan {
+  int cluster, blocks;   // blocks: of a shared launch, 0 where clusters do
+};
+static Kv4Plan kv4_plan(int64_t units, int64_t keys, int resident, int most, int turn, bool may_share) {
+  Kv4Plan plan = {1, 0};
+  const int64_t slots = resident * kSms;
   int64_t least = INT64_MAX;
   for (int c = 1; c <= most; c *= 2) {
-    const int64_t cost = (units * c + resident * kSms - 1) / (resident * kSms) * (512 + 16 * c + keys / c);
+    const int64_t cost = (units * c + slots - 1) / slots * (512 + 16 * c + keys / c);
     if (cost < least) {
       least = cost;
-      best = c;
+      plan.cluster = c;
     }
   }
-  return best;
+  if (may_share && least > 1536 && units * ((keys + turn - 1) / turn) < (1ll << 31)) plan.blocks = (int)std::min(std::min(slots, units * 64), units * ((keys + turn - 1) / turn));
+  return plan;
 }
-template <int HD, int NT, int W>
-static int launch_warps(Launcher& L, const Kv4AttnParams& p, int64_t units) {
-  static std::atomic<bool> done[64];
-  CKI(with_smem(kv4_attn_kernel<HD, NT, W>, kv4_attn_smem(HD, NT, W), kSmemClusters, done));
-  const int64_t tiles = units / ((int64_t)p.B * p.kv_heads);
-  if (tiles > 65535) return fail("paged_attn_kv4: q_len=%d", p.Q);
-  L.cluster = kv4_cluster(units, (int64_t)p.max_blocks * p.block_size, 16 / NT / W, kKv4Most);
-  return L.go(kv4_attn_kernel<HD, NT, W>, dim3(p.kv_heads * L.cluster, p.B, (unsigned)tiles), dim3(W * 32), kv4_attn_smem(HD, NT, W), p);
+constexpr int kKv4Warps = 4, kMaxShared = 1024;   // warps of a block; sequences of a shared launch (each block goes through their lengths)
+static Kv4Plan kv4_few_plan(int batch, int q_len, int heads, int kv_heads, int64_t keys) {
+  const int tiles = (heads / kv_heads * q_len + 7) / 8;
+  return kv4_plan((int64_t)batch * kv_heads, keys, 16 / tiles / kKv4Warps, kKv4Most, kKv4Warps * kKv4Keys, batch <= kMaxShared);
 }
 template <int HD, int NT>
 static int launch_attn(Launcher& L, const Kv4AttnParams& p) {
-  const int64_t rows = (int64_t)(p.heads / p.kv_heads) * p.Q, units = (rows + 8 * NT - 1) / (8 * NT) * p.B * p.kv_heads;
-  if (units * kKv4Most <= kSms) return launch_warps<HD, NT, 16 / NT>(L, p, units);   // a block to an SM at most
-  return launch_warps<HD, NT, 4>(L, p, units);
+  constexpr int W = kKv4Warps, smem = kv4_attn_smem(HD, NT, W);
+  const Kv4Plan plan = kv4_few_plan(p.B, p.Q, p.heads, p.kv_heads, (int64_t)p.max_blocks * p.block_size);
+  if (plan.blocks) {
+    static std::atomic<bool> done[64];
+    CKI(with_smem(kv4_attn_kernel<HD, NT, W, true>, smem, kSmemCarveout, done));
+    if (!p.parts) return fail("paged_attn_kv4: null argument (scratch)");
+    CKI(L.go(kv4_attn_kernel<HD, NT, W, true>, dim3(plan.blocks), dim3(W * 32), smem, p));
+    return L.go(kv4_join_kernel<HD, W * kKv4Keys>, dim3(p.heads / p.kv_heads * p.Q, p.kv_heads, p.B), dim3(kKv4JoinThreads), 0, p, plan.blocks);
+  }
+  static std::atomic<bool> done[64];
+  CKI(with_smem(kv4_attn_kernel<HD, NT, W, false>, smem, kSmemClusters, done));
+  L.cluster = plan.cluster;
+  return L.go(kv4_attn_kernel<HD, NT, W, false>, dim3(p.kv_heads * L.cluster, p.B), dim3(W * 32), smem, p);
 }
 template <int HD, bool TWIN>
 static int launch_tiles(Launcher& L, const Kv4AttnParams& a) {
@@ -84,7 +95,7 @@ static int launch_tiles(Launcher& L, const Kv4AttnParams& a) {
   p.tokens = (a.Q + tiles - 1) / tiles;
   p.timeout = waits->word;
   const int blocks = TWIN && HD == 64 ? 8 : kKv4Most;   // (their join has a lane of HD / 4 for each part)
-  L.cluster = kv4_cluster((int64_t)a.B * a.kv_heads * tiles, (int64_t)a.max_blocks * a.block_size, 2, blocks);
+  L.cluster = kv4_plan((int64_t)a.B * a.kv_heads * tiles, (int64_t)a.max_blocks * a.block_size, 2, blocks, kKv4TileKeys, false).cluster;
   return L.go(kv4_tile_kernel<HD, TWIN>, dim3(a.kv_heads * L.cluster, a.B, tiles), dim3(kKv4TileThreads), kv4_tile_smem(HD), p);
 }
 
@@ -151,8 +162,14 @@ int ssdk_load_kv4(const void* k_cache, const void* v_cache, const int32_t* slot_
   return head_dim == 64 ? L.go(kv4_load_kernel<64>, grid, block, 0, p) : L.go(kv4_load_kernel<128>, grid, block, 0, p);
 }
 
+int64_t ssdk_paged_attn_kv4_scratch_bytes(int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size, int max_blocks_per_seq) {
+  if (batch < 1 || q_len < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || block_size < 1 || max_blocks_per_seq < 1) return 0;
+  const int64_t rows = (int64_t)(heads / kv_heads) * q_len;
+  if (rows > 16) return 0;
+  return 8ll * kv4_few_plan(batch, q_len, heads, kv_heads, (int64_t)max_blocks_per_seq * block_size).blocks * rows * (head_dim + 4);
+}
 int ssdk_paged_attn_kv4(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables, const int32_t* context_lens,
-                        void* out, int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size, int max_blocks_per_seq,
+                        void* out, void* scratch, int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size, int max_blocks_per_seq,
                         int64_t num_blocks, float scale, void* stream) {
   CKI(check_kv4("paged_attn_kv4", num_blocks, block_size, kv_heads, head_dim));
   CKI(check_pages("paged_attn_kv4", batch, block_size, max_blocks_per_seq, num_blocks));
@@ -161,14 +178,14 @@ int ssdk_paged_attn_kv4(const void* q, const void* k_cache, const void* v_cache,
     return fail("paged_attn_kv4: q_len=%d, %d heads over %d (at most 32 to a key head), scale %g (finite, log2(e) times it too)", q_len, heads, kv_heads, (double)scale);
   if ((int64_t)batch * q_len >= (1ll << 31) || (int64_t)q_len * (heads / kv_heads) >= (1ll << 31) - 65536) return fail("paged_attn_kv4: %d rows of %d sequences", q_len, batch);
   if (!q || !k_cache || !v_cache || !block_tables || !context_lens || !out) return fail("paged_attn_kv4: null argument");
-  if (off16(q, k_cache, v_cache, out)) return fail("paged_attn_kv4: arrays must start at multiples of 16 bytes");
+  if (off16(q, k_cache, v_cache, out) || off16(scratch)) return fail("paged_attn_kv4: arrays must start at multiples of 16 bytes");
   const int64_t rows = 2ll * batch * q_len * heads * head_dim, cache = kv4_bytes(num_blocks, block_size, kv_heads, head_dim);
-  CKI(check_apart("paged_attn_kv4", {{"out", out, rows}},
+  CKI(check_apart("paged_attn_kv4", {{"out", out, rows}, {"scratch", scratch, ssdk_paged_attn_kv4_scratch_bytes(batch, q_len, heads, kv_heads, head_dim, block_size, max_blocks_per_seq)}},
                   {{"q", q, rows}, {"k_cache", k_cache, cache}, {"v_cache", v_cache, cache}, {"block_tables", block_tables, 4ll * batch * max_blocks_per_seq}, {"context_lens", context_lens, 4ll * batch}}));
   Kv4AttnParams p;
   p.q = (const bf16*)q; p.k_cache = (const uint8_t*)k_cache; p.v_cache = (const uint8_t*)v_cache; p.tables = block_tables; p.lens = context_lens; p.out = (bf16*)out;
   p.num_blocks = num_blocks; p.B = batch; p.Q = q_len; p.heads = heads; p.kv_heads = kv_heads; p.block_size = block_size; p.max_blocks = max_blocks_per_seq;
-  p.scale_log2 = scale_log2;
+  p.scale_log2 = scale_log2; p.parts = (float*)scratch;
   Launcher L = launcher(stream);
   if ((int64_t)(heads / kv_heads) * q_len <= 8) return head_dim == 64 ? launch_attn<64, 1>(L, p) : launch_attn<128, 1>(L, p);
   if ((int64_t)(heads / kv_heads) * q_len <= 16) return head_dim == 64 ? launch_attn<64, 2>(L, p) : launch_attn<128, 2>(L, p);

@@ -155,7 +155,8 @@ SIGNATURES: dict[str, tuple] = {
     "ssdk_rope_store_kv4": (C.c_int, [VP] * 4 + [C.c_int64, C.c_int, VP, VP, C.c_float] + [VP] * 5 + [C.c_int64] + [C.c_int] * 5 + [VP]),
     "ssdk_store_kv4": (C.c_int, [VP, VP, C.c_int64, C.c_int64] + [VP] * 5 + [C.c_int64] + [C.c_int] * 4 + [VP]),
     "ssdk_load_kv4": (C.c_int, [VP] * 5 + [C.c_int64] + [C.c_int] * 4 + [VP]),
-    "ssdk_paged_attn_kv4": (C.c_int, [VP] * 6 + [C.c_int] * 7 + [C.c_int64, C.c_float, VP]),
+    "ssdk_paged_attn_kv4_scratch_bytes": (C.c_int64, [C.c_int] * 7),
+    "ssdk_paged_attn_kv4": (C.c_int, [VP] * 7 + [C.c_int] * 7 + [C.c_int64, C.c_float, VP]),
     "ssdk_sample": (C.c_int, [VP, C.c_int64, VP, C.c_int, C.c_int, C.c_uint64, C.c_uint64, VP, VP]),
     "ssdk_verify_scratch_bytes": (C.c_int64, [C.c_int, C.c_int]),
     "ssdk_verify": (C.c_int, [VP, VP, VP, VP, VP, VP, C.c_int, C.c_int, C.c_int, C.c_int, C.c_uint64, C.c_uint64,

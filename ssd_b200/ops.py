@@ -432,6 +432,11 @@ def load_kv4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.T
     return both
 
 
+@functools.lru_cache(maxsize=256)
+def _kv4_scratch(*sizes: int) -> int:
+    return _L.load().ssdk_paged_attn_kv4_scratch_bytes(*sizes) // 2
+
+
 def paged_attention_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor, q_len: int,
                         scale: float) -> torch.Tensor:
     """paged_attention over a cache of 4 bits (kv4_caches): q [B * q_len, H, hd] bf16, block_tables int32 [B, max_blocks], context_lens int32 [B] with the new tokens.
@@ -442,7 +447,9 @@ def paged_attention_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     cache, block_size = _kv4("paged_attention_kv4", k_cache, hd)
     gpu = _check("paged_attention_kv4", (q, "q", _BF, (B * q_len, H, hd)), (k_cache, "k_cache", _U8, cache), (v_cache, "v_cache", _U8, cache),
                  (block_tables, "block_tables", _I32, (B, width)), (context_lens, "context_lens", _I32, (B,)))
-    out = q.new_empty(B * q_len, H * hd)
-    _launch("ssdk_paged_attn_kv4", gpu, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(), B, q_len, H, cache[1],
+    out, scratch = q.new_empty(B * q_len, H * hd), _kv4_scratch(B, q_len, H, cache[1], hd, block_size, width)
+    if scratch:
+        scratch = (room := q.new_empty(scratch)).data_ptr()
+    _launch("ssdk_paged_attn_kv4", gpu, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(), scratch or None, B, q_len, H, cache[1],
             hd, block_size, width, cache[0], scale)
     return out

@@ -1,4 +1,4 @@
-"""The paged cache held in 4 bits (ops.rope_store_kv4, store_kv4, load_kv4, paged_attention_kv4) from its definitions, in 64 bits, one row after the other."""
+"""The paged cache held in 4 bits (ops.rope_store_kv4, store_kv4, load_kv4, paged_attention_kv4) from its definitions, in 64 bits, read as they are written."""
 import math
 
 import torch
@@ -41,11 +41,10 @@ def put(cache, hd, x, slots):
     codes, scale, low = held(x)
     pair = torch.cat([scale, low], -1).contiguous().view(torch.uint8)   # [M, KV, 4]
     byte = (codes[..., ::2] + 16 * codes[..., 1::2]).to(torch.uint8)
-    for m, slot in enumerate(slots.tolist()):
-        if 0 <= slot < num * S:
-            page, off = divmod(slot, S)
-            cache[page, :, off * (hd // 2):(off + 1) * (hd // 2)] = byte[m]
-            cache[page, :, S * (hd // 2) + 4 * off:S * (hd // 2) + 4 * off + 4] = pair[m]
+    keep = (slots >= 0) & (slots < num * S)
+    page, off = slots[keep].long() // S, slots[keep].long() % S
+    cache[:, :, :S * (hd // 2)].unflatten(2, (S, hd // 2))[page, :, off] = byte[keep]
+    cache[:, :, S * (hd // 2):].unflatten(2, (S, 4))[page, :, off] = pair[keep]
     return values(codes, scale, low)
 
 

@@ -164,7 +164,7 @@ P = 1 << 20   # addresses that no call below gets to use
 ROPE = [P * i for i in range(1, 5)] + [100, 64, None, None, 1e-6] + [P * i for i in range(5, 10)] + [2, 16, 3, 2, 1, 64, None]
 STORE = [P, 2 * P, 64, 64] + [P * i for i in range(3, 8)] + [2, 16, 3, 1, 64, None]
 LOAD = [P * i for i in range(1, 6)] + [2, 16, 3, 1, 64, None]
-ATTN = [P * i for i in range(1, 7)] + [2, 1, 2, 1, 64, 16, 3, 2, 1.0, None]
+ATTN = [P * i for i in range(1, 7)] + [None, 2, 1, 2, 1, 64, 16, 3, 2, 1.0, None]
 
 
 @pytest.mark.parametrize("name,good,bad", [
@@ -172,8 +172,8 @@ ATTN = [P * i for i in range(1, 7)] + [2, 1, 2, 1, 64, 16, 3, 2, 1.0, None]
                                    (14, 0), (14, 1 << 28), (15, 8), (15, 24), (15, 65552), (16, 0), (17, 0), (17, 65536), (18, 0), (18, 65536), (19, 96), (19, 256)]),
     ("ssdk_store_kv4", STORE, [(0, 0), (1, 2 * P + 2), (2, -64), (2, 4), (3, 1 << 31), (4, 0), (5, 5 * P), (6, 0), (6, 2 * P), (7, 0), (8, 0), (8, 6 * P), (9, 0), (9, 1 << 40), (10, 0), (11, 0), (11, -1), (12, 0), (13, 32)]),
     ("ssdk_load_kv4", LOAD, [(0, 0), (1, 8), (2, 0), (3, 0), (3, 5 * P), (4, 2 * P), (4, 5 * P + 4), (5, 0), (6, 20), (7, 0), (7, (1 << 30) + 1), (8, 0), (9, 96)]),
-    ("ssdk_paged_attn_kv4", ATTN, [(0, 0), (0, P + 2), (1, 0), (2, 8), (3, 0), (4, 0), (5, 0), (5, P), (5, 3 * P), (6, 0), (6, 65536), (7, 0), (7, 1 << 30), (8, 0), (8, 33), (9, 0), (9, 3), (10, 80), (11, 8), (12, 0),
-                                   (12, 1 << 27), (13, 0), (13, 1 << 27), (14, float("inf")), (14, float("nan")), (14, 3e38)]),
+    ("ssdk_paged_attn_kv4", ATTN, [(0, 0), (0, P + 2), (1, 0), (2, 8), (3, 0), (4, 0), (5, 0), (5, P), (5, 3 * P), (6, 8), (7, 0), (7, 65536), (8, 0), (8, 1 << 30), (9, 0), (9, 33), (10, 0), (10, 3), (11, 80), (12, 8),
+                                   (13, 0), (13, 1 << 27), (14, 0), (14, 1 << 27), (15, float("inf")), (15, float("nan")), (15, 3e38)]),
 ])
 def test_refusals_of_the_entry_points(name, good, bad):
     from ssd_b200 import lib

@@ -146,9 +146,9 @@ def a_case(g, KV, hd, S, lens, width=None, stale=True):
         x = (torch.randn(total * S, KV, hd, generator=g) * (0.5 + torch.rand(KV, hd, generator=g)) + torch.randn(KV, hd, generator=g)) * size
         if stale:
             of = torch.zeros(total * S, dtype=torch.bool)
-            for row, n in zip(table.tolist(), lens):
-                for i in range(n):
-                    of[row[i // S] * S + i % S] = True
+            for row, n in zip(table.long(), lens):
+                i = torch.arange(max(n, 0))
+                of[row[i // S] * S + i % S] = True
             x[~of] = NAN
         plain.put(cache, hd, x.to(BF), torch.arange(total * S))
         if stale:   # (the codes of a NaN row are zero; here they are anything)
@@ -184,6 +184,20 @@ def test_long_and_many(dev, B, Q, H, KV, hd, S, ctx):
     for scale in (hd ** -0.5, -0.5, 0.0):
         got = ops.paged_attention_kv4(q.to(dev), kc.to(dev), vc.to(dev), table.to(dev), i32(lens, dev), Q, scale)
         within(got, *plain.attention(q, kc, vc, table, lens, Q, scale))
+
+
+@pytest.mark.parametrize("Q,H,KV,hd,S,lens,width", [
+    (1, 8, 1, 128, 256, [30000], 118), (1, 4, 2, 64, 64, [1, 0, 25000, 31, 128, 129, 4000], 400), (2, 16, 2, 128, 16, [700, 9000, 2], 5000), (1, 5, 5, 128, 256, [3000, 60, 0], 2000),
+    (7, 2, 1, 64, 80, [12000, 7, 3, 333], 300), (1, 2, 2, 64, 16, [130] * 37, 4000), (8, 16, 2, 64, 64, [20000, 100, 8], 400), (7, 16, 2, 128, 256, [5000, 3, 9000], 200), (40, 8, 2, 64, 16, [4000, 50], 3000),
+])
+def test_shares_of_long_tables(dev, Q, H, KV, hd, S, lens, width):
+    """Tables with room for much: blocks have equal stretches of all sequences' keys, which begin and end anywhere, or none; short and empty sequences between long ones."""
+    from ssd_b200 import ops
+    g = gen(Q, H, KV, hd, sum(lens))
+    kc, vc, table = a_case(g, KV, hd, S, lens, width=width)
+    q = torch.randn(len(lens) * Q, H, hd, generator=g).to(BF)
+    got = ops.paged_attention_kv4(q.to(dev), kc.to(dev), vc.to(dev), table.to(dev), i32(lens, dev), Q, hd ** -0.5)
+    within(got, *plain.attention(q, kc, vc, table, lens, Q, hd ** -0.5))
 
 
 @pytest.mark.parametrize("Q,H", [(1, 4), (6, 16)])
