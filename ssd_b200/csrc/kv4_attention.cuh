@@ -18,12 +18,11 @@ namespace ssdk {
 // Bound by the bytes of the cache, then by the instructions that make codes into fragments.  The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that
 // keys (sixteen) and channels (sixteen) are the m of mma and the eight query rows of a usual group its n.
 //   Scores are whole numbers: a mask (and a shift) makes four codes of a word bytes, and a query row, scaled by a power of two so that its largest lies in 2^14 .. 2^15 and rounded, is 256 h + l with a
-// byte each, so that its values are off by at most 2^-15 of its largest (those above 2^-7 of it by nothing).  The sums start at the word of 1.5 2^23, so that they are floats without a
-// conversion.  (bf16 codes take 64 instructions for sixteen keys where these take 24; mma on e4m3 is made of conversions and f16 here: four times as slow.)  Which channels a product's k stands for is
-// free: a quad's lanes read a key's row, 16 bytes each, and the query's fragments follow.
-//   Values: P has no such range, it is bf16 and so are the codes: 16 + c has c in the top of bf16's mantissa; of two values' words one byte_perm makes words whose halves are the
-// two keys of a fragment's register.  A product of P s' with ones beside them sums what the 16 + 8 too many amount to, of the rounded weights, and is taken off every 512 keys, while the sums
-// that cancel are small (32 subtractions a piece less).
+// byte each, so that its values are off by at most 2^-15 of its largest (those above 2^-7 of it by nothing).  (bf16 codes take 64 instructions for sixteen keys where these take 24; mma on e4m3 is
+// made of conversions and f16 here: four times as slow.)  Which channels a product's k stands for is free: a quad's lanes read a key's row, 16 bytes each, and the query's fragments follow.
+//   Values: P has no such range, it is bf16 and so are the codes: 16 + c has c in the top of bf16's mantissa, 128 + c in its end (no shift for the first of four codes).  ldmatrix turns the rows of
+// codes so that a register's halves are four channels each of two keys, which is what the fragments of four products need.  A product of P s' with ones beside them sums what the constants too many
+// amount to, of the rounded weights, and is taken off every 256 keys, while the sums that cancel are small.
 // Chunks of 32 keys go round a block's warps, each with a ring of its own (cp.async, no barrier between warps) and a softmax of its own; at the end warps meet, then blocks.
 // Which blocks work on which keys: few keys are shared by the blocks of a cluster, one to a sequence and key head, whose parts meet in shared memory (one launch).  Many keys (SHARED) are one
 // long row of turns, W chunks each, of which every block has an equal stretch, whatever the lengths: where a stretch begins or ends inside a head's keys it leaves a part in global memory, and
@@ -60,23 +59,28 @@ SSDK_DEVINL uint32_t transpose_8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
   return d;
 }
-// 16 x 8 = c + codes (bytes) x 32 bytes of a query, signed or not
-template <bool SIGNED>
-SSDK_DEVINL void mma_u8_16832(uint32_t* d, const uint32_t* a, uint32_t b0, uint32_t b1, const uint32_t* c) {
-  if (SIGNED)
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
-                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
-  else
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
-                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+// 16 x 8 (+)= codes (bytes) x 32 bytes of a query, signed or not; the first product of a sum takes zeros that need no registers
+template <bool SIGNED, bool FIRST>
+SSDK_DEVINL void mma_u8_16832(int (&c)[4], const uint32_t* a, uint32_t b0, uint32_t b1) {
+#define SSDK_U8(TYPE)                                                                                                                                                             \
+  if (FIRST)                                                                                                                                                                      \
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8." TYPE ".s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"                                           \
+                 : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));                                       \
+  else                                                                                                                                                                            \
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8." TYPE ".s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"                                             \
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  if constexpr (SIGNED) { SSDK_U8("s8") } else { SSDK_U8("u8") }
+#undef SSDK_U8
 }
-constexpr float kKv4Whole = 12582912.f;            // 1.5 2^23
-constexpr uint32_t kKv4WholeWord = 0x4b400000u;    // its word: a whole number below 2^22 added to it is added to the float
-// where the 16-byte piece c of the codes of value r lies in its stage: four lanes read the rows 2 t + const at a time, 8 (4) bytes a lane, from banks of their own
+// where the 16-byte piece c of the codes of value r lies in its stage: pieces c of eight rows, which ldmatrix reads together, are in banks of their own
 template <int HD>
 SSDK_DEVINL int kv4_v_place(int r, int c) {
-  if (HD == 128) return (r >> 1) * 128 + (((r ^ (r >> 1)) & 1) << 6) + ((c ^ ((r >> 2 & 1) << 1)) << 4);
-  return (r >> 3) * 256 + ((r & 1) << 7) + ((r >> 1 & 3) << 5) + (c << 4);
+  return HD == 128 ? r * 64 + ((c ^ (r >> 1 & 3)) << 4) : r * 32 + ((c ^ (r >> 2 & 1)) << 4);
+}
+// nibble P of both halves of a word as 16 + c (128 + c for the first) in bf16
+template <int P>
+SSDK_DEVINL uint32_t kv4_nibble(uint32_t w) {
+  return P == 0 ? (w & 0x000f000fu) | 0x43004300u : (w >> (4 * P - 3) & 0x00780078u) | 0x41804180u;
 }
 
 // ---- shares of all turns: turn x of the row of them is one of the key heads of sequence b, kv_heads * (turns of a head of those in front) + head * turns(b) + ..; fewer than 2^31 in all (the host sees
@@ -314,7 +318,7 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
   }
 
   // scores of a chunk's keys g, g + 8, .. and rows 2 t, 2 t + 1 to weights, and their product with the values.  MASK: some row does not see some key, or a page is missing
-  const uint32_t start[4] = {kKv4WholeWord, kKv4WholeWord, kKv4WholeWord, kKv4WholeWord}, ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+  const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
   auto work = [&](const uint8_t* in, int x, int pos, uint32_t none, auto mask) {   // (x: which sixteen of the chunk)
     constexpr bool MASK = decltype(mask)::value;
     const uint32_t* pairs = reinterpret_cast<const uint32_t*>(in + 2 * K * CODES) + g;
@@ -333,14 +337,19 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
           k[h][0] = w.x; k[h][1] = w.y;
         }
       }
-      uint32_t whole[NT][2][4];
+      int whole[NT][2][4];
 #pragma unroll
       for (int j = 0; j < KW; ++j) {
         const uint32_t a[4] = {k[0][j] & 0x0f0f0f0fu, k[1][j] & 0x0f0f0f0fu, k[0][j] >> 4 & 0x0f0f0f0fu, k[1][j] >> 4 & 0x0f0f0f0fu};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma_u8_16832<true>(whole[nt][0], a, qb[nt][j][0][0], qb[nt][j][0][1], j ? whole[nt][0] : start);
-          mma_u8_16832<false>(whole[nt][1], a, qb[nt][j][1][0], qb[nt][j][1][1], j ? whole[nt][1] : start);
+          if (j == 0) {
+            mma_u8_16832<true, true>(whole[nt][0], a, qb[nt][j][0][0], qb[nt][j][0][1]);
+            mma_u8_16832<false, true>(whole[nt][1], a, qb[nt][j][1][0], qb[nt][j][1][1]);
+          } else {
+            mma_u8_16832<true, false>(whole[nt][0], a, qb[nt][j][0][0], qb[nt][j][0][1]);
+            mma_u8_16832<false, false>(whole[nt][1], a, qb[nt][j][1][0], qb[nt][j][1][1]);
+          }
         }
       }
 #pragma unroll
@@ -352,7 +361,7 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float& v = s[nt][2 * h + e];
-            v = fmaf(__uint_as_float(whole[nt][0][2 * h + e]) - kKv4Whole, 256.f, __uint_as_float(whole[nt][1][2 * h + e]) - kKv4Whole);   // (exact to 2^-24)
+            v = (float)(whole[nt][0][2 * h + e] * 256 + whole[nt][1][2 * h + e]);   // (below 2^27)
             v = fmaf(v, sk * qf[nt][e], mk * qs[nt][e]);
             if (MASK && ((none >> x & 1u) || pos + x * 16 + h * 8 + g >= lim[nt][e])) {
               v = -INFINITY;
@@ -416,24 +425,13 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
           pb[nt][h] = transpose_8x8(pack_bf16x2(w[0], w[1]));
         }
       }
-      const uint8_t* values = in + K * CODES + x * 16 * CODES;
-      uint32_t v[4][VW];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {   // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-        const uint8_t* row = values + kv4_v_place<HD>(2 * t + (i & 1) + 8 * (i >> 1), g * (CODES / 8) / 16) + g * (CODES / 8) % 16;
-        if constexpr (HD == 128) {
-          const uint2 w = *reinterpret_cast<const uint2*>(row);
-          v[i][0] = w.x; v[i][1] = w.y;
-        } else {
-          v[i][0] = *reinterpret_cast<const uint32_t*>(row);
-        }
-      }
+      // [keys 0 .. 7, 8 .. 15][32 channels of 64]: lane 8 i + r names row r of matrix i
 #pragma unroll
       for (int j = 0; j < VW; ++j) {
-        const uint32_t a01 = __byte_perm(v[0][j], v[1][j], 0x5410), b01 = __byte_perm(v[0][j], v[1][j], 0x7632);
-        const uint32_t a23 = __byte_perm(v[2][j], v[3][j], 0x5410), b23 = __byte_perm(v[2][j], v[3][j], 0x7632);
-        const uint32_t a[4][4] = {{kv4_pair16<0>(a01), kv4_pair16<0>(b01), kv4_pair16<0>(a23), kv4_pair16<0>(b23)}, {kv4_pair16<1>(a01), kv4_pair16<1>(b01), kv4_pair16<1>(a23), kv4_pair16<1>(b23)},
-                                  {kv4_pair16<2>(a01), kv4_pair16<2>(b01), kv4_pair16<2>(a23), kv4_pair16<2>(b23)}, {kv4_pair16<3>(a01), kv4_pair16<3>(b01), kv4_pair16<3>(a23), kv4_pair16<3>(b23)}};
+        uint32_t w[4];   // keys 2 t, 2 t + 1 of channels 64 j + 4 g .., of 32 more; the same of keys 8 on
+        ldmatrix_x4_trans(w, in + K * CODES + x * 16 * CODES + kv4_v_place<HD>((lane & 7) + 8 * (lane >> 4), 2 * j + (lane >> 3 & 1)));
+        const uint32_t a[4][4] = {{kv4_nibble<0>(w[0]), kv4_nibble<0>(w[1]), kv4_nibble<0>(w[2]), kv4_nibble<0>(w[3])}, {kv4_nibble<1>(w[0]), kv4_nibble<1>(w[1]), kv4_nibble<1>(w[2]), kv4_nibble<1>(w[3])},
+                                  {kv4_nibble<2>(w[0]), kv4_nibble<2>(w[1]), kv4_nibble<2>(w[2]), kv4_nibble<2>(w[3])}, {kv4_nibble<3>(w[0]), kv4_nibble<3>(w[1]), kv4_nibble<3>(w[2]), kv4_nibble<3>(w[3])}};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -450,7 +448,7 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[nt][i][e] = fmaf(-24.f, one[nt][e], o[nt][i][e]);
+        for (int e = 0; e < 4; ++e) o[nt][i][e] = fmaf(i & 3 ? -24.f : -136.f, one[nt][e], o[nt][i][e]);   // (codes less 8)
       one[nt][0] = one[nt][1] = one[nt][2] = one[nt][3] = 0.f;
     }
   };
@@ -469,7 +467,7 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
 #pragma unroll 1
       for (int x = 0; x < 2; ++x) work(ring + stage * STAGE, x, pos, none, std::true_type());
     }
-    if ((i & 15) == 15) take_off();
+    if ((i & 7) == 7) take_off();
   }
   take_off();
   cp_async_wait<0>();
@@ -490,10 +488,10 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
       }
       float* row = parts + (warp * ROWS + nt * 8 + 2 * t + e) * LDO;
 #pragma unroll
-      for (int j = 0; j < VW; ++j)   // channels g HD / 8 + 8 j ..
+      for (int j = 0; j < VW; ++j)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          *reinterpret_cast<float4*>(row + g * (HD / 8) + 8 * j + 4 * h) =
+          *reinterpret_cast<float4*>(row + 64 * j + 32 * h + 4 * g) =
               make_float4(o[nt][4 * j][2 * h + e] + low[nt][e], o[nt][4 * j + 1][2 * h + e] + low[nt][e], o[nt][4 * j + 2][2 * h + e] + low[nt][e], o[nt][4 * j + 3][2 * h + e] + low[nt][e]);
       if (g == 0) *reinterpret_cast<float2*>(row + HD) = make_float2(ref[nt][e], l[nt][e]);
     }
@@ -565,53 +563,68 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
 }
 
 // ----------------------------------------------------------------------------------
-// kv4_join_kernel: the parts that the blocks of a shared launch left of a head's keys, put together; heads that one block had whole are in their place already.  A block a row, its warps take the
-// parts in turns.  KEYS: of a turn; blocks: of the launch in front.
+// kv4_join_kernel: the parts that the blocks of a shared launch left of a head's keys, put together; heads that one block had whole are in their place already.  KEYS: of a turn; blocks: of the
+// launch in front.  A warp puts a row together, a lane asks for a part's reference and sum, and then for the columns that are its own.  SPREAD: few heads in many parts, a block's warps take
+// them in turns and meet in shared memory (one context of 32000 in 64 parts a head: 7.5 us with four warps and loads in fours).
 // ----------------------------------------------------------------------------------
-constexpr int kKv4JoinThreads = 128;
-template <int HD, int KEYS>
-__global__ void __launch_bounds__(kKv4JoinThreads) kv4_join_kernel(const __grid_constant__ Kv4AttnParams p, const int blocks) {
+constexpr int kKv4JoinThreads = 256;
+template <int HD, int KEYS, bool SPREAD>
+__global__ void __launch_bounds__(kKv4JoinThreads, 2) kv4_join_kernel(const __grid_constant__ Kv4AttnParams p, const int blocks) {
   constexpr int W = kKv4JoinThreads / 32, V = HD / 32;   // channels of a lane
-  __shared__ float sums[W][HD], tops[W], totals[W];
+  __shared__ float sums[SPREAD ? W : 1][HD];
+  __shared__ float2 totals[W];
   pdl_wait();
   pdl_launch_dependents();
-  const int G = p.heads / p.kv_heads, R = G * p.Q, r = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = p.heads / p.kv_heads, R = G * p.Q, kvh = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int2 heads = kv4_turns_of_all<KEYS>(p, b);
   const Kv4Stretch stretch(heads.x * p.kv_heads, blocks);
   const int turns = kv4_turns<KEYS>(p, b), first = heads.y * p.kv_heads + kvh * turns, from = stretch.block(first), to = stretch.block(first + turns - 1);
   if (from == to) return;   // (the whole block)
-  float top = -INFINITY, sum = 0.f, acc[V] = {};
-#pragma unroll 4
-  for (int x = from + warp; x <= to; x += W) {
-    const float* part = p.parts + ((size_t)(2 * x + (x == from)) * R + r) * (HD + 4);
-    const float2 ml = *reinterpret_cast<const float2*>(part + HD);
-    float v[V];
+  for (int r = SPREAD ? (int)blockIdx.z : warp; r < R; r += SPREAD ? (int)gridDim.z : W) {
+    const int step = SPREAD ? W : 1;
+    float top = -INFINITY, sum = 0.f, acc[V] = {};
+    for (int base = from + (SPREAD ? warp : 0); base <= to; base += 32 * step) {   // 32 parts
+      const int n = min(32, (to - base) / step + 1), mine = base + lane * step;
+      auto part = [&](int x) { return p.parts + ((size_t)(2 * x + (x == from)) * R + r) * (HD + 4); };
+      const float2 ml = lane < n ? *reinterpret_cast<const float2*>(part(mine) + HD) : make_float2(-INFINITY, 0.f);
+      const float now = fmaxf(top, warp_max(ml.x)), f = now == -INFINITY ? 1.f : exp2f(top - now);   // (no score, or NaN only: zeros and NaN add up)
+      const float w = now == -INFINITY ? 1.f : exp2f(ml.x - now);
+      top = now;
+      sum = sum * f + warp_sum(ml.y * w);
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = part[lane + 32 * i];
-    const float now = fmaxf(top, ml.x), f = now == -INFINITY ? 1.f : exp2f(top - now), w = now == -INFINITY ? 1.f : exp2f(ml.x - now);   // (no score, or NaN only: zeros and NaN add up)
-    top = now;
-    sum = sum * f + ml.y * w;
+      for (int i = 0; i < V; ++i) acc[i] *= f;
+#pragma unroll 8
+      for (int x = 0; x < n; ++x) {
+        const float* at = part(base + x * step);
+        const float g = __shfl_sync(0xffffffffu, w, x);
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = acc[i] * f + v[i] * w;
-  }
-#pragma unroll
-  for (int i = 0; i < V; ++i) sums[warp][lane + 32 * i] = acc[i];
-  if (lane == 0) {
-    tops[warp] = top;
-    totals[warp] = sum;
-  }
-  __syncthreads();
-  for (int d = threadIdx.x; d < HD; d += kKv4JoinThreads) {
-    float most = -INFINITY, out = 0.f, total = 0.f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) most = fmaxf(most, tops[w]);
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float f = most == -INFINITY ? 1.f : exp2f(tops[w] - most);
-      out += sums[w][d] * f;
-      total += totals[w] * f;
+        for (int i = 0; i < V; ++i) acc[i] = fmaf(at[lane + 32 * i], g, acc[i]);
+      }
     }
-    p.out[((size_t)(b * p.Q + r / G) * p.heads + kvh * G + r % G) * HD + d] = f2bf(out * (total > 0.f ? 1.f / total : total == 0.f ? 0.f : total));
+    if constexpr (SPREAD) {
+      __syncthreads();   // (of the row in front, all is read)
+#pragma unroll
+      for (int i = 0; i < V; ++i) sums[warp][lane + 32 * i] = acc[i];
+      if (lane == 0) totals[warp] = make_float2(top, sum);
+      __syncthreads();
+      if (warp > 0) continue;
+      const float2 ml = lane < W ? totals[lane] : make_float2(-INFINITY, 0.f);
+      top = warp_max(ml.x);
+      const float w = top == -INFINITY ? 1.f : exp2f(ml.x - top);
+      sum = warp_sum(ml.y * w);
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] = 0.f;
+#pragma unroll
+      for (int x = 0; x < W; ++x) {
+        const float g = __shfl_sync(0xffffffffu, w, x);
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = fmaf(sums[x][lane + 32 * i], g, acc[i]);
+      }
+    }
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;   // (a row that sees no key is zero, NaN stays)
+    __nv_bfloat16* dst = p.out + ((size_t)(b * p.Q + r / G) * p.heads + kvh * G + r % G) * HD;
+#pragma unroll
+    for (int i = 0; i < V; ++i) dst[lane + 32 * i] = f2bf(acc[i] * inv);
   }
 }
 

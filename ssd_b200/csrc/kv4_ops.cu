@@ -57,13 +57,22 @@ static Kv4Plan kv4_plan(int64_t units, int64_t keys, int resident, int most, int
       plan.cluster = c;
     }
   }
-  if (may_share && least > 1536 && units * ((keys + turn - 1) / turn) < (1ll << 31)) plan.blocks = (int)std::min(std::min(slots, units * 64), units * ((keys + turn - 1) / turn));
+  // Equal stretches cost a second launch, but their time goes by the sum of all lengths, not by the longest, and more than the blocks of a cluster can share a head.  us, clusters and stretches: one context
+  // of 16000 (8 heads) 15.7 and 17.0, of 32000 25.7 and 22.3, of 64000 44.9 and 31.3, 4 of 32000 43.9 and 39.1, 16 of 8000 40.5 and 39.4, 48 of 16000 144 and 147; with a head or more to every
+  // place on the device blocks are dealt out as others end: 148 of 4000 105 and 126.
+  if (may_share && least > 2048 && units < slots && units * ((keys + turn - 1) / turn) < (1ll << 31)) plan.blocks = (int)std::min(std::min(slots, units * 64), units * ((keys + turn - 1) / turn));
   return plan;
 }
 constexpr int kKv4Warps = 4, kMaxShared = 1024;   // warps of a block; sequences of a shared launch (each block goes through their lengths)
 static Kv4Plan kv4_few_plan(int batch, int q_len, int heads, int kv_heads, int64_t keys) {
   const int tiles = (heads / kv_heads * q_len + 7) / 8;
   return kv4_plan((int64_t)batch * kv_heads, keys, 16 / tiles / kKv4Warps, kKv4Most, kKv4Warps * kKv4Keys, batch <= kMaxShared);
+}
+template <int HD, int KEYS>
+static int launch_join(Launcher& L, const Kv4AttnParams& p, int blocks) {
+  const int rows = p.heads / p.kv_heads * p.Q;
+  if (blocks > 8 * p.B * p.kv_heads) return L.go(kv4_join_kernel<HD, KEYS, true>, dim3(p.kv_heads, p.B, rows), dim3(kKv4JoinThreads), 0, p, blocks);
+  return L.go(kv4_join_kernel<HD, KEYS, false>, dim3(p.kv_heads, p.B), dim3(kKv4JoinThreads), 0, p, blocks);
 }
 template <int HD, int NT>
 static int launch_attn(Launcher& L, const Kv4AttnParams& p) {
@@ -74,7 +83,7 @@ static int launch_attn(Launcher& L, const Kv4AttnParams& p) {
     CKI(with_smem(kv4_attn_kernel<HD, NT, W, true>, smem, kSmemCarveout, done));
     if (!p.parts) return fail("paged_attn_kv4: null argument (scratch)");
     CKI(L.go(kv4_attn_kernel<HD, NT, W, true>, dim3(plan.blocks), dim3(W * 32), smem, p));
-    return L.go(kv4_join_kernel<HD, W * kKv4Keys>, dim3(p.heads / p.kv_heads * p.Q, p.kv_heads, p.B), dim3(kKv4JoinThreads), 0, p, plan.blocks);
+    return launch_join<HD, W * kKv4Keys>(L, p, plan.blocks);
   }
   static std::atomic<bool> done[64];
   CKI(with_smem(kv4_attn_kernel<HD, NT, W, false>, smem, kSmemClusters, done));
