@@ -13,11 +13,21 @@ namespace ssdk {
 constexpr int kv4_row_bytes(int HD) { return HD / 2 + 4; }   // of a token and head: codes and pair
 constexpr uint32_t kKv4Nan = 0x7fc07fc0u;
 
+#ifndef SSDK_HOST_EMU
+// 1 where a >= b, else 0
+SSDK_DEVINL float one_if_ge(float a, float b) {
+  float d;
+  asm("set.ge.f32.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+#endif
+
 // Codes of a row whose 16 x LPH values lie with LPH neighbouring lanes, 16 a lane in two pieces of eight.  code: a word of eight channels for each piece; pair: scale | minimum;
 // VALUES: the pieces become what the codes stand for.
 // A quotient is often a code and a half exactly (x - m has some sixteen bits, s has eight), where a product with 1 / s goes either way.  So the product is made with something below
 // 1 / s, which gives the code or the one in front of it, and what it leaves, x - m - code s, is exact in fp32 and decides.  The nearest whole number stands in the low bits of
-// (x - m) r + 1.5 2^23; these words are put together as they are, and their constant parts taken off at the end.
+// (x - m) r + 1.5 2^23; these words are put together as they are, and their constant parts taken off at the end.  Two values at once: seven instructions a value (32003 rows of 16 heads of 128
+// 105 us with one at a time, twice as many; see kv4_store_kernel).
 template <int LPH, bool VALUES>
 SSDK_DEVINL void kv4_codes(uint4& x, uint4& y, uint32_t (&code)[2], uint32_t& pair) {
   uint32_t w[2][4] = {{x.x, x.y, x.z, x.w}, {y.x, y.y, y.z, y.w}};
@@ -44,21 +54,24 @@ SSDK_DEVINL void kv4_codes(uint4& x, uint4& y, uint32_t (&code)[2], uint32_t& pa
   const float r = s > 0.f ? 1.f / s * (1.f - 0x1p-20f) : 0.f, half = s > 0.f ? 0.5f * s : INFINITY;
   constexpr float kWhole = 12582912.f;   // 1.5 2^23, the word 0x4b400000
   constexpr uint32_t kOff = 0x4b400000u * 0x11111111u;
+  const uint64_t one2 = pack2(1.f, 1.f), r2 = pack2(r, r), whole2 = pack2(kWhole, kWhole), less2 = pack2(-kWhole, -kWhole), minus_m2 = pack2(-m, -m), m2 = pack2(m, m), s2 = pack2(s, s), minus_s2 = pack2(-s, -s);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint32_t acc = 0;
 #pragma unroll
     for (int i = 3; i >= 0; --i) {
-      float v[2];
-#pragma unroll
-      for (int e = 1; e >= 0; --e) {
-        const float d = __uint_as_float(e ? w[h][i] & 0xffff0000u : w[h][i] << 16) - m;
-        const float u = fmaf(d, r, kWhole), c = u - kWhole;
-        const bool up = fmaf(-c, s, d) >= half;
-        acc = acc * 16u + __float_as_uint(u) + (up ? 1u : 0u);
-        if (VALUES) v[e] = fmaf(s, up ? c + 1.f : c, m);
+      const uint64_t d = fma2((uint64_t)(w[h][i] & 0xffff0000u) << 32 | w[h][i] << 16, one2, minus_m2), c = fma2(fma2(d, r2, whole2), one2, less2);
+      float e0, e1;
+      unpack2(fma2(c, minus_s2, d), &e0, &e1);
+      const uint64_t up = fma2(c, one2, pack2(one_if_ge(e0, half), one_if_ge(e1, half)));   // the codes
+      float u0, u1;
+      unpack2(fma2(up, one2, whole2), &u0, &u1);
+      acc = acc * 256u + (__float_as_uint(u1) * 16u + __float_as_uint(u0));
+      if (VALUES) {
+        float v0, v1;
+        unpack2(fma2(up, s2, m2), &v0, &v1);
+        w[h][i] = pack_bf16x2(v0, v1);
       }
-      if (VALUES) w[h][i] = pack_bf16x2(v[0], v[1]);
     }
     code[h] = fine ? acc - kOff : 0u;
   }
@@ -73,11 +86,11 @@ SSDK_DEVINL void kv4_codes(uint4& x, uint4& y, uint32_t (&code)[2], uint32_t& pa
 // as they are.  Queries are fp32 with one rounding.  A key is rounded to bf16 (what an unquantised cache would hold) and then quantised, and that rounding decides its code next to a
 // border: keys' norm and rotation are in 64 bits, so that codes are those of the definition whatever the order of sums.  (Keys are an eighth to a third of the heads.)
 // Bound by memory: 2 bytes read a channel, 2 written for queries and values that are asked for, 0.53 for codes.  HD / 16 lanes own a head, a warp takes groups of
-// 32 / (HD / 16) heads of one kind, the next group's loads in flight; the rows' groups lie one behind the other and each warp has a stretch of them.
+// 32 / (HD / 16) heads of a row (queries, keys, values behind one another), kKv4Ahead groups' loads in flight; the rows' groups lie one behind the other and each warp has a stretch of them.
 // A row with a position outside the table has NaN queries (and values) and stores nothing; slots outside the cache store nothing.
 // ----------------------------------------------------------------------------------
 struct Kv4StoreParams {
-  const __nv_bfloat16 *q, *k, *v;   // rows of heads
+  const __nv_bfloat16 *q, *k, *v;   // rows of heads; ROPE: of one array, q | k | v
   int64_t q_row, k_row, v_row;      // elements from row to row
   const int64_t* positions;         // [M]
   const int32_t* slots;             // [M]
@@ -88,10 +101,12 @@ struct Kv4StoreParams {
   int64_t top, num_slots;
   float eps;
   int M, heads, kv_heads, rot, block_size;
-  int q_groups, kv_groups;          // of heads that a warp takes at once, in a row
+  int groups;                       // of heads that a warp takes at once, in a row
   int warps, each, longer;          // the rows' groups one behind the other: a warp has a stretch of `each`, the first `longer` one more
 };
-constexpr int kKv4StoreThreads = 128;
+constexpr int kKv4StoreThreads = 128, kKv4Ahead = 2;
+constexpr int kv4_store_blocks(bool rope) { return rope ? 4 : 6; }   // resident on an SM
+constexpr int kv4_store_heads(int HD) { return 32 / (HD / 16); }   // of a group
 
 SSDK_DEVINL double shfl_xor_f64(double v, int o) {
   union { double d; uint32_t w[2]; } u;
@@ -101,44 +116,96 @@ SSDK_DEVINL double shfl_xor_f64(double v, int o) {
   return u.d;
 }
 
-// norm (weights w0, w1 of the two pieces, or none) and rotation of a lane's two pieces in T, rounded to bf16 by way of fp32
-template <typename T, int LPH>
-SSDK_DEVINL void kv4_turn(uint4& x, uint4& y, const __nv_bfloat16* w0, const __nv_bfloat16* w1, float eps, bool turns, const float (&co)[8], const float (&si)[8]) {
+// norm (weights w0, w1 of the two pieces, or none) and rotation of a lane's two pieces: in 64 bits, rounded to bf16 by way of fp32
+template <int LPH>
+SSDK_DEVINL void kv4_turn_f64(uint4& x, uint4& y, const __nv_bfloat16* w0, const __nv_bfloat16* w1, float eps, bool turns, const uint64_t (&co)[4], const uint64_t (&si)[4]) {
   float a[8], b[8];
   unpack_bf16x8(x, a);
   unpack_bf16x8(y, b);
-  T scale = 1;
+  double scale = 1;
   float wa[8], wb[8];
   if (w0) {   // (the whole warp)
-    T sum = 0;
+    double sum = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += (T)a[i] * (T)a[i] + (T)b[i] * (T)b[i];
+    for (int i = 0; i < 8; ++i) sum += (double)a[i] * (double)a[i] + (double)b[i] * (double)b[i];
 #pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1) {
-      if constexpr (sizeof(T) == 8) sum += shfl_xor_f64(sum, o);
-      else sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    }
-    if constexpr (sizeof(T) == 8) scale = 1.0 / sqrt(sum / (16.0 * LPH) + (double)eps);
-    else scale = rsqrtf(sum / (16.f * LPH) + eps);
+    for (int o = LPH / 2; o > 0; o >>= 1) sum += shfl_xor_f64(sum, o);
+    scale = 1.0 / sqrt(sum / (16.0 * LPH) + (double)eps);
     unpack_bf16x8(*reinterpret_cast<const uint4*>(w0), wa);
     unpack_bf16x8(*reinterpret_cast<const uint4*>(w1), wb);
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    T u = a[i], v = b[i];
+    double u = a[i], v = b[i];
     if (w0) {
-      u = u * scale * (T)wa[i];
-      v = v * scale * (T)wb[i];
+      u = u * scale * (double)wa[i];
+      v = v * scale * (double)wb[i];
     }
-    a[i] = (float)(turns ? u * (T)co[i] - v * (T)si[i] : u);
-    b[i] = (float)(turns ? v * (T)co[i] + u * (T)si[i] : v);
+    float c[2], s[2];
+    unpack2(co[i >> 1], &c[0], &c[1]);
+    unpack2(si[i >> 1], &s[0], &s[1]);
+    a[i] = (float)(turns ? u * (double)c[i & 1] - v * (double)s[i & 1] : u);
+    b[i] = (float)(turns ? v * (double)c[i & 1] + u * (double)s[i & 1] : v);
   }
   x = pack_bf16x8(a);
   y = pack_bf16x8(b);
 }
+// the same in fp32, two values at once
+template <int LPH>
+SSDK_DEVINL void kv4_turn_f32(uint4& x, uint4& y, const __nv_bfloat16* w0, const __nv_bfloat16* w1, float eps, bool turns, const uint64_t (&co)[4], const uint64_t (&si)[4]) {
+  auto pairs = [](const uint4& v, uint64_t* f) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = (uint64_t)(w[i] & 0xffff0000u) << 32 | w[i] << 16;
+  };
+  auto rounded = [](const uint64_t* f) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      unpack2(f[i], &a, &b);
+      w[i] = pack_bf16x2(a, b);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  uint64_t a[4], b[4];
+  pairs(x, a);
+  pairs(y, b);
+  if (w0) {
+    uint64_t sum2 = mul2(a[0], a[0]);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) sum2 = fma2(a[i], a[i], sum2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum2 = fma2(b[i], b[i], sum2);
+    float s0, s1;
+    unpack2(sum2, &s0, &s1);
+    s0 += s1;
+#pragma unroll
+    for (int o = LPH / 2; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+    const float scale = rsqrtf(s0 / (16.f * LPH) + eps);
+    const uint64_t scale2 = pack2(scale, scale);
+    uint64_t w[4];
+    pairs(*reinterpret_cast<const uint4*>(w0), w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = mul2(mul2(a[i], scale2), w[i]);
+    pairs(*reinterpret_cast<const uint4*>(w1), w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = mul2(mul2(b[i], scale2), w[i]);
+  }
+  if (turns) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t t = fma2(a[i], co[i], mul2(b[i], si[i] ^ 0x8000000080000000ull));
+      b[i] = fma2(b[i], co[i], mul2(a[i], si[i]));
+      a[i] = t;
+    }
+  }
+  x = rounded(a);
+  y = rounded(b);
+}
 
 template <int HD, bool ROPE, bool VALUES>
-__global__ void __launch_bounds__(kKv4StoreThreads, 4) kv4_store_kernel(Kv4StoreParams p) {
+__global__ void __launch_bounds__(kKv4StoreThreads, kv4_store_blocks(ROPE)) kv4_store_kernel(const __grid_constant__ Kv4StoreParams p) {
   constexpr int LPH = HD / 16, SIDE = 32 / LPH;   // lanes of a head, heads side by side
   pdl_wait();
   pdl_launch_dependents();
@@ -146,30 +213,41 @@ __global__ void __launch_bounds__(kKv4StoreThreads, 4) kv4_store_kernel(Kv4Store
   if (warp >= p.warps) return;
   int unit = warp * p.each + min(warp, p.longer);   // (below 2^31: the host sees to it)
   const int last = unit + p.each + (warp < p.longer);
-  const int piece = threadIdx.x % LPH, side = threadIdx.x % 32 / LPH, half = p.rot / 2, groups = p.q_groups + 2 * p.kv_groups;
+  const int piece = threadIdx.x % LPH, side = threadIdx.x % 32 / LPH, half = p.rot / 2;
+  const int first_k = ROPE ? p.heads : 0, first_v = first_k + p.kv_heads, end = first_v + p.kv_heads;   // of a row's heads
   const bool turns = ROPE && piece < p.rot / 16;
   // channels of a lane's pieces: of heads that turn, and of others
   const int t0 = turns ? piece * 8 : p.rot + (piece - p.rot / 16) * 16, t1 = turns ? half + piece * 8 : t0 + 8;
+  const int record = p.block_size * kv4_row_bytes(HD);   // bytes of a page and head
 
-  uint4 a, b;
-  auto load = [&](int m, int group) {
-    const int kind = group < p.q_groups ? 0 : group < p.q_groups + p.kv_groups ? 1 : 2;
-    const int head = (group - (kind ? p.q_groups : 0) - (kind == 2 ? p.kv_groups : 0)) * SIDE + side;
-    const __nv_bfloat16* row = kind == 0 ? p.q + m * p.q_row : kind == 1 ? p.k + m * p.k_row : p.v + m * p.v_row;
-    const bool turned = ROPE && kind != 2;
-    a = b = make_uint4(0, 0, 0, 0);
-    if (head < (kind == 0 ? p.heads : p.kv_heads)) {
-      a = ld_nc_v4(row + head * HD + (turned ? t0 : piece * 16));
-      b = ld_nc_v4(row + head * HD + (turned ? t1 : piece * 16 + 8));
+  uint4 a[kKv4Ahead], b[kKv4Ahead];
+  int at_m = unit / p.groups, at_head = (unit - at_m * p.groups) * SIDE + side;   // row and head that are asked for next
+  auto load = [&](uint4& x, uint4& y) {
+    x = y = make_uint4(0, 0, 0, 0);
+    if (at_head < end) {
+      const bool value = at_head >= first_v;
+      const __nv_bfloat16* src;
+      if (ROPE) src = p.q + at_m * p.q_row + at_head * HD;
+      else src = value ? p.v + at_m * p.v_row + (at_head - first_v) * HD : p.k + at_m * p.k_row + at_head * HD;
+      const bool turned = ROPE && !value;
+      x = ld_nc_v4(src + (turned ? t0 : piece * 16));
+      y = ld_nc_v4(src + (turned ? t1 : piece * 16 + 8));
+    }
+    at_head += SIDE;
+    if (at_head - side >= p.groups * SIDE) {
+      at_head = side;
+      ++at_m;
     }
   };
-  int m = unit / groups, group = unit - m * groups, row = -1;
-  if (unit < last) load(m, group);
+  int m = at_m, head0 = at_head - side, row = -1;
+#pragma unroll
+  for (int i = 0; i < kKv4Ahead; ++i)
+    if (unit + i < last) load(a[i], b[i]);
   bool known = true, stores = false;
-  float co[8] = {}, si[8] = {};
-  size_t page = 0;
+  uint64_t co[4] = {}, si[4] = {};
+  uint8_t *k_page = p.k_cache, *v_page = p.v_cache;   // of the row's slot: its codes in the page of the first head
   int off = 0;
-  for (; unit < last; ++unit) {
+  auto work = [&](uint4& next_x, uint4& next_y) {
     if (m != row) {
       row = m;
       const int slot = p.slots[m];
@@ -180,46 +258,86 @@ __global__ void __launch_bounds__(kKv4StoreThreads, 4) kv4_store_kernel(Kv4Store
         if (turns && known) {
           const float* angles = p.table + (size_t)at * p.rot + piece * 8;
 #pragma unroll
-          for (int i = 0; i < 8; i += 4) {
-            const float4 c = *reinterpret_cast<const float4*>(angles + i), s = *reinterpret_cast<const float4*>(angles + half + i);
-            co[i] = c.x; co[i + 1] = c.y; co[i + 2] = c.z; co[i + 3] = c.w;
-            si[i] = s.x; si[i + 1] = s.y; si[i + 2] = s.z; si[i + 3] = s.w;
+          for (int i = 0; i < 4; i += 2) {
+            const float4 c = *reinterpret_cast<const float4*>(angles + 2 * i), s = *reinterpret_cast<const float4*>(angles + half + 2 * i);
+            co[i] = pack2(c.x, c.y); co[i + 1] = pack2(c.z, c.w);
+            si[i] = pack2(s.x, s.y); si[i + 1] = pack2(s.z, s.w);
           }
         }
       }
       stores = known && slot >= 0 && slot < p.num_slots;
-      page = stores ? slot / p.block_size : 0;
-      off = stores ? slot - (int)page * p.block_size : 0;
+      if (stores) {
+        const int page = slot / p.block_size;
+        off = slot - page * p.block_size;
+        const int64_t at = (int64_t)page * p.kv_heads * record;
+        k_page = p.k_cache + at;
+        v_page = p.v_cache + at;
+      }
     }
-    uint4 x = a, y = b;
-    const int kind = group < p.q_groups ? 0 : group < p.q_groups + p.kv_groups ? 1 : 2;
-    const int head = (group - (kind ? p.q_groups : 0) - (kind == 2 ? p.kv_groups : 0)) * SIDE + side;
-    const bool there = head < (kind == 0 ? p.heads : p.kv_heads);
-    if (++group == groups) {
-      group = 0;
+    uint4 x = next_x, y = next_y;
+    const int head = head0 + side;
+    const bool key = head >= first_k && head < first_v, value = head >= first_v, there = head < end;
+    const bool some_q = ROPE && head0 < first_k, some_k = head0 < first_v && head0 + SIDE > first_k, some_kv = head0 + SIDE > first_k;   // (of the warp's heads)
+    head0 += SIDE;
+    if (head0 >= p.groups * SIDE) {
+      head0 = 0;
       ++m;
     }
-    if (unit + 1 < last) load(m, group);
-    const bool turned = ROPE && kind != 2;
+    if (unit + kKv4Ahead < last) load(next_x, next_y);
+    const bool turned = ROPE && !value;
     const int c0 = turned ? t0 : piece * 16, c1 = turned ? t1 : piece * 16 + 8;
-    if (ROPE && kind == 0) kv4_turn<float, LPH>(x, y, p.q_norm_w ? p.q_norm_w + c0 : nullptr, p.q_norm_w ? p.q_norm_w + c1 : nullptr, p.eps, turns, co, si);
-    if (ROPE && kind == 1) kv4_turn<double, LPH>(x, y, p.k_norm_w ? p.k_norm_w + c0 : nullptr, p.k_norm_w ? p.k_norm_w + c1 : nullptr, p.eps, turns, co, si);
+    if (some_q) {
+      uint4 u = x, v = y;
+      kv4_turn_f32<LPH>(u, v, p.q_norm_w ? p.q_norm_w + t0 : nullptr, p.q_norm_w ? p.q_norm_w + t1 : nullptr, p.eps, turns, co, si);
+      if (head < first_k) {
+        x = u;
+        y = v;
+      }
+    }
+    if (ROPE && some_k) {
+      uint4 u = x, v = y;
+      kv4_turn_f64<LPH>(u, v, p.k_norm_w ? p.k_norm_w + t0 : nullptr, p.k_norm_w ? p.k_norm_w + t1 : nullptr, p.eps, turns, co, si);
+      if (key) {
+        x = u;
+        y = v;
+      }
+    }
     uint32_t code[2], pair;
-    if (kind) kv4_codes<LPH, VALUES>(x, y, code, pair);
+    if (some_kv) {
+      uint4 u = x, v = y;
+      kv4_codes<LPH, VALUES>(u, v, code, pair);
+      if (VALUES && (key || value)) {
+        x = u;
+        y = v;
+      }
+    }
     if (ROPE && !known) x = y = make_uint4(kKv4Nan, kKv4Nan, kKv4Nan, kKv4Nan);
-    if (!there) continue;
-    if (kind == 0 || VALUES) {
-      __nv_bfloat16* dst = kind == 0 ? p.q_out + ((size_t)row * p.heads + head) * HD : (kind == 1 ? p.k_values : p.v_values) + ((size_t)row * p.kv_heads + head) * HD;
+    if (!there) return;
+    const int kv_head = head - (value ? first_v : first_k);
+    if (!(key || value) || VALUES) {
+      __nv_bfloat16* dst = key ? p.k_values + ((size_t)row * p.kv_heads + kv_head) * HD : value ? p.v_values + ((size_t)row * p.kv_heads + kv_head) * HD : p.q_out + ((size_t)row * p.heads + head) * HD;
       *reinterpret_cast<uint4*>(dst + c0) = x;
       *reinterpret_cast<uint4*>(dst + c1) = y;
     }
-    if (kind && stores) {
-      uint8_t* at = (kind == 1 ? p.k_cache : p.v_cache) + (page * p.kv_heads + head) * ((size_t)p.block_size * kv4_row_bytes(HD));
-      uint8_t* codes = at + (size_t)off * (HD / 2);
-      *reinterpret_cast<uint32_t*>(codes + c0 / 2) = code[0];
-      *reinterpret_cast<uint32_t*>(codes + c1 / 2) = code[1];
-      if (piece == 0) *reinterpret_cast<uint32_t*>(at + (size_t)p.block_size * (HD / 2) + off * 4) = pair;
+    if ((key || value) && stores) {
+      uint8_t* at = (value ? v_page : k_page) + (int64_t)kv_head * record;
+      uint8_t* codes = at + off * (HD / 2);
+      if (turned) {
+        *reinterpret_cast<uint32_t*>(codes + c0 / 2) = code[0];
+        *reinterpret_cast<uint32_t*>(codes + c1 / 2) = code[1];
+      } else {
+        *reinterpret_cast<uint2*>(codes + c0 / 2) = make_uint2(code[0], code[1]);
+      }
+      if (piece == 0) *reinterpret_cast<uint32_t*>(at + p.block_size * (HD / 2) + off * 4) = pair;
     }
+  };
+  while (unit < last) {
+#pragma unroll
+    for (int i = 0; i < kKv4Ahead; ++i)
+      if (unit < last) {
+        work(a[i], b[i]);
+        ++unit;
+      }
   }
 }
 

@@ -25,12 +25,11 @@ static int64_t kv4_bytes(int64_t num_blocks, int block_size, int kv_heads, int h
 
 template <int HD, bool ROPE, bool VALUES>
 static int launch_store(Launcher& L, Kv4StoreParams p) {
-  constexpr int SIDE = 32 / (HD / 16), W = kKv4StoreThreads / 32;
-  p.q_groups = ROPE ? (p.heads + SIDE - 1) / SIDE : 0;
-  p.kv_groups = (p.kv_heads + SIDE - 1) / SIDE;
-  const int64_t units = (int64_t)p.M * (p.q_groups + 2 * p.kv_groups);
+  constexpr int SIDE = kv4_store_heads(HD), W = kKv4StoreThreads / 32;
+  p.groups = ((ROPE ? p.heads : 0) + 2 * p.kv_heads + SIDE - 1) / SIDE;
+  const int64_t units = (int64_t)p.M * p.groups;
   if (units >= (1ll << 31)) return fail("store_kv4: %d rows of %d heads", p.M, p.heads + 2 * p.kv_heads);
-  p.warps = (int)std::min<int64_t>(units, kSms * 4 * W);   // four blocks on an SM
+  p.warps = (int)std::min<int64_t>(units, kSms * kv4_store_blocks(ROPE) * W);
   p.each = (int)(units / p.warps);
   p.longer = (int)(units - (int64_t)p.each * p.warps);
   return L.go(kv4_store_kernel<HD, ROPE, VALUES>, dim3((unsigned)((p.warps + W - 1) / W)), dim3(kKv4StoreThreads), 0, p);

@@ -13,6 +13,9 @@ inline uint32_t __float_as_uint(float f) {
   return u;
 }
 #include "pairs_emu.h"
+namespace ssdk {
+inline float one_if_ge(float a, float b) { return a >= b ? 1.f : 0.f; }
+}  // namespace ssdk
 #include "../../ssd_b200/csrc/kv4.cuh"
 
 #include <fstream>
@@ -37,10 +40,9 @@ static void wr(std::ofstream& o, const Exact<T>& v) { o.write(reinterpret_cast<c
 
 template <int HD, bool ROPE, bool VALUES>
 static void store(ssdk::Kv4StoreParams p, int most) {
-  constexpr int SIDE = 32 / (HD / 16);
-  p.q_groups = (p.heads + SIDE - 1) / SIDE;
-  p.kv_groups = (p.kv_heads + SIDE - 1) / SIDE;
-  const int units = p.M * (p.q_groups + 2 * p.kv_groups);
+  constexpr int SIDE = ssdk::kv4_store_heads(HD);
+  p.groups = (p.heads + 2 * p.kv_heads + SIDE - 1) / SIDE;
+  const int units = p.M * p.groups;
   p.warps = std::min(units, most);
   p.each = units / p.warps;
   p.longer = units % p.warps;
