@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(kKv4JoinThreads, 2) kv4_join_kernel(const __gr
   const Kv4Stretch stretch(heads.x * p.kv_heads, blocks);
   const int turns = kv4_turns<KEYS>(p, b), first = heads.y * p.kv_heads + kvh * turns, from = stretch.block(first), to = stretch.block(first + turns - 1);
   if (from == to) return;   // (the whole block)
-  for (int r = SPREAD ? (int)blockIdx.z : warp; r < R; r += SPREAD ? (int)gridDim.z : W) {
+  for (int r = SPREAD ? (int)blockIdx.z : (int)blockIdx.z * W + warp; r < R; r += SPREAD ? (int)gridDim.z : (int)gridDim.z * W) {
     const int step = SPREAD ? W : 1;
     float top = -INFINITY, sum = 0.f, acc[V] = {};
     for (int base = from + (SPREAD ? warp : 0); base <= to; base += 32 * step) {   // 32 parts

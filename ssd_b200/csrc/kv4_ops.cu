@@ -45,7 +45,7 @@ static int store(const Kv4StoreParams& p, int head_dim, void* stream) {
 struct Kv4Plan {
   int cluster, blocks;   // blocks: of a shared launch, 0 where clusters do
 };
-static Kv4Plan kv4_plan(int64_t units, int64_t keys, int resident, int most, int turn, bool may_share) {
+static Kv4Plan kv4_plan(int64_t units, int64_t keys, int resident, int most, int turn, int64_t share_from, bool may_share) {
   Kv4Plan plan = {1, 0};
   const int64_t slots = resident * kSms;
   int64_t least = INT64_MAX;
@@ -59,19 +59,31 @@ static Kv4Plan kv4_plan(int64_t units, int64_t keys, int resident, int most, int
   // Equal stretches cost a second launch, but their time goes by the sum of all lengths, not by the longest, and more than the blocks of a cluster can share a head.  us, clusters and stretches: one context
   // of 16000 (8 heads) 15.7 and 17.0, of 32000 25.7 and 22.3, of 64000 44.9 and 31.3, 4 of 32000 43.9 and 39.1, 16 of 8000 40.5 and 39.4, 48 of 16000 144 and 147; with a head or more to every
   // place on the device blocks are dealt out as others end: 148 of 4000 105 and 126.
-  if (may_share && least > 2048 && units < slots && units * ((keys + turn - 1) / turn) < (1ll << 31)) plan.blocks = (int)std::min(std::min(slots, units * 64), units * ((keys + turn - 1) / turn));
+  if (may_share && least > share_from && units < slots && units * ((keys + turn - 1) / turn) < (1ll << 31)) plan.blocks = (int)std::min(std::min(slots, units * 64), units * ((keys + turn - 1) / turn));
   return plan;
 }
 constexpr int kKv4Warps = 4, kMaxShared = 1024;   // warps of a block; sequences of a shared launch (each block goes through their lengths)
 static Kv4Plan kv4_few_plan(int batch, int q_len, int heads, int kv_heads, int64_t keys) {
   const int tiles = (heads / kv_heads * q_len + 7) / 8;
-  return kv4_plan((int64_t)batch * kv_heads, keys, 16 / tiles / kKv4Warps, kKv4Most, kKv4Warps * kKv4Keys, batch <= kMaxShared);
+  return kv4_plan((int64_t)batch * kv_heads, keys, 16 / tiles / kKv4Warps, kKv4Most, kKv4Warps * kKv4Keys, 2048, batch <= kMaxShared);
+}
+// of tiles: up to 64 rows lie in one twice
+static int kv4_tile_tokens(int q_len, int group, int* tiles) {
+  const int most = (group * q_len <= 64 ? kKv4TileRows / 2 : kKv4TileRows) / group;
+  *tiles = (q_len + most - 1) / most;
+  return (q_len + *tiles - 1) / *tiles;
+}
+static Kv4Plan kv4_tile_plan(int batch, int q_len, int heads, int kv_heads, int head_dim, int64_t keys) {
+  int tiles;
+  kv4_tile_tokens(q_len, heads / kv_heads, &tiles);
+  const int most = head_dim == 64 && heads / kv_heads * q_len <= 64 ? 8 : kKv4Most;   // (their join has a lane of HD / 4 for each part)
+  return kv4_plan((int64_t)batch * kv_heads * tiles, keys, 2, most, kKv4TileKeys, 1280, tiles == 1 && batch <= kMaxShared);
 }
 template <int HD, int KEYS>
 static int launch_join(Launcher& L, const Kv4AttnParams& p, int blocks) {
   const int rows = p.heads / p.kv_heads * p.Q;
   if (blocks > 8 * p.B * p.kv_heads) return L.go(kv4_join_kernel<HD, KEYS, true>, dim3(p.kv_heads, p.B, rows), dim3(kKv4JoinThreads), 0, p, blocks);
-  return L.go(kv4_join_kernel<HD, KEYS, false>, dim3(p.kv_heads, p.B), dim3(kKv4JoinThreads), 0, p, blocks);
+  return L.go(kv4_join_kernel<HD, KEYS, false>, dim3(p.kv_heads, p.B, (rows + kKv4JoinThreads / 32 - 1) / (kKv4JoinThreads / 32)), dim3(kKv4JoinThreads), 0, p, blocks);
 }
 template <int HD, int NT>
 static int launch_attn(Launcher& L, const Kv4AttnParams& p) {
@@ -91,20 +103,27 @@ static int launch_attn(Launcher& L, const Kv4AttnParams& p) {
 }
 template <int HD, bool TWIN>
 static int launch_tiles(Launcher& L, const Kv4AttnParams& a) {
-  static std::atomic<bool> done[64];
-  CKI(with_smem(kv4_tile_kernel<HD, TWIN>, kv4_tile_smem(HD), kSmemClusters, done));
   WaitWord* waits = op_waits();
   if (!waits) return fail("paged_attn_kv4: pinned word for bounded waits not allocated");
   CKI(waits->check("an earlier call of attention without an engine left is not complete (NaN rows)"));
   Kv4TileParams p;
+  int tiles;
   p.a = a;
-  const int most = kKv4TileRows / (TWIN ? 2 : 1) / (a.heads / a.kv_heads), tiles = (a.Q + most - 1) / most;
-  if (tiles > 65535) return fail("paged_attn_kv4: q_len=%d", a.Q);
-  p.tokens = (a.Q + tiles - 1) / tiles;
+  p.tokens = kv4_tile_tokens(a.Q, a.heads / a.kv_heads, &tiles);
   p.timeout = waits->word;
-  const int blocks = TWIN && HD == 64 ? 8 : kKv4Most;   // (their join has a lane of HD / 4 for each part)
-  L.cluster = kv4_plan((int64_t)a.B * a.kv_heads * tiles, (int64_t)a.max_blocks * a.block_size, 2, blocks, kKv4TileKeys, false).cluster;
-  return L.go(kv4_tile_kernel<HD, TWIN>, dim3(a.kv_heads * L.cluster, a.B, tiles), dim3(kKv4TileThreads), kv4_tile_smem(HD), p);
+  if (tiles > 65535) return fail("paged_attn_kv4: q_len=%d", a.Q);
+  const Kv4Plan plan = kv4_tile_plan(a.B, a.Q, a.heads, a.kv_heads, HD, (int64_t)a.max_blocks * a.block_size);
+  if (plan.blocks) {
+    static std::atomic<bool> done[64];
+    CKI(with_smem(kv4_tile_kernel<HD, TWIN, true>, kv4_tile_smem(HD), kSmemCarveout, done));
+    if (!a.parts) return fail("paged_attn_kv4: null argument (scratch)");
+    CKI(L.go(kv4_tile_kernel<HD, TWIN, true>, dim3(plan.blocks), dim3(kKv4TileThreads), kv4_tile_smem(HD), p));
+    return launch_join<HD, kKv4TileKeys>(L, a, plan.blocks);
+  }
+  static std::atomic<bool> done[64];
+  CKI(with_smem(kv4_tile_kernel<HD, TWIN, false>, kv4_tile_smem(HD), kSmemClusters, done));
+  L.cluster = plan.cluster;
+  return L.go(kv4_tile_kernel<HD, TWIN, false>, dim3(a.kv_heads * L.cluster, a.B, tiles), dim3(kKv4TileThreads), kv4_tile_smem(HD), p);
 }
 
 extern "C" {
@@ -171,10 +190,12 @@ int ssdk_load_kv4(const void* k_cache, const void* v_cache, const int32_t* slot_
 }
 
 int64_t ssdk_paged_attn_kv4_scratch_bytes(int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size, int max_blocks_per_seq) {
-  if (batch < 1 || q_len < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || block_size < 1 || max_blocks_per_seq < 1) return 0;
+  if (batch < 1 || q_len < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || heads / kv_heads > 32 || head_dim < 1 || block_size < 1 || max_blocks_per_seq < 1) return 0;
   const int64_t rows = (int64_t)(heads / kv_heads) * q_len;
-  if (rows > 16) return 0;
-  return 8ll * kv4_few_plan(batch, q_len, heads, kv_heads, (int64_t)max_blocks_per_seq * block_size).blocks * rows * (head_dim + 4);
+  if (rows >= (1ll << 31) - 65536) return 0;
+  const int64_t keys = (int64_t)max_blocks_per_seq * block_size;
+  const Kv4Plan plan = rows <= 16 ? kv4_few_plan(batch, q_len, heads, kv_heads, keys) : kv4_tile_plan(batch, q_len, heads, kv_heads, head_dim, keys);
+  return 8ll * plan.blocks * rows * (head_dim + 4);
 }
 int ssdk_paged_attn_kv4(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables, const int32_t* context_lens,
                         void* out, void* scratch, int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size, int max_blocks_per_seq,

@@ -65,7 +65,8 @@ struct Kv4TileParams {
   unsigned* timeout;             // (rows whose waits ran out are NaN)
 };
 
-template <int HD, bool TWIN>
+// SHARED: calls of one tile, whose blocks have equal stretches of all sequences' keys (kv4_attn_kernel, kv4_join_kernel; a turn is a chunk), one head's piece after another
+template <int HD, bool TWIN, bool SHARED>
 __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __grid_constant__ Kv4TileParams pp) {
   namespace cg = cooperative_groups;
   constexpr int HALVES = HD / 64, CODES = HD / 2, K = kKv4TileKeys;
@@ -82,9 +83,10 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
   uint8_t* sK = sQ + HALVES * kQHalf;
   uint8_t* sV = sK + 2 * kKTile;
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = cluster.num_blocks(), rank = cluster.block_rank();
+  const int C = SHARED ? 1 : (int)cluster.num_blocks(), rank = SHARED ? 0 : (int)cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kvh = blockIdx.x / C, b = blockIdx.y, tile = (int)gridDim.z - 1 - (int)blockIdx.z;   // (the tiles that see most keys first)
+  int kvh = blockIdx.x / C, b = blockIdx.y;
+  const int tile = SHARED ? 0 : (int)gridDim.z - 1 - (int)blockIdx.z;   // (the tiles that see most keys first)
   const int G = p.heads / p.kv_heads, tok0 = tile * pp.tokens, tq = min(pp.tokens, p.Q - tok0), rows = tq * G;
   const int half = (rows + 31) & ~31;                // rows of the warps that have some
   const int live = TWIN ? 2 * half : half;           // threads that hand P over
@@ -105,14 +107,54 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     tmem_relinquish();
   }
   pdl_wait();
+  // SHARED: this block's turns at .. end, the first of them turn `turn` of its head
+  int at = 0, end = 1, turn = 0, turns = 0, done = 0;   // done: chunks of the pieces before (of stages and barriers)
+  if constexpr (SHARED) {
+    const Kv4Stretch stretch(kv4_turns_of_all<K>(p, 0).x * p.kv_heads, gridDim.x);
+    at = stretch.first(blockIdx.x);
+    end = stretch.first(blockIdx.x + 1);
+    if (at >= end) {   // nothing to do but to give the tensor memory back
+      __syncthreads();
+      pdl_launch_dependents();
+      if (warp == 8) tmem_dealloc(tmem_slot, 256);
+      return;
+    }
+    int before;
+    b = kv4_sequence_of<K>(p, at, &before);
+    turns = kv4_turns<K>(p, b);
+    const int from = at - before * p.kv_heads;
+    kvh = from / turns;
+    turn = from - kvh * turns;
+  }
+  uint32_t tmem = 0;
+#pragma unroll 1
+  for (bool again = false; at < end; again = true) {
+  if constexpr (SHARED) {
+    if (again) {
+      turn = 0;
+      if (++kvh == p.kv_heads) {
+        kvh = 0;
+        turns = kv4_turns<K>(p, ++b);
+      }
+    }
+  }
+  const int last_turn = SHARED ? min(turns, turn + (end - at)) : 0;
   // Queries: HD / 8 lanes a row, eight channels each.  Heads of 128: high and low parts in halves of their own, heads of 64: in a row's 128 bytes behind one another (the keys' codes stand there twice).
   // Rows behind the last one are zero.
-  constexpr int LPR = HD / 8;
-#pragma unroll 1
-  for (int i = threadIdx.x; i < kKv4TileRows * LPR; i += kKv4TileThreads) {   // (a warp's lanes stay together: both numbers are multiples of 32)
-    const int at = i / LPR, c = i % LPR, r = TWIN ? at & 63 : at;
+  constexpr int LPR = HD / 8, PIECES = (TWIN ? 64 : kKv4TileRows) * LPR, LOADS = (PIECES + kKv4TileThreads - 1) / kKv4TileThreads;
+  uint4 q_now[LOADS];
+#pragma unroll
+  for (int x = 0; x < LOADS; ++x) {
+    const int i = x * kKv4TileThreads + (int)threadIdx.x, r = i / LPR;
+    q_now[x] = make_uint4(0, 0, 0, 0);
+    if (r < rows) q_now[x] = ld_nc_v4(p.q + ((size_t)(b * p.Q + tok0 + r / G) * p.heads + kvh * G + r % G) * HD + i % LPR * 8);
+  }
+#pragma unroll
+  for (int x = 0; x < LOADS; ++x) {
+    const int i = x * kKv4TileThreads + (int)threadIdx.x, r = i / LPR, c = i % LPR;
+    if (i >= PIECES) break;   // (a warp's lanes stay together: both numbers are multiples of 32)
     float f[8], sum = 0.f, top = 0.f;
-    unpack_bf16x8(r < rows ? *reinterpret_cast<const uint4*>(p.q + ((size_t)(b * p.Q + tok0 + r / G) * p.heads + kvh * G + r % G) * HD + c * 8) : make_uint4(0, 0, 0, 0), f);
+    unpack_bf16x8(q_now[x], f);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       sum += f[j];
@@ -129,28 +171,34 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     uint2 high, low;
     e4m3_twice(even, &high.x, &low.x);
     e4m3_twice(odd, &high.y, &low.y);
-    uint8_t* to = sQ + swizzled(at, c >> 1) + (c & 1) * 8;
-    *reinterpret_cast<uint2*>(to) = high;
-    if (HD == 128) *reinterpret_cast<uint2*>(to + kQHalf) = low;
-    else *reinterpret_cast<uint2*>(sQ + swizzled(at, 4 + (c >> 1)) + (c & 1) * 8) = low;
-    if (c == 0) row_units[at] = fabsf(sum) < INFINITY && e < 255 ? make_float2(unit, sum / unit) : make_float2(__uint_as_float(kKv4Nan), 0.f);
+#pragma unroll
+    for (int at_row = r; at_row < kKv4TileRows; at_row += TWIN ? 64 : kKv4TileRows) {
+      uint8_t* to = sQ + swizzled(at_row, c >> 1) + (c & 1) * 8;
+      *reinterpret_cast<uint2*>(to) = high;
+      if (HD == 128) *reinterpret_cast<uint2*>(to + kQHalf) = low;
+      else *reinterpret_cast<uint2*>(sQ + swizzled(at_row, 4 + (c >> 1)) + (c & 1) * 8) = low;
+      if (c == 0) row_units[at_row] = fabsf(sum) < INFINITY && e < 255 ? make_float2(unit, sum / unit) : make_float2(__uint_as_float(kKv4Nan), 0.f);
+    }
   }
   fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot, tmem_o = tmem + 128;   // S / P buffers at columns 0 and 64, O behind them
+  tmem = tmem_slot;
+  const uint32_t tmem_o = tmem + 128;   // S / P buffers at columns 0 and 64, O behind them
   pdl_launch_dependents();   // (this block has its tensor memory: what is scheduled now may take the rest of the SM's and wait for this grid)
 
   const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size), ctx = len - p.Q + tok0;
   const int seen = max(0, min(len, ctx + tq)), seen_by_all = ctx + 1;   // positions that some row sees, that all do
-  const int chunks = (seen + K - 1) / K, n = rank < chunks ? (chunks - rank + C - 1) / C : 0;   // chunk i of this block is rank + i C
-  // Chunk i is in stage and on barriers i & 1, parity(i) is that use's.  A wait by parity is only right while the barrier is in that use or the one behind it:
+  const int chunks = (seen + K - 1) / K, front = SHARED ? turn : rank;   // chunk i of this piece is front + i C
+  const int n = SHARED ? max(0, min(chunks, last_turn) - turn) : front < chunks ? (chunks - front + C - 1) / C : 0;
+  // Chunk i is in stage and on barriers use(i), parity(i) is that use's.  A wait by parity is only right while the barrier is in that use or the one behind it:
   //   k_full, v_full: whoever waits for chunk i has to be through with it before its stage is written anew (the keys' behind s_full, the values' behind pv_done, which needs every row's P).
   //   s_full: the producers and the rows ask for chunk i, and chunk i + 2's needs keys of the former and, through p_full, P of the latter.
   //   p_full: chunk i + 2's needs the rows to have seen its scores, which are issued behind the product of chunk i.
   //   pv_done: the scores of chunk i + 1 ask for chunk i - 1; the producers ask for chunk i - 2 before they bring chunk i's values; the rows ask for chunk i - 1, and chunk i + 1's product needs their P.
-  auto parity = [](int i) { return (uint32_t)(i >> 1) & 1u; };
+  auto use = [&](int i) { return (done + i) & 1; };
+  auto parity = [&](int i) { return (uint32_t)((done + i) >> 1) & 1u; };
   float l = 0.f, m = -INFINITY, low = 0.f;
   bool ok = true;
 
@@ -175,7 +223,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     struct Place { int x, off, pos, page, at; };   // the next chunk's entry of the table, offset in its page and position, and the page and offset that were looked up
     auto first = [&](int sixteen) {
       Place w;
-      w.pos = rank * K + sixteen * 16;
+      w.pos = front * K + sixteen * 16;
       w.x = w.pos / p.block_size;
       w.off = w.pos - w.x * p.block_size;
       w.page = -1;
@@ -248,9 +296,9 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
         v_now[u] = vc[u];
       }
       const uint32_t pair_now = pair;
-      const int pos_now = pos, s = i & 1;
+      const int pos_now = pos, s = use(i);
       if (i + 1 < n) load();
-      if (i >= 2 && !tile_wait_warp(&s_full[s], parity(i - 2), pp.timeout)) break;   // the scores of chunk i - 2 have read their keys
+      if (done + i >= 2 && !tile_wait_warp(&s_full[s], parity(i - 2), pp.timeout)) break;   // the scores of chunk i - 2 have read their keys
 #pragma unroll
       for (int u = 0; u < PER; ++u) {
         const uint32_t w[4] = {k_now[u].x, k_now[u].y, k_now[u].z, k_now[u].w};
@@ -263,7 +311,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
       }
       fence_proxy_async_smem();
       mbar_arrive(&k_full[s]);
-      if (i >= 2 && !tile_wait_warp(&pv_done[s], parity(i - 2), pp.timeout)) break;   // its product has read its values, its rows their pairs
+      if (done + i >= 2 && !tile_wait_warp(&pv_done[s], parity(i - 2), pp.timeout)) break;   // its product has read its values, its rows their pairs
 #pragma unroll
       for (int u = 0; u < PER; ++u) {
         const uint32_t w[4] = {v_now[u].x, v_now[u].y, v_now[u].z, v_now[u].w};
@@ -286,16 +334,16 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     constexpr uint32_t idesc_o = make_umma_idesc_bf16(kKv4TileRows, HD) | (1u << 16);   // V: b_major = MN
     const uint64_t q_desc = make_umma_desc_k128(sQ), k_desc = make_umma_desc_k128(sK), v_desc = make_umma_desc_mn128(sV, kVHalf);
     auto scores = [&](int i) {
-      if (!tile_wait_warp(&k_full[i & 1], parity(i), pp.timeout)) return false;
+      if (!tile_wait_warp(&k_full[use(i)], parity(i), pp.timeout)) return false;
       tc_fence_after();
-      const uint64_t kd = k_desc + (uint64_t)((i & 1) * (kKTile >> 4));
-      const uint32_t to = tmem + (uint32_t)(i & 1) * 64u;
+      const uint64_t kd = k_desc + (uint64_t)(use(i) * (kKTile >> 4));
+      const uint32_t to = tmem + (uint32_t)use(i) * 64u;
       if (elect_one()) {
 #pragma unroll
         for (int h = 0; h < HALVES; ++h)
 #pragma unroll
           for (int k = 0; k < 4; ++k) umma_e4m3_ss(to, q_desc + (h * kQHalf >> 4) + 2 * k, kd + 2 * k, idesc_s, (uint32_t)((h | k) != 0));   // (heads of 128: high parts, then low)
-        umma_commit(&s_full[i & 1]);
+        umma_commit(&s_full[use(i)]);
       }
       __syncwarp();
       return true;
@@ -303,17 +351,17 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     bool go = n > 0 && scores(0);
     for (int i = 0; i < n && go; ++i) {
       // the scores of chunk i + 1 go over the P that the product of chunk i - 1 reads
-      if (i > 0 && !(go = tile_wait_warp(&pv_done[(i - 1) & 1], parity(i - 1), pp.timeout))) break;
+      if (i > 0 && !(go = tile_wait_warp(&pv_done[use(i - 1)], parity(i - 1), pp.timeout))) break;
       if (i + 1 < n && !(go = scores(i + 1))) break;
-      if (!(go = tile_wait_warp(&v_full[i & 1], parity(i), pp.timeout) && tile_wait_warp(&p_full[i & 1], parity(i), pp.timeout))) break;
+      if (!(go = tile_wait_warp(&v_full[use(i)], parity(i), pp.timeout) && tile_wait_warp(&p_full[use(i)], parity(i), pp.timeout))) break;
       tc_fence_after();
-      const uint64_t vd = v_desc + (uint64_t)((i & 1) * (kVTile >> 4));
-      const uint32_t from = tmem + (uint32_t)(i & 1) * 64u;
+      const uint64_t vd = v_desc + (uint64_t)(use(i) * (kVTile >> 4));
+      const uint32_t from = tmem + (uint32_t)use(i) * 64u;
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < K / 16; ++k)   // 16 keys: 2048 B of V, 8 columns of P
           umma_bf16_ts(tmem_o, from + 8 * k, vd + 128 * k, idesc_o, (uint32_t)((i | k) != 0));
-        umma_commit(&pv_done[i & 1]);
+        umma_commit(&pv_done[use(i)]);
       }
       __syncwarp();
     }
@@ -324,15 +372,15 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     const float unit = row_units[at].x;
     const uint64_t sum2 = pack2(row_units[at].y, row_units[at].y);
     for (int i = 0; i < n && ok; ++i) {
-      const uint32_t sp = tmem + lanes + (uint32_t)(i & 1) * 64u;
-      if (!(ok = tile_wait_warp(&v_full[i & 1], parity(i), pp.timeout) && tile_wait_warp(&s_full[i & 1], parity(i), pp.timeout))) break;
+      const uint32_t sp = tmem + lanes + (uint32_t)use(i) * 64u;
+      if (!(ok = tile_wait_warp(&v_full[use(i)], parity(i), pp.timeout) && tile_wait_warp(&s_full[use(i)], parity(i), pp.timeout))) break;
       tc_fence_after();
 #pragma unroll 1
       for (int h = TWIN ? warp >> 1 : 0; h < (TWIN ? (warp >> 1) + 1 : 2); ++h) {   // 32 keys
-        const int2 pos2 = *reinterpret_cast<const int2*>(&at_pos[i & 1][2 * h]);
+        const int2 pos2 = *reinterpret_cast<const int2*>(&at_pos[use(i)][2 * h]);
         const int pos[2] = {pos2.x, pos2.y};
         const bool whole = max(pos[0], pos[1]) + 16 <= seen_by_all;
-        const ulonglong2 *kp = reinterpret_cast<const ulonglong2*>(key_pairs[i & 1]) + 16 * h, *vp = reinterpret_cast<const ulonglong2*>(value_pairs[i & 1]) + 16 * h;
+        const ulonglong2 *kp = reinterpret_cast<const ulonglong2*>(key_pairs[use(i)]) + 16 * h, *vp = reinterpret_cast<const ulonglong2*>(value_pairs[use(i)]) + 16 * h;
         uint32_t u[32];
         tmem_ld_32x32b_x16(sp + 32 * h, u);
         tmem_ld_32x32b_x16(sp + 32 * h + 16, u + 16);
@@ -365,7 +413,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
           l *= f;
           low *= f;
           if (i > 0) {
-            if (!(ok = tile_wait_warp(&pv_done[(i - 1) & 1], parity(i - 1), pp.timeout))) break;
+            if (!(ok = tile_wait_warp(&pv_done[use(i - 1)], parity(i - 1), pp.timeout))) break;
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < HD; c += 16) {
@@ -408,7 +456,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
           unpack2(lows, &x, &y);
           low += x + y;
         } else {   // (a pair that a row does not see may be NaN: 0 x NaN)
-          const float* w = value_pairs[i & 1] + 64 * h;
+          const float* w = value_pairs[use(i)] + 64 * h;
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
             float z[2];
@@ -433,9 +481,9 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
       if (!ok) break;
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&p_full[i & 1]);
+      mbar_arrive(&p_full[use(i)]);
     }
-    if (ok && n > 0) ok = tile_wait_warp(&pv_done[(n - 1) & 1], parity(n - 1), pp.timeout);
+    if (ok && n > 0) ok = tile_wait_warp(&pv_done[use(n - 1)], parity(n - 1), pp.timeout);
     tc_fence_after();
   }
 
@@ -466,14 +514,17 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tmem, 256);   // (before the other blocks are waited for: they may wait for tensor memory)
-  cluster.sync();
+  if constexpr (!SHARED) {
+    if (warp == 8) tmem_dealloc(tmem, 256);   // (before the other blocks are waited for: they may wait for tensor memory)
+    cluster.sync();
+  }
+  const bool whole_head = !SHARED || (turn == 0 && last_turn == turns);   // (else a part of it)
   constexpr int PER = HD / 4, SIDE = 32 / PER, W = kKv4TileThreads / 32;   // lanes of a row, rows side by side in a warp
   const int part_lane = lane % PER, parts = TWIN ? 2 * C : C;
   for (int base = (rank * W + warp) * SIDE; base < rows; base += C * W * SIDE) {
     const int row = min(base + lane / PER, rows - 1);
     // a part: a block's, or one of the two of a block
-    auto part = [&](int x) { return cluster.map_shared_rank(joined, TWIN ? x >> 1 : x) + (row + (TWIN ? (x & 1) * 64 : 0)) * LDO; };
+    auto part = [&](int x) { return (SHARED ? joined : cluster.map_shared_rank(joined, TWIN ? x >> 1 : x)) + (row + (TWIN ? (x & 1) * 64 : 0)) * LDO; };
     float2 ml = make_float2(-INFINITY, 0.f);
     if (part_lane < parts) ml = *reinterpret_cast<const float2*>(part(part_lane) + HD);
     float top = ml.x;
@@ -482,7 +533,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     float f = top == -INFINITY ? 1.f : exp2f(ml.x - top), total = part_lane < parts ? ml.y * f : 0.f;   // (of this lane's part; no score, or NaN only: zeros and NaN add up)
 #pragma unroll
     for (int w = PER / 2; w > 0; w >>= 1) total += __shfl_xor_sync(0xffffffffu, total, w);
-    f *= total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;   // (a row that sees no key is zero, NaN stays)
+    if (whole_head) f *= total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;   // (a row that sees no key is zero, NaN stays)
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int c = 0; c < parts; ++c) {
@@ -490,11 +541,25 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
       const float w = __shfl_sync(0xffffffffu, f, (lane & ~(PER - 1)) + c);
       acc.x += x.x * w; acc.y += x.y * w; acc.z += x.z * w; acc.w += x.w * w;
     }
-    if (base + lane / PER < rows)
-      *reinterpret_cast<uint2*>(p.out + ((size_t)(b * p.Q + tok0 + row / G) * p.heads + kvh * G + row % G) * HD + part_lane * 4) =
-          make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+    if (base + lane / PER >= rows) continue;
+    if (!whole_head) {
+      float* to = p.parts + ((size_t)(2 * blockIdx.x + (turn == 0)) * rows + row) * (HD + 4);
+      *reinterpret_cast<float4*>(to + part_lane * 4) = acc;
+      if (part_lane == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(top, total);
+      continue;
+    }
+    *reinterpret_cast<uint2*>(p.out + ((size_t)(b * p.Q + tok0 + row / G) * p.heads + kvh * G + row % G) * HD + part_lane * 4) = make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
   }
-  cluster.sync();   // no block leaves while its part is read
+  if constexpr (SHARED) {
+    at += last_turn - turn;
+    done += n;
+    __syncthreads();   // (the sums are read: their memory is the queries' and stages' again)
+  } else {
+    cluster.sync();   // no block leaves while its part is read
+    return;
+  }
+  }
+  if (SHARED && warp == 8) tmem_dealloc(tmem, 256);
 }
 
 }  // namespace ssdk

@@ -12,6 +12,8 @@ inline uint32_t __float_as_uint(float f) {
   std::memcpy(&u, &f, 4);
   return u;
 }
+template <typename T>
+inline void __stcs(T* p, const T& v) { *p = v; }
 #include "pairs_emu.h"
 namespace ssdk {
 inline float one_if_ge(float a, float b) { return a >= b ? 1.f : 0.f; }
