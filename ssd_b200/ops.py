@@ -364,13 +364,15 @@ def kv4_caches(num_blocks: int, block_size: int, kv_heads: int, head_dim: int, d
 
 def _kv4(name: str, k_cache: torch.Tensor, head_dim: int):
     """Shape of the caches, and the tokens of a page."""
-    n, KV, size = k_cache.shape if k_cache.dim() == 3 else (-1,) * 3
+    row = 68 if head_dim == 128 else 36
+    if k_cache.dim() == 3 and (head_dim == 128 or head_dim == 64):
+        shape = k_cache.shape
+        block_size, rest = divmod(shape[2], row)
+        if not rest and 0 < block_size < _TOP:
+            return shape, block_size
     if not (head_dim == 64 or head_dim == 128):
         raise ValueError(f"{name}: heads of {head_dim} (64 or 128)")
-    row = head_dim // 2 + 4
-    if size < row or size % row or size // row >= _TOP:
-        raise ValueError(f"{name}: k_cache: {tuple(k_cache.shape)} is not [num_blocks, KV, block_size * {row}]")
-    return (n, KV, size), size // row
+    raise ValueError(f"{name}: k_cache: {tuple(k_cache.shape)} is not [num_blocks, KV, block_size * {row}]")
 
 
 def rope_store_kv4(qkv: torch.Tensor, positions: torch.Tensor, slot_mapping: torch.Tensor, rope_table: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -392,7 +394,7 @@ def rope_store_kv4(qkv: torch.Tensor, positions: torch.Tensor, slot_mapping: tor
             args.append((w, what, _BF, (head_dim,)))
     gpu = _check("rope_store_kv4", *args)
     q = qkv.new_empty(M, heads * head_dim)
-    k, v = qkv.new_empty(2, M, kv_heads, head_dim).unbind(0) if values else (None, None)
+    k, v = (qkv.new_empty(M, kv_heads, head_dim), qkv.new_empty(M, kv_heads, head_dim)) if values else (None, None)
     _launch("ssdk_rope_store_kv4", gpu, qkv.data_ptr(), positions.data_ptr(), slot_mapping.data_ptr(), rope_table.data_ptr(), top, rot, _ptr(q_norm_w), _ptr(k_norm_w),
             norm_eps, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k), _ptr(v), cache[0], block_size, M, heads, kv_heads, head_dim)
     return (q, k, v) if values else q
@@ -406,19 +408,21 @@ def store_kv4(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_ca
     M, KV, hd = shape = k.shape if k.dim() == 3 else (-1,) * 3
     cache, block_size = _kv4("store_kv4", k_cache, hd)
     cache = (cache[0], KV, cache[2])
-    for t, what in ((k, "k"), (v, "v")):
-        if t.dtype is not _BF:
-            raise TypeError(f"store_kv4: {what}: expected {_BF}, got {t.dtype}")
-        if t.shape != shape:
-            raise ValueError(f"store_kv4: {what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-        if t.get_device() != slot_mapping.get_device():
-            raise ValueError(f"store_kv4: {what}: on {t.device}, slot_mapping on {slot_mapping.device}")
-        if t.stride(2) != 1 or (KV > 1 and t.stride(1) != hd):
-            raise ValueError(f"store_kv4: {what}: heads and channels of a row must be contiguous")
+    plain = k.dtype is _BF and v.dtype is _BF and v.shape == shape and k.get_device() == v.get_device() == slot_mapping.get_device() and k.is_contiguous() and v.is_contiguous()
+    if not plain:
+        for t, what in ((k, "k"), (v, "v")):
+            if t.dtype is not _BF:
+                raise TypeError(f"store_kv4: {what}: expected {_BF}, got {t.dtype}")
+            if t.shape != shape:
+                raise ValueError(f"store_kv4: {what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+            if t.get_device() != slot_mapping.get_device():
+                raise ValueError(f"store_kv4: {what}: on {t.device}, slot_mapping on {slot_mapping.device}")
+            if t.stride(2) != 1 or (KV > 1 and t.stride(1) != hd):
+                raise ValueError(f"store_kv4: {what}: heads and channels of a row must be contiguous")
     gpu = _check("store_kv4", (slot_mapping, "slot_mapping", _I32, (M,)), (k_cache, "k_cache", _U8, cache), (v_cache, "v_cache", _U8, cache))
-    a, b = both = k.new_empty(2, M, KV, hd).unbind(0) if values else (None, None)
-    _launch("ssdk_store_kv4", gpu, k.data_ptr(), v.data_ptr(), k.stride(0) if M > 1 else 0, v.stride(0) if M > 1 else 0, slot_mapping.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            _ptr(a), _ptr(b), cache[0], block_size, M, KV, hd)
+    k_row, v_row = (KV * hd, KV * hd) if plain else (k.stride(0) if M > 1 else 0, v.stride(0) if M > 1 else 0)
+    a, b = both = (k.new_empty(M, KV, hd), k.new_empty(M, KV, hd)) if values else (None, None)
+    _launch("ssdk_store_kv4", gpu, k.data_ptr(), v.data_ptr(), k_row, v_row, slot_mapping.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(a), _ptr(b), cache[0], block_size, M, KV, hd)
     return both if values else None
 
 
@@ -427,7 +431,7 @@ def load_kv4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.T
     M = _last(slot_mapping, 1)
     cache, block_size = _kv4("load_kv4", k_cache, head_dim)
     gpu = _check("load_kv4", (k_cache, "k_cache", _U8, cache), (v_cache, "v_cache", _U8, cache), (slot_mapping, "slot_mapping", _I32, (M,)))
-    k, v = both = torch.empty(2, M, cache[1], head_dim, dtype=_BF, device=k_cache.device).unbind(0)
+    k, v = both = k_cache.new_empty(M, cache[1], head_dim, dtype=_BF), k_cache.new_empty(M, cache[1], head_dim, dtype=_BF)
     _launch("ssdk_load_kv4", gpu, k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr(), k.data_ptr(), v.data_ptr(), cache[0], block_size, M, cache[1], head_dim)
     return both
 
