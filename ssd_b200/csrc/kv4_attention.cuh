@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
     if (at >= end) return;
     int before;
     b = kv4_sequence_of<W * K>(p, at, &before);
+    if (b >= p.B) return;   // (only where lengths change meanwhile)
     turns = kv4_turns<W * K>(p, b);
     const int from = at - before * p.kv_heads;
     kvh = from / turns;
@@ -169,7 +170,8 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
       turn = 0;
       if (++kvh == p.kv_heads) {
         kvh = 0;
-        turns = kv4_turns<W * K>(p, ++b);
+        if (++b >= p.B) break;   // (only where lengths change meanwhile)
+        turns = kv4_turns<W * K>(p, b);
       }
     }
   }
@@ -573,13 +575,13 @@ __global__ void __launch_bounds__(kKv4JoinThreads, 2) kv4_join_kernel(const __gr
   constexpr int W = kKv4JoinThreads / 32, V = HD / 32;   // channels of a lane
   __shared__ float sums[SPREAD ? W : 1][HD];
   __shared__ float2 totals[W];
-  pdl_wait();
-  pdl_launch_dependents();
   const int G = p.heads / p.kv_heads, R = G * p.Q, kvh = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int2 heads = kv4_turns_of_all<KEYS>(p, b);
   const Kv4Stretch stretch(heads.x * p.kv_heads, blocks);
   const int turns = kv4_turns<KEYS>(p, b), first = heads.y * p.kv_heads + kvh * turns, from = stretch.block(first), to = stretch.block(first + turns - 1);
-  if (from == to) return;   // (the whole block)
+  pdl_wait();   // (the lengths are there before: the kernel in front, which lets this one begin behind its own wait, has read them)
+  pdl_launch_dependents();
+  if (from == to) return;   // (the whole block; behind the wait, as whoever waits for this grid waits for the one in front too)
   for (int r = SPREAD ? (int)blockIdx.z : (int)blockIdx.z * W + warp; r < R; r += SPREAD ? (int)gridDim.z : (int)gridDim.z * W) {
     const int step = SPREAD ? W : 1;
     float top = -INFINITY, sum = 0.f, acc[V] = {};

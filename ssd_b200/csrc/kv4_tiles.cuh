@@ -113,20 +113,19 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     const Kv4Stretch stretch(kv4_turns_of_all<K>(p, 0).x * p.kv_heads, gridDim.x);
     at = stretch.first(blockIdx.x);
     end = stretch.first(blockIdx.x + 1);
-    if (at >= end) {   // nothing to do but to give the tensor memory back
+    int before = 0;
+    if (at < end) b = kv4_sequence_of<K>(p, at, &before);
+    if (at >= end || b >= p.B) {   // nothing to do but to give the tensor memory back (no sequence: only where lengths change meanwhile)
       __syncthreads();
       pdl_launch_dependents();
       if (warp == 8) tmem_dealloc(tmem_slot, 256);
       return;
     }
-    int before;
-    b = kv4_sequence_of<K>(p, at, &before);
     turns = kv4_turns<K>(p, b);
     const int from = at - before * p.kv_heads;
     kvh = from / turns;
     turn = from - kvh * turns;
   }
-  uint32_t tmem = 0;
 #pragma unroll 1
   for (bool again = false; at < end; again = true) {
   if constexpr (SHARED) {
@@ -134,60 +133,19 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
       turn = 0;
       if (++kvh == p.kv_heads) {
         kvh = 0;
-        turns = kv4_turns<K>(p, ++b);
+        if (++b >= p.B) break;   // (only where lengths change meanwhile)
+        turns = kv4_turns<K>(p, b);
       }
     }
   }
   const int last_turn = SHARED ? min(turns, turn + (end - at)) : 0;
-  // Queries: HD / 8 lanes a row, eight channels each.  Heads of 128: high and low parts in halves of their own, heads of 64: in a row's 128 bytes behind one another (the keys' codes stand there twice).
-  // Rows behind the last one are zero.
-  constexpr int LPR = HD / 8, PIECES = (TWIN ? 64 : kKv4TileRows) * LPR, LOADS = (PIECES + kKv4TileThreads - 1) / kKv4TileThreads;
-  uint4 q_now[LOADS];
-#pragma unroll
-  for (int x = 0; x < LOADS; ++x) {
-    const int i = x * kKv4TileThreads + (int)threadIdx.x, r = i / LPR;
-    q_now[x] = make_uint4(0, 0, 0, 0);
-    if (r < rows) q_now[x] = ld_nc_v4(p.q + ((size_t)(b * p.Q + tok0 + r / G) * p.heads + kvh * G + r % G) * HD + i % LPR * 8);
+  if (!again) {   // the barriers, and where tensor memory is
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_launch_dependents();   // (this block has its tensor memory: what is scheduled now may take the rest of the SM's and wait for this grid)
   }
-#pragma unroll
-  for (int x = 0; x < LOADS; ++x) {
-    const int i = x * kKv4TileThreads + (int)threadIdx.x, r = i / LPR, c = i % LPR;
-    if (i >= PIECES) break;   // (a warp's lanes stay together: both numbers are multiples of 32)
-    float f[8], sum = 0.f, top = 0.f;
-    unpack_bf16x8(q_now[x], f);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      sum += f[j];
-      top = fmaxf(top, fabsf(f[j]));
-    }
-#pragma unroll
-    for (int w = 1; w < LPR; w *= 2) {
-      sum += __shfl_xor_sync(0xffffffffu, sum, w);
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-    }
-    const int e = max((int)(__float_as_uint(top) >> 23), 9);   // (biased exponent; a unit is 2^9 2^(e - 134), of which the keys' scales have 2^2)
-    const float up = __uint_as_float((uint32_t)(261 - e) << 23), unit = __uint_as_float((uint32_t)min(e, 254) << 23);   // 2^(7 - (e - 127)), 2^(e - 127)
-    const float even[4] = {f[0] * up, f[2] * up, f[4] * up, f[6] * up}, odd[4] = {f[1] * up, f[3] * up, f[5] * up, f[7] * up};
-    uint2 high, low;
-    e4m3_twice(even, &high.x, &low.x);
-    e4m3_twice(odd, &high.y, &low.y);
-#pragma unroll
-    for (int at_row = r; at_row < kKv4TileRows; at_row += TWIN ? 64 : kKv4TileRows) {
-      uint8_t* to = sQ + swizzled(at_row, c >> 1) + (c & 1) * 8;
-      *reinterpret_cast<uint2*>(to) = high;
-      if (HD == 128) *reinterpret_cast<uint2*>(to + kQHalf) = low;
-      else *reinterpret_cast<uint2*>(sQ + swizzled(at_row, 4 + (c >> 1)) + (c & 1) * 8) = low;
-      if (c == 0) row_units[at_row] = fabsf(sum) < INFINITY && e < 255 ? make_float2(unit, sum / unit) : make_float2(__uint_as_float(kKv4Nan), 0.f);
-    }
-  }
-  fence_proxy_async_smem();
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  tmem = tmem_slot;
-  const uint32_t tmem_o = tmem + 128;   // S / P buffers at columns 0 and 64, O behind them
-  pdl_launch_dependents();   // (this block has its tensor memory: what is scheduled now may take the rest of the SM's and wait for this grid)
-
+  const uint32_t tmem = tmem_slot, tmem_o = tmem + 128;   // S / P buffers at columns 0 and 64, O behind them
   const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size), ctx = len - p.Q + tok0;
   const int seen = max(0, min(len, ctx + tq)), seen_by_all = ctx + 1;   // positions that some row sees, that all do
   const int chunks = (seen + K - 1) / K, front = SHARED ? turn : rank;   // chunk i of this piece is front + i C
@@ -202,6 +160,55 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
   float l = 0.f, m = -INFINITY, low = 0.f;
   bool ok = true;
 
+  if (warp < 4 || warp == 8) {
+    // Queries: HD / 8 lanes a row, eight channels each.  Heads of 128: high and low parts in halves of their own, heads of 64: in a row's 128 bytes behind one another (the keys' codes stand there twice).
+    // Rows behind the last one are zero.
+    constexpr int LPR = HD / 8, PIECES = (TWIN ? 64 : kKv4TileRows) * LPR, T = kKv4TileThreads - kKv4Producers, LOADS = (PIECES + T - 1) / T, BATCH = SHARED && LOADS > 7 ? 7 : LOADS;
+    const int mine = warp < 4 ? threadIdx.x : threadIdx.x - kKv4Producers;
+#pragma unroll 1
+    for (int x0 = 0; x0 < LOADS; x0 += BATCH) {
+      uint4 q_now[BATCH];
+#pragma unroll
+      for (int x = 0; x < BATCH; ++x) {
+        const int i = (x0 + x) * T + mine, r = i / LPR;
+        q_now[x] = make_uint4(0, 0, 0, 0);
+        if (r < rows) q_now[x] = ld_nc_v4(p.q + ((size_t)(b * p.Q + tok0 + r / G) * p.heads + kvh * G + r % G) * HD + i % LPR * 8);
+      }
+#pragma unroll
+      for (int x = 0; x < BATCH; ++x) {
+        const int i = (x0 + x) * T + mine, r = i / LPR, c = i % LPR;
+        if (i >= PIECES) break;   // (a warp's lanes stay together: both numbers are multiples of 32)
+        float f[8], sum = 0.f, top = 0.f;
+        unpack_bf16x8(q_now[x], f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          sum += f[j];
+          top = fmaxf(top, fabsf(f[j]));
+        }
+#pragma unroll
+        for (int w = 1; w < LPR; w *= 2) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, w);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+        }
+        const int e = max((int)(__float_as_uint(top) >> 23), 9);   // (biased exponent; a unit is 2^9 2^(e - 134), of which the keys' scales have 2^2)
+        const float up = __uint_as_float((uint32_t)(261 - e) << 23), unit = __uint_as_float((uint32_t)min(e, 254) << 23);   // 2^(7 - (e - 127)), 2^(e - 127)
+        const float even[4] = {f[0] * up, f[2] * up, f[4] * up, f[6] * up}, odd[4] = {f[1] * up, f[3] * up, f[5] * up, f[7] * up};
+        uint2 high, low;
+        e4m3_twice(even, &high.x, &low.x);
+        e4m3_twice(odd, &high.y, &low.y);
+#pragma unroll
+        for (int at_row = r; at_row < kKv4TileRows; at_row += TWIN ? 64 : kKv4TileRows) {
+          uint8_t* to = sQ + swizzled(at_row, c >> 1) + (c & 1) * 8;
+          *reinterpret_cast<uint2*>(to) = high;
+          if (HD == 128) *reinterpret_cast<uint2*>(to + kQHalf) = low;
+          else *reinterpret_cast<uint2*>(sQ + swizzled(at_row, 4 + (c >> 1)) + (c & 1) * 8) = low;
+          if (c == 0) row_units[at_row] = fabsf(sum) < INFINITY && e < 255 ? make_float2(unit, sum / unit) : make_float2(__uint_as_float(kKv4Nan), 0.f);
+        }
+      }
+    }
+    fence_proxy_async_smem();
+    asm volatile("bar.sync 1, %0;" ::"r"(T) : "memory");   // (of these warps: codes are on their way meanwhile)
+  }
   if (warp >= 4 && warp < 8) {
     // ---- codes: a thread has PER pieces of 32 channels (eight lanes are eight rows) of the keys and of the values, and the pair of one of either ----
     constexpr int NP = HD / 32, PER = K * NP / kKv4Producers;   // (PER = 2: the second piece is 32 rows on)
@@ -559,7 +566,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     return;
   }
   }
-  if (SHARED && warp == 8) tmem_dealloc(tmem, 256);
+  if (SHARED && warp == 8) tmem_dealloc(tmem_slot, 256);
 }
 
 }  // namespace ssdk
