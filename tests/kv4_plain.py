@@ -71,7 +71,7 @@ def turned(x, positions, table, w, eps):
 
 
 def attention(q, k_cache, v_cache, table, lens, q_len, scale):
-    """-> out in 64 bits and how far it may be off."""
+    """-> out in 64 bits and how far it may be off.  More than sixteen rows to a key head see values as load_kv4 gives them, in bf16."""
     M, H, hd = q.shape
     (kv, kc, kp), (vv, vc, vp) = get(k_cache, hd), get(v_cache, hd)
     num, S, KV, _ = kv.shape
@@ -87,6 +87,8 @@ def attention(q, k_cache, v_cache, table, lens, q_len, scale):
         for g in range(KV):
             k, c, pair = kv[pages, off, g], kc[pages, off, g].to(F64), kp[pages, off, g].to(F64)
             v, vcode, vpair = vv[pages, off, g], vc[pages, off, g].to(F64), vp[pages, off, g].to(F64)
+            if G * q_len > 16:
+                k, v = rounded(k).to(F64), rounded(v).to(F64)
             for j in range(q_len):
                 seen = pos <= n - q_len + j
                 if not bool(seen.any()):
@@ -95,7 +97,7 @@ def attention(q, k_cache, v_cache, table, lens, q_len, scale):
                 p = torch.softmax(rows @ k[seen].t() * scale, 1)
                 o = p @ v[seen]
                 # the two sums of an output: codes around their middle, and what is left
-                one = p @ (vpair[seen, :1] * (vcode[seen] - 8)).abs()
+                one = p @ (v[seen] if G * q_len > 16 else vpair[seen, :1] * (vcode[seen] - 8)).abs()
                 two = p @ (vpair[seen, 1:] + 8 * vpair[seen, :1]).abs().expand(-1, hd)
                 # scores: hd / 16 sums of 16 products with 16 + code in fp32 at most, each off by 2^-22 of the terms' size, and the minimum's part; a weight moves by as much as its score
                 size = rows.abs() @ (pair[seen, :1].abs() * (16 + c[seen])).t() + rows.abs().sum(1, keepdim=True) * (pair[seen, 1:] - 16 * pair[seen, :1]).abs().t()
