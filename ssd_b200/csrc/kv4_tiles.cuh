@@ -18,8 +18,8 @@
 
 namespace ssdk {
 
-constexpr int kKv4TileRows = 128, kKv4TileKeys = 64, kKv4TileThreads = 288, kKv4Producers = 128;   // warps: 4 of rows, 4 of codes, one of products
-constexpr int kv4_tile_body(int HD) { return kKv4TileRows * HD * 2 + 4 * kKv4TileKeys * HD * 2; }   // queries | two stages of keys | of values
+constexpr int kKv4TileRows = 128, kKv4TileKeys = 64, kKv4TileThreads = 320, kKv4Producers = 128;   // warps: 4 of rows, 4 of values, one of products, one of copies
+constexpr int kv4_tile_body(int HD) { return kKv4TileRows * HD * 2 + 4 * kKv4TileKeys * HD * 2 + 2 * kKv4TileKeys * kv4_row_bytes(HD); }   // queries | two stages of keys | of values | a chunk as the cache has it
 constexpr int kv4_tile_smem(int HD) {
   const int join = kKv4TileRows * (HD + 4) * 4, body = kv4_tile_body(HD);
   return (body > join ? body : join) + 1024;
@@ -39,6 +39,14 @@ SSDK_DEVINL uint4 kv4_value8(uint32_t w, uint32_t scale, uint32_t low) {
 // A scale that rounding has brought so high that code 15 passes the largest number of bf16 goes one step back (values are of finite rows, so that is below their largest then).
 SSDK_DEVINL uint32_t kv4_in_range(uint32_t pair) { return fmaf(15.f, __uint_as_float(pair << 16), __uint_as_float(pair & 0xffff0000u)) >= 0x1.ffp127f ? pair - 1 : pair; }
 SSDK_DEVINL bool kv4_finite(uint32_t pair) { return (pair & 0x7f80u) != 0x7f80u && (pair & 0x7f800000u) != 0x7f800000u; }
+SSDK_DEVINL void bulk_copy(void* smem_dst, const void* from, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem_dst)), "l"(from), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+// of a warp: what its threads did before is there for whoever waits
+SSDK_DEVINL void mbar_arrive_warp(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
 // 16-byte piece c of a row of 128 bytes under the 128-byte swizzle
 SSDK_DEVINL int swizzled(int row, int c) { return row * 128 + ((c ^ (row & 7)) << 4); }
 
@@ -56,7 +64,8 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
   constexpr int kQHalf = kKv4TileRows * 128, kHalf = K * 128, kTile = HALVES * kHalf;   // 64 channels of the queries, of the keys or values of a chunk; all of them
   const Kv4AttnParams& p = pp.a;
   extern __shared__ uint8_t kv4_tile_raw[];
-  __shared__ __align__(8) uint64_t k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2];
+  __shared__ __align__(8) uint64_t k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], codes_full, codes_free;
+  __shared__ int codes_pos[4];                 // where a chunk's four sixteens of keys that were copied are in their context: behind every one where they have no page
   __shared__ __align__(16) int at_pos[2][4];   // position of a chunk's sixteen keys, behind every context where they have no page
   __shared__ float row_units[kKv4TileRows];   // of a row of queries: what a unit of its scores is (NaN: it is not finite)
   __shared__ uint32_t tmem_slot;
@@ -64,6 +73,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + HALVES * kQHalf;
   uint8_t* sV = sK + 2 * kTile;
+  uint8_t* sC = sV + 2 * kTile;   // codes of keys, of values, pairs of keys, of values
   cg::cluster_group cluster = cg::this_cluster();
   const int C = SHARED ? 1 : (int)cluster.num_blocks(), rank = SHARED ? 0 : (int)cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -71,17 +81,19 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
   const int tile = SHARED ? 0 : (int)gridDim.z - 1 - (int)blockIdx.z;   // (the tiles that see most keys first)
   const int G = p.heads / p.kv_heads, tok0 = tile * pp.tokens, tq = min(pp.tokens, p.Q - tok0), rows = tq * G;
   const int half = (rows + 31) & ~31;                // rows of the warps that have some
-  const int live = TWIN ? 2 * half : half;           // threads that hand P over
+  const int live = (TWIN ? 2 * half : half) / 32;    // warps that hand P over
 
   if (warp == 8) {
     if (lane == 0) {
       for (int s = 0; s < 2; ++s) {
-        mbar_init(&k_full[s], kKv4Producers);
-        mbar_init(&v_full[s], kKv4Producers);
+        mbar_init(&k_full[s], kKv4Producers / 32);
+        mbar_init(&v_full[s], kKv4Producers / 32);
         mbar_init(&s_full[s], 1);
         mbar_init(&p_full[s], live);
         mbar_init(&pv_done[s], 1);
       }
+      mbar_init(&codes_full, 1);
+      mbar_init(&codes_free, kKv4Producers / 32);
       fence_mbar_init();
     }
     __syncwarp();
@@ -144,7 +156,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
 
   if (warp < 4 || warp == 8) {
     // Queries: HD / 8 lanes a row, eight channels each; rows behind the last one are zero.
-    constexpr int LPR = HD / 8, PIECES = (TWIN ? 64 : kKv4TileRows) * LPR, T = kKv4TileThreads - kKv4Producers, LOADS = (PIECES + T - 1) / T, BATCH = SHARED && LOADS > 7 ? 7 : LOADS;
+    constexpr int LPR = HD / 8, PIECES = (TWIN ? 64 : kKv4TileRows) * LPR, T = 160, LOADS = (PIECES + T - 1) / T, BATCH = SHARED && LOADS > 7 ? 7 : LOADS;
     const int mine = warp < 4 ? threadIdx.x : threadIdx.x - kKv4Producers;
 #pragma unroll 1
     for (int x0 = 0; x0 < LOADS; x0 += BATCH) {
@@ -184,59 +196,9 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     asm volatile("bar.sync 1, %0;" ::"r"(T) : "memory");   // (of these warps: codes are on their way meanwhile)
   }
   if (warp >= 4 && warp < 8) {
-    // ---- keys and values: a thread has PER pieces of 32 channels of either ----
+    // ---- keys and values in bf16: a thread has PER pieces of 32 channels of either ----
     constexpr int NP = HD / 32, PER = K * NP / kKv4Producers;   // (PER = 2: the second piece is 32 rows on)
     const int tid = threadIdx.x - 128, piece = tid % NP, row = tid / NP;   // (neighbours are next to one another in the cache)
-    const int record = p.block_size * kv4_row_bytes(HD), pairs = p.block_size * CODES;   // (bytes of a page and head, of its codes)
-    const int64_t page_step = (int64_t)p.kv_heads * record;
-    const uint8_t *k_from = p.k_cache + (int64_t)kvh * record, *v_from = p.v_cache + (int64_t)kvh * record;
-    const int32_t* table = p.tables + (size_t)b * p.max_blocks;
-    const int step = C * K, step_x = step / p.block_size, step_off = step - step_x * p.block_size;
-    uint4 kc[PER], vc[PER];   // (without a page they stay what they were: their pairs are zero)
-    uint32_t k_pair[PER], v_pair[PER];
-    int pos[PER];
-#pragma unroll
-    for (int u = 0; u < PER; ++u) kc[u] = vc[u] = make_uint4(0, 0, 0, 0);
-    // The next chunk's entry of the table, offset in its page and position, by sixteens of keys.  What a page is, is looked at where it is used, a chunk later.
-    struct Place { int x, off, pos, page, at; } of[PER];
-    auto look_up = [&](Place& w) {   // (positions stay below 2^31: the host sees to it)
-      w.page = w.pos < seen ? table[w.x] : -1;
-      w.at = w.off;
-      w.pos += step;
-      w.x += step_x;
-      w.off += step_off;
-      if (w.off >= p.block_size) {
-        w.off -= p.block_size;
-        ++w.x;
-      }
-    };
-#pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      of[u].pos = front * K + ((row + 32 * u) & ~15);
-      of[u].x = of[u].pos / p.block_size;
-      of[u].off = of[u].pos - of[u].x * p.block_size;
-      look_up(of[u]);
-    }
-    auto load = [&]() {   // of the chunk that was looked up; then the next one's pages
-#pragma unroll
-      for (int u = 0; u < PER; ++u) {
-        pos[u] = kNoPosition;
-        k_pair[u] = v_pair[u] = 0;
-        const int page = of[u].page;
-        if (page >= 0 && page < p.num_blocks) {
-          const int64_t start = page * page_step;
-          const int at = of[u].at + (row & 15);
-          kc[u] = ld_nc_v4(k_from + start + at * CODES + piece * 16);
-          vc[u] = ld_nc_v4(v_from + start + at * CODES + piece * 16);
-          pos[u] = of[u].pos - step;
-          if (pos[u] + (row & 15) < len) {   // (behind the context it may be anything)
-            k_pair[u] = *reinterpret_cast<const uint32_t*>(k_from + start + pairs + at * 4);
-            v_pair[u] = *reinterpret_cast<const uint32_t*>(v_from + start + pairs + at * 4);
-          }
-        }
-        look_up(of[u]);
-      }
-    };
     // Where a piece's four words (16 bytes of bf16 each) go in a stage.  Heads of 128: of eight lanes, two rows of four pieces, the upper two begin with their third word, so that all go to banks of their own.
     const bool later = HD == 128 && piece >= 2;
     int to[4];
@@ -248,43 +210,79 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
 #pragma unroll
       for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stage + to[j]) = kv4_value8(w[j], scale, low);
     };
-    if (n > 0) load();
     for (int i = 0; i < n; ++i) {
-      uint4 k_now[PER], v_now[PER];
-      uint32_t kp_now[PER], vp_now[PER];
-      int pos_now[PER];
-#pragma unroll
-      for (int u = 0; u < PER; ++u) {
-        k_now[u] = kc[u];
-        v_now[u] = vc[u];
-        kp_now[u] = k_pair[u];
-        vp_now[u] = v_pair[u];
-        pos_now[u] = pos[u];
-      }
       const int s = use(i);
-      if (i + 1 < n) load();
+      if (!tile_wait_warp(&codes_full, (uint32_t)(done + i) & 1u, pp.timeout)) break;
+      uint4 kc[PER], vc[PER];
+      uint32_t k_pair[PER], v_pair[PER];
+      int pos[PER];
 #pragma unroll
       for (int u = 0; u < PER; ++u) {
-        kp_now[u] = kv4_in_range(kp_now[u]);
-        if (!kv4_finite(vp_now[u])) {
-          kp_now[u] = 0x7fc07fc0u;
-          vp_now[u] = 0;
+        const int key = row + 32 * u;
+        kc[u] = *reinterpret_cast<const uint4*>(sC + key * CODES + piece * 16);
+        vc[u] = *reinterpret_cast<const uint4*>(sC + (K + key) * CODES + piece * 16);
+        k_pair[u] = *reinterpret_cast<const uint32_t*>(sC + 2 * K * CODES + key * 4);
+        v_pair[u] = *reinterpret_cast<const uint32_t*>(sC + 2 * K * CODES + (K + key) * 4);
+        pos[u] = codes_pos[key >> 4];
+      }
+      mbar_arrive_warp(&codes_free);
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        if (pos[u] + (row & 15) >= len) k_pair[u] = v_pair[u] = 0;   // (behind the context they may be anything; without a page they are left from before)
+        k_pair[u] = kv4_in_range(k_pair[u]);
+        if (!kv4_finite(v_pair[u])) {
+          k_pair[u] = 0x7fc07fc0u;
+          v_pair[u] = 0;
         }
       }
       if (done + i >= 2 && !tile_wait_warp(&s_full[s], parity(i - 2), pp.timeout)) break;   // the scores of chunk i - 2 have read their keys
 #pragma unroll
-      for (int u = 0; u < PER; ++u) write(sK + s * kTile + u * 32 * 128, k_now[u], kp_now[u]);
+      for (int u = 0; u < PER; ++u) write(sK + s * kTile + u * 32 * 128, kc[u], k_pair[u]);
       fence_proxy_async_smem();
-      mbar_arrive(&k_full[s]);
+      mbar_arrive_warp(&k_full[s]);
       if (done + i >= 2 && !tile_wait_warp(&pv_done[s], parity(i - 2), pp.timeout)) break;   // its product has read its values, its rows their positions
 #pragma unroll
       for (int u = 0; u < PER; ++u) {
-        write(sV + s * kTile + u * 32 * 128, v_now[u], kv4_in_range(vp_now[u]));
-        if (piece == 0 && (row & 15) == 0) at_pos[s][(row + 32 * u) >> 4] = pos_now[u];
+        write(sV + s * kTile + u * 32 * 128, vc[u], kv4_in_range(v_pair[u]));
+        if (piece == 0 && (row & 15) == 0) at_pos[s][(row + 32 * u) >> 4] = pos[u];
       }
       fence_proxy_async_smem();
-      mbar_arrive(&v_full[s]);
+      mbar_arrive_warp(&v_full[s]);
     }
+  } else if (warp == 9) {
+    // ---- copies of a chunk, as soon as the one before has been taken to registers: four lanes have sixteen keys each, whose pages they look up a chunk ahead ----
+    const int record = p.block_size * kv4_row_bytes(HD), pairs = p.block_size * CODES;   // (bytes of a page and head, of its codes)
+    const int64_t page_step = (int64_t)p.kv_heads * record, head = (int64_t)kvh * record;
+    const int32_t* table = p.tables + (size_t)b * p.max_blocks;
+    const int step = C * K, step_x = step / p.block_size, step_off = step - step_x * p.block_size;
+    int pos = front * K + (lane & 3) * 16, x = pos / p.block_size, off = pos - x * p.block_size;   // (positions stay below 2^31: the host sees to it)
+    int page = lane < 4 && pos < seen ? table[x] : -1, i = 0;
+    for (; i < n; ++i) {
+      if (done + i >= 1 && !tile_wait_warp(&codes_free, (uint32_t)(done + i - 1) & 1u, pp.timeout)) break;
+      const bool is = page >= 0 && page < p.num_blocks;
+      const int64_t from = page * page_step + head, codes = from + off * CODES, two = from + pairs + off * 4;
+      if (lane < 4) codes_pos[lane] = is ? pos : kNoPosition;
+      const int count = __popc(__ballot_sync(0xffffffffu, is));
+      if (lane == 0) mbar_arrive_expect_tx(&codes_full, (uint32_t)(count * 32 * kv4_row_bytes(HD)));
+      __syncwarp();
+      if (is) {
+        uint8_t* to = sC + lane * 16 * CODES;
+        bulk_copy(to, p.k_cache + codes, 16 * CODES, &codes_full);
+        bulk_copy(to + K * CODES, p.v_cache + codes, 16 * CODES, &codes_full);
+        to = sC + 2 * K * CODES + lane * 64;
+        bulk_copy(to, p.k_cache + two, 64, &codes_full);
+        bulk_copy(to + K * 4, p.v_cache + two, 64, &codes_full);
+      }
+      pos += step;
+      x += step_x;
+      off += step_off;
+      if (off >= p.block_size) {
+        off -= p.block_size;
+        ++x;
+      }
+      page = lane < 4 && pos < seen ? table[x] : -1;
+    }
+    if (i > 0) tile_wait_warp(&codes_full, (uint32_t)(done + i - 1) & 1u, pp.timeout);   // (no copy is on its way when the block ends)
   } else if (warp == 8) {
     // (the whole warp goes through the waits, and one lane issues: what a product takes stays uniform)
     constexpr uint32_t idesc_s = make_umma_idesc_bf16(kKv4TileRows, K);
@@ -419,7 +417,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
       if (!ok) break;
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&p_full[use(i)]);
+      mbar_arrive_warp(&p_full[use(i)]);
     }
     if (ok && n > 0) ok = tile_wait_warp(&pv_done[use(n - 1)], parity(n - 1), pp.timeout);
     tc_fence_after();
