@@ -51,8 +51,9 @@ constexpr int kv4_attn_smem(int HD, int NT, int W) {
 // nibbles P and P + 4 of a word as 16 + c in bf16
 template <int P>
 SSDK_DEVINL uint32_t kv4_pair16(uint32_t w) {
-  const uint32_t x = P == 0 ? w << 3 : w >> (4 * P - 3);
-  return (x & 0x00780078u) | 0x41804180u;
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(P == 0 ? w << 3 : w >> (4 * P - 3)), "r"(0x00780078u), "r"(0x41804180u));   // (x & a) | b
+  return d;
 }
 SSDK_DEVINL uint32_t transpose_8x8(uint32_t x) {
   uint32_t d;
