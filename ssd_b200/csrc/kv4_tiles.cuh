@@ -19,7 +19,8 @@
 namespace ssdk {
 
 constexpr int kKv4TileRows = 128, kKv4TileKeys = 64, kKv4TileThreads = 320, kKv4Producers = 128;   // warps: 4 of rows, 4 of values, one of products, one of copies
-constexpr int kv4_tile_body(int HD) { return kKv4TileRows * HD * 2 + 4 * kKv4TileKeys * HD * 2 + 2 * kKv4TileKeys * kv4_row_bytes(HD); }   // queries | two stages of keys | of values | a chunk as the cache has it
+constexpr int kKv4Copies = 3;   // chunks on their way or there as the cache has them
+constexpr int kv4_tile_body(int HD) { return kKv4TileRows * HD * 2 + 3 * kKv4TileKeys * HD * 2 + kKv4Copies * 2 * kKv4TileKeys * kv4_row_bytes(HD); }   // queries | keys | two stages of values | copies
 constexpr int kv4_tile_smem(int HD) {
   const int join = kKv4TileRows * (HD + 4) * 4, body = kv4_tile_body(HD);
   return (body > join ? body : join) + 1024;
@@ -61,18 +62,18 @@ template <int HD, bool TWIN, bool SHARED>
 __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __grid_constant__ Kv4TileParams pp) {
   namespace cg = cooperative_groups;
   constexpr int HALVES = HD / 64, CODES = HD / 2, K = kKv4TileKeys;
-  constexpr int kQHalf = kKv4TileRows * 128, kHalf = K * 128, kTile = HALVES * kHalf;   // 64 channels of the queries, of the keys or values of a chunk; all of them
+  constexpr int kQHalf = kKv4TileRows * 128, kHalf = K * 128, kTile = HALVES * kHalf, kCopy = 2 * K * kv4_row_bytes(HD);   // 64 channels of the queries, of the keys or values of a chunk; all of them
   const Kv4AttnParams& p = pp.a;
   extern __shared__ uint8_t kv4_tile_raw[];
-  __shared__ __align__(8) uint64_t k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], codes_full, codes_free;
-  __shared__ int codes_pos[4];                 // where a chunk's four sixteens of keys that were copied are in their context: behind every one where they have no page
+  __shared__ __align__(8) uint64_t k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], codes_full[kKv4Copies], codes_free[kKv4Copies];
+  __shared__ int codes_pos[kKv4Copies][4];                 // where a chunk's four sixteens of keys that were copied are in their context: behind every one where they have no page
   __shared__ __align__(16) int at_pos[2][4];   // position of a chunk's sixteen keys, behind every context where they have no page
   __shared__ float row_units[kKv4TileRows];   // of a row of queries: what a unit of its scores is (NaN: it is not finite)
   __shared__ uint32_t tmem_slot;
   uint8_t* smem = kv4_tile_raw + ((1024u - (smem_u32(kv4_tile_raw) & 1023u)) & 1023u);
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + HALVES * kQHalf;
-  uint8_t* sV = sK + 2 * kTile;
+  uint8_t* sV = sK + kTile;
   uint8_t* sC = sV + 2 * kTile;   // codes of keys, of values, pairs of keys, of values
   cg::cluster_group cluster = cg::this_cluster();
   const int C = SHARED ? 1 : (int)cluster.num_blocks(), rank = SHARED ? 0 : (int)cluster.block_rank();
@@ -92,8 +93,10 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
         mbar_init(&p_full[s], live);
         mbar_init(&pv_done[s], 1);
       }
-      mbar_init(&codes_full, 1);
-      mbar_init(&codes_free, kKv4Producers / 32);
+      for (int s = 0; s < kKv4Copies; ++s) {
+        mbar_init(&codes_full[s], 1);
+        mbar_init(&codes_free[s], kKv4Producers / 32);
+      }
       fence_mbar_init();
     }
     __syncwarp();
@@ -211,21 +214,22 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
       for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stage + to[j]) = kv4_value8(w[j], scale, low);
     };
     for (int i = 0; i < n; ++i) {
-      const int s = use(i);
-      if (!tile_wait_warp(&codes_full, (uint32_t)(done + i) & 1u, pp.timeout)) break;
+      const int s = use(i), c = (done + i) % kKv4Copies;
+      if (!tile_wait_warp(&codes_full[c], (uint32_t)((done + i) / kKv4Copies) & 1u, pp.timeout)) break;
+      const uint8_t* from = sC + c * kCopy;
       uint4 kc[PER], vc[PER];
       uint32_t k_pair[PER], v_pair[PER];
       int pos[PER];
 #pragma unroll
       for (int u = 0; u < PER; ++u) {
         const int key = row + 32 * u;
-        kc[u] = *reinterpret_cast<const uint4*>(sC + key * CODES + piece * 16);
-        vc[u] = *reinterpret_cast<const uint4*>(sC + (K + key) * CODES + piece * 16);
-        k_pair[u] = *reinterpret_cast<const uint32_t*>(sC + 2 * K * CODES + key * 4);
-        v_pair[u] = *reinterpret_cast<const uint32_t*>(sC + 2 * K * CODES + (K + key) * 4);
-        pos[u] = codes_pos[key >> 4];
+        kc[u] = *reinterpret_cast<const uint4*>(from + key * CODES + piece * 16);
+        vc[u] = *reinterpret_cast<const uint4*>(from + (K + key) * CODES + piece * 16);
+        k_pair[u] = *reinterpret_cast<const uint32_t*>(from + 2 * K * CODES + key * 4);
+        v_pair[u] = *reinterpret_cast<const uint32_t*>(from + 2 * K * CODES + (K + key) * 4);
+        pos[u] = codes_pos[c][key >> 4];
       }
-      mbar_arrive_warp(&codes_free);
+      mbar_arrive_warp(&codes_free[c]);
 #pragma unroll
       for (int u = 0; u < PER; ++u) {
         if (pos[u] + (row & 15) >= len) k_pair[u] = v_pair[u] = 0;   // (behind the context they may be anything; without a page they are left from before)
@@ -235,9 +239,9 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
           v_pair[u] = 0;
         }
       }
-      if (done + i >= 2 && !tile_wait_warp(&s_full[s], parity(i - 2), pp.timeout)) break;   // the scores of chunk i - 2 have read their keys
+      if (done + i >= 1 && !tile_wait_warp(&s_full[use(i - 1)], parity(i - 1), pp.timeout)) break;   // the scores of chunk i - 1 have read their keys
 #pragma unroll
-      for (int u = 0; u < PER; ++u) write(sK + s * kTile + u * 32 * 128, kc[u], k_pair[u]);
+      for (int u = 0; u < PER; ++u) write(sK + u * 32 * 128, kc[u], k_pair[u]);
       fence_proxy_async_smem();
       mbar_arrive_warp(&k_full[s]);
       if (done + i >= 2 && !tile_wait_warp(&pv_done[s], parity(i - 2), pp.timeout)) break;   // its product has read its values, its rows their positions
@@ -258,20 +262,21 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     int pos = front * K + (lane & 3) * 16, x = pos / p.block_size, off = pos - x * p.block_size;   // (positions stay below 2^31: the host sees to it)
     int page = lane < 4 && pos < seen ? table[x] : -1, i = 0;
     for (; i < n; ++i) {
-      if (done + i >= 1 && !tile_wait_warp(&codes_free, (uint32_t)(done + i - 1) & 1u, pp.timeout)) break;
+      const int c = (done + i) % kKv4Copies;
+      if (done + i >= kKv4Copies && !tile_wait_warp(&codes_free[c], (uint32_t)((done + i) / kKv4Copies - 1) & 1u, pp.timeout)) break;
       const bool is = page >= 0 && page < p.num_blocks;
       const int64_t from = page * page_step + head, codes = from + off * CODES, two = from + pairs + off * 4;
-      if (lane < 4) codes_pos[lane] = is ? pos : kNoPosition;
+      if (lane < 4) codes_pos[c][lane] = is ? pos : kNoPosition;
       const int count = __popc(__ballot_sync(0xffffffffu, is));
-      if (lane == 0) mbar_arrive_expect_tx(&codes_full, (uint32_t)(count * 32 * kv4_row_bytes(HD)));
+      if (lane == 0) mbar_arrive_expect_tx(&codes_full[c], (uint32_t)(count * 32 * kv4_row_bytes(HD)));
       __syncwarp();
       if (is) {
-        uint8_t* to = sC + lane * 16 * CODES;
-        bulk_copy(to, p.k_cache + codes, 16 * CODES, &codes_full);
-        bulk_copy(to + K * CODES, p.v_cache + codes, 16 * CODES, &codes_full);
-        to = sC + 2 * K * CODES + lane * 64;
-        bulk_copy(to, p.k_cache + two, 64, &codes_full);
-        bulk_copy(to + K * 4, p.v_cache + two, 64, &codes_full);
+        uint8_t* to = sC + c * kCopy + lane * 16 * CODES;
+        bulk_copy(to, p.k_cache + codes, 16 * CODES, &codes_full[c]);
+        bulk_copy(to + K * CODES, p.v_cache + codes, 16 * CODES, &codes_full[c]);
+        to = sC + c * kCopy + 2 * K * CODES + lane * 64;
+        bulk_copy(to, p.k_cache + two, 64, &codes_full[c]);
+        bulk_copy(to + K * 4, p.v_cache + two, 64, &codes_full[c]);
       }
       pos += step;
       x += step_x;
@@ -282,7 +287,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
       }
       page = lane < 4 && pos < seen ? table[x] : -1;
     }
-    if (i > 0) tile_wait_warp(&codes_full, (uint32_t)(done + i - 1) & 1u, pp.timeout);   // (no copy is on its way when the block ends)
+    for (int x = max(0, i - kKv4Copies); x < i; ++x) tile_wait_warp(&codes_full[(done + x) % kKv4Copies], (uint32_t)((done + x) / kKv4Copies) & 1u, pp.timeout);   // (no copy is on its way when the block ends)
   } else if (warp == 8) {
     // (the whole warp goes through the waits, and one lane issues: what a product takes stays uniform)
     constexpr uint32_t idesc_s = make_umma_idesc_bf16(kKv4TileRows, K);
@@ -291,13 +296,12 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     auto scores = [&](int i) {
       if (!tile_wait_warp(&k_full[use(i)], parity(i), pp.timeout)) return false;
       tc_fence_after();
-      const uint64_t kd = k_desc + (uint64_t)(use(i) * (kTile >> 4));
-      const uint32_t to = tmem + (uint32_t)use(i) * 64u;
+            const uint32_t to = tmem + (uint32_t)use(i) * 64u;
       if (elect_one()) {
 #pragma unroll
         for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16_ss(to, q_desc + (h * kQHalf >> 4) + 2 * k, kd + (h * kHalf >> 4) + 2 * k, idesc_s, (uint32_t)((h | k) != 0));
+          for (int k = 0; k < 4; ++k) umma_bf16_ss(to, q_desc + (h * kQHalf >> 4) + 2 * k, k_desc + (h * kHalf >> 4) + 2 * k, idesc_s, (uint32_t)((h | k) != 0));
         umma_commit(&s_full[use(i)]);
       }
       __syncwarp();
