@@ -40,7 +40,9 @@ struct Kv4AttnParams {
   float scale_log2;              // scale * log2(e)
   float* parts;                  // SHARED: [blocks][2][rows of a key head][HD + 4]: O, reference, sum of a block's first stretch where it began in front of it, and of its last
 };
-constexpr float kKv4Slack = 8.f;
+// Weights are exp2(score - reference), the reference 2^32 above the largest score that it was raised for and raised again when a score passes that by 2^8: with the sum of weights all sums are 2^-32 of what they
+// would be, and values up to bf16's largest number (here times codes less 8 that come with 128 more) pass fp32's in none.  What that costs is weights below 2^-94 of the largest.
+constexpr float kKv4Slack = 8.f, kKv4Above = 32.f;
 constexpr int kKv4Most = 16, kKv4Stages = 3, kKv4Keys = 32;   // blocks of a cluster, a warp's ring, keys of a chunk
 constexpr int kv4_stage_bytes(int HD) { return 2 * kKv4Keys * (HD / 2 + 4); }   // keys' codes | values' codes | keys' pairs | values' pairs
 constexpr int kv4_attn_smem(int HD, int NT, int W) {
@@ -381,7 +383,7 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         most[nt][e] = fmaxf(s[nt][e], s[nt][2 + e]);
-        grow = grow || most[nt][e] > ref[nt][e] + kKv4Slack;
+        grow = grow || most[nt][e] > ref[nt][e] + (kKv4Slack - kKv4Above);
       }
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -391,7 +393,7 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
           float top = most[nt][e];
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)), ref[nt][e]);
+          top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) + kKv4Above, ref[nt][e]);
           const float f = top == ref[nt][e] ? 1.f : ex2_ftz(ref[nt][e] - top);   // (from -inf: 0)
           ref[nt][e] = top;
           l[nt][e] *= f;

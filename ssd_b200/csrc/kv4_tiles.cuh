@@ -106,6 +106,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
   pdl_wait();
   // SHARED: this block's turns at .. end, the first of them turn `turn` of its head
   int at = 0, end = 1, turn = 0, turns = 0, done = 0;   // done: chunks of the pieces before (of stages and barriers)
+  bool lost = false;                                    // a wait ran out: all rows from there on are NaN
   if constexpr (SHARED) {
     const Kv4Stretch stretch(kv4_turns_of_all<K>(p, 0).x * p.kv_heads, gridDim.x);
     at = stretch.first(blockIdx.x);
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
   const int len = tokens_of(p.lens, b, p.max_blocks, p.block_size), ctx = len - p.Q + tok0;
   const int seen = max(0, min(len, ctx + tq)), seen_by_all = ctx + 1;   // positions that some row sees, that all do
   const int chunks = (seen + K - 1) / K, front = SHARED ? turn : rank;   // chunk i of this piece is front + i C
-  const int n = SHARED ? max(0, min(chunks, last_turn) - turn) : front < chunks ? (chunks - front + C - 1) / C : 0;
+  const int n = SHARED ? lost ? 0 : max(0, min(chunks, last_turn) - turn) : front < chunks ? (chunks - front + C - 1) / C : 0;
   // Chunk i is in stage and on barriers use(i), parity(i) is that use's.  A wait by parity is only right while the barrier is in that use or the one behind it:
   //   k_full, v_full: whoever waits for chunk i has to be through with it before its stage is written anew (the keys' behind s_full, the values' behind pv_done, which needs every row's P).
   //   s_full: the producers and the rows ask for chunk i, and chunk i + 2's needs keys of the former and, through p_full, P of the latter.
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
   auto use = [&](int i) { return (done + i) & 1; };
   auto parity = [&](int i) { return (uint32_t)((done + i) >> 1) & 1u; };
   float l = 0.f, m = -INFINITY;
-  bool ok = true;
+  bool ok = !lost;
 
   if (warp < 4 || warp == 8) {
     // Queries: HD / 8 lanes a row, eight channels each; rows behind the last one are zero.
@@ -355,10 +356,10 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
 #pragma unroll
           for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(u[c + e]), __uint_as_float(u[c + 4 + e]));
         const float mx = fmaxf(max3(max3(top[0], top[1], __uint_as_float(u[28])), max3(top[2], top[3], __uint_as_float(u[29])), __uint_as_float(u[30])), __uint_as_float(u[31])) * unit;
-        const bool grow = mx > m + kPromptSlack;
+        const bool grow = mx > m + (kKv4Slack - kKv4Above);
         if (__any_sync(0xffffffffu, grow)) {
-          const float f = grow ? exp2f(m - mx) : 1.f;   // (m = -inf: 0)
-          if (grow) m = mx;
+          const float f = grow ? exp2f(m - (mx + kKv4Above)) : 1.f;   // (m = -inf: 0)
+          if (grow) m = mx + kKv4Above;
           l *= f;
           if (i > 0) {
             if (!(ok = tile_wait_warp(&pv_done[use(i - 1)], parity(i - 1), pp.timeout))) break;
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
   if constexpr (SHARED) {
     at += last_turn - turn;
     done += n;
-    __syncthreads();   // (the sums are read: their memory is the queries' and stages' again)
+    lost = __syncthreads_or(!ok) != 0;   // (and the sums are read: their memory is the queries' and stages' again)
   } else {
     cluster.sync();   // no block leaves while its part is read
     return;

@@ -385,3 +385,92 @@ def test_refusals_leave_the_device_alone(dev):
     with pytest.raises(RuntimeError, match="lies over"):
         ops.store_kv4(q[:, :2], q[:, :2], i32([0, 1], dev), kc, kc)
     assert math.isfinite(float(s.run()[0].float().sum()))
+
+
+# ---------------------------------------------------------------------------------------------------- more than sixteen rows to a key head
+@pytest.mark.parametrize("Q,H,KV,hd,S,lens,width", [
+    (9, 16, 2, 128, 16, [500, 9, 100, 0], None), (33, 4, 2, 128, 48, [90, 33, 4], None), (300, 8, 1, 128, 64, [300, 700], None), (3, 6, 1, 128, 112, [113, 64, 2], None),
+    (5, 32, 1, 64, 32, [63, 65], None), (16, 16, 2, 128, 80, [6000, 16, 0, 300], 200), (11, 9, 1, 128, 256, [256, 20000, 257], 100), (2, 32, 1, 128, 16, [1] * 9 + [700], 2000), (6, 3, 1, 64, 16, [48] * 40, 1500),
+])
+def test_tiles(dev, Q, H, KV, hd, S, lens, width):
+    """One tile and several, rows that lie in one twice or not, clusters and equal stretches; pages that end inside a chunk of keys, holes in tables."""
+    from ssd_b200 import ops
+    g = gen(70, Q, H, KV, hd, S)
+    kc, vc, table = a_case(g, KV, hd, S, lens, width=width)
+    for b in range(0, len(lens), 2):
+        if lens[b] > 3 * S:
+            table[b, 1] = -1 - b
+    q = torch.randn(len(lens) * Q, H, hd, generator=g).to(BF)
+    for scale in (hd ** -0.5, -0.2):
+        got = ops.paged_attention_kv4(q.to(dev), kc.to(dev), vc.to(dev), table.to(dev), i32(lens, dev), Q, scale)
+        within(got, *plain.attention(q, kc, vc, table, lens, Q, scale))
+
+
+@pytest.mark.parametrize("Q,H,hd", [(1, 4, 128), (8, 8, 128), (20, 8, 64)])
+def test_largest_numbers(dev, Q, H, hd):
+    """Rows up to bf16's largest number, whose scale is rounded up so far that code 15 would pass it: a query of zeros has their mean."""
+    from ssd_b200 import ops
+    top, low = 255 * 2.0 ** 120, 5 * 2.0 ** 119
+    scale = float(torch.tensor((top - low) / 15).to(BF))
+    assert 15 * scale + low >= 511 * 2.0 ** 119   # what fp32 rounds to bf16's infinity
+    n, S = 40, 16
+    x = torch.ones(n, 1, hd)
+    x[7, 0, ::2], x[7, 0, 1::2] = top, low
+    x = x.to(BF).to(dev)
+    kc, vc = ops.kv4_caches(5, S, 1, hd, dev)
+    ops.store_kv4(x, x, i32(range(n), dev), kc, vc)
+    got = ops.paged_attention_kv4(torch.zeros(Q, H, hd, dtype=BF, device=dev), kc, vc, i32([[0, 1, 2, 3, 4]], dev), i32([n + Q - 1], dev), Q, 1.0).double().cpu().view(Q, H, hd)
+    x = x.double().cpu()[:, 0]
+    for j in range(Q):
+        rows = n + j   # those behind the n that are stored are zero
+        want = x.sum(0) / rows
+        # half a code, a scale that is a step off (15 2^-7 of it), a weight and the output rounded
+        assert ((got[j] - want).abs() <= (scale / 2 + 15 * scale * 2 ** -7) / rows + want * 2 ** -7).all()
+
+
+def test_a_wait_that_ran_out_is_reported_once(dev):
+    """The word that a bounded wait would set is set by the host here: calls on tiles look at it, the others leave it."""
+    from ssd_b200 import lib
+    word = lib.load().ssdk_debug_op_wait_word()
+    s, few = Step(dev, 71, [300, 64], 6, H=16), Step(dev, 72, [300, 64], 1)
+    s.run()
+    torch.cuda.synchronize()
+    word[0] = 1
+    few.run()
+    assert word[0] == 1
+    with pytest.raises(RuntimeError, match="ran out"):
+        s.run()
+    assert word[0] == 0
+    s.dev["table"].copy_(s.table.to(dev))
+    s.run()
+
+
+@pytest.mark.parametrize("Q", [1, 7])
+def test_calls_at_once(dev, Q):
+    """Calls with parts of their own on streams of their own, over the same cache, and one whose inputs another stream has just written."""
+    from ssd_b200 import ops
+    g = gen(73, Q)
+    KV, hd, S, lens = 2, 128, 64, [9000, 5, 700]
+    kc, vc, table = (t.to(dev) for t in a_case(g, KV, hd, S, lens, width=400))
+    qs = [torch.randn(3 * Q, 16, hd, generator=g).to(BF).to(dev) for _ in range(3)]
+    lens = i32(lens, dev)
+    want = [ops.paged_attention_kv4(q, kc, vc, table, lens, Q, 0.1).clone() for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for q, st in zip(qs, streams):
+            with torch.cuda.stream(st):
+                got.append(ops.paged_attention_kv4(q, kc, vc, table, lens, Q, 0.1))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    with torch.cuda.stream(streams[0]):
+        torch.cuda._sleep(20000000)
+        late = qs[0].clone()
+        ready = torch.cuda.Event()
+        ready.record()
+    torch.cuda.current_stream().wait_event(ready)
+    got = ops.paged_attention_kv4(late, kc, vc, table, lens, Q, 0.1)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want[0])
