@@ -343,10 +343,11 @@ int ssdk_store_kv4(const void* k, const void* v, int64_t k_row, int64_t v_row, c
 /* ssdk_load_kv4: the values of the slots, k and v bf16 [M, KV, head_dim]; rows with a slot outside the cache are zero. */
 int ssdk_load_kv4(const void* k_cache, const void* v_cache, const int32_t* slot_mapping, void* k, void* v, int64_t num_blocks, int block_size,
                   int M, int kv_heads, int head_dim, void* stream);
-/* ssdk_paged_attn_kv4: ssdk_paged_attn over the values scale * code + minimum (not rounded to bf16), causal to the end of the context.  At most 32 query heads to a key head.  Pages
- * outside the cache are passed over, lengths are held to what a table has room for, a row that sees no key is zero.  A NaN row of the cache makes NaN of the rows that see it, a query that is
- * not finite, or whose sum passes fp32, makes its row NaN.  `scratch`: ssdk_paged_attn_kv4_scratch_bytes(...) bytes of the call's own (0: null).  More than sixteen query rows to a key head take a kernel
- * with bounded waits: as with ssdk_paged_attn_pages, a wait that runs out leaves NaN rows, and the next such call of the process returns an error. */
+/* ssdk_paged_attn_kv4: ssdk_paged_attn over the values scale * code + minimum, causal to the end of the context.  Up to sixteen query rows to a key head they are not rounded, with more they are rounded to
+ * bf16, as ssdk_load_kv4 gives them (one that would pass bf16's largest number by that stays below it).  At most 32 query heads to a key head.  Pages outside the cache are passed over, lengths are held
+ * to what a table has room for, a row that sees no key is zero.  A NaN row of the cache makes NaN of the rows that see it, a query that is not finite, or (up to sixteen rows) whose sum passes fp32, makes
+ * its row NaN.  `scratch`: ssdk_paged_attn_kv4_scratch_bytes(...) bytes of the call's own (0: null).  More than sixteen query rows to a key head take a kernel with bounded waits: as with
+ * ssdk_paged_attn_pages, a wait that runs out leaves NaN rows, and the next such call of the process returns an error. */
 int64_t ssdk_paged_attn_kv4_scratch_bytes(int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size, int max_blocks_per_seq);
 int ssdk_paged_attn_kv4(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables, const int32_t* context_lens,
                         void* out, void* scratch, int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size,

@@ -56,9 +56,11 @@ static Kv4Plan kv4_plan(int64_t units, int64_t keys, int resident, int most, int
       plan.cluster = c;
     }
   }
-  // Equal stretches cost a second launch, but their time goes by the sum of all lengths, not by the longest, and more than the blocks of a cluster can share a head.  us, clusters and stretches: one context
-  // of 16000 (8 heads) 15.7 and 17.0, of 32000 25.7 and 22.3, of 64000 44.9 and 31.3, 4 of 32000 43.9 and 39.1, 16 of 8000 40.5 and 39.4, 48 of 16000 144 and 147; with a head or more to every
-  // place on the device blocks are dealt out as others end: 148 of 4000 105 and 126.
+  // Equal stretches cost a second launch, but their time goes by the sum of all lengths, not by the longest, and more than the blocks of a cluster can share a head: they are taken where the clusters' cost
+  // passes share_from.  With a head or more to every place on the device blocks are dealt out as others end.  us, clusters and stretches, of the streaming kernel: one context of 16000 (8 heads) 15.7 and 17.0,
+  // of 32000 25.7 and 22.3, of 64000 44.9 and 31.3, 4 of 32000 43.9 and 39.1, 16 of 8000 40.5 and 39.4, 48 of 16000 144 and 147, 148 of 4000 105 and 126; of 56 rows on tiles: one context of 8000 25.7 and
+  // 27.4, of 16000 35.6 and 32.8, of 32000 56 and 42, 4 of 16000 55.6 and 61, 8 of 4000 32.6 and 38, 8 of 16000 96 and 84, 16 of 4000 52 and 56, 16 of 16000 175 and 145, 32 of 16000 334 and 268 (the other
+  // way: 2 of 4000, 32.7 and 28.2).
   if (may_share && least > share_from && units < slots && units * ((keys + turn - 1) / turn) < (1ll << 31)) plan.blocks = (int)std::min(std::min(slots, units * 64), units * ((keys + turn - 1) / turn));
   return plan;
 }
@@ -77,7 +79,8 @@ static Kv4Plan kv4_tile_plan(int batch, int q_len, int heads, int kv_heads, int 
   int tiles;
   kv4_tile_tokens(q_len, heads / kv_heads, &tiles);
   const int most = head_dim == 64 && heads / kv_heads * q_len <= 64 ? 8 : kKv4Most;   // (their join has a lane of HD / 4 for each part)
-  return kv4_plan((int64_t)batch * kv_heads * tiles, keys, 2, most, kKv4TileKeys, 1280, tiles == 1 && batch <= kMaxShared);
+  const int64_t units = (int64_t)batch * kv_heads * tiles;
+  return kv4_plan(units, keys, 2, most, kKv4TileKeys, 1100 + (int64_t)((double)units * keys / (2 * kSms)), tiles == 1 && batch <= kMaxShared);   // (a block's start and its two parts; its share)
 }
 template <int HD, int KEYS>
 static int launch_join(Launcher& L, const Kv4AttnParams& p, int blocks) {

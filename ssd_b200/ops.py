@@ -445,8 +445,8 @@ def paged_attention_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
                         scale: float) -> torch.Tensor:
     """paged_attention over a cache of 4 bits (kv4_caches): q [B * q_len, H, hd] bf16, block_tables int32 [B, max_blocks], context_lens int32 [B] with the new tokens.
 
-    Returns [B * q_len, H * hd].  Scale and minimum of a row act on scores and weights, so keys and values are not rounded.  Pages outside the cache are passed over, a row
-    that sees no key is zero, a NaN row of the cache makes NaN of the rows that see it."""
+    Returns [B * q_len, H * hd].  Keys and values are scale * code + minimum, not rounded up to sixteen rows (H / KV * q_len) to a key head, in bf16 as load_kv4 gives them with
+    more.  Pages outside the cache are passed over, a row that sees no key is zero, a NaN row of the cache makes NaN of the rows that see it."""
     B, width, H, hd = _last(context_lens, 1), _last(block_tables, 2), *(q.shape[1:] if q.dim() == 3 else (-1, -1))
     cache, block_size = _kv4("paged_attention_kv4", k_cache, hd)
     gpu = _check("paged_attention_kv4", (q, "q", _BF, (B * q_len, H, hd)), (k_cache, "k_cache", _U8, cache), (v_cache, "v_cache", _U8, cache),
