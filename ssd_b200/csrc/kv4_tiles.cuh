@@ -2,16 +2,19 @@
 //
 // S = Q K^T of up to 128 rows (query tokens x the heads that share a key head) and 64 keys into TMEM, P = exp2(S scale - reference) one row per thread, O += P V with P out of TMEM: the usual two
 // products in bf16, over what the codes stand for, bf16(scale x code + minimum), which load_kv4 gives too.  That rounding (half a step of bf16) is what lets a row take a score as it comes: with codes as
-// operands each of them needs its key's scale and minimum, and each weight its value's, which is twice the work of a row and a read of shared memory for every two keys of it (8 x 7 rows over 16000:
-// 101 us).
+// operands each of them needs its key's scale and minimum, and each weight its value's, which is twice the work of a row and a read of shared memory for every two keys of it (8 x 7 rows over 16000
+// 101 us then, 95 so; 512 rows over 8000 119 and 97).
 // A query row is scaled by a power of two so that its largest lies in 2^-9 .. 2^-8 (exact but for what is below 2^-133 then): no sum with keys up to the largest number passes it, and scores are scaled back
 // in fp32.  A word of eight channels' codes gives them in the
 // order 0, 4, 1, 5, 2, 6, 3, 7: queries are stored in that order, outputs are put back.
 // A pair that is not finite makes NaN of the rows that see its key and of no others: a NaN value counts as a NaN key, and is zero itself, since weights of zero meet it too.
-// Four warps bring keys and values (codes in registers, a chunk ahead of the one that they write, its pages two ahead), one issues the products, four have the rows.  A cluster of blocks shares the chunks of
-// a key head; their sums meet in shared memory.
+// Four kinds of warps: one copies codes as the cache has them (bulk copies, up to three chunks on their way, their pages looked up a chunk ahead), four make them bf16, one issues the products, four have the
+// rows.  A cluster of blocks shares the chunks of a key head; their sums meet in shared memory.  SHARED: as in kv4_attn_kernel.
 // A row takes 32 keys at a time.  TWIN: up to 64 rows lie in the tile twice, rows 0 .. 63 take a chunk's first 32 keys and 64 .. 127 the others, each with zeros for weights of the other half and a reference
 // of its own: all four warps work on half of the scores where two would on all, and the products are no more.
+// Bound by instructions and by the hand-offs between the warps: 8 x 7 rows over 16000 (64 heads over 8 of 128) 84 us, where the bytes ask for 17, 66 without making bf16 of codes, 79 without the softmax, 64
+// without either; 32 x 7 rows 268; 512 rows over 8000 (32 heads over 8 of 64) 97, 89, 71 and 64.  Two blocks to an SM hide each other's hand-offs (one with chunks of 128 keys: 109 where two had 104).  Loads
+// by the warps that make bf16 cost more than the copies (95 and 91), one chunk of copies more than three (91 and 85), which fit because keys have one stage: they are written while the values' product runs.
 #pragma once
 #include "kv4_attention.cuh"
 #include "prompt_attention.cuh"
