@@ -151,11 +151,13 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
   const int seen = max(0, min(len, ctx + tq)), seen_by_all = ctx + 1;   // positions that some row sees, that all do
   const int chunks = (seen + K - 1) / K, front = SHARED ? turn : rank;   // chunk i of this piece is front + i C
   const int n = SHARED ? lost ? 0 : max(0, min(chunks, last_turn) - turn) : front < chunks ? (chunks - front + C - 1) / C : 0;
-  // Chunk i is in stage and on barriers use(i), parity(i) is that use's.  A wait by parity is only right while the barrier is in that use or the one behind it:
-  //   k_full, v_full: whoever waits for chunk i has to be through with it before its stage is written anew (the keys' behind s_full, the values' behind pv_done, which needs every row's P).
-  //   s_full: the producers and the rows ask for chunk i, and chunk i + 2's needs keys of the former and, through p_full, P of the latter.
+  // Chunk i is on barriers use(i), its values and positions in that stage (keys have one), parity(i) is that use's.  A wait by parity is only right while the barrier is in that use or the one behind it:
+  //   k_full, v_full: whoever waits for chunk i has to be through with it before the next but one comes: keys are written behind the scores of the chunk in front, values behind the product of the one before that,
+  //     which needs every row's P.
+  //   s_full: the producers and the rows ask for chunk i; chunk i + 2's needs chunk i + 1's keys, behind the former's wait, and through pv_done P of the latter.
   //   p_full: chunk i + 2's needs the rows to have seen its scores, which are issued behind the product of chunk i.
-  //   pv_done: the scores of chunk i + 1 ask for chunk i - 1; the producers ask for chunk i - 2 before they bring chunk i's values; the rows ask for chunk i - 1, and chunk i + 1's product needs their P.
+  //   pv_done: the scores of chunk i + 1 ask for chunk i - 1; the producers ask for chunk i - 2 before they write chunk i's values; the rows ask for chunk i - 1, and chunk i + 1's product needs their P.
+  //   codes_full, codes_free (kKv4Copies of either, in turn): the producers ask for chunk i, whose place is filled again only when they have freed it, and each use is freed once.
   auto use = [&](int i) { return (done + i) & 1; };
   auto parity = [&](int i) { return (uint32_t)((done + i) >> 1) & 1u; };
   float l = 0.f, m = -INFINITY;
