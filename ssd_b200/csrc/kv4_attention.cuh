@@ -51,12 +51,16 @@ constexpr int kv4_attn_smem(int HD, int NT, int W) {
   return ring > join ? ring : join;
 }
 
+// (x & a) | b in one operation (two constants would be two)
+SSDK_DEVINL uint32_t and_or(uint32_t x, uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(x), "r"(a), "r"(b));
+  return d;
+}
 // nibbles P and P + 4 of a word as 16 + c in bf16
 template <int P>
 SSDK_DEVINL uint32_t kv4_pair16(uint32_t w) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(P == 0 ? w << 3 : w >> (4 * P - 3)), "r"(0x00780078u), "r"(0x41804180u));   // (x & a) | b
-  return d;
+  return and_or(P == 0 ? w << 3 : w >> (4 * P - 3), 0x00780078u, 0x41804180u);
 }
 SSDK_DEVINL uint32_t transpose_8x8(uint32_t x) {
   uint32_t d;
@@ -84,7 +88,7 @@ SSDK_DEVINL int kv4_v_place(int r, int c) {
 // nibble P of both halves of a word as 16 + c (128 + c for the first) in bf16
 template <int P>
 SSDK_DEVINL uint32_t kv4_nibble(uint32_t w) {
-  return P == 0 ? (w & 0x000f000fu) | 0x43004300u : (w >> (4 * P - 3) & 0x00780078u) | 0x41804180u;
+  return P == 0 ? and_or(w, 0x000f000fu, 0x43004300u) : and_or(w >> (4 * P - 3), 0x00780078u, 0x41804180u);
 }
 
 // ---- shares of all turns: turn x of the row of them is one of the key heads of sequence b, kv_heads * (turns of a head of those in front) + head * turns(b) + ..; fewer than 2^31 in all (the host sees
