@@ -14,6 +14,12 @@ constexpr int kv4_row_bytes(int HD) { return HD / 2 + 4; }   // of a token and h
 constexpr uint32_t kKv4Nan = 0x7fc07fc0u;
 
 #ifndef SSDK_HOST_EMU
+// (x & a) | b in one operation (two constants would be two)
+SSDK_DEVINL uint32_t and_or(uint32_t x, uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(x), "r"(a), "r"(b));
+  return d;
+}
 // 1 where a >= b, else 0
 SSDK_DEVINL float one_if_ge(float a, float b) {
   float d;
@@ -371,7 +377,7 @@ SSDK_DEVINL uint4 kv4_values(uint32_t codes, uint32_t pair) {
   const float s = __uint_as_float(pair << 16), m = __uint_as_float(pair & 0xffff0000u);
   float f[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = fmaf(s, (float)(codes >> (4 * i) & 15u), m);
+  for (int i = 0; i < 8; ++i) f[i] = fmaf(s, __uint_as_float(and_or(codes >> (4 * i), 15u, 0x4b000000u)) - 8388608.f, m);   // (2^23 + code: a conversion takes four times as long)
   return pack_bf16x8(f);
 }
 
@@ -381,10 +387,11 @@ __global__ void __launch_bounds__(kKv4LoadThreads) kv4_load_kernel(Kv4LoadParams
   pdl_wait();
   pdl_launch_dependents();
   const int piece = threadIdx.x % LPR, side = threadIdx.x % 32 / LPR;
-  const long long tiles = (long long)((p.M + SIDE * ROWS - 1) / (SIDE * ROWS)) * p.kv_heads, step = (long long)gridDim.x * (kKv4LoadThreads / 32);
+  const uint32_t kv_heads = p.kv_heads, block_size = p.block_size, tiles = (uint32_t)((p.M + SIDE * ROWS - 1) / (SIDE * ROWS)) * kv_heads, step = gridDim.x * (kKv4LoadThreads / 32);   // (below 2^31: the host sees to it)
   const size_t record = (size_t)p.block_size * kv4_row_bytes(HD), pairs = (size_t)p.block_size * (HD / 2);
-  for (long long tile = (long long)blockIdx.x * (kKv4LoadThreads / 32) + (threadIdx.x >> 5); tile < tiles; tile += step) {
-    const int m0 = (int)(tile / p.kv_heads) * (SIDE * ROWS) + side, head = (int)(tile % p.kv_heads);
+  for (uint32_t tile = blockIdx.x * (kKv4LoadThreads / 32) + (threadIdx.x >> 5); tile < tiles; tile += step) {
+    const uint32_t group = tile / kv_heads, head = tile - group * kv_heads;
+    const int m0 = (int)group * (SIDE * ROWS) + side;
     int slot[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
@@ -396,8 +403,8 @@ __global__ void __launch_bounds__(kKv4LoadThreads) kv4_load_kernel(Kv4LoadParams
     for (int i = 0; i < ROWS; ++i) {
       c[0][i] = c[1][i] = w[0][i] = w[1][i] = 0;
       if (slot[i] >= 0 && slot[i] < p.num_slots) {
-        const int page = slot[i] / p.block_size, off = slot[i] - page * p.block_size;
-        const size_t at = ((size_t)page * p.kv_heads + head) * record, code = at + (size_t)off * (HD / 2) + piece * 4, pair = at + pairs + (size_t)off * 4;
+        const uint32_t page = (uint32_t)slot[i] / block_size, off = slot[i] - page * block_size;
+        const size_t at = ((size_t)page * kv_heads + head) * record, code = at + (size_t)off * (HD / 2) + piece * 4, pair = at + pairs + (size_t)off * 4;
         c[0][i] = *reinterpret_cast<const uint32_t*>(p.k_cache + code);
         c[1][i] = *reinterpret_cast<const uint32_t*>(p.v_cache + code);
         w[0][i] = *reinterpret_cast<const uint32_t*>(p.k_cache + pair);

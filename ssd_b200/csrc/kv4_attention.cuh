@@ -51,12 +51,6 @@ constexpr int kv4_attn_smem(int HD, int NT, int W) {
   return ring > join ? ring : join;
 }
 
-// (x & a) | b in one operation (two constants would be two)
-SSDK_DEVINL uint32_t and_or(uint32_t x, uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(x), "r"(a), "r"(b));
-  return d;
-}
 // nibbles P and P + 4 of a word as 16 + c in bf16
 template <int P>
 SSDK_DEVINL uint32_t kv4_pair16(uint32_t w) {

@@ -188,6 +188,7 @@ int ssdk_load_kv4(const void* k_cache, const void* v_cache, const int32_t* slot_
   Launcher L = launcher(stream);
   const int tile = kv4_load_tile(head_dim), W = kKv4LoadThreads / 32;
   const int64_t tiles = (int64_t)((M + tile - 1) / tile) * kv_heads;
+  if (tiles >= (1ll << 31)) return fail("load_kv4: %d rows of %d heads", M, kv_heads);
   const dim3 grid((unsigned)std::min<int64_t>((tiles + W - 1) / W, kSms * 32)), block(kKv4LoadThreads);
   return head_dim == 64 ? L.go(kv4_load_kernel<64>, grid, block, 0, p) : L.go(kv4_load_kernel<128>, grid, block, 0, p);
 }

@@ -17,6 +17,7 @@ inline void __stcs(T* p, const T& v) { *p = v; }
 #include "pairs_emu.h"
 namespace ssdk {
 inline float one_if_ge(float a, float b) { return a >= b ? 1.f : 0.f; }
+inline uint32_t and_or(uint32_t x, uint32_t a, uint32_t b) { return (x & a) | b; }
 }  // namespace ssdk
 #include "../../ssd_b200/csrc/kv4.cuh"
 
