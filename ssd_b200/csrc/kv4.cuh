@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(kKv4StoreThreads, kv4_store_blocks(ROPE)) kv4_
 
 // ----------------------------------------------------------------------------------
 // kv4_load_kernel: value = s code + m of the rows in `slots`, rounded once; rows with a slot outside the cache are zero.
-// Bound by memory, mostly by what is written, 2 bytes a channel of 2.53: 64004 rows of 8 heads of 128 60 us, 86 % of the copy rate.  HD / 8 lanes own a row of a head, eight channels each; a warp takes kKv4LoadRows times as many rows
+// Bound by memory, mostly by what is written, 2 bytes a channel of 2.53: 64004 rows of 8 heads of 128 57 us, 91 % of the copy rate (with conversions and places in 64 bits 60).  HD / 8 lanes own a row of a head, eight channels each; a warp takes kKv4LoadRows times as many rows
 // as it has room for, all loads in front of the first use.
 // ----------------------------------------------------------------------------------
 struct Kv4LoadParams {

@@ -49,7 +49,7 @@ static Kv4Plan kv4_plan(int64_t units, int64_t keys, int resident, int most, int
   Kv4Plan plan = {1, 0};
   const int64_t slots = resident * kSms;
   int64_t least = INT64_MAX;
-  for (int c = 1; c <= most; c *= 2) {
+  for (int c = 1; c <= (units > 8 ? std::min(most, 8) : most); c *= 2) {   // (more than eight clusters of sixteen, which wait for one another's places: us with them and without, 4 contexts of 4000 17.1 and 9.8, 2 with 56 rows 32.6 and 20.5)
     const int64_t cost = (units * c + slots - 1) / slots * (512 + 16 * c + keys / c);
     if (cost < least) {
       least = cost;
@@ -57,10 +57,9 @@ static Kv4Plan kv4_plan(int64_t units, int64_t keys, int resident, int most, int
     }
   }
   // Equal stretches cost a second launch, but their time goes by the sum of all lengths, not by the longest, and more than the blocks of a cluster can share a head: they are taken where the clusters' cost
-  // passes share_from.  With a head or more to every place on the device blocks are dealt out as others end.  us, clusters and stretches, of the streaming kernel: one context of 16000 (8 heads) 15.7 and 17.0,
-  // of 32000 25.7 and 22.3, of 64000 44.9 and 31.3, 4 of 32000 43.9 and 39.1, 16 of 8000 40.5 and 39.4, 48 of 16000 144 and 147, 148 of 4000 105 and 126; of 56 rows on tiles: one context of 8000 25.7 and
-  // 27.4, of 16000 35.6 and 32.8, of 32000 56 and 42, 4 of 16000 55.6 and 61, 8 of 4000 32.6 and 38, 8 of 16000 96 and 84, 16 of 4000 52 and 56, 16 of 16000 175 and 145, 32 of 16000 334 and 268 (the other
-  // way: 2 of 4000, 32.7 and 28.2).
+  // passes share_from.  With a head or more to every place on the device blocks are dealt out as others end.  us, clusters and stretches, of the streaming kernel: one context of 8000 (8 heads) 10.6
+  // and 11.7, of 16000 14.7 and 14.8, of 32000 23.5 and 20.5, of 64000 40 and 26.7, 8 of 8000 24 and 26.5, 16 of 8000 37 and 35, 48 of 16000 130 and 127, 148 of 4000 94 and 112; of 56 rows on tiles: one context of 8000 25.7 and
+  // 27.4, of 16000 35.6 and 32.8, of 32000 56 and 42, 4 of 16000 55.6 and 61, 8 of 4000 32.6 and 38, 8 of 16000 96 and 84, 16 of 4000 52 and 56, 16 of 16000 175 and 145, 32 of 16000 334 and 268.
   if (may_share && least > share_from && units < slots && units * ((keys + turn - 1) / turn) < (1ll << 31)) plan.blocks = (int)std::min(std::min(slots, units * 64), units * ((keys + turn - 1) / turn));
   return plan;
 }
