@@ -274,6 +274,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
       const int64_t from = page * page_step + head, codes = from + off * CODES, two = from + pairs + off * 4;
       if (lane < 4) codes_pos[c][lane] = is ? pos : kNoPosition;
       const int count = __popc(__ballot_sync(0xffffffffu, is));
+      __syncwarp();   // (all four positions are there before lane 0 arrives for them: a vote orders no memory)
       if (lane == 0) mbar_arrive_expect_tx(&codes_full[c], (uint32_t)(count * 32 * kv4_row_bytes(HD)));
       __syncwarp();
       if (is) {
