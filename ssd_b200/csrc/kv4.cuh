@@ -26,12 +26,31 @@ SSDK_DEVINL float one_if_ge(float a, float b) {
   asm("set.ge.f32.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
+// two differences a - b, rounded toward zero
+SSDK_DEVINL uint64_t less2_rz(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("sub.rz.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+#else   // the same on the host
+inline float less_rz(float x, float y) {
+  const double a = x, b = y, d = a - b, t = d - a, rest = (a - (d - t)) - (b + t);   // d + rest is the difference
+  const float f = (float)d;
+  return std::fabs((double)f) > std::fabs(d) || ((double)f == d && rest * d < 0) ? std::nextafter(f, 0.f) : f;
+}
+inline uint64_t less2_rz(uint64_t a, uint64_t b) {
+  float x[2], y[2];
+  unpack2(a, x, x + 1);
+  unpack2(b, y, y + 1);
+  return pack2(less_rz(x[0], y[0]), less_rz(x[1], y[1]));
+}
 #endif
 
 // Codes of a row whose 16 x LPH values lie with LPH neighbouring lanes, 16 a lane in two pieces of eight.  code: a word of eight channels for each piece; pair: scale | minimum;
 // VALUES: the pieces become what the codes stand for.
 // A quotient is often a code and a half exactly (x - m has some sixteen bits, s has eight), where a product with 1 / s goes either way.  So the product is made with something below
-// 1 / s, which gives the code or the one in front of it, and what it leaves, x - m - code s, is exact in fp32 and decides.  The nearest whole number stands in the low bits of
+// 1 / s, which gives the code or the one in front of it, and what it leaves, x - m - code s, is exact in fp32 and decides.  (x - m itself is not, where one of them lies far below the other: it is rounded down,
+// which never brings a value to a border that it lies under, and borders are fp32 numbers.)  The nearest whole number stands in the low bits of
 // (x - m) r + 1.5 2^23; these words are put together as they are, and their constant parts taken off at the end.  Two values at once: seven instructions a value (32003 rows of 16 heads of 128
 // 105 us with one at a time, twice as many; see kv4_store_kernel).
 template <int LPH, bool VALUES>
@@ -60,13 +79,13 @@ SSDK_DEVINL void kv4_codes(uint4& x, uint4& y, uint32_t (&code)[2], uint32_t& pa
   const float r = s > 0.f ? 1.f / s * (1.f - 0x1p-20f) : 0.f, half = s > 0.f ? 0.5f * s : INFINITY;
   constexpr float kWhole = 12582912.f;   // 1.5 2^23, the word 0x4b400000
   constexpr uint32_t kOff = 0x4b400000u * 0x11111111u;
-  const uint64_t one2 = pack2(1.f, 1.f), r2 = pack2(r, r), whole2 = pack2(kWhole, kWhole), less2 = pack2(-kWhole, -kWhole), minus_m2 = pack2(-m, -m), m2 = pack2(m, m), s2 = pack2(s, s), minus_s2 = pack2(-s, -s);
+  const uint64_t one2 = pack2(1.f, 1.f), r2 = pack2(r, r), whole2 = pack2(kWhole, kWhole), less2 = pack2(-kWhole, -kWhole), m2 = pack2(m, m), s2 = pack2(s, s), minus_s2 = pack2(-s, -s);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint32_t acc = 0;
 #pragma unroll
     for (int i = 3; i >= 0; --i) {
-      const uint64_t d = fma2((uint64_t)(w[h][i] & 0xffff0000u) << 32 | w[h][i] << 16, one2, minus_m2), c = fma2(fma2(d, r2, whole2), one2, less2);
+      const uint64_t d = less2_rz((uint64_t)(w[h][i] & 0xffff0000u) << 32 | w[h][i] << 16, m2), c = fma2(fma2(d, r2, whole2), one2, less2);
       float e0, e1;
       unpack2(fma2(c, minus_s2, d), &e0, &e1);
       const uint64_t up = fma2(c, one2, pack2(one_if_ge(e0, half), one_if_ge(e1, half)));   // the codes

@@ -1,6 +1,16 @@
-"""The paged cache held in 4 bits without a GPU, where it can go wrong: the order of hand-offs in its sources."""
+"""The paged cache held in 4 bits without a GPU, where it can go wrong: the order of hand-offs in its sources; the source of
+kv4_store_kernel on host threads against the definition in fractions, on rows at the borders of codes."""
 import re
 from pathlib import Path
+
+import numpy as np
+import pytest
+import torch
+
+from tests import kv4_exact as exact
+from tests.cache_ops_util import BF
+from tests.test_kv4_cpu import _run, _take, i32, needs_gxx
+from tests.test_kv4_gpu import same_bits
 
 CSRC = Path(__file__).resolve().parent.parent / "ssd_b200" / "csrc"
 
@@ -18,3 +28,23 @@ def test_positions_are_written_before_their_chunk_is_announced():
     assert len(written) == len(arrives) == 1
     between = body[written[0]:arrives[0]]
     assert "__syncwarp()" in between and between.rindex("__syncwarp()") < between.rindex("if (lane == 0)")
+
+
+# ---------------------------------------------------------------------------------------------------- codes and values
+def _stored(tmp_path, x, values):
+    """Rows x [M, 1, hd] stored as keys and as values by the kernel's source: caches (and values) as it leaves them."""
+    M, KV, hd = x.shape
+    pages = -(-M // 16)
+    data = _run("store", [i32([M, 0, KV, hd, 0, 0, 16, pages, 0, int(values), 16]), np.float32([0]), np.zeros(M, np.int64), torch.arange(M, dtype=torch.int32), torch.zeros(2 * hd, dtype=BF),
+                          torch.cat([x, x], 1), torch.zeros(2, pages, KV, 16 * (hd // 2 + 4), dtype=torch.uint8)], tmp_path)
+    return _take(data, *[(torch.uint8, (pages, KV, 16 * (hd // 2 + 4)))] * 2, *[(BF, (M, KV, hd))] * (2 * values))
+
+
+@needs_gxx
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows", [exact.far_below_borders, exact.every_scale])
+def test_codes_at_borders(tmp_path, rows, hd):
+    x = rows(hd)
+    want, _ = exact.cache_of(x, range(len(x)), -(-len(x) // 16), 16)
+    for got in _stored(tmp_path, x, False):
+        same_bits(got, want)
