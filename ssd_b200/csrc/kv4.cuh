@@ -32,6 +32,17 @@ SSDK_DEVINL uint64_t less2_rz(uint64_t a, uint64_t b) {
   asm("sub.rz.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+// a - b and a b + c of two bf16 values, each rounded once
+SSDK_DEVINL uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+SSDK_DEVINL uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
 #else   // the same on the host
 inline float less_rz(float x, float y) {
   const double a = x, b = y, d = a - b, t = d - a, rest = (a - (d - t)) - (b + t);   // d + rest is the difference
@@ -44,7 +55,34 @@ inline uint64_t less2_rz(uint64_t a, uint64_t b) {
   unpack2(b, y, y + 1);
   return pack2(less_rz(x[0], y[0]), less_rz(x[1], y[1]));
 }
+inline uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t out[2];
+  for (int i = 0; i < 2; ++i) {
+    const double p = (double)__uint_as_float(a >> (16 * i) << 16) * __uint_as_float(b >> (16 * i) << 16), q = __uint_as_float(c >> (16 * i) << 16), d = p + q, t = d - p, rest = (p - (d - t)) + (q - t);
+    float f = (float)d;   // toward zero, the last bit set where that is not the sum: such a number is rounded once more as the sum would be
+    if (std::isfinite(d) && ((double)f != d || rest != 0)) {
+      if (std::fabs((double)f) > std::fabs(d) || ((double)f == d && rest * d < 0)) f = std::nextafter(f, 0.f);
+      f = __uint_as_float(__float_as_uint(f) | 1u);
+    }
+    out[i] = pack_bf16x2(f, 0.f);
+  }
+  return out[1] << 16 | out[0];
+}
+inline uint32_t sub_bf16x2(uint32_t a, uint32_t b) { return fma_bf16x2(0x3f803f80u, a, b ^ 0x80008000u); }
 #endif
+
+// nibbles P and P + 4 of a word as 16 + c in bf16, and as scale c + low, both of which are there twice
+template <int P>
+SSDK_DEVINL uint32_t kv4_pair16(uint32_t w) {
+  return and_or(P == 0 ? w << 3 : w >> (4 * P - 3), 0x00780078u, 0x41804180u);
+}
+template <int P>
+SSDK_DEVINL uint32_t kv4_value(uint32_t w, uint32_t scale, uint32_t low) {
+  return fma_bf16x2(sub_bf16x2(kv4_pair16<P>(w), 0x41804180u), scale, low);
+}
+// a pair's scale and minimum, twice each
+SSDK_DEVINL uint32_t kv4_scales(uint32_t pair) { return __byte_perm(pair, 0, 0x1010); }
+SSDK_DEVINL uint32_t kv4_lows(uint32_t pair) { return __byte_perm(pair, 0, 0x3232); }
 
 // Codes of a row whose 16 x LPH values lie with LPH neighbouring lanes, 16 a lane in two pieces of eight.  code: a word of eight channels for each piece; pair: scale | minimum;
 // VALUES: the pieces become what the codes stand for.
@@ -79,7 +117,7 @@ SSDK_DEVINL void kv4_codes(uint4& x, uint4& y, uint32_t (&code)[2], uint32_t& pa
   const float r = s > 0.f ? 1.f / s * (1.f - 0x1p-20f) : 0.f, half = s > 0.f ? 0.5f * s : INFINITY;
   constexpr float kWhole = 12582912.f;   // 1.5 2^23, the word 0x4b400000
   constexpr uint32_t kOff = 0x4b400000u * 0x11111111u;
-  const uint64_t one2 = pack2(1.f, 1.f), r2 = pack2(r, r), whole2 = pack2(kWhole, kWhole), less2 = pack2(-kWhole, -kWhole), m2 = pack2(m, m), s2 = pack2(s, s), minus_s2 = pack2(-s, -s);
+  const uint64_t one2 = pack2(1.f, 1.f), r2 = pack2(r, r), whole2 = pack2(kWhole, kWhole), less2 = pack2(-kWhole, -kWhole), m2 = pack2(m, m), minus_s2 = pack2(-s, -s);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint32_t acc = 0;
@@ -92,10 +130,10 @@ SSDK_DEVINL void kv4_codes(uint4& x, uint4& y, uint32_t (&code)[2], uint32_t& pa
       float u0, u1;
       unpack2(fma2(up, one2, whole2), &u0, &u1);
       acc = acc * 256u + (__float_as_uint(u1) * 16u + __float_as_uint(u0));
-      if (VALUES) {
-        float v0, v1;
-        unpack2(fma2(up, s2, m2), &v0, &v1);
-        w[h][i] = pack_bf16x2(v0, v1);
+      if (VALUES) {   // (by way of fp32 a value would be rounded twice)
+        float c0, c1;
+        unpack2(up, &c0, &c1);
+        w[h][i] = fma_bf16x2(pack_bf16x2(c0, c1), kv4_scales(pair), kv4_lows(pair));
       }
     }
     code[h] = fine ? acc - kOff : 0u;
@@ -379,7 +417,7 @@ __global__ void __launch_bounds__(kKv4StoreThreads, kv4_store_blocks(ROPE)) kv4_
 
 // ----------------------------------------------------------------------------------
 // kv4_load_kernel: value = s code + m of the rows in `slots`, rounded once; rows with a slot outside the cache are zero.
-// Bound by memory, mostly by what is written, 2 bytes a channel of 2.53: 64004 rows of 8 heads of 128 57 us, 91 % of the copy rate (with conversions and places in 64 bits 60).  HD / 8 lanes own a row of a head, eight channels each; a warp takes kKv4LoadRows times as many rows
+// Bound by memory, mostly by what is written, 2 bytes a channel of 2.53: 64004 rows of 8 heads of 128 56 us, 92 % of the copy rate (codes to floats without conversions, two channels at once; with conversions and places in 64 bits 60).  HD / 8 lanes own a row of a head, eight channels each; a warp takes kKv4LoadRows times as many rows
 // as it has room for, all loads in front of the first use.
 // ----------------------------------------------------------------------------------
 struct Kv4LoadParams {
@@ -393,11 +431,9 @@ constexpr int kKv4LoadThreads = 256, kKv4LoadRows = 4;
 constexpr int kv4_load_tile(int HD) { return 32 / (HD / 8) * kKv4LoadRows; }   // rows of a warp's tile, of one head
 
 SSDK_DEVINL uint4 kv4_values(uint32_t codes, uint32_t pair) {
-  const float s = __uint_as_float(pair << 16), m = __uint_as_float(pair & 0xffff0000u);
-  float f[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = fmaf(s, __uint_as_float(and_or(codes >> (4 * i), 15u, 0x4b000000u)) - 8388608.f, m);   // (2^23 + code: a conversion takes four times as long)
-  return pack_bf16x8(f);
+  const uint32_t s = kv4_scales(pair), m = kv4_lows(pair);
+  const uint32_t v[4] = {kv4_value<0>(codes, s, m), kv4_value<1>(codes, s, m), kv4_value<2>(codes, s, m), kv4_value<3>(codes, s, m)};   // channels P and P + 4
+  return make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
 }
 
 template <int HD>

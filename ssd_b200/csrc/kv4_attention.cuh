@@ -51,11 +51,6 @@ constexpr int kv4_attn_smem(int HD, int NT, int W) {
   return ring > join ? ring : join;
 }
 
-// nibbles P and P + 4 of a word as 16 + c in bf16
-template <int P>
-SSDK_DEVINL uint32_t kv4_pair16(uint32_t w) {
-  return and_or(P == 0 ? w << 3 : w >> (4 * P - 3), 0x00780078u, 0x41804180u);
-}
 SSDK_DEVINL uint32_t transpose_8x8(uint32_t x) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));

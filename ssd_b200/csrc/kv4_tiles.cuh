@@ -29,14 +29,6 @@ constexpr int kv4_tile_smem(int HD) {
   return (body > join ? body : join) + 1024;
 }
 
-// nibbles P and P + 4 of a word as bf16(scale x code + minimum), both of which are there twice
-template <int P>
-SSDK_DEVINL uint32_t kv4_value(uint32_t w, uint32_t scale, uint32_t low) {
-  uint32_t d;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(kv4_pair16<P>(w)), "r"(0x41804180u));
-  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(d), "r"(scale), "r"(low));
-  return d;
-}
 SSDK_DEVINL uint4 kv4_value8(uint32_t w, uint32_t scale, uint32_t low) {
   return make_uint4(kv4_value<0>(w, scale, low), kv4_value<1>(w, scale, low), kv4_value<2>(w, scale, low), kv4_value<3>(w, scale, low));
 }
@@ -214,7 +206,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
 #pragma unroll
     for (int j = 0; j < 4; ++j) to[j] = (piece >> 1) * kHalf + swizzled(row, (piece & 1) * 4 + (later ? j ^ 2 : j));
     auto write = [&](uint8_t* stage, const uint4& codes, uint32_t pair) {
-      const uint32_t scale = __byte_perm(pair, 0, 0x1010), low = __byte_perm(pair, 0, 0x3232);
+      const uint32_t scale = kv4_scales(pair), low = kv4_lows(pair);
       const uint32_t w[4] = {later ? codes.z : codes.x, later ? codes.w : codes.y, later ? codes.x : codes.z, later ? codes.y : codes.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stage + to[j]) = kv4_value8(w[j], scale, low);

@@ -1,5 +1,5 @@
-"""The paged cache held in 4 bits without a GPU, where it can go wrong: the order of hand-offs in its sources; the source of
-kv4_store_kernel on host threads against the definition in fractions, on rows at the borders of codes."""
+"""The paged cache held in 4 bits without a GPU, where it can go wrong: the order of hand-offs in its sources; the sources of
+kv4_store_kernel and kv4_load_kernel on host threads against the definition in fractions, on rows at the borders of codes and of bf16."""
 import re
 from pathlib import Path
 
@@ -47,4 +47,19 @@ def test_codes_at_borders(tmp_path, rows, hd):
     x = rows(hd)
     want, _ = exact.cache_of(x, range(len(x)), -(-len(x) // 16), 16)
     for got in _stored(tmp_path, x, False):
+        same_bits(got, want)
+
+
+@needs_gxx
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows", [exact.rounded_twice, exact.far_below_borders])
+def test_values_are_rounded_once(tmp_path, rows, hd):
+    """What a write returns and a read gives is scale x code + minimum rounded to bf16, not to fp32 first."""
+    x = rows(hd)
+    M, pages = len(x), -(-len(x) // 16)
+    cache, want = exact.cache_of(x, range(M), pages, 16)
+    for got in _stored(tmp_path, x, True)[2:]:
+        same_bits(got, want)
+    data = _run("load", [i32([M, 1, hd, 16, pages, 2]), cache, cache, torch.arange(M, dtype=torch.int32)], tmp_path)
+    for got in _take(data, *[(BF, (M, 1, hd))] * 2):
         same_bits(got, want)
