@@ -345,7 +345,8 @@ int ssdk_load_kv4(const void* k_cache, const void* v_cache, const int32_t* slot_
                   int M, int kv_heads, int head_dim, void* stream);
 /* ssdk_paged_attn_kv4: ssdk_paged_attn over the values scale * code + minimum, causal to the end of the context.  Up to sixteen query rows to a key head they are not rounded, with more they are rounded to
  * bf16, as ssdk_load_kv4 gives them (one that would pass bf16's largest number by that stays below it).  At most 32 query heads to a key head.  Pages outside the cache are passed over, lengths are held
- * to what a table has room for, a row that sees no key is zero.  A NaN row of the cache makes NaN of the rows that see it, a query that is not finite, or (up to sixteen rows) whose sum passes fp32, makes
+ * to what a table has room for, a row that sees no key is zero.  Weights below 2^-126 of the largest are
+ * zero (2^-94 beside values of 2^65 and more, next to which values below 2^-94 may lose bits).  A NaN row of the cache makes NaN of the rows that see it, a query that is not finite, or (up to sixteen rows) whose sum passes fp32, makes
  * its row NaN.  `scratch`: ssdk_paged_attn_kv4_scratch_bytes(...) bytes of the call's own (0: null).  More than sixteen query rows to a key head take a kernel with bounded waits: as with
  * ssdk_paged_attn_pages, a wait that runs out leaves NaN rows, and the next such call of the process returns an error. */
 int64_t ssdk_paged_attn_kv4_scratch_bytes(int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size, int max_blocks_per_seq);

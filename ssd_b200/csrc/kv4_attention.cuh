@@ -41,9 +41,11 @@ struct Kv4AttnParams {
   float scale_log2;              // scale * log2(e)
   float* parts;                  // SHARED: [blocks][2][rows of a key head][HD + 4]: O, reference, sum of a block's first stretch where it began in front of it, and of its last
 };
-// Weights are exp2(score - reference), the reference 2^32 above the largest score that it was raised for and raised again when a score passes that by 2^8: with the sum of weights all sums are 2^-32 of what they
-// would be, and values up to bf16's largest number (here times codes less 8 that come with 128 more) pass fp32's in none.  What that costs is weights below 2^-94 of the largest.
+// Weights are exp2(score - reference), the reference the largest score that it was raised for, raised again when a score passes that by 2^8.  Keys whose values have a scale or minimum of 2^65 or more find it
+// 2^32 above their scores: of them and the sum of weights all sums are 2^-32 of what they would be, and values up to bf16's largest number (here times codes less 8 that come with 128 more) pass fp32's in none.
+// What that costs is weights below 2^-94 of the largest (else 2^-126); in front of small values it would cost their own bits, since P s' is subnormal in bf16 then (for scales below 2^-94; zero from 2^-102 on).
 constexpr float kKv4Slack = 8.f, kKv4Above = 32.f;
+SSDK_DEVINL bool kv4_large(uint32_t pair) { return (pair & pair << 1 & 0x40004000u) != 0; }   // (an exponent's two top bits)
 constexpr int kKv4Most = 16, kKv4Stages = 3, kKv4Keys = 32;   // blocks of a cluster, a warp's ring, keys of a chunk
 constexpr int kv4_stage_bytes(int HD) { return 2 * kKv4Keys * (HD / 2 + 4); }   // keys' codes | values' codes | keys' pairs | values' pairs
 constexpr int kv4_attn_smem(int HD, int NT, int W) {
@@ -318,7 +320,7 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
 
   // scores of a chunk's keys g, g + 8, .. and rows 2 t, 2 t + 1 to weights, and their product with the values.  MASK: some row does not see some key, or a page is missing
   const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-  auto work = [&](const uint8_t* in, int x, int pos, uint32_t none, auto mask) {   // (x: which sixteen of the chunk)
+  auto work = [&](const uint8_t* in, int x, int pos, uint32_t none, bool large, auto mask) {   // (x: which sixteen of the chunk; large: some value of it is, kKv4Above)
     constexpr bool MASK = decltype(mask)::value;
     const uint32_t* pairs = reinterpret_cast<const uint32_t*>(in + 2 * K * CODES) + g;
     float s[NT][4];
@@ -371,15 +373,16 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
     }
     // a row's reference is raised, and its sums rescaled, only when a score passes it by kKv4Slack (base 2)
     float most[NT][2];
-    bool grow = false;
+    bool grow = large;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         most[nt][e] = fmaxf(s[nt][e], s[nt][2 + e]);
-        grow = grow || most[nt][e] > ref[nt][e] + (kKv4Slack - kKv4Above);
+        grow = grow || most[nt][e] > ref[nt][e] + kKv4Slack;
       }
     if (__any_sync(0xffffffffu, grow)) {
+      const float above = __any_sync(0xffffffffu, large) ? kKv4Above : 0.f;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -387,7 +390,7 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
           float top = most[nt][e];
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) + kKv4Above, ref[nt][e]);
+          top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) + above, ref[nt][e]);
           const float f = top == ref[nt][e] ? 1.f : ex2_ftz(ref[nt][e] - top);   // (from -inf: 0)
           ref[nt][e] = top;
           l[nt][e] *= f;
@@ -459,12 +462,15 @@ __global__ void __launch_bounds__(W * 32, 16 / NT / W) kv4_attn_kernel(const __g
     __syncwarp();   // every lane's copies of this stage have landed
     const int pos = (own + i * stride) * K;
     const uint32_t none = missing >> (2 * stage) & 3u;
-    if (pos + K <= seen_by_all && !none) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) work(ring + stage * STAGE, x, pos, 0u, std::false_type());
-    } else {
+    const bool whole = pos + K <= seen_by_all && !none;
+    const bool large = kv4_large(reinterpret_cast<const uint32_t*>(ring + stage * STAGE + 2 * K * CODES)[K + lane]);   // a lane looks at one pair of the values
+    if (whole) {
+      work(ring + stage * STAGE, 0, pos, 0u, large, std::false_type());
+      work(ring + stage * STAGE, 1, pos, 0u, large, std::false_type());
+    } else {   // (behind the context's end, seen_by_all + Q - 1, or without a page a pair may be anything)
+      const bool there = large && pos + lane < seen_by_all + p.Q - 1 && !(none >> (lane >> 4) & 1u);
 #pragma unroll 1
-      for (int x = 0; x < 2; ++x) work(ring + stage * STAGE, x, pos, none, std::true_type());
+      for (int x = 0; x < 2; ++x) work(ring + stage * STAGE, x, pos, none, there, std::true_type());
     }
     if ((i & 7) == 7) take_off();
   }

@@ -16,6 +16,8 @@
 // without either; 32 x 7 rows 268; 512 rows over 8000 (32 heads over 8 of 64) 97, 89, 71 and 64.  Two blocks to an SM hide each other's hand-offs (one with chunks of 128 keys: 109 where two had 104).  Loads
 // by the warps that make bf16 cost more than the copies (95 and 91), one chunk of copies more than three (91 and 85), which fit because keys have one stage: they are written while the values' product runs.
 #pragma once
+#include <climits>
+
 #include "kv4_attention.cuh"
 #include "prompt_attention.cuh"
 
@@ -63,6 +65,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
   __shared__ __align__(8) uint64_t k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], codes_full[kKv4Copies], codes_free[kKv4Copies];
   __shared__ int codes_pos[kKv4Copies][4];                 // where a chunk's four sixteens of keys that were copied are in their context: behind every one where they have no page
   __shared__ __align__(16) int at_pos[2][4];   // position of a chunk's sixteen keys, behind every context where they have no page
+  __shared__ int first_large;                  // the first chunk of this piece with large values (kKv4Above), of those that have been made bf16
   __shared__ float row_units[kKv4TileRows];   // of a row of queries: what a unit of its scores is (NaN: it is not finite)
   __shared__ uint32_t tmem_slot;
   uint8_t* smem = kv4_tile_raw + ((1024u - (smem_u32(kv4_tile_raw) & 1023u)) & 1023u);
@@ -92,6 +95,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
         mbar_init(&codes_full[s], 1);
         mbar_init(&codes_free[s], kKv4Producers / 32);
       }
+      first_large = INT_MAX;
       fence_mbar_init();
     }
     __syncwarp();
@@ -236,6 +240,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
           k_pair[u] = 0x7fc07fc0u;
           v_pair[u] = 0;
         }
+        if (kv4_large(v_pair[u])) atomicMin(&first_large, done + i);
       }
       if (done + i >= 1 && !tile_wait_warp(&s_full[use(i - 1)], parity(i - 1), pp.timeout)) break;   // the scores of chunk i - 1 have read their keys
 #pragma unroll
@@ -330,7 +335,9 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     const float unit = row_units[at];
     for (int i = 0; i < n && ok; ++i) {
       const uint32_t sp = tmem + lanes + (uint32_t)use(i) * 64u;
-      if (!(ok = tile_wait_warp(&v_full[use(i)], parity(i), pp.timeout) && tile_wait_warp(&s_full[use(i)], parity(i), pp.timeout))) break;
+      if (!(ok = tile_wait_warp(&v_full[use(i)], parity(i), pp.timeout))) break;
+      const float above = *(volatile int*)&first_large <= done + i ? kKv4Above : 0.f;
+      if (!(ok = tile_wait_warp(&s_full[use(i)], parity(i), pp.timeout))) break;
       tc_fence_after();
 #pragma unroll 1
       for (int h = TWIN ? warp >> 1 : 0; h < (TWIN ? (warp >> 1) + 1 : 2); ++h) {   // 32 keys
@@ -354,10 +361,10 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
 #pragma unroll
           for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(u[c + e]), __uint_as_float(u[c + 4 + e]));
         const float mx = fmaxf(max3(max3(top[0], top[1], __uint_as_float(u[28])), max3(top[2], top[3], __uint_as_float(u[29])), __uint_as_float(u[30])), __uint_as_float(u[31])) * unit;
-        const bool grow = mx > m + (kKv4Slack - kKv4Above);
+        const bool grow = mx > m + (kKv4Slack - above);
         if (__any_sync(0xffffffffu, grow)) {
-          const float f = grow ? exp2f(m - (mx + kKv4Above)) : 1.f;   // (m = -inf: 0)
-          if (grow) m = mx + kKv4Above;
+          const float f = grow ? exp2f(m - (mx + above)) : 1.f;   // (m = -inf: 0)
+          if (grow) m = mx + above;
           l *= f;
           if (i > 0) {
             if (!(ok = tile_wait_warp(&pv_done[use(i - 1)], parity(i - 1), pp.timeout))) break;
@@ -492,6 +499,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
   if constexpr (SHARED) {
     at += last_turn - turn;
     done += n;
+    if (threadIdx.x == 0) first_large = INT_MAX;
     lost = __syncthreads_or(!ok) != 0;   // (and the sums are read: their memory is the queries' and stages' again)
   } else {
     cluster.sync();   // no block leaves while its part is read
