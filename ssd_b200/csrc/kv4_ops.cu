@@ -28,7 +28,7 @@ static int launch_store(Launcher& L, Kv4StoreParams p) {
   constexpr int SIDE = kv4_store_heads(HD), W = kKv4StoreThreads / 32;
   p.groups = ((ROPE ? p.heads : 0) + 2 * p.kv_heads + SIDE - 1) / SIDE;
   const int64_t units = (int64_t)p.M * p.groups;
-  if (units >= (1ll << 31)) return fail("store_kv4: %d rows of %d heads", p.M, p.heads + 2 * p.kv_heads);
+  if (units >= (1ll << 31)) return fail("%s: %d rows of %d heads", ROPE ? "rope_store_kv4" : "store_kv4", p.M, p.heads + 2 * p.kv_heads);
   p.warps = (int)std::min<int64_t>(units, kSms * kv4_store_blocks(ROPE) * W);
   p.each = (int)(units / p.warps);
   p.longer = (int)(units - (int64_t)p.each * p.warps);

@@ -63,3 +63,15 @@ def test_values_are_rounded_once(tmp_path, rows, hd):
     data = _run("load", [i32([M, 1, hd, 16, pages, 2]), cache, cache, torch.arange(M, dtype=torch.int32)], tmp_path)
     for got in _take(data, *[(BF, (M, 1, hd))] * 2):
         same_bits(got, want)
+
+
+# ---------------------------------------------------------------------------------------------------- refusals
+def test_too_many_heads_of_rows_are_refused_by_their_own_name():
+    """More groups of heads than 32 bits count, arrays far apart: the call that is refused says who it is."""
+    from ssd_b200 import lib
+    so, P = lib.load(), 1 << 50   # addresses that no call gets to use
+    rope = [P, 2 * P, 3 * P, 4 * P, 100, 64, None, None, 1e-6, *(P * i for i in range(5, 10)), 2, 16, 1 << 20, 65535, 1, 64, None]
+    rows = [P, 2 * P, 64 * 65535, 64 * 65535, *(P * i for i in range(3, 8)), 2, 16, 1 << 20, 65535, 64, None]
+    for name, args in (("rope_store_kv4", rope), ("store_kv4", rows)):
+        assert getattr(so, "ssdk_" + name)(*args) != 0
+        assert so.ssdk_last_error().decode().startswith(name + ": 1048576 rows of "), so.ssdk_last_error()
