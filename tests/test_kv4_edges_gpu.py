@@ -1,10 +1,12 @@
-"""The paged cache held in 4 bits on the GPU, where it can go wrong: rows at the borders of codes and of bf16 against the definition in fractions (tests/kv4_exact.py)."""
+"""The paged cache held in 4 bits on the GPU, where it can go wrong: rows at the borders of codes and of bf16 against the definition in fractions (tests/kv4_exact.py), values and scores of all sizes, attention on
+tiles to its own roundings (tests/kv4_tiles_plain.py), calls that no other test makes."""
 import pytest
 import torch
 
 from tests import kv4_exact as exact
 from tests import kv4_plain as plain
-from tests.cache_ops_util import BF, gen, within
+from tests import kv4_tiles_plain as tiles
+from tests.cache_ops_util import BF, angles, gen, within
 from tests.test_kv4_gpu import a_case, i32, same_bits
 
 pytestmark = pytest.mark.gpu
@@ -102,3 +104,104 @@ def test_large_values_among_small_ones(dev, Q, H, KV, hd, S, lens, width):
         far = slice(Q, None)   # (the other sequences see none of them)
         within(got, want, slack)
         within(got[far].double() * 2.0 ** 60, want[far] * 2.0 ** 60, slack[far] * 2.0 ** 60)
+
+
+@pytest.mark.parametrize("Q,H,KV,hd,S,lens,width", FORMS)
+@pytest.mark.parametrize("e", [-100, -60, 100])
+def test_scores_of_queries_and_keys_far_apart(dev, Q, H, KV, hd, S, lens, width, e):
+    """Keys 2^e as large under queries 2^-e as large: the same scores."""
+    from ssd_b200 import ops
+    g = gen(86, Q, H, hd)
+    kc, vc, table = a_case(g, KV, hd, S, lens, width=width)
+    q = torch.randn(len(lens) * Q, H, hd, generator=g).to(BF)
+    up = (q.double() * 2.0 ** -e).to(BF)   # (exact)
+    got = ops.paged_attention_kv4(up.to(dev), times(kc, hd, e).to(dev), vc.to(dev), table.to(dev), i32(lens, dev), Q, hd ** -0.5)
+    within(got, *plain.attention(q, kc, vc, table, lens, Q, hd ** -0.5))
+
+
+# ---------------------------------------------------------------------------------------------------- attention on tiles, to its own roundings
+def parts_of(B, Q, H, KV, hd, S, width):
+    """Bytes that a call leaves of its parts: not zero where blocks have equal stretches of all keys."""
+    from ssd_b200 import lib
+    return lib.load().ssdk_paged_attn_kv4_scratch_bytes(B, Q, H, KV, hd, S, width)
+
+
+@pytest.mark.parametrize("Q,H,KV,hd,S,lens,width,shared", [
+    (20, 8, 2, 64, 64, [9000, 5, 0, 700], 400, True), (11, 9, 1, 64, 80, [12000, 63, 65], 200, True), (128, 1, 1, 64, 16, [6000, 300], 500, True),   # heads of 64, one tile whose rows lie in it once
+    (16, 8, 1, 128, 256, [9000, 40], 80, True), (7, 8, 1, 128, 64, [8000, 9, 70], 300, True), (5, 8, 2, 64, 64, [9000, 17], 400, True),
+    (20, 8, 2, 64, 64, [300, 20], None, False), (7, 8, 1, 128, 256, [700, 7, 8], None, False), (3, 32, 1, 64, 16, [100, 64], None, False), (300, 2, 1, 128, 48, [700], None, False),
+    (77, 6, 2, 64, 4096, [5000, 76], None, False),
+])
+def test_tiles_to_their_own_roundings(dev, Q, H, KV, hd, S, lens, width, shared):
+    """Over keys and values in bf16, as load_kv4 gives them, and over scale x code + minimum as they are."""
+    from ssd_b200 import ops
+    g = gen(83, Q, H, KV, hd, S)
+    kc, vc, table = a_case(g, KV, hd, S, lens, width=width)
+    assert bool(parts_of(len(lens), Q, H, KV, hd, S, table.shape[1])) == shared
+    q = torch.randn(len(lens) * Q, H, hd, generator=g).to(BF)
+    got = ops.paged_attention_kv4(q.to(dev), kc.to(dev), vc.to(dev), table.to(dev), i32(lens, dev), Q, hd ** -0.5)
+    for rounded in (True, False):
+        within(got, *tiles.attention(q, kc, vc, table, lens, Q, hd ** -0.5, rounded))
+
+
+def test_a_prompt_over_what_its_write_returns(dev):
+    """Rotation and write of a prompt's rows, attention over the cache: softmax over the values that the write returned, to the kernel's roundings; its last tokens again, few rows to a key head."""
+    from ssd_b200 import ops
+    g = gen(84)
+    M, H, KV, hd, S = 150, 8, 2, 64, 16
+    qkv = torch.randn(M, (H + 2 * KV) * hd, generator=g).to(BF).to(dev)
+    kc, vc = ops.kv4_caches(12, S, KV, hd, dev)
+    table = torch.randperm(12, generator=g)[:10].to(torch.int32)[None].to(dev)
+    pos = torch.arange(M, device=dev)
+    slots = (table[0, pos // S] * S + pos % S).to(torch.int32)
+    q, k, v = ops.rope_store_kv4(qkv, pos, slots, angles(M, hd).to(dev), kc, vc, H, KV, hd, values=True)
+    q = q.view(M, H, hd)
+    got = ops.paged_attention_kv4(q, kc, vc, table, i32([M], dev), M, 0.125)
+    few = ops.paged_attention_kv4(q[-3:], kc, vc, table, i32([M], dev), 3, 0.125)
+    seen = (torch.arange(M) <= torch.arange(M)[:, None]).repeat_interleave(H // KV, 0)
+    want, slack = torch.empty(2, M, H, hd, dtype=torch.float64).unbind(0)
+    for h in range(KV):
+        heads = slice(h * H // KV, (h + 1) * H // KV)
+        out = tiles.attend(q[:, heads].double().cpu().reshape(-1, hd), k[:, h].double().cpu(), v[:, h].double().cpu(), seen, 0.125)
+        for t, x in zip((want, slack), out):
+            t[:, heads] = x.view(M, -1, hd)
+    within(got, want.view(M, -1), slack.view(M, -1))
+    within(few, *plain.attention(q[-3:].cpu(), kc.cpu(), vc.cpu(), table.cpu(), [M], 3, 0.125))
+
+
+@pytest.mark.parametrize("Q,H", [(1, 2), (20, 1)])
+def test_more_sequences_than_share_a_launch(dev, Q, H):
+    """Beyond 1024 sequences no block goes through all lengths: clusters take long tables too."""
+    from ssd_b200 import ops
+    g = gen(85, Q)
+    B, KV, hd, S = 1100, 1, 64, 16
+    lens = [(7 * i) % 40 for i in range(B)]
+    lens[3], lens[1050], lens[1099] = 900, 1500, 33
+    kc, vc, table = a_case(g, KV, hd, S, lens, width=2000)
+    assert parts_of(B, Q, H, KV, hd, S, 2000) == 0 and parts_of(64, Q, H, KV, hd, S, 2000) > 0
+    q = torch.randn(B * Q, H, hd, generator=g).to(BF)
+    got = ops.paged_attention_kv4(q.to(dev), kc.to(dev), vc.to(dev), table.to(dev), i32(lens, dev), Q, 0.125)
+    within(got, *(plain.attention(q, kc, vc, table, lens, Q, 0.125) if Q == 1 else tiles.attention(q, kc, vc, table, lens, Q, 0.125, True)))
+
+
+@pytest.mark.parametrize("which", ["q", "k"])
+def test_one_norm_of_the_two(dev, which):
+    """A norm of queries without one of keys, and the other way round."""
+    from ssd_b200 import ops
+    g = gen(87)
+    M, H, KV, hd, S, eps = 41, 5, 2, 128, 16, 1e-5
+    qkv = torch.randn(M, (H + 2 * KV) * hd, generator=g).to(BF)
+    w = (1 + 0.2 * torch.randn(hd, generator=g)).to(BF)
+    qn, kn = (w, None) if which == "q" else (None, w)
+    table, positions, slots = angles(60, 64), torch.randint(0, 60, (M,), generator=g), torch.randperm(64, generator=g)[:M].to(torch.int32)
+    kc, vc = plain.empty(4, S, KV, hd), plain.empty(4, S, KV, hd)
+    kd, vd = kc.to(dev), vc.to(dev)
+    up = lambda t: None if t is None else t.to(dev)  # noqa: E731
+    got = ops.rope_store_kv4(up(qkv), up(positions), up(slots), up(table), kd, vd, H, KV, hd, up(qn), up(kn), eps)
+    x = qkv.view(M, -1, hd)
+    want, size = plain.turned(x[:, :H], positions, table, qn, eps)
+    within(got, want.view(M, -1), (want.abs() * 2 ** -8 + size * 2 ** -19).view(M, -1))   # (test_rope_store_kv4 has the bound's parts)
+    plain.put(kc, hd, plain.rounded(plain.turned(x[:, H:H + KV], positions, table, kn, eps)[0]), slots)
+    plain.put(vc, hd, x[:, H + KV:], slots)
+    same_bits(kd, kc)
+    same_bits(vd, vc)
