@@ -154,23 +154,6 @@ struct RopeAxesParams {
 constexpr int kRopeAxesThreads = 128, kRopeAxesAhead = 2;
 constexpr int rope_axes_heads(int HD) { return 32 / (HD / 16) * kRopeAxesAhead; }   // that a warp asks for at once
 
-// eight bf16 values as four pairs of fp32, and back
-SSDK_DEVINL void pairs_of(const uint4& v, uint64_t* f) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = (uint64_t)(w[i] & 0xffff0000u) << 32 | w[i] << 16;
-}
-SSDK_DEVINL uint4 bf16_of(const uint64_t* f) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float x, y;
-    unpack2(f[i], &x, &y);
-    w[i] = pack_bf16x2(x, y);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 template <int HD, bool NORM>
 __global__ void __launch_bounds__(kRopeAxesThreads, 4) rope_axes_kernel(RopeAxesParams p) {
   constexpr int LPH = HD / 16, SIDE = 32 / LPH;   // lanes of a head, heads side by side

@@ -218,24 +218,9 @@ SSDK_DEVINL void kv4_turn_f64(uint4& x, uint4& y, const __nv_bfloat16* w0, const
 // the same in fp32, two values at once
 template <int LPH>
 SSDK_DEVINL void kv4_turn_f32(uint4& x, uint4& y, const __nv_bfloat16* w0, const __nv_bfloat16* w1, float eps, bool turns, const uint64_t (&co)[4], const uint64_t (&si)[4]) {
-  auto pairs = [](const uint4& v, uint64_t* f) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = (uint64_t)(w[i] & 0xffff0000u) << 32 | w[i] << 16;
-  };
-  auto rounded = [](const uint64_t* f) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float a, b;
-      unpack2(f[i], &a, &b);
-      w[i] = pack_bf16x2(a, b);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  };
   uint64_t a[4], b[4];
-  pairs(x, a);
-  pairs(y, b);
+  pairs_of(x, a);
+  pairs_of(y, b);
   if (w0) {
     uint64_t sum2 = mul2(a[0], a[0]);
 #pragma unroll
@@ -250,10 +235,10 @@ SSDK_DEVINL void kv4_turn_f32(uint4& x, uint4& y, const __nv_bfloat16* w0, const
     const float scale = rsqrtf(s0 / (16.f * LPH) + eps);
     const uint64_t scale2 = pack2(scale, scale);
     uint64_t w[4];
-    pairs(*reinterpret_cast<const uint4*>(w0), w);
+    pairs_of(*reinterpret_cast<const uint4*>(w0), w);
 #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = mul2(mul2(a[i], scale2), w[i]);
-    pairs(*reinterpret_cast<const uint4*>(w1), w);
+    pairs_of(*reinterpret_cast<const uint4*>(w1), w);
 #pragma unroll
     for (int i = 0; i < 4; ++i) b[i] = mul2(mul2(b[i], scale2), w[i]);
   }
@@ -265,8 +250,8 @@ SSDK_DEVINL void kv4_turn_f32(uint4& x, uint4& y, const __nv_bfloat16* w0, const
       a[i] = t;
     }
   }
-  x = rounded(a);
-  y = rounded(b);
+  x = bf16_of(a);
+  y = bf16_of(b);
 }
 
 template <int HD, bool ROPE, bool VALUES>

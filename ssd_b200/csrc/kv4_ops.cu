@@ -11,7 +11,7 @@
 using namespace ssdk;
 typedef __nv_bfloat16 bf16;
 
-constexpr int kSms = 148, kMaxSmem = 227 * 1024 - 1024;   // (statics beside it)
+constexpr int kSms = 148;
 
 // a cache of pages whose slots are numbered in 32 bits
 static int check_kv4(const char* who, int64_t num_blocks, int block_size, int kv_heads, int head_dim) {

@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 2) kv4_tile_kernel(const __gr
     auto scores = [&](int i) {
       if (!tile_wait_warp(&k_full[use(i)], parity(i), pp.timeout)) return false;
       tc_fence_after();
-            const uint32_t to = tmem + (uint32_t)use(i) * 64u;
+      const uint32_t to = tmem + (uint32_t)use(i) * 64u;
       if (elect_one()) {
 #pragma unroll
         for (int h = 0; h < HALVES; ++h)

@@ -47,6 +47,23 @@ SSDK_DEVINL bool tile_wait(uint64_t* bar, uint32_t parity, unsigned* timeout) {
 SSDK_DEVINL bool tile_wait_warp(uint64_t* bar, uint32_t parity, unsigned* timeout) { return __all_sync(0xffffffffu, tile_wait(bar, parity, timeout)); }
 #endif
 
+// eight bf16 values as four pairs of fp32, and back
+SSDK_DEVINL void pairs_of(const uint4& v, uint64_t* f) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = (uint64_t)(w[i] & 0xffff0000u) << 32 | w[i] << 16;
+}
+SSDK_DEVINL uint4 bf16_of(const uint64_t* f) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float x, y;
+    unpack2(f[i], &x, &y);
+    w[i] = pack_bf16x2(x, y);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 constexpr int kNoPosition = 0x7fffff00;   // of a key that is not there: behind every context
 
 }  // namespace ssdk
