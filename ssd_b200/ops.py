@@ -357,8 +357,8 @@ _U8 = torch.uint8
 def kv4_caches(num_blocks: int, block_size: int, kv_heads: int, head_dim: int, device="cuda"):
     """(k_cache, v_cache) of zeros: uint8 [num_blocks, kv_heads, block_size * (head_dim / 2 + 4)], the codes of a page's tokens and behind them their scales and
     minima (include/ssdk.h has the format).  17 bytes where the bf16 cache has 64 (heads of 128); a page of one head is one piece, so pages are copied as they are."""
-    if head_dim not in (64, 128) or block_size < 16 or block_size % 16 or num_blocks < 1 or kv_heads < 1:
-        raise ValueError(f"kv4_caches: {num_blocks} pages of {block_size} tokens (a multiple of 16), {kv_heads} heads of {head_dim} (64 or 128)")
+    if head_dim not in (64, 128) or not 16 <= block_size <= 65536 or block_size % 16 or num_blocks < 1 or num_blocks * block_size >= _TOP or not 1 <= kv_heads <= 65535:
+        raise ValueError(f"kv4_caches: {num_blocks} pages of {block_size} tokens (a multiple of 16 up to 65536, fewer than 2^31 in all), {kv_heads} heads (at most 65535) of {head_dim} (64 or 128)")
     return tuple(torch.zeros(2, num_blocks, kv_heads, block_size * (head_dim // 2 + 4), dtype=_U8, device=device).unbind(0))
 
 
@@ -446,7 +446,7 @@ def paged_attention_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     """paged_attention over a cache of 4 bits (kv4_caches): q [B * q_len, H, hd] bf16, block_tables int32 [B, max_blocks], context_lens int32 [B] with the new tokens.
 
     Returns [B * q_len, H * hd].  Keys and values are scale * code + minimum, not rounded up to sixteen rows (H / KV * q_len) to a key head, in bf16 as load_kv4 gives them with
-    more.  Pages outside the cache are passed over, a row that sees no key is zero, a NaN row of the cache makes NaN of the rows that see it."""
+    more.  At most 32 query heads to a key head.  Pages outside the cache are passed over, a row that sees no key is zero, a NaN row of the cache makes NaN of the rows that see it."""
     B, width, H, hd = _last(context_lens, 1), _last(block_tables, 2), *(q.shape[1:] if q.dim() == 3 else (-1, -1))
     cache, block_size = _kv4("paged_attention_kv4", k_cache, hd)
     gpu = _check("paged_attention_kv4", (q, "q", _BF, (B * q_len, H, hd)), (k_cache, "k_cache", _U8, cache), (v_cache, "v_cache", _U8, cache),

@@ -75,3 +75,12 @@ def test_too_many_heads_of_rows_are_refused_by_their_own_name():
     for name, args in (("rope_store_kv4", rope), ("store_kv4", rows)):
         assert getattr(so, "ssdk_" + name)(*args) != 0
         assert so.ssdk_last_error().decode().startswith(name + ": 1048576 rows of "), so.ssdk_last_error()
+
+
+@pytest.mark.parametrize("sizes", [(1 << 20, 2048, 1, 64), (2, 65552, 1, 128), (2, 16, 65536, 64)])
+def test_caches_that_no_operator_takes_are_not_made(sizes):
+    """Slots past 32 bits, pages of more than 65536 tokens, more than 65535 heads: refused before memory is asked for, as the operators refuse them."""
+    from ssd_b200 import ops
+    with pytest.raises(ValueError, match="kv4_caches"):
+        ops.kv4_caches(*sizes, device="meta")
+    assert ops.kv4_caches((1 << 20) - 1, 2048, 1, 64, device="meta")[1].shape == ((1 << 20) - 1, 1, 2048 * 36)
