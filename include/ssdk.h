@@ -331,7 +331,7 @@ int ssdk_span_attn(const void* q, const void* k_cache, const void* v_cache, cons
  * scale * code + minimum, rounded once to bf16.  A row that holds something that is not finite, or whose spread passes fp32, is NaN as a whole.  head_dim 64 or 128, block_size a multiple of 16
  * of at most 65536, fewer than 2^31 slots.  Written or read rows of one call have distinct slots where they are written; slots outside the cache store nothing. */
 /* ssdk_rope_store_kv4: ssdk_rope_store_kv into such a cache.  positions int64 [M]; rope_table fp32 [max_pos, rot_dim] cos | sin: the first rot_dim channels of a head turn (a
- * multiple of 16).  Queries: fp32, one rounding, to q_out [M, heads * head_dim].  Keys: norm and rotation in 64 bits, rounded to bf16, then quantised.  k_values, v_values [M, KV, head_dim] (both or
+ * multiple of 16).  Queries: fp32, one rounding, to q_out [M, heads * head_dim].  Keys: norm and rotation in 64 bits, rounded to fp32 and then to bf16, then quantised.  k_values, v_values [M, KV, head_dim] (both or
  * null): the values that then stand in the cache, of every row, also of those without a slot.  A row with a position outside the table has NaN queries and values and stores nothing. */
 int ssdk_rope_store_kv4(const void* qkv, const int64_t* positions, const int32_t* slot_mapping, const float* rope_table, int64_t max_pos,
                         int rot_dim, const void* q_norm_w, const void* k_norm_w, float norm_eps, void* q_out, void* k_cache, void* v_cache,
@@ -344,10 +344,11 @@ int ssdk_store_kv4(const void* k, const void* v, int64_t k_row, int64_t v_row, c
 int ssdk_load_kv4(const void* k_cache, const void* v_cache, const int32_t* slot_mapping, void* k, void* v, int64_t num_blocks, int block_size,
                   int M, int kv_heads, int head_dim, void* stream);
 /* ssdk_paged_attn_kv4: ssdk_paged_attn over the values scale * code + minimum, causal to the end of the context.  Up to sixteen query rows to a key head they are not rounded, with more they are rounded to
- * bf16, as ssdk_load_kv4 gives them (one that would pass bf16's largest number by that stays below it).  At most 32 query heads to a key head.  Pages outside the cache are passed over, lengths are held
- * to what a table has room for, a row that sees no key is zero.  Weights below 2^-126 of the largest are
- * zero (2^-94 beside values of 2^65 and more, next to which values below 2^-94 may lose bits).  A NaN row of the cache makes NaN of the rows that see it, a query that is not finite, or (up to sixteen rows) whose sum passes fp32, makes
- * its row NaN.  `scratch`: ssdk_paged_attn_kv4_scratch_bytes(...) bytes of the call's own (0: null).  More than sixteen query rows to a key head take a kernel with bounded waits: as with
+ * bf16, as ssdk_load_kv4 gives them (one that would pass bf16's largest number by that stays below it).  At most 32 query heads to a key head, and queries of
+ * a sequence in at most 65535 tiles of whole tokens and up to 128 rows.  Pages outside the cache are passed over, lengths are held to what a table has room for, a row that sees no key is zero.  Weights are bf16
+ * (up to sixteen rows: times their value's scale), queries up to sixteen rows whole numbers of 16 bits of their row's largest, sums and references fp32.  Weights below 2^-126 of the largest are zero (2^-94 beside values of
+ * 2^65 and more, next to which values below 2^-94 may lose bits).  A NaN row of the cache makes NaN of the rows that see it, a query that is not finite, or (up to sixteen rows) whose sum passes fp32, makes its row NaN;
+ * one whose largest value or sum, times scale * log2(e), reaches 2^118 may.  `scratch`: ssdk_paged_attn_kv4_scratch_bytes(...) bytes of the call's own (0: null).  More than sixteen query rows to a key head take a kernel with bounded waits: as with
  * ssdk_paged_attn_pages, a wait that runs out leaves NaN rows, and the next such call of the process returns an error. */
 int64_t ssdk_paged_attn_kv4_scratch_bytes(int batch, int q_len, int heads, int kv_heads, int head_dim, int block_size, int max_blocks_per_seq);
 int ssdk_paged_attn_kv4(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables, const int32_t* context_lens,

@@ -148,8 +148,9 @@ SSDK_DEVINL void kv4_codes(uint4& x, uint4& y, uint32_t (&code)[2], uint32_t& pa
 // kv4_store_kernel.  ROPE: queries and keys turn (rope_axes_kernel with one axis), optional norms in front, queries go to q_out; without it rows of keys and values are quantised
 // as they are.  Queries are fp32 with one rounding.  A key is rounded to bf16 (what an unquantised cache would hold) and then quantised, and that rounding decides its code next to a
 // border: keys' norm and rotation are in 64 bits, so that codes are those of the definition whatever the order of sums.  (Keys are an eighth to a third of the heads.)
-// 2 bytes read a channel, 2 written for queries and values that are asked for, 0.53 for codes.  Bound by instructions (issue slots 58 % with rotation, 68 % without) beside memory: 16000 rows of 32 heads over
-// 8 of 128 91 us (71 % of the copy rate; 103 with norms), 32003 rows of 8 heads as they are 60 (76 %), both with the values written back; 7 rows 2.8.  HD / 16 lanes own a head, a warp takes groups of
+// 2 bytes read a channel, 2 written for queries and values that are asked for, 0.53 for codes.  Issue slots 60 % busy with rotation, 69 % without, beside memory: 16000 rows of 32 heads over
+// 8 of 128 91 us (71 % of the copy rate; 103 with norms), 32003 rows of 8 heads as they are 60 (76 %), both with the values written back; without them 85 (64 %) and 49 (53 %); 7 rows 2.8.
+// Of the 91 and 103 keys in 64 bits make 5 and 11, the remainder that settles a code 1 (none of the 60).  HD / 16 lanes own a head, a warp takes groups of
 // 32 / (HD / 16) heads of a row (queries, keys, values behind one another), one or two groups' loads in flight; the rows' groups lie one behind the other and each warp has a stretch of them.
 // A row with a position outside the table has NaN queries (and values) and stores nothing; slots outside the cache store nothing.
 // ----------------------------------------------------------------------------------

@@ -15,8 +15,8 @@ namespace ssdk {
 //   q k = s (q c) + m sum(q)          O = sum_j (P_j s'_j) (c'_j - 8) + sum_j P_j (m'_j + 8 s'_j)
 // so that what meets in the products are codes, which are exact: keys and values are not rounded at all.  What is rounded is P s' (bf16, 2^-8 of a term at most, the codes
 // around their middle so that it is of the value's size); sums, references and the second term are fp32.
-// Bound by the instructions that make codes into fragments, then by the bytes of the cache: 48 contexts of 16000 (64 heads over 8 of 128) 127 us, 77 % of the copy rate, integer pipe 56 % (in
-// loops of seconds the power limit makes that 143); one of 32000 (32 heads) 20.5, where it is latency.  The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that
+// Bound by the instructions that make codes into fragments, then by the bytes of the cache: 48 contexts of 16000 (64 heads over 8 of 128) 129 us, 76 % of the copy rate, integer pipe 56 % (in
+// loops of seconds the power limit makes that 144, 68 %); one of 32000 (32 heads) 20, where it is latency.  The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that
 // keys (sixteen) and channels (sixteen) are the m of mma and the eight query rows of a usual group its n.
 //   Scores are whole numbers: a mask (and a shift) makes four codes of a word bytes, and a query row, scaled by a power of two so that its largest lies in 2^14 .. 2^15 and rounded, is 256 h + l with a
 // byte each, so that its values are off by at most 2^-15 of its largest (those above 2^-7 of it by nothing).  (bf16 codes take 64 instructions for sixteen keys where these take 24; mma on e4m3 is

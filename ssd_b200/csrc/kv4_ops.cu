@@ -57,9 +57,10 @@ static Kv4Plan kv4_plan(int64_t units, int64_t keys, int resident, int most, int
     }
   }
   // Equal stretches cost a second launch, but their time goes by the sum of all lengths, not by the longest, and more than the blocks of a cluster can share a head: they are taken where the clusters' cost
-  // passes share_from.  With a head or more to every place on the device blocks are dealt out as others end.  us, clusters and stretches, of the streaming kernel: one context of 8000 (8 heads) 10.6
-  // and 11.7, of 16000 14.7 and 14.8, of 32000 23.5 and 20.5, of 64000 40 and 26.7, 8 of 8000 24 and 26.5, 16 of 8000 37 and 35, 48 of 16000 130 and 127, 148 of 4000 94 and 112; of 56 rows on tiles: one context of 8000 25.7 and
-  // 27.4, of 16000 35.6 and 32.8, of 32000 56 and 42, 4 of 16000 55.6 and 61, 8 of 4000 32.6 and 38, 8 of 16000 96 and 84, 16 of 4000 52 and 56, 16 of 16000 175 and 145, 32 of 16000 334 and 268.
+  // passes share_from.  With a head or more to every place on the device blocks are dealt out as others end.  us, clusters and stretches, of the streaming kernel: one context of 8000 (8 heads) 10.5
+  // and 11.9, of 16000 14.7 and 15.1, of 32000 22.9 and 19.3, of 64000 40 and 26.8, 8 of 8000 23 and 26, 16 of 8000 37 and 35, 48 of 16000 131 and 128, 148 of 4000 95 and 113; of 56 rows on tiles: one context of 8000 25.9 and
+  // 27.5, of 16000 36.5 and 32.8, of 32000 59 and 42, 4 of 16000 56 and 61, 8 of 4000 33 and 38, 8 of 16000 99 and 85, 16 of 4000 53 and 56, 16 of 16000 181 and 146, 32 of 16000 347 and 270.
+  // (What counts is the table's room, since lengths are on the device: short contexts in tables made for long ones take the second launch for nothing, one of 500 5.4 and, in a table of 64000, 7.5; 8 x 7 rows of 500 14 and 24.)
   if (may_share && least > share_from && units < slots && units * ((keys + turn - 1) / turn) < (1ll << 31)) plan.blocks = (int)std::min(std::min(slots, units * 64), units * ((keys + turn - 1) / turn));
   return plan;
 }

@@ -12,8 +12,8 @@
 // rows.  A cluster of blocks shares the chunks of a key head; their sums meet in shared memory.  SHARED: as in kv4_attn_kernel.
 // A row takes 32 keys at a time.  TWIN: up to 64 rows lie in the tile twice, rows 0 .. 63 take a chunk's first 32 keys and 64 .. 127 the others, each with zeros for weights of the other half and a reference
 // of its own: all four warps work on half of the scores where two would on all, and the products are no more.
-// Bound by instructions and by the hand-offs between the warps: 8 x 7 rows over 16000 (64 heads over 8 of 128) 84 us, where the bytes ask for 17, 66 without making bf16 of codes, 79 without the softmax, 64
-// without either; 32 x 7 rows 268; 512 rows over 8000 (32 heads over 8 of 64) 97, 89, 71 and 64.  Two blocks to an SM hide each other's hand-offs (one with chunks of 128 keys: 109 where two had 104).  Loads
+// Bound by instructions and by the hand-offs between the warps: 8 x 7 rows over 16000 (64 heads over 8 of 128) 85 us, where the bytes ask for 17, 66 without making bf16 of codes, 79 without the softmax, 64
+// without either; 32 x 7 rows 271; 512 rows over 8000 (32 heads over 8 of 64) 97, 89, 71 and 64.  Two blocks to an SM hide each other's hand-offs (one with chunks of 128 keys: 109 where two had 104).  Loads
 // by the warps that make bf16 cost more than the copies (95 and 91), one chunk of copies more than three (91 and 85), which fit because keys have one stage: they are written while the values' product runs.
 #pragma once
 #include <climits>
